@@ -48,6 +48,16 @@ namespace {
 #define API_NULL(p) \
   if (!(p)) return fail(FA_ERR_INVALID, std::string(__func__) + ": null argument " #p)
 
+// no C++ exception leaves a C entry
+template <typename F>
+int guarded(F f) {
+  try {
+    return f();
+  } catch (const std::bad_alloc &) {
+    return fail(FA_ERR_OOM, "out of host memory");
+  }
+}
+
 void copy_str(const std::string &s, char *buf, size_t cap) {
   if (!buf || !cap) return;
   size_t n = std::min(cap - 1, s.size());
@@ -136,13 +146,15 @@ int create_kv(Model &m, uint32_t n_seq, uint32_t max_ctx, int dtype, KvCache *kv
   }
   API_CUDA(cudaMemset(kv->base, 0, bytes));
   std::vector<uint32_t> pt(pages);
-  for (uint64_t i = 0; i < pages; ++i) pt[i] = (uint32_t)i;  // static page assignment per sequence
+  for (uint64_t i = 0; i < pages; ++i) pt[i] = (uint32_t)i;  // until sequences share pages
   if (cudaMalloc(&kv->page_table, pages * 4) != cudaSuccess) {
     cudaGetLastError();
     kv->page_table = nullptr;
     return fail(FA_ERR_OOM, "page table allocation failed");
   }
   API_CUDA(cudaMemcpy(kv->page_table, pt.data(), pages * 4, cudaMemcpyHostToDevice));
+  kv->table = std::move(pt);
+  kv->refs.assign(pages, 1);
   return m.ensure_rope(max_ctx + 1);
 }
 
@@ -602,12 +614,11 @@ int fa_kv_create(fa_model *m, uint32_t n_seq, uint32_t max_ctx, int32_t dtype, f
 void fa_kv_free(fa_kv *kv) { delete kv; }
 int fa_kv_clear(fa_kv *kv, int32_t seq) {
   API_NULL(kv);
-  if (seq < 0) {
-    std::fill(kv->kv.len.begin(), kv->kv.len.end(), 0u);
-    return FA_OK;
+  if (seq >= 0 && (uint32_t)seq >= kv->kv.n_seq) return fail(FA_ERR_INVALID, "sequence index out of range");
+  for (uint32_t s = seq < 0 ? 0 : (uint32_t)seq; s < (seq < 0 ? kv->kv.n_seq : (uint32_t)seq + 1); ++s) {
+    const int rc = guarded([&] { return kv->kv.truncate(s, 0); });
+    if (rc) return rc;
   }
-  if ((uint32_t)seq >= kv->kv.n_seq) return fail(FA_ERR_INVALID, "sequence index out of range");
-  kv->kv.len[seq] = 0;
   return FA_OK;
 }
 int fa_kv_seq_len(const fa_kv *kv, uint32_t seq, uint32_t *len) {
@@ -644,6 +655,49 @@ int fa_kv_get(const fa_kv *kv, uint32_t seq, uint32_t layer, float *k_host, floa
             if (dst) dst[((size_t)(p * 16 + s) * KVH + h) * hd + dd] = v;
           }
   }
+  return FA_OK;
+}
+int fa_kv_pages(const fa_kv *kv, fa_pages *out) {
+  API_NULL(kv);
+  API_NULL(out);
+  if (!kv->kv.m) return fail(FA_ERR_INVALID, "fa_kv_pages: the cache's model was freed");
+  *out = kv->kv.pages();
+  return FA_OK;
+}
+int fa_kv_fork(fa_kv *kv, uint32_t src, uint32_t dst) {
+  API_NULL(kv);
+  if (src >= kv->kv.n_seq || dst >= kv->kv.n_seq) return fail(FA_ERR_INVALID, "fa_kv_fork: sequence index out of range");
+  return guarded([&] { return kv->kv.fork(src, dst); });
+}
+int fa_kv_reorder(fa_kv *kv, const uint32_t *parents, uint32_t n) {
+  API_NULL(kv);
+  if (n > kv->kv.n_seq) return fail(FA_ERR_INVALID, "fa_kv_reorder: more parents than sequences");
+  if (!n) return FA_OK;
+  API_NULL(parents);
+  for (uint32_t i = 0; i < n; ++i)
+    if (parents[i] >= n) return fail(FA_ERR_INVALID, "fa_kv_reorder: parent out of range");
+  return guarded([&] { return kv->kv.reorder(parents, n); });
+}
+int fa_kv_truncate(fa_kv *kv, uint32_t seq, uint32_t len) {
+  API_NULL(kv);
+  if (seq >= kv->kv.n_seq) return fail(FA_ERR_INVALID, "fa_kv_truncate: sequence index out of range");
+  if (len > kv->kv.len[seq]) return fail(FA_ERR_INVALID, "fa_kv_truncate: longer than the sequence");
+  return guarded([&] { return kv->kv.truncate(seq, len); });
+}
+int fa_kv_compact(fa_kv *kv, uint32_t seq, const uint32_t *keep, uint32_t n) {
+  API_NULL(kv);
+  if (seq >= kv->kv.n_seq) return fail(FA_ERR_INVALID, "fa_kv_compact: sequence index out of range");
+  if (n > kv->kv.len[seq]) return fail(FA_ERR_INVALID, "fa_kv_compact: more positions than the sequence has");
+  if (n) API_NULL(keep);
+  for (uint32_t i = 0; i < n; ++i)
+    if (keep[i] >= kv->kv.len[seq] || (i && keep[i] <= keep[i - 1]))
+      return fail(FA_ERR_INVALID, "fa_kv_compact: positions are ascending and below the sequence's length");
+  return guarded([&] { return kv->kv.compact(seq, keep, n); });
+}
+int fa_kv_page_count(const fa_kv *kv, uint32_t *used, uint32_t *total) {
+  API_NULL(kv);
+  if (used) *used = kv->kv.used_pages();
+  if (total) *total = (uint32_t)kv->kv.refs.size();
   return FA_OK;
 }
 

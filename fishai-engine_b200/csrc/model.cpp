@@ -540,6 +540,7 @@ KvCache::~KvCache() {
   }
   cudaFree(base);
   cudaFree(page_table);
+  cudaFree(scratch);
 }
 
 KvView KvCache::view() const {

@@ -210,8 +210,33 @@ struct KvCache {
   int f16 = 0;
   uint64_t layer_stride = 0;  // elements
   std::vector<uint32_t> len;  // positions stored per sequence
+  // Pages shared between sequences (fork, reorder).  Every table entry holds a
+  // page; refs counts the entries of a page.  A sequence's entries from its
+  // last, partly filled page on are its own (refs 1): decode writes there
+  // without asking.  The pool has one page an entry, so whenever an entry has
+  // to get a page of its own because its page is shared, a free one exists.
+  std::vector<uint32_t> table;      // host copy of page_table
+  std::vector<uint32_t> refs, free_pages;
+  uint32_t *scratch = nullptr;      // device lists of the page operators
   ~KvCache();
   KvView view() const;
+  fa_pages pages() const;
+  int fork(uint32_t src, uint32_t dst);
+  int reorder(const uint32_t *parents, uint32_t n);
+  int truncate(uint32_t seq, uint32_t n);
+  int compact(uint32_t seq, const uint32_t *keep, uint32_t n);
+  uint32_t used_pages() const;
+
+ private:
+  struct Move {
+    uint32_t src, dst, slots;
+  };
+  uint32_t *row(uint32_t seq) { return table.data() + (size_t)seq * max_pages; }
+  uint32_t take();
+  void drop(uint32_t page);
+  int upload(uint32_t seq);                          // a sequence's table row to the device
+  int copy(const std::vector<Move> &moves);          // pages, in every layer
+  int ensure_scratch();
 };
 
 int config_from_gguf(const Gguf &g, fa_config *cfg);

@@ -15,7 +15,11 @@ OK = 0
 ERR_INVALID, ERR_GGUF, ERR_UNSUPPORTED, ERR_OOM, ERR_CUDA, ERR_NCCL, ERR_CONTEXT, ERR_TIMEOUT = -1, -2, -3, -4, -5, -6, -7, -8
 
 F32, F16, Q4_0, Q4_1, Q5_0, Q8_0, Q4_K, Q6_K = 0, 1, 2, 3, 6, 8, 12, 14
-KV_F32, KV_F16 = 0, 1
+KV_F32, KV_F16, KV_BF16 = 0, 1, 2
+FLAG_PAGE, FLAG_RANGE = 16, 32
+ROPE_INTERLEAVED, ROPE_HALF = 0, 1
+ROPE_PLAIN, ROPE_LINEAR, ROPE_NTK, ROPE_LLAMA3, ROPE_YARN = 0, 1, 2, 3, 4
+NO_TOKEN = 4294967295
 DEBUG_WAIT_LIMIT_NS, DEBUG_WITHHOLD_WEIGHTS, DEBUG_FIXED_ORDER_SUMS = 1, 2, 3
 
 
@@ -56,6 +60,19 @@ class fa_synth_spec(C.Structure):
                 ("norm_eps", C.c_float), ("sigma", C.c_float), ("type_embd", C.c_int32), ("type_q", C.c_int32),
                 ("type_k", C.c_int32), ("type_v", C.c_int32), ("type_o", C.c_int32), ("type_gate", C.c_int32),
                 ("type_up", C.c_int32), ("type_down", C.c_int32), ("type_out", C.c_int32), ("threads", C.c_uint32)]
+
+
+class fa_pages(C.Structure):
+    _fields_ = [("base", C.c_void_p), ("layer_stride", C.c_uint64), ("dtype", C.c_int32), ("n_layers", C.c_uint32),
+                ("n_pages", C.c_uint32), ("n_kv_heads", C.c_uint32), ("head_dim", C.c_uint32),
+                ("page_table", C.c_void_p), ("n_seq", C.c_uint32), ("max_pages", C.c_uint32)]
+
+
+class fa_rope_config(C.Structure):
+    _fields_ = [("head_dim", C.c_uint32), ("rot_dim", C.c_uint32), ("layout", C.c_int32), ("scaling", C.c_int32),
+                ("base", C.c_double), ("factor", C.c_double), ("context", C.c_uint32), ("low_turns", C.c_double),
+                ("high_turns", C.c_double), ("beta_fast", C.c_double), ("beta_slow", C.c_double),
+                ("attn_factor", C.c_double)]
 
 
 # every entry point of include/fishai_cuda.h with its ctypes signature
@@ -128,6 +145,26 @@ SIGNATURES = {
     "fa_sdpa": ([_vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32, _vp, _vp], _i),
     "fa_sdpa_noalloc": ([_vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32, _vp, _vp], _i),
     "fa_sdpa_host": ([_pf, _pf, _pf, _u32, _u32, _u32, _u32, _u32, _pf], _i),
+    "fa_kv_pages": ([_vp, C.POINTER(fa_pages)], _i),
+    "fa_kv_fork": ([_vp, _u32, _u32], _i),
+    "fa_kv_reorder": ([_vp, _pu32, _u32], _i),
+    "fa_kv_truncate": ([_vp, _u32, _u32], _i),
+    "fa_kv_compact": ([_vp, _u32, _pu32, _u32], _i),
+    "fa_kv_page_count": ([_vp, _pu32, _pu32], _i),
+    "fa_rope_config_default": ([C.POINTER(fa_rope_config), _u32, C.c_double], None),
+    "fa_rope_create": ([C.POINTER(fa_rope_config), C.POINTER(_vp)], _i),
+    "fa_rope_free": ([_vp], None),
+    "fa_rope_freqs": ([_vp, C.POINTER(C.c_double), C.POINTER(C.c_double)], _i),
+    "fa_rope_append": ([_vp, _vp, _u32, C.c_int32, _vp, _u64, _vp, _u64, _vp, _u64, _u32, _u32, _vp, _vp, _vp, _vp,
+                        _u64, _vp, _vp], _i),
+    "fa_attn_chunks": ([_vp, _u32, _vp, _u64, _u32, _u32, _vp, _vp, _vp, _u32, _u32, _f, _u32, _vp, _u64, _vp, _sz,
+                        _vp, _vp], _i),
+    "fa_attn_chunks_ws": ([_u32], _sz),
+    "fa_pages_copy": ([_vp, _vp, _vp, _vp, _u32, _vp, _vp], _i),
+    "fa_pages_compact": ([_vp, _vp, _vp, _vp, _u32, _u32, _vp, _vp], _i),
+    "fa_beam_select": ([_vp, C.c_int32, _u64, _u32, _u32, _u32, _vp, _vp, _u32, _u32, _u32, _vp, _vp, _vp, _vp, _vp,
+                        _sz, _vp], _i),
+    "fa_beam_select_ws": ([_u32, _u32, _u32, _u32], _sz),
     "fa_synth_write": ([C.c_char_p, C.POINTER(fa_synth_spec), _u64], _i),
 }
 

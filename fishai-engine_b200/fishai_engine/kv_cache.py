@@ -64,3 +64,31 @@ class KVCache:
     def clear(self, seq: int = -1):
         """src/kv_cache.rs:98-103"""
         L.check(L.lib().fa_kv_clear(self._h, seq))
+
+    # ---- sequences that share pages (n_seq > 1; no counterpart in the reference) ----
+    def fork(self, src: int, dst: int):
+        """sequence dst becomes a copy of sequence src: whole pages are shared,
+        a partly filled last page is copied"""
+        L.check(L.lib().fa_kv_fork(self._h, src, dst))
+
+    def reorder(self, parents):
+        """sequence i becomes a copy of what sequence parents[i] was, all at once
+        (the step between two selections of a beam search)"""
+        a, p = L.u32_array(parents)
+        L.check(L.lib().fa_kv_reorder(self._h, p, a.size))
+
+    def truncate(self, seq: int, length: int):
+        """drops the positions from `length` on"""
+        L.check(L.lib().fa_kv_truncate(self._h, seq, length))
+
+    def compact(self, seq: int, keep):
+        """keeps the given ascending positions, as positions 0, 1, ...; their keys
+        stay turned as they were stored"""
+        a, p = L.u32_array(keep)
+        L.check(L.lib().fa_kv_compact(self._h, seq, p, a.size))
+
+    def pages_used(self):
+        """(pages that hold positions, each shared one once; pages of the cache)"""
+        u, t = C.c_uint32(), C.c_uint32()
+        L.check(L.lib().fa_kv_page_count(self._h, C.byref(u), C.byref(t)))
+        return u.value, t.value

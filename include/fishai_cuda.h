@@ -185,6 +185,7 @@ int fa_debug_set(fa_model *m, int32_t key, uint64_t value);
 typedef struct fa_kv fa_kv;
 #define FA_KV_F32 0
 #define FA_KV_F16 1
+#define FA_KV_BF16 2  /* pages of a caller only (fa_pages below): fa_kv_create refuses it */
 /* KVCache::new (src/kv_cache.rs:27-40), device resident and paged:
  * n_seq sequences, each up to max_ctx positions, pages of 16 positions. */
 int fa_kv_create(fa_model *m, uint32_t n_seq, uint32_t max_ctx, int32_t dtype, fa_kv **out);
@@ -252,6 +253,140 @@ int fa_sdpa_host(const float *q_host, const float *k_host, const float *v_host, 
 int fa_sdpa_noalloc(const float *q_dev, const float *k_dev, const float *v_dev, uint32_t q_len, uint32_t kv_len,
                     uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, float *out_dev, void *stream);
 
+/* ------------------------------------------------- paged K/V operators */
+/* No counterpart in the reference, whose cache is one growing vector per
+ * sequence (src/kv_cache.rs:13-104).  These work on device buffers: pages of
+ * a caller, or the pages of an fa_kv (fa_kv_pages).  Common to all of them:
+ *  - every pointer is checked to be memory of one device, and the kernels run
+ *    there whatever device is current; a host pointer is FA_ERR_INVALID.
+ *  - work is enqueued on `stream` (cudaStream_t, NULL: the legacy default
+ *    stream) and nothing waits, allocates or is kept after the call, so every
+ *    call may be captured into a graph.
+ *  - indices in device memory (pages, sequences, slots, lengths) are checked
+ *    by the kernels: one out of range sets a bit in *err (device uint32, not
+ *    cleared by the call; NULL: not reported) and is skipped, the rows or
+ *    copies that it names stay as they were.
+ *  - element types are FA_KV_F32, FA_KV_F16, FA_KV_BF16; sums are f32. */
+typedef struct {
+  void *base;             /* [n_layers][n_pages][k | v][n_kv_heads][16][head_dim], 16-byte aligned */
+  uint64_t layer_stride;  /* elements from one layer to the next, a multiple of 8 */
+  int32_t dtype;          /* FA_KV_* */
+  uint32_t n_layers, n_pages, n_kv_heads;
+  uint32_t head_dim;      /* a multiple of 8, at most 256 */
+  const uint32_t *page_table;  /* device [n_seq][max_pages]: positions 16 i .. 16 i + 15 are in page [seq][i] */
+  uint32_t n_seq, max_pages;
+} fa_pages;
+#define FA_FLAG_PAGE 16   /* *err: a page number >= n_pages */
+#define FA_FLAG_RANGE 32  /* *err: a sequence, slot, length, row or index out of range */
+/* the pages of a cache, for the calls below; valid until the cache is freed */
+int fa_kv_pages(const fa_kv *kv, fa_pages *out);
+
+/* Rotary positions.  Pair i of the first rot_dim elements of a head (elements
+ * 2i and 2i+1, or i and i + rot_dim/2) at position p is turned by p f_i, where
+ * f_i = base^(-2i / rot_dim) (src/tensor.rs:331-392), scaled for contexts
+ * beyond `context` positions by one of
+ *   LINEAR f / factor;  NTK base * factor^(rot_dim / (rot_dim - 2));
+ *   LLAMA3 f where the wave 2 pi / f turns more than high_turns times in
+ *          `context`, f / factor below low_turns, between them blended evenly
+ *          over the turns;
+ *   YARN   f above beta_fast turns in `context`, f / factor below beta_slow,
+ *          between them blended evenly over i, and the result times
+ *          attn_factor (0: 0.1 ln(factor) + 1).
+ * The other elements of a head are copied.  Angles are reduced in 64 bits, so
+ * positions of any size keep their exactness. */
+#define FA_ROPE_INTERLEAVED 0
+#define FA_ROPE_HALF 1
+#define FA_ROPE_PLAIN 0
+#define FA_ROPE_LINEAR 1
+#define FA_ROPE_NTK 2
+#define FA_ROPE_LLAMA3 3
+#define FA_ROPE_YARN 4
+typedef struct {
+  uint32_t head_dim, rot_dim;  /* rot_dim even, 2 .. head_dim */
+  int32_t layout, scaling;     /* FA_ROPE_* */
+  double base, factor;         /* base > 1, factor >= 1 */
+  uint32_t context;            /* the context the model was made for */
+  double low_turns, high_turns;      /* LLAMA3: 1, 4 */
+  double beta_fast, beta_slow;       /* YARN: 32, 1 */
+  double attn_factor;
+} fa_rope_config;
+typedef struct fa_rope fa_rope;
+/* interleaved, the whole head, unscaled; the values named above */
+void fa_rope_config_default(fa_rope_config *cfg, uint32_t head_dim, double base);
+/* a handle with the frequencies (host memory; any number of threads and
+ * devices may use it at once) */
+int fa_rope_create(const fa_rope_config *cfg, fa_rope **out);
+void fa_rope_free(fa_rope *r);
+/* the rot_dim/2 frequencies and the factor on the result */
+int fa_rope_freqs(const fa_rope *r, double *freqs, double *scale);
+/* Turns q and k of n_tokens tokens and puts k, v into the pages of `layer`.
+ * Token t: RoPE position pos[t], cache sequence seq[t], cache position
+ * slot[t] (slot NULL: pos[t]); q row t of n_heads * head_dim elements at
+ * q + t q_stride goes to out + t out_stride (out may be q), k and v rows of
+ * n_kv_heads * head_dim elements.  q, k, v have type in_dtype, out the pages'
+ * type.  seq[t] = FA_NO_TOKEN marks a row that is left out (padding).  Two
+ * tokens of a call must not name the same sequence and slot: the cache row
+ * would hold some of each. */
+#define FA_NO_TOKEN 4294967295u
+int fa_rope_append(const fa_rope *r, const fa_pages *pages, uint32_t layer, int32_t in_dtype, const void *q,
+                   uint64_t q_stride, const void *k, uint64_t k_stride, const void *v, uint64_t v_stride,
+                   uint32_t n_tokens, uint32_t n_heads, const uint32_t *pos, const uint32_t *seq, const uint32_t *slot,
+                   void *out, uint64_t out_stride, uint32_t *err, void *stream);
+
+/* Attention of chunks of new tokens over the pages of `layer`
+ * (src/tensor.rs:451-551 with the causal order of src/model.rs:644-650).
+ * Chunk c: rows q_start[c] .. q_start[c+1] - 1 of q and out, cache sequence
+ * seq[c] (seq NULL: c), whose first kv_len[c] positions hold the cache with
+ * the chunk's own tokens last.  Token i of the q_len is at position
+ * p = kv_len - q_len + i and sees the positions t with 0 <= t <= p, and
+ * t > p - window where window > 0; a token that sees none gives zeros.
+ * Scores are scaled by `scale` (0: 1 / sqrt(head_dim)).  Chunks may have any
+ * lengths, zero and one among them, in any mix; none is longer than max_q
+ * (one that is sets FA_FLAG_RANGE and is left out).  Rows outside every chunk
+ * are left as they were.  q and out have the pages' type and rows of n_heads *
+ * head_dim elements, q_stride and out_stride apart; out must not overlap q.
+ * The positions that some token of a chunk sees should hold finite K and V;
+ * whatever is behind kv_len or before every token's window is not used.  A
+ * page out of range (FA_FLAG_PAGE) spoils the chunk's own rows only.
+ * ws: at least fa_attn_chunks_ws(...) bytes of device memory, 16-byte aligned,
+ * used by no other call that may run at the same time; its content is free. */
+int fa_attn_chunks(const fa_pages *pages, uint32_t layer, const void *q, uint64_t q_stride, uint32_t n_heads,
+                   uint32_t n_chunks, const uint32_t *q_start, const uint32_t *kv_len, const uint32_t *seq,
+                   uint32_t n_tokens, uint32_t max_q, float scale, uint32_t window, void *out, uint64_t out_stride,
+                   void *ws, size_t ws_bytes, uint32_t *err, void *stream);
+size_t fa_attn_chunks_ws(uint32_t head_dim);
+
+/* Copies the first slots[i] positions (slots NULL: all 16) of page src[i] to
+ * page dst[i], keys and values, in every layer, i < n; src, dst, slots are
+ * device arrays.  No page may be both a source and a destination, or twice a
+ * destination, within a call. */
+int fa_pages_copy(const fa_pages *pages, const uint32_t *src, const uint32_t *dst, const uint32_t *slots, uint32_t n,
+                  uint32_t *err, void *stream);
+/* Keeps some positions of n sequences, in place and in every layer: position
+ * j of sequence seq[i] becomes its position keep[keep_start[i] + j], for
+ * j < keep_start[i+1] - keep_start[i].  keep is strictly ascending within a
+ * sequence (a position that is not sets FA_FLAG_RANGE and is left out); no
+ * sequence may come twice, nor two share a page that is written.  Keys stay
+ * turned as they were stored.  n_keep: the length of keep. */
+int fa_pages_compact(const fa_pages *pages, const uint32_t *seq, const uint32_t *keep, const uint32_t *keep_start,
+                     uint32_t n, uint32_t n_keep, uint32_t *err, void *stream);
+
+/* ---- pages of a cache shared between its sequences ---- */
+/* Sequence dst becomes a copy of sequence src: whole pages are shared, the
+ * last one is copied if it is partly filled.  src == dst does nothing. */
+int fa_kv_fork(fa_kv *kv, uint32_t src, uint32_t dst);
+/* Sequence i becomes a copy of what sequence parents[i] was, for all i < n at
+ * once (host array); n <= n_seq, parents[i] < n. */
+int fa_kv_reorder(fa_kv *kv, const uint32_t *parents, uint32_t n);
+/* Drops the positions from `len` on (len <= the sequence's length) and frees
+ * their pages. */
+int fa_kv_truncate(fa_kv *kv, uint32_t seq, uint32_t len);
+/* Keeps the positions keep[0] < keep[1] < ... of a sequence (host array) as
+ * its positions 0 .. n - 1; their keys stay turned as they were stored. */
+int fa_kv_compact(fa_kv *kv, uint32_t seq, const uint32_t *keep, uint32_t n);
+/* pages in use (each shared one once) and pages of the cache */
+int fa_kv_page_count(const fa_kv *kv, uint32_t *used, uint32_t *total);
+
 /* ------------------------------------------------------------ tokenizer */
 /* BpeTokenizer (src/tokenizer.rs:148-600): the text step before the token
  * loop.  Ids -1 mean "none" (the reference's Option<u32>). */
@@ -316,6 +451,33 @@ int fa_sampler_observe(fa_sampler *s, uint32_t seq, uint32_t token);
 int fa_sampler_reset(fa_sampler *s, int32_t seq);  /* seq < 0: every sequence */
 /* token_freq[token] of sequence seq (0 for ids never observed) */
 int fa_sampler_freq(fa_sampler *s, uint32_t seq, uint32_t token, uint32_t *count);
+
+/* --------------------------------------------------------- beam search */
+/* One selection step over n_batch requests of n_beams beams (no counterpart
+ * in the reference; beside Sampler::sample).  Row b * n_beams + j of logits
+ * (device, ld elements apart, type FA_KV_*) belongs to beam j of request b;
+ * its candidates are (j, v), v < vocab, with the score
+ *   scores[b][j] + logit_v - log(sum over the row of exp(logit)),
+ * computed in 64 bits; those of one beam stand in the order of its logits.  A
+ * beam with done[b][j] != 0 (done may be NULL) has the
+ * one candidate (j, pad) at its own score, and its logits are not read.  The
+ * k best candidates of a request, equal scores by lowest beam then token, go
+ * to out_*[b][0 .. k) in descending order: score, parent beam, token, and
+ * whether the new beam is done (its parent was, or the token is eos; eos =
+ * FA_NO_TOKEN: none).  Logits of -inf and NaN are no candidates and add
+ * nothing to the sum; +inf counts as the largest f32.  A beam whose score is
+ * not finite takes no part.  Where fewer than k candidates exist the rest are
+ * score -inf, parent place % n_beams, token pad, done 1.  Any out array may be
+ * the matching input (k = n_beams); out_done may be NULL.
+ * n_beams, k <= 64, pad < vocab.  ws: fa_beam_select_ws(...) bytes of device
+ * memory, 16-byte aligned, used by no other call that may run at the same
+ * time.  Runs as the operators on pages do: same device, stream and capture
+ * rules. */
+int fa_beam_select(const void *logits, int32_t dtype, uint64_t ld, uint32_t n_batch, uint32_t n_beams, uint32_t vocab,
+                   const float *scores, const uint32_t *done, uint32_t k, uint32_t eos, uint32_t pad, float *out_scores,
+                   uint32_t *out_parents, uint32_t *out_tokens, uint32_t *out_done, void *ws, size_t ws_bytes,
+                   void *stream);
+size_t fa_beam_select_ws(uint32_t n_batch, uint32_t n_beams, uint32_t vocab, uint32_t k);
 
 /* ------------------------------------------------ token-parallel GEMM */
 /* Y[T][n_out] = X[T][K] . W for one weight group of the model (proj 0 qkv,
