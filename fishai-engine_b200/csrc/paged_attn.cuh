@@ -202,6 +202,8 @@ struct Walk {
 // joins the pieces of split items (R: rows of an item; ctas: grid of the launch before)
 int launch_attn_join(const AttnChunksParams &p, uint32_t R, uint32_t ctas, cudaStream_t st);
 int launch_attn_any(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st);
+bool attn_mma_takes(const AttnChunksParams &p);
+int launch_attn_mma(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st);
 
 constexpr uint32_t kAttnMaxCtas = 480;  // most CTAs of a launch (the workspace holds two slots of each)
 constexpr uint32_t kAttnMaxRows = 64;   // most rows of an item

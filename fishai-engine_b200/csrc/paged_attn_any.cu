@@ -303,6 +303,7 @@ int launch_attn_chunks(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st
   AttnChunksParams a = p;
   a.rows_min = 1;
   a.rows_max = 0xFFFFFFFFu;
+  if (attn_mma_takes(a)) return launch_attn_mma(a, n_sm, st);
   return launch_attn_any(a, n_sm, st);
 }
 

@@ -1,0 +1,473 @@
+// Attention of chunks over paged f16 / bf16 K/V with few rows per kv head:
+// single tokens and short chunks, head sizes 64 and 128.  Same mathematics as
+// paged_attn_any.cu, products on mma.sync m16n8k16 with f32 accumulators.  The
+// weights p = 2^(s - m) <= 1 are rounded to the cache's type for the product
+// with V (the type V itself was rounded to); their sum is taken before that
+// rounding, in f32.
+//
+// HBM bounds it: every K and V row is used for at most 64 rows of Q, far below
+// the 250 operations a byte where tensor cores would bind, so all that counts
+// is copies in flight.  Sub-tiles of 32 positions (two pages) go to shared
+// memory by cp.async in 16-byte pieces, XOR-swizzled by row so that ldmatrix
+// reads eight rows from distinct banks; rows nobody sees are filled with
+// zeros, so stale or NaN slots do not reach a product.
+//   up to 16 rows (k_attn_rows16): each warp runs through its own sub-tiles
+//     and keeps its own (max, sum, output); the four are merged at the end of
+//     a piece.  The next K is fetched as soon as the scores are formed, the
+//     next V after its product, so both buffers are nearly always in flight.
+//   up to 64 rows (k_attn_rows64): a warp has 16 of the rows, and all warps
+//     share tiles of 64 positions, the next one in flight.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "paged_attn.cuh"
+
+namespace fa {
+namespace {
+
+constexpr uint32_t kSub = 32;       // positions of a sub-tile
+constexpr uint32_t kThreads = 128;  // 4 warps
+
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (sizeof(T) == 2 && __is_same(T, __half))
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t &r0, uint32_t &r1, uint32_t &r2, uint32_t &r3) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t &r0, uint32_t &r1, uint32_t &r2, uint32_t &r3) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool ok) {  // 16 bytes, or zeros
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16u : 0u) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {  // 2^x, 2 ulp; below 2^-126: 0
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (__is_same(T, __half)) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+  }
+}
+template <typename T>
+__device__ __forceinline__ T round_to(float x) {
+  if constexpr (__is_same(T, __half)) return __float2half_rn(x);
+  else return __float2bfloat16_rn(x);
+}
+
+// byte offset of 16-byte piece c of row r
+template <uint32_t HD>
+__device__ __forceinline__ uint32_t sw(uint32_t r, uint32_t c) {
+  return r * (HD * 2) + ((c ^ (r & 7)) << 4);
+}
+
+// The rows of one warp: 16 rows of the item, this thread's rows g and g + 8
+// (MMA fragment layout), with the running softmax and output.
+template <typename T, uint32_t HD>
+struct Rows {
+  uint32_t qa[HD / 16][4];
+  float o[HD / 8][4], m[2], l[2];
+  int32_t pos[2];           // positions of the tokens; -1: no row (sees nothing)
+  int32_t pos_min, pos_max; // over the warp's real rows
+
+  __device__ void load(const AttnChunksParams &p, const Segment &s, uint32_t first_row) {
+    const uint32_t lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    const T *q[2];
+    bool ok[2];
+#pragma unroll
+    for (uint32_t i = 0; i < 2; ++i) {
+      const uint32_t row = first_row + g + 8 * i;
+      ok[i] = row < s.r1;
+      const uint32_t tok = ok[i] ? row / p.rep : 0, h = ok[i] ? row - tok * p.rep : 0;
+      pos[i] = ok[i] ? s.chunk.first + (int32_t)tok : -1;
+      q[i] = reinterpret_cast<const T *>(p.q) + (uint64_t)(s.chunk.q0 + tok) * p.qs + (s.head * p.rep + h) * HD;
+      m[i] = -INFINITY;
+      l[i] = 0.0f;
+    }
+    const uint32_t last = min(s.r1, first_row + 16) - 1;  // the caller's rows are not empty
+    pos_min = s.chunk.first + (int32_t)(first_row / p.rep);
+    pos_max = s.chunk.first + (int32_t)(last / p.rep);
+#pragma unroll
+    for (uint32_t kt = 0; kt < HD / 16; ++kt)
+#pragma unroll
+      for (uint32_t e = 0; e < 4; ++e) {  // rows g, g+8; columns 2c, 2c+8
+        const T *x = q[e & 1] + 16 * kt + 2 * c + 8 * (e >> 1);
+        uint32_t w = 0;
+        if (ok[e & 1]) {
+          if (p.aligned) w = *reinterpret_cast<const uint32_t *>(x);
+          else w = (uint32_t)*reinterpret_cast<const uint16_t *>(x) | (uint32_t)*reinterpret_cast<const uint16_t *>(x + 1) << 16;
+        }
+        qa[kt][e] = w;
+      }
+#pragma unroll
+    for (uint32_t j = 0; j < HD / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
+  }
+
+  // scores of 32 positions from t0 on
+  __device__ void scores(uint32_t ktile, float (&s)[kSub / 8][4]) const {
+    const uint32_t lane = threadIdx.x & 31, mi = lane >> 3;
+#pragma unroll
+    for (uint32_t j = 0; j < kSub / 8; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.0f;
+#pragma unroll
+    for (uint32_t kt = 0; kt < HD / 16; ++kt)
+#pragma unroll
+      for (uint32_t j = 0; j < kSub / 8; j += 2) {
+        uint32_t b0, b1, b2, b3;
+        ldsm4(ktile + sw<HD>(8 * j + 8 * (mi >> 1) + (lane & 7), 2 * kt + (mi & 1)), b0, b1, b2, b3);
+        mma16816<T>(s[j], qa[kt], b0, b1);
+        mma16816<T>(s[j + 1], qa[kt], b2, b3);
+      }
+  }
+
+  // s -> weights; the running maximum, sum and output follow
+  __device__ void softmax(const AttnChunksParams &p, uint32_t t0, float (&s)[kSub / 8][4]) {
+    const uint32_t c = threadIdx.x & 3;
+    const bool all = (int32_t)(t0 + kSub - 1) <= pos_min && (!p.window || pos_max - (int32_t)t0 < (int32_t)p.window);
+    float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (uint32_t j = 0; j < kSub / 8; ++j)
+#pragma unroll
+      for (uint32_t e = 0; e < 4; ++e) {
+        const int32_t t = (int32_t)(t0 + 8 * j + 2 * c + (e & 1));
+        if (!all) {
+          const bool see = t <= pos[e >> 1] && (!p.window || (uint32_t)(pos[e >> 1] - t) < p.window);
+          if (!see) s[j][e] = -INFINITY;
+        }
+        mx[e >> 1] = fmaxf(mx[e >> 1], s[j][e]);
+      }
+#pragma unroll
+    for (uint32_t i = 0; i < 2; ++i) {
+      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xFFFFFFFFu, mx[i], 1));
+      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xFFFFFFFFu, mx[i], 2));
+      const float mn = fmaxf(m[i], mx[i] * p.scale_log2), ms = mn == -INFINITY ? 0.0f : mn;
+      const float f = ex2(m[i] - ms);
+      m[i] = mn;
+      float sum = 0.0f;
+#pragma unroll
+      for (uint32_t j = 0; j < kSub / 8; ++j)
+#pragma unroll
+        for (uint32_t e = 2 * i; e < 2 * i + 2; ++e) {
+          s[j][e] = ex2(fmaf(s[j][e], p.scale_log2, -ms));
+          sum += s[j][e];
+        }
+      l[i] = fmaf(l[i], f, sum);  // of this thread's columns: summed over the four at the end
+#pragma unroll
+      for (uint32_t j = 0; j < HD / 8; ++j) {
+        o[j][2 * i] *= f;
+        o[j][2 * i + 1] *= f;
+      }
+    }
+  }
+
+  __device__ void add_values(uint32_t vtile, const float (&s)[kSub / 8][4]) {
+    const uint32_t lane = threadIdx.x & 31, mi = lane >> 3;
+#pragma unroll
+    for (uint32_t kt = 0; kt < kSub / 16; ++kt) {
+      const uint32_t a[4] = {pack2<T>(s[2 * kt][0], s[2 * kt][1]), pack2<T>(s[2 * kt][2], s[2 * kt][3]),
+                             pack2<T>(s[2 * kt + 1][0], s[2 * kt + 1][1]), pack2<T>(s[2 * kt + 1][2], s[2 * kt + 1][3])};
+#pragma unroll
+      for (uint32_t j = 0; j < HD / 8; j += 2) {
+        uint32_t b0, b1, b2, b3;
+        ldsm4_t(vtile + sw<HD>(16 * kt + 8 * (mi & 1) + (lane & 7), j + (mi >> 1)), b0, b1, b2, b3);
+        mma16816<T>(o[j], a, b0, b1);
+        mma16816<T>(o[j + 1], a, b2, b3);
+      }
+    }
+  }
+  __device__ void finish() {
+#pragma unroll
+    for (uint32_t i = 0; i < 2; ++i) {
+      l[i] += __shfl_xor_sync(0xFFFFFFFFu, l[i], 1);
+      l[i] += __shfl_xor_sync(0xFFFFFFFFu, l[i], 2);
+    }
+  }
+};
+
+// Where a warp's copies of 32 positions come from: pages of positions t0 and
+// t0 + 16 (looked up one sub-tile ahead).
+struct PagePair {
+  uint32_t page[2];
+};
+__device__ __forceinline__ PagePair look_up(const uint32_t *pt, uint32_t t0, uint32_t lo, uint32_t hi) {
+  PagePair r;
+#pragma unroll
+  for (uint32_t i = 0; i < 2; ++i) {
+    const uint32_t t = t0 + 16 * i;
+    r.page[i] = t < hi && t + 16 > lo ? __ldg(pt + t / kPageLen) : 0u;  // only pages that are read are looked up
+  }
+  return r;
+}
+// K (is_v 0) or V rows of positions [t0, t0 + 32) to a tile; THREADS threads,
+// thread i of them.  Positions outside [lo, hi) and bad pages become zeros.
+template <typename T, uint32_t HD>
+__device__ __forceinline__ void stage(const AttnChunksParams &p, const T *base, const PagePair &pg, uint32_t head, uint32_t is_v,
+                                      uint32_t t0, uint32_t lo, uint32_t hi, uint32_t tile, uint32_t i, uint32_t threads) {
+  constexpr uint32_t CH = HD / 8;  // pieces of a row
+  const uint32_t c = i % CH, r0 = i / CH, step = threads / CH;
+#pragma unroll
+  for (uint32_t half = 0; half < 2; ++half) {
+    const bool good = pg.page[half] < p.pg.n_pages;
+    const T *src = base + page_row(p.pg, good ? pg.page[half] : 0, is_v, head, 0) + c * 8;
+#pragma unroll
+    for (uint32_t r = 0; r < 16; r += step) {
+      const uint32_t row = r + r0, t = t0 + 16 * half + row;
+      cp16(tile + sw<HD>(16 * half + row, c), src + row * HD, good && t >= lo && t < hi);
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ T *out_row(const AttnChunksParams &p, const Segment &s, uint32_t row, uint32_t hd) {
+  const uint32_t tok = row / p.rep;
+  return reinterpret_cast<T *>(p.out) + (uint64_t)(s.chunk.q0 + tok) * p.os + (s.head * p.rep + row - tok * p.rep) * hd;
+}
+
+__device__ __forceinline__ void flag_bad_pages(const AttnChunksParams &p, const PagePair &pg) {
+  if ((pg.page[0] >= p.pg.n_pages || pg.page[1] >= p.pg.n_pages) && p.err) atomicOr(p.err, kFlagPage);
+}
+
+// ------------------------------------------------------------ up to 16 rows
+template <typename T, uint32_t HD>
+__global__ void __launch_bounds__(kThreads, 3) k_attn_rows16(const AttnChunksParams p) {
+  extern __shared__ __align__(128) uint8_t dsm[];
+  __shared__ uint64_t red[kThreads / 32 + 2];
+  constexpr uint32_t kTileBytes = kSub * HD * 2;
+  using W = Walk<16, kSub, kThreads>;
+  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
+  const uint32_t ktile = smem_u32(dsm) + warp * 2 * kTileBytes, vtile = ktile + kTileBytes;
+  const T *base = reinterpret_cast<const T *>(p.pg.base) + (uint64_t)p.layer * p.pg.layer_stride;
+  W w;
+  w.start(p, 4, red);
+  if (tid == 0) p.desc[blockIdx.x].w = 0;
+  while (!w.done()) {
+    const Segment s = w.next(p);
+    const uint32_t *pt = p.pg.page_table + (uint64_t)s.chunk.seq * p.pg.max_pages;
+    Rows<T, HD> rows;
+    rows.load(p, s, s.r0);
+    const uint32_t first = s.lo / kSub;  // sub-tile of the item's unit 0
+    uint32_t u = s.hi > s.lo ? s.u0 + warp : s.u1;
+    uint32_t t0 = (first + u) * kSub;
+    PagePair pg = look_up(pt, t0, s.lo, s.hi);
+    if (u < s.u1) {
+      flag_bad_pages(p, pg);
+      stage<T, HD>(p, base, pg, s.head, 0, t0, s.lo, s.hi, ktile, lane, 32);
+      cp_commit();
+      stage<T, HD>(p, base, pg, s.head, 1, t0, s.lo, s.hi, vtile, lane, 32);
+      cp_commit();
+    }
+    PagePair ahead = look_up(pt, t0 + 4 * kSub, s.lo, s.hi);
+    for (; u < s.u1; u += 4) {
+      const bool more = u + 4 < s.u1;
+      const uint32_t t1 = t0 + 4 * kSub;
+      float sc[kSub / 8][4];
+      cp_wait<1>();
+      __syncwarp();
+      rows.scores(ktile, sc);
+      __syncwarp();
+      pg = ahead;
+      if (more) {
+        flag_bad_pages(p, pg);
+        stage<T, HD>(p, base, pg, s.head, 0, t1, s.lo, s.hi, ktile, lane, 32);
+      }
+      cp_commit();
+      ahead = look_up(pt, t1 + 4 * kSub, s.lo, s.hi);
+      rows.softmax(p, t0, sc);
+      cp_wait<1>();
+      __syncwarp();
+      rows.add_values(vtile, sc);
+      __syncwarp();
+      if (more) stage<T, HD>(p, base, pg, s.head, 1, t1, s.lo, s.hi, vtile, lane, 32);
+      cp_commit();
+      t0 = t1;
+    }
+    cp_wait<0>();
+    rows.finish();
+    // merge the four warps: outputs [warp][16][HD + 4], then (max, sum)
+    __syncthreads();
+    constexpr uint32_t LD = HD + 4;
+    float *scr = reinterpret_cast<float *>(dsm), *ml = scr + 4 * 16 * LD;
+#pragma unroll
+    for (uint32_t j = 0; j < HD / 8; ++j)
+#pragma unroll
+      for (uint32_t i = 0; i < 2; ++i)
+        *reinterpret_cast<float2 *>(scr + (warp * 16 + g + 8 * i) * LD + 8 * j + 2 * c) = make_float2(rows.o[j][2 * i], rows.o[j][2 * i + 1]);
+    if (c == 0)
+#pragma unroll
+      for (uint32_t i = 0; i < 2; ++i) {
+        ml[(warp * 16 + g + 8 * i) * 2] = rows.m[i];
+        ml[(warp * 16 + g + 8 * i) * 2 + 1] = rows.l[i];
+      }
+    __syncthreads();
+    const bool whole = W::whole(s);
+    float *slot = W::slot(p, s);
+    const uint32_t n_rows = s.r1 - s.r0;
+    for (uint32_t i = tid; i < n_rows * (HD / 4); i += kThreads) {
+      const uint32_t r = i / (HD / 4), d = i % (HD / 4) * 4;
+      float M = -INFINITY, L = 0.0f;
+      float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (uint32_t v = 0; v < 4; ++v) M = fmaxf(M, ml[(v * 16 + r) * 2]);
+      const float Ms = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+      for (uint32_t v = 0; v < 4; ++v) {
+        const float e = ex2(ml[(v * 16 + r) * 2] - Ms);
+        const float4 x = *reinterpret_cast<const float4 *>(scr + (v * 16 + r) * LD + d);
+        L = fmaf(ml[(v * 16 + r) * 2 + 1], e, L);
+        acc.x = fmaf(x.x, e, acc.x);
+        acc.y = fmaf(x.y, e, acc.y);
+        acc.z = fmaf(x.z, e, acc.z);
+        acc.w = fmaf(x.w, e, acc.w);
+      }
+      if (whole) {
+        const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+        T *o = out_row<T>(p, s, s.r0 + r, HD) + d;
+        if (p.aligned) {
+          *reinterpret_cast<uint2 *>(o) = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+        } else {
+          o[0] = round_to<T>(acc.x * inv);
+          o[1] = round_to<T>(acc.y * inv);
+          o[2] = round_to<T>(acc.z * inv);
+          o[3] = round_to<T>(acc.w * inv);
+        }
+      } else {
+        *reinterpret_cast<float4 *>(slot + r * HD + d) = acc;
+        if (d == 0) *reinterpret_cast<float2 *>(slot + 16 * HD + 2 * r) = make_float2(M, L);
+      }
+    }
+    if (!whole && s.u0 == 0 && tid == 0) p.desc[blockIdx.x] = w.describe(s);
+    __syncthreads();  // the next piece copies over the scratch
+  }
+  pdl_launch_dependents();
+}
+
+// ------------------------------------------------------------ up to 64 rows
+template <typename T, uint32_t HD>
+__global__ void __launch_bounds__(kThreads, 3) k_attn_rows64(const AttnChunksParams p) {
+  extern __shared__ __align__(128) uint8_t dsm[];
+  __shared__ uint64_t red[kThreads / 32 + 2];
+  constexpr uint32_t kPos = 2 * kSub, kTileBytes = kSub * HD * 2;  // a stage: K, K, V, V sub-tiles
+  using W = Walk<64, kPos, kThreads>;
+  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
+  const uint32_t smem = smem_u32(dsm);
+  const T *base = reinterpret_cast<const T *>(p.pg.base) + (uint64_t)p.layer * p.pg.layer_stride;
+  W w;
+  w.start(p, 2, red);
+  if (tid == 0) p.desc[blockIdx.x].w = 0;
+  while (!w.done()) {
+    const Segment s = w.next(p);
+    const uint32_t *pt = p.pg.page_table + (uint64_t)s.chunk.seq * p.pg.max_pages;
+    const uint32_t row0 = s.r0 + 16 * warp;
+    const bool live = row0 < s.r1;
+    Rows<T, HD> rows;
+    if (live) rows.load(p, s, row0);
+    const uint32_t first = s.lo / kPos, end = s.hi > s.lo ? s.u1 : s.u0;
+    auto fetch = [&](uint32_t u) {  // unit u to its stage; one group
+      if (u < end) {
+        const uint32_t t0 = (first + u) * kPos, st = smem + (u & 1) * 4 * kTileBytes;
+#pragma unroll
+        for (uint32_t h = 0; h < 2; ++h) {
+          const PagePair pg = look_up(pt, t0 + kSub * h, s.lo, s.hi);
+          flag_bad_pages(p, pg);
+          stage<T, HD>(p, base, pg, s.head, 0, t0 + kSub * h, s.lo, s.hi, st + h * kTileBytes, tid, kThreads);
+          stage<T, HD>(p, base, pg, s.head, 1, t0 + kSub * h, s.lo, s.hi, st + (2 + h) * kTileBytes, tid, kThreads);
+        }
+      }
+      cp_commit();
+    };
+    fetch(s.u0);
+    for (uint32_t u = s.u0; u < end; ++u) {
+      fetch(u + 1);
+      cp_wait<1>();
+      __syncthreads();
+      const uint32_t t0 = (first + u) * kPos, st = smem + (u & 1) * 4 * kTileBytes;
+#pragma unroll 1
+      for (uint32_t h = 0; h < 2; ++h) {
+        const uint32_t t = t0 + kSub * h;
+        if (!live || (int32_t)t > rows.pos_max) break;  // later than every row of the warp
+        float sc[kSub / 8][4];
+        rows.scores(st + h * kTileBytes, sc);
+        rows.softmax(p, t, sc);
+        rows.add_values(st + (2 + h) * kTileBytes, sc);
+      }
+      __syncthreads();  // the stage is fetched into again
+    }
+    cp_wait<0>();
+    __syncthreads();
+    const bool whole = W::whole(s);
+    float *slot = W::slot(p, s);
+    if (live) {
+      rows.finish();
+#pragma unroll
+      for (uint32_t i = 0; i < 2; ++i) {
+        const uint32_t row = row0 + g + 8 * i, r = row - s.r0;
+        if (row >= s.r1) continue;
+        const float inv = rows.l[i] == 0.0f ? 0.0f : 1.0f / rows.l[i];
+        T *o = out_row<T>(p, s, row, HD);
+#pragma unroll
+        for (uint32_t j = 0; j < HD / 8; ++j) {
+          const float x = rows.o[j][2 * i], y = rows.o[j][2 * i + 1];
+          const uint32_t d = 8 * j + 2 * c;
+          if (!whole) {
+            *reinterpret_cast<float2 *>(slot + r * HD + d) = make_float2(x, y);
+          } else if (p.aligned) {
+            *reinterpret_cast<uint32_t *>(o + d) = pack2<T>(x * inv, y * inv);
+          } else {
+            o[d] = round_to<T>(x * inv);
+            o[d + 1] = round_to<T>(y * inv);
+          }
+        }
+        if (!whole && c == 0) *reinterpret_cast<float2 *>(slot + 64 * HD + 2 * r) = make_float2(rows.m[i], rows.l[i]);
+      }
+    }
+    if (!whole && s.u0 == 0 && tid == 0) p.desc[blockIdx.x] = w.describe(s);
+  }
+  pdl_launch_dependents();
+}
+
+template <typename T, uint32_t HD>
+int launch_hd(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st) {
+  // up to 16 rows: two 32-position tiles a warp, and the merge's 4 x 16 rows
+  const uint32_t smem = 4 * 2 * kSub * HD * 2;
+  const uint32_t merge = 4 * 16 * (HD + 4) * 4 + 4 * 16 * 8;
+  const uint32_t bytes = smem > merge ? smem : merge;
+  const bool few = (uint64_t)p.max_q * p.rep <= 16;
+  const uint32_t grid = 3 * n_sm < kAttnMaxCtas ? 3 * n_sm : kAttnMaxCtas;
+  const void *f = few ? (const void *)k_attn_rows16<T, HD> : (const void *)k_attn_rows64<T, HD>;
+  if (cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) return -1;
+  if (few) k_attn_rows16<T, HD><<<grid, kThreads, bytes, st>>>(p);
+  else k_attn_rows64<T, HD><<<grid, kThreads, bytes, st>>>(p);
+  if (cudaGetLastError() != cudaSuccess) return -1;
+  return launch_attn_join(p, few ? 16 : 64, grid, st);
+}
+
+}  // namespace
+
+bool attn_mma_takes(const AttnChunksParams &p) {
+  return p.pg.dtype != FA_KV_F32 && (p.pg.head_dim == 64 || p.pg.head_dim == 128);
+}
+
+int launch_attn_mma(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st) {
+  if (p.pg.dtype == FA_KV_F16) return p.pg.head_dim == 64 ? launch_hd<__half, 64>(p, n_sm, st) : launch_hd<__half, 128>(p, n_sm, st);
+  return p.pg.head_dim == 64 ? launch_hd<__nv_bfloat16, 64>(p, n_sm, st) : launch_hd<__nv_bfloat16, 128>(p, n_sm, st);
+}
+
+}  // namespace fa
