@@ -11,9 +11,12 @@
 //
 // The candidates of a tile of 4096 logits: a thread's largest value that does
 // not beat the range's k-th best so far ends the matter for its 16 elements,
-// and a tile in which nothing does is passed by.  Else the k-th largest of the
-// 256 threads' largest bounds the tile's k-th best from below; what reaches the
-// bound (at most 16 k elements) is ranked against the list by counting.
+// and a tile in which nothing does is passed by.  Where more than 64 threads
+// have candidates (the first tile, rising rows) the k-th largest of the
+// threads' largest bounds the tile's k-th best from below, so that at most
+// 16 * 64 elements are left; these are ranked against the list by counting.
+// Bounding every tile made the scan 4 times as long (137 us for 256 rows of
+// 128256).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -26,7 +29,7 @@ namespace fa {
 namespace {
 
 constexpr uint32_t kScanThreads = 256, kScanElems = 16, kTile = kScanThreads * kScanElems;
-constexpr uint32_t kPickThreads = 512;
+constexpr uint32_t kPickThreads = 256;
 constexpr float kLog2e = 1.4426950408889634f;
 
 // (ordered value, lower token first) as one number; 0: no candidate
@@ -34,116 +37,139 @@ __device__ __forceinline__ unsigned long long cand_key(float x, uint32_t token) 
   return ((unsigned long long)float_key(x) << 32) | (uint32_t)~token;
 }
 
-template <typename T>
-__device__ __forceinline__ float logit(T x) {
-  const float f = (float)x;
-  return f == f ? fminf(f, FLT_MAX) : -INFINITY;  // NaN: no candidate; +inf: the largest f32
+__device__ __forceinline__ float ex2(float x) {  // 2^x, 2 ulp
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
-// 16 logits of a thread: four groups of four, group j at (j * 256 + tid) * 4
-template <typename T, bool VEC>
-__device__ __forceinline__ void load_tile(const T *row, uint32_t v0, uint32_t end, float (&x)[kScanElems]) {
+// 16 logits of a thread as they are stored: four groups of four, group j at
+// (j * 256 + tid) * 4; past the end: -inf
+template <typename T>
+struct Raw {
   struct alignas(4 * sizeof(T)) T4 {
     T e[4];
-  };
-  T4 raw[4];
+  } g[4];
+};
+template <typename T, bool VEC>
+__device__ __forceinline__ void load_tile(const T *row, uint32_t v0, uint32_t end, Raw<T> &raw) {
 #pragma unroll
   for (uint32_t j = 0; j < 4; ++j) {
     const uint32_t v = v0 + (j * kScanThreads + threadIdx.x) * 4;
     if (VEC && v + 4 <= end) {
-      raw[j] = *reinterpret_cast<const T4 *>(row + v);
+      raw.g[j] = *reinterpret_cast<const typename Raw<T>::T4 *>(row + v);
     } else {
 #pragma unroll
-      for (uint32_t e = 0; e < 4; ++e) raw[j].e[e] = v + e < end ? row[v + e] : (T)(-INFINITY);
+      for (uint32_t e = 0; e < 4; ++e) raw.g[j].e[e] = v + e < end ? row[v + e] : (T)(-INFINITY);
     }
   }
-#pragma unroll
-  for (uint32_t j = 0; j < 4; ++j)
-#pragma unroll
-    for (uint32_t e = 0; e < 4; ++e) x[4 * j + e] = logit(raw[j].e[e]);
 }
 
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(kScanThreads) k_beam_scan(const BeamParams p) {
+__global__ void __launch_bounds__(kScanThreads, 4) k_beam_scan(const BeamParams p) {
   pdl_launch_dependents();
-  __shared__ unsigned long long list[2][kBeamMaxK], tops[kScanThreads], buf[kScanElems * kBeamMaxK + kBeamMaxK];
-  __shared__ uint32_t n_buf;
+  __shared__ __align__(16) unsigned long long tops[kScanThreads];
+  __shared__ unsigned long long list[2][kBeamMaxK], buf[kScanElems * kBeamMaxK + kBeamMaxK];
+  __shared__ uint32_t n_buf[2], n_list[2];
   __shared__ unsigned long long bound;
   __shared__ float wm[kScanThreads / 32], wsum[kScanThreads / 32];
   const uint32_t row = blockIdx.y, split = blockIdx.x, tid = threadIdx.x, K = p.k;
-  if (!isfinite(p.scores[row]) || (p.done && p.done[row])) return;
   const uint32_t begin = split * p.per, end = min(p.vocab, begin + p.per);
   const T *x_row = reinterpret_cast<const T *>(p.logits) + row * p.ld;
+  const bool open = isfinite(p.scores[row]) && !(p.done && p.done[row]);
+  Raw<T> ahead;
+  if (open) load_tile<T, VEC>(x_row, begin, end, ahead);
   for (uint32_t i = tid; i < K; i += kScanThreads) list[0][i] = 0;
-  if (tid == 0) n_buf = 0;
+  if (tid < 2) n_buf[tid] = n_list[tid] = 0;
+  if (!open) return;
   uint32_t cur = 0;
   float m = -INFINITY, s = 0.0f;
   __syncthreads();
   for (uint32_t v0 = begin; v0 < end; v0 += kTile) {
     float x[kScanElems];
-    load_tile<T, VEC>(x_row, v0, end, x);
-    float t = x[0];
 #pragma unroll
-    for (uint32_t i = 1; i < kScanElems; ++i) t = fmaxf(t, x[i]);
-    if (t != -INFINITY) {
-      if (t > m) {
-        s *= exp2f((m - t) * kLog2e);
-        m = t;
-      }
+    for (uint32_t j = 0; j < 4; ++j)
 #pragma unroll
-      for (uint32_t i = 0; i < kScanElems; ++i) s += exp2f((x[i] - m) * kLog2e);
+      for (uint32_t e = 0; e < 4; ++e) x[4 * j + e] = (float)ahead.g[j].e[e];
+    if (v0 + kTile < end) load_tile<T, VEC>(x_row, v0 + kTile, end, ahead);  // in flight over the work on this one
+    float t, add;
+    for (;;) {  // a second time where there is a NaN or +inf among the 16
+      t = x[0];
+#pragma unroll
+      for (uint32_t i = 1; i < kScanElems; ++i) t = fmaxf(t, x[i]);
+      const float r = t == -INFINITY ? 0.0f : t;
+      add = 0.0f;
+      float a[4] = {};
+#pragma unroll
+      for (uint32_t i = 0; i < kScanElems; ++i) a[i % 4] += ex2((x[i] - r) * kLog2e);
+      add = (a[0] + a[1]) + (a[2] + a[3]);
+      if (add == add) break;  // +inf - +inf is NaN too
+#pragma unroll
+      for (uint32_t i = 0; i < kScanElems; ++i) x[i] = x[i] == x[i] ? fminf(x[i], FLT_MAX) : -INFINITY;
     }
-    // the thread's best element (the lowest token among equals)
-    unsigned long long best = 0;
+    if (t > m) {
+      s = fmaf(s, ex2((m - t) * kLog2e), add);
+      m = t;
+    } else if (t != -INFINITY) {
+      s = fmaf(add, ex2((t - m) * kLog2e), s);
+    }
+    // does the thread's largest element beat the list's last?  (A later equal
+    // token does not.)
     const unsigned long long kth = list[cur][K - 1];
-    if (t != -INFINITY && float_key(t) > (uint32_t)(kth >> 32)) {  // a later equal token does not beat the list's
+    const float kv = kth ? key_float((uint32_t)(kth >> 32)) : -INFINITY;
+    const bool beats = t > kv;
+    const uint32_t n_tops = __syncthreads_count(beats);
+    if (!n_tops) continue;
+    unsigned long long low = 1;
+    if (n_tops > kBeamMaxK) {  // too many for the buffer, as in the first tile: bound them
+      unsigned long long best = 0;
+      if (beats) {
 #pragma unroll
-      for (int i = kScanElems - 1; i >= 0; --i)
-        if (x[i] == t) best = cand_key(t, v0 + (i / 4 * kScanThreads + tid) * 4 + i % 4);
-    }
-    if (!__syncthreads_or(best != 0)) continue;
-    tops[tid] = best;
-    __syncthreads();
-    uint32_t above = 0;
-    for (uint32_t i = 0; i < kScanThreads; ++i) above += tops[i] > best;
-    if (best && above == K - 1) bound = best;
-    const uint32_t n_tops = __syncthreads_count(best != 0);
-    const unsigned long long low = n_tops >= K ? bound : 1;
-    if (best >= low && best) {
-#pragma unroll
-      for (uint32_t i = 0; i < kScanElems; ++i) {
-        const unsigned long long c =
-            x[i] == -INFINITY ? 0 : cand_key(x[i], v0 + (i / 4 * kScanThreads + tid) * 4 + i % 4);
-        if (c >= low && c > kth) buf[atomicAdd(&n_buf, 1u)] = c;
+        for (int i = kScanElems - 1; i >= 0; --i)
+          if (x[i] == t) best = cand_key(t, v0 + (i / 4 * kScanThreads + tid) * 4 + i % 4);
       }
+      tops[tid] = best;
+      __syncthreads();
+      uint32_t above = 0;
+#pragma unroll 8
+      for (uint32_t i = 0; i < kScanThreads; i += 2) {
+        const ulonglong2 o = *reinterpret_cast<const ulonglong2 *>(tops + i);
+        above += (o.x > best) + (o.y > best);
+      }
+      if (best && above == K - 1) bound = best;  // n_tops > 64 >= K: one thread's
+      __syncthreads();
+      low = bound;
+    }
+    if (beats) {
+#pragma unroll
+      for (uint32_t i = 0; i < kScanElems; ++i)
+        if (x[i] > kv) {
+          const unsigned long long c = cand_key(x[i], v0 + (i / 4 * kScanThreads + tid) * 4 + i % 4);
+          if (c >= low) buf[atomicAdd(&n_buf[cur], 1u)] = c;  // at most 16 of each of 64 threads
+        }
     }
     __syncthreads();
     // the list and the tile's candidates, ranked by counting (all keys differ)
-    const uint32_t n = n_buf;
-    if (tid < K && list[cur][tid]) buf[n + tid] = list[cur][tid];
-    __shared__ uint32_t n_old;
-    if (tid == 0) n_old = 0;
+    const uint32_t n = n_buf[cur], n_old = n_list[cur], all = n + n_old;
+    if (tid < n_old) buf[n + tid] = list[cur][tid];
+    if (tid >= 64 && tid < 64 + K) list[cur ^ 1][tid - 64] = 0;
+    if (tid == 0) n_buf[cur ^ 1] = 0;
     __syncthreads();
-    if (tid < K && list[cur][tid] && (tid + 1 == K || !list[cur][tid + 1])) n_old = tid + 1;
-    if (tid < K) list[cur ^ 1][tid] = 0;
-    __syncthreads();
-    const uint32_t all = n + n_old;
     for (uint32_t i = tid; i < all; i += kScanThreads) {
       const unsigned long long c = buf[i];
       uint32_t rank = 0;
       for (uint32_t j = 0; j < all; ++j) rank += buf[j] > c;
       if (rank < K) list[cur ^ 1][rank] = c;
     }
+    if (tid == 0) n_list[cur ^ 1] = min(all, K);
     __syncthreads();
     cur ^= 1;
-    if (tid == 0) n_buf = 0;
-    __syncthreads();
   }
   // the range's (max, sum), warps then lanes in a fixed order
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
     const float m2 = __shfl_xor_sync(0xFFFFFFFFu, m, o), s2 = __shfl_xor_sync(0xFFFFFFFFu, s, o), mm = fmaxf(m, m2);
-    if (mm != -INFINITY) s = s * exp2f((m - mm) * kLog2e) + s2 * exp2f((m2 - mm) * kLog2e);
+    if (mm != -INFINITY) s = s * ex2((m - mm) * kLog2e) + s2 * ex2((m2 - mm) * kLog2e);
     m = mm;
   }
   if (tid % 32 == 0) {
@@ -155,7 +181,7 @@ __global__ void __launch_bounds__(kScanThreads) k_beam_scan(const BeamParams p) 
     float M = -INFINITY, S = 0.0f;
     for (uint32_t w = 0; w < kScanThreads / 32; ++w) M = fmaxf(M, wm[w]);
     if (M != -INFINITY)
-      for (uint32_t w = 0; w < kScanThreads / 32; ++w) S += wsum[w] * exp2f((wm[w] - M) * kLog2e);
+      for (uint32_t w = 0; w < kScanThreads / 32; ++w) S += wsum[w] * ex2((wm[w] - M) * kLog2e);
     p.stats[row * p.splits + split] = make_float2(M, S);
   }
   for (uint32_t i = tid; i < K; i += kScanThreads) {
@@ -182,93 +208,104 @@ __device__ __forceinline__ double key_double(unsigned long long k) {
   return __longlong_as_double((k >> 63) ? (k & 0x7FFFFFFFFFFFFFFFull) : ~k);
 }
 
+// The lane of the warp's best candidate.  Field by field (scores differ in
+// their first 32 bits almost always): a maximum and a ballot each.
+__device__ __forceinline__ uint32_t best_lane(const Best &x) {
+  const uint32_t f[5] = {(uint32_t)(x.hi >> 32), (uint32_t)x.hi, (uint32_t)(x.mid >> 32), (uint32_t)x.mid, x.lo};
+  uint32_t in = 0xFFFFFFFFu;
+#pragma unroll
+  for (int i = 0; i < 5; ++i) {
+    const bool mine = (in >> (threadIdx.x & 31)) & 1;
+    const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, mine ? f[i] : 0u);
+    in = __ballot_sync(0xFFFFFFFFu, mine && f[i] == top);
+    if (!(in & (in - 1))) break;  // the same for the whole warp
+  }
+  return __ffs(in) - 1;
+}
+
 __global__ void __launch_bounds__(kPickThreads) k_beam_pick(const BeamParams p) {
-  pdl_wait();
+  constexpr uint32_t kWarps = kPickThreads / 32, kHold = 4;  // candidates a thread holds
   __shared__ double base[kBeamMaxBeams], lse[kBeamMaxBeams];  // score, log sum exp
   __shared__ uint32_t kind[kBeamMaxBeams];                    // 0 out, 1 open, 2 done
-  __shared__ Best wbest[kPickThreads / 32];
-  __shared__ uint32_t wthread[kPickThreads / 32];
+  __shared__ Best wbest[2][kWarps];
+  __shared__ uint32_t wthread[2][kWarps];
   __shared__ Best won[kBeamMaxK];
   const uint32_t b = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, NB = p.n_beams, K = p.k;
-  for (uint32_t j = warp; j < NB; j += kPickThreads / 32) {
-    const uint32_t row = b * NB + j;
-    const float sc = p.scores[row];
-    const uint32_t kd = !isfinite(sc) ? 0 : (p.done && p.done[row]) ? 2 : 1;
-    if (kd == 1) {
-      const float2 st = lane < p.splits ? p.stats[row * p.splits + lane] : make_float2(-INFINITY, 0.0f);
-      float M = st.x;
-#pragma unroll
-      for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xFFFFFFFFu, M, o));
-      double S = st.x == -INFINITY ? 0.0 : (double)st.y * exp((double)st.x - (double)M);
-#pragma unroll
-      for (int o = 16; o; o >>= 1) S += __shfl_xor_sync(0xFFFFFFFFu, S, o);
-      if (lane == 0) lse[j] = (double)M + log(S);
-    }
-    if (lane == 0) {
-      base[j] = sc;
-      kind[j] = kd;
-    }
+  // the inputs, which the scan does not write: before it ends
+  for (uint32_t j = tid; j < NB; j += kPickThreads) {
+    const float sc = p.scores[b * NB + j];
+    const uint32_t dn = p.done ? p.done[b * NB + j] : 0;
+    base[j] = sc;
+    kind[j] = !isfinite(sc) ? 0 : dn ? 2 : 1;
   }
-  __syncthreads();
   const uint32_t each = p.splits * K, N = NB * each;
   const uint2 *cand = p.cand + (uint64_t)b * N;
+  pdl_wait();
+  uint2 raw[kHold];
+#pragma unroll
+  for (uint32_t h = 0; h < kHold; ++h) {
+    const uint32_t i = tid + h * kPickThreads;
+    raw[h] = i < N ? __ldcg(cand + i) : make_uint2(0, 0);  // of a beam that is not open: not used
+  }
+  for (uint32_t j = warp; j < NB; j += kWarps) {
+    const float2 st = lane < p.splits ? __ldcg(p.stats + (b * NB + j) * p.splits + lane) : make_float2(-INFINITY, 0.0f);
+    float M = st.x;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xFFFFFFFFu, M, o));
+    double S = M == -INFINITY ? 0.0 : (double)(st.y * ex2((st.x - M) * kLog2e));
+#pragma unroll
+    for (int o = 16; o; o >>= 1) S += __shfl_xor_sync(0xFFFFFFFFu, S, o);
+    if (lane == 0) lse[j] = (double)M + log(S);
+  }
+  __syncthreads();
   // candidate i of the request; a done beam's only one stands in its first place
-  auto get = [&](uint32_t i) -> Best {
+  auto make = [&](uint32_t i, const uint2 &c) -> Best {
     const uint32_t j = i / each;
     if (kind[j] == 1) {
-      const uint2 c = cand[i];
       if (!c.x) return {0, 0, 0};
       return {double_key(base[j] + ((double)key_float(c.x) - lse[j])), (unsigned long long)~j << 32 | c.x, ~c.y};
     }
     if (kind[j] == 2 && i == j * each) return {double_key(base[j]), (unsigned long long)~j << 32, ~p.pad};
     return {0, 0, 0};
   };
+  Best held[kHold];
+#pragma unroll
+  for (uint32_t h = 0; h < kHold; ++h) {
+    const uint32_t i = tid + h * kPickThreads;
+    held[h] = i < N ? make(i, raw[h]) : Best{0, 0, 0};
+  }
   // k rounds: the best of the threads' own best; the winner looks for its next
   auto scan = [&](const Best &below) -> Best {
     Best r{0, 0, 0};
-    for (uint32_t i = tid; i < N; i += kPickThreads) {
-      const Best c = get(i);
+#pragma unroll
+    for (uint32_t h = 0; h < kHold; ++h)
+      if (better(below, held[h]) && better(held[h], r)) r = held[h];
+    for (uint32_t i = tid + kHold * kPickThreads; i < N; i += kPickThreads) {
+      const Best c = make(i, __ldcg(cand + i));
       if (better(below, c) && better(c, r)) r = c;
     }
     return r;
   };
   Best mine = scan(Best{~0ull, ~0ull, ~0u});
   for (uint32_t r = 0; r < K; ++r) {
-    Best w = mine;
-    uint32_t who = tid;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      Best x;
-      x.hi = __shfl_xor_sync(0xFFFFFFFFu, w.hi, o);
-      x.mid = __shfl_xor_sync(0xFFFFFFFFu, w.mid, o);
-      x.lo = __shfl_xor_sync(0xFFFFFFFFu, w.lo, o);
-      const uint32_t xw = __shfl_xor_sync(0xFFFFFFFFu, who, o);
-      if (better(x, w)) {
-        w = x;
-        who = xw;
-      }
-    }
-    if (lane == 0) {
-      wbest[warp] = w;
-      wthread[warp] = who;
+    const uint32_t buf = r & 1;
+    uint32_t l = best_lane(mine);
+    if (lane == l) {
+      wbest[buf][warp] = mine;
+      wthread[buf][warp] = tid;
     }
     __syncthreads();
-    w = wbest[0];
-    who = wthread[0];
-#pragma unroll
-    for (uint32_t i = 1; i < kPickThreads / 32; ++i)
-      if (better(wbest[i], w)) {
-        w = wbest[i];
-        who = wthread[i];
-      }
-    if (tid == 0) won[r] = w;
-    if (w.hi == 0) {  // nothing is left: the same for every thread
+    const Best w = lane < kWarps ? wbest[buf][lane] : Best{0, 0, 0};
+    l = best_lane(w);
+    if (l >= kWarps) l = 0;  // nothing is left anywhere: all are {0, 0, 0}
+    const Best top = wbest[buf][l];
+    if (tid == 0) won[r] = top;
+    if (top.hi == 0) {  // the same for every thread
       if (tid == 0)
         for (uint32_t i = r; i < K; ++i) won[i] = Best{0, 0, 0};
       break;
     }
-    if (tid == who) mine = scan(w);
-    __syncthreads();
+    if (tid == wthread[buf][l]) mine = scan(top);
   }
   __syncthreads();
   for (uint32_t r = tid; r < K; r += kPickThreads) {
@@ -304,11 +341,12 @@ int launch_t(const BeamParams &p, cudaStream_t st) {
 
 }  // namespace
 
-// Ranges of a row: enough CTAs to fill the GPU twice over, none smaller than a
-// tile.
+// Ranges of a row: as many CTAs as the GPU holds at once (four an SM), none
+// smaller than a tile.  (One more range a row than that, for 256 rows, ran a
+// second wave of a third of the SMs: 75 us.)
 uint32_t beam_splits(uint32_t rows, uint32_t vocab, uint32_t *per) {
   const uint32_t tiles = (vocab + kTile - 1) / kTile;
-  uint32_t want = rows ? (4 * 148 + rows - 1) / rows : 1;
+  uint32_t want = rows ? 4 * 148 / rows : 1;
   if (want > kBeamMaxSplits) want = kBeamMaxSplits;
   if (want > tiles) want = tiles;
   if (!want) want = 1;

@@ -206,47 +206,86 @@ __global__ void __launch_bounds__(kAnyThreads) k_attn_any(const AttnChunksParams
   pdl_launch_dependents();
 }
 
-// The item that CTA blockIdx.x of the launch before began and others finished:
-// a warp a row, the pieces in the order of the positions.
+// The item that CTA blockIdx.x of the launch before began and others finished.
+// A row at a time: warp w adds the pieces w, w + 8, .. in the order of the
+// positions (four loads in flight each), then the warps' sums are added in
+// order.  With a warp to a whole row the 60 pieces of one long cache were one
+// chain of loads: 44 us for 8 kv heads x 4 rows, against 4 us so.
+constexpr uint32_t kJoinWarps = 8;
 template <typename T>
-__global__ void __launch_bounds__(256) k_attn_join(const AttnChunksParams p, uint32_t R) {
+__global__ void __launch_bounds__(kJoinWarps * 32) k_attn_join(const AttnChunksParams p, uint32_t R) {
+  __shared__ float part[kJoinWarps][kMaxHeadDim];
+  __shared__ float wm[kJoinWarps], wl[kJoinWarps];
   pdl_wait();
   const uint4 d = p.desc[blockIdx.x];
   if (!d.w) return;
-  const uint32_t hd = p.pg.head_dim, lane = threadIdx.x & 31, head = d.z & 0xFFFF, rows = d.z >> 16;
+  const uint32_t hd = p.pg.head_dim, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, head = d.z & 0xFFFF, rows = d.z >> 16;
   const uint64_t slot = (uint64_t)R * (hd + 2);
   const float *first = p.part + ((uint64_t)blockIdx.x * 2 + 1) * slot;
   // piece i: slot 1 of this CTA, then slot 0 of the next ones
   auto piece = [&](uint32_t i) { return i ? first + (2 * (uint64_t)i - 1) * slot : first; };
-  for (uint32_t r = blockIdx.y * 8 + threadIdx.x / 32; r < rows; r += gridDim.y * 8) {
-    float M = -INFINITY;
-    for (uint32_t i = lane; i < d.w; i += 32) M = fmaxf(M, __ldcg(piece(i) + R * hd + 2 * r));
+  for (uint32_t r = blockIdx.y; r < rows; r += gridDim.y) {
+    // running maximum, sum and output of this warp's pieces (a piece's maximum
+    // is -inf where its row saw nothing there: weight 0)
+    float m = -INFINITY, l = 0.0f, acc[kMaxHeadDim / 32] = {};
+    for (uint32_t i0 = warp; i0 < d.w; i0 += 4 * kJoinWarps) {
+      float2 ml[4];
+      float x[4][kMaxHeadDim / 32];
 #pragma unroll
-    for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xFFFFFFFFu, M, o));
-    const float Ms = M == -INFINITY ? 0.0f : M;
-    float L = 0.0f, acc[kMaxHeadDim / 32] = {};
-    for (uint32_t i0 = 0; i0 < d.w; i0 += 32) {
-      float wt = 0.0f, l = 0.0f;
-      if (i0 + lane < d.w) {
-        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(piece(i0 + lane) + R * hd + 2 * r));
-        wt = exp2f(ml.x - Ms);
-        l = ml.y * wt;
-      }
-      const uint32_t n = min(32u, d.w - i0);
-      for (uint32_t i = 0; i < n; ++i) {
-        const float e = __shfl_sync(0xFFFFFFFFu, wt, i);
-        L += __shfl_sync(0xFFFFFFFFu, l, i);
-        const float *o = piece(i0 + i) + r * hd;
+      for (uint32_t k = 0; k < 4; ++k) {
+        const uint32_t i = i0 + k * kJoinWarps;
+        ml[k] = make_float2(-INFINITY, 0.0f);
+        if (i < d.w) {
+          const float *q = piece(i);
+          ml[k] = __ldcg(reinterpret_cast<const float2 *>(q + R * hd + 2 * r));
 #pragma unroll
-        for (uint32_t j = 0; j < kMaxHeadDim / 32; ++j)
-          if (lane + 32 * j < hd) acc[j] = fmaf(__ldcg(o + lane + 32 * j), e, acc[j]);
+          for (uint32_t j = 0; j < kMaxHeadDim / 32; ++j)
+            x[k][j] = lane + 32 * j < hd ? __ldcg(q + r * hd + lane + 32 * j) : 0.0f;
+        } else {
+#pragma unroll
+          for (uint32_t j = 0; j < kMaxHeadDim / 32; ++j) x[k][j] = 0.0f;
+        }
       }
+      const float mn = fmaxf(fmaxf(fmaxf(m, ml[0].x), fmaxf(ml[1].x, ml[2].x)), ml[3].x), ms = mn == -INFINITY ? 0.0f : mn;
+      const float f = exp2f(m - ms);
+      l *= f;
+#pragma unroll
+      for (uint32_t j = 0; j < kMaxHeadDim / 32; ++j) acc[j] *= f;
+#pragma unroll
+      for (uint32_t k = 0; k < 4; ++k) {
+        const float e = exp2f(ml[k].x - ms);
+        l = fmaf(ml[k].y, e, l);
+#pragma unroll
+        for (uint32_t j = 0; j < kMaxHeadDim / 32; ++j) acc[j] = fmaf(x[k][j], e, acc[j]);
+      }
+      m = mn;
     }
-    const uint32_t row = d.y + r;
-    T *out = reinterpret_cast<T *>(p.out) + (uint64_t)(d.x + row / p.rep) * p.os + (head * p.rep + row % p.rep) * hd;
+    __syncthreads();  // the row before has been read
+    if (lane == 0) {
+      wm[warp] = m;
+      wl[warp] = l;
+    }
 #pragma unroll
     for (uint32_t j = 0; j < kMaxHeadDim / 32; ++j)
-      if (lane + 32 * j < hd) put(out + lane + 32 * j, L == 0.0f ? 0.0f : acc[j] / L);
+      if (lane + 32 * j < hd) part[warp][lane + 32 * j] = acc[j];
+    __syncthreads();
+    const uint32_t row = d.y + r;
+    T *out = reinterpret_cast<T *>(p.out) + (uint64_t)(d.x + row / p.rep) * p.os + (head * p.rep + row % p.rep) * hd;
+    float M = wm[0], L = 0.0f, e[kJoinWarps];
+#pragma unroll
+    for (uint32_t w = 1; w < kJoinWarps; ++w) M = fmaxf(M, wm[w]);
+    const float Ms = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+    for (uint32_t w = 0; w < kJoinWarps; ++w) {
+      e[w] = exp2f(wm[w] - Ms);
+      L = fmaf(wl[w], e[w], L);
+    }
+    for (uint32_t x = threadIdx.x; x < hd; x += kJoinWarps * 32) {
+      float y = 0.0f;
+#pragma unroll
+      for (uint32_t w = 0; w < kJoinWarps; ++w) y = fmaf(part[w][x], e[w], y);
+      put(out + x, L == 0.0f ? 0.0f : y / L);
+    }
   }
 }
 
@@ -285,7 +324,7 @@ int launch_attn_any(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st) {
 }
 
 int launch_attn_join(const AttnChunksParams &p, uint32_t R, uint32_t ctas, cudaStream_t st) {
-  const dim3 grid(ctas, (R + 7) / 8), block(256);
+  const dim3 grid(ctas, R < 8 ? R : 8), block(kJoinWarps * 32);
   switch (p.pg.dtype) {
     case FA_KV_F32: return launch_pdl(k_attn_join<float>, grid, block, 0, st, p, R);
     case FA_KV_F16: return launch_pdl(k_attn_join<__half>, grid, block, 0, st, p, R);

@@ -46,10 +46,11 @@ __global__ void __launch_bounds__(kCopyThreads) k_page_copy(const PageCopyParams
 
 // grid (n_kv heads, K or V, layers x sequences); one CTA moves all kept rows of
 // one (sequence, layer, K or V, head) in ascending order, a tile of them at a
-// time: all of a tile's reads, a barrier, its writes.  keep ascends, so row j
-// comes from keep[j] >= j: what a tile writes lies at or below its own sources
-// and below every later tile's, and nothing is read after it was overwritten.
-constexpr uint32_t kCompactThreads = 256, kCompactUnroll = 8;
+// time.  keep ascends, so row j comes from keep[j] >= j: what a tile writes lies
+// at or below its own sources and below every later tile's.  So a tile may be
+// written as soon as it and all before it are read: the next tile is read
+// ahead, a barrier, this one written.
+constexpr uint32_t kCompactThreads = 256, kCompactUnroll = 4;
 __global__ void __launch_bounds__(kCompactThreads) k_page_compact(const PageCompactParams p, uint32_t row16) {
   const uint32_t h = blockIdx.x, is_v = blockIdx.y, layer = blockIdx.z % p.pg.n_layers, i = blockIdx.z / p.pg.n_layers;
   const uint32_t seq = p.seq[i], k0 = p.start[i], k1 = p.start[i + 1];
@@ -63,35 +64,42 @@ __global__ void __launch_bounds__(kCompactThreads) k_page_compact(const PageComp
   uint4 *base = reinterpret_cast<uint4 *>(static_cast<char *>(p.pg.base) + (uint64_t)layer * p.pg.layer_stride * esz);
   const uint64_t page16 = (uint64_t)2 * p.pg.n_kv_heads * kPageLen * row16;
   const uint64_t block = (uint64_t)(is_v * p.pg.n_kv_heads + h) * kPageLen * row16;
-  const uint32_t total = n * row16;  // cap * row16 <= 2^26 * 64: checked on the host
+  const uint32_t total = n * row16;  // below 2^25 * 64: checked on the host
   uint32_t bad = 0;
-  for (uint32_t e0 = 0; e0 < total; e0 += kCompactThreads * kCompactUnroll) {
+  constexpr uint64_t kNone = ~0ull;
+  struct Tile {
     uint4 v[kCompactUnroll];
     uint64_t to[kCompactUnroll];
+  } cur, nxt;
+  auto read = [&](uint32_t e0, Tile &t) {
 #pragma unroll
     for (uint32_t u = 0; u < kCompactUnroll; ++u) {
       const uint32_t e = e0 + u * kCompactThreads + threadIdx.x, j = e / row16, c = e - j * row16;
-      to[u] = ~0ull;
-      if (e >= total) continue;
-      const uint32_t from = keep[j];
+      t.to[u] = kNone;
+      if (e0 >= total || e >= total) continue;
+      const uint32_t from = __ldg(keep + j);
       if (from == j) continue;
-      if (from < j || from >= cap || (j && keep[j - 1] >= from)) {
+      if (from < j || from >= cap || (j && __ldg(keep + j - 1) >= from)) {
         bad |= kFlagRange;
         continue;
       }
-      const uint32_t sp = pt[from / kPageLen], dp = pt[j / kPageLen];
+      const uint32_t sp = __ldg(pt + from / kPageLen), dp = __ldg(pt + j / kPageLen);
       if (sp >= p.pg.n_pages || dp >= p.pg.n_pages) {
         bad |= kFlagPage;
         continue;
       }
-      v[u] = __ldcs(base + sp * page16 + block + (from % kPageLen) * row16 + c);
-      to[u] = dp * page16 + block + (j % kPageLen) * row16 + c;
+      t.v[u] = __ldcs(base + sp * page16 + block + (from % kPageLen) * row16 + c);
+      t.to[u] = dp * page16 + block + (j % kPageLen) * row16 + c;
     }
+  };
+  read(0, cur);
+  for (uint32_t e0 = 0; e0 < total; e0 += kCompactThreads * kCompactUnroll) {
+    read(e0 + kCompactThreads * kCompactUnroll, nxt);
     __syncthreads();
 #pragma unroll
     for (uint32_t u = 0; u < kCompactUnroll; ++u)
-      if (to[u] != ~0ull) __stcs(base + to[u], v[u]);
-    __syncthreads();
+      if (cur.to[u] != kNone) __stcs(base + cur.to[u], cur.v[u]);
+    cur = nxt;
   }
   if (bad && p.err) atomicOr(p.err, bad);
 }
