@@ -308,10 +308,8 @@ int fa_attn_chunks(const fa_pages *pages, uint32_t layer, const void *q, uint64_
   p.window = window;
   p.aligned = reinterpret_cast<uintptr_t>(q) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0 &&
               q_stride * es % 16 == 0 && out_stride * es % 16 == 0;
-  p.part = static_cast<float *>(ws);
-  p.desc = reinterpret_cast<uint4 *>(static_cast<char *>(ws) + attn_chunks_ws(pages->head_dim)) - attn_max_ctas();
   p.err = err;
-  return launched(who, launch_attn_chunks(p, (uint32_t)dev.sms(), (cudaStream_t)stream));
+  return launched(who, launch_attn_chunks(p, ws, (uint32_t)dev.sms(), (cudaStream_t)stream));
 }
 
 // ------------------------------------------------------------ pages

@@ -199,14 +199,22 @@ struct Walk {
     return p.part + ((uint64_t)blockIdx.x * 2 + (s.u0 ? 0 : 1)) * R * (p.pg.head_dim + 2);
   }
 };
-// joins the pieces of split items (R: rows of an item; ctas: grid of the launch before)
-int launch_attn_join(const AttnChunksParams &p, uint32_t R, uint32_t ctas, cudaStream_t st);
-int launch_attn_any(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st);
+// Split items of one launch, as k_attn_join takes them.
+struct JoinSet {
+  const float *part;
+  const uint4 *desc;
+  uint32_t R, ctas;
+};
+// The kernels; each returns its grid, or 0 where the launch failed.
 bool attn_mma_takes(const AttnChunksParams &p);
-int launch_attn_mma(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st);
+uint32_t launch_attn_any(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st, uint32_t *R);
+uint32_t launch_attn_mma(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st, uint32_t *R);
+uint32_t launch_attn_tc(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st);
 
-constexpr uint32_t kAttnMaxCtas = 480;  // most CTAs of a launch (the workspace holds two slots of each)
-constexpr uint32_t kAttnMaxRows = 64;   // most rows of an item
+// Most CTAs and rows of an item of the launch for few rows, and of the launch
+// for many: what the workspace holds two slots of each for.
+constexpr uint32_t kAttnMaxCtas = 480, kAttnMaxRows = 64;
+constexpr uint32_t kTcMaxCtas = 160, kTcRows = 256;
 
 // element offset of (page, k | v, head, position in page) in a layer
 __device__ __forceinline__ uint64_t page_row(const fa_pages &pg, uint32_t page, uint32_t is_v, uint32_t h, uint32_t slot) {

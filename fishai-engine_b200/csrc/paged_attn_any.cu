@@ -206,144 +206,38 @@ __global__ void __launch_bounds__(kAnyThreads) k_attn_any(const AttnChunksParams
   pdl_launch_dependents();
 }
 
-// The item that CTA blockIdx.x of the launch before began and others finished.
-// A row at a time: warp w adds the pieces w, w + 8, .. in the order of the
-// positions (four loads in flight each), then the warps' sums are added in
-// order.  With a warp to a whole row the 60 pieces of one long cache were one
-// chain of loads: 44 us for 8 kv heads x 4 rows, against 4 us so.
-constexpr uint32_t kJoinWarps = 8;
-template <typename T>
-__global__ void __launch_bounds__(kJoinWarps * 32) k_attn_join(const AttnChunksParams p, uint32_t R) {
-  __shared__ float part[kJoinWarps][kMaxHeadDim];
-  __shared__ float wm[kJoinWarps], wl[kJoinWarps];
-  pdl_wait();
-  const uint4 d = p.desc[blockIdx.x];
-  if (!d.w) return;
-  const uint32_t hd = p.pg.head_dim, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, head = d.z & 0xFFFF, rows = d.z >> 16;
-  const uint64_t slot = (uint64_t)R * (hd + 2);
-  const float *first = p.part + ((uint64_t)blockIdx.x * 2 + 1) * slot;
-  // piece i: slot 1 of this CTA, then slot 0 of the next ones
-  auto piece = [&](uint32_t i) { return i ? first + (2 * (uint64_t)i - 1) * slot : first; };
-  for (uint32_t r = blockIdx.y; r < rows; r += gridDim.y) {
-    // running maximum, sum and output of this warp's pieces (a piece's maximum
-    // is -inf where its row saw nothing there: weight 0)
-    float m = -INFINITY, l = 0.0f, acc[kMaxHeadDim / 32] = {};
-    for (uint32_t i0 = warp; i0 < d.w; i0 += 4 * kJoinWarps) {
-      float2 ml[4];
-      float x[4][kMaxHeadDim / 32];
-#pragma unroll
-      for (uint32_t k = 0; k < 4; ++k) {
-        const uint32_t i = i0 + k * kJoinWarps;
-        ml[k] = make_float2(-INFINITY, 0.0f);
-        if (i < d.w) {
-          const float *q = piece(i);
-          ml[k] = __ldcg(reinterpret_cast<const float2 *>(q + R * hd + 2 * r));
-#pragma unroll
-          for (uint32_t j = 0; j < kMaxHeadDim / 32; ++j)
-            x[k][j] = lane + 32 * j < hd ? __ldcg(q + r * hd + lane + 32 * j) : 0.0f;
-        } else {
-#pragma unroll
-          for (uint32_t j = 0; j < kMaxHeadDim / 32; ++j) x[k][j] = 0.0f;
-        }
-      }
-      const float mn = fmaxf(fmaxf(fmaxf(m, ml[0].x), fmaxf(ml[1].x, ml[2].x)), ml[3].x), ms = mn == -INFINITY ? 0.0f : mn;
-      const float f = exp2f(m - ms);
-      l *= f;
-#pragma unroll
-      for (uint32_t j = 0; j < kMaxHeadDim / 32; ++j) acc[j] *= f;
-#pragma unroll
-      for (uint32_t k = 0; k < 4; ++k) {
-        const float e = exp2f(ml[k].x - ms);
-        l = fmaf(ml[k].y, e, l);
-#pragma unroll
-        for (uint32_t j = 0; j < kMaxHeadDim / 32; ++j) acc[j] = fmaf(x[k][j], e, acc[j]);
-      }
-      m = mn;
-    }
-    __syncthreads();  // the row before has been read
-    if (lane == 0) {
-      wm[warp] = m;
-      wl[warp] = l;
-    }
-#pragma unroll
-    for (uint32_t j = 0; j < kMaxHeadDim / 32; ++j)
-      if (lane + 32 * j < hd) part[warp][lane + 32 * j] = acc[j];
-    __syncthreads();
-    const uint32_t row = d.y + r;
-    T *out = reinterpret_cast<T *>(p.out) + (uint64_t)(d.x + row / p.rep) * p.os + (head * p.rep + row % p.rep) * hd;
-    float M = wm[0], L = 0.0f, e[kJoinWarps];
-#pragma unroll
-    for (uint32_t w = 1; w < kJoinWarps; ++w) M = fmaxf(M, wm[w]);
-    const float Ms = M == -INFINITY ? 0.0f : M;
-#pragma unroll
-    for (uint32_t w = 0; w < kJoinWarps; ++w) {
-      e[w] = exp2f(wm[w] - Ms);
-      L = fmaf(wl[w], e[w], L);
-    }
-    for (uint32_t x = threadIdx.x; x < hd; x += kJoinWarps * 32) {
-      float y = 0.0f;
-#pragma unroll
-      for (uint32_t w = 0; w < kJoinWarps; ++w) y = fmaf(part[w][x], e[w], y);
-      put(out + x, L == 0.0f ? 0.0f : y / L);
-    }
-  }
-}
-
 template <typename T, uint32_t R, uint32_t HJ>
-int launch_hj(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st) {
+uint32_t launch_hj(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st, uint32_t *rows) {
   const uint32_t smem = any_smem(R, p.pg.head_dim);
   if (cudaFuncSetAttribute(k_attn_any<T, R, HJ>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)any_smem(R, 64 * HJ)) !=
       cudaSuccess)
-    return -1;
+    return 0;
   uint32_t per_sm = 224 * 1024 / (smem + 1024);
   per_sm = per_sm > 3 ? 3 : per_sm;
   const uint32_t grid = n_sm * per_sm < kAttnMaxCtas ? n_sm * per_sm : kAttnMaxCtas;
   k_attn_any<T, R, HJ><<<grid, kAnyThreads, smem, st>>>(p);
-  if (cudaGetLastError() != cudaSuccess) return -1;
-  return launch_attn_join(p, R, grid, st);
+  *rows = R;
+  return cudaGetLastError() == cudaSuccess ? grid : 0;
 }
 template <typename T>
-int launch_any_t(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st) {
+uint32_t launch_any_t(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st, uint32_t *rows) {
   const uint32_t hd = p.pg.head_dim;
   // items of 8 rows while no chunk has more: a decode's 1 to 8 rows would leave
   // most of 32 idle in the FMA loops
   const bool few = (uint64_t)p.max_q * p.rep <= 8;
-  if (hd <= 64) return few ? launch_hj<T, 8, 1>(p, n_sm, st) : launch_hj<T, 32, 1>(p, n_sm, st);
-  if (hd <= 128) return few ? launch_hj<T, 8, 2>(p, n_sm, st) : launch_hj<T, 32, 2>(p, n_sm, st);
-  return few ? launch_hj<T, 8, 4>(p, n_sm, st) : launch_hj<T, 32, 4>(p, n_sm, st);
+  if (hd <= 64) return few ? launch_hj<T, 8, 1>(p, n_sm, st, rows) : launch_hj<T, 32, 1>(p, n_sm, st, rows);
+  if (hd <= 128) return few ? launch_hj<T, 8, 2>(p, n_sm, st, rows) : launch_hj<T, 32, 2>(p, n_sm, st, rows);
+  return few ? launch_hj<T, 8, 4>(p, n_sm, st, rows) : launch_hj<T, 32, 4>(p, n_sm, st, rows);
 }
 
 }  // namespace
 
-int launch_attn_any(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st) {
+uint32_t launch_attn_any(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st, uint32_t *R) {
   switch (p.pg.dtype) {
-    case FA_KV_F32: return launch_any_t<float>(p, n_sm, st);
-    case FA_KV_F16: return launch_any_t<__half>(p, n_sm, st);
-    default: return launch_any_t<__nv_bfloat16>(p, n_sm, st);
+    case FA_KV_F32: return launch_any_t<float>(p, n_sm, st, R);
+    case FA_KV_F16: return launch_any_t<__half>(p, n_sm, st, R);
+    default: return launch_any_t<__nv_bfloat16>(p, n_sm, st, R);
   }
-}
-
-int launch_attn_join(const AttnChunksParams &p, uint32_t R, uint32_t ctas, cudaStream_t st) {
-  const dim3 grid(ctas, R < 8 ? R : 8), block(kJoinWarps * 32);
-  switch (p.pg.dtype) {
-    case FA_KV_F32: return launch_pdl(k_attn_join<float>, grid, block, 0, st, p, R);
-    case FA_KV_F16: return launch_pdl(k_attn_join<__half>, grid, block, 0, st, p, R);
-    default: return launch_pdl(k_attn_join<__nv_bfloat16>, grid, block, 0, st, p, R);
-  }
-}
-
-size_t attn_chunks_ws(uint32_t head_dim) {
-  return kAttnMaxCtas * (sizeof(uint4) + (size_t)2 * kAttnMaxRows * (head_dim + 2) * 4);
-}
-
-uint32_t attn_max_ctas() { return kAttnMaxCtas; }
-
-int launch_attn_chunks(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st) {
-  AttnChunksParams a = p;
-  a.rows_min = 1;
-  a.rows_max = 0xFFFFFFFFu;
-  if (attn_mma_takes(a)) return launch_attn_mma(a, n_sm, st);
-  return launch_attn_any(a, n_sm, st);
 }
 
 }  // namespace fa

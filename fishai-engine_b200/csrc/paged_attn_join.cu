@@ -1,0 +1,157 @@
+// Joins the pieces of attention items that were split between CTAs, and chooses
+// the kernels of a call.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "paged_attn.cuh"
+
+namespace fa {
+namespace {
+
+__device__ __forceinline__ void put(float *p, float x) { *p = x; }
+__device__ __forceinline__ void put(__half *p, float x) { *p = __float2half_rn(x); }
+__device__ __forceinline__ void put(__nv_bfloat16 *p, float x) { *p = __float2bfloat16_rn(x); }
+
+// CTA x takes the item that CTA x of the launch before began and others
+// finished.  A row's pieces (m_i, l_i, o_i) give
+//   o = sum o_i 2^(m_i - m) / sum l_i 2^(m_i - m),  m = max m_i,
+// added in the order of the positions.  Few pieces (long prompts): a warp a
+// row.  Many (one long cache): the eight warps take the pieces in turn, four
+// loads in flight each, and their sums are added in order; with a warp to a
+// whole row the 60 pieces of one 8192-position cache were one chain of loads:
+// 44 us for 8 kv heads x 4 rows, against 6 us so.
+constexpr uint32_t kJoinWarps = 8, kJoinFew = 8, kPer = kMaxHeadDim / 32;
+
+struct Sum {
+  float m, l, acc[kPer];
+};
+// adds the pieces i0, i0 + step, .. i0 + 3 step of row r
+template <typename P>
+__device__ __forceinline__ void add4(Sum &s, P piece, uint32_t i0, uint32_t step, uint32_t n, uint32_t R, uint32_t r, uint32_t hd,
+                                     uint32_t lane) {
+  float2 ml[4];
+  float x[4][kPer];
+#pragma unroll
+  for (uint32_t k = 0; k < 4; ++k) {
+    const uint32_t i = i0 + k * step;
+    const float *q = piece(i < n ? i : 0);
+    ml[k] = i < n ? __ldcg(reinterpret_cast<const float2 *>(q + R * hd + 2 * r)) : make_float2(-INFINITY, 0.0f);
+#pragma unroll
+    for (uint32_t j = 0; j < kPer; ++j) x[k][j] = i < n && lane + 32 * j < hd ? __ldcg(q + r * hd + lane + 32 * j) : 0.0f;
+  }
+  const float mn = fmaxf(fmaxf(fmaxf(s.m, ml[0].x), fmaxf(ml[1].x, ml[2].x)), ml[3].x), ms = mn == -INFINITY ? 0.0f : mn;
+  const float f = exp2f(s.m - ms);
+  s.l *= f;
+#pragma unroll
+  for (uint32_t j = 0; j < kPer; ++j) s.acc[j] *= f;
+#pragma unroll
+  for (uint32_t k = 0; k < 4; ++k) {
+    const float e = exp2f(ml[k].x - ms);
+    s.l = fmaf(ml[k].y, e, s.l);
+#pragma unroll
+    for (uint32_t j = 0; j < kPer; ++j) s.acc[j] = fmaf(x[k][j], e, s.acc[j]);
+  }
+  s.m = mn;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kJoinWarps * 32) k_attn_join(const AttnChunksParams p, JoinSet a, JoinSet b) {
+  __shared__ float part[kJoinWarps][kMaxHeadDim];
+  __shared__ float wm[kJoinWarps], wl[kJoinWarps];
+  pdl_wait();
+  const bool second = blockIdx.x >= a.ctas;
+  const uint32_t cta = second ? blockIdx.x - a.ctas : blockIdx.x, R = second ? b.R : a.R;
+  const uint4 d = second ? b.desc[cta] : a.desc[cta];
+  if (!d.w) return;
+  const uint32_t hd = p.pg.head_dim, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, head = d.z & 0xFFFF, rows = d.z >> 16;
+  const uint64_t slot = (uint64_t)R * (hd + 2);
+  const float *first = (second ? b.part : a.part) + ((uint64_t)cta * 2 + 1) * slot;
+  // piece i: slot 1 of the CTA, then slot 0 of the next ones
+  auto piece = [&](uint32_t i) { return i ? first + (2 * (uint64_t)i - 1) * slot : first; };
+  auto out = [&](uint32_t r) {
+    const uint32_t row = d.y + r;
+    return reinterpret_cast<T *>(p.out) + (uint64_t)(d.x + row / p.rep) * p.os + (head * p.rep + row % p.rep) * hd;
+  };
+  if (d.w <= kJoinFew) {
+    for (uint32_t r = blockIdx.y * kJoinWarps + warp; r < rows; r += gridDim.y * kJoinWarps) {
+      Sum s{-INFINITY, 0.0f, {}};
+      for (uint32_t i = 0; i < d.w; i += 4) add4(s, piece, i, 1, d.w, R, r, hd, lane);
+      T *o = out(r);
+#pragma unroll
+      for (uint32_t j = 0; j < kPer; ++j)
+        if (lane + 32 * j < hd) put(o + lane + 32 * j, s.l == 0.0f ? 0.0f : s.acc[j] / s.l);
+    }
+    return;
+  }
+  for (uint32_t r = blockIdx.y; r < rows; r += gridDim.y) {
+    Sum s{-INFINITY, 0.0f, {}};
+    for (uint32_t i = warp; i < d.w; i += 4 * kJoinWarps) add4(s, piece, i, kJoinWarps, d.w, R, r, hd, lane);
+    __syncthreads();  // the row before has been read
+    if (lane == 0) {
+      wm[warp] = s.m;
+      wl[warp] = s.l;
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < kPer; ++j)
+      if (lane + 32 * j < hd) part[warp][lane + 32 * j] = s.acc[j];
+    __syncthreads();
+    float M = wm[0], L = 0.0f, e[kJoinWarps];
+#pragma unroll
+    for (uint32_t w = 1; w < kJoinWarps; ++w) M = fmaxf(M, wm[w]);
+    const float Ms = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+    for (uint32_t w = 0; w < kJoinWarps; ++w) {
+      e[w] = exp2f(wm[w] - Ms);
+      L = fmaf(wl[w], e[w], L);
+    }
+    T *o = out(r);
+    for (uint32_t x = threadIdx.x; x < hd; x += kJoinWarps * 32) {
+      float y = 0.0f;
+#pragma unroll
+      for (uint32_t w = 0; w < kJoinWarps; ++w) y = fmaf(part[w][x], e[w], y);
+      put(o + x, L == 0.0f ? 0.0f : y / L);
+    }
+  }
+}
+
+constexpr size_t kSmallSlots = (size_t)2 * kAttnMaxCtas * kAttnMaxRows, kTcSlots = (size_t)2 * kTcMaxCtas * kTcRows;
+
+}  // namespace
+
+// slots of the launch for few rows, of the one for many, descriptors
+size_t attn_chunks_ws(uint32_t head_dim) {
+  return (kSmallSlots + kTcSlots) * (head_dim + 2) * 4 + (kAttnMaxCtas + kTcMaxCtas) * sizeof(uint4);
+}
+
+int launch_attn_chunks(const AttnChunksParams &p, void *ws, uint32_t n_sm, cudaStream_t st) {
+  AttnChunksParams a = p, b = p;
+  a.part = static_cast<float *>(ws);
+  b.part = a.part + kSmallSlots * (p.pg.head_dim + 2);
+  a.desc = reinterpret_cast<uint4 *>(b.part + kTcSlots * (p.pg.head_dim + 2));
+  b.desc = a.desc + kAttnMaxCtas;
+  a.rows_min = 1;
+  a.rows_max = 0xFFFFFFFFu;
+  JoinSet ja{a.part, a.desc, 0, 0}, jb{b.part, b.desc, kTcRows, 0};
+  if (attn_mma_takes(p)) {
+    // chunks of up to 64 rows are bound by the copies of K and V, which mma.sync
+    // keeps up with; above, the 256-row items of tcgen05
+    const bool many = (uint64_t)p.max_q * p.rep > kAttnMaxRows;
+    if (many) a.rows_max = kAttnMaxRows;
+    if (!(ja.ctas = launch_attn_mma(a, n_sm, st, &ja.R))) return -1;
+    if (many) {
+      b.rows_min = kAttnMaxRows + 1;
+      b.rows_max = 0xFFFFFFFFu;
+      if (!(jb.ctas = launch_attn_tc(b, n_sm, st))) return -1;
+    }
+  } else if (!(ja.ctas = launch_attn_any(a, n_sm, st, &ja.R))) {
+    return -1;
+  }
+  const dim3 grid(ja.ctas + jb.ctas, jb.ctas ? 16 : ja.R < 8 ? ja.R : 8), block(kJoinWarps * 32);
+  switch (p.pg.dtype) {
+    case FA_KV_F32: return launch_pdl(k_attn_join<float>, grid, block, 0, st, p, ja, jb);
+    case FA_KV_F16: return launch_pdl(k_attn_join<__half>, grid, block, 0, st, p, ja, jb);
+    default: return launch_pdl(k_attn_join<__nv_bfloat16>, grid, block, 0, st, p, ja, jb);
+  }
+}
+
+}  // namespace fa

@@ -255,6 +255,7 @@ __global__ void __launch_bounds__(kThreads, 3) k_attn_rows16(const AttnChunksPar
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   const uint32_t ktile = smem_u32(dsm) + warp * 2 * kTileBytes, vtile = ktile + kTileBytes;
   const T *base = reinterpret_cast<const T *>(p.pg.base) + (uint64_t)p.layer * p.pg.layer_stride;
+  pdl_launch_dependents();
   W w;
   w.start(p, 4, red);
   if (tid == 0) p.desc[blockIdx.x].w = 0;
@@ -356,7 +357,6 @@ __global__ void __launch_bounds__(kThreads, 3) k_attn_rows16(const AttnChunksPar
     if (!whole && s.u0 == 0 && tid == 0) p.desc[blockIdx.x] = w.describe(s);
     __syncthreads();  // the next piece copies over the scratch
   }
-  pdl_launch_dependents();
 }
 
 // ------------------------------------------------------------ up to 64 rows
@@ -369,6 +369,7 @@ __global__ void __launch_bounds__(kThreads, 3) k_attn_rows64(const AttnChunksPar
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   const uint32_t smem = smem_u32(dsm);
   const T *base = reinterpret_cast<const T *>(p.pg.base) + (uint64_t)p.layer * p.pg.layer_stride;
+  pdl_launch_dependents();
   W w;
   w.start(p, 2, red);
   if (tid == 0) p.desc[blockIdx.x].w = 0;
@@ -440,11 +441,10 @@ __global__ void __launch_bounds__(kThreads, 3) k_attn_rows64(const AttnChunksPar
     }
     if (!whole && s.u0 == 0 && tid == 0) p.desc[blockIdx.x] = w.describe(s);
   }
-  pdl_launch_dependents();
 }
 
 template <typename T, uint32_t HD>
-int launch_hd(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st) {
+uint32_t launch_hd(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st, uint32_t *R) {
   // up to 16 rows: two 32-position tiles a warp, and the merge's 4 x 16 rows
   const uint32_t smem = 4 * 2 * kSub * HD * 2;
   const uint32_t merge = 4 * 16 * (HD + 4) * 4 + 4 * 16 * 8;
@@ -452,22 +452,25 @@ int launch_hd(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st) {
   const bool few = (uint64_t)p.max_q * p.rep <= 16;
   const uint32_t grid = 3 * n_sm < kAttnMaxCtas ? 3 * n_sm : kAttnMaxCtas;
   const void *f = few ? (const void *)k_attn_rows16<T, HD> : (const void *)k_attn_rows64<T, HD>;
-  if (cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) return -1;
+  if (cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) return 0;
   if (few) k_attn_rows16<T, HD><<<grid, kThreads, bytes, st>>>(p);
   else k_attn_rows64<T, HD><<<grid, kThreads, bytes, st>>>(p);
-  if (cudaGetLastError() != cudaSuccess) return -1;
-  return launch_attn_join(p, few ? 16 : 64, grid, st);
+  *R = few ? 16 : 64;
+  return cudaGetLastError() == cudaSuccess ? grid : 0;
 }
 
 }  // namespace
 
+// 16-bit types at head sizes 64 and 128; TMA counts the rows of a layer's pages
+// in 31 bits
 bool attn_mma_takes(const AttnChunksParams &p) {
-  return p.pg.dtype != FA_KV_F32 && (p.pg.head_dim == 64 || p.pg.head_dim == 128);
+  return p.pg.dtype != FA_KV_F32 && (p.pg.head_dim == 64 || p.pg.head_dim == 128) &&
+         (uint64_t)p.pg.n_pages * 2 * p.pg.n_kv_heads * kPageLen < 0x7FFFFFFFull;
 }
 
-int launch_attn_mma(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st) {
-  if (p.pg.dtype == FA_KV_F16) return p.pg.head_dim == 64 ? launch_hd<__half, 64>(p, n_sm, st) : launch_hd<__half, 128>(p, n_sm, st);
-  return p.pg.head_dim == 64 ? launch_hd<__nv_bfloat16, 64>(p, n_sm, st) : launch_hd<__nv_bfloat16, 128>(p, n_sm, st);
+uint32_t launch_attn_mma(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st, uint32_t *R) {
+  if (p.pg.dtype == FA_KV_F16) return p.pg.head_dim == 64 ? launch_hd<__half, 64>(p, n_sm, st, R) : launch_hd<__half, 128>(p, n_sm, st, R);
+  return p.pg.head_dim == 64 ? launch_hd<__nv_bfloat16, 64>(p, n_sm, st, R) : launch_hd<__nv_bfloat16, 128>(p, n_sm, st, R);
 }
 
 }  // namespace fa

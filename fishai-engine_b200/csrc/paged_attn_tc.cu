@@ -1,0 +1,516 @@
+// Attention of chunks over paged f16 / bf16 K/V with many rows per kv head, on
+// tcgen05 (head sizes 64 and 128).  Same mathematics as paged_attn_any.cu:
+//   S = Q K^T,  P = 2^(scale S - m),  O += P V,  l += row sums of P,  O / l.
+//
+// The tensor pipe bounds it, and beside it the 16 exponentials a clock and SM:
+// 128 x 128 scores take 512 clocks of MMA for S, 512 for P V (head size 128)
+// and 1024 of exponentials.  So an item is 256 rows, two Q tiles of 128, and
+// the tiles take turns: while one's scores are turned into weights, the tensor
+// pipe works on the other's.  Rows are (token, query head of the kv head)
+// pairs, so all query heads of a kv head share its K and V.
+//
+//   warps 0-3, 4-7   softmax of Q tile 0, 1: a thread a row.  Scores come from
+//                    tensor memory, weights go back over them (16 bits, as V
+//                    was rounded), read by the second MMA as its A operand.
+//   warp 8           issues the MMAs (one lane); owns the tensor memory
+//   warp 9           TMA: K and V tiles of 128 positions, a box per page of 16
+//                    (pages outside the item's range start past the end of the
+//                    tensor and arrive as zeros), 128-byte swizzle, a ring
+// Order of the MMAs per tile: P0 V, S0 of the next tile, P1 V, S1 of the next.
+// They run in the order of issue, so S0 may overwrite P0 without a wait.
+// The reference point m of a row only moves when a maximum exceeds it by 2^8:
+// weights stay below 2^8 and sums in f32 are exact to the same relative error,
+// and the output in tensor memory is rescaled only then (by the softmax warps,
+// after the P V before it is done).
+// Waits are bounded; one that runs out sets an abort flag that the others see,
+// and the kernel drains its copies and MMAs, frees the tensor memory and sets
+// FA_FLAG_TIMEOUT.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <mutex>
+
+#include "paged_attn.cuh"
+
+namespace fa {
+namespace {
+
+constexpr uint32_t kTcThreads = 384, kTcPos = 128;
+
+template <uint32_t HD>
+struct TcCfg {
+  static constexpr uint32_t kHalf = kTcPos * 128;           // 128 positions (or rows) x 64 elements
+  static constexpr uint32_t kTile = kHalf * (HD / 64);      // one of K, V, or a Q tile
+  static constexpr uint32_t kStages = HD == 128 ? 5 : 8;
+  static constexpr uint32_t kBarOff = 2 * kTile + kStages * kTile;
+  static constexpr uint32_t kSmem = 1024 + kBarOff + 512;   // alignment, barriers
+  static_assert(kSmem <= 227 * 1024, "shared memory of a CTA");
+};
+struct TcBars {
+  uint64_t full[8], empty[8], q_full[2], s_full[2], p_full[2], o_full[2], tail, done;
+  uint64_t red[kTcThreads / 32 + 2];
+  uint32_t tmem, abort;
+};
+static_assert(sizeof(TcBars) <= 512, "barrier space");
+
+// tensor memory columns: scores (and weights over them) of tile i, outputs
+__device__ __forceinline__ uint32_t s_col(uint32_t i) { return 128 * i; }
+__device__ __forceinline__ uint32_t o_col(uint32_t i) { return 256 + 128 * i; }
+
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void commit(uint64_t *bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+// descriptor of a shared-memory operand with 128-byte swizzle: 8-row groups
+// 1024 bytes apart, `lead` bytes between blocks of 64 elements (rows-contiguous
+// operand V) or unused (K, Q)
+__device__ __forceinline__ uint64_t sdesc(uint32_t addr, uint32_t lead) {
+  return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
+         ((uint64_t)2 << 61);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc),
+      "r"(0u)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc),
+      "r"(0u)
+      : "memory");
+}
+__device__ __forceinline__ void tma_2d(uint32_t dst, const void *map, int32_t x, int32_t y, uint64_t *bar) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+               "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar))
+               : "memory");
+}
+#define TC_R32(v)                                                                                                                  \
+  v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7], v[8], v[9], v[10], v[11], v[12], v[13], v[14], v[15], v[16], v[17], v[18], v[19], \
+      v[20], v[21], v[22], v[23], v[24], v[25], v[26], v[27], v[28], v[29], v[30], v[31]
+__device__ __forceinline__ void ld32(uint32_t addr, float *v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,"
+      "%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]),
+        "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]),
+        "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]),
+        "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+      : "r"(addr));
+}
+__device__ __forceinline__ void st32(uint32_t addr, const uint32_t *v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,"
+      "%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+      "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]),
+      "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]),
+      "r"(v[31])
+      : "memory");
+}
+__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ float ex2(float x) {  // 2^x, 2 ulp; below 2^-126: 0
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (__is_same(T, __half)) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+  }
+}
+
+// Bounded wait; false: it ran out here or elsewhere in the CTA
+__device__ __forceinline__ bool wait_bar(TcBars &b, uint64_t *bar, uint32_t parity) {
+  const uint32_t addr = smem_u32(bar);
+  for (uint32_t i = 0; i < kMaxWaitTries; ++i) {
+    uint32_t ok;
+    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+                 : "=r"(ok)
+                 : "r"(addr), "r"(parity)
+                 : "memory");
+    if (ok) return true;
+    if ((i & 255) == 255 && *reinterpret_cast<volatile uint32_t *>(&b.abort)) return false;
+  }
+  *reinterpret_cast<volatile uint32_t *>(&b.abort) = 1;
+  return false;
+}
+
+using TcWalk = Walk<kTcRows, kTcPos, kTcThreads>;
+
+// Q rows [first, first + 128) of the item to a swizzled tile, 128 threads
+template <typename T, uint32_t HD>
+__device__ __forceinline__ void load_q(const AttnChunksParams &p, const Segment &s, uint32_t first, uint32_t tile, uint32_t tid) {
+  constexpr uint32_t CH = HD / 8;
+#pragma unroll 4
+  for (uint32_t i = tid; i < 128 * CH; i += 128) {
+    const uint32_t r = i / CH, c = i % CH, row = first + r;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (row < s.r1) {
+      const uint32_t tok = row / p.rep;
+      const T *x = reinterpret_cast<const T *>(p.q) + (uint64_t)(s.chunk.q0 + tok) * p.qs + (s.head * p.rep + row - tok * p.rep) * HD + c * 8;
+      if (p.aligned) {
+        v = *reinterpret_cast<const uint4 *>(x);
+      } else {
+        const uint16_t *y = reinterpret_cast<const uint16_t *>(x);
+        v = make_uint4(y[0] | (uint32_t)y[1] << 16, y[2] | (uint32_t)y[3] << 16, y[4] | (uint32_t)y[5] << 16, y[6] | (uint32_t)y[7] << 16);
+      }
+    }
+    const uint32_t dst = tile + (c >> 3) * TcCfg<HD>::kHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+  }
+}
+
+template <typename T, uint32_t HD>
+__device__ void softmax_role(const AttnChunksParams &p, TcWalk w, TcBars &b, uint32_t qtile, uint32_t tmem, uint32_t g) {
+  const uint32_t tid = threadIdx.x & 127, warp = tid >> 5;
+  const uint32_t lanes = tmem + ((warp * 32) << 16);
+  uint32_t n = 0;  // tiles of this group so far
+  while (!w.done()) {
+    const Segment s = w.next(p);
+    const uint32_t row = s.r0 + 128 * g + tid;
+    if (s.r0 + 128 * g >= s.r1) continue;  // the second Q tile is empty
+    const bool live = row < s.r1, whole = TcWalk::whole(s);
+    const int32_t pos = live ? s.chunk.first + (int32_t)(row / p.rep) : -1;
+    const uint32_t tiles = s.hi > s.lo ? s.u1 - s.u0 : 0;
+    float m = -INFINITY, l = 0.0f;
+    if (tiles) {
+      load_q<T, HD>(p, s, s.r0 + 128 * g, qtile, tid);
+      fence_proxy_async_smem();
+      mbar_arrive(&b.q_full[g]);
+    }
+    for (uint32_t k = 0; k < tiles; ++k, ++n) {
+      const uint32_t t0 = (s.lo / kTcPos + s.u0 + k) * kTcPos;
+      if (!wait_bar(b, &b.s_full[g], n & 1)) return;
+      fence_after();
+      float x[kTcPos];
+#pragma unroll
+      for (uint32_t c = 0; c < 4; ++c) ld32(lanes + s_col(g) + 32 * c, x + 32 * c);
+      wait_ld();
+      // rows of a warp that see all 128 positions need no mask
+      const bool all = (int32_t)(t0 + kTcPos - 1) <= pos && (!p.window || (uint32_t)(pos - (int32_t)t0) < p.window);
+      if (!__all_sync(0xFFFFFFFFu, all)) {
+        // visible columns: [from, to)
+        const int32_t to = pos - (int32_t)t0 + 1, from = p.window ? to - (int32_t)p.window : 0;
+#pragma unroll
+        for (int32_t c = 0; c < (int32_t)kTcPos; ++c)
+          if (c >= to || c < from) x[c] = -INFINITY;
+      }
+      float mx[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+      for (uint32_t c = 4; c < kTcPos; ++c) mx[c % 4] = fmaxf(mx[c % 4], x[c]);
+      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
+      float f = 1.0f;
+      if (top > m + 8.0f) {
+        f = ex2(m - top);
+        m = top;
+        l *= f;
+      }
+      if (k && __any_sync(0xFFFFFFFFu, f != 1.0f)) {
+        if (!wait_bar(b, &b.o_full[g], (n - 1) & 1)) return;
+        fence_after();
+#pragma unroll 1
+        for (uint32_t c = 0; c < HD; c += 32) {
+          float o[32];
+          ld32(lanes + o_col(g) + c, o);
+          wait_ld();
+#pragma unroll
+          for (uint32_t e = 0; e < 32; ++e) o[e] *= f;
+          st32(lanes + o_col(g) + c, reinterpret_cast<const uint32_t *>(o));
+        }
+      }
+      const float ms = m == -INFINITY ? 0.0f : m;
+      float sum[4] = {};
+      uint32_t pk[32];
+#pragma unroll
+      for (uint32_t h = 0; h < 2; ++h) {
+#pragma unroll
+        for (uint32_t c = 0; c < 32; ++c) {
+          const float a = ex2(fmaf(x[64 * h + 2 * c], p.scale_log2, -ms)), d = ex2(fmaf(x[64 * h + 2 * c + 1], p.scale_log2, -ms));
+          sum[(2 * c) % 4] += a;
+          sum[(2 * c + 1) % 4] += d;
+          pk[c] = pack2<T>(a, d);
+        }
+        st32(lanes + s_col(g) + 32 * h, pk);
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      wait_st();
+      fence_before();
+      mbar_arrive(&b.p_full[g]);
+    }
+    float *slot = TcWalk::slot(p, s);
+    const uint32_t r = row - s.r0, tok = row / p.rep;
+    T *out = reinterpret_cast<T *>(p.out) + (uint64_t)(s.chunk.q0 + tok) * p.os + (s.head * p.rep + row - tok * p.rep) * HD;
+    if (tiles) {
+      if (!wait_bar(b, &b.o_full[g], (n - 1) & 1)) return;
+      fence_after();
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll 1
+    for (uint32_t c = 0; c < HD; c += 32) {
+      float o[32];
+      if (tiles) {
+        ld32(lanes + o_col(g) + c, o);
+        wait_ld();
+      }
+      if (!tiles || l == 0.0f) {  // no position seen, or (within a split item) none yet
+#pragma unroll
+        for (uint32_t e = 0; e < 32; ++e) o[e] = 0.0f;
+      }
+      if (!live) continue;
+      if (!whole) {
+#pragma unroll
+        for (uint32_t e = 0; e < 32; e += 4) *reinterpret_cast<float4 *>(slot + r * HD + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+      } else if (p.aligned) {
+#pragma unroll
+        for (uint32_t e = 0; e < 32; e += 8)
+          *reinterpret_cast<uint4 *>(out + c + e) = make_uint4(pack2<T>(o[e] * inv, o[e + 1] * inv), pack2<T>(o[e + 2] * inv, o[e + 3] * inv),
+                                                              pack2<T>(o[e + 4] * inv, o[e + 5] * inv), pack2<T>(o[e + 6] * inv, o[e + 7] * inv));
+      } else {
+#pragma unroll
+        for (uint32_t e = 0; e < 32; e += 2) {
+          const uint32_t v = pack2<T>(o[e] * inv, o[e + 1] * inv);
+          reinterpret_cast<uint16_t *>(out)[c + e] = (uint16_t)v;
+          reinterpret_cast<uint16_t *>(out)[c + e + 1] = (uint16_t)(v >> 16);
+        }
+      }
+    }
+    if (!whole && live) *reinterpret_cast<float2 *>(slot + kTcRows * HD + 2 * r) = make_float2(m, l);
+    if (!whole && s.u0 == 0 && g == 0 && tid == 0) p.desc[blockIdx.x] = w.describe(s);
+    fence_before();  // the next item's MMAs follow its q_full and p_full arrivals
+  }
+}
+
+template <typename T, uint32_t HD>
+__device__ void mma_role(const AttnChunksParams &p, TcWalk w, TcBars &b, uint32_t smem, uint32_t tmem) {
+  using C = TcCfg<HD>;
+  constexpr uint32_t kType = __is_same(T, __half) ? 0u : 1u;  // f16 / bf16, A and B
+  constexpr uint32_t kS = (1u << 4) | (kType << 7) | (kType << 10) | ((kTcPos / 8) << 17) | ((128 / 16) << 24);
+  constexpr uint32_t kO = (1u << 4) | (kType << 7) | (kType << 10) | (1u << 16) | ((HD / 8) << 17) | ((128 / 16) << 24);  // B = V: rows are K
+  const uint32_t ring = smem + 2 * C::kTile;
+  uint32_t seq = 0, n[2] = {0, 0}, q_phase[2] = {0, 0};
+  auto stage = [&](uint32_t i) { return ring + i % C::kStages * C::kTile; };
+  auto filled = [&](uint32_t i) { return wait_bar(b, &b.full[i % C::kStages], i / C::kStages & 1); };
+  auto scores = [&](uint32_t g, uint32_t kt) {
+    const uint32_t q = smem + g * C::kTile, k = stage(kt);
+#pragma unroll
+    for (uint32_t kk = 0; kk < HD / 16; ++kk) {
+      const uint32_t off = kk / 4 * C::kHalf + kk % 4 * 32;
+      mma_ss(tmem + s_col(g), sdesc(q + off, 16), sdesc(k + off, 16), kS, kk);
+    }
+    commit(&b.s_full[g]);
+  };
+  while (!w.done()) {
+    const Segment s = w.next(p);
+    const uint32_t tiles = s.hi > s.lo ? s.u1 - s.u0 : 0, groups = s.r1 - s.r0 > 128 ? 2 : 1;
+    if (!tiles) continue;
+    for (uint32_t g = 0; g < groups; ++g) {
+      if (!wait_bar(b, &b.q_full[g], q_phase[g])) return;
+      q_phase[g] ^= 1;
+    }
+    // fills come K0 V0 K1 V1 ..
+    if (!filled(seq)) return;
+    fence_after();
+    for (uint32_t g = 0; g < groups; ++g) scores(g, seq);
+    commit(&b.empty[seq % C::kStages]);
+    for (uint32_t k = 0; k < tiles; ++k) {
+      const uint32_t v = seq + 1, next = seq + 2;
+      const bool more = k + 1 < tiles;
+      if (!filled(v)) return;
+      for (uint32_t g = 0; g < groups; ++g) {
+        if (!wait_bar(b, &b.p_full[g], n[g] & 1)) return;
+        ++n[g];
+        fence_after();
+#pragma unroll
+        for (uint32_t kk = 0; kk < kTcPos / 16; ++kk)
+          mma_ts(tmem + o_col(g), tmem + s_col(g) + 8 * kk, sdesc(stage(v) + kk * 2048, C::kHalf), kO, k || kk);
+        commit(&b.o_full[g]);
+        if (g + 1 == groups) commit(&b.empty[v % C::kStages]);
+        if (more) {
+          if (g == 0 && !filled(next)) return;
+          scores(g, next);
+        }
+      }
+      if (more) commit(&b.empty[next % C::kStages]);
+      seq += 2;
+    }
+  }
+}
+
+// one warp
+template <typename T, uint32_t HD>
+__device__ void load_role(const AttnChunksParams &p, TcWalk w, TcBars &b, uint32_t smem, const CUtensorMap *map, uint32_t &fills) {
+  using C = TcCfg<HD>;
+  const uint32_t lane = threadIdx.x & 31, ring = smem + 2 * C::kTile;
+  const int32_t none = (int32_t)(p.pg.n_pages * 2 * p.pg.n_kv_heads * kPageLen);  // a row past the end: zeros
+  uint32_t seq = 0, tail = 0;
+  while (!w.done()) {
+    const Segment s = w.next(p);
+    const uint32_t tiles = s.hi > s.lo ? s.u1 - s.u0 : 0;
+    const uint32_t *pt = p.pg.page_table + (uint64_t)s.chunk.seq * p.pg.max_pages;
+    const uint32_t first = (s.lo / kTcPos + s.u0) * kTcPos;
+    auto look_up = [&](uint32_t t0) -> uint32_t {  // the lane's page of the tile
+      const uint32_t t = t0 + (lane & 7) * kPageLen;
+      return t < s.hi && t + kPageLen > s.lo ? __ldg(pt + t / kPageLen) : 0xFFFFFFFFu;
+    };
+    uint32_t ahead = tiles ? look_up(first) : 0;
+    for (uint32_t k = 0; k < tiles; ++k) {
+      const uint32_t t0 = first + k * kTcPos, page = ahead;
+      if (k + 1 < tiles) ahead = look_up(t0 + kTcPos);
+      const bool used = t0 + (lane & 7) * kPageLen < s.hi && t0 + (lane & 7) * kPageLen + kPageLen > s.lo;
+      if (used && page >= p.pg.n_pages && p.err) atomicOr(p.err, kFlagPage);
+      // slots of a page that nobody sees: V must not be NaN there (its weight 0
+      // would not help)
+      const bool ragged = (s.hi < t0 + kTcPos && s.hi % kPageLen) || (s.lo > t0 && s.lo % kPageLen);
+      for (uint32_t is_v = 0; is_v < 2; ++is_v, ++seq) {
+        const uint32_t st = seq % C::kStages, dst = ring + st * C::kTile;
+        if (!wait_bar(b, &b.empty[st], (seq / C::kStages & 1) ^ 1)) return;
+        uint64_t *bar = is_v && ragged ? &b.tail : &b.full[st];
+        if (lane == 0) mbar_arrive_expect_tx(bar, C::kTile);
+        __syncwarp();
+        if (lane < 8 * (HD / 64)) {
+          const int32_t y = page < p.pg.n_pages ? (int32_t)(((page * 2 + is_v) * p.pg.n_kv_heads + s.head) * kPageLen) : none;
+          tma_2d(dst + (lane >> 3) * C::kHalf + (lane & 7) * 2048, map, (int32_t)(lane >> 3) * 64, y, bar);
+        }
+        if (is_v && ragged) {
+          if (!mbar_wait(&b.tail, tail & 1)) {
+            *reinterpret_cast<volatile uint32_t *>(&b.abort) = 1;
+            return;
+          }
+          ++tail;
+          for (uint32_t r = lane; r < kTcPos; r += 32)
+            if (t0 + r < s.lo || t0 + r >= s.hi)
+              for (uint32_t c = 0; c < HD / 8; ++c)
+                asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(dst + (c >> 3) * C::kHalf + r * 128 + (c & 7) * 16), "r"(0u) : "memory");
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&b.full[st]);
+        } else {
+          fills = seq + 1;
+        }
+      }
+    }
+  }
+}
+
+template <typename T, uint32_t HD>
+__global__ void __launch_bounds__(kTcThreads, 1) k_attn_tc(const AttnChunksParams p, const __grid_constant__ CUtensorMap map) {
+  using C = TcCfg<HD>;
+  extern __shared__ __align__(1024) uint8_t raw[];
+  const uint32_t pad = (1024u - (smem_u32(raw) & 1023u)) & 1023u, smem = smem_u32(raw) + pad;
+  TcBars &b = *reinterpret_cast<TcBars *>(raw + pad + C::kBarOff);
+  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  TcWalk w;
+  w.start(p, 1, b.red);
+  if (tid == 0) {
+    p.desc[blockIdx.x].w = 0;
+    for (uint32_t i = 0; i < C::kStages; ++i) {
+      mbar_init(&b.full[i], 1);
+      mbar_init(&b.empty[i], 1);
+    }
+    for (uint32_t i = 0; i < 2; ++i) {
+      mbar_init(&b.q_full[i], 128);
+      mbar_init(&b.s_full[i], 1);
+      mbar_init(&b.p_full[i], 128);
+      mbar_init(&b.o_full[i], 1);
+    }
+    mbar_init(&b.tail, 1);
+    mbar_init(&b.done, 1);
+    b.abort = 0;
+    fence_mbar_init();
+  }
+  const bool any = !w.done();  // the same for the CTA
+  if (any) {
+    if (warp == 8) {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&b.tmem)));
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = b.tmem;
+    // 384 x 168 registers at launch: 256 x 216 + 128 x 72
+    if (warp < 8) {
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+      softmax_role<T, HD>(p, w, b, smem + (warp >> 2) * C::kTile, tmem, warp >> 2);
+    } else {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+      if (warp == 8) {
+        if (lane == 0) {
+          mma_role<T, HD>(p, w, b, smem, tmem);
+          commit(&b.done);
+          mbar_wait(&b.done, 0);  // nothing is on its way to tensor memory after this
+        }
+      } else if (warp == 9) {
+        uint32_t fills = 0;
+        load_role<T, HD>(p, w, b, smem, &map, fills);
+        if (*reinterpret_cast<volatile uint32_t *>(&b.abort))  // copies that nobody waited for
+          for (uint32_t i = fills > C::kStages ? fills - C::kStages : 0; i < fills; ++i)
+            mbar_wait(&b.full[i % C::kStages], i / C::kStages & 1);
+      }
+    }
+    __syncwarp();
+    fence_before();
+    __syncthreads();
+    if (tid == 0 && b.abort && p.err) atomicOr(p.err, kFlagTimeout);
+    if (warp == 8) {
+      fence_after();
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    }
+  }
+  pdl_wait();  // the launch before this one, with which it may have overlapped: the join waits for this one only
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encoder() {
+  static std::mutex mu;
+  static PFN_cuTensorMapEncodeTiled_v12000 f = nullptr;
+  std::lock_guard<std::mutex> lock(mu);
+  if (!f) {
+    cudaDriverEntryPointQueryResult q;
+    void *fn = nullptr;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
+      return nullptr;
+    f = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+  }
+  return f;
+}
+
+template <typename T, uint32_t HD>
+int launch_hd(const AttnChunksParams &p, uint32_t ctas, cudaStream_t st) {
+  const PFN_cuTensorMapEncodeTiled_v12000 encode = encoder();
+  if (!encode) return -1;
+  // the layer's pages as rows of a head: [page][k | v][kv head][16] x head_dim, boxes of 16 rows x 64 elements
+  CUtensorMap map;
+  const cuuint64_t dims[2] = {HD, (cuuint64_t)p.pg.n_pages * 2 * p.pg.n_kv_heads * kPageLen}, strides[1] = {HD * 2};
+  const cuuint32_t box[2] = {64, kPageLen}, one[2] = {1, 1};
+  void *base = static_cast<char *>(p.pg.base) + (uint64_t)p.layer * p.pg.layer_stride * 2;
+  if (encode(&map, __is_same(T, __half) ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, dims, strides, box, one,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    return -1;
+  if (cudaFuncSetAttribute(k_attn_tc<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)TcCfg<HD>::kSmem) != cudaSuccess) return -1;
+  return launch_pdl(k_attn_tc<T, HD>, dim3(ctas), dim3(kTcThreads), TcCfg<HD>::kSmem, st, p, map);
+}
+
+}  // namespace
+
+uint32_t launch_attn_tc(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st) {
+  const uint32_t ctas = n_sm < kTcMaxCtas ? n_sm : kTcMaxCtas;  // one an SM
+  int rc;
+  if (p.pg.dtype == FA_KV_F16) rc = p.pg.head_dim == 64 ? launch_hd<__half, 64>(p, ctas, st) : launch_hd<__half, 128>(p, ctas, st);
+  else rc = p.pg.head_dim == 64 ? launch_hd<__nv_bfloat16, 64>(p, ctas, st) : launch_hd<__nv_bfloat16, 128>(p, ctas, st);
+  return rc ? 0 : ctas;
+}
+
+}  // namespace fa

@@ -9,7 +9,7 @@
 namespace fa {
 
 // bits of the operators' error words (FA_FLAG_*), apart from the kErr* bits
-enum : uint32_t { kFlagPage = FA_FLAG_PAGE, kFlagRange = FA_FLAG_RANGE };
+enum : uint32_t { kFlagPage = FA_FLAG_PAGE, kFlagRange = FA_FLAG_RANGE, kFlagTimeout = FA_FLAG_TIMEOUT };
 
 constexpr uint32_t kMaxHeadDim = 256;  // of the operators on pages
 constexpr uint32_t kPageLen = 16;      // positions of a page
@@ -56,9 +56,9 @@ struct AttnChunksParams {
   uint4 *desc;                       // per CTA: the item it starts and later CTAs continue (w = CTAs, 0: none)
   uint32_t *err;
 };
-int launch_attn_chunks(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st);
-size_t attn_chunks_ws(uint32_t head_dim);  // the slots, then the descriptors
-uint32_t attn_max_ctas();
+size_t attn_chunks_ws(uint32_t head_dim);
+// ws: attn_chunks_ws(head_dim) bytes; p.part and p.desc are set from it
+int launch_attn_chunks(const AttnChunksParams &p, void *ws, uint32_t n_sm, cudaStream_t st);
 
 // ---- page copies ----
 struct PageCopyParams {

@@ -16,7 +16,7 @@ ERR_INVALID, ERR_GGUF, ERR_UNSUPPORTED, ERR_OOM, ERR_CUDA, ERR_NCCL, ERR_CONTEXT
 
 F32, F16, Q4_0, Q4_1, Q5_0, Q8_0, Q4_K, Q6_K = 0, 1, 2, 3, 6, 8, 12, 14
 KV_F32, KV_F16, KV_BF16 = 0, 1, 2
-FLAG_PAGE, FLAG_RANGE = 16, 32
+FLAG_PAGE, FLAG_RANGE, FLAG_TIMEOUT = 16, 32, 64
 ROPE_INTERLEAVED, ROPE_HALF = 0, 1
 ROPE_PLAIN, ROPE_LINEAR, ROPE_NTK, ROPE_LLAMA3, ROPE_YARN = 0, 1, 2, 3, 4
 NO_TOKEN = 4294967295

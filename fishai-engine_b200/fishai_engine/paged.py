@@ -17,7 +17,7 @@ from . import _lib as L
 
 PAGE = 16  # positions of a page
 NO_TOKEN = -1  # in int32 `seqs` of rope_append: the row is left out
-FLAG_PAGE, FLAG_RANGE = L.FLAG_PAGE, L.FLAG_RANGE
+FLAG_PAGE, FLAG_RANGE, FLAG_TIMEOUT = L.FLAG_PAGE, L.FLAG_RANGE, L.FLAG_TIMEOUT
 
 _DTYPES = {}  # torch dtype -> FA_KV_*
 

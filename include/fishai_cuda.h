@@ -278,6 +278,7 @@ typedef struct {
 } fa_pages;
 #define FA_FLAG_PAGE 16   /* *err: a page number >= n_pages */
 #define FA_FLAG_RANGE 32  /* *err: a sequence, slot, length, row or index out of range */
+#define FA_FLAG_TIMEOUT 64  /* *err: a bounded device wait gave up; the outputs are not complete */
 /* the pages of a cache, for the calls below; valid until the cache is freed */
 int fa_kv_pages(const fa_kv *kv, fa_pages *out);
 
