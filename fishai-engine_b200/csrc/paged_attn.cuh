@@ -204,6 +204,7 @@ struct JoinSet {
   const float *part;
   const uint4 *desc;
   uint32_t R, ctas;
+  uint32_t parts;  // CTAs of the join to an item
 };
 // The kernels; each returns its grid, or 0 where the launch failed.
 bool attn_mma_takes(const AttnChunksParams &p);

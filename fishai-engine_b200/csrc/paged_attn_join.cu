@@ -15,19 +15,20 @@ __device__ __forceinline__ void put(__nv_bfloat16 *p, float x) { *p = __float2bf
 // CTA x takes the item that CTA x of the launch before began and others
 // finished.  A row's pieces (m_i, l_i, o_i) give
 //   o = sum o_i 2^(m_i - m) / sum l_i 2^(m_i - m),  m = max m_i,
-// added in the order of the positions.  Few pieces (long prompts): a warp a
-// row.  Many (one long cache): the eight warps take the pieces in turn, four
-// loads in flight each, and their sums are added in order; with a warp to a
-// whole row the 60 pieces of one 8192-position cache were one chain of loads:
-// 44 us for 8 kv heads x 4 rows, against 6 us so.
-constexpr uint32_t kJoinWarps = 8, kJoinFew = 8, kPer = kMaxHeadDim / 32;
+// added in the order of the positions, four loads in flight.  Items of many
+// rows, or of few pieces: a warp a row.  Few rows of many pieces (one long
+// cache): the eight warps take the pieces in turn and their sums are added in
+// order; with a warp to a whole row the 60 pieces of one 8192-position cache
+// were one chain of loads: 44 us for 8 kv heads x 4 rows, against 6 us so.
+constexpr uint32_t kJoinWarps = 8, kJoinFew = 8;
 
+template <uint32_t kPer>
 struct Sum {
   float m, l, acc[kPer];
 };
 // adds the pieces i0, i0 + step, .. i0 + 3 step of row r
-template <typename P>
-__device__ __forceinline__ void add4(Sum &s, P piece, uint32_t i0, uint32_t step, uint32_t n, uint32_t R, uint32_t r, uint32_t hd,
+template <uint32_t kPer, typename P>
+__device__ __forceinline__ void add4(Sum<kPer> &s, P piece, uint32_t i0, uint32_t step, uint32_t n, uint32_t R, uint32_t r, uint32_t hd,
                                      uint32_t lane) {
   float2 ml[4];
   float x[4][kPer];
@@ -54,13 +55,15 @@ __device__ __forceinline__ void add4(Sum &s, P piece, uint32_t i0, uint32_t step
   s.m = mn;
 }
 
-template <typename T>
+// kPer: head elements of a lane (hd <= 32 kPer)
+template <typename T, uint32_t kPer>
 __global__ void __launch_bounds__(kJoinWarps * 32) k_attn_join(const AttnChunksParams p, JoinSet a, JoinSet b) {
-  __shared__ float part[kJoinWarps][kMaxHeadDim];
+  __shared__ float part[kJoinWarps][32 * kPer];
   __shared__ float wm[kJoinWarps], wl[kJoinWarps];
   pdl_wait();
-  const bool second = blockIdx.x >= a.ctas;
-  const uint32_t cta = second ? blockIdx.x - a.ctas : blockIdx.x, R = second ? b.R : a.R;
+  const bool second = blockIdx.x >= a.ctas * a.parts;
+  const uint32_t parts = second ? b.parts : a.parts, at = second ? blockIdx.x - a.ctas * a.parts : blockIdx.x;
+  const uint32_t cta = at / parts, y = at % parts, R = second ? b.R : a.R;
   const uint4 d = second ? b.desc[cta] : a.desc[cta];
   if (!d.w) return;
   const uint32_t hd = p.pg.head_dim, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, head = d.z & 0xFFFF, rows = d.z >> 16;
@@ -72,9 +75,9 @@ __global__ void __launch_bounds__(kJoinWarps * 32) k_attn_join(const AttnChunksP
     const uint32_t row = d.y + r;
     return reinterpret_cast<T *>(p.out) + (uint64_t)(d.x + row / p.rep) * p.os + (head * p.rep + row % p.rep) * hd;
   };
-  if (d.w <= kJoinFew) {
-    for (uint32_t r = blockIdx.y * kJoinWarps + warp; r < rows; r += gridDim.y * kJoinWarps) {
-      Sum s{-INFINITY, 0.0f, {}};
+  if (d.w <= kJoinFew || rows > 16) {
+    for (uint32_t r = y * kJoinWarps + warp; r < rows; r += parts * kJoinWarps) {
+      Sum<kPer> s{-INFINITY, 0.0f, {}};
       for (uint32_t i = 0; i < d.w; i += 4) add4(s, piece, i, 1, d.w, R, r, hd, lane);
       T *o = out(r);
 #pragma unroll
@@ -83,8 +86,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) k_attn_join(const AttnChunksP
     }
     return;
   }
-  for (uint32_t r = blockIdx.y; r < rows; r += gridDim.y) {
-    Sum s{-INFINITY, 0.0f, {}};
+  for (uint32_t r = y; r < rows; r += parts) {
+    Sum<kPer> s{-INFINITY, 0.0f, {}};
     for (uint32_t i = warp; i < d.w; i += 4 * kJoinWarps) add4(s, piece, i, kJoinWarps, d.w, R, r, hd, lane);
     __syncthreads();  // the row before has been read
     if (lane == 0) {
@@ -114,6 +117,13 @@ __global__ void __launch_bounds__(kJoinWarps * 32) k_attn_join(const AttnChunksP
   }
 }
 
+template <typename T>
+int launch_join(const AttnChunksParams &p, const JoinSet &a, const JoinSet &b, cudaStream_t st) {
+  const dim3 grid(a.ctas * a.parts + b.ctas * b.parts), block(kJoinWarps * 32);
+  return p.pg.head_dim <= 128 ? launch_pdl(k_attn_join<T, 4>, grid, block, 0, st, p, a, b)
+                              : launch_pdl(k_attn_join<T, 8>, grid, block, 0, st, p, a, b);
+}
+
 constexpr size_t kSmallSlots = (size_t)2 * kAttnMaxCtas * kAttnMaxRows, kTcSlots = (size_t)2 * kTcMaxCtas * kTcRows;
 
 }  // namespace
@@ -131,7 +141,7 @@ int launch_attn_chunks(const AttnChunksParams &p, void *ws, uint32_t n_sm, cudaS
   b.desc = a.desc + kAttnMaxCtas;
   a.rows_min = 1;
   a.rows_max = 0xFFFFFFFFu;
-  JoinSet ja{a.part, a.desc, 0, 0}, jb{b.part, b.desc, kTcRows, 0};
+  JoinSet ja{a.part, a.desc, 0, 0, 0}, jb{b.part, b.desc, kTcRows, 0, 16};
   if (attn_mma_takes(p)) {
     // chunks of up to 64 rows are bound by the copies of K and V, which mma.sync
     // keeps up with; above, the 256-row items of tcgen05
@@ -146,11 +156,12 @@ int launch_attn_chunks(const AttnChunksParams &p, void *ws, uint32_t n_sm, cudaS
   } else if (!(ja.ctas = launch_attn_any(a, n_sm, st, &ja.R))) {
     return -1;
   }
-  const dim3 grid(ja.ctas + jb.ctas, jb.ctas ? 16 : ja.R < 8 ? ja.R : 8), block(kJoinWarps * 32);
+  // CTAs to an item: eight rows each, or the few rows of one long cache
+  ja.parts = jb.ctas ? 2 : ja.R < 16 ? ja.R : 8;
   switch (p.pg.dtype) {
-    case FA_KV_F32: return launch_pdl(k_attn_join<float>, grid, block, 0, st, p, ja, jb);
-    case FA_KV_F16: return launch_pdl(k_attn_join<__half>, grid, block, 0, st, p, ja, jb);
-    default: return launch_pdl(k_attn_join<__nv_bfloat16>, grid, block, 0, st, p, ja, jb);
+    case FA_KV_F32: return launch_join<float>(p, ja, jb, st);
+    case FA_KV_F16: return launch_join<__half>(p, ja, jb, st);
+    default: return launch_join<__nv_bfloat16>(p, ja, jb, st);
   }
 }
 

@@ -16,6 +16,9 @@
 //   warp 9           TMA: K and V tiles of 128 positions, a box per page of 16
 //                    (pages outside the item's range start past the end of the
 //                    tensor and arrive as zeros), 128-byte swizzle, a ring
+//   warps 10, 11     copy the next item's Q rows (a row is a token and a head,
+//                    so they are gathered) as soon as the last scores of the
+//                    item before are formed
 // Order of the MMAs per tile: P0 V, S0 of the next tile, P1 V, S1 of the next.
 // They run in the order of issue, so S0 may overwrite P0 without a wait.
 // The reference point m of a row only moves when a maximum exceeds it by 2^8:
@@ -49,7 +52,7 @@ struct TcCfg {
   static_assert(kSmem <= 227 * 1024, "shared memory of a CTA");
 };
 struct TcBars {
-  uint64_t full[8], empty[8], q_full[2], s_full[2], p_full[2], o_full[2], tail, done;
+  uint64_t full[8], empty[8], q_full[2], q_empty[2], s_full[2], p_half[2], p_full[2], o_full[2], tail, done;
   uint64_t red[kTcThreads / 32 + 2];
   uint32_t tmem, abort;
 };
@@ -149,31 +152,71 @@ __device__ __forceinline__ bool wait_bar(TcBars &b, uint64_t *bar, uint32_t pari
 
 using TcWalk = Walk<kTcRows, kTcPos, kTcThreads>;
 
-// Q rows [first, first + 128) of the item to a swizzled tile, 128 threads
+// Q rows [first, first + 128) of the item to a swizzled tile, 64 threads; rows
+// past the item's are zeros
 template <typename T, uint32_t HD>
 __device__ __forceinline__ void load_q(const AttnChunksParams &p, const Segment &s, uint32_t first, uint32_t tile, uint32_t tid) {
-  constexpr uint32_t CH = HD / 8;
-#pragma unroll 4
-  for (uint32_t i = tid; i < 128 * CH; i += 128) {
-    const uint32_t r = i / CH, c = i % CH, row = first + r;
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (row < s.r1) {
-      const uint32_t tok = row / p.rep;
-      const T *x = reinterpret_cast<const T *>(p.q) + (uint64_t)(s.chunk.q0 + tok) * p.qs + (s.head * p.rep + row - tok * p.rep) * HD + c * 8;
-      if (p.aligned) {
-        v = *reinterpret_cast<const uint4 *>(x);
-      } else {
-        const uint16_t *y = reinterpret_cast<const uint16_t *>(x);
-        v = make_uint4(y[0] | (uint32_t)y[1] << 16, y[2] | (uint32_t)y[3] << 16, y[4] | (uint32_t)y[5] << 16, y[6] | (uint32_t)y[7] << 16);
-      }
-    }
+  constexpr uint32_t CH = HD / 8, kStep = 64 / CH;  // pieces of a row; rows between a thread's pieces
+  const uint32_t c = tid % CH, r0 = tid / CH;
+  // row -> (token, head of the group), carried along: a division a piece made
+  // these two warps the slowest part of short items
+  const uint32_t rep = p.rep, dt = kStep / rep, dh = kStep - dt * rep;
+  uint32_t tok = (first + r0) / rep, h = first + r0 - tok * rep;
+  const T *base = reinterpret_cast<const T *>(p.q) + (uint64_t)s.chunk.q0 * p.qs + s.head * rep * HD + c * 8;
+  const uint32_t rows = s.r1 - first;
+#pragma unroll 8
+  for (uint32_t r = r0; r < 128; r += kStep) {
+    const bool live = r < rows;
+    const T *x = live ? base + tok * p.qs + h * HD : base;
     const uint32_t dst = tile + (c >> 3) * TcCfg<HD>::kHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+    if (p.aligned) {
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(x), "r"(live ? 16u : 0u) : "memory");
+    } else {
+      const uint16_t *y = reinterpret_cast<const uint16_t *>(x);
+      uint32_t v[4] = {};
+      if (live)
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) v[i] = y[2 * i] | (uint32_t)y[2 * i + 1] << 16;
+      asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+    }
+    tok += dt;
+    h += dh;
+    if (h >= rep) {
+      h -= rep;
+      ++tok;
+    }
   }
 }
 
 template <typename T, uint32_t HD>
-__device__ void softmax_role(const AttnChunksParams &p, TcWalk w, TcBars &b, uint32_t qtile, uint32_t tmem, uint32_t g) {
+__device__ void q_role(const AttnChunksParams &p, TcWalk w, TcBars &b, uint32_t smem) {
+  const uint32_t tid = threadIdx.x & 63;
+  uint32_t n[2] = {0, 0};  // fills of each tile so far
+  while (!w.done()) {
+    const Segment s = w.next(p);
+    if (s.hi <= s.lo) continue;
+#pragma unroll
+    for (uint32_t g = 0; g < 2; ++g) {
+      if (s.r0 + 128 * g >= s.r1) break;
+      if (!wait_bar(b, &b.q_empty[g], (n[g] & 1) ^ 1)) return;
+      load_q<T, HD>(p, s, s.r0 + 128 * g, smem + g * TcCfg<HD>::kTile, tid);
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      fence_proxy_async_smem();
+      mbar_arrive(&b.q_full[g]);
+      ++n[g];
+    }
+  }
+}
+
+// 32 consecutive f32 or 16-bit values of a thread's row, 32 bytes a store
+__device__ __forceinline__ void st8(void *p, const uint32_t (&v)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]),
+               "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
+template <typename T, uint32_t HD>
+__device__ void softmax_role(const AttnChunksParams &p, TcWalk w, TcBars &b, uint32_t tmem, uint32_t g) {
   const uint32_t tid = threadIdx.x & 127, warp = tid >> 5;
   const uint32_t lanes = tmem + ((warp * 32) << 16);
   uint32_t n = 0;  // tiles of this group so far
@@ -185,11 +228,6 @@ __device__ void softmax_role(const AttnChunksParams &p, TcWalk w, TcBars &b, uin
     const int32_t pos = live ? s.chunk.first + (int32_t)(row / p.rep) : -1;
     const uint32_t tiles = s.hi > s.lo ? s.u1 - s.u0 : 0;
     float m = -INFINITY, l = 0.0f;
-    if (tiles) {
-      load_q<T, HD>(p, s, s.r0 + 128 * g, qtile, tid);
-      fence_proxy_async_smem();
-      mbar_arrive(&b.q_full[g]);
-    }
     for (uint32_t k = 0; k < tiles; ++k, ++n) {
       const uint32_t t0 = (s.lo / kTcPos + s.u0 + k) * kTcPos;
       if (!wait_bar(b, &b.s_full[g], n & 1)) return;
@@ -243,11 +281,11 @@ __device__ void softmax_role(const AttnChunksParams &p, TcWalk w, TcBars &b, uin
           pk[c] = pack2<T>(a, d);
         }
         st32(lanes + s_col(g) + 32 * h, pk);
+        wait_st();  // (also of a rescaled output)
+        fence_before();
+        mbar_arrive(h ? &b.p_full[g] : &b.p_half[g]);  // the product with V begins with the first half
       }
       l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      wait_st();
-      fence_before();
-      mbar_arrive(&b.p_full[g]);
     }
     float *slot = TcWalk::slot(p, s);
     const uint32_t r = row - s.r0, tok = row / p.rep;
@@ -271,18 +309,25 @@ __device__ void softmax_role(const AttnChunksParams &p, TcWalk w, TcBars &b, uin
       if (!live) continue;
       if (!whole) {
 #pragma unroll
-        for (uint32_t e = 0; e < 32; e += 4) *reinterpret_cast<float4 *>(slot + r * HD + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-      } else if (p.aligned) {
+        for (uint32_t e = 0; e < 32; e += 8) {
+          uint32_t v[8];
 #pragma unroll
-        for (uint32_t e = 0; e < 32; e += 8)
-          *reinterpret_cast<uint4 *>(out + c + e) = make_uint4(pack2<T>(o[e] * inv, o[e + 1] * inv), pack2<T>(o[e + 2] * inv, o[e + 3] * inv),
-                                                              pack2<T>(o[e + 4] * inv, o[e + 5] * inv), pack2<T>(o[e + 6] * inv, o[e + 7] * inv));
+          for (uint32_t j = 0; j < 8; ++j) v[j] = __float_as_uint(o[e + j]);
+          st8(slot + r * HD + c + e, v);
+        }
+        continue;
+      }
+      uint32_t v[16];
+#pragma unroll
+      for (uint32_t e = 0; e < 16; ++e) v[e] = pack2<T>(o[2 * e] * inv, o[2 * e + 1] * inv);
+      if (reinterpret_cast<uintptr_t>(out) % 32 == 0) {
+        st8(out + c, reinterpret_cast<const uint32_t(&)[8]>(v[0]));
+        st8(out + c + 16, reinterpret_cast<const uint32_t(&)[8]>(v[8]));
       } else {
 #pragma unroll
-        for (uint32_t e = 0; e < 32; e += 2) {
-          const uint32_t v = pack2<T>(o[e] * inv, o[e + 1] * inv);
-          reinterpret_cast<uint16_t *>(out)[c + e] = (uint16_t)v;
-          reinterpret_cast<uint16_t *>(out)[c + e + 1] = (uint16_t)(v >> 16);
+        for (uint32_t e = 0; e < 16; ++e) {
+          reinterpret_cast<uint16_t *>(out)[c + 2 * e] = (uint16_t)v[e];
+          reinterpret_cast<uint16_t *>(out)[c + 2 * e + 1] = (uint16_t)(v[e] >> 16);
         }
       }
     }
@@ -322,24 +367,31 @@ __device__ void mma_role(const AttnChunksParams &p, TcWalk w, TcBars &b, uint32_
     // fills come K0 V0 K1 V1 ..
     if (!filled(seq)) return;
     fence_after();
-    for (uint32_t g = 0; g < groups; ++g) scores(g, seq);
+    for (uint32_t g = 0; g < groups; ++g) {
+      scores(g, seq);
+      if (tiles == 1) commit(&b.q_empty[g]);
+    }
     commit(&b.empty[seq % C::kStages]);
     for (uint32_t k = 0; k < tiles; ++k) {
       const uint32_t v = seq + 1, next = seq + 2;
       const bool more = k + 1 < tiles;
       if (!filled(v)) return;
       for (uint32_t g = 0; g < groups; ++g) {
-        if (!wait_bar(b, &b.p_full[g], n[g] & 1)) return;
-        ++n[g];
-        fence_after();
 #pragma unroll
-        for (uint32_t kk = 0; kk < kTcPos / 16; ++kk)
-          mma_ts(tmem + o_col(g), tmem + s_col(g) + 8 * kk, sdesc(stage(v) + kk * 2048, C::kHalf), kO, k || kk);
+        for (uint32_t h = 0; h < 2; ++h) {
+          if (!wait_bar(b, h ? &b.p_full[g] : &b.p_half[g], n[g] & 1)) return;
+          fence_after();
+#pragma unroll
+          for (uint32_t kk = 4 * h; kk < 4 * h + 4; ++kk)
+            mma_ts(tmem + o_col(g), tmem + s_col(g) + 8 * kk, sdesc(stage(v) + kk * 2048, C::kHalf), kO, k || kk);
+        }
+        ++n[g];
         commit(&b.o_full[g]);
         if (g + 1 == groups) commit(&b.empty[v % C::kStages]);
         if (more) {
           if (g == 0 && !filled(next)) return;
           scores(g, next);
+          if (k + 2 == tiles) commit(&b.q_empty[g]);  // the item's last scores
         }
       }
       if (more) commit(&b.empty[next % C::kStages]);
@@ -420,8 +472,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_tc(const AttnChunksParam
       mbar_init(&b.empty[i], 1);
     }
     for (uint32_t i = 0; i < 2; ++i) {
-      mbar_init(&b.q_full[i], 128);
+      mbar_init(&b.q_full[i], 64);
+      mbar_init(&b.q_empty[i], 1);
       mbar_init(&b.s_full[i], 1);
+      mbar_init(&b.p_half[i], 128);
       mbar_init(&b.p_full[i], 128);
       mbar_init(&b.o_full[i], 1);
     }
@@ -443,7 +497,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_tc(const AttnChunksParam
     // 384 x 168 registers at launch: 256 x 216 + 128 x 72
     if (warp < 8) {
       asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-      softmax_role<T, HD>(p, w, b, smem + (warp >> 2) * C::kTile, tmem, warp >> 2);
+      softmax_role<T, HD>(p, w, b, tmem, warp >> 2);
     } else {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
       if (warp == 8) {
@@ -458,6 +512,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_tc(const AttnChunksParam
         if (*reinterpret_cast<volatile uint32_t *>(&b.abort))  // copies that nobody waited for
           for (uint32_t i = fills > C::kStages ? fills - C::kStages : 0; i < fills; ++i)
             mbar_wait(&b.full[i % C::kStages], i / C::kStages & 1);
+      } else {
+        q_role<T, HD>(p, w, b, smem);
       }
     }
     __syncwarp();

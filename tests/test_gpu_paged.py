@@ -152,12 +152,14 @@ def attn(pages, table, q, q_start, kv_len, heads, max_q=None, seqs=None, scale=0
 
 def attn_check(qs, kvs, heads, kvh, hd, dtype, window=0, scale=0.0, seed=0, **kw):
     pages, table = R.make_cache(kvs, 1, kvh, hd, dtype, seed, junk=10 ** 6)
+    err = kw.setdefault("err", torch.zeros(1, dtype=torch.int32, device="cuda"))
     start = [sum(qs[:i]) for i in range(len(qs) + 1)]
     q = randn(seed + 1, start[-1] + 2, heads * hd, dtype=dtype)  # two rows behind the last chunk
     out = attn(pages, table, q, start, kvs, heads, window=window, scale=scale, **kw)
     want, tol = R.attention(pages, table, 0, q, i32(start), i32(kvs), None, heads, scale, window)
     got = out.double().view_as(want)
     n = start[-1]
+    assert int(err) == 0
     assert bool((got[n:] == 7.0).all())
     off = ((got - want).abs() - tol)[:n]
     assert not bool(torch.isnan(got).any())
@@ -208,6 +210,15 @@ def test_attention_split_long_cache(t):
     attn_check([1], [12345], 8, 1, 128, R.TYPES[t], window=7000, seed=7)
     attn_check([5], [8000], 8, 8, 128, R.TYPES[t], seed=8)
     attn_check([200], [6000], 2, 1, 128, R.TYPES[t], seed=8)
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_several_items_a_cta(t, hd):
+    """more items than SMs, of one to a dozen tiles: buffers and barriers are used again and again"""
+    attn_check([700, 900, 500, 130], [700, 1400, 600, 130], 32, 8, hd, R.TYPES[t], seed=16)
+    attn_check([33] * 60, [33 + 7 * i for i in range(60)], 16, 4, hd, R.TYPES[t], seed=17)
+    attn_check([2000], [2000], 16, 8, hd, R.TYPES[t], window=300, seed=18)
 
 
 @pytest.mark.parametrize("t", ["f16", "f32"])
