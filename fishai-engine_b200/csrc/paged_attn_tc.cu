@@ -12,7 +12,7 @@
 //   warps 0-3, 4-7   softmax of Q tile 0, 1: a thread a row.  Scores come from
 //                    tensor memory, weights go back over them (16 bits, as V
 //                    was rounded), read by the second MMA as its A operand.
-//   warp 8           issues the MMAs (one lane); owns the tensor memory
+//   warp 8           issues the MMAs (an elected lane); owns the tensor memory
 //   warp 9           TMA: K and V tiles of 128 positions, a box per page of 16
 //                    (pages outside the item's range start past the end of the
 //                    tensor and arrive as zeros), 128-byte swizzle, a ring
@@ -67,25 +67,27 @@ __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::aft
 __device__ __forceinline__ void commit(uint64_t *bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-// descriptor of a shared-memory operand with 128-byte swizzle: 8-row groups
+// Descriptor of a shared-memory operand with 128-byte swizzle: 8-row groups
 // 1024 bytes apart, `lead` bytes between blocks of 64 elements (rows-contiguous
-// operand V) or unused (K, Q)
-__device__ __forceinline__ uint64_t sdesc(uint32_t addr, uint32_t lead) {
-  return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
-         ((uint64_t)2 << 61);
+// operand V) or unused (K, Q).  The address is in the low word, so a tile's
+// descriptors differ by an addition there.
+__device__ __forceinline__ uint32_t sdesc_lo(uint32_t addr, uint32_t lead) { return ((addr >> 4) & 0x3FFFu) | ((lead >> 4) << 16); }
+constexpr uint32_t kDescHi = (1024 >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint64_t sdesc(uint32_t lo) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(kDescHi));
+  return d;
 }
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
       "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc),
-      "r"(0u)
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc)
       : "memory");
 }
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
       "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc),
-      "r"(0u)
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc)
       : "memory");
 }
 __device__ __forceinline__ void tma_2d(uint32_t dst, const void *map, int32_t x, int32_t y, uint64_t *bar) {
@@ -93,9 +95,6 @@ __device__ __forceinline__ void tma_2d(uint32_t dst, const void *map, int32_t x,
                "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar))
                : "memory");
 }
-#define TC_R32(v)                                                                                                                  \
-  v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7], v[8], v[9], v[10], v[11], v[12], v[13], v[14], v[15], v[16], v[17], v[18], v[19], \
-      v[20], v[21], v[22], v[23], v[24], v[25], v[26], v[27], v[28], v[29], v[30], v[31]
 __device__ __forceinline__ void ld32(uint32_t addr, float *v) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,"
@@ -116,6 +115,12 @@ __device__ __forceinline__ void st32(uint32_t addr, const uint32_t *v) {
       "r"(v[31])
       : "memory");
 }
+__device__ __forceinline__ void st16(uint32_t addr, const uint32_t (&v)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr), "r"(v[0]),
+               "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]),
+               "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+               : "memory");
+}
 __device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ float ex2(float x) {  // 2^x, 2 ulp; below 2^-126: 0
@@ -131,6 +136,41 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   } else {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t *>(&h);
+  }
+}
+
+// two f32 in a register pair
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// Weights 2^(scale x - m) of 32 scores: 16 packed pairs, their sums added to
+// `sum`.  (A polynomial on the FMA pipes for 3 of 8 pairs, to unburden the
+// special-function unit, was slower: 2048 rows over 16384 positions 495 us
+// against 472; the chain of instructions of a row counts for more.)
+template <typename T>
+__device__ __forceinline__ void weights32(const float *x, uint64_t scale, uint64_t minus_m, uint64_t (&sum)[2], uint32_t (&pk)[16]) {
+#pragma unroll
+  for (uint32_t c = 0; c < 16; ++c) {
+    float a, b;
+    unpair(fma2(pair(x[2 * c], x[2 * c + 1]), scale, minus_m), a, b);
+    a = ex2(a);
+    b = ex2(b);
+    sum[c & 1] = add2(sum[c & 1], pair(a, b));
+    pk[c] = pack2<T>(a, b);
   }
 }
 
@@ -237,8 +277,8 @@ __device__ void softmax_role(const AttnChunksParams &p, TcWalk w, TcBars &b, uin
       for (uint32_t c = 0; c < 4; ++c) ld32(lanes + s_col(g) + 32 * c, x + 32 * c);
       wait_ld();
       // rows of a warp that see all 128 positions need no mask
-      const bool all = (int32_t)(t0 + kTcPos - 1) <= pos && (!p.window || (uint32_t)(pos - (int32_t)t0) < p.window);
-      if (!__all_sync(0xFFFFFFFFu, all)) {
+      const bool all = __all_sync(0xFFFFFFFFu, (int32_t)(t0 + kTcPos - 1) <= pos && (!p.window || (uint32_t)(pos - (int32_t)t0) < p.window));
+      if (!all) {
         // visible columns: [from, to)
         const int32_t to = pos - (int32_t)t0 + 1, from = p.window ? to - (int32_t)p.window : 0;
 #pragma unroll
@@ -247,7 +287,11 @@ __device__ void softmax_role(const AttnChunksParams &p, TcWalk w, TcBars &b, uin
       }
       float mx[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-      for (uint32_t c = 4; c < kTcPos; ++c) mx[c % 4] = fmaxf(mx[c % 4], x[c]);
+      for (uint32_t c = 4; c + 8 <= kTcPos; c += 8)
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], fmaxf(x[c + e], x[c + 4 + e]));
+#pragma unroll
+      for (uint32_t e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], x[kTcPos - 4 + e]);
       const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
       float f = 1.0f;
       if (top > m + 8.0f) {
@@ -269,23 +313,26 @@ __device__ void softmax_role(const AttnChunksParams &p, TcWalk w, TcBars &b, uin
         }
       }
       const float ms = m == -INFINITY ? 0.0f : m;
-      float sum[4] = {};
-      uint32_t pk[32];
+      const uint64_t scale = pair(p.scale_log2, p.scale_log2), minus_m = pair(-ms, -ms);
+      uint64_t sum[2] = {0, 0};
 #pragma unroll
-      for (uint32_t h = 0; h < 2; ++h) {
-#pragma unroll
-        for (uint32_t c = 0; c < 32; ++c) {
-          const float a = ex2(fmaf(x[64 * h + 2 * c], p.scale_log2, -ms)), d = ex2(fmaf(x[64 * h + 2 * c + 1], p.scale_log2, -ms));
-          sum[(2 * c) % 4] += a;
-          sum[(2 * c + 1) % 4] += d;
-          pk[c] = pack2<T>(a, d);
+      for (uint32_t h = 0; h < 4; ++h) {
+        uint32_t pk[16];
+        weights32<T>(x + 32 * h, scale, minus_m, sum, pk);
+        if (h == 2) {  // the first half is stored by now (and a rescaled output): its product with V begins
+          wait_st();
+          fence_before();
+          mbar_arrive(&b.p_half[g]);
         }
-        st32(lanes + s_col(g) + 32 * h, pk);
-        wait_st();  // (also of a rescaled output)
-        fence_before();
-        mbar_arrive(h ? &b.p_full[g] : &b.p_half[g]);  // the product with V begins with the first half
+        st16(lanes + s_col(g) + 16 * h, pk);
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      wait_st();
+      fence_before();
+      mbar_arrive(&b.p_full[g]);
+      float s0, s1, s2, s3;
+      unpair(sum[0], s0, s1);
+      unpair(sum[1], s2, s3);
+      l += (s0 + s1) + (s2 + s3);
     }
     float *slot = TcWalk::slot(p, s);
     const uint32_t r = row - s.r0, tok = row / p.rep;
@@ -343,59 +390,77 @@ __device__ void mma_role(const AttnChunksParams &p, TcWalk w, TcBars &b, uint32_
   constexpr uint32_t kType = __is_same(T, __half) ? 0u : 1u;  // f16 / bf16, A and B
   constexpr uint32_t kS = (1u << 4) | (kType << 7) | (kType << 10) | ((kTcPos / 8) << 17) | ((128 / 16) << 24);
   constexpr uint32_t kO = (1u << 4) | (kType << 7) | (kType << 10) | (1u << 16) | ((HD / 8) << 17) | ((128 / 16) << 24);  // B = V: rows are K
-  const uint32_t ring = smem + 2 * C::kTile;
-  uint32_t seq = 0, n[2] = {0, 0}, q_phase[2] = {0, 0};
-  auto stage = [&](uint32_t i) { return ring + i % C::kStages * C::kTile; };
-  auto filled = [&](uint32_t i) { return wait_bar(b, &b.full[i % C::kStages], i / C::kStages & 1); };
-  auto scores = [&](uint32_t g, uint32_t kt) {
-    const uint32_t q = smem + g * C::kTile, k = stage(kt);
-#pragma unroll
-    for (uint32_t kk = 0; kk < HD / 16; ++kk) {
-      const uint32_t off = kk / 4 * C::kHalf + kk % 4 * 32;
-      mma_ss(tmem + s_col(g), sdesc(q + off, 16), sdesc(k + off, 16), kS, kk);
+  // The warp stays together and one elected lane issues: with the whole loop in
+  // one lane the operands' way into uniform registers made each MMA take some
+  // 130 clocks to issue (637 us for 2048 rows over 16384 positions, 495 so).
+  // Ring places and phases are counted on.
+  const uint32_t q_lo = sdesc_lo(smem, 16), k_lo = sdesc_lo(smem + 2 * C::kTile, 16), v_lo = sdesc_lo(smem + 2 * C::kTile, C::kHalf);
+  struct Place {  // of a fill in the ring (fills come K0 V0 K1 V1 ..)
+    uint32_t st, ph;
+    __device__ void step() {
+      if (++st == C::kStages) {
+        st = 0;
+        ph ^= 1;
+      }
     }
-    commit(&b.s_full[g]);
+  } at{0, 0};
+  uint32_t n[2] = {0, 0}, q_phase[2] = {0, 0};
+  uint32_t lead;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xFFFFFFFF;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(lead));
+  auto scores = [&](uint32_t g, uint32_t st) {
+    const uint32_t q = q_lo + g * (C::kTile >> 4), k = k_lo + st * (C::kTile >> 4);
+    if (lead) {
+#pragma unroll
+      for (uint32_t kk = 0; kk < HD / 16; ++kk) {
+        const uint32_t off = kk / 4 * (C::kHalf >> 4) + kk % 4 * 2;
+        mma_ss(tmem + s_col(g), sdesc(q + off), sdesc(k + off), kS, kk);
+      }
+      commit(&b.s_full[g]);
+    }
+    __syncwarp();
   };
   while (!w.done()) {
     const Segment s = w.next(p);
     const uint32_t tiles = s.hi > s.lo ? s.u1 - s.u0 : 0, groups = s.r1 - s.r0 > 128 ? 2 : 1;
     if (!tiles) continue;
+    if (!wait_bar(b, &b.full[at.st], at.ph)) return;
     for (uint32_t g = 0; g < groups; ++g) {
       if (!wait_bar(b, &b.q_full[g], q_phase[g])) return;
       q_phase[g] ^= 1;
+      fence_after();
+      scores(g, at.st);
+      if (tiles == 1 && lead) commit(&b.q_empty[g]);
     }
-    // fills come K0 V0 K1 V1 ..
-    if (!filled(seq)) return;
-    fence_after();
-    for (uint32_t g = 0; g < groups; ++g) {
-      scores(g, seq);
-      if (tiles == 1) commit(&b.q_empty[g]);
-    }
-    commit(&b.empty[seq % C::kStages]);
+    if (lead) commit(&b.empty[at.st]);
+    at.step();
     for (uint32_t k = 0; k < tiles; ++k) {
-      const uint32_t v = seq + 1, next = seq + 2;
+      const Place v = at;
+      at.step();
+      const Place next = at;
       const bool more = k + 1 < tiles;
-      if (!filled(v)) return;
+      if (more) at.step();
+      if (!wait_bar(b, &b.full[v.st], v.ph)) return;
+      const uint32_t vt = v_lo + v.st * (C::kTile >> 4);
       for (uint32_t g = 0; g < groups; ++g) {
 #pragma unroll
         for (uint32_t h = 0; h < 2; ++h) {
           if (!wait_bar(b, h ? &b.p_full[g] : &b.p_half[g], n[g] & 1)) return;
           fence_after();
+if (lead)
 #pragma unroll
           for (uint32_t kk = 4 * h; kk < 4 * h + 4; ++kk)
-            mma_ts(tmem + o_col(g), tmem + s_col(g) + 8 * kk, sdesc(stage(v) + kk * 2048, C::kHalf), kO, k || kk);
+            mma_ts(tmem + o_col(g), tmem + s_col(g) + 8 * kk, sdesc(vt + kk * (2048 >> 4)), kO, k || kk);
         }
         ++n[g];
-        commit(&b.o_full[g]);
-        if (g + 1 == groups) commit(&b.empty[v % C::kStages]);
+        if (lead) commit(&b.o_full[g]);
+        if (g + 1 == groups && lead) commit(&b.empty[v.st]);
         if (more) {
-          if (g == 0 && !filled(next)) return;
-          scores(g, next);
-          if (k + 2 == tiles) commit(&b.q_empty[g]);  // the item's last scores
+          if (g == 0 && !wait_bar(b, &b.full[next.st], next.ph)) return;
+          scores(g, next.st);
+          if (k + 2 == tiles && lead) commit(&b.q_empty[g]);  // the item's last scores
         }
       }
-      if (more) commit(&b.empty[next % C::kStages]);
-      seq += 2;
+      if (more && lead) commit(&b.empty[next.st]);
     }
   }
 }
@@ -501,11 +566,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_tc(const AttnChunksParam
     } else {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
       if (warp == 8) {
-        if (lane == 0) {
-          mma_role<T, HD>(p, w, b, smem, tmem);
-          commit(&b.done);
-          mbar_wait(&b.done, 0);  // nothing is on its way to tensor memory after this
-        }
+        mma_role<T, HD>(p, w, b, smem, tmem);
+        if (lane == 0) commit(&b.done);
+        __syncwarp();
+        mbar_wait(&b.done, 0);  // nothing is on its way to tensor memory after this
       } else if (warp == 9) {
         uint32_t fills = 0;
         load_role<T, HD>(p, w, b, smem, &map, fills);
