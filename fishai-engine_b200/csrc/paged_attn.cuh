@@ -216,6 +216,12 @@ uint32_t launch_attn_tc(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t s
 // for many: what the workspace holds two slots of each for.
 constexpr uint32_t kAttnMaxCtas = 480, kAttnMaxRows = 64;
 constexpr uint32_t kTcMaxCtas = 160, kTcRows = 256;
+// Where element d (a multiple of 4, and the three behind it) of row r is in a
+// slot of the launch for many rows, whose threads have a row each; after the
+// kTcRows x hd outputs come the pairs (max, sum).
+__host__ __device__ constexpr uint32_t tc_part(uint32_t r, uint32_t d, uint32_t hd) {
+  return ((r / 32) * (hd / 4) + d / 4) * 128 + (r % 32) * 4;
+}
 
 // element offset of (page, k | v, head, position in page) in a layer
 __device__ __forceinline__ uint64_t page_row(const fa_pages &pg, uint32_t page, uint32_t is_v, uint32_t h, uint32_t slot) {

@@ -56,6 +56,50 @@ __device__ __forceinline__ void add4(Sum<kPer> &s, P piece, uint32_t i0, uint32_
 }
 
 // kPer: head elements of a lane (hd <= 32 kPer)
+// An item of the launch for many rows: a thread has 16 elements of a row, as
+// they lie in the slots (tc_part), and writes them as 32 bytes.
+template <typename T>
+__device__ __forceinline__ void join_tc(const AttnChunksParams &p, const float *part, const uint4 &d, uint32_t cta, uint32_t at) {
+  const uint32_t hd = p.pg.head_dim, head = d.z & 0xFFFF, rows = d.z >> 16;
+  const uint32_t block = at * kJoinWarps + threadIdx.x / 32;  // (32 rows, 16 elements)
+  const uint32_t r = block / (hd / 16) * 32 + threadIdx.x % 32, e0 = block % (hd / 16) * 16;
+  if (r >= rows) return;
+  const uint64_t slot = (uint64_t)kTcRows * (hd + 2);
+  const float *first = part + ((uint64_t)cta * 2 + 1) * slot;
+  float m = -INFINITY, l = 0.0f, acc[16] = {};
+  for (uint32_t i = 0; i < d.w; ++i) {
+    const float *q = i ? first + (2 * (uint64_t)i - 1) * slot : first;  // slot 1 of the CTA, then slot 0 of the next ones
+    const float2 ml = __ldcg(reinterpret_cast<const float2 *>(q + kTcRows * hd + 2 * r));
+    float4 x[4];
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j) x[j] = __ldcg(reinterpret_cast<const float4 *>(q + tc_part(r, e0 + 4 * j, hd)));
+    const float mn = fmaxf(m, ml.x), ms = mn == -INFINITY ? 0.0f : mn, f = exp2f(m - ms), e = exp2f(ml.x - ms);
+    l = fmaf(l, f, ml.y * e);
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j) {
+      acc[4 * j] = fmaf(acc[4 * j], f, x[j].x * e);
+      acc[4 * j + 1] = fmaf(acc[4 * j + 1], f, x[j].y * e);
+      acc[4 * j + 2] = fmaf(acc[4 * j + 2], f, x[j].z * e);
+      acc[4 * j + 3] = fmaf(acc[4 * j + 3], f, x[j].w * e);
+    }
+    m = mn;
+  }
+  const uint32_t row = d.y + r;
+  T *out = reinterpret_cast<T *>(p.out) + (uint64_t)(d.x + row / p.rep) * p.os + (head * p.rep + row % p.rep) * hd + e0;
+  struct alignas(16) Out {
+    T v[8];
+  } o[2];
+#pragma unroll
+  for (uint32_t j = 0; j < 16; ++j) put(&o[j / 8].v[j % 8], l == 0.0f ? 0.0f : acc[j] / l);
+  if (p.aligned) {
+    reinterpret_cast<Out *>(out)[0] = o[0];
+    reinterpret_cast<Out *>(out)[1] = o[1];
+  } else {
+#pragma unroll
+    for (uint32_t j = 0; j < 16; ++j) out[j] = o[j / 8].v[j % 8];
+  }
+}
+
 template <typename T, uint32_t kPer>
 __global__ void __launch_bounds__(kJoinWarps * 32) k_attn_join(const AttnChunksParams p, JoinSet a, JoinSet b) {
   __shared__ float part[kJoinWarps][32 * kPer];
@@ -63,12 +107,18 @@ __global__ void __launch_bounds__(kJoinWarps * 32) k_attn_join(const AttnChunksP
   pdl_wait();
   const bool second = blockIdx.x >= a.ctas * a.parts;
   const uint32_t parts = second ? b.parts : a.parts, at = second ? blockIdx.x - a.ctas * a.parts : blockIdx.x;
-  const uint32_t cta = at / parts, y = at % parts, R = second ? b.R : a.R;
+  const uint32_t cta = at / parts, y = at % parts, R = a.R;
   const uint4 d = second ? b.desc[cta] : a.desc[cta];
   if (!d.w) return;
+  if constexpr (sizeof(T) == 2 && kPer == 4) {
+    if (second) {
+      join_tc<T>(p, b.part, d, cta, y);
+      return;
+    }
+  }
   const uint32_t hd = p.pg.head_dim, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, head = d.z & 0xFFFF, rows = d.z >> 16;
   const uint64_t slot = (uint64_t)R * (hd + 2);
-  const float *first = (second ? b.part : a.part) + ((uint64_t)cta * 2 + 1) * slot;
+  const float *first = a.part + ((uint64_t)cta * 2 + 1) * slot;
   // piece i: slot 1 of the CTA, then slot 0 of the next ones
   auto piece = [&](uint32_t i) { return i ? first + (2 * (uint64_t)i - 1) * slot : first; };
   auto out = [&](uint32_t r) {
@@ -141,7 +191,7 @@ int launch_attn_chunks(const AttnChunksParams &p, void *ws, uint32_t n_sm, cudaS
   b.desc = a.desc + kAttnMaxCtas;
   a.rows_min = 1;
   a.rows_max = 0xFFFFFFFFu;
-  JoinSet ja{a.part, a.desc, 0, 0, 0}, jb{b.part, b.desc, kTcRows, 0, 16};
+  JoinSet ja{a.part, a.desc, 0, 0, 0}, jb{b.part, b.desc, kTcRows, 0, kTcRows / 32 * (p.pg.head_dim / 16) / kJoinWarps};
   if (attn_mma_takes(p)) {
     // chunks of up to 64 rows are bound by the copies of K and V, which mma.sync
     // keeps up with; above, the 256-row items of tcgen05

@@ -248,7 +248,7 @@ __device__ void q_role(const AttnChunksParams &p, TcWalk w, TcBars &b, uint32_t 
   }
 }
 
-// 32 consecutive f32 or 16-bit values of a thread's row, 32 bytes a store
+// 32 bytes of a thread's row (aligned to 32)
 __device__ __forceinline__ void st8(void *p, const uint32_t (&v)[8]) {
   asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]),
                "r"(v[6]), "r"(v[7])
@@ -354,14 +354,10 @@ __device__ void softmax_role(const AttnChunksParams &p, TcWalk w, TcBars &b, uin
         for (uint32_t e = 0; e < 32; ++e) o[e] = 0.0f;
       }
       if (!live) continue;
-      if (!whole) {
+      if (!whole) {  // [32 rows][4 elements] blocks: a warp's store is 512 bytes in a row
 #pragma unroll
-        for (uint32_t e = 0; e < 32; e += 8) {
-          uint32_t v[8];
-#pragma unroll
-          for (uint32_t j = 0; j < 8; ++j) v[j] = __float_as_uint(o[e + j]);
-          st8(slot + r * HD + c + e, v);
-        }
+        for (uint32_t e = 0; e < 32; e += 4)
+          *reinterpret_cast<float4 *>(slot + tc_part(r, c + e, HD)) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
         continue;
       }
       uint32_t v[16];
