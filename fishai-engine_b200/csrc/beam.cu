@@ -12,11 +12,9 @@
 // The candidates of a tile of 4096 logits: a thread's largest value that does
 // not beat the range's k-th best so far ends the matter for its 16 elements,
 // and a tile in which nothing does is passed by.  Where more than 64 threads
-// have candidates (the first tile, rising rows) the k-th largest of the
-// threads' largest bounds the tile's k-th best from below, so that at most
-// 16 * 64 elements are left; these are ranked against the list by counting.
-// Bounding every tile made the scan 4 times as long (137 us for 256 rows of
-// 128256).
+// have candidates a bound leaves a few dozen; what is left is ranked against
+// the list by counting.  (Bounding every tile exactly made the scan three times
+// as long: 137 us for 256 rows of 128256.)
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -29,6 +27,7 @@ namespace fa {
 namespace {
 
 constexpr uint32_t kScanThreads = 256, kScanElems = 16, kTile = kScanThreads * kScanElems;
+constexpr uint32_t kBuf = kScanElems * kBeamMaxK;  // candidates of a tile
 constexpr uint32_t kPickThreads = 256;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -69,7 +68,7 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(kScanThreads, 4) k_beam_scan(const BeamParams p) {
   pdl_launch_dependents();
   __shared__ __align__(16) unsigned long long tops[kScanThreads];
-  __shared__ unsigned long long list[2][kBeamMaxK], buf[kScanElems * kBeamMaxK + kBeamMaxK];
+  __shared__ unsigned long long list[2][kBeamMaxK], buf[kBuf + kBeamMaxK];
   __shared__ uint32_t n_buf[2], n_list[2];
   __shared__ unsigned long long bound;
   __shared__ float wm[kScanThreads / 32], wsum[kScanThreads / 32];
@@ -120,8 +119,40 @@ __global__ void __launch_bounds__(kScanThreads, 4) k_beam_scan(const BeamParams 
     const bool beats = t > kv;
     const uint32_t n_tops = __syncthreads_count(beats);
     if (!n_tops) continue;
+    // What may be among the tile's best: all that beats the list, or, where
+    // many threads have some (the first tile, rising rows), what reaches the
+    // least of the largest values of as many groups of threads as there are to
+    // choose: 8 warps, or 64 groups of 4 lanes.
     unsigned long long low = 1;
-    if (n_tops > kBeamMaxK) {  // too many for the buffer, as in the first tile: bound them
+    const bool many = n_tops > kBeamMaxK;
+    if (many) {
+      float g = t;
+      const uint32_t span = K <= kScanThreads / 32 ? 32 : 4;
+      for (uint32_t o = 1; o < span; o <<= 1) g = fmaxf(g, __shfl_xor_sync(0xFFFFFFFFu, g, o));
+      for (uint32_t o = span; o < 32; o <<= 1) g = fminf(g, __shfl_xor_sync(0xFFFFFFFFu, g, o));
+      if (tid % 32 == 0) tops[tid / 32] = float_key(g);
+      __syncthreads();
+      unsigned long long v = tops[0];
+#pragma unroll
+      for (uint32_t i = 1; i < kScanThreads / 32; ++i) v = min(v, tops[i]);
+      low = max(v << 32, 1ull);
+    }
+    auto append = [&] {
+      if (!beats) return;
+#pragma unroll
+      for (uint32_t i = 0; i < kScanElems; ++i)
+        if (x[i] > kv) {
+          const unsigned long long c = cand_key(x[i], v0 + (i / 4 * kScanThreads + tid) * 4 + i % 4);
+          if (c < low) continue;
+          const uint32_t to = atomicAdd(&n_buf[cur], 1u);
+          if (to < kBuf) buf[to] = c;
+        }
+    };
+    append();
+    __syncthreads();
+    if (n_buf[cur] > kBuf) {
+      // more than the buffer holds: the exact bound, the k-th largest of the
+      // threads' largest, which at most 16 k elements reach
       unsigned long long best = 0;
       if (beats) {
 #pragma unroll
@@ -137,18 +168,12 @@ __global__ void __launch_bounds__(kScanThreads, 4) k_beam_scan(const BeamParams 
         above += (o.x > best) + (o.y > best);
       }
       if (best && above == K - 1) bound = best;  // n_tops > 64 >= K: one thread's
+      if (tid == 0) n_buf[cur] = 0;
       __syncthreads();
       low = bound;
+      append();
+      __syncthreads();
     }
-    if (beats) {
-#pragma unroll
-      for (uint32_t i = 0; i < kScanElems; ++i)
-        if (x[i] > kv) {
-          const unsigned long long c = cand_key(x[i], v0 + (i / 4 * kScanThreads + tid) * 4 + i % 4);
-          if (c >= low) buf[atomicAdd(&n_buf[cur], 1u)] = c;  // at most 16 of each of 64 threads
-        }
-    }
-    __syncthreads();
     // the list and the tile's candidates, ranked by counting (all keys differ)
     const uint32_t n = n_buf[cur], n_old = n_list[cur], all = n + n_old;
     if (tid < n_old) buf[n + tid] = list[cur][tid];

@@ -25,11 +25,6 @@ constexpr uint32_t kAnyThreads = 128, kAnyPos = 64;
 template <typename T>
 __device__ __forceinline__ void load8(const T *p, float (&x)[8]);  // 16-byte aligned
 template <>
-__device__ __forceinline__ void load8<float>(const float *p, float (&x)[8]) {
-  const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 4);
-  x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-}
-template <>
 __device__ __forceinline__ void load8<__half>(const __half *p, float (&x)[8]) {
   const uint4 a = *reinterpret_cast<const uint4 *>(p);
   const __half2 *h = reinterpret_cast<const __half2 *>(&a);
@@ -53,6 +48,50 @@ __device__ __forceinline__ void put(float *p, float x) { *p = x; }
 __device__ __forceinline__ void put(__half *p, float x) { *p = __float2half_rn(x); }
 __device__ __forceinline__ void put(__nv_bfloat16 *p, float x) { *p = __float2bfloat16_rn(x); }
 
+// K and V of positions [t0, t0 + 64) to shared memory as f32; positions outside
+// the item's range and bad pages as zeros.  The tile's four pages are looked up
+// first and the copies are independent, so that they are all in flight: f32 by
+// cp.async, 16-bit types through registers.  (A look-up with each 32-byte load
+// took 19 us for a tile where this takes 8.)
+template <typename T>
+__device__ __forceinline__ void fetch(const AttnChunksParams &p, const T *base, const uint32_t *pt, const Segment &s, uint32_t t0,
+                                      float *sk, float *sv, uint32_t ld, uint32_t tid) {
+  constexpr uint32_t kV = 16 / sizeof(T);  // elements of a copy
+  const uint32_t hd = p.pg.head_dim, per_row = hd / kV, total = 2 * kAnyPos * per_row;
+  uint32_t page[kAnyPos / kPageLen];
+#pragma unroll
+  for (uint32_t j = 0; j < kAnyPos / kPageLen; ++j) {
+    const uint32_t t = t0 + j * kPageLen;
+    page[j] = t < s.hi && t + kPageLen > s.lo ? __ldg(pt + t / kPageLen) : 0u;
+  }
+  bool bad = false;
+  uint64_t row0[kAnyPos / kPageLen];
+#pragma unroll
+  for (uint32_t j = 0; j < kAnyPos / kPageLen; ++j) {
+    bad |= page[j] >= p.pg.n_pages;
+    row0[j] = page[j] < p.pg.n_pages ? page_row(p.pg, page[j], 0, s.head, 0) : ~0ull;
+  }
+  if (bad && p.err) atomicOr(p.err, kFlagPage);
+  const uint64_t v_off = (uint64_t)p.pg.n_kv_heads * kPageLen * hd;  // V after the heads' K
+#pragma unroll 4
+  for (uint32_t i = tid; i < total; i += kAnyThreads) {
+    const uint32_t e = i / per_row, d = (i - e * per_row) * kV, is_v = e / kAnyPos, r = e % kAnyPos, t = t0 + r, j = r / kPageLen;
+    const uint64_t r0 = j == 0 ? row0[0] : j == 1 ? row0[1] : j == 2 ? row0[2] : row0[3];
+    const bool ok = t >= s.lo && t < s.hi && r0 != ~0ull;
+    const T *src = base + (ok ? r0 + is_v * v_off + (t % kPageLen) * hd + d : 0);
+    float *dst = (is_v ? sv : sk) + r * ld + d;
+    if constexpr (sizeof(T) == 4) {
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(ok ? 16u : 0u) : "memory");
+    } else {
+      float x[8] = {};
+      if (ok) load8(src, x);
+      reinterpret_cast<float4 *>(dst)[0] = make_float4(x[0], x[1], x[2], x[3]);
+      reinterpret_cast<float4 *>(dst)[1] = make_float4(x[4], x[5], x[6], x[7]);
+    }
+  }
+  if constexpr (sizeof(T) == 4) asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
 constexpr uint32_t any_smem(uint32_t R, uint32_t hd) { return ((R + 2 * kAnyPos) * (hd + 4) + R * (kAnyPos + 4)) * 4; }
 
 // HJ: groups of 64 head elements (hd <= 64 HJ)
@@ -73,14 +112,15 @@ __global__ void __launch_bounds__(kAnyThreads) k_attn_any(const AttnChunksParams
     const Segment s = w.next(p);
     const uint32_t *pt = p.pg.page_table + (uint64_t)s.chunk.seq * p.pg.max_pages;
     __syncthreads();
-    // Q rows times the scale (log2 domain); rows past the item's are zero
-    for (uint32_t i = tid; i < R * hd; i += kAnyThreads) {
-      const uint32_t r = i / hd, d = i - r * hd, row = s.r0 + r;
-      float x = 0.0f;
-      if (row < s.r1)
-        x = (float)reinterpret_cast<const T *>(p.q)[(uint64_t)(s.chunk.q0 + row / p.rep) * p.qs +
-                                                   (s.head * p.rep + row % p.rep) * hd + d];
-      sq[r * ld + d] = x;
+    // Q rows; past the item's: zeros
+    for (uint32_t r = tid / 32; r < R; r += kAnyThreads / 32) {  // a warp a row
+      const uint32_t row = s.r0 + r, tok = row / p.rep;
+      const T *x = reinterpret_cast<const T *>(p.q) + (uint64_t)(s.chunk.q0 + tok) * p.qs + (s.head * p.rep + row - tok * p.rep) * hd;
+#pragma unroll
+      for (uint32_t j = 0; j < 2 * HJ; ++j) {
+        const uint32_t d = tid % 32 + 32 * j;
+        if (d < hd) sq[r * ld + d] = row < s.r1 ? (float)x[d] : 0.0f;
+      }
     }
     float m[RT], l[RT], o[RT][HJ][4];
     int32_t pos[RT];  // position of each row's token
@@ -96,19 +136,7 @@ __global__ void __launch_bounds__(kAnyThreads) k_attn_any(const AttnChunksParams
     for (uint32_t u = s.u0; u < s.u1 && s.hi > s.lo; ++u) {
       const uint32_t t0 = (s.lo / kAnyPos + u) * kAnyPos;
       __syncthreads();
-      for (uint32_t i = tid; i < 2 * kAnyPos * (hd / 8); i += kAnyThreads) {
-        const uint32_t is_v = i >= kAnyPos * (hd / 8), e = i - is_v * kAnyPos * (hd / 8), r = e / (hd / 8), d = e % (hd / 8) * 8;
-        const uint32_t t = t0 + r;
-        float x[8] = {};
-        if (t >= s.lo && t < s.hi) {
-          const uint32_t page = pt[t / kPageLen];
-          if (page < p.pg.n_pages) load8(base + page_row(p.pg, page, is_v, s.head, t % kPageLen) + d, x);
-          else if (p.err) atomicOr(p.err, kFlagPage);
-        }
-        float4 *dst = reinterpret_cast<float4 *>((is_v ? sv : sk) + r * ld + d);
-        dst[0] = make_float4(x[0], x[1], x[2], x[3]);
-        dst[1] = make_float4(x[4], x[5], x[6], x[7]);
-      }
+      fetch<T>(p, base, pt, s, t0, sk, sv, ld, tid);
       __syncthreads();
       float a[RT][4];
 #pragma unroll

@@ -20,48 +20,60 @@ NO_TOKEN = -1  # in int32 `seqs` of rope_append: the row is left out
 FLAG_PAGE, FLAG_RANGE, FLAG_TIMEOUT = L.FLAG_PAGE, L.FLAG_RANGE, L.FLAG_TIMEOUT
 
 _DTYPES = {}  # torch dtype -> FA_KV_*
+_INTS = set()  # the 32-bit index types
+_ONE = (1,)
 
 
+def _learn():
+    torch = sys.modules["torch"]
+    _DTYPES.update({torch.float32: L.KV_F32, torch.float16: L.KV_F16, torch.bfloat16: L.KV_BF16})
+    _INTS.update({torch.int32, torch.uint32})
+
+
+# The checks run at every call, in front of kernels of a few microseconds: one
+# look at dtype, stride and length each, the reasons worked out only on failure.
 def _code(t, name):
     """the FA_KV_* id of a tensor's element type"""
-    if not _DTYPES:
-        torch = sys.modules["torch"]
-        _DTYPES.update({torch.float32: L.KV_F32, torch.float16: L.KV_F16, torch.bfloat16: L.KV_BF16})
     code = _DTYPES.get(t.dtype)
     if code is None:
+        if not _DTYPES:
+            _learn()
+            return _code(t, name)
         raise ValueError(f"{name}: element type {t.dtype} is not float32, float16 or bfloat16")
     return code
 
 
-def _index(t, name, n=None):
-    """address of a contiguous array of n 32-bit whole numbers; None passes"""
-    if t is None:
-        return None
-    if t.dim() != 1 or t.element_size() != 4 or t.is_floating_point() or not t.is_contiguous():
-        raise ValueError(f"{name}: a contiguous 1-d int32 tensor is needed")
-    if n is not None and t.shape[0] != n:
-        raise ValueError(f"{name}: {t.shape[0]} entries, {n} needed")
+def _index(t, name, n):
+    """address of a contiguous array of n 32-bit whole numbers"""
+    if t.dtype not in _INTS or (t.stride() != _ONE and t.dim() != 1) or len(t) != n or (n > 1 and t.stride() != _ONE):
+        if not _INTS:
+            _learn()
+            return _index(t, name, n)
+        if t.dtype not in _INTS or t.dim() != 1 or not t.is_contiguous():
+            raise ValueError(f"{name}: a contiguous 1-d int32 tensor is needed")
+        raise ValueError(f"{name}: {len(t)} entries, {n} needed")
     return t.data_ptr()
 
 
-def _rows(t, name, width):
-    """address and row stride of [n, width] rows with unit inner stride"""
-    shape = t.shape
+def _rows(t, name, n, width):
+    """address and row stride of n rows of `width` consecutive elements, [n, width] or [n, heads, head_dim]"""
+    shape, stride = t.shape, t.stride()
     if len(shape) == 2:
-        if shape[1] != width:
-            raise ValueError(f"{name}: rows of {shape[1]}, {width} needed")
-        stride, inner = t.stride()
-    elif len(shape) == 3:
-        if shape[1] * shape[2] != width:
-            raise ValueError(f"{name}: rows of {shape[1]} x {shape[2]}, {width} in all needed")
-        stride, mid, inner = t.stride()
-        if shape[1] > 1 and mid != shape[2]:
-            raise ValueError(f"{name}: the heads of a row are not consecutive")
+        ok = shape[1] == width and stride[1] == 1
     else:
-        raise ValueError(f"{name}: [tokens, heads * head_dim] or [tokens, heads, head_dim] needed")
-    if inner != 1 and width > 1:
-        raise ValueError(f"{name}: the elements of a row are not consecutive")
-    return t.data_ptr(), max(stride, width) if shape[0] <= 1 else stride
+        ok = len(shape) == 3 and shape[1] * shape[2] == width and stride[2] == 1 and (shape[1] == 1 or stride[1] == shape[2])
+    if not ok or shape[0] != n:
+        raise ValueError(f"{name}: {n} rows of {width} consecutive elements are needed, got {list(shape)} with strides {stride}")
+    return t.data_ptr(), stride[0] if n > 1 else width
+
+
+def _width(q, head_dim):
+    """elements of a row of whole heads"""
+    shape = q.shape
+    width = shape[1] if len(shape) == 2 else shape[1] * shape[2] if len(shape) == 3 else 0
+    if not width or width % head_dim:
+        raise ValueError(f"q: [tokens, heads * {head_dim}] or [tokens, heads, {head_dim}] needed, got {list(shape)}")
+    return width
 
 
 class PagedKV:
@@ -147,24 +159,31 @@ def rope_append(kv: PagedKV, layer: int, rope: Rope, q, k, v, positions, seqs, o
     at cache position slots[t] (default positions[t]) of sequence seqs[t].  q, k
     and v are rows of one type, with any row stride (slices of a fused
     projection).  seqs[t] = NO_TOKEN leaves a row out."""
-    n = q.shape[0]
+    n = len(q)
     dt = _code(q, "q")
     if k.dtype != q.dtype or v.dtype != q.dtype:
         raise ValueError("q, k and v have one element type")
     if _code(out, "out") != kv.dtype:
         raise ValueError("out has another element type than the pages")
-    if k.shape[0] != n or v.shape[0] != n or out.shape[0] != n:
-        raise ValueError("q, k, v and out have one row for each token")
-    width = q.shape[1] if len(q.shape) == 2 else q.shape[1] * q.shape[2]
-    if width % kv.head_dim:
-        raise ValueError("q: rows are whole heads")
-    qp, qs = _rows(q, "q", width)
-    kp, ks = _rows(k, "k", kv._kv_width)
-    vp, vs = _rows(v, "v", kv._kv_width)
-    op, os = _rows(out, "out", width)
-    L.check(L.lib().fa_rope_append(rope._h, kv._ref, layer, dt, qp, qs, kp, ks, vp, vs, n, width // kv.head_dim,
-                                   _index(positions, "positions", n), _index(seqs, "seqs", n),
-                                   _index(slots, "slots", n), op, os, _index(err, "err"), stream))
+    hd, kw = kv.head_dim, kv._kv_width
+    width = _width(q, hd)
+    qp, qs = _rows(q, "q", n, width)
+    kp, ks = _rows(k, "k", n, kw)
+    vp, vs = _rows(v, "v", n, kw)
+    op, os = _rows(out, "out", n, width)
+    rc = L.lib().fa_rope_append(rope._h, kv._ref, layer, dt, qp, qs, kp, ks, vp, vs, n, width // hd,
+                                _index(positions, "positions", n), _index(seqs, "seqs", n),
+                                None if slots is None else _index(slots, "slots", n), op, os,
+                                None if err is None else _index(err, "err", 1), stream)
+    if rc:
+        L.check(rc)
+
+
+def _space(t):
+    """address and bytes of a contiguous workspace tensor"""
+    if not t.is_contiguous():
+        raise ValueError("workspace: contiguous")
+    return t.data_ptr(), t.numel() * t.element_size()
 
 
 def workspace_bytes(head_dim: int) -> int:
@@ -181,38 +200,36 @@ def attention(kv: PagedKV, layer: int, q, q_start, kv_len, out, max_q: int, work
     max_q: no chunk is longer.  workspace: a uint8 tensor of
     workspace_bytes(head_dim), used by no other call that may run at the same
     time.  scale 0: 1 / sqrt(head_dim)."""
-    n = q_start.shape[0] - 1
-    if n < 0:
-        raise ValueError("q_start: chunks + 1 entries")
+    n, t = len(kv_len), len(q)
     if _code(q, "q") != kv.dtype or out.dtype != q.dtype:
         raise ValueError("q and out have the pages' element type")
-    width = q.shape[1] if len(q.shape) == 2 else q.shape[1] * q.shape[2]
-    if width % kv.head_dim or out.shape[0] != q.shape[0]:
-        raise ValueError("q: rows are whole heads, and out has as many rows")
     if window < 0 or max_q < 0:
         raise ValueError("window and max_q are not negative")
-    qp, qs = _rows(q, "q", width)
-    op, os = _rows(out, "out", width)
-    if not workspace.is_contiguous():
-        raise ValueError("workspace: contiguous")
-    L.check(L.lib().fa_attn_chunks(kv._ref, layer, qp, qs, width // kv.head_dim, n, _index(q_start, "q_start"),
-                                   _index(kv_len, "kv_len", n), _index(seqs, "seqs", n), q.shape[0], max_q, scale,
-                                   window, op, os, workspace.data_ptr(), workspace.numel() * workspace.element_size(),
-                                   _index(err, "err"), stream))
+    hd = kv.head_dim
+    width = _width(q, hd)
+    qp, qs = _rows(q, "q", t, width)
+    op, os = _rows(out, "out", t, width)
+    rc = L.lib().fa_attn_chunks(kv._ref, layer, qp, qs, width // hd, n, _index(q_start, "q_start", n + 1),
+                                _index(kv_len, "kv_len", n), None if seqs is None else _index(seqs, "seqs", n), t, max_q,
+                                scale, window, op, os, *_space(workspace), None if err is None else _index(err, "err", 1),
+                                stream)
+    if rc:
+        L.check(rc)
 
 
 def copy_pages(kv: PagedKV, src, dst, slots=None, err=None, stream: int = 0):
     """Copies the first slots[i] positions (default: all 16) of page src[i] to
     page dst[i] in every layer."""
-    n = src.shape[0]
-    L.check(L.lib().fa_pages_copy(kv._ref, _index(src, "src"), _index(dst, "dst", n), _index(slots, "slots", n), n,
-                                  _index(err, "err"), stream))
+    n = len(src)
+    L.check(L.lib().fa_pages_copy(kv._ref, _index(src, "src", n), _index(dst, "dst", n),
+                                  None if slots is None else _index(slots, "slots", n), n,
+                                  None if err is None else _index(err, "err", 1), stream))
 
 
 def compact(kv: PagedKV, seqs, keep, keep_start, err=None, stream: int = 0):
     """Keeps the positions keep[keep_start[i]:keep_start[i+1]] (ascending) of
     sequence seqs[i] as its first positions, in place and in every layer."""
-    n = seqs.shape[0]
-    L.check(L.lib().fa_pages_compact(kv._ref, _index(seqs, "seqs"), _index(keep, "keep"),
-                                     _index(keep_start, "keep_start", n + 1), n, keep.shape[0], _index(err, "err"),
-                                     stream))
+    n = len(seqs)
+    L.check(L.lib().fa_pages_compact(kv._ref, _index(seqs, "seqs", n), _index(keep, "keep", len(keep)),
+                                     _index(keep_start, "keep_start", n + 1), n, len(keep),
+                                     None if err is None else _index(err, "err", 1), stream))
