@@ -3,10 +3,28 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
-#include "paged_attn.cuh"
+#include <cudaTypedefs.h>
+
+#include <mutex>
+
+#include "paged_tma.cuh"
 
 namespace fa {
 namespace {
+
+PFN_cuTensorMapEncodeTiled_v12000 encoder() {
+  static std::mutex mu;
+  static PFN_cuTensorMapEncodeTiled_v12000 f = nullptr;
+  std::lock_guard<std::mutex> lock(mu);
+  if (!f) {
+    cudaDriverEntryPointQueryResult q;
+    void *fn = nullptr;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
+      return nullptr;
+    f = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+  }
+  return f;
+}
 
 __device__ __forceinline__ void put(float *p, float x) { *p = x; }
 __device__ __forceinline__ void put(__half *p, float x) { *p = __float2half_rn(x); }
@@ -178,6 +196,18 @@ constexpr size_t kSmallSlots = (size_t)2 * kAttnMaxCtas * kAttnMaxRows, kTcSlots
 
 }  // namespace
 
+bool page_map(const AttnChunksParams &p, CUtensorMap *map) {
+  const PFN_cuTensorMapEncodeTiled_v12000 encode = encoder();
+  if (!encode) return false;
+  const uint32_t es = elem_size(p.pg.dtype);
+  const cuuint64_t dims[2] = {p.pg.head_dim, (cuuint64_t)p.pg.n_pages * 2 * p.pg.n_kv_heads * kPageLen}, strides[1] = {(cuuint64_t)p.pg.head_dim * es};
+  const cuuint32_t box[2] = {64, kPageLen}, one[2] = {1, 1};
+  void *base = static_cast<char *>(p.pg.base) + (uint64_t)p.layer * p.pg.layer_stride * es;
+  return encode(map, p.pg.dtype == FA_KV_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, dims, strides, box,
+                one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // slots of the launch for few rows, of the one for many, descriptors
 size_t attn_chunks_ws(uint32_t head_dim) {
   return (kSmallSlots + kTcSlots) * (head_dim + 2) * 4 + (kAttnMaxCtas + kTcMaxCtas) * sizeof(uint4);
@@ -206,8 +236,9 @@ int launch_attn_chunks(const AttnChunksParams &p, void *ws, uint32_t n_sm, cudaS
   } else if (!(ja.ctas = launch_attn_any(a, n_sm, st, &ja.R))) {
     return -1;
   }
-  // CTAs to an item: eight rows each, or the few rows of one long cache
-  ja.parts = jb.ctas ? 2 : ja.R < 16 ? ja.R : 8;
+  // CTAs to an item: a row each, for the few rows of one long cache
+  const uint64_t rows = (uint64_t)p.max_q * p.rep;
+  ja.parts = jb.ctas ? 2 : rows < 8 ? (uint32_t)rows : 8;
   switch (p.pg.dtype) {
     case FA_KV_F32: return launch_join<float>(p, ja, jb, st);
     case FA_KV_F16: return launch_join<__half>(p, ja, jb, st);

@@ -28,14 +28,10 @@
 // Waits are bounded; one that runs out sets an abort flag that the others see,
 // and the kernel drains its copies and MMAs, frees the tensor memory and sets
 // FA_FLAG_TIMEOUT.
-#include <cuda.h>
-#include <cudaTypedefs.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
-#include <mutex>
-
-#include "paged_attn.cuh"
+#include "paged_tma.cuh"
 
 namespace fa {
 namespace {
@@ -89,11 +85,6 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
       "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
       " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc)
       : "memory");
-}
-__device__ __forceinline__ void tma_2d(uint32_t dst, const void *map, int32_t x, int32_t y, uint64_t *bar) {
-  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
-               "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar))
-               : "memory");
 }
 __device__ __forceinline__ void ld32(uint32_t addr, float *v) {
   asm volatile(
@@ -174,22 +165,6 @@ __device__ __forceinline__ void weights32(const float *x, uint64_t scale, uint64
   }
 }
 
-// Bounded wait; false: it ran out here or elsewhere in the CTA
-__device__ __forceinline__ bool wait_bar(TcBars &b, uint64_t *bar, uint32_t parity) {
-  const uint32_t addr = smem_u32(bar);
-  for (uint32_t i = 0; i < kMaxWaitTries; ++i) {
-    uint32_t ok;
-    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
-                 : "=r"(ok)
-                 : "r"(addr), "r"(parity)
-                 : "memory");
-    if (ok) return true;
-    if ((i & 255) == 255 && *reinterpret_cast<volatile uint32_t *>(&b.abort)) return false;
-  }
-  *reinterpret_cast<volatile uint32_t *>(&b.abort) = 1;
-  return false;
-}
-
 using TcWalk = Walk<kTcRows, kTcPos, kTcThreads>;
 
 // Q rows [first, first + 128) of the item to a swizzled tile, 64 threads; rows
@@ -238,7 +213,7 @@ __device__ void q_role(const AttnChunksParams &p, TcWalk w, TcBars &b, uint32_t 
 #pragma unroll
     for (uint32_t g = 0; g < 2; ++g) {
       if (s.r0 + 128 * g >= s.r1) break;
-      if (!wait_bar(b, &b.q_empty[g], (n[g] & 1) ^ 1)) return;
+      if (!wait_bar(&b.abort, &b.q_empty[g], (n[g] & 1) ^ 1)) return;
       load_q<T, HD>(p, s, s.r0 + 128 * g, smem + g * TcCfg<HD>::kTile, tid);
       asm volatile("cp.async.wait_all;" ::: "memory");
       fence_proxy_async_smem();
@@ -270,7 +245,7 @@ __device__ void softmax_role(const AttnChunksParams &p, TcWalk w, TcBars &b, uin
     float m = -INFINITY, l = 0.0f;
     for (uint32_t k = 0; k < tiles; ++k, ++n) {
       const uint32_t t0 = (s.lo / kTcPos + s.u0 + k) * kTcPos;
-      if (!wait_bar(b, &b.s_full[g], n & 1)) return;
+      if (!wait_bar(&b.abort, &b.s_full[g], n & 1)) return;
       fence_after();
       float x[kTcPos];
 #pragma unroll
@@ -300,7 +275,7 @@ __device__ void softmax_role(const AttnChunksParams &p, TcWalk w, TcBars &b, uin
         l *= f;
       }
       if (k && __any_sync(0xFFFFFFFFu, f != 1.0f)) {
-        if (!wait_bar(b, &b.o_full[g], (n - 1) & 1)) return;
+        if (!wait_bar(&b.abort, &b.o_full[g], (n - 1) & 1)) return;
         fence_after();
 #pragma unroll 1
         for (uint32_t c = 0; c < HD; c += 32) {
@@ -338,7 +313,7 @@ __device__ void softmax_role(const AttnChunksParams &p, TcWalk w, TcBars &b, uin
     const uint32_t r = row - s.r0, tok = row / p.rep;
     T *out = reinterpret_cast<T *>(p.out) + (uint64_t)(s.chunk.q0 + tok) * p.os + (s.head * p.rep + row - tok * p.rep) * HD;
     if (tiles) {
-      if (!wait_bar(b, &b.o_full[g], (n - 1) & 1)) return;
+      if (!wait_bar(&b.abort, &b.o_full[g], (n - 1) & 1)) return;
       fence_after();
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -419,9 +394,9 @@ __device__ void mma_role(const AttnChunksParams &p, TcWalk w, TcBars &b, uint32_
     const Segment s = w.next(p);
     const uint32_t tiles = s.hi > s.lo ? s.u1 - s.u0 : 0, groups = s.r1 - s.r0 > 128 ? 2 : 1;
     if (!tiles) continue;
-    if (!wait_bar(b, &b.full[at.st], at.ph)) return;
+    if (!wait_bar(&b.abort, &b.full[at.st], at.ph)) return;
     for (uint32_t g = 0; g < groups; ++g) {
-      if (!wait_bar(b, &b.q_full[g], q_phase[g])) return;
+      if (!wait_bar(&b.abort, &b.q_full[g], q_phase[g])) return;
       q_phase[g] ^= 1;
       fence_after();
       scores(g, at.st);
@@ -435,12 +410,12 @@ __device__ void mma_role(const AttnChunksParams &p, TcWalk w, TcBars &b, uint32_
       const Place next = at;
       const bool more = k + 1 < tiles;
       if (more) at.step();
-      if (!wait_bar(b, &b.full[v.st], v.ph)) return;
+      if (!wait_bar(&b.abort, &b.full[v.st], v.ph)) return;
       const uint32_t vt = v_lo + v.st * (C::kTile >> 4);
       for (uint32_t g = 0; g < groups; ++g) {
 #pragma unroll
         for (uint32_t h = 0; h < 2; ++h) {
-          if (!wait_bar(b, h ? &b.p_full[g] : &b.p_half[g], n[g] & 1)) return;
+          if (!wait_bar(&b.abort, h ? &b.p_full[g] : &b.p_half[g], n[g] & 1)) return;
           fence_after();
 if (lead)
 #pragma unroll
@@ -451,7 +426,7 @@ if (lead)
         if (lead) commit(&b.o_full[g]);
         if (g + 1 == groups && lead) commit(&b.empty[v.st]);
         if (more) {
-          if (g == 0 && !wait_bar(b, &b.full[next.st], next.ph)) return;
+          if (g == 0 && !wait_bar(&b.abort, &b.full[next.st], next.ph)) return;
           scores(g, next.st);
           if (k + 2 == tiles && lead) commit(&b.q_empty[g]);  // the item's last scores
         }
@@ -466,7 +441,6 @@ template <typename T, uint32_t HD>
 __device__ void load_role(const AttnChunksParams &p, TcWalk w, TcBars &b, uint32_t smem, const CUtensorMap *map, uint32_t &fills) {
   using C = TcCfg<HD>;
   const uint32_t lane = threadIdx.x & 31, ring = smem + 2 * C::kTile;
-  const int32_t none = (int32_t)(p.pg.n_pages * 2 * p.pg.n_kv_heads * kPageLen);  // a row past the end: zeros
   uint32_t seq = 0, tail = 0;
   while (!w.done()) {
     const Segment s = w.next(p);
@@ -488,13 +462,12 @@ __device__ void load_role(const AttnChunksParams &p, TcWalk w, TcBars &b, uint32
       const bool ragged = (s.hi < t0 + kTcPos && s.hi % kPageLen) || (s.lo > t0 && s.lo % kPageLen);
       for (uint32_t is_v = 0; is_v < 2; ++is_v, ++seq) {
         const uint32_t st = seq % C::kStages, dst = ring + st * C::kTile;
-        if (!wait_bar(b, &b.empty[st], (seq / C::kStages & 1) ^ 1)) return;
+        if (!wait_bar(&b.abort, &b.empty[st], (seq / C::kStages & 1) ^ 1)) return;
         uint64_t *bar = is_v && ragged ? &b.tail : &b.full[st];
         if (lane == 0) mbar_arrive_expect_tx(bar, C::kTile);
         __syncwarp();
         if (lane < 8 * (HD / 64)) {
-          const int32_t y = page < p.pg.n_pages ? (int32_t)(((page * 2 + is_v) * p.pg.n_kv_heads + s.head) * kPageLen) : none;
-          tma_2d(dst + (lane >> 3) * C::kHalf + (lane & 7) * 2048, map, (int32_t)(lane >> 3) * 64, y, bar);
+          tma_2d(dst + (lane >> 3) * C::kHalf + (lane & 7) * 2048, map, (int32_t)(lane >> 3) * 64, map_row(p.pg, page, is_v, s.head), bar);
         }
         if (is_v && ragged) {
           if (!mbar_wait(&b.tail, tail & 1)) {
@@ -588,33 +561,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_tc(const AttnChunksParam
   pdl_wait();  // the launch before this one, with which it may have overlapped: the join waits for this one only
 }
 
-PFN_cuTensorMapEncodeTiled_v12000 encoder() {
-  static std::mutex mu;
-  static PFN_cuTensorMapEncodeTiled_v12000 f = nullptr;
-  std::lock_guard<std::mutex> lock(mu);
-  if (!f) {
-    cudaDriverEntryPointQueryResult q;
-    void *fn = nullptr;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
-      return nullptr;
-    f = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
-  }
-  return f;
-}
-
 template <typename T, uint32_t HD>
 int launch_hd(const AttnChunksParams &p, uint32_t ctas, cudaStream_t st) {
-  const PFN_cuTensorMapEncodeTiled_v12000 encode = encoder();
-  if (!encode) return -1;
-  // the layer's pages as rows of a head: [page][k | v][kv head][16] x head_dim, boxes of 16 rows x 64 elements
   CUtensorMap map;
-  const cuuint64_t dims[2] = {HD, (cuuint64_t)p.pg.n_pages * 2 * p.pg.n_kv_heads * kPageLen}, strides[1] = {HD * 2};
-  const cuuint32_t box[2] = {64, kPageLen}, one[2] = {1, 1};
-  void *base = static_cast<char *>(p.pg.base) + (uint64_t)p.layer * p.pg.layer_stride * 2;
-  if (encode(&map, __is_same(T, __half) ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, dims, strides, box, one,
-             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-    return -1;
+  if (!page_map(p, &map)) return -1;
   if (cudaFuncSetAttribute(k_attn_tc<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)TcCfg<HD>::kSmem) != cudaSuccess) return -1;
   return launch_pdl(k_attn_tc<T, HD>, dim3(ctas), dim3(kTcThreads), TcCfg<HD>::kSmem, st, p, map);
 }

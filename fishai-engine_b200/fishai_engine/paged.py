@@ -45,13 +45,16 @@ def _code(t, name):
 
 def _index(t, name, n):
     """address of a contiguous array of n 32-bit whole numbers"""
-    if t.dtype not in _INTS or (t.stride() != _ONE and t.dim() != 1) or len(t) != n or (n > 1 and t.stride() != _ONE):
+    if t.dtype not in _INTS or t.stride() != _ONE or t.shape[0] != n:
         if not _INTS:
             _learn()
             return _index(t, name, n)
-        if t.dtype not in _INTS or t.dim() != 1 or not t.is_contiguous():
+        if t.dtype not in _INTS or t.dim() != 1:
             raise ValueError(f"{name}: a contiguous 1-d int32 tensor is needed")
-        raise ValueError(f"{name}: {len(t)} entries, {n} needed")
+        if t.shape[0] != n:
+            raise ValueError(f"{name}: {t.shape[0]} entries, {n} needed")
+        if n > 1:
+            raise ValueError(f"{name}: a contiguous 1-d int32 tensor is needed")
     return t.data_ptr()
 
 
@@ -141,7 +144,7 @@ class Rope:
         self._h = h
 
     def __del__(self):
-        if getattr(self, "_h", None):
+        if getattr(self, "_h", None) and L is not None:  # None: the interpreter is ending
             L.lib().fa_rope_free(self._h)
             self._h = None
 
@@ -159,7 +162,7 @@ def rope_append(kv: PagedKV, layer: int, rope: Rope, q, k, v, positions, seqs, o
     at cache position slots[t] (default positions[t]) of sequence seqs[t].  q, k
     and v are rows of one type, with any row stride (slices of a fused
     projection).  seqs[t] = NO_TOKEN leaves a row out."""
-    n = len(q)
+    n = q.shape[0]
     dt = _code(q, "q")
     if k.dtype != q.dtype or v.dtype != q.dtype:
         raise ValueError("q, k and v have one element type")
@@ -200,7 +203,7 @@ def attention(kv: PagedKV, layer: int, q, q_start, kv_len, out, max_q: int, work
     max_q: no chunk is longer.  workspace: a uint8 tensor of
     workspace_bytes(head_dim), used by no other call that may run at the same
     time.  scale 0: 1 / sqrt(head_dim)."""
-    n, t = len(kv_len), len(q)
+    n, t = kv_len.shape[0], q.shape[0]
     if _code(q, "q") != kv.dtype or out.dtype != q.dtype:
         raise ValueError("q and out have the pages' element type")
     if window < 0 or max_q < 0:
@@ -220,7 +223,7 @@ def attention(kv: PagedKV, layer: int, q, q_start, kv_len, out, max_q: int, work
 def copy_pages(kv: PagedKV, src, dst, slots=None, err=None, stream: int = 0):
     """Copies the first slots[i] positions (default: all 16) of page src[i] to
     page dst[i] in every layer."""
-    n = len(src)
+    n = src.shape[0]
     L.check(L.lib().fa_pages_copy(kv._ref, _index(src, "src", n), _index(dst, "dst", n),
                                   None if slots is None else _index(slots, "slots", n), n,
                                   None if err is None else _index(err, "err", 1), stream))
@@ -229,7 +232,7 @@ def copy_pages(kv: PagedKV, src, dst, slots=None, err=None, stream: int = 0):
 def compact(kv: PagedKV, seqs, keep, keep_start, err=None, stream: int = 0):
     """Keeps the positions keep[keep_start[i]:keep_start[i+1]] (ascending) of
     sequence seqs[i] as its first positions, in place and in every layer."""
-    n = len(seqs)
-    L.check(L.lib().fa_pages_compact(kv._ref, _index(seqs, "seqs", n), _index(keep, "keep", len(keep)),
-                                     _index(keep_start, "keep_start", n + 1), n, len(keep),
+    n = seqs.shape[0]
+    L.check(L.lib().fa_pages_compact(kv._ref, _index(seqs, "seqs", n), _index(keep, "keep", keep.shape[0]),
+                                     _index(keep_start, "keep_start", n + 1), n, keep.shape[0],
                                      None if err is None else _index(err, "err", 1), stream))

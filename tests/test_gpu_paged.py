@@ -221,6 +221,17 @@ def test_attention_several_items_a_cta(t, hd):
     attn_check([2000], [2000], 16, 8, hd, R.TYPES[t], window=300, seed=18)
 
 
+@pytest.mark.parametrize("t", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_batches_of_long_caches(t, hd):
+    """each CTA goes round its ring of copies dozens of times, over several items"""
+    kvs = [37 + i * 911 % 2960 for i in range(40)]
+    attn_check([1] * 40, kvs, 32, 8, hd, R.TYPES[t], seed=19)
+    attn_check([1 + i % 3 for i in range(40)], kvs, 64, 8, hd, R.TYPES[t], seed=20)
+    attn_check([1 + i % 8 for i in range(40)], kvs, 32, 8, hd, R.TYPES[t], window=1500, seed=21)
+    attn_check([16 - i % 3 for i in range(40)], kvs, 16, 4, hd, R.TYPES[t], seed=22)
+
+
 @pytest.mark.parametrize("t", ["f16", "f32"])
 def test_attention_many_chunks(t):
     rng = random.Random(3)
