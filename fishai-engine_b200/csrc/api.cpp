@@ -1282,3 +1282,57 @@ extern "C" int fa_decode_batch(fa_model *fm, fa_kv *kv, uint32_t b, const uint32
   return m.decode_batch(kv->kv, b, tokens, pos, sp, steps, ids_out, logits_out);
 }
 
+
+extern "C" int fa_generate_beams(fa_model *fm, const fa_beam_config *cfg, const uint32_t *prompt, uint32_t n_prompt,
+                                 uint32_t *out_ids, uint32_t *out_len, float *out_scores) {
+  API_NULL(fm);
+  API_NULL(cfg);
+  API_NULL(prompt);
+  API_NULL(out_ids);
+  Model &m = fm->m;
+  const uint32_t b = cfg->n_beams;
+  if (!b || b > 64) return fail(FA_ERR_INVALID, "fa_generate_beams: 1 to 64 beams");
+  if (!n_prompt) return fail(FA_ERR_INVALID, "fa_generate_beams: empty prompt");
+  if (!cfg->max_new) return fail(FA_ERR_INVALID, "fa_generate_beams: max_new is zero");
+  if (!std::isfinite(cfg->length_penalty)) return fail(FA_ERR_INVALID, "fa_generate_beams: length_penalty is not finite");
+  if (cfg->kv_dtype != FA_KV_F32 && cfg->kv_dtype != FA_KV_F16) return fail(FA_ERR_INVALID, "fa_generate_beams: bad kv_dtype");
+  if ((uint64_t)n_prompt + cfg->max_new > 0x7FFFFFFFu) return fail(FA_ERR_INVALID, "fa_generate_beams: too many positions");
+  for (uint32_t i = 0; i < n_prompt; ++i)
+    if (prompt[i] >= m.cfg.vocab_size) return fail(FA_ERR_INVALID, "token id out of range");
+  if (!m.tc_ok || m.tied || !m.head.mma)
+    return fail(FA_ERR_UNSUPPORTED, "beam search needs every projection and the output head in the MMA layout");
+  return guarded([&]() -> int {
+    API_CUDA(cudaSetDevice(m.device));
+    fa_kv kvh;
+    int rc;
+    if ((rc = create_kv(m, b, n_prompt + cfg->max_new, cfg->kv_dtype, &kvh.kv))) return rc;
+    if (n_prompt > 1 && (rc = fa_prefill(fm, &kvh, 0, prompt, n_prompt - 1, 0, nullptr, nullptr))) return rc;
+    std::vector<uint32_t> parents, tokens;
+    std::vector<float> scores;
+    uint32_t steps = 0;
+    if ((rc = m.beam_search(kvh.kv, prompt[n_prompt - 1], *cfg, parents, tokens, scores, &steps))) return rc;
+    // hypotheses backwards along the parents; what a finished beam was fed after
+    // its eos is not part of it
+    std::vector<std::vector<uint32_t>> hyp(b);
+    std::vector<std::pair<double, uint32_t>> rank(b);
+    for (uint32_t r = 0; r < b; ++r) {
+      uint32_t at = r;
+      for (uint32_t s = steps; s-- > 0;) {
+        hyp[r].push_back(tokens[(size_t)s * b + at]);
+        at = parents[(size_t)s * b + at];
+      }
+      std::reverse(hyp[r].begin(), hyp[r].end());
+      const auto end = std::find(hyp[r].begin(), hyp[r].end(), cfg->eos);
+      if (end != hyp[r].end()) hyp[r].erase(end + 1, hyp[r].end());
+      rank[r] = {-(double)scores[r] / std::pow((double)hyp[r].size(), (double)cfg->length_penalty), r};
+    }
+    std::sort(rank.begin(), rank.end());
+    for (uint32_t i = 0; i < b; ++i) {
+      const uint32_t r = rank[i].second;
+      std::copy(hyp[r].begin(), hyp[r].end(), out_ids + (size_t)i * cfg->max_new);
+      if (out_len) out_len[i] = (uint32_t)hyp[r].size();
+      if (out_scores) out_scores[i] = scores[r];
+    }
+    return FA_OK;
+  });
+}

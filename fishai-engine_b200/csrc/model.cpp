@@ -1262,13 +1262,11 @@ int Model::ensure_batch_ws(uint32_t b) {
   return ensure_qg_part((uint64_t)8 * b * std::max(d, qkv_n));
 }
 
-int Model::enqueue_batch_step(const KvCache &kv, uint32_t b, const SamplerParams &sp, uint32_t *hist,
-                              uint32_t max_steps) {
+int Model::enqueue_batch_forward(const KvCache &kv, uint32_t b, const uint32_t *tok) {
   const uint32_t d = cfg.n_embd, hd = cfg.head_dim, Hq = cfg.n_heads, Hkv = cfg.n_kv_heads;
   const uint32_t F = layers[0].down.K, qkv_n = layers[0].qkv.n_out, gu_n = layers[0].gateup.n_out;
   const KvView kvv = kv.view();
   int rc;
-  uint32_t *tok = sp.ids;  // the sampler's ids are the next step's input tokens
   if (launch_embed_rows(emb, emb_type, tok, b, d, cfg.vocab_size, bws.X, bws.err, stream))
     return fail(FA_ERR_CUDA, "embed launch failed");
   for (uint32_t l = 0; l < cfg.n_layers; ++l) {
@@ -1312,7 +1310,14 @@ int Model::enqueue_batch_step(const KvCache &kv, uint32_t b, const SamplerParams
   }
   if (launch_norm_rows_h(bws.X, out_norm, cfg.norm_eps, b, d, bws.Xn, bws.err, stream))
     return fail(FA_ERR_CUDA, "norm launch failed");
-  if ((rc = run_qgemm(head, bws.mxn, b, bws.logits, cfg.vocab_size, kQgStore))) return rc;
+  return run_qgemm(head, bws.mxn, b, bws.logits, cfg.vocab_size, kQgStore);
+}
+
+int Model::enqueue_batch_step(const KvCache &kv, uint32_t b, const SamplerParams &sp, uint32_t *hist,
+                              uint32_t max_steps) {
+  uint32_t *tok = sp.ids;  // the sampler's ids are the next step's input tokens
+  int rc;
+  if ((rc = enqueue_batch_forward(kv, b, tok))) return rc;
   if (launch_sample(sp, b, stream)) return fail(FA_ERR_CUDA, "sampler launch failed");
   if (launch_batch_step_end(bws.states, b, tok, hist, max_steps, bws.step, stream))
     return fail(FA_ERR_CUDA, "step end launch failed");

@@ -153,7 +153,14 @@ struct Model {
   // batched decode (f16 tensor-core GEMMs at T = b)
   BatchWs bws;
   int ensure_batch_ws(uint32_t b);
+  // embedding to logits (bws.logits) of rows 0..b-1, which hold tokens tok (device)
+  int enqueue_batch_forward(const KvCache &kv, uint32_t b, const uint32_t *tok);
   int enqueue_batch_step(const KvCache &kv, uint32_t b, const SamplerParams &sp, uint32_t *hist, uint32_t max_steps);
+  // Beam search from sequence 0 of kv, which holds the prompt but its last
+  // token: cfg.n_beams beams for up to cfg.max_new steps.  Per step the chosen
+  // (parent, token) of every beam, the beams' final scores and lengths.
+  int beam_search(KvCache &kv, uint32_t last_token, const fa_beam_config &cfg, std::vector<uint32_t> &parents,
+                  std::vector<uint32_t> &tokens, std::vector<float> &scores, uint32_t *steps);
   // `steps` decode steps of sequences 0..b-1 of kv: row r starts from token
   // tok[r] at RoPE position pos[r] after its cached positions; every step
   // samples each row with sp (row r = sampler row r) and observes the id.

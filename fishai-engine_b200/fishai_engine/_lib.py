@@ -75,6 +75,11 @@ class fa_rope_config(C.Structure):
                 ("attn_factor", C.c_double)]
 
 
+class fa_beam_config(C.Structure):
+    _fields_ = [("n_beams", C.c_uint32), ("max_new", C.c_uint32), ("eos", C.c_uint32), ("length_penalty", C.c_float),
+                ("kv_dtype", C.c_int32)]
+
+
 # every entry point of include/fishai_cuda.h with its ctypes signature
 _vp, _sz, _i, _u32, _u64, _f = C.c_void_p, C.c_size_t, C.c_int, C.c_uint32, C.c_uint64, C.c_float
 _pu32, _pu64, _pf, _pi, _pi64 = C.POINTER(C.c_uint32), C.POINTER(C.c_uint64), C.POINTER(C.c_float), C.POINTER(C.c_int), C.POINTER(C.c_int64)
@@ -164,6 +169,7 @@ SIGNATURES = {
     "fa_pages_compact": ([_vp, _vp, _vp, _vp, _u32, _u32, _vp, _vp], _i),
     "fa_beam_select": ([_vp, C.c_int32, _u64, _u32, _u32, _u32, _vp, _vp, _u32, _u32, _u32, _vp, _vp, _vp, _vp, _vp,
                         _sz, _vp], _i),
+    "fa_generate_beams": ([_vp, C.POINTER(fa_beam_config), _pu32, _u32, _pu32, _pu32, _pf], _i),
     "fa_beam_select_ws": ([_u32, _u32, _u32, _u32], _sz),
     "fa_synth_write": ([C.c_char_p, C.POINTER(fa_synth_spec), _u64], _i),
 }

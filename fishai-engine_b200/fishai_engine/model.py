@@ -171,6 +171,19 @@ class ModelWeights:
                                         L.f32_ptr(lg) if want_logits else None))
         return (ids, lg) if want_logits else ids
 
+    def generate_beams(self, prompt_tokens, n_beams: int, max_new: int, eos: Optional[int] = None,
+                       length_penalty: float = 1.0, kv_dtype: int = L.KV_F16):
+        """Beam search (fa_generate_beams): [(ids, sum of log-probabilities)],
+        best score / length^length_penalty first; ids include the eos."""
+        p, pp = L.u32_array(prompt_tokens)
+        ids = np.zeros((n_beams, max_new), dtype=np.uint32)
+        n, sc = np.zeros(n_beams, dtype=np.uint32), np.zeros(n_beams, dtype=np.float32)
+        c = L.fa_beam_config(n_beams, max_new, L.NO_TOKEN if eos is None else eos, length_penalty, kv_dtype)
+        pu = C.POINTER(C.c_uint32)
+        L.check(L.lib().fa_generate_beams(self._h, C.byref(c), pp, p.size, ids.ctypes.data_as(pu), n.ctypes.data_as(pu),
+                                          L.f32_ptr(sc)))
+        return [(ids[i, : n[i]].tolist(), float(sc[i])) for i in range(n_beams)]
+
     def decode_greedy(self, kv_cache: KVCache, first_token: int, pos: int, steps: int, seq: int = 0):
         ids = np.zeros(steps, dtype=np.uint32)
         L.check(L.lib().fa_decode_greedy(self._h, kv_cache._h, seq, first_token, pos, steps,

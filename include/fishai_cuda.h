@@ -480,6 +480,23 @@ int fa_beam_select(const void *logits, int32_t dtype, uint64_t ld, uint32_t n_ba
                    void *stream);
 size_t fa_beam_select_ws(uint32_t n_batch, uint32_t n_beams, uint32_t vocab, uint32_t k);
 
+/* Beam search on a model (no counterpart in the reference, whose generation is
+ * greedy or sampled, src/model.rs:638-705): prefill, then steps of the batched
+ * decode with fa_beam_select on the device's logits and fa_kv_reorder between
+ * them; beams share the pages of their common past. */
+typedef struct {
+  uint32_t n_beams;        /* 1 .. 64 */
+  uint32_t max_new;        /* most tokens of a hypothesis */
+  uint32_t eos;            /* ends a hypothesis; FA_NO_TOKEN: none */
+  float length_penalty;    /* hypotheses rank by score / length^length_penalty */
+  int32_t kv_dtype;        /* FA_KV_F32 or FA_KV_F16 */
+} fa_beam_config;
+/* out_ids [n_beams][max_new]: the hypotheses, best first, eos included;
+ * out_len and out_scores [n_beams] (either may be NULL): their lengths and their
+ * sums of log-probabilities.  The model needs what fa_decode_batch needs. */
+int fa_generate_beams(fa_model *m, const fa_beam_config *cfg, const uint32_t *prompt_host, uint32_t n_prompt,
+                      uint32_t *out_ids, uint32_t *out_len, float *out_scores);
+
 /* ------------------------------------------------ token-parallel GEMM */
 /* Y[T][n_out] = X[T][K] . W for one weight group of the model (proj 0 qkv,
  * 1 o, 2 gate/up interleaved per 1024-column chunk, 3 down, 4 output head)
