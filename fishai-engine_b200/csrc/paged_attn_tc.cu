@@ -240,25 +240,37 @@ __device__ void softmax_role(const AttnChunksParams &p, TcWalk w, TcBars &b, uin
     const uint32_t row = s.r0 + 128 * g + tid;
     if (s.r0 + 128 * g >= s.r1) continue;  // the second Q tile is empty
     const bool live = row < s.r1, whole = TcWalk::whole(s);
-    const int32_t pos = live ? s.chunk.first + (int32_t)(row / p.rep) : -1;
+    const int32_t pos = s.chunk.first + (int32_t)(row / p.rep);
+    // a warp past the item's last row only hands its (unused) rows on; within a
+    // warp such rows ask for no masks
+    const bool idle = row - tid % 32 >= s.r1;
     const uint32_t tiles = s.hi > s.lo ? s.u1 - s.u0 : 0;
     float m = -INFINITY, l = 0.0f;
     for (uint32_t k = 0; k < tiles; ++k, ++n) {
       const uint32_t t0 = (s.lo / kTcPos + s.u0 + k) * kTcPos;
       if (!wait_bar(&b.abort, &b.s_full[g], n & 1)) return;
+      if (idle) {
+        mbar_arrive(&b.p_half[g]);
+        mbar_arrive(&b.p_full[g]);
+        continue;
+      }
       fence_after();
       float x[kTcPos];
 #pragma unroll
       for (uint32_t c = 0; c < 4; ++c) ld32(lanes + s_col(g) + 32 * c, x + 32 * c);
       wait_ld();
       // rows of a warp that see all 128 positions need no mask
-      const bool all = __all_sync(0xFFFFFFFFu, (int32_t)(t0 + kTcPos - 1) <= pos && (!p.window || (uint32_t)(pos - (int32_t)t0) < p.window));
-      if (!all) {
-        // visible columns: [from, to)
-        const int32_t to = pos - (int32_t)t0 + 1, from = p.window ? to - (int32_t)p.window : 0;
+      const int32_t to = pos - (int32_t)t0 + 1;  // visible columns: [to - window, to)
+      if (!__all_sync(0xFFFFFFFFu, !live || to >= (int32_t)kTcPos)) {
 #pragma unroll
         for (int32_t c = 0; c < (int32_t)kTcPos; ++c)
-          if (c >= to || c < from) x[c] = -INFINITY;
+          if (c >= to) x[c] = -INFINITY;
+      }
+      if (p.window && !__all_sync(0xFFFFFFFFu, !live || to <= (int32_t)p.window)) {
+        const int32_t from = to - (int32_t)p.window;
+#pragma unroll
+        for (int32_t c = 0; c < (int32_t)kTcPos; ++c)
+          if (c < from) x[c] = -INFINITY;
       }
       float mx[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
