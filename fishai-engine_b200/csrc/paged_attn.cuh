@@ -76,9 +76,10 @@ struct Segment {  // a piece of an item
 // A CTA's walk along its stretch.  Every thread holds the same state.
 template <uint32_t R, uint32_t U, uint32_t THREADS>
 struct Walk {
-  uint64_t at, end, per;  // units of the line
+  uint32_t left, per;     // units of the stretch that are left, and of a whole one (below 2^32: the line has
+                          // at most 2^31 rows / R items of 2^25 / U units for at least 100 CTAs)
   uint32_t c, tile, head;
-  uint64_t rem;           // units into the current item
+  uint32_t rem;           // units into the current item
   Chunk chunk;
 
   // All threads of the CTA; `red` is scratch of THREADS / 32 + 2 words.
@@ -97,13 +98,12 @@ struct Walk {
     uint64_t total = 0;
 #pragma unroll
     for (uint32_t w = 0; w < THREADS / 32; ++w) total += red[w];
-    per = (total + gridDim.x - 1) / gridDim.x;
+    per = (uint32_t)((total + gridDim.x - 1) / gridDim.x);
     if (per < min_units) per = min_units;
-    at = blockIdx.x * per;
-    end = min(total, at + per);
-    c = tile = head = 0;
-    rem = 0;
-    if (at >= end) return;  // the same for all threads of the CTA
+    const uint64_t at = (uint64_t)blockIdx.x * per;
+    c = tile = head = rem = left = 0;
+    if (at >= total) return;  // the same for all threads of the CTA
+    left = (uint32_t)min((uint64_t)per, total - at);
     // the chunk that holds `at`: blocks of THREADS chunks, then a scan
     uint64_t before = 0;
     uint64_t *found = red + THREADS / 32;  // [0] chunk, [1] units before it
@@ -141,24 +141,21 @@ struct Walk {
     }
     __syncthreads();
     c = (uint32_t)found[0];
-    rem = at - found[1];
     chunk = load_chunk(p, c);
-    skip(p);
-  }
-  // from (chunk, units into it) to (tile, head, units into the item)
-  __device__ void skip(const AttnChunksParams &p) {
-    for (;;) {
-      const uint64_t n = tile_units<R, U>(p, chunk, tile), all = n * p.pg.n_kv_heads;
-      if (rem < all) {
-        head = (uint32_t)(rem / n);
-        rem -= head * n;
+    // from the units into the chunk to (tile, head, units into the item)
+    uint64_t in = at - found[1];
+    for (;; ++tile) {
+      const uint32_t n = tile_units<R, U>(p, chunk, tile);
+      const uint64_t all = (uint64_t)n * p.pg.n_kv_heads;
+      if (in < all) {
+        head = (uint32_t)(in / n);
+        rem = (uint32_t)(in - (uint64_t)head * n);
         return;
       }
-      rem -= all;
-      ++tile;
+      in -= all;
     }
   }
-  __device__ bool done() const { return at >= end; }
+  __device__ bool done() const { return left == 0; }
   // the next piece; moves on behind it
   __device__ Segment next(const AttnChunksParams &p) {
     Segment s;
@@ -169,18 +166,18 @@ struct Walk {
     s.r1 = min(chunk.rows, s.r0 + R);
     tile_range(p, chunk, s.r0, s.r1, s.lo, s.hi);
     s.n = range_units<U>(s.lo, s.hi);
-    s.u0 = (uint32_t)rem;
-    const uint64_t take = min((uint64_t)(s.n - s.u0), end - at);
-    s.u1 = s.u0 + (uint32_t)take;
-    at += take;
+    s.u0 = rem;
+    const uint32_t take = min(s.n - s.u0, left);
+    s.u1 = s.u0 + take;
+    left -= take;
     rem = 0;
-    if (s.u1 == s.n && at < end) {  // the next item
+    if (s.u1 == s.n && left) {  // the next item
       if (++head == p.pg.n_kv_heads) {
         head = 0;
         if (++tile * R >= chunk.rows) {
           tile = 0;
           do chunk = load_chunk(p, ++c);
-          while (!chunk.rows);  // at < end <= total: a chunk with rows follows
+          while (!chunk.rows);  // units are left, so a chunk with rows follows
         }
       }
     }
@@ -188,10 +185,9 @@ struct Walk {
   }
   __device__ static bool whole(const Segment &s) { return s.u0 == 0 && s.u1 == s.n; }
   // What k_attn_join has to know of an item that this CTA begins and does not
-  // end (`at` is then the CTA's end): its rows, its head, and the CTAs on it.
+  // end: its rows, its head, and the CTAs on it.
   __device__ uint4 describe(const Segment &s) const {
-    const uint64_t left = s.n - s.u1;
-    return make_uint4(s.chunk.q0, s.r0, s.head | (s.r1 - s.r0) << 16, 1 + (uint32_t)((left + per - 1) / per));
+    return make_uint4(s.chunk.q0, s.r0, s.head | (s.r1 - s.r0) << 16, 1 + (s.n - s.u1 - 1) / per + 1);
   }
   // The slot of a piece that is not a whole item: slot 1 of the CTA that begins
   // the item, slot 0 of the others; R x hd outputs, then R x (max, sum)

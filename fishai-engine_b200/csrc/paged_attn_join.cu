@@ -85,22 +85,33 @@ __device__ __forceinline__ void join_tc(const AttnChunksParams &p, const float *
   const uint64_t slot = (uint64_t)kTcRows * (hd + 2);
   const float *first = part + ((uint64_t)cta * 2 + 1) * slot;
   float m = -INFINITY, l = 0.0f, acc[16] = {};
-  for (uint32_t i = 0; i < d.w; ++i) {
-    const float *q = i ? first + (2 * (uint64_t)i - 1) * slot : first;  // slot 1 of the CTA, then slot 0 of the next ones
-    const float2 ml = __ldcg(reinterpret_cast<const float2 *>(q + kTcRows * hd + 2 * r));
-    float4 x[4];
+  // four pieces' loads in flight (one at a time took 19 us for the 17 pieces of
+  // 128 rows over 8192 positions)
+  for (uint32_t i0 = 0; i0 < d.w; i0 += 4) {
+    float2 ml[4];
+    float4 x[4][4];
 #pragma unroll
-    for (uint32_t j = 0; j < 4; ++j) x[j] = __ldcg(reinterpret_cast<const float4 *>(q + tc_part(r, e0 + 4 * j, hd)));
-    const float mn = fmaxf(m, ml.x), ms = mn == -INFINITY ? 0.0f : mn, f = exp2f(m - ms), e = exp2f(ml.x - ms);
-    l = fmaf(l, f, ml.y * e);
+    for (uint32_t k = 0; k < 4; ++k) {
+      const uint32_t i = min(i0 + k, d.w - 1);
+      const float *q = i ? first + (2 * (uint64_t)i - 1) * slot : first;  // slot 1 of the CTA, then slot 0 of the next ones
+      ml[k] = __ldcg(reinterpret_cast<const float2 *>(q + kTcRows * hd + 2 * r));
 #pragma unroll
-    for (uint32_t j = 0; j < 4; ++j) {
-      acc[4 * j] = fmaf(acc[4 * j], f, x[j].x * e);
-      acc[4 * j + 1] = fmaf(acc[4 * j + 1], f, x[j].y * e);
-      acc[4 * j + 2] = fmaf(acc[4 * j + 2], f, x[j].z * e);
-      acc[4 * j + 3] = fmaf(acc[4 * j + 3], f, x[j].w * e);
+      for (uint32_t j = 0; j < 4; ++j) x[k][j] = __ldcg(reinterpret_cast<const float4 *>(q + tc_part(r, e0 + 4 * j, hd)));
     }
-    m = mn;
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k) {
+      if (i0 + k >= d.w) break;
+      const float mn = fmaxf(m, ml[k].x), ms = mn == -INFINITY ? 0.0f : mn, f = exp2f(m - ms), e = exp2f(ml[k].x - ms);
+      l = fmaf(l, f, ml[k].y * e);
+#pragma unroll
+      for (uint32_t j = 0; j < 4; ++j) {
+        acc[4 * j] = fmaf(acc[4 * j], f, x[k][j].x * e);
+        acc[4 * j + 1] = fmaf(acc[4 * j + 1], f, x[k][j].y * e);
+        acc[4 * j + 2] = fmaf(acc[4 * j + 2], f, x[k][j].z * e);
+        acc[4 * j + 3] = fmaf(acc[4 * j + 3], f, x[k][j].w * e);
+      }
+      m = mn;
+    }
   }
   const uint32_t row = d.y + r;
   T *out = reinterpret_cast<T *>(p.out) + (uint64_t)(d.x + row / p.rep) * p.os + (head * p.rep + row % p.rep) * hd + e0;
@@ -196,12 +207,12 @@ constexpr size_t kSmallSlots = (size_t)2 * kAttnMaxCtas * kAttnMaxRows, kTcSlots
 
 }  // namespace
 
-bool page_map(const AttnChunksParams &p, CUtensorMap *map) {
+bool page_map(const AttnChunksParams &p, uint32_t rows, CUtensorMap *map) {
   const PFN_cuTensorMapEncodeTiled_v12000 encode = encoder();
   if (!encode) return false;
   const uint32_t es = elem_size(p.pg.dtype);
   const cuuint64_t dims[2] = {p.pg.head_dim, (cuuint64_t)p.pg.n_pages * 2 * p.pg.n_kv_heads * kPageLen}, strides[1] = {(cuuint64_t)p.pg.head_dim * es};
-  const cuuint32_t box[2] = {64, kPageLen}, one[2] = {1, 1};
+  const cuuint32_t box[2] = {64, rows}, one[2] = {1, 1};
   void *base = static_cast<char *>(p.pg.base) + (uint64_t)p.layer * p.pg.layer_stride * es;
   return encode(map, p.pg.dtype == FA_KV_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, dims, strides, box,
                 one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,

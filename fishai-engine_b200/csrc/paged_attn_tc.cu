@@ -48,7 +48,7 @@ struct TcCfg {
   static_assert(kSmem <= 227 * 1024, "shared memory of a CTA");
 };
 struct TcBars {
-  uint64_t full[8], empty[8], q_full[2], q_empty[2], s_full[2], p_half[2], p_full[2], o_full[2], tail, done;
+  uint64_t full[8], empty[8], q_full[2], q_empty[2], s_full[2], p_half[2], p_full[2], o_full[2], done;
   uint64_t red[kTcThreads / 32 + 2];
   uint32_t tmem, abort;
 };
@@ -336,7 +336,7 @@ __device__ void softmax_role(const AttnChunksParams &p, TcWalk w, TcBars &b, uin
         ld32(lanes + o_col(g) + c, o);
         wait_ld();
       }
-      if (!tiles || l == 0.0f) {  // no position seen, or (within a split item) none yet
+      if (l == 0.0f) {  // nothing seen (yet, within a split item): zeros, whatever the product left
 #pragma unroll
         for (uint32_t e = 0; e < 32; ++e) o[e] = 0.0f;
       }
@@ -347,17 +347,19 @@ __device__ void softmax_role(const AttnChunksParams &p, TcWalk w, TcBars &b, uin
           *reinterpret_cast<float4 *>(slot + tc_part(r, c + e, HD)) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
         continue;
       }
-      uint32_t v[16];
 #pragma unroll
-      for (uint32_t e = 0; e < 16; ++e) v[e] = pack2<T>(o[2 * e] * inv, o[2 * e + 1] * inv);
-      if (reinterpret_cast<uintptr_t>(out) % 32 == 0) {
-        st8(out + c, reinterpret_cast<const uint32_t(&)[8]>(v[0]));
-        st8(out + c + 16, reinterpret_cast<const uint32_t(&)[8]>(v[8]));
-      } else {
+      for (uint32_t q = 0; q < 32; q += 16) {
+        uint32_t v[8];
 #pragma unroll
-        for (uint32_t e = 0; e < 16; ++e) {
-          reinterpret_cast<uint16_t *>(out)[c + 2 * e] = (uint16_t)v[e];
-          reinterpret_cast<uint16_t *>(out)[c + 2 * e + 1] = (uint16_t)(v[e] >> 16);
+        for (uint32_t e = 0; e < 8; ++e) v[e] = pack2<T>(o[q + 2 * e] * inv, o[q + 2 * e + 1] * inv);
+        if (reinterpret_cast<uintptr_t>(out) % 32 == 0) {
+          st8(out + c + q, v);
+        } else {
+#pragma unroll
+          for (uint32_t e = 0; e < 8; ++e) {
+            reinterpret_cast<uint16_t *>(out)[c + q + 2 * e] = (uint16_t)v[e];
+            reinterpret_cast<uint16_t *>(out)[c + q + 2 * e + 1] = (uint16_t)(v[e] >> 16);
+          }
         }
       }
     }
@@ -450,10 +452,11 @@ if (lead)
 
 // one warp
 template <typename T, uint32_t HD>
-__device__ void load_role(const AttnChunksParams &p, TcWalk w, TcBars &b, uint32_t smem, const CUtensorMap *map, uint32_t &fills) {
+__device__ void load_role(const AttnChunksParams &p, TcWalk w, TcBars &b, uint32_t smem, const CUtensorMap *map, const CUtensorMap *row_map,
+                          uint32_t &fills) {
   using C = TcCfg<HD>;
   const uint32_t lane = threadIdx.x & 31, ring = smem + 2 * C::kTile;
-  uint32_t seq = 0, tail = 0;
+  uint32_t st = 0, ph = 1;
   while (!w.done()) {
     const Segment s = w.next(p);
     const uint32_t tiles = s.hi > s.lo ? s.u1 - s.u0 : 0;
@@ -469,33 +472,31 @@ __device__ void load_role(const AttnChunksParams &p, TcWalk w, TcBars &b, uint32
       if (k + 1 < tiles) ahead = look_up(t0 + kTcPos);
       const bool used = t0 + (lane & 7) * kPageLen < s.hi && t0 + (lane & 7) * kPageLen + kPageLen > s.lo;
       if (used && page >= p.pg.n_pages && p.err) atomicOr(p.err, kFlagPage);
-      // slots of a page that nobody sees: V must not be NaN there (its weight 0
-      // would not help)
-      const bool ragged = (s.hi < t0 + kTcPos && s.hi % kPageLen) || (s.lo > t0 && s.lo % kPageLen);
-      for (uint32_t is_v = 0; is_v < 2; ++is_v, ++seq) {
-        const uint32_t st = seq % C::kStages, dst = ring + st * C::kTile;
-        if (!wait_bar(&b.abort, &b.empty[st], (seq / C::kStages & 1) ^ 1)) return;
-        uint64_t *bar = is_v && ragged ? &b.tail : &b.full[st];
-        if (lane == 0) mbar_arrive_expect_tx(bar, C::kTile);
+      // A page with slots that nobody sees: V must not be NaN there (its weight 0
+      // would not help), so its rows come one by one, the unseen ones from past
+      // the end of the tensor, as zeros.
+      const uint32_t at = t0 + (lane & 7) * kPageLen;
+      const bool part = used && (at < s.lo || at + kPageLen > s.hi);
+      const uint32_t parts = __ballot_sync(0xFFFFFFFFu, part && lane < 8);
+      for (uint32_t is_v = 0; is_v < 2; ++is_v) {
+        const uint32_t dst = ring + st * C::kTile;
+        if (!wait_bar(&b.abort, &b.empty[st], ph)) return;
+        if (lane == 0) mbar_arrive_expect_tx(&b.full[st], C::kTile);
         __syncwarp();
-        if (lane < 8 * (HD / 64)) {
-          tma_2d(dst + (lane >> 3) * C::kHalf + (lane & 7) * 2048, map, (int32_t)(lane >> 3) * 64, map_row(p.pg, page, is_v, s.head), bar);
-        }
-        if (is_v && ragged) {
-          if (!mbar_wait(&b.tail, tail & 1)) {
-            *reinterpret_cast<volatile uint32_t *>(&b.abort) = 1;
-            return;
+        if (lane < 8 * (HD / 64) && !(is_v && part))
+          tma_2d(dst + (lane >> 3) * C::kHalf + (lane & 7) * 2048, map, (int32_t)(lane >> 3) * 64, map_row(p.pg, page, is_v, s.head), &b.full[st]);
+        if (is_v)
+          for (uint32_t m = parts; m; m &= m - 1) {
+            const uint32_t j = __ffs(m) - 1, pg = __shfl_sync(0xFFFFFFFFu, page, j), t = t0 + j * kPageLen + (lane & 15), half = lane >> 4;
+            const bool seen = t >= s.lo && t < s.hi;
+            if (half < HD / 64)
+              tma_2d(dst + half * C::kHalf + j * 2048 + (lane & 15) * 128, row_map, (int32_t)half * 64,
+                     map_row(p.pg, seen ? pg : 0xFFFFFFFFu, 1, s.head) + (int32_t)(seen && pg < p.pg.n_pages ? lane & 15 : 0), &b.full[st]);
           }
-          ++tail;
-          for (uint32_t r = lane; r < kTcPos; r += 32)
-            if (t0 + r < s.lo || t0 + r >= s.hi)
-              for (uint32_t c = 0; c < HD / 8; ++c)
-                asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(dst + (c >> 3) * C::kHalf + r * 128 + (c & 7) * 16), "r"(0u) : "memory");
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&b.full[st]);
-        } else {
-          fills = seq + 1;
+        ++fills;
+        if (++st == C::kStages) {
+          st = 0;
+          ph ^= 1;
         }
       }
     }
@@ -503,7 +504,8 @@ __device__ void load_role(const AttnChunksParams &p, TcWalk w, TcBars &b, uint32
 }
 
 template <typename T, uint32_t HD>
-__global__ void __launch_bounds__(kTcThreads, 1) k_attn_tc(const AttnChunksParams p, const __grid_constant__ CUtensorMap map) {
+__global__ void __launch_bounds__(kTcThreads, 1) k_attn_tc(const AttnChunksParams p, const __grid_constant__ CUtensorMap map,
+                                                            const __grid_constant__ CUtensorMap row_map) {
   using C = TcCfg<HD>;
   extern __shared__ __align__(1024) uint8_t raw[];
   const uint32_t pad = (1024u - (smem_u32(raw) & 1023u)) & 1023u, smem = smem_u32(raw) + pad;
@@ -525,7 +527,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_tc(const AttnChunksParam
       mbar_init(&b.p_full[i], 128);
       mbar_init(&b.o_full[i], 1);
     }
-    mbar_init(&b.tail, 1);
     mbar_init(&b.done, 1);
     b.abort = 0;
     fence_mbar_init();
@@ -540,12 +541,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_tc(const AttnChunksParam
     __syncthreads();
     fence_after();
     const uint32_t tmem = b.tmem;
-    // 384 x 168 registers at launch: 256 x 216 + 128 x 72
+    // 384 x 168 registers at launch: 256 x 224 + 128 x 56
     if (warp < 8) {
-      asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
       softmax_role<T, HD>(p, w, b, tmem, warp >> 2);
     } else {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
       if (warp == 8) {
         mma_role<T, HD>(p, w, b, smem, tmem);
         if (lane == 0) commit(&b.done);
@@ -553,7 +554,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_tc(const AttnChunksParam
         mbar_wait(&b.done, 0);  // nothing is on its way to tensor memory after this
       } else if (warp == 9) {
         uint32_t fills = 0;
-        load_role<T, HD>(p, w, b, smem, &map, fills);
+        load_role<T, HD>(p, w, b, smem, &map, &row_map, fills);
         if (*reinterpret_cast<volatile uint32_t *>(&b.abort))  // copies that nobody waited for
           for (uint32_t i = fills > C::kStages ? fills - C::kStages : 0; i < fills; ++i)
             mbar_wait(&b.full[i % C::kStages], i / C::kStages & 1);
@@ -575,10 +576,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_tc(const AttnChunksParam
 
 template <typename T, uint32_t HD>
 int launch_hd(const AttnChunksParams &p, uint32_t ctas, cudaStream_t st) {
-  CUtensorMap map;
-  if (!page_map(p, &map)) return -1;
+  CUtensorMap map, row_map;
+  if (!page_map(p, kPageLen, &map) || !page_map(p, 1, &row_map)) return -1;
   if (cudaFuncSetAttribute(k_attn_tc<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)TcCfg<HD>::kSmem) != cudaSuccess) return -1;
-  return launch_pdl(k_attn_tc<T, HD>, dim3(ctas), dim3(kTcThreads), TcCfg<HD>::kSmem, st, p, map);
+  return launch_pdl(k_attn_tc<T, HD>, dim3(ctas), dim3(kTcThreads), TcCfg<HD>::kSmem, st, p, map, row_map);
 }
 
 }  // namespace

@@ -31,8 +31,8 @@ __device__ __forceinline__ bool wait_bar(uint32_t *abort, uint64_t *bar, uint32_
 }
 
 // The layer's pages as rows of a head: [page][k | v][kv head][16] x head_dim,
-// boxes of 16 rows x 64 elements, 128-byte swizzle.  False: the driver refused.
-bool page_map(const AttnChunksParams &p, CUtensorMap *map);
+// boxes of `rows` rows x 64 elements, 128-byte swizzle.  False: the driver refused.
+bool page_map(const AttnChunksParams &p, uint32_t rows, CUtensorMap *map);
 // row of (page, k | v, head); a row past the end (zeros) for a bad or unused page
 __device__ __forceinline__ int32_t map_row(const fa_pages &pg, uint32_t page, uint32_t is_v, uint32_t head) {
   return (int32_t)((page < pg.n_pages ? (page * 2 + is_v) * pg.n_kv_heads + head : pg.n_pages * 2 * pg.n_kv_heads) * kPageLen);
