@@ -3,9 +3,8 @@
 // An item is (chunk, row tile, kv head): R rows of one kv head, row r of a
 // chunk being query token r / rep and query head kvh * rep + r % rep, so the
 // rows of an item read the same K and V.  It covers the positions that any of
-// its rows sees, in units of U positions.  The units of all items, in chunk,
-// row tile, head order, are one line, and each CTA takes an equal stretch of
-// it: chunks of any lengths then load the GPU evenly, and a single long cache
+// its rows sees, in units of U positions.  The items' costs, in chunk, row tile,
+// head order, are one line, and each CTA takes an equal stretch of it: chunks of any lengths then load the GPU evenly, and a single long cache
 // is spread over all of it.  A CTA finishes the items that lie inside its
 // stretch; the ends of a stretch leave (max, sum, unnormalised output) in the
 // CTA's two slots, and k_attn_join adds the pieces in the order of the
@@ -52,17 +51,36 @@ template <uint32_t U>
 __device__ __forceinline__ uint32_t range_units(uint32_t lo, uint32_t hi) {
   return hi > lo ? (hi - 1) / U - lo / U + 1 : 1;  // at least one: somebody writes the zeros
 }
-template <uint32_t R, uint32_t U>
-__device__ __forceinline__ uint32_t tile_units(const AttnChunksParams &p, const Chunk &k, uint32_t tile) {
+// Cost of a row tile on the line: its units, and OVER for what an item costs
+// apart from them (Q, filling the pipeline, the output), so that many short
+// items do not make a CTA late.
+template <uint32_t R, uint32_t U, uint32_t OVER>
+__device__ __forceinline__ uint32_t tile_cost(const AttnChunksParams &p, const Chunk &k, uint32_t tile) {
   uint32_t lo, hi;
   tile_range(p, k, tile * R, min(k.rows, tile * R + R), lo, hi);
-  return range_units<U>(lo, hi);
+  return range_units<U>(lo, hi) + OVER;
 }
-template <uint32_t R, uint32_t U>
-__device__ __forceinline__ uint64_t chunk_units(const AttnChunksParams &p, const Chunk &k) {
-  uint64_t n = 0;
-  for (uint32_t t = 0; t * R < k.rows; ++t) n += tile_units<R, U>(p, k, t);
-  return n * p.pg.n_kv_heads;
+// Cost of the lane's chunk, its row tiles times the heads; long chunks by the
+// whole warp (a thread to itself took 6 us for the 16 tiles of 1024 tokens)
+template <uint32_t R, uint32_t U, uint32_t OVER>
+__device__ __forceinline__ uint64_t chunk_cost(const AttnChunksParams &p, const Chunk &k) {
+  const uint32_t lane = threadIdx.x & 31;
+  uint64_t mine = 0;
+  const bool small = k.rows <= 2 * R;
+  if (small)
+    for (uint32_t t = 0; t * R < k.rows; ++t) mine += tile_cost<R, U, OVER>(p, k, t);
+  for (uint32_t big = __ballot_sync(0xFFFFFFFFu, !small); big; big &= big - 1) {
+    const uint32_t who = __ffs(big) - 1;
+    Chunk c;
+    c.rows = __shfl_sync(0xFFFFFFFFu, k.rows, who);
+    c.first = __shfl_sync(0xFFFFFFFFu, k.first, who);
+    uint64_t sum = 0;
+    for (uint32_t t = lane; (uint64_t)t * R < c.rows; t += 32) sum += tile_cost<R, U, OVER>(p, c, t);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+    if (lane == who) mine = sum;
+  }
+  return mine * p.pg.n_kv_heads;
 }
 
 struct Segment {  // a piece of an item
@@ -74,22 +92,25 @@ struct Segment {  // a piece of an item
 };
 
 // A CTA's walk along its stretch.  Every thread holds the same state.
-template <uint32_t R, uint32_t U, uint32_t THREADS>
+template <uint32_t R, uint32_t U, uint32_t OVER, uint32_t THREADS>
 struct Walk {
-  uint32_t left, per;     // units of the stretch that are left, and of a whole one (below 2^32: the line has
-                          // at most 2^31 rows / R items of 2^25 / U units for at least 100 CTAs)
+  uint32_t left, per;     // cost of the stretch that is left, and of a whole one (below 2^32: the line has at most
+                          // 2^31 rows / R items of 2^25 / U units for at least 100 CTAs)
   uint32_t c, tile, head;
-  uint32_t rem;           // units into the current item
+  uint32_t rem;           // cost into the current item; its first OVER stand for no work
   Chunk chunk;
 
   // All threads of the CTA; `red` is scratch of THREADS / 32 + 2 words.
-  __device__ void start(const AttnChunksParams &p, uint32_t min_units, uint64_t *red) {
+  __device__ void start(const AttnChunksParams &p, uint32_t min_cost, uint64_t *red) {
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    auto cost = [&](uint32_t i) -> uint64_t {  // of chunk i, whole warps
+      Chunk k;
+      k.rows = 0;
+      if (i < p.n_chunks) k = load_chunk(p, i);
+      return chunk_cost<R, U, OVER>(p, k);
+    };
     uint64_t sum = 0;
-    for (uint32_t i = tid; i < p.n_chunks; i += THREADS) {
-      const Chunk k = load_chunk(p, i);
-      sum += chunk_units<R, U>(p, k);
-    }
+    for (uint32_t b = 0; b < p.n_chunks; b += THREADS) sum += cost(b + tid);
     const uint64_t own = sum;  // of chunk tid, where a thread has one at most
 #pragma unroll
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
@@ -99,23 +120,17 @@ struct Walk {
 #pragma unroll
     for (uint32_t w = 0; w < THREADS / 32; ++w) total += red[w];
     per = (uint32_t)((total + gridDim.x - 1) / gridDim.x);
-    if (per < min_units) per = min_units;
+    if (per < min_cost) per = min_cost;
     const uint64_t at = (uint64_t)blockIdx.x * per;
     c = tile = head = rem = left = 0;
     if (at >= total) return;  // the same for all threads of the CTA
     left = (uint32_t)min((uint64_t)per, total - at);
     // the chunk that holds `at`: blocks of THREADS chunks, then a scan
     uint64_t before = 0;
-    uint64_t *found = red + THREADS / 32;  // [0] chunk, [1] units before it
+    uint64_t *found = red + THREADS / 32;  // [0] chunk, [1] cost before it
     for (uint32_t b = 0;; b += THREADS) {
       const uint32_t i = b + tid;
-      uint64_t mine = 0;
-      if (p.n_chunks <= THREADS) {
-        mine = own;
-      } else if (i < p.n_chunks) {
-        const Chunk k = load_chunk(p, i);
-        mine = chunk_units<R, U>(p, k);
-      }
+      const uint64_t mine = p.n_chunks <= THREADS ? own : cost(i);
       uint64_t inc = mine;  // inclusive scan of the block
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -142,46 +157,59 @@ struct Walk {
     __syncthreads();
     c = (uint32_t)found[0];
     chunk = load_chunk(p, c);
-    // from the units into the chunk to (tile, head, units into the item)
+    // from the cost into the chunk to (tile, head, cost into the item), 32 tiles
+    // at a time
     uint64_t in = at - found[1];
-    for (;; ++tile) {
-      const uint32_t n = tile_units<R, U>(p, chunk, tile);
-      const uint64_t all = (uint64_t)n * p.pg.n_kv_heads;
-      if (in < all) {
-        head = (uint32_t)(in / n);
-        rem = (uint32_t)(in - (uint64_t)head * n);
+    for (uint32_t t0 = 0;; t0 += 32) {
+      const uint32_t t = t0 + lane, n = (uint64_t)t * R < chunk.rows ? tile_cost<R, U, OVER>(p, chunk, t) : 0;
+      uint64_t inc = (uint64_t)n * p.pg.n_kv_heads;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint64_t x = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+        if (lane >= (uint32_t)o) inc += x;
+      }
+      const uint32_t behind = __ballot_sync(0xFFFFFFFFu, inc > in);
+      if (behind) {
+        const uint32_t l = __ffs(behind) - 1;
+        const uint32_t one = __shfl_sync(0xFFFFFFFFu, n, l);
+        in -= __shfl_sync(0xFFFFFFFFu, inc, l) - (uint64_t)one * p.pg.n_kv_heads;
+        tile = t0 + l;
+        head = (uint32_t)(in / one);
+        rem = (uint32_t)(in - (uint64_t)head * one);
         return;
       }
-      in -= all;
+      in -= __shfl_sync(0xFFFFFFFFu, inc, 31);
     }
   }
   __device__ bool done() const { return left == 0; }
-  // the next piece; moves on behind it
-  __device__ Segment next(const AttnChunksParams &p) {
-    Segment s;
-    s.chunk = chunk;
-    s.tile = tile;
-    s.head = head;
-    s.r0 = tile * R;
-    s.r1 = min(chunk.rows, s.r0 + R);
-    tile_range(p, chunk, s.r0, s.r1, s.lo, s.hi);
-    s.n = range_units<U>(s.lo, s.hi);
-    s.u0 = rem;
-    const uint32_t take = min(s.n - s.u0, left);
-    s.u1 = s.u0 + take;
-    left -= take;
-    rem = 0;
-    if (s.u1 == s.n && left) {  // the next item
-      if (++head == p.pg.n_kv_heads) {
-        head = 0;
-        if (++tile * R >= chunk.rows) {
-          tile = 0;
-          do chunk = load_chunk(p, ++c);
-          while (!chunk.rows);  // units are left, so a chunk with rows follows
+  // the next piece with work in it; false: there is none left
+  __device__ bool next(const AttnChunksParams &p, Segment &s) {
+    while (left) {
+      s.chunk = chunk;
+      s.tile = tile;
+      s.head = head;
+      s.r0 = tile * R;
+      s.r1 = min(chunk.rows, s.r0 + R);
+      tile_range(p, chunk, s.r0, s.r1, s.lo, s.hi);
+      s.n = range_units<U>(s.lo, s.hi);
+      const uint32_t take = min(s.n + OVER - rem, left), end = rem + take;
+      s.u0 = rem > OVER ? rem - OVER : 0;
+      s.u1 = end > OVER ? end - OVER : 0;
+      left -= take;
+      rem = 0;
+      if (end == s.n + OVER && left) {  // the next item
+        if (++head == p.pg.n_kv_heads) {
+          head = 0;
+          if (++tile * R >= chunk.rows) {
+            tile = 0;
+            do chunk = load_chunk(p, ++c);
+            while (!chunk.rows);  // some cost is left, so a chunk with rows follows
+          }
         }
       }
+      if (s.u1 > s.u0) return true;
     }
-    return s;
+    return false;
   }
   __device__ static bool whole(const Segment &s) { return s.u0 == 0 && s.u1 == s.n; }
   // What k_attn_join has to know of an item that this CTA begins and does not

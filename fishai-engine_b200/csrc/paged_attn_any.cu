@@ -104,12 +104,11 @@ __global__ void __launch_bounds__(kAnyThreads) k_attn_any(const AttnChunksParams
   float *sq = sm, *sk = sq + R * ld, *sv = sk + kAnyPos * ld, *sp = sv + kAnyPos * ld;
   const uint32_t tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
   const T *base = reinterpret_cast<const T *>(p.pg.base) + (uint64_t)p.layer * p.pg.layer_stride;
-  using W = Walk<R, kAnyPos, kAnyThreads>;
+  using W = Walk<R, kAnyPos, 0, kAnyThreads>;
   W w;
   w.start(p, 1, red);
   if (tid == 0) p.desc[blockIdx.x].w = 0;
-  while (!w.done()) {
-    const Segment s = w.next(p);
+  for (Segment s; w.next(p, s);) {
     const uint32_t *pt = p.pg.page_table + (uint64_t)s.chunk.seq * p.pg.max_pages;
     __syncthreads();
     // Q rows; past the item's: zeros

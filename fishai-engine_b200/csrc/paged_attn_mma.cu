@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(kThreads, 3) k_attn_rows16(const AttnChunksPar
   extern __shared__ __align__(128) uint8_t dsm[];
   __shared__ uint64_t red[kThreads / 32 + 2];
   constexpr uint32_t kTileBytes = kSub * HD * 2;
-  using W = Walk<16, kSub, kThreads>;
+  using W = Walk<16, kSub, 2, kThreads>;
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   const uint32_t ktile = smem_u32(dsm) + warp * 2 * kTileBytes, vtile = ktile + kTileBytes;
   const T *base = reinterpret_cast<const T *>(p.pg.base) + (uint64_t)p.layer * p.pg.layer_stride;
@@ -259,8 +259,7 @@ __global__ void __launch_bounds__(kThreads, 3) k_attn_rows16(const AttnChunksPar
   W w;
   w.start(p, 4, red);
   if (tid == 0) p.desc[blockIdx.x].w = 0;
-  while (!w.done()) {
-    const Segment s = w.next(p);
+  for (Segment s; w.next(p, s);) {
     const uint32_t *pt = p.pg.page_table + (uint64_t)s.chunk.seq * p.pg.max_pages;
     Rows<T, HD> rows;
     rows.load(p, s, s.r0);
@@ -365,7 +364,7 @@ __global__ void __launch_bounds__(kThreads, 3) k_attn_rows64(const AttnChunksPar
   extern __shared__ __align__(128) uint8_t dsm[];
   __shared__ uint64_t red[kThreads / 32 + 2];
   constexpr uint32_t kPos = 2 * kSub, kTileBytes = kSub * HD * 2;  // a stage: K, K, V, V sub-tiles
-  using W = Walk<64, kPos, kThreads>;
+  using W = Walk<64, kPos, 1, kThreads>;
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   const uint32_t smem = smem_u32(dsm);
   const T *base = reinterpret_cast<const T *>(p.pg.base) + (uint64_t)p.layer * p.pg.layer_stride;
@@ -373,8 +372,7 @@ __global__ void __launch_bounds__(kThreads, 3) k_attn_rows64(const AttnChunksPar
   W w;
   w.start(p, 2, red);
   if (tid == 0) p.desc[blockIdx.x].w = 0;
-  while (!w.done()) {
-    const Segment s = w.next(p);
+  for (Segment s; w.next(p, s);) {
     const uint32_t *pt = p.pg.page_table + (uint64_t)s.chunk.seq * p.pg.max_pages;
     const uint32_t row0 = s.r0 + 16 * warp;
     const bool live = row0 < s.r1;
