@@ -233,16 +233,17 @@ struct JoinSet {
 // The kernels; each returns its grid, or 0 where the launch failed.
 bool attn_mma_takes(const AttnChunksParams &p);
 uint32_t launch_attn_any(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st, uint32_t *R);
-uint32_t launch_attn_mma(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st, uint32_t *R);
-uint32_t launch_attn_tc(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st);
+uint32_t launch_attn_mma(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st);  // items of kMmaRows
+// overlap: the launch before is launch_attn_mma's, with which this one may run at the same time
+uint32_t launch_attn_tc(const AttnChunksParams &p, uint32_t n_sm, bool overlap, cudaStream_t st, uint32_t *R);
 
-// Most CTAs and rows of an item of the launch for few rows, and of the launch
-// for many: what the workspace holds two slots of each for.
-constexpr uint32_t kAttnMaxCtas = 480, kAttnMaxRows = 64;
-constexpr uint32_t kTcMaxCtas = 160, kTcRows = 256;
+// Most CTAs and rows of an item of the launch for few rows (or of the f32 one),
+// and of the launch for many: what the workspace holds two slots of each for.
+constexpr uint32_t kAttnMaxCtas = 480, kAttnMaxRows = 32, kMmaRows = 16;
+constexpr uint32_t kTcMaxCtas = 160, kTcRows = 256;  // or twice as many CTAs of 128 rows
 // Where element d (a multiple of 4, and the three behind it) of row r is in a
 // slot of the launch for many rows, whose threads have a row each; after the
-// kTcRows x hd outputs come the pairs (max, sum).
+// R x hd outputs come the pairs (max, sum).
 __host__ __device__ constexpr uint32_t tc_part(uint32_t r, uint32_t d, uint32_t hd) {
   return ((r / 32) * (hd / 4) + d / 4) * 128 + (r % 32) * 4;
 }

@@ -77,12 +77,12 @@ __device__ __forceinline__ void add4(Sum<kPer> &s, P piece, uint32_t i0, uint32_
 // An item of the launch for many rows: a thread has 16 elements of a row, as
 // they lie in the slots (tc_part), and writes them as 32 bytes.
 template <typename T>
-__device__ __forceinline__ void join_tc(const AttnChunksParams &p, const float *part, const uint4 &d, uint32_t cta, uint32_t at) {
+__device__ __forceinline__ void join_tc(const AttnChunksParams &p, const float *part, const uint4 &d, uint32_t cta, uint32_t at, uint32_t R) {
   const uint32_t hd = p.pg.head_dim, head = d.z & 0xFFFF, rows = d.z >> 16;
   const uint32_t block = at * kJoinWarps + threadIdx.x / 32;  // (32 rows, 16 elements)
   const uint32_t r = block / (hd / 16) * 32 + threadIdx.x % 32, e0 = block % (hd / 16) * 16;
   if (r >= rows) return;
-  const uint64_t slot = (uint64_t)kTcRows * (hd + 2);
+  const uint64_t slot = (uint64_t)R * (hd + 2);
   const float *first = part + ((uint64_t)cta * 2 + 1) * slot;
   float m = -INFINITY, l = 0.0f, acc[16] = {};
   // four pieces' loads in flight (one at a time took 19 us for the 17 pieces of
@@ -94,7 +94,7 @@ __device__ __forceinline__ void join_tc(const AttnChunksParams &p, const float *
     for (uint32_t k = 0; k < 4; ++k) {
       const uint32_t i = min(i0 + k, d.w - 1);
       const float *q = i ? first + (2 * (uint64_t)i - 1) * slot : first;  // slot 1 of the CTA, then slot 0 of the next ones
-      ml[k] = __ldcg(reinterpret_cast<const float2 *>(q + kTcRows * hd + 2 * r));
+      ml[k] = __ldcg(reinterpret_cast<const float2 *>(q + R * hd + 2 * r));
 #pragma unroll
       for (uint32_t j = 0; j < 4; ++j) x[k][j] = __ldcg(reinterpret_cast<const float4 *>(q + tc_part(r, e0 + 4 * j, hd)));
     }
@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) k_attn_join(const AttnChunksP
   if (!d.w) return;
   if constexpr (sizeof(T) == 2 && kPer == 4) {
     if (second) {
-      join_tc<T>(p, b.part, d, cta, y);
+      join_tc<T>(p, b.part, d, cta, y, b.R);
       return;
     }
   }
@@ -221,7 +221,7 @@ bool page_map(const AttnChunksParams &p, uint32_t rows, CUtensorMap *map) {
 
 // slots of the launch for few rows, of the one for many, descriptors
 size_t attn_chunks_ws(uint32_t head_dim) {
-  return (kSmallSlots + kTcSlots) * (head_dim + 2) * 4 + (kAttnMaxCtas + kTcMaxCtas) * sizeof(uint4);
+  return (kSmallSlots + kTcSlots) * (head_dim + 2) * 4 + (kAttnMaxCtas + 2 * kTcMaxCtas) * sizeof(uint4);
 }
 
 int launch_attn_chunks(const AttnChunksParams &p, void *ws, uint32_t n_sm, cudaStream_t st) {
@@ -232,17 +232,27 @@ int launch_attn_chunks(const AttnChunksParams &p, void *ws, uint32_t n_sm, cudaS
   b.desc = a.desc + kAttnMaxCtas;
   a.rows_min = 1;
   a.rows_max = 0xFFFFFFFFu;
-  JoinSet ja{a.part, a.desc, 0, 0, 0}, jb{b.part, b.desc, kTcRows, 0, kTcRows / 32 * (p.pg.head_dim / 16) / kJoinWarps};
+  JoinSet ja{a.part, a.desc, 0, 0, 0}, jb{b.part, b.desc, 0, 0, 0};
   if (attn_mma_takes(p)) {
-    // chunks of up to 64 rows are bound by the copies of K and V, which mma.sync
-    // keeps up with; above, the 256-row items of tcgen05
-    const bool many = (uint64_t)p.max_q * p.rep > kAttnMaxRows;
-    if (many) a.rows_max = kAttnMaxRows;
-    if (!(ja.ctas = launch_attn_mma(a, n_sm, st, &ja.R))) return -1;
+    // Up to 16 rows mma.sync keeps up with the copies of K and V; above, the
+    // items of tcgen05, also where they are mostly empty: 64 sequences of 4096
+    // positions with 32 and 64 rows take 200 and 208 us, and took 264 and 316
+    // with mma.sync and a warp for each 16 rows (which was the faster one over
+    // short caches: 300 of 300 positions with 20 rows 129 us against 139).
+    // Chunks of both kinds: both kernels, each leaving out the other's.  Where
+    // all chunks are as long as the longest the second kernel takes them alone,
+    // whatever their rows.
+    const bool many = (uint64_t)p.max_q * p.rep > kMmaRows, alike = p.n_tokens == (uint64_t)p.n_chunks * p.max_q;
+    if (many) a.rows_max = kMmaRows;
+    if (!many || !alike) {
+      ja.R = kMmaRows;
+      if (!(ja.ctas = launch_attn_mma(a, n_sm, st))) return -1;
+    }
     if (many) {
-      b.rows_min = kAttnMaxRows + 1;
+      b.rows_min = alike ? 1 : kMmaRows + 1;
       b.rows_max = 0xFFFFFFFFu;
-      if (!(jb.ctas = launch_attn_tc(b, n_sm, st))) return -1;
+      if (!(jb.ctas = launch_attn_tc(b, n_sm, !alike, st, &jb.R))) return -1;
+      jb.parts = jb.R / 32 * (p.pg.head_dim / 16) / kJoinWarps;  // a thread 16 elements of a row
     }
   } else if (!(ja.ctas = launch_attn_any(a, n_sm, st, &ja.R))) {
     return -1;

@@ -1,22 +1,22 @@
-// Attention of chunks over paged f16 / bf16 K/V with few rows per kv head:
-// single tokens and short chunks, head sizes 64 and 128.  Same mathematics as
+// Attention of chunks over paged f16 / bf16 K/V with up to 16 rows per kv head:
+// single tokens and a few at a time, head sizes 64 and 128.  Same mathematics as
 // paged_attn_any.cu, products on mma.sync m16n8k16 with f32 accumulators.  The
 // weights p = 2^(s - m) <= 1 are rounded to the cache's type for the product
 // with V (the type V itself was rounded to); their sum is taken before that
 // rounding, in f32.
 //
-// HBM bounds it: every K and V row is used for at most 64 rows of Q, far below
+// HBM bounds it: every K and V row is used for at most 16 rows of Q, far below
 // the 250 operations a byte where tensor cores would bind, so all that counts
 // is copies in flight.  Sub-tiles of 32 positions (two pages) go to shared
 // memory by cp.async in 16-byte pieces, XOR-swizzled by row so that ldmatrix
 // reads eight rows from distinct banks; rows nobody sees are filled with
-// zeros, so stale or NaN slots do not reach a product.
-//   up to 16 rows (k_attn_rows16): each warp runs through its own sub-tiles
-//     and keeps its own (max, sum, output); the four are merged at the end of
-//     a piece.  The next K is fetched as soon as the scores are formed, the
-//     next V after its product, so both buffers are nearly always in flight.
-//   up to 64 rows (k_attn_rows64): a warp has 16 of the rows, and all warps
-//     share tiles of 64 positions, the next one in flight.
+// zeros, so stale or NaN slots do not reach a product.  Each warp runs through
+// its own sub-tiles and keeps its own (max, sum, output); the four of a CTA are
+// merged at the end of a piece.  The next K is fetched as soon as the scores are
+// formed, the next V after its product, so both buffers are nearly always in
+// flight; three CTAs an SM.  64 sequences of 4096 positions, 32/8 heads x 128:
+// 178 us, 6.0 TB/s; of 37 to 4096 positions: 95 us, 5.6 TB/s.  (One CTA an SM
+// whose ring of copies a TMA warp keeps filled across items: 225 and 138 us.)
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(kThreads, 3) k_attn_rows16(const AttnChunksPar
   extern __shared__ __align__(128) uint8_t dsm[];
   __shared__ uint64_t red[kThreads / 32 + 2];
   constexpr uint32_t kTileBytes = kSub * HD * 2;
-  using W = Walk<16, kSub, 2, kThreads>;
+  using W = Walk<kMmaRows, kSub, 6, kThreads>;
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   const uint32_t ktile = smem_u32(dsm) + warp * 2 * kTileBytes, vtile = ktile + kTileBytes;
   const T *base = reinterpret_cast<const T *>(p.pg.base) + (uint64_t)p.layer * p.pg.layer_stride;
@@ -358,102 +358,13 @@ __global__ void __launch_bounds__(kThreads, 3) k_attn_rows16(const AttnChunksPar
   }
 }
 
-// ------------------------------------------------------------ up to 64 rows
 template <typename T, uint32_t HD>
-__global__ void __launch_bounds__(kThreads, 3) k_attn_rows64(const AttnChunksParams p) {
-  extern __shared__ __align__(128) uint8_t dsm[];
-  __shared__ uint64_t red[kThreads / 32 + 2];
-  constexpr uint32_t kPos = 2 * kSub, kTileBytes = kSub * HD * 2;  // a stage: K, K, V, V sub-tiles
-  using W = Walk<64, kPos, 1, kThreads>;
-  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
-  const uint32_t smem = smem_u32(dsm);
-  const T *base = reinterpret_cast<const T *>(p.pg.base) + (uint64_t)p.layer * p.pg.layer_stride;
-  pdl_launch_dependents();
-  W w;
-  w.start(p, 2, red);
-  if (tid == 0) p.desc[blockIdx.x].w = 0;
-  for (Segment s; w.next(p, s);) {
-    const uint32_t *pt = p.pg.page_table + (uint64_t)s.chunk.seq * p.pg.max_pages;
-    const uint32_t row0 = s.r0 + 16 * warp;
-    const bool live = row0 < s.r1;
-    Rows<T, HD> rows;
-    if (live) rows.load(p, s, row0);
-    const uint32_t first = s.lo / kPos, end = s.hi > s.lo ? s.u1 : s.u0;
-    auto fetch = [&](uint32_t u) {  // unit u to its stage; one group
-      if (u < end) {
-        const uint32_t t0 = (first + u) * kPos, st = smem + (u & 1) * 4 * kTileBytes;
-#pragma unroll
-        for (uint32_t h = 0; h < 2; ++h) {
-          const PagePair pg = look_up(pt, t0 + kSub * h, s.lo, s.hi);
-          flag_bad_pages(p, pg);
-          stage<T, HD>(p, base, pg, s.head, 0, t0 + kSub * h, s.lo, s.hi, st + h * kTileBytes, tid, kThreads);
-          stage<T, HD>(p, base, pg, s.head, 1, t0 + kSub * h, s.lo, s.hi, st + (2 + h) * kTileBytes, tid, kThreads);
-        }
-      }
-      cp_commit();
-    };
-    fetch(s.u0);
-    for (uint32_t u = s.u0; u < end; ++u) {
-      fetch(u + 1);
-      cp_wait<1>();
-      __syncthreads();
-      const uint32_t t0 = (first + u) * kPos, st = smem + (u & 1) * 4 * kTileBytes;
-#pragma unroll 1
-      for (uint32_t h = 0; h < 2; ++h) {
-        const uint32_t t = t0 + kSub * h;
-        if (!live || (int32_t)t > rows.pos_max) break;  // later than every row of the warp
-        float sc[kSub / 8][4];
-        rows.scores(st + h * kTileBytes, sc);
-        rows.softmax(p, t, sc);
-        rows.add_values(st + (2 + h) * kTileBytes, sc);
-      }
-      __syncthreads();  // the stage is fetched into again
-    }
-    cp_wait<0>();
-    __syncthreads();
-    const bool whole = W::whole(s);
-    float *slot = W::slot(p, s);
-    if (live) {
-      rows.finish();
-#pragma unroll
-      for (uint32_t i = 0; i < 2; ++i) {
-        const uint32_t row = row0 + g + 8 * i, r = row - s.r0;
-        if (row >= s.r1) continue;
-        const float inv = rows.l[i] == 0.0f ? 0.0f : 1.0f / rows.l[i];
-        T *o = out_row<T>(p, s, row, HD);
-#pragma unroll
-        for (uint32_t j = 0; j < HD / 8; ++j) {
-          const float x = rows.o[j][2 * i], y = rows.o[j][2 * i + 1];
-          const uint32_t d = 8 * j + 2 * c;
-          if (!whole) {
-            *reinterpret_cast<float2 *>(slot + r * HD + d) = make_float2(x, y);
-          } else if (p.aligned) {
-            *reinterpret_cast<uint32_t *>(o + d) = pack2<T>(x * inv, y * inv);
-          } else {
-            o[d] = round_to<T>(x * inv);
-            o[d + 1] = round_to<T>(y * inv);
-          }
-        }
-        if (!whole && c == 0) *reinterpret_cast<float2 *>(slot + 64 * HD + 2 * r) = make_float2(rows.m[i], rows.l[i]);
-      }
-    }
-    if (!whole && s.u0 == 0 && tid == 0) p.desc[blockIdx.x] = w.describe(s);
-  }
-}
-
-template <typename T, uint32_t HD>
-uint32_t launch_hd(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st, uint32_t *R) {
-  // up to 16 rows: two 32-position tiles a warp, and the merge's 4 x 16 rows
-  const uint32_t smem = 4 * 2 * kSub * HD * 2;
-  const uint32_t merge = 4 * 16 * (HD + 4) * 4 + 4 * 16 * 8;
-  const uint32_t bytes = smem > merge ? smem : merge;
-  const bool few = (uint64_t)p.max_q * p.rep <= 16;
+uint32_t launch_hd(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st) {
+  // two tiles of 32 positions a warp, or the merge's 4 x 16 rows
+  constexpr uint32_t kTiles = 4 * 2 * kSub * HD * 2, kMerge = 4 * 16 * (HD + 4) * 4 + 4 * 16 * 8, kBytes = kTiles > kMerge ? kTiles : kMerge;
   const uint32_t grid = 3 * n_sm < kAttnMaxCtas ? 3 * n_sm : kAttnMaxCtas;
-  const void *f = few ? (const void *)k_attn_rows16<T, HD> : (const void *)k_attn_rows64<T, HD>;
-  if (cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) return 0;
-  if (few) k_attn_rows16<T, HD><<<grid, kThreads, bytes, st>>>(p);
-  else k_attn_rows64<T, HD><<<grid, kThreads, bytes, st>>>(p);
-  *R = few ? 16 : 64;
+  if (cudaFuncSetAttribute(k_attn_rows16<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kBytes) != cudaSuccess) return 0;
+  k_attn_rows16<T, HD><<<grid, kThreads, kBytes, st>>>(p);
   return cudaGetLastError() == cudaSuccess ? grid : 0;
 }
 
@@ -466,9 +377,9 @@ bool attn_mma_takes(const AttnChunksParams &p) {
          (uint64_t)p.pg.n_pages * 2 * p.pg.n_kv_heads * kPageLen < 0x7FFFFFFFull;
 }
 
-uint32_t launch_attn_mma(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st, uint32_t *R) {
-  if (p.pg.dtype == FA_KV_F16) return p.pg.head_dim == 64 ? launch_hd<__half, 64>(p, n_sm, st, R) : launch_hd<__half, 128>(p, n_sm, st, R);
-  return p.pg.head_dim == 64 ? launch_hd<__nv_bfloat16, 64>(p, n_sm, st, R) : launch_hd<__nv_bfloat16, 128>(p, n_sm, st, R);
+uint32_t launch_attn_mma(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st) {
+  if (p.pg.dtype == FA_KV_F16) return p.pg.head_dim == 64 ? launch_hd<__half, 64>(p, n_sm, st) : launch_hd<__half, 128>(p, n_sm, st);
+  return p.pg.head_dim == 64 ? launch_hd<__nv_bfloat16, 64>(p, n_sm, st) : launch_hd<__nv_bfloat16, 128>(p, n_sm, st);
 }
 
 }  // namespace fa

@@ -9,6 +9,8 @@
 // pipe works on the other's.  Rows are (token, query head of the kv head)
 // pairs, so all query heads of a kv head share its K and V.
 //
+// (Chunks of up to 128 rows: one Q tile an item, softmax warps 0-3, the others
+// from 4 on, two CTAs an SM.)
 //   warps 0-3, 4-7   softmax of Q tile 0, 1: a thread a row.  Scores come from
 //                    tensor memory, weights go back over them (16 bits, as V
 //                    was rounded), read by the second MMA as its A operand.
@@ -36,27 +38,34 @@
 namespace fa {
 namespace {
 
-constexpr uint32_t kTcThreads = 384, kTcPos = 128;
+constexpr uint32_t kTcPos = 128;
 
-template <uint32_t HD>
+// G Q tiles to an item
+template <uint32_t HD, uint32_t G>
 struct TcCfg {
+  static constexpr uint32_t kThreads = 128 * G + 128, kRows = 128 * G;
   static constexpr uint32_t kHalf = kTcPos * 128;           // 128 positions (or rows) x 64 elements
   static constexpr uint32_t kTile = kHalf * (HD / 64);      // one of K, V, or a Q tile
-  static constexpr uint32_t kStages = HD == 128 ? 5 : 8;
-  static constexpr uint32_t kBarOff = 2 * kTile + kStages * kTile;
+  static constexpr uint32_t kStages = HD == 128 ? (G == 2 ? 5 : 2) : (G == 2 ? 8 : 5);
+  static constexpr uint32_t kBarOff = G * kTile + kStages * kTile;
   static constexpr uint32_t kSmem = 1024 + kBarOff + 512;   // alignment, barriers
-  static_assert(kSmem <= 227 * 1024, "shared memory of a CTA");
+  static_assert(kSmem <= (G == 2 ? 227 : 113) * 1024, "shared memory of a CTA");
+  static constexpr uint32_t kTmem = 256 * G;
 };
+template <uint32_t G>
+using TcWalk = Walk<128 * G, kTcPos, 3, 128 * G + 128>;  // an item costs some 5 us beside its tiles of 1.9
 struct TcBars {
   uint64_t full[8], empty[8], q_full[2], q_empty[2], s_full[2], p_half[2], p_full[2], o_full[2], done;
-  uint64_t red[kTcThreads / 32 + 2];
+  uint64_t red[384 / 32 + 2];
   uint32_t tmem, abort;
 };
 static_assert(sizeof(TcBars) <= 512, "barrier space");
 
 // tensor memory columns: scores (and weights over them) of tile i, outputs
+template <uint32_t G>
 __device__ __forceinline__ uint32_t s_col(uint32_t i) { return 128 * i; }
-__device__ __forceinline__ uint32_t o_col(uint32_t i) { return 256 + 128 * i; }
+template <uint32_t G>
+__device__ __forceinline__ uint32_t o_col(uint32_t i) { return 128 * (G + i); }
 
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -165,8 +174,6 @@ __device__ __forceinline__ void weights32(const float *x, uint64_t scale, uint64
   }
 }
 
-using TcWalk = Walk<kTcRows, kTcPos, 3, kTcThreads>;  // an item costs some 5 us beside its tiles of 1.9
-
 // Q rows [first, first + 128) of the item to a swizzled tile, 64 threads; rows
 // past the item's are zeros
 template <typename T, uint32_t HD>
@@ -183,7 +190,7 @@ __device__ __forceinline__ void load_q(const AttnChunksParams &p, const Segment 
   for (uint32_t r = r0; r < 128; r += kStep) {
     const bool live = r < rows;
     const T *x = live ? base + tok * p.qs + h * HD : base;
-    const uint32_t dst = tile + (c >> 3) * TcCfg<HD>::kHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+    const uint32_t dst = tile + (c >> 3) * (kTcPos * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
     if (p.aligned) {
       asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(x), "r"(live ? 16u : 0u) : "memory");
     } else {
@@ -203,17 +210,17 @@ __device__ __forceinline__ void load_q(const AttnChunksParams &p, const Segment 
   }
 }
 
-template <typename T, uint32_t HD>
-__device__ void q_role(const AttnChunksParams &p, TcWalk w, TcBars &b, uint32_t smem) {
+template <typename T, uint32_t HD, uint32_t G>
+__device__ void q_role(const AttnChunksParams &p, TcWalk<G> w, TcBars &b, uint32_t smem) {
   const uint32_t tid = threadIdx.x & 63;
   uint32_t n[2] = {0, 0};  // fills of each tile so far
   for (Segment s; w.next(p, s);) {
     if (s.hi <= s.lo) continue;
 #pragma unroll
-    for (uint32_t g = 0; g < 2; ++g) {
+    for (uint32_t g = 0; g < G; ++g) {
       if (s.r0 + 128 * g >= s.r1) break;
       if (!wait_bar(&b.abort, &b.q_empty[g], (n[g] & 1) ^ 1)) return;
-      load_q<T, HD>(p, s, s.r0 + 128 * g, smem + g * TcCfg<HD>::kTile, tid);
+      load_q<T, HD>(p, s, s.r0 + 128 * g, smem + g * TcCfg<HD, G>::kTile, tid);
       asm volatile("cp.async.wait_all;" ::: "memory");
       fence_proxy_async_smem();
       mbar_arrive(&b.q_full[g]);
@@ -229,15 +236,15 @@ __device__ __forceinline__ void st8(void *p, const uint32_t (&v)[8]) {
                : "memory");
 }
 
-template <typename T, uint32_t HD>
-__device__ void softmax_role(const AttnChunksParams &p, TcWalk w, TcBars &b, uint32_t tmem, uint32_t g) {
+template <typename T, uint32_t HD, uint32_t G>
+__device__ void softmax_role(const AttnChunksParams &p, TcWalk<G> w, TcBars &b, uint32_t tmem, uint32_t g) {
   const uint32_t tid = threadIdx.x & 127, warp = tid >> 5;
   const uint32_t lanes = tmem + ((warp * 32) << 16);
   uint32_t n = 0;  // tiles of this group so far
   for (Segment s; w.next(p, s);) {
     const uint32_t row = s.r0 + 128 * g + tid;
     if (s.r0 + 128 * g >= s.r1) continue;  // the second Q tile is empty
-    const bool live = row < s.r1, whole = TcWalk::whole(s);
+    const bool live = row < s.r1, whole = TcWalk<G>::whole(s);
     const int32_t pos = s.chunk.first + (int32_t)(row / p.rep);
     // a warp past the item's last row only hands its (unused) rows on; within a
     // warp such rows ask for no masks
@@ -255,7 +262,7 @@ __device__ void softmax_role(const AttnChunksParams &p, TcWalk w, TcBars &b, uin
       fence_after();
       float x[kTcPos];
 #pragma unroll
-      for (uint32_t c = 0; c < 4; ++c) ld32(lanes + s_col(g) + 32 * c, x + 32 * c);
+      for (uint32_t c = 0; c < 4; ++c) ld32(lanes + s_col<G>(g) + 32 * c, x + 32 * c);
       wait_ld();
       // rows of a warp that see all 128 positions need no mask
       const int32_t to = pos - (int32_t)t0 + 1;  // visible columns: [to - window, to)
@@ -290,11 +297,11 @@ __device__ void softmax_role(const AttnChunksParams &p, TcWalk w, TcBars &b, uin
 #pragma unroll 1
         for (uint32_t c = 0; c < HD; c += 32) {
           float o[32];
-          ld32(lanes + o_col(g) + c, o);
+          ld32(lanes + o_col<G>(g) + c, o);
           wait_ld();
 #pragma unroll
           for (uint32_t e = 0; e < 32; ++e) o[e] *= f;
-          st32(lanes + o_col(g) + c, reinterpret_cast<const uint32_t *>(o));
+          st32(lanes + o_col<G>(g) + c, reinterpret_cast<const uint32_t *>(o));
         }
       }
       const float ms = m == -INFINITY ? 0.0f : m;
@@ -309,7 +316,7 @@ __device__ void softmax_role(const AttnChunksParams &p, TcWalk w, TcBars &b, uin
           fence_before();
           mbar_arrive(&b.p_half[g]);
         }
-        st16(lanes + s_col(g) + 16 * h, pk);
+        st16(lanes + s_col<G>(g) + 16 * h, pk);
       }
       wait_st();
       fence_before();
@@ -319,7 +326,7 @@ __device__ void softmax_role(const AttnChunksParams &p, TcWalk w, TcBars &b, uin
       unpair(sum[1], s2, s3);
       l += (s0 + s1) + (s2 + s3);
     }
-    float *slot = TcWalk::slot(p, s);
+    float *slot = TcWalk<G>::slot(p, s);
     const uint32_t r = row - s.r0, tok = row / p.rep;
     T *out = reinterpret_cast<T *>(p.out) + (uint64_t)(s.chunk.q0 + tok) * p.os + (s.head * p.rep + row - tok * p.rep) * HD;
     if (tiles) {
@@ -331,7 +338,7 @@ __device__ void softmax_role(const AttnChunksParams &p, TcWalk w, TcBars &b, uin
     for (uint32_t c = 0; c < HD; c += 32) {
       float o[32];
       if (tiles) {
-        ld32(lanes + o_col(g) + c, o);
+        ld32(lanes + o_col<G>(g) + c, o);
         wait_ld();
       }
       if (l == 0.0f) {  // nothing seen (yet, within a split item): zeros, whatever the product left
@@ -361,15 +368,15 @@ __device__ void softmax_role(const AttnChunksParams &p, TcWalk w, TcBars &b, uin
         }
       }
     }
-    if (!whole && live) *reinterpret_cast<float2 *>(slot + kTcRows * HD + 2 * r) = make_float2(m, l);
+    if (!whole && live) *reinterpret_cast<float2 *>(slot + 128 * G * HD + 2 * r) = make_float2(m, l);
     if (!whole && s.u0 == 0 && g == 0 && tid == 0) p.desc[blockIdx.x] = w.describe(s);
     fence_before();  // the next item's MMAs follow its q_full and p_full arrivals
   }
 }
 
-template <typename T, uint32_t HD>
-__device__ void mma_role(const AttnChunksParams &p, TcWalk w, TcBars &b, uint32_t smem, uint32_t tmem) {
-  using C = TcCfg<HD>;
+template <typename T, uint32_t HD, uint32_t G>
+__device__ void mma_role(const AttnChunksParams &p, TcWalk<G> w, TcBars &b, uint32_t smem, uint32_t tmem) {
+  using C = TcCfg<HD, G>;
   constexpr uint32_t kType = __is_same(T, __half) ? 0u : 1u;  // f16 / bf16, A and B
   constexpr uint32_t kS = (1u << 4) | (kType << 7) | (kType << 10) | ((kTcPos / 8) << 17) | ((128 / 16) << 24);
   constexpr uint32_t kO = (1u << 4) | (kType << 7) | (kType << 10) | (1u << 16) | ((HD / 8) << 17) | ((128 / 16) << 24);  // B = V: rows are K
@@ -377,7 +384,7 @@ __device__ void mma_role(const AttnChunksParams &p, TcWalk w, TcBars &b, uint32_
   // one lane the operands' way into uniform registers made each MMA take some
   // 130 clocks to issue (637 us for 2048 rows over 16384 positions, 495 so).
   // Ring places and phases are counted on.
-  const uint32_t q_lo = sdesc_lo(smem, 16), k_lo = sdesc_lo(smem + 2 * C::kTile, 16), v_lo = sdesc_lo(smem + 2 * C::kTile, C::kHalf);
+  const uint32_t q_lo = sdesc_lo(smem, 16), k_lo = sdesc_lo(smem + G * C::kTile, 16), v_lo = sdesc_lo(smem + G * C::kTile, C::kHalf);
   struct Place {  // of a fill in the ring (fills come K0 V0 K1 V1 ..)
     uint32_t st, ph;
     __device__ void step() {
@@ -396,14 +403,14 @@ __device__ void mma_role(const AttnChunksParams &p, TcWalk w, TcBars &b, uint32_
 #pragma unroll
       for (uint32_t kk = 0; kk < HD / 16; ++kk) {
         const uint32_t off = kk / 4 * (C::kHalf >> 4) + kk % 4 * 2;
-        mma_ss(tmem + s_col(g), sdesc(q + off), sdesc(k + off), kS, kk);
+        mma_ss(tmem + s_col<G>(g), sdesc(q + off), sdesc(k + off), kS, kk);
       }
       commit(&b.s_full[g]);
     }
     __syncwarp();
   };
   for (Segment s; w.next(p, s);) {
-    const uint32_t tiles = s.hi > s.lo ? s.u1 - s.u0 : 0, groups = s.r1 - s.r0 > 128 ? 2 : 1;
+    const uint32_t tiles = s.hi > s.lo ? s.u1 - s.u0 : 0, groups = G == 2 && s.r1 - s.r0 > 128 ? 2 : 1;
     if (!tiles) continue;
     if (!wait_bar(&b.abort, &b.full[at.st], at.ph)) return;
     for (uint32_t g = 0; g < groups; ++g) {
@@ -431,7 +438,7 @@ __device__ void mma_role(const AttnChunksParams &p, TcWalk w, TcBars &b, uint32_
 if (lead)
 #pragma unroll
           for (uint32_t kk = 4 * h; kk < 4 * h + 4; ++kk)
-            mma_ts(tmem + o_col(g), tmem + s_col(g) + 8 * kk, sdesc(vt + kk * (2048 >> 4)), kO, k || kk);
+            mma_ts(tmem + o_col<G>(g), tmem + s_col<G>(g) + 8 * kk, sdesc(vt + kk * (2048 >> 4)), kO, k || kk);
         }
         ++n[g];
         if (lead) commit(&b.o_full[g]);
@@ -448,11 +455,11 @@ if (lead)
 }
 
 // one warp
-template <typename T, uint32_t HD>
-__device__ void load_role(const AttnChunksParams &p, TcWalk w, TcBars &b, uint32_t smem, const CUtensorMap *map, const CUtensorMap *row_map,
+template <typename T, uint32_t HD, uint32_t G>
+__device__ void load_role(const AttnChunksParams &p, TcWalk<G> w, TcBars &b, uint32_t smem, const CUtensorMap *map, const CUtensorMap *row_map,
                           uint32_t &fills) {
-  using C = TcCfg<HD>;
-  const uint32_t lane = threadIdx.x & 31, ring = smem + 2 * C::kTile;
+  using C = TcCfg<HD, G>;
+  const uint32_t lane = threadIdx.x & 31, ring = smem + G * C::kTile;
   uint32_t st = 0, ph = 1;
   for (Segment s; w.next(p, s);) {
     const uint32_t tiles = s.hi > s.lo ? s.u1 - s.u0 : 0;
@@ -499,10 +506,10 @@ __device__ void load_role(const AttnChunksParams &p, TcWalk w, TcBars &b, uint32
   }
 }
 
-template <typename T, uint32_t HD>
-__global__ void __launch_bounds__(kTcThreads, 1) k_attn_tc(const AttnChunksParams p, const __grid_constant__ CUtensorMap map,
+template <typename T, uint32_t HD, uint32_t G>
+__global__ void __launch_bounds__(128 * G + 128, 3 - G) k_attn_tc(const AttnChunksParams p, const __grid_constant__ CUtensorMap map,
                                                             const __grid_constant__ CUtensorMap row_map) {
-  using C = TcCfg<HD>;
+  using C = TcCfg<HD, G>;
   extern __shared__ __align__(1024) uint8_t raw[];
   const uint32_t pad = (1024u - (smem_u32(raw) & 1023u)) & 1023u, smem = smem_u32(raw) + pad;
   TcBars &b = *reinterpret_cast<TcBars *>(raw + pad + C::kBarOff);
@@ -511,7 +518,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_tc(const AttnChunksParam
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&row_map) : "memory");
   }
-  TcWalk w;
+  TcWalk<G> w;
   w.start(p, 4, b.red);
   if (tid == 0) {
     p.desc[blockIdx.x].w = 0;
@@ -533,63 +540,74 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_tc(const AttnChunksParam
   }
   const bool any = !w.done();  // the same for the CTA
   if (any) {
-    if (warp == 8) {
-      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&b.tmem)));
+    if (warp == 4 * G) {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&b.tmem)), "r"(C::kTmem));
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
     fence_before();
     __syncthreads();
     fence_after();
     const uint32_t tmem = b.tmem;
-    // 384 x 168 registers at launch: 256 x 224 + 128 x 56
-    if (warp < 8) {
-      asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
-      softmax_role<T, HD>(p, w, b, tmem, warp >> 2);
+    // registers at launch: 384 x 168 = 256 x 224 + 128 x 56, or 256 x 128 =
+    // 128 x 200 + 128 x 56
+    if (warp < 4 * G) {
+      if constexpr (G == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+      else asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+      softmax_role<T, HD, G>(p, w, b, tmem, warp >> 2);
     } else {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-      if (warp == 8) {
-        mma_role<T, HD>(p, w, b, smem, tmem);
+      if (warp == 4 * G) {
+        mma_role<T, HD, G>(p, w, b, smem, tmem);
         if (lane == 0) commit(&b.done);
         __syncwarp();
         mbar_wait(&b.done, 0);  // nothing is on its way to tensor memory after this
-      } else if (warp == 9) {
+      } else if (warp == 4 * G + 1) {
         uint32_t fills = 0;
-        load_role<T, HD>(p, w, b, smem, &map, &row_map, fills);
+        load_role<T, HD, G>(p, w, b, smem, &map, &row_map, fills);
         if (*reinterpret_cast<volatile uint32_t *>(&b.abort))  // copies that nobody waited for
           for (uint32_t i = fills > C::kStages ? fills - C::kStages : 0; i < fills; ++i)
             mbar_wait(&b.full[i % C::kStages], i / C::kStages & 1);
       } else {
-        q_role<T, HD>(p, w, b, smem);
+        q_role<T, HD, G>(p, w, b, smem);
       }
     }
     __syncwarp();
     fence_before();
     __syncthreads();
     if (tid == 0 && b.abort && p.err) atomicOr(p.err, kFlagTimeout);
-    if (warp == 8) {
+    if (warp == 4 * G) {
       fence_after();
-      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kTmem));
     }
   }
   pdl_wait();  // the launch before this one, with which it may have overlapped: the join waits for this one only
 }
 
-template <typename T, uint32_t HD>
-int launch_hd(const AttnChunksParams &p, uint32_t ctas, cudaStream_t st) {
+template <typename T, uint32_t HD, uint32_t G>
+uint32_t launch_g(const AttnChunksParams &p, uint32_t n_sm, bool overlap, cudaStream_t st) {
+  using C = TcCfg<HD, G>;
   CUtensorMap map, row_map;
-  if (!page_map(p, kPageLen, &map) || !page_map(p, 1, &row_map)) return -1;
-  if (cudaFuncSetAttribute(k_attn_tc<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)TcCfg<HD>::kSmem) != cudaSuccess) return -1;
-  return launch_pdl(k_attn_tc<T, HD>, dim3(ctas), dim3(kTcThreads), TcCfg<HD>::kSmem, st, p, map, row_map);
+  if (!page_map(p, kPageLen, &map) || !page_map(p, 1, &row_map)) return 0;
+  if (cudaFuncSetAttribute(k_attn_tc<T, HD, G>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::kSmem) != cudaSuccess) return 0;
+  const uint32_t ctas = (n_sm < kTcMaxCtas ? n_sm : kTcMaxCtas) * (3 - G);  // one or two an SM
+  if (overlap) return launch_pdl(k_attn_tc<T, HD, G>, dim3(ctas), dim3(C::kThreads), C::kSmem, st, p, map, row_map) ? 0 : ctas;
+  k_attn_tc<T, HD, G><<<ctas, C::kThreads, C::kSmem, st>>>(p, map, row_map);
+  return cudaGetLastError() == cudaSuccess ? ctas : 0;
+}
+template <typename T>
+uint32_t launch_t(const AttnChunksParams &p, uint32_t n_sm, bool overlap, cudaStream_t st, uint32_t *R) {
+  // No chunk above 128 rows: items of one Q tile, two CTAs an SM, which hide one
+  // another's waits as the two Q tiles of a longer chunk's item do
+  const bool one = (uint64_t)p.max_q * p.rep <= 128;
+  *R = one ? 128 : 256;
+  if (p.pg.head_dim == 64) return one ? launch_g<T, 64, 1>(p, n_sm, overlap, st) : launch_g<T, 64, 2>(p, n_sm, overlap, st);
+  return one ? launch_g<T, 128, 1>(p, n_sm, overlap, st) : launch_g<T, 128, 2>(p, n_sm, overlap, st);
 }
 
 }  // namespace
 
-uint32_t launch_attn_tc(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st) {
-  const uint32_t ctas = n_sm < kTcMaxCtas ? n_sm : kTcMaxCtas;  // one an SM
-  int rc;
-  if (p.pg.dtype == FA_KV_F16) rc = p.pg.head_dim == 64 ? launch_hd<__half, 64>(p, ctas, st) : launch_hd<__half, 128>(p, ctas, st);
-  else rc = p.pg.head_dim == 64 ? launch_hd<__nv_bfloat16, 64>(p, ctas, st) : launch_hd<__nv_bfloat16, 128>(p, ctas, st);
-  return rc ? 0 : ctas;
+uint32_t launch_attn_tc(const AttnChunksParams &p, uint32_t n_sm, bool overlap, cudaStream_t st, uint32_t *R) {
+  return p.pg.dtype == FA_KV_F16 ? launch_t<__half>(p, n_sm, overlap, st, R) : launch_t<__nv_bfloat16>(p, n_sm, overlap, st, R);
 }
 
 }  // namespace fa
