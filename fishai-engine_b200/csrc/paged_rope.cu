@@ -166,9 +166,11 @@ int launch_io(const RopeAppendParams &p, const RopeTable &t, cudaStream_t st) {
   };
   const uint32_t W = sizeof(TI) == 2 && sizeof(TO) == 2 && fits(8) ? 8 : fits(4) ? 4 : 1;  // accesses of up to 16 bytes
   const uint32_t units = (p.n_heads + 2 * p.pg.n_kv_heads) * (hd / (2 * W));
-  // few tokens: small CTAs, the heads spread over the SMs; many: four tokens a
-  // CTA, one CTA for all heads where it can be
-  const uint32_t each = p.n_tokens < 2048 ? 1 : kRopeTokens;
+  // few tokens: small CTAs, the heads spread over the SMs; many: up to four
+  // tokens a CTA as long as two CTAs an SM remain, one CTA for all heads where it
+  // can be (2000 tokens: 20.8 us with one token a CTA, 17.0 with four; 8192: 43
+  // with four, 51 with two, 45 with eight)
+  const uint32_t each = p.n_tokens < 600 ? 1 : p.n_tokens < 1200 ? 2 : kRopeTokens;
   uint32_t block = p.n_tokens < 296 ? 128 : (units + 31) / 32 * 32;
   if (block > 512) block = (units / ((units + 511) / 512) + 31) / 32 * 32;
   const dim3 grid((p.n_tokens + each - 1) / each, (units + block - 1) / block);
