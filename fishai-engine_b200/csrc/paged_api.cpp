@@ -262,7 +262,7 @@ int fa_attn_chunks(const fa_pages *pages, uint32_t layer, const void *q, uint64_
   if (layer >= pages->n_layers) return invalid(who, "layer out of range");
   if (!n_heads || n_heads > 32767 || n_heads % pages->n_kv_heads)
     return invalid(who, "n_heads is a multiple of the pages' kv heads, at most 32767");
-  if (!std::isfinite(scale) || scale < 0) return invalid(who, "scale is a finite number, at least 0");
+  if (!std::isfinite(scale) || scale < 0 || scale > 1e30f) return invalid(who, "scale is a number from 0 to 1e30");
   if ((uint64_t)n_tokens * n_heads > 0x7FFFFFFFu) return invalid(who, "2^31 or more query rows");
   if (window > 0x7FFFFFFFu) window = 0;  // wider than any cache: none
   const uint64_t hd = pages->head_dim, qw = n_heads * hd;
@@ -317,6 +317,7 @@ int fa_pages_copy(const fa_pages *pages, const uint32_t *src, const uint32_t *ds
                   uint32_t *err, void *stream) {
   const char *who = "fa_pages_copy";
   TRY(check_pages(who, pages, false));
+  if (n > 0x7FFFFFFFu) return invalid(who, "too many pages");
   if (!n) return FA_OK;
   if (!src || !dst) return invalid(who, "null argument");
   OnDevice dev(who);
@@ -338,7 +339,7 @@ int fa_pages_compact(const fa_pages *pages, const uint32_t *seq, const uint32_t 
                      uint32_t n, uint32_t n_keep, uint32_t *err, void *stream) {
   const char *who = "fa_pages_compact";
   TRY(check_pages(who, pages, true));
-  if (n_keep > 0x7FFFFFFFu) return invalid(who, "too many kept positions");
+  if (n_keep > 0x7FFFFFFFu || n > 0x7FFFFFFFu) return invalid(who, "too many kept positions or sequences");
   if (!n || !n_keep) return FA_OK;
   if (!seq || !keep || !keep_start) return invalid(who, "null argument");
   OnDevice dev(who);

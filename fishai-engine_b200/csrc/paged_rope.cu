@@ -173,6 +173,7 @@ int launch_io(const RopeAppendParams &p, const RopeTable &t, cudaStream_t st) {
   const uint32_t each = p.n_tokens < 600 ? 1 : p.n_tokens < 1200 ? 2 : kRopeTokens;
   uint32_t block = p.n_tokens < 296 ? 128 : (units + 31) / 32 * 32;
   if (block > 512) block = (units / ((units + 511) / 512) + 31) / 32 * 32;
+  if ((units + block - 1) / block > 65535) block = 512;  // grid y (thousands of heads)
   const dim3 grid((p.n_tokens + each - 1) / each, (units + block - 1) / block);
   if constexpr (sizeof(TI) == 2 && sizeof(TO) == 2) {
     if (W == 8) k_rope_append<TI, TO, 8><<<grid, block, 0, st>>>(p, t, each);

@@ -325,9 +325,9 @@ int fa_rope_freqs(const fa_rope *r, double *freqs, double *scale);
  * slot[t] (slot NULL: pos[t]); q row t of n_heads * head_dim elements at
  * q + t q_stride goes to out + t out_stride (out may be q), k and v rows of
  * n_kv_heads * head_dim elements.  q, k, v have type in_dtype, out the pages'
- * type.  seq[t] = FA_NO_TOKEN marks a row that is left out (padding).  Two
- * tokens of a call must not name the same sequence and slot: the cache row
- * would hold some of each. */
+ * type.  out shares no memory with k, v or the pages.  seq[t] = FA_NO_TOKEN
+ * marks a row that is left out (padding).  Two tokens of a call must not name
+ * the same sequence and slot: the cache row would hold some of each. */
 #define FA_NO_TOKEN 4294967295u
 int fa_rope_append(const fa_rope *r, const fa_pages *pages, uint32_t layer, int32_t in_dtype, const void *q,
                    uint64_t q_stride, const void *k, uint64_t k_stride, const void *v, uint64_t v_stride,
@@ -341,7 +341,7 @@ int fa_rope_append(const fa_rope *r, const fa_pages *pages, uint32_t layer, int3
  * the chunk's own tokens last.  Token i of the q_len is at position
  * p = kv_len - q_len + i and sees the positions t with 0 <= t <= p, and
  * t > p - window where window > 0; a token that sees none gives zeros.
- * Scores are scaled by `scale` (0: 1 / sqrt(head_dim)).  Chunks may have any
+ * Scores are scaled by `scale` (0: 1 / sqrt(head_dim); at most 1e30).  Chunks may have any
  * lengths, zero and one among them, in any mix; none is longer than max_q
  * (one that is sets FA_FLAG_RANGE and is left out).  Rows outside every chunk
  * are left as they were.  q and out have the pages' type and rows of n_heads *

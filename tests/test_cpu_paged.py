@@ -87,7 +87,7 @@ def test_null_handles():
 
 
 @pytest.mark.parametrize("bad", [dict(layer=2), dict(heads=0), dict(heads=6), dict(qs=511), dict(os=500), dict(scale=-1.0),
-                                 dict(scale=math.nan), dict(scale=math.inf), dict(q=None), dict(starts=None), dict(kv=None),
+                                 dict(scale=math.nan), dict(scale=math.inf), dict(scale=1e31), dict(q=None), dict(starts=None), dict(kv=None),
                                  dict(out=None), dict(ws=None), dict(chunks=3), dict(ws_bytes=100), dict(ws=P * 16 + 8),
                                  dict(q=P + 1), dict(out=P), dict(out=P + 1024), dict(n=1 << 30)], ids=str)
 def test_attention_refuses(bad):

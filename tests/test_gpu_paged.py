@@ -539,3 +539,60 @@ def test_work_is_on_the_given_stream():
         paged.attention(paged.PagedKV(pages, table), 0, q, start, kv, out, 1, ws, stream=s.cuda_stream)
     s.synchronize()
     assert same_bits(out, want)
+
+
+def test_two_streams_with_workspaces_of_their_own():
+    """two attention calls and two selections that may run at the same time"""
+    pages, table = R.make_cache([5000, 900], 1, 2, 128, torch.float16, 32)
+    q = randn(6, 300, 8 * 128, dtype=torch.float16)
+    kv = paged.PagedKV(pages, table)
+    calls = [([0, 1, 3], [5000, 900], 2), ([0, 200, 300], [4000, 800], 200)]
+    want = [attn(pages, table, q, a, b, 8, max_q=m) for a, b, m in calls]
+    streams = [torch.cuda.Stream() for _ in calls]
+    ws = [torch.empty(paged.workspace_bytes(128), dtype=torch.uint8, device="cuda") for _ in calls]
+    out = [torch.full_like(q, 7.0) for _ in calls]
+    args = [(i32(a), i32(b), m) for a, b, m in calls]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for (a, b, m), s, w, o in zip(args, streams, ws, out):
+            paged.attention(kv, 0, q, a, b, o, m, w, stream=s.cuda_stream)
+    torch.cuda.synchronize()
+    assert all(same_bits(o, w) for o, w in zip(out, want))
+    x = 3 * randn(8, 2, 8, 50000)
+    scores = -torch.rand(2, 8, device="cuda")
+    sel = [beam_run(x[i], scores[i: i + 1], None, 8) for i in range(2)]
+    outs = [[torch.empty(1, 8, dtype=d, device="cuda") for d in (torch.float32, torch.int32, torch.int32, torch.int32)] for _ in range(2)]
+    bw = [torch.empty(beam.workspace_bytes(1, 8, 50000, 8), dtype=torch.uint8, device="cuda") for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for i in range(2):
+            beam.select(x[i], scores[i: i + 1], None, *outs[i], workspace=bw[i], eos=2, stream=streams[i].cuda_stream)
+    torch.cuda.synchronize()
+    for o, w in zip(outs, sel):
+        assert all(torch.equal(a.cpu(), b) for a, b in zip(o, w))
+
+
+@pytest.mark.parametrize("t,n_pages", [("f16", 140000), ("f32", 70000)])
+def test_offsets_beyond_32_bits(t, n_pages):
+    """a layer of more than 2^31 elements (f16: 2^32), sequences in its last pages"""
+    dtype, kvh, hd, H = R.TYPES[t], 8, 128, 16
+    small, stable = R.make_cache([700, 40, 333], 1, kvh, hd, dtype, 33)
+    n = small.shape[1]
+    pages = torch.empty(1, n_pages, 2, kvh, 16, hd, dtype=dtype, device="cuda")
+    pages[0, n_pages - n:] = small[0]
+    table = torch.where(stable < n, stable + (n_pages - n), stable).to(torch.int32).contiguous()
+    kv = paged.PagedKV(pages, table)
+    for start, lens in (([0, 1, 2, 3], [700, 40, 333]), ([0, 200, 201, 230], [700, 40, 333])):
+        q = randn(7, start[-1], H * hd, dtype=dtype)
+        a, b = attn(pages, table, q, start, lens, H), attn(small, stable, q, start, lens, H)
+        assert same_bits(a, b)
+    rows = randn(8, 3, (H + 2 * kvh) * hd, dtype=dtype)
+    parts = rows[:, : H * hd], rows[:, H * hd: (H + kvh) * hd], rows[:, (H + kvh) * hd:]
+    outs = []
+    for p, tb in ((pages, table), (small, stable)):
+        out = torch.empty(3, H * hd, dtype=dtype, device="cuda")
+        paged.rope_append(paged.PagedKV(p, tb), 0, paged.Rope(hd), *parts, i32([5, 6, 7]), i32([0, 2, 1]), out)
+        paged.copy_pages(paged.PagedKV(p, tb), tb[0, :3].contiguous(), tb[2, :3].contiguous(), slots=i32([16, 3, 9]))
+        paged.compact(paged.PagedKV(p, tb), i32([0]), i32([3, 8, 200, 699]), i32([0, 4]))
+        outs.append(out)
+    assert same_bits(*outs) and same_bits(pages[0, n_pages - n:], small[0])
