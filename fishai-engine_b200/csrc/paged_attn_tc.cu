@@ -375,7 +375,7 @@ __device__ void softmax_role(const AttnChunksParams &p, TcWalk<G> w, TcBars &b, 
 }
 
 template <typename T, uint32_t HD, uint32_t G>
-__device__ void mma_role(const AttnChunksParams &p, TcWalk<G> w, TcBars &b, uint32_t smem, uint32_t tmem) {
+__device__ void mma_role(const AttnChunksParams &p, TcWalk<G> w, TcBars &b, uint32_t smem, uint32_t tmem, uint32_t lead) {
   using C = TcCfg<HD, G>;
   constexpr uint32_t kType = __is_same(T, __half) ? 0u : 1u;  // f16 / bf16, A and B
   constexpr uint32_t kS = (1u << 4) | (kType << 7) | (kType << 10) | ((kTcPos / 8) << 17) | ((128 / 16) << 24);
@@ -395,8 +395,6 @@ __device__ void mma_role(const AttnChunksParams &p, TcWalk<G> w, TcBars &b, uint
     }
   } at{0, 0};
   uint32_t n[2] = {0, 0}, q_phase[2] = {0, 0};
-  uint32_t lead;
-  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xFFFFFFFF;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(lead));
   auto scores = [&](uint32_t g, uint32_t st) {
     const uint32_t q = q_lo + g * (C::kTile >> 4), k = k_lo + st * (C::kTile >> 4);
     if (lead) {
@@ -435,10 +433,11 @@ __device__ void mma_role(const AttnChunksParams &p, TcWalk<G> w, TcBars &b, uint
         for (uint32_t h = 0; h < 2; ++h) {
           if (!wait_bar(&b.abort, h ? &b.p_full[g] : &b.p_half[g], n[g] & 1)) return;
           fence_after();
-if (lead)
+          if (lead) {
 #pragma unroll
-          for (uint32_t kk = 4 * h; kk < 4 * h + 4; ++kk)
-            mma_ts(tmem + o_col<G>(g), tmem + s_col<G>(g) + 8 * kk, sdesc(vt + kk * (2048 >> 4)), kO, k || kk);
+            for (uint32_t kk = 4 * h; kk < 4 * h + 4; ++kk)
+              mma_ts(tmem + o_col<G>(g), tmem + s_col<G>(g) + 8 * kk, sdesc(vt + kk * (2048 >> 4)), kO, k || kk);
+          }
         }
         ++n[g];
         if (lead) commit(&b.o_full[g]);
@@ -513,7 +512,7 @@ __global__ void __launch_bounds__(128 * G + 128, 3 - G) k_attn_tc(const AttnChun
   extern __shared__ __align__(1024) uint8_t raw[];
   const uint32_t pad = (1024u - (smem_u32(raw) & 1023u)) & 1023u, smem = smem_u32(raw) + pad;
   TcBars &b = *reinterpret_cast<TcBars *>(raw + pad + C::kBarOff);
-  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t tid = threadIdx.x, warp = tid >> 5;
   if (tid == 0) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&row_map) : "memory");
@@ -557,8 +556,11 @@ __global__ void __launch_bounds__(128 * G + 128, 3 - G) k_attn_tc(const AttnChun
     } else {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
       if (warp == 4 * G) {
-        mma_role<T, HD, G>(p, w, b, smem, tmem);
-        if (lane == 0) commit(&b.done);
+        uint32_t lead;  // issues the MMAs and the commits, which follow only its own MMAs
+        asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xFFFFFFFF;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(lead));
+        mma_role<T, HD, G>(p, w, b, smem, tmem, lead);
+        __syncwarp();
+        if (lead) commit(&b.done);
         __syncwarp();
         mbar_wait(&b.done, 0);  // nothing is on its way to tensor memory after this
       } else if (warp == 4 * G + 1) {
