@@ -1294,7 +1294,8 @@ extern "C" int fa_generate_beams(fa_model *fm, const fa_beam_config *cfg, const 
   if (!b || b > 64) return fail(FA_ERR_INVALID, "fa_generate_beams: 1 to 64 beams");
   if (!n_prompt) return fail(FA_ERR_INVALID, "fa_generate_beams: empty prompt");
   if (!cfg->max_new) return fail(FA_ERR_INVALID, "fa_generate_beams: max_new is zero");
-  if (!std::isfinite(cfg->length_penalty)) return fail(FA_ERR_INVALID, "fa_generate_beams: length_penalty is not finite");
+  // within +-30 the power of any length is a positive f64, and every rank a number
+  if (!(std::fabs(cfg->length_penalty) <= 30.0f)) return fail(FA_ERR_INVALID, "fa_generate_beams: length_penalty is -30 to 30");
   if (cfg->kv_dtype != FA_KV_F32 && cfg->kv_dtype != FA_KV_F16) return fail(FA_ERR_INVALID, "fa_generate_beams: bad kv_dtype");
   if ((uint64_t)n_prompt + cfg->max_new > 0x7FFFFFFFu) return fail(FA_ERR_INVALID, "fa_generate_beams: too many positions");
   for (uint32_t i = 0; i < n_prompt; ++i)

@@ -341,11 +341,12 @@ int fa_rope_append(const fa_rope *r, const fa_pages *pages, uint32_t layer, int3
  * the chunk's own tokens last.  Token i of the q_len is at position
  * p = kv_len - q_len + i and sees the positions t with 0 <= t <= p, and
  * t > p - window where window > 0; a token that sees none gives zeros.
- * Scores are scaled by `scale` (0: 1 / sqrt(head_dim); at most 1e30).  Chunks may have any
- * lengths, zero and one among them, in any mix; none is longer than max_q
+ * Scores are scaled by `scale` (0: 1 / sqrt(head_dim); at most 1e30).  Chunks
+ * may have any lengths, zero and one among them, in any mix; none is longer than max_q
  * (one that is sets FA_FLAG_RANGE and is left out).  Rows outside every chunk
  * are left as they were.  q and out have the pages' type and rows of n_heads *
- * head_dim elements, q_stride and out_stride apart; out must not overlap q.
+ * head_dim elements, q_stride and out_stride apart; out must not
+ * overlap q, the pages or ws.
  * The positions that some token of a chunk sees should hold finite K and V;
  * whatever is behind kv_len or before every token's window is not used.  A
  * page out of range (FA_FLAG_PAGE) spoils the chunk's own rows only.
@@ -488,7 +489,7 @@ typedef struct {
   uint32_t n_beams;        /* 1 .. 64 */
   uint32_t max_new;        /* most tokens of a hypothesis */
   uint32_t eos;            /* ends a hypothesis; FA_NO_TOKEN: none */
-  float length_penalty;    /* hypotheses rank by score / length^length_penalty */
+  float length_penalty;    /* hypotheses rank by score / length^length_penalty; -30 to 30 */
   int32_t kv_dtype;        /* FA_KV_F32 or FA_KV_F16 */
 } fa_beam_config;
 /* out_ids [n_beams][max_new]: the hypotheses, best first, eos included;

@@ -256,3 +256,12 @@ def test_generate_beams_refusals(dev):
         assert e.value.code == L.ERR_INVALID
     with pytest.raises(L.FishaiError):
         dev.new_kv_cache(16, dtype=L.KV_BF16)
+
+
+@pytest.mark.parametrize("penalty", [31.0, -1e4, math.inf])
+def test_generate_beams_refuses_penalties_without_a_rank(dev, penalty):
+    """length^penalty would leave the range of f64: score / it could be 0 / 0"""
+    with pytest.raises(L.FishaiError) as e:
+        dev.generate_beams([5], 2, 2, length_penalty=penalty)
+    assert e.value.code == L.ERR_INVALID
+    assert len(dev.generate_beams([5], 2, 2, length_penalty=math.copysign(30.0, penalty))) == 2
