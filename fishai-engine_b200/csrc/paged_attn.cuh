@@ -10,6 +10,8 @@
 // CTA's two slots, and k_attn_join adds the pieces in the order of the
 // positions, so results do not depend on timing.
 #pragma once
+#include <atomic>
+
 #include "fa_device.cuh"
 #include "paged_ops.hpp"
 
@@ -223,6 +225,99 @@ struct Walk {
     return p.part + ((uint64_t)blockIdx.x * 2 + (s.u0 ? 0 : 1)) * R * (p.pg.head_dim + 2);
   }
 };
+// ---- an item on a cluster of CTAs, for few items ----
+// The CTAs take the item's units in turn and add their pieces from one another's
+// shared memory: no second launch, which is half of a short call's time.
+constexpr uint32_t kOneCtas = 8;  // of a cluster (the portable most; of 16, the GPU holds 7 at once, for 8 kv heads)
+
+// Most positions that a token of the call can see, as far as the host knows.
+inline uint64_t one_span(const AttnChunksParams &p) {
+  const uint64_t cap = (uint64_t)p.pg.max_pages * kPageLen, seen = (uint64_t)p.window + p.max_q;
+  return p.window && seen < cap ? seen : cap;
+}
+// Cluster blockIdx.x / kOneCtas takes (chunk, head); false: the chunk has no
+// rows (the same for the whole cluster).
+__device__ __forceinline__ bool one_item(const AttnChunksParams &p, Segment &s) {
+  const uint32_t item = blockIdx.x / kOneCtas;
+  s.chunk = load_chunk(p, item / p.pg.n_kv_heads);
+  if (!s.chunk.rows) return false;
+  s.tile = 0;
+  s.head = item % p.pg.n_kv_heads;
+  s.r0 = 0;
+  s.r1 = s.chunk.rows;
+  tile_range(p, s.chunk, 0, s.r1, s.lo, s.hi);
+  return true;
+}
+// The cluster's rows from the CTAs' pieces, each (max, sum) [rows] and
+// unnormalised outputs [rows][hd] in shared memory (16-byte aligned), as in
+// k_attn_join, in the order of the CTAs: the threads of all CTAs share the
+// elements, with the loads of all pieces in flight.  put(row, d, f32 x 4).
+template <uint32_t THREADS, typename Put>
+__device__ __forceinline__ void one_join(const Segment &s, uint32_t hd, const float *o, const float *ml, Put put) {
+  cluster_sync();
+  const uint32_t n4 = s.r1 * (hd / 4), per = (n4 + kOneCtas - 1) / kOneCtas, i0 = cluster_ctarank() * per;
+  for (uint32_t i = i0 + threadIdx.x; i < min(n4, i0 + per); i += THREADS) {
+    const uint32_t r = i / (hd / 4), d = (i - r * (hd / 4)) * 4;
+    float m[kOneCtas], l[kOneCtas];
+    float4 x[kOneCtas];
+#pragma unroll
+    for (uint32_t k = 0; k < kOneCtas; ++k) {
+      asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(m[k]), "=f"(l[k]) : "r"(dsmem_addr(ml + 2 * r, k)) : "memory");
+      asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+                   : "=f"(x[k].x), "=f"(x[k].y), "=f"(x[k].z), "=f"(x[k].w)
+                   : "r"(dsmem_addr(o + r * hd + d, k))
+                   : "memory");
+    }
+    float M = m[0], L = 0.0f;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (uint32_t k = 1; k < kOneCtas; ++k) M = fmaxf(M, m[k]);
+    const float Ms = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+    for (uint32_t k = 0; k < kOneCtas; ++k) {
+      const float e = exp2f(m[k] - Ms);
+      L = fmaf(l[k], e, L);
+      acc.x = fmaf(x[k].x, e, acc.x);
+      acc.y = fmaf(x[k].y, e, acc.y);
+      acc.z = fmaf(x[k].z, e, acc.z);
+      acc.w = fmaf(x[k].w, e, acc.w);
+    }
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+    put(r, d, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+  }
+  cluster_sync();  // the pieces have been read
+}
+// Launches a cluster for each of (chunk, kv head), where the GPU holds that many
+// at once; 1: it does not, -1: an error.
+template <auto kern>
+int launch_one(const AttnChunksParams &p, uint32_t threads, uint32_t smem, cudaStream_t st) {
+  static std::atomic<int> known[64];  // clusters at once, by device (0: not asked yet)
+  const uint64_t items = (uint64_t)p.n_chunks * p.pg.n_kv_heads;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(kOneCtas);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = kOneCtas;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return -1;
+  int device = 0, at_once = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return -1;
+  const bool keep = device >= 0 && device < 64;
+  if (keep) at_once = known[device].load(std::memory_order_relaxed);
+  if (!at_once) {
+    if (cudaOccupancyMaxActiveClusters(&at_once, kern, &cfg) != cudaSuccess) return -1;
+    if (keep && at_once > 0) known[device].store(at_once, std::memory_order_relaxed);
+  }
+  if (items > (uint64_t)(at_once > 0 ? at_once : 0)) return 1;
+  cfg.gridDim = dim3((uint32_t)items * kOneCtas);
+  return cudaLaunchKernelEx(&cfg, kern, p) == cudaSuccess ? 0 : -1;
+}
+
 // Split items of one launch, as k_attn_join takes them.
 struct JoinSet {
   const float *part;
@@ -230,6 +325,9 @@ struct JoinSet {
   uint32_t R, ctas;
   uint32_t parts;  // CTAs of the join to an item
 };
+// One launch for few items, each a cluster; 1: the call is not of that kind.
+int launch_one_any(const AttnChunksParams &p, cudaStream_t st);
+int launch_one_mma(const AttnChunksParams &p, cudaStream_t st);
 // The kernels; each returns its grid, or 0 where the launch failed.
 bool attn_mma_takes(const AttnChunksParams &p);
 uint32_t launch_attn_any(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st, uint32_t *R);

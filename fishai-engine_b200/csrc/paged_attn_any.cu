@@ -15,6 +15,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "paged_attn.cuh"
 
 namespace fa {
@@ -94,23 +96,20 @@ __device__ __forceinline__ void fetch(const AttnChunksParams &p, const T *base, 
 
 constexpr uint32_t any_smem(uint32_t R, uint32_t hd) { return ((R + 2 * kAnyPos) * (hd + 4) + R * (kAnyPos + 4)) * 4; }
 
-// HJ: groups of 64 head elements (hd <= 64 HJ)
+// HJ: groups of 64 head elements (hd <= 64 HJ).  A thread's rows are ty + 8 i, its
+// elements 64 j + 4 tx + e.
 template <typename T, uint32_t R, uint32_t HJ>
-__global__ void __launch_bounds__(kAnyThreads) k_attn_any(const AttnChunksParams p) {
-  extern __shared__ __align__(16) float sm[];
-  __shared__ uint64_t red[kAnyThreads / 32 + 2];
-  constexpr uint32_t RT = R / 8;
-  const uint32_t hd = p.pg.head_dim, ld = hd + 4, lds = kAnyPos + 4;
-  float *sq = sm, *sk = sq + R * ld, *sv = sk + kAnyPos * ld, *sp = sv + kAnyPos * ld;
-  const uint32_t tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-  const T *base = reinterpret_cast<const T *>(p.pg.base) + (uint64_t)p.layer * p.pg.layer_stride;
-  using W = Walk<R, kAnyPos, 0, kAnyThreads>;
-  W w;
-  w.start(p, 1, red);
-  if (tid == 0) p.desc[blockIdx.x].w = 0;
-  for (Segment s; w.next(p, s);) {
+struct AnyRows {
+  static constexpr uint32_t RT = R / 8;
+  float m[RT], l[RT], o[RT][HJ][4];
+
+  // units u, u + step, .. < n of an item
+  __device__ void run(const AttnChunksParams &p, const Segment &s, uint32_t u, uint32_t n, uint32_t step, float *sm) {
+    const uint32_t hd = p.pg.head_dim, ld = hd + 4, lds = kAnyPos + 4;
+    float *sq = sm, *sk = sq + R * ld, *sv = sk + kAnyPos * ld, *sp = sv + kAnyPos * ld;
+    const uint32_t tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+    const T *base = reinterpret_cast<const T *>(p.pg.base) + (uint64_t)p.layer * p.pg.layer_stride;
     const uint32_t *pt = p.pg.page_table + (uint64_t)s.chunk.seq * p.pg.max_pages;
-    __syncthreads();
     // Q rows; past the item's: zeros
     for (uint32_t r = tid / 32; r < R; r += kAnyThreads / 32) {  // a warp a row
       const uint32_t row = s.r0 + r, tok = row / p.rep;
@@ -121,7 +120,6 @@ __global__ void __launch_bounds__(kAnyThreads) k_attn_any(const AttnChunksParams
         if (d < hd) sq[r * ld + d] = row < s.r1 ? (float)x[d] : 0.0f;
       }
     }
-    float m[RT], l[RT], o[RT][HJ][4];
     int32_t pos[RT];  // position of each row's token
 #pragma unroll
     for (uint32_t i = 0; i < RT; ++i) {
@@ -132,7 +130,7 @@ __global__ void __launch_bounds__(kAnyThreads) k_attn_any(const AttnChunksParams
 #pragma unroll
       for (uint32_t j = 0; j < HJ; ++j) o[i][j][0] = o[i][j][1] = o[i][j][2] = o[i][j][3] = 0.0f;
     }
-    for (uint32_t u = s.u0; u < s.u1 && s.hi > s.lo; ++u) {
+    for (; u < n && s.hi > s.lo; u += step) {
       const uint32_t t0 = (s.lo / kAnyPos + u) * kAnyPos;
       __syncthreads();
       fetch<T>(p, base, pt, s, t0, sk, sv, ld, tid);
@@ -204,15 +202,31 @@ __global__ void __launch_bounds__(kAnyThreads) k_attn_any(const AttnChunksParams
         }
       }
     }
+  }
+};
+
+template <typename T, uint32_t R, uint32_t HJ>
+__global__ void __launch_bounds__(kAnyThreads) k_attn_any(const AttnChunksParams p) {
+  extern __shared__ __align__(16) float sm[];
+  __shared__ uint64_t red[kAnyThreads / 32 + 2];
+  const uint32_t hd = p.pg.head_dim, tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+  using W = Walk<R, kAnyPos, 0, kAnyThreads>;
+  W w;
+  w.start(p, 1, red);
+  if (tid == 0) p.desc[blockIdx.x].w = 0;
+  for (Segment s; w.next(p, s);) {
+    __syncthreads();
+    AnyRows<T, R, HJ> x;
+    x.run(p, s, s.u0, s.u1, 1, sm);
     const bool whole = W::whole(s);
     float *slot = W::slot(p, s);
 #pragma unroll
-    for (uint32_t i = 0; i < RT; ++i) {
+    for (uint32_t i = 0; i < R / 8; ++i) {
       const uint32_t r = ty + 8 * i, row = s.r0 + r;
       if (row >= s.r1) continue;
       if (!whole && tx == 0) {
-        slot[R * hd + 2 * r] = m[i];
-        slot[R * hd + 2 * r + 1] = l[i];
+        slot[R * hd + 2 * r] = x.m[i];
+        slot[R * hd + 2 * r + 1] = x.l[i];
       }
 #pragma unroll
       for (uint32_t j = 0; j < HJ; ++j) {
@@ -220,17 +234,47 @@ __global__ void __launch_bounds__(kAnyThreads) k_attn_any(const AttnChunksParams
         if (d >= hd) continue;
 #pragma unroll
         for (uint32_t e = 0; e < 4; ++e) {
-          if (!whole) slot[r * hd + d + e] = o[i][j][e];
+          if (!whole) slot[r * hd + d + e] = x.o[i][j][e];
           else
             put(reinterpret_cast<T *>(p.out) + (uint64_t)(s.chunk.q0 + row / p.rep) * p.os +
                     (s.head * p.rep + row % p.rep) * hd + d + e,
-                l[i] == 0.0f ? 0.0f : o[i][j][e] / l[i]);
+                x.l[i] == 0.0f ? 0.0f : x.o[i][j][e] / x.l[i]);
         }
       }
     }
     if (!whole && s.u0 == 0 && tid == 0) p.desc[blockIdx.x] = w.describe(s);
   }
   pdl_launch_dependents();
+}
+
+// few items of up to R rows: a cluster each (paged_attn.cuh)
+template <typename T, uint32_t R, uint32_t HJ>
+__global__ void __launch_bounds__(kAnyThreads) k_attn_any_one(const AttnChunksParams p) {
+  extern __shared__ __align__(16) float sm[];
+  const uint32_t hd = p.pg.head_dim, tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+  Segment s;
+  if (!one_item(p, s)) return;
+  AnyRows<T, R, HJ> x;
+  x.run(p, s, cluster_ctarank(), range_units<kAnyPos>(s.lo, s.hi), kOneCtas, sm);
+  float *o = sm + R * (hd + 4), *ml = o + R * hd;  // over K and V, which have been read
+  __syncthreads();
+#pragma unroll
+  for (uint32_t i = 0; i < R / 8; ++i) {
+    const uint32_t r = ty + 8 * i;
+    if (tx == 0) *reinterpret_cast<float2 *>(ml + 2 * r) = make_float2(x.m[i], x.l[i]);
+#pragma unroll
+    for (uint32_t j = 0; j < HJ; ++j) {
+      const uint32_t d = 64 * j + 4 * tx;
+      if (d < hd) *reinterpret_cast<float4 *>(o + r * hd + d) = make_float4(x.o[i][j][0], x.o[i][j][1], x.o[i][j][2], x.o[i][j][3]);
+    }
+  }
+  one_join<kAnyThreads>(s, hd, o, ml, [&](uint32_t r, uint32_t d, float4 y) {
+    T *out = reinterpret_cast<T *>(p.out) + (uint64_t)(s.chunk.q0 + r / p.rep) * p.os + (s.head * p.rep + r % p.rep) * hd + d;
+    put(out, y.x);
+    put(out + 1, y.y);
+    put(out + 2, y.z);
+    put(out + 3, y.w);
+  });
 }
 
 template <typename T, uint32_t R, uint32_t HJ>
@@ -246,25 +290,48 @@ uint32_t launch_hj(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st, ui
   *rows = R;
   return cudaGetLastError() == cudaSuccess ? grid : 0;
 }
-template <typename T>
-uint32_t launch_any_t(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st, uint32_t *rows) {
+template <typename T, uint32_t R, uint32_t HJ>
+struct LaunchAny {
+  static uint32_t walk(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st, uint32_t *rows) { return launch_hj<T, R, HJ>(p, n_sm, st, rows); }
+  static int one(const AttnChunksParams &p, cudaStream_t st) {
+    return launch_one<k_attn_any_one<T, R, HJ>>(p, kAnyThreads, any_smem(R, 64 * HJ), st);
+  }
+};
+// f(LaunchAny of the call's type, rows and head size)
+template <typename T, typename F>
+auto with_hd(const AttnChunksParams &p, F f) {
   const uint32_t hd = p.pg.head_dim;
-  // items of 8 rows while no chunk has more: a decode's 1 to 8 rows would leave
-  // most of 32 idle in the FMA loops
-  const bool few = (uint64_t)p.max_q * p.rep <= 8;
-  if (hd <= 64) return few ? launch_hj<T, 8, 1>(p, n_sm, st, rows) : launch_hj<T, 32, 1>(p, n_sm, st, rows);
-  if (hd <= 128) return few ? launch_hj<T, 8, 2>(p, n_sm, st, rows) : launch_hj<T, 32, 2>(p, n_sm, st, rows);
-  return few ? launch_hj<T, 8, 4>(p, n_sm, st, rows) : launch_hj<T, 32, 4>(p, n_sm, st, rows);
+  // items of 8 or 16 rows while no chunk has more: few rows would leave most of
+  // 32 idle in the FMA loops
+  const uint64_t rows = (uint64_t)p.max_q * p.rep;
+  auto with_rows = [&](auto hj) {
+    constexpr uint32_t HJ = decltype(hj)::value;
+    return rows <= 8 ? f(LaunchAny<T, 8, HJ>()) : rows <= 16 ? f(LaunchAny<T, 16, HJ>()) : f(LaunchAny<T, 32, HJ>());
+  };
+  if (hd <= 64) return with_rows(std::integral_constant<uint32_t, 1>());
+  if (hd <= 128) return with_rows(std::integral_constant<uint32_t, 2>());
+  return with_rows(std::integral_constant<uint32_t, 4>());
+}
+template <typename F>
+auto with_kind(const AttnChunksParams &p, F f) {
+  switch (p.pg.dtype) {
+    case FA_KV_F32: return with_hd<float>(p, f);
+    case FA_KV_F16: return with_hd<__half>(p, f);
+    default: return with_hd<__nv_bfloat16>(p, f);
+  }
 }
 
 }  // namespace
 
 uint32_t launch_attn_any(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st, uint32_t *R) {
-  switch (p.pg.dtype) {
-    case FA_KV_F32: return launch_any_t<float>(p, n_sm, st, R);
-    case FA_KV_F16: return launch_any_t<__half>(p, n_sm, st, R);
-    default: return launch_any_t<__nv_bfloat16>(p, n_sm, st, R);
-  }
+  return with_kind(p, [&](auto k) { return k.walk(p, n_sm, st, R); });
+}
+int launch_one_any(const AttnChunksParams &p, cudaStream_t st) {
+  if ((uint64_t)p.max_q * p.rep > 32) return 1;
+  // While a CTA has one tile: 5 sequences of 512 positions with 12 rows, 2 kv heads
+  // x 64, 13.1 us against 18.1 in two launches; of 2048 36.7 against 23.3.
+  if (one_span(p) > kOneCtas * kAnyPos) return 1;
+  return with_kind(p, [&](auto k) { return k.one(p, st); });
 }
 
 }  // namespace fa

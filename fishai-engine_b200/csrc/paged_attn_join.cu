@@ -233,7 +233,10 @@ int launch_attn_chunks(const AttnChunksParams &p, void *ws, uint32_t n_sm, cudaS
   a.rows_min = 1;
   a.rows_max = 0xFFFFFFFFu;
   JoinSet ja{a.part, a.desc, 0, 0, 0}, jb{b.part, b.desc, 0, 0, 0};
-  if (attn_mma_takes(p)) {
+  const bool mma = attn_mma_takes(p);
+  const int one = mma ? launch_one_mma(a, st) : launch_one_any(a, st);
+  if (one <= 0) return one;
+  if (mma) {
     // Up to 16 rows mma.sync keeps up with the copies of K and V; above, the
     // items of tcgen05, also where they are mostly empty: 64 sequences of 4096
     // positions with 32 and 64 rows take 200 and 208 us, and took 264 and 316

@@ -245,71 +245,21 @@ __device__ __forceinline__ void flag_bad_pages(const AttnChunksParams &p, const 
   if ((pg.page[0] >= p.pg.n_pages || pg.page[1] >= p.pg.n_pages) && p.err) atomicOr(p.err, kFlagPage);
 }
 
-// ------------------------------------------------------------ up to 16 rows
-template <typename T, uint32_t HD>
-__global__ void __launch_bounds__(kThreads, 3) k_attn_rows16(const AttnChunksParams p) {
-  extern __shared__ __align__(128) uint8_t dsm[];
-  __shared__ uint64_t red[kThreads / 32 + 2];
-  constexpr uint32_t kTileBytes = kSub * HD * 2;
-  using W = Walk<kMmaRows, kSub, 6, kThreads>;
-  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
-  const uint32_t ktile = smem_u32(dsm) + warp * 2 * kTileBytes, vtile = ktile + kTileBytes;
-  const T *base = reinterpret_cast<const T *>(p.pg.base) + (uint64_t)p.layer * p.pg.layer_stride;
-  pdl_launch_dependents();
-  W w;
-  w.start(p, 4, red);
-  if (tid == 0) p.desc[blockIdx.x].w = 0;
-  for (Segment s; w.next(p, s);) {
-    const uint32_t *pt = p.pg.page_table + (uint64_t)s.chunk.seq * p.pg.max_pages;
-    Rows<T, HD> rows;
-    rows.load(p, s, s.r0);
-    const uint32_t first = s.lo / kSub;  // sub-tile of the item's unit 0
-    uint32_t u = s.hi > s.lo ? s.u0 + warp : s.u1;
-    uint32_t t0 = (first + u) * kSub;
-    PagePair pg = look_up(pt, t0, s.lo, s.hi);
-    if (u < s.u1) {
-      flag_bad_pages(p, pg);
-      stage<T, HD>(p, base, pg, s.head, 0, t0, s.lo, s.hi, ktile, lane, 32);
-      cp_commit();
-      stage<T, HD>(p, base, pg, s.head, 1, t0, s.lo, s.hi, vtile, lane, 32);
-      cp_commit();
-    }
-    PagePair ahead = look_up(pt, t0 + 4 * kSub, s.lo, s.hi);
-    for (; u < s.u1; u += 4) {
-      const bool more = u + 4 < s.u1;
-      const uint32_t t1 = t0 + 4 * kSub;
-      float sc[kSub / 8][4];
-      cp_wait<1>();
-      __syncwarp();
-      rows.scores(ktile, sc);
-      __syncwarp();
-      pg = ahead;
-      if (more) {
-        flag_bad_pages(p, pg);
-        stage<T, HD>(p, base, pg, s.head, 0, t1, s.lo, s.hi, ktile, lane, 32);
-      }
-      cp_commit();
-      ahead = look_up(pt, t1 + 4 * kSub, s.lo, s.hi);
-      rows.softmax(p, t0, sc);
-      cp_wait<1>();
-      __syncwarp();
-      rows.add_values(vtile, sc);
-      __syncwarp();
-      if (more) stage<T, HD>(p, base, pg, s.head, 1, t1, s.lo, s.hi, vtile, lane, 32);
-      cp_commit();
-      t0 = t1;
-    }
-    cp_wait<0>();
-    rows.finish();
-    // merge the four warps: outputs [warp][16][HD + 4], then (max, sum)
+// The warps' rows to shared memory, [warp][16][HD + 4], then (max, sum); over
+// the tiles, which all warps have read
+template <uint32_t HD, uint32_t WARPS>
+struct Merge {
+  static constexpr uint32_t LD = HD + 4, kBytes = WARPS * 16 * LD * 4 + WARPS * 16 * 8;
+  float *o, *ml;
+  template <typename T>
+  __device__ Merge(uint8_t *at, const Rows<T, HD> &rows) : o(reinterpret_cast<float *>(at)), ml(o + WARPS * 16 * LD) {
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     __syncthreads();
-    constexpr uint32_t LD = HD + 4;
-    float *scr = reinterpret_cast<float *>(dsm), *ml = scr + 4 * 16 * LD;
 #pragma unroll
     for (uint32_t j = 0; j < HD / 8; ++j)
 #pragma unroll
       for (uint32_t i = 0; i < 2; ++i)
-        *reinterpret_cast<float2 *>(scr + (warp * 16 + g + 8 * i) * LD + 8 * j + 2 * c) = make_float2(rows.o[j][2 * i], rows.o[j][2 * i + 1]);
+        *reinterpret_cast<float2 *>(o + (warp * 16 + g + 8 * i) * LD + 8 * j + 2 * c) = make_float2(rows.o[j][2 * i], rows.o[j][2 * i + 1]);
     if (c == 0)
 #pragma unroll
       for (uint32_t i = 0; i < 2; ++i) {
@@ -317,37 +267,116 @@ __global__ void __launch_bounds__(kThreads, 3) k_attn_rows16(const AttnChunksPar
         ml[(warp * 16 + g + 8 * i) * 2 + 1] = rows.l[i];
       }
     __syncthreads();
+  }
+  // elements d .. d + 3 of row r, with its (max, sum), of all warps in order
+  __device__ float4 sum(uint32_t r, uint32_t d, float &M, float &L) const {
+    M = -INFINITY;
+    L = 0.0f;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (uint32_t v = 0; v < WARPS; ++v) M = fmaxf(M, ml[(v * 16 + r) * 2]);
+    const float Ms = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+    for (uint32_t v = 0; v < WARPS; ++v) {
+      const float e = ex2(ml[(v * 16 + r) * 2] - Ms);
+      const float4 x = *reinterpret_cast<const float4 *>(o + (v * 16 + r) * LD + d);
+      L = fmaf(ml[(v * 16 + r) * 2 + 1], e, L);
+      acc.x = fmaf(x.x, e, acc.x);
+      acc.y = fmaf(x.y, e, acc.y);
+      acc.z = fmaf(x.z, e, acc.z);
+      acc.w = fmaf(x.w, e, acc.w);
+    }
+    return acc;
+  }
+};
+template <typename T>
+__device__ __forceinline__ void put4(const AttnChunksParams &p, T *o, float4 x) {
+  if (p.aligned) {
+    *reinterpret_cast<uint2 *>(o) = make_uint2(pack2<T>(x.x, x.y), pack2<T>(x.z, x.w));
+  } else {
+    o[0] = round_to<T>(x.x);
+    o[1] = round_to<T>(x.y);
+    o[2] = round_to<T>(x.z);
+    o[3] = round_to<T>(x.w);
+  }
+}
+
+// A warp's sub-tiles u, u + step, .. < n of an item (from its first one on), its
+// K and V tiles the only ones it uses.  q: called once the first copies are on
+// their way.
+template <typename T, uint32_t HD, typename Q>
+__device__ __forceinline__ void walk_tiles(const AttnChunksParams &p, const T *base, const Segment &s, uint32_t u, uint32_t n, uint32_t step,
+                                           uint32_t ktile, uint32_t vtile, Rows<T, HD> &rows, Q q) {
+  const uint32_t *pt = p.pg.page_table + (uint64_t)s.chunk.seq * p.pg.max_pages;
+  const uint32_t lane = threadIdx.x & 31;
+  uint32_t t0 = (s.lo / kSub + u) * kSub;
+  PagePair pg = look_up(pt, t0, s.lo, s.hi);
+  if (u < n) {
+    flag_bad_pages(p, pg);
+    stage<T, HD>(p, base, pg, s.head, 0, t0, s.lo, s.hi, ktile, lane, 32);
+    cp_commit();
+    stage<T, HD>(p, base, pg, s.head, 1, t0, s.lo, s.hi, vtile, lane, 32);
+    cp_commit();
+  }
+  PagePair ahead = look_up(pt, t0 + step * kSub, s.lo, s.hi);
+  q();
+  for (; u < n; u += step) {
+    const bool more = u + step < n;
+    const uint32_t t1 = t0 + step * kSub;
+    float sc[kSub / 8][4];
+    cp_wait<1>();
+    __syncwarp();
+    rows.scores(ktile, sc);
+    __syncwarp();
+    pg = ahead;
+    if (more) {
+      flag_bad_pages(p, pg);
+      stage<T, HD>(p, base, pg, s.head, 0, t1, s.lo, s.hi, ktile, lane, 32);
+    }
+    cp_commit();
+    ahead = look_up(pt, t1 + step * kSub, s.lo, s.hi);
+    rows.softmax(p, t0, sc);
+    cp_wait<1>();
+    __syncwarp();
+    rows.add_values(vtile, sc);
+    __syncwarp();
+    if (more) stage<T, HD>(p, base, pg, s.head, 1, t1, s.lo, s.hi, vtile, lane, 32);
+    cp_commit();
+    t0 = t1;
+  }
+  cp_wait<0>();
+  rows.finish();
+}
+
+// ------------------------------------------------------------ up to 16 rows
+template <typename T, uint32_t HD>
+__global__ void __launch_bounds__(kThreads, 3) k_attn_rows16(const AttnChunksParams p) {
+  extern __shared__ __align__(128) uint8_t dsm[];
+  __shared__ uint64_t red[kThreads / 32 + 2];
+  constexpr uint32_t kTileBytes = kSub * HD * 2;
+  using W = Walk<kMmaRows, kSub, 6, kThreads>;
+  const uint32_t tid = threadIdx.x, warp = tid >> 5;
+  const uint32_t ktile = smem_u32(dsm) + warp * 2 * kTileBytes, vtile = ktile + kTileBytes;
+  const T *base = reinterpret_cast<const T *>(p.pg.base) + (uint64_t)p.layer * p.pg.layer_stride;
+  pdl_launch_dependents();
+  W w;
+  w.start(p, 4, red);
+  if (tid == 0) p.desc[blockIdx.x].w = 0;
+  for (Segment s; w.next(p, s);) {
+    Rows<T, HD> rows;
+    rows.load(p, s, s.r0);
+    walk_tiles<T, HD>(p, base, s, s.hi > s.lo ? s.u0 + warp : s.u1, s.u1, kThreads / 32, ktile, vtile, rows, [] {});
+    const Merge<HD, kThreads / 32> pieces(dsm, rows);
     const bool whole = W::whole(s);
     float *slot = W::slot(p, s);
     const uint32_t n_rows = s.r1 - s.r0;
     for (uint32_t i = tid; i < n_rows * (HD / 4); i += kThreads) {
       const uint32_t r = i / (HD / 4), d = i % (HD / 4) * 4;
-      float M = -INFINITY, L = 0.0f;
-      float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-      for (uint32_t v = 0; v < 4; ++v) M = fmaxf(M, ml[(v * 16 + r) * 2]);
-      const float Ms = M == -INFINITY ? 0.0f : M;
-#pragma unroll
-      for (uint32_t v = 0; v < 4; ++v) {
-        const float e = ex2(ml[(v * 16 + r) * 2] - Ms);
-        const float4 x = *reinterpret_cast<const float4 *>(scr + (v * 16 + r) * LD + d);
-        L = fmaf(ml[(v * 16 + r) * 2 + 1], e, L);
-        acc.x = fmaf(x.x, e, acc.x);
-        acc.y = fmaf(x.y, e, acc.y);
-        acc.z = fmaf(x.z, e, acc.z);
-        acc.w = fmaf(x.w, e, acc.w);
-      }
+      float M, L;
+      const float4 acc = pieces.sum(r, d, M, L);
       if (whole) {
         const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-        T *o = out_row<T>(p, s, s.r0 + r, HD) + d;
-        if (p.aligned) {
-          *reinterpret_cast<uint2 *>(o) = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
-        } else {
-          o[0] = round_to<T>(acc.x * inv);
-          o[1] = round_to<T>(acc.y * inv);
-          o[2] = round_to<T>(acc.z * inv);
-          o[3] = round_to<T>(acc.w * inv);
-        }
+        put4(p, out_row<T>(p, s, s.r0 + r, HD) + d, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
       } else {
         *reinterpret_cast<float4 *>(slot + r * HD + d) = acc;
         if (d == 0) *reinterpret_cast<float2 *>(slot + 16 * HD + 2 * r) = make_float2(M, L);
@@ -361,14 +390,70 @@ __global__ void __launch_bounds__(kThreads, 3) k_attn_rows16(const AttnChunksPar
 template <typename T, uint32_t HD>
 uint32_t launch_hd(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st) {
   // two tiles of 32 positions a warp, or the merge's 4 x 16 rows
-  constexpr uint32_t kTiles = 4 * 2 * kSub * HD * 2, kMerge = 4 * 16 * (HD + 4) * 4 + 4 * 16 * 8, kBytes = kTiles > kMerge ? kTiles : kMerge;
+  constexpr uint32_t kTiles = 4 * 2 * kSub * HD * 2, kMerge = Merge<HD, 4>::kBytes, kBytes = kTiles > kMerge ? kTiles : kMerge;
   const uint32_t grid = 3 * n_sm < kAttnMaxCtas ? 3 * n_sm : kAttnMaxCtas;
   if (cudaFuncSetAttribute(k_attn_rows16<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kBytes) != cudaSuccess) return 0;
   k_attn_rows16<T, HD><<<grid, kThreads, kBytes, st>>>(p);
   return cudaGetLastError() == cudaSuccess ? grid : 0;
 }
 
+// ------------------------------------- few items of up to 16 rows: a cluster each
+template <uint32_t HD, uint32_t WARPS>
+struct OneCfg {
+  static constexpr uint32_t kTiles = WARPS * 2 * kSub * HD * 2;  // a K and a V tile a warp
+  static constexpr uint32_t kPiece = Merge<HD, WARPS>::kBytes;   // over them the warps' pieces, behind those the CTA's
+  static constexpr uint32_t kEnd = kPiece + 16 * HD * 4 + 16 * 8, kBytes = kTiles > kEnd ? kTiles : kEnd;
+};
+template <typename T, uint32_t HD, uint32_t WARPS>
+__global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 1 : 2) k_attn_one16(const AttnChunksParams p) {
+  extern __shared__ __align__(128) uint8_t dsm[];
+  constexpr uint32_t kTileBytes = kSub * HD * 2;
+  const uint32_t tid = threadIdx.x, warp = tid >> 5;
+  const uint32_t ktile = smem_u32(dsm) + warp * 2 * kTileBytes, vtile = ktile + kTileBytes;
+  const T *base = reinterpret_cast<const T *>(p.pg.base) + (uint64_t)p.layer * p.pg.layer_stride;
+  Segment s;
+  if (!one_item(p, s)) return;
+  const uint32_t n = s.hi > s.lo ? range_units<kSub>(s.lo, s.hi) : 0;
+  Rows<T, HD> rows;
+  walk_tiles<T, HD>(p, base, s, cluster_ctarank() * WARPS + warp, n, kOneCtas * WARPS, ktile, vtile, rows, [&] { rows.load(p, s, 0); });
+  const Merge<HD, WARPS> pieces(dsm, rows);
+  float *o = reinterpret_cast<float *>(dsm + OneCfg<HD, WARPS>::kPiece), *ml = o + 16 * HD;
+  for (uint32_t i = tid; i < s.r1 * (HD / 4); i += 32 * WARPS) {
+    const uint32_t r = i / (HD / 4), d = i % (HD / 4) * 4;
+    float M, L;
+    *reinterpret_cast<float4 *>(o + r * HD + d) = pieces.sum(r, d, M, L);
+    if (d == 0) *reinterpret_cast<float2 *>(ml + 2 * r) = make_float2(M, L);
+  }
+  one_join<32 * WARPS>(s, HD, o, ml, [&](uint32_t r, uint32_t d, float4 x) { put4(p, out_row<T>(p, s, r, HD) + d, x); });
+}
+// Eight warps, one CTA an SM, or six and two CTAs: the former keep more copies in
+// flight (8 kv heads over 8192 positions 11.9 us against 15.0), the latter take
+// twice the items and are ahead where their first sub-tiles are all there is (1024
+// positions: 5.8 us against 6.4).
+template <typename T, uint32_t HD>
+int launch_one_hd(const AttnChunksParams &p, uint64_t span, cudaStream_t st) {
+  if (span > kOneCtas * 6 * kSub) {
+    const int rc = launch_one<k_attn_one16<T, HD, 8>>(p, 256, OneCfg<HD, 8>::kBytes, st);
+    if (rc <= 0) return rc;
+  }
+  return launch_one<k_attn_one16<T, HD, 6>>(p, 192, OneCfg<HD, 6>::kBytes, st);
+}
+
 }  // namespace
+
+int launch_one_mma(const AttnChunksParams &p, cudaStream_t st) {
+  if ((uint64_t)p.max_q * p.rep > kMmaRows) return 1;
+  // A cluster streams some 0.7 TB/s, so the longer the cache the more of them
+  // must run beside one another to keep up with the even split over all SMs, which
+  // costs a join.  One token, kv heads x 128, clusters against split: 8 heads over
+  // 1024, 8192, 16384 and 65536 positions 6.4, 11.9, 17.8 and 55 us against 9.8,
+  // 17.0, 21.2 and 53; 2 heads over 1024, 8192 and 32768 6.1, 11.1 and 29.7 against
+  // 9.2, 11.0 and 19.1; three sequences x 8 heads of 8192 21.6 against 26.8.
+  const uint64_t span = one_span(p), items = (uint64_t)p.n_chunks * p.pg.n_kv_heads;
+  if (span > (items >= 8 ? 16384 : 8192)) return 1;
+  if (p.pg.dtype == FA_KV_F16) return p.pg.head_dim == 64 ? launch_one_hd<__half, 64>(p, span, st) : launch_one_hd<__half, 128>(p, span, st);
+  return p.pg.head_dim == 64 ? launch_one_hd<__nv_bfloat16, 64>(p, span, st) : launch_one_hd<__nv_bfloat16, 128>(p, span, st);
+}
 
 // 16-bit types at head sizes 64 and 128; TMA counts the rows of a layer's pages
 // in 31 bits
