@@ -24,77 +24,58 @@ namespace {
 
 constexpr uint32_t kAnyThreads = 128, kAnyPos = 64;
 
-template <typename T>
-__device__ __forceinline__ void load8(const T *p, float (&x)[8]);  // 16-byte aligned
-template <>
-__device__ __forceinline__ void load8<__half>(const __half *p, float (&x)[8]) {
-  const uint4 a = *reinterpret_cast<const uint4 *>(p);
-  const __half2 *h = reinterpret_cast<const __half2 *>(&a);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = __half22float2(h[i]);
-    x[2 * i] = f.x, x[2 * i + 1] = f.y;
-  }
+// four elements, aligned to their size
+__device__ __forceinline__ float4 load4(const float *p) { return *reinterpret_cast<const float4 *>(p); }
+__device__ __forceinline__ float4 load4(const __half *p) {
+  const uint2 a = *reinterpret_cast<const uint2 *>(p);
+  const float2 x = __half22float2(*reinterpret_cast<const __half2 *>(&a.x)), y = __half22float2(*reinterpret_cast<const __half2 *>(&a.y));
+  return make_float4(x.x, x.y, y.x, y.y);
 }
-template <>
-__device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16 *p, float (&x)[8]) {
-  const uint4 a = *reinterpret_cast<const uint4 *>(p);
-  const __nv_bfloat162 *h = reinterpret_cast<const __nv_bfloat162 *>(&a);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = __bfloat1622float2(h[i]);
-    x[2 * i] = f.x, x[2 * i + 1] = f.y;
-  }
+__device__ __forceinline__ float4 load4(const __nv_bfloat16 *p) {
+  const uint2 a = *reinterpret_cast<const uint2 *>(p);
+  const float2 x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&a.x)), y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&a.y));
+  return make_float4(x.x, x.y, y.x, y.y);
 }
 __device__ __forceinline__ void put(float *p, float x) { *p = x; }
 __device__ __forceinline__ void put(__half *p, float x) { *p = __float2half_rn(x); }
 __device__ __forceinline__ void put(__nv_bfloat16 *p, float x) { *p = __float2bfloat16_rn(x); }
 
-// K and V of positions [t0, t0 + 64) to shared memory as f32; positions outside
-// the item's range and bad pages as zeros.  The tile's four pages are looked up
-// first and the copies are independent, so that they are all in flight: f32 by
-// cp.async, 16-bit types through registers.  (A look-up with each 32-byte load
-// took 19 us for a tile where this takes 8.)
-template <typename T>
-__device__ __forceinline__ void fetch(const AttnChunksParams &p, const T *base, const uint32_t *pt, const Segment &s, uint32_t t0,
-                                      float *sk, float *sv, uint32_t ld, uint32_t tid) {
-  constexpr uint32_t kV = 16 / sizeof(T);  // elements of a copy
-  const uint32_t hd = p.pg.head_dim, per_row = hd / kV, total = 2 * kAnyPos * per_row;
-  uint32_t page[kAnyPos / kPageLen];
-#pragma unroll
-  for (uint32_t j = 0; j < kAnyPos / kPageLen; ++j) {
-    const uint32_t t = t0 + j * kPageLen;
-    page[j] = t < s.hi && t + kPageLen > s.lo ? __ldg(pt + t / kPageLen) : 0u;
+// Copies of a tile's K or V rows, 16 bytes a thread and step: piece c of row r,
+// both carried along (a division a piece took longer than the copies).
+struct Copier {
+  uint32_t r0, c0, dr, dc, per_row;
+  __device__ Copier(uint32_t per_row) : per_row(per_row) {
+    r0 = threadIdx.x / per_row, c0 = threadIdx.x - r0 * per_row;
+    dr = kAnyThreads / per_row, dc = kAnyThreads - dr * per_row;
   }
-  bool bad = false;
-  uint64_t row0[kAnyPos / kPageLen];
-#pragma unroll
-  for (uint32_t j = 0; j < kAnyPos / kPageLen; ++j) {
-    bad |= page[j] >= p.pg.n_pages;
-    row0[j] = page[j] < p.pg.n_pages ? page_row(p.pg, page[j], 0, s.head, 0) : ~0ull;
-  }
-  if (bad && p.err) atomicOr(p.err, kFlagPage);
-  const uint64_t v_off = (uint64_t)p.pg.n_kv_heads * kPageLen * hd;  // V after the heads' K
-#pragma unroll 4
-  for (uint32_t i = tid; i < total; i += kAnyThreads) {
-    const uint32_t e = i / per_row, d = (i - e * per_row) * kV, is_v = e / kAnyPos, r = e % kAnyPos, t = t0 + r, j = r / kPageLen;
-    const uint64_t r0 = j == 0 ? row0[0] : j == 1 ? row0[1] : j == 2 ? row0[2] : row0[3];
-    const bool ok = t >= s.lo && t < s.hi && r0 != ~0ull;
-    const T *src = base + (ok ? r0 + is_v * v_off + (t % kPageLen) * hd + d : 0);
-    float *dst = (is_v ? sv : sk) + r * ld + d;
-    if constexpr (sizeof(T) == 4) {
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(ok ? 16u : 0u) : "memory");
-    } else {
-      float x[8] = {};
-      if (ok) load8(src, x);
-      reinterpret_cast<float4 *>(dst)[0] = make_float4(x[0], x[1], x[2], x[3]);
-      reinterpret_cast<float4 *>(dst)[1] = make_float4(x[4], x[5], x[6], x[7]);
+  // src: rows of a page from at[page of the tile] on; positions outside
+  // [lo, hi) and bad pages (~0) become zeros
+  template <typename T>
+  __device__ void copy(const T *src, const uint64_t *at, uint32_t t0, uint32_t lo, uint32_t hi, uint32_t hd, T *dst, uint32_t ld) const {
+    constexpr uint32_t kV = 16 / sizeof(T);
+    for (uint32_t r = r0, c = c0; r < kAnyPos;) {
+      const uint64_t row0 = at[r / kPageLen];
+      const bool ok = t0 + r >= lo && t0 + r < hi && row0 != ~0ull;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst + r * ld + c * kV)),
+                   "l"(ok ? src + row0 + (r % kPageLen) * hd + c * kV : src), "r"(ok ? 16u : 0u)
+                   : "memory");
+      r += dr;
+      c += dc;
+      if (c >= per_row) {
+        c -= per_row;
+        ++r;
+      }
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
   }
-  if constexpr (sizeof(T) == 4) asm volatile("cp.async.wait_all;" ::: "memory");
-}
+};
+__device__ __forceinline__ void copied_but_one() { asm volatile("cp.async.wait_group 1;" ::: "memory"); }
 
-constexpr uint32_t any_smem(uint32_t R, uint32_t hd) { return ((R + 2 * kAnyPos) * (hd + 4) + R * (kAnyPos + 4)) * 4; }
+// bytes: Q rows and weights in f32, K and V tiles in their own type, rows 16 bytes apart
+template <typename T>
+constexpr uint32_t any_smem(uint32_t R, uint32_t hd) {
+  return (R * (hd + 4) + R * (kAnyPos + 4)) * 4 + 2 * kAnyPos * (hd * (uint32_t)sizeof(T) + 16);
+}
 
 // HJ: groups of 64 head elements (hd <= 64 HJ).  A thread's rows are ty + 8 i, its
 // elements 64 j + 4 tx + e.
@@ -103,13 +84,37 @@ struct AnyRows {
   static constexpr uint32_t RT = R / 8;
   float m[RT], l[RT], o[RT][HJ][4];
 
-  // units u, u + step, .. < n of an item
+  // units u, u + step, .. < n of an item; the tile behind the one worked on is on
+  // its way: its K once the scores are formed, its V once that product is done
   __device__ void run(const AttnChunksParams &p, const Segment &s, uint32_t u, uint32_t n, uint32_t step, float *sm) {
-    const uint32_t hd = p.pg.head_dim, ld = hd + 4, lds = kAnyPos + 4;
-    float *sq = sm, *sk = sq + R * ld, *sv = sk + kAnyPos * ld, *sp = sv + kAnyPos * ld;
+    __shared__ uint64_t at[2][kAnyPos / kPageLen];  // element offsets of the tile's pages, and of the next tile's
+    const uint32_t hd = p.pg.head_dim, ld = hd + 4, lds = kAnyPos + 4, ldk = hd + 16 / sizeof(T);
+    float *sq = sm, *sp = sq + R * ld;
+    T *sk = reinterpret_cast<T *>(sp + R * lds), *sv = sk + kAnyPos * ldk;
     const uint32_t tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
     const T *base = reinterpret_cast<const T *>(p.pg.base) + (uint64_t)p.layer * p.pg.layer_stride;
+    const T *vbase = base + (uint64_t)p.pg.n_kv_heads * kPageLen * hd;  // V after the heads' K
     const uint32_t *pt = p.pg.page_table + (uint64_t)s.chunk.seq * p.pg.max_pages;
+    if (s.hi <= s.lo) n = 0;
+    const Copier copier(hd * sizeof(T) / 16);
+    // thread j < 4: page j of the tile at t0; only pages that are read are looked up
+    auto look_up = [&](uint32_t t0) -> uint32_t {
+      const uint32_t t = t0 + tid * kPageLen;
+      return tid < kAnyPos / kPageLen && t < s.hi && t + kPageLen > s.lo ? __ldg(pt + t / kPageLen) : 0u;
+    };
+    auto note = [&](uint32_t page, uint32_t which) {
+      if (tid >= kAnyPos / kPageLen) return;
+      const bool good = page < p.pg.n_pages;
+      at[which][tid] = good ? page_row(p.pg, page, 0, s.head, 0) : ~0ull;
+      if (!good && p.err) atomicOr(p.err, kFlagPage);
+    };
+    if (u < n) {
+      const uint32_t t0 = (s.lo / kAnyPos + u) * kAnyPos;
+      note(look_up(t0), 0);
+      __syncthreads();
+      copier.copy(base, at[0], t0, s.lo, s.hi, hd, sk, ldk);
+      copier.copy(vbase, at[0], t0, s.lo, s.hi, hd, sv, ldk);
+    }
     // Q rows; past the item's: zeros
     for (uint32_t r = tid / 32; r < R; r += kAnyThreads / 32) {  // a warp a row
       const uint32_t row = s.r0 + r, tok = row / p.rep;
@@ -130,10 +135,11 @@ struct AnyRows {
 #pragma unroll
       for (uint32_t j = 0; j < HJ; ++j) o[i][j][0] = o[i][j][1] = o[i][j][2] = o[i][j][3] = 0.0f;
     }
-    for (; u < n && s.hi > s.lo; u += step) {
-      const uint32_t t0 = (s.lo / kAnyPos + u) * kAnyPos;
-      __syncthreads();
-      fetch<T>(p, base, pt, s, t0, sk, sv, ld, tid);
+    for (uint32_t which = 0; u < n; u += step, which ^= 1) {
+      const uint32_t t0 = (s.lo / kAnyPos + u) * kAnyPos, t1 = t0 + step * kAnyPos;
+      const bool more = u + step < n;
+      const uint32_t ahead = more ? look_up(t1) : 0;
+      copied_but_one();
       __syncthreads();
       float a[RT][4];
 #pragma unroll
@@ -141,7 +147,7 @@ struct AnyRows {
       for (uint32_t d = 0; d < hd; d += 4) {
         float4 kk[4];
 #pragma unroll
-        for (uint32_t j = 0; j < 4; ++j) kk[j] = *reinterpret_cast<const float4 *>(sk + (tx + 16 * j) * ld + d);
+        for (uint32_t j = 0; j < 4; ++j) kk[j] = load4(sk + (tx + 16 * j) * ldk + d);
 #pragma unroll
         for (uint32_t i = 0; i < RT; ++i) {
           const float4 q = *reinterpret_cast<const float4 *>(sq + (ty + 8 * i) * ld + d);
@@ -150,6 +156,10 @@ struct AnyRows {
             a[i][j] = fmaf(q.x, kk[j].x, fmaf(q.y, kk[j].y, fmaf(q.z, kk[j].z, fmaf(q.w, kk[j].w, a[i][j]))));
         }
       }
+      if (more) note(ahead, which ^ 1);
+      __syncthreads();
+      if (more) copier.copy(base, at[which ^ 1], t1, s.lo, s.hi, hd, sk, ldk);
+      else asm volatile("cp.async.commit_group;" ::: "memory");
 #pragma unroll
       for (uint32_t i = 0; i < RT; ++i) {
         float mx = -INFINITY;
@@ -178,6 +188,7 @@ struct AnyRows {
 #pragma unroll
         for (uint32_t j = 0; j < HJ; ++j) o[i][j][0] *= f, o[i][j][1] *= f, o[i][j][2] *= f, o[i][j][3] *= f;
       }
+      copied_but_one();
       __syncthreads();
       for (uint32_t t = 0; t < kAnyPos; t += 4) {
         float4 pp[RT];
@@ -189,7 +200,7 @@ struct AnyRows {
           if (d >= hd) continue;
 #pragma unroll
           for (uint32_t e = 0; e < 4; ++e) {
-            const float4 v = *reinterpret_cast<const float4 *>(sv + (t + e) * ld + d);
+            const float4 v = load4(sv + (t + e) * ldk + d);
 #pragma unroll
             for (uint32_t i = 0; i < RT; ++i) {
               const float x = e == 0 ? pp[i].x : e == 1 ? pp[i].y : e == 2 ? pp[i].z : pp[i].w;
@@ -201,7 +212,11 @@ struct AnyRows {
           }
         }
       }
+      __syncthreads();
+      if (more) copier.copy(vbase, at[which ^ 1], t1, s.lo, s.hi, hd, sv, ldk);
+      else asm volatile("cp.async.commit_group;" ::: "memory");
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
   }
 };
 
@@ -256,7 +271,7 @@ __global__ void __launch_bounds__(kAnyThreads) k_attn_any_one(const AttnChunksPa
   if (!one_item(p, s)) return;
   AnyRows<T, R, HJ> x;
   x.run(p, s, cluster_ctarank(), range_units<kAnyPos>(s.lo, s.hi), kOneCtas, sm);
-  float *o = sm + R * (hd + 4), *ml = o + R * hd;  // over K and V, which have been read
+  float *o = sm, *ml = o + R * hd;  // over Q and the weights, which have been read
   __syncthreads();
 #pragma unroll
   for (uint32_t i = 0; i < R / 8; ++i) {
@@ -279,8 +294,8 @@ __global__ void __launch_bounds__(kAnyThreads) k_attn_any_one(const AttnChunksPa
 
 template <typename T, uint32_t R, uint32_t HJ>
 uint32_t launch_hj(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st, uint32_t *rows) {
-  const uint32_t smem = any_smem(R, p.pg.head_dim);
-  if (cudaFuncSetAttribute(k_attn_any<T, R, HJ>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)any_smem(R, 64 * HJ)) !=
+  const uint32_t smem = any_smem<T>(R, p.pg.head_dim);
+  if (cudaFuncSetAttribute(k_attn_any<T, R, HJ>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)any_smem<T>(R, 64 * HJ)) !=
       cudaSuccess)
     return 0;
   uint32_t per_sm = 224 * 1024 / (smem + 1024);
@@ -294,7 +309,7 @@ template <typename T, uint32_t R, uint32_t HJ>
 struct LaunchAny {
   static uint32_t walk(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st, uint32_t *rows) { return launch_hj<T, R, HJ>(p, n_sm, st, rows); }
   static int one(const AttnChunksParams &p, cudaStream_t st) {
-    return launch_one<k_attn_any_one<T, R, HJ>>(p, kAnyThreads, any_smem(R, 64 * HJ), st);
+    return launch_one<k_attn_any_one<T, R, HJ>>(p, kAnyThreads, any_smem<T>(R, 64 * HJ), st);
   }
 };
 // f(LaunchAny of the call's type, rows and head size)
