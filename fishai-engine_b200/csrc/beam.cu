@@ -10,10 +10,13 @@
 // bits and picks the k best of beams x ranges x k candidates.
 //
 // Candidates of a range: what beats the k-th best of the list so far goes to a
-// buffer, after one barrier a tile of 4096 logits that counts the threads which
-// have some; the list is made anew, by counting ranks, when the buffer might
-// overflow and at the end.  (Making it anew at every tile that had a candidate:
-// 39 us for 256 rows of 128256, against 37 us so.)
+// buffer, and the list is made anew, by counting ranks, after the first tile of
+// 4096 logits and then after groups of 1, 2, 4, .. tiles: in random order each
+// group has about k candidates.  Within a group nothing waits for other warps; a
+// group that fills the buffer (rows that rise) is gone through once more, tile by
+// tile.  256 rows of 128256 f32, k = 8: 35 us, of which the stream of logits is 24
+// (5.4 TB/s), the first tile, the lists and the pick the rest; bf16 36, k = 64 101.
+// (A barrier a tile and a list whenever the buffer might overflow: 41, 63 and 111.)
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -67,16 +70,43 @@ struct Raw {
     T e[4];
   } g[4];
 };
-template <typename T, bool VEC>
+template <typename T>
 __device__ __forceinline__ void load_tile(const T *row, uint32_t v0, uint32_t end, Raw<T> &raw) {
 #pragma unroll
   for (uint32_t j = 0; j < 4; ++j) {
     const uint32_t v = v0 + (j * kScanThreads + threadIdx.x) * 4;
-    if (VEC && v + 4 <= end) {
-      raw.g[j] = *reinterpret_cast<const typename Raw<T>::T4 *>(row + v);
-    } else {
 #pragma unroll
-      for (uint32_t e = 0; e < 4; ++e) raw.g[j].e[e] = v + e < end ? row[v + e] : (T)(-INFINITY);
+    for (uint32_t e = 0; e < 4; ++e) raw.g[j].e[e] = v + e < end ? row[v + e] : (T)(-INFINITY);
+  }
+}
+
+// The same to a slot of shared memory, by cp.async where rows are aligned to four
+// elements; a thread reads only what it copied, so its own wait is all it needs.
+template <typename T>
+__device__ __forceinline__ void stage_tile(const T *row, uint32_t v0, uint32_t end, Raw<T> *slot) {
+  using T4 = typename Raw<T>::T4;
+  T4 *to = reinterpret_cast<T4 *>(slot) + threadIdx.x;
+  const T *from = row + v0 + threadIdx.x * 4;
+  auto copy = [&](uint32_t j) {
+    if constexpr (sizeof(T) == 4)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to + j * kScanThreads)), "l"(from + j * kScanThreads * 4) : "memory");
+    else
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(to + j * kScanThreads)), "l"(from + j * kScanThreads * 4) : "memory");
+  };
+  if (v0 + kTile <= end) {
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j) copy(j);
+  } else if (v0 < end) {
+    for (uint32_t j = 0; j < 4; ++j) {
+      const uint32_t v = v0 + (j * kScanThreads + threadIdx.x) * 4;
+      if (v + 4 <= end) {
+        copy(j);
+        continue;
+      }
+      T4 x;
+#pragma unroll
+      for (uint32_t e = 0; e < 4; ++e) x.e[e] = v + e < end ? row[v + e] : (T)(-INFINITY);
+      to[j * kScanThreads] = x;
     }
   }
 }
@@ -85,7 +115,8 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(kScanThreads, 4) k_beam_scan(const BeamParams p) {
   pdl_launch_dependents();
   __shared__ __align__(16) unsigned long long tops[kScanThreads];
-  __shared__ unsigned long long list[2][kBeamMaxK], buf[kBuf + kBeamMaxK];
+  __shared__ unsigned long long list[2][kBeamMaxK];
+  __shared__ __align__(16) unsigned long long buf[kBuf + kBeamMaxK + 2];
   __shared__ uint32_t n_buf, n_list;
   __shared__ unsigned long long bound;
   __shared__ float wm[kScanThreads / 32], wsum[kScanThreads / 32];
@@ -93,26 +124,35 @@ __global__ void __launch_bounds__(kScanThreads, 4) k_beam_scan(const BeamParams 
   const uint32_t begin = split * p.per, end = min(p.vocab, begin + p.per);
   const T *x_row = reinterpret_cast<const T *>(p.logits) + row * p.ld;
   const bool open = isfinite(p.scores[row]) && !(p.done && p.done[row]);
+  // the next tile, on its way over the work on one (two of them: 38 -> 41 us for
+  // 256 rows of 128256)
+  __shared__ __align__(16) Raw<T> slot[VEC ? kScanThreads : 1];
   Raw<T> ahead;
-  if (open) load_tile<T, VEC>(x_row, begin, end, ahead);
+  if (open) {
+    if constexpr (VEC) stage_tile(x_row, begin, end, slot);
+    else load_tile(x_row, begin, end, ahead);
+  }
   for (uint32_t i = tid; i < K; i += kScanThreads) list[0][i] = 0;
   if (tid == 0) n_buf = n_list = 0;
   if (!open) return;
   uint32_t cur = 0;
   float m = -INFINITY, s = 0.0f, kv = -INFINITY;  // kv: the list's k-th value
   __syncthreads();
-  uint32_t pend = 0;  // entries of the buffer, at most
   // The list and the buffer, ranked by counting (all keys differ), become the
   // list; the buffer is empty after it.  Starts with the buffer complete.
   auto flush = [&] {
     const uint32_t n = n_buf, n_old = n_list, all = n + n_old;
     if (tid < n_old) buf[n + tid] = list[cur][tid];
     if (tid >= 64 && tid < 64 + K) list[cur ^ 1][tid - 64] = 0;
+    if (tid == 128) buf[all] = 0;
     __syncthreads();
     for (uint32_t i = tid; i < all; i += kScanThreads) {
       const unsigned long long c = buf[i];
       uint32_t rank = 0;
-      for (uint32_t j = 0; j < all; ++j) rank += buf[j] > c;
+      for (uint32_t j = 0; j < all; j += 2) {
+        const ulonglong2 o = *reinterpret_cast<const ulonglong2 *>(buf + j);
+        rank += (o.x > c) + (o.y > c);
+      }
       if (rank < K) list[cur ^ 1][rank] = c;
     }
     if (tid == 0) {
@@ -121,23 +161,41 @@ __global__ void __launch_bounds__(kScanThreads, 4) k_beam_scan(const BeamParams 
     }
     __syncthreads();
     cur ^= 1;
-    pend = 0;
     const unsigned long long kth = list[cur][K - 1];
     kv = kth ? key_float((uint32_t)(kth >> 32)) : -INFINITY;
   };
-  for (uint32_t v0 = begin; v0 < end; v0 += kTile) {
-    float x[kScanElems];
+  float x[kScanElems], t;  // a tile's values of the thread, and their largest
+  auto largest = [&] {
+    t = x[0];
+#pragma unroll
+    for (uint32_t i = 1; i + 1 < kScanElems; i += 2) t = fmaxf(t, fmaxf(x[i], x[i + 1]));
+    t = fmaxf(t, x[kScanElems - 1]);
+  };
+  auto clean = [&] {
+#pragma unroll
+    for (uint32_t i = 0; i < kScanElems; ++i) x[i] = x[i] == x[i] ? fminf(x[i], FLT_MAX) : -INFINITY;
+  };
+  auto take = [&](const Raw<T> &raw) {
 #pragma unroll
     for (uint32_t j = 0; j < 4; ++j)
 #pragma unroll
-      for (uint32_t e = 0; e < 4; ++e) x[4 * j + e] = (float)ahead.g[j].e[e];
-    if (v0 + kTile < end) load_tile<T, VEC>(x_row, v0 + kTile, end, ahead);  // in flight over the work on this one
-    float t, add;
-    for (;;) {  // a second time where there is a NaN or +inf among the 16
-      t = x[0];
+      for (uint32_t e = 0; e < 4; ++e) x[4 * j + e] = (float)raw.g[j].e[e];
+  };
+  // the next tile to x and t, and into (m, s); the one behind it on its way
+  auto next = [&](uint32_t v0) {
+    if constexpr (VEC) {
+      asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll
-      for (uint32_t i = 1; i + 1 < kScanElems; i += 2) t = fmaxf(t, fmaxf(x[i], x[i + 1]));
-      t = fmaxf(t, x[kScanElems - 1]);
+      for (uint32_t j = 0; j < 4; ++j) ahead.g[j] = reinterpret_cast<const typename Raw<T>::T4 *>(slot)[j * kScanThreads + tid];
+      take(ahead);
+      stage_tile(x_row, v0 + kTile, end, slot);
+    } else {
+      take(ahead);
+      if (v0 + kTile < end) load_tile(x_row, v0 + kTile, end, ahead);
+    }
+    float add;
+    for (;;) {  // a second time where there is a NaN or +inf among the 16
+      largest();
       const float r = t == -INFINITY ? 0.0f : t;
       const uint64_t less = pair(-r, -r), l2e = pair(kLog2e, kLog2e);
       uint64_t a = 0;
@@ -151,8 +209,7 @@ __global__ void __launch_bounds__(kScanThreads, 4) k_beam_scan(const BeamParams 
       unpair(a, a0, a1);
       add = a0 + a1;
       if (add == add) break;  // +inf - +inf is NaN too
-#pragma unroll
-      for (uint32_t i = 0; i < kScanElems; ++i) x[i] = x[i] == x[i] ? fminf(x[i], FLT_MAX) : -INFINITY;
+      clean();
     }
     if (t > m) {
       s = fmaf(s, ex2((m - t) * kLog2e), add);
@@ -160,46 +217,43 @@ __global__ void __launch_bounds__(kScanThreads, 4) k_beam_scan(const BeamParams 
     } else if (t != -INFINITY) {
       s = fmaf(add, ex2((t - m) * kLog2e), s);
     }
-    // What beats the list goes to the buffer (a later token of an equal value
-    // does not beat it).
+  };
+  // what beats the list goes to the buffer (a later token of an equal value does
+  // not beat it), as far as it has room
+  auto append = [&](uint32_t v0, unsigned long long low) {
+    if (t > kv) {
+#pragma unroll
+      for (uint32_t i = 0; i < kScanElems; ++i)
+        if (x[i] > kv) {
+          const unsigned long long c = cand_key(x[i], v0 + (i / 4 * kScanThreads + tid) * 4 + i % 4);
+          if (c < low) continue;
+          const uint32_t to = atomicAdd(&n_buf, 1u);
+          if (to < kBuf) buf[to] = c;
+        }
+    }
+  };
+  // a tile by itself, however many of its values beat the list; starts and ends
+  // with an empty buffer
+  auto choose = [&](uint32_t v0) {
+    const uint32_t n_tops = __syncthreads_count(t > kv);
+    if (!n_tops) return;
     unsigned long long low = 1;
-    auto append = [&] {
-      if (t > kv) {
+    if (n_tops * kScanElems > kBuf) {
+      // Many (the first tile, rising rows): bounded from below by the least of the
+      // largest values of as many groups of threads as there are to choose: 8
+      // warps, or 64 groups of 4 lanes.
+      float g = t;
+      const uint32_t span = K <= kScanThreads / 32 ? 32 : 4;
+      for (uint32_t o = 1; o < span; o <<= 1) g = fmaxf(g, __shfl_xor_sync(0xFFFFFFFFu, g, o));
+      for (uint32_t o = span; o < 32; o <<= 1) g = fminf(g, __shfl_xor_sync(0xFFFFFFFFu, g, o));
+      if (tid % 32 == 0) tops[tid / 32] = float_key(g);
+      __syncthreads();
+      unsigned long long v = tops[0];
 #pragma unroll
-        for (uint32_t i = 0; i < kScanElems; ++i)
-          if (x[i] > kv) {
-            const unsigned long long c = cand_key(x[i], v0 + (i / 4 * kScanThreads + tid) * 4 + i % 4);
-            if (c < low) continue;
-            const uint32_t to = atomicAdd(&n_buf, 1u);
-            if (to < kBuf) buf[to] = c;
-          }
-      }
-    };
-    uint32_t n_tops = __syncthreads_count(t > kv);
-    if (!n_tops) continue;
-    if (pend + n_tops * kScanElems > kBuf) {
-      flush();
-      n_tops = __syncthreads_count(t > kv);
+      for (uint32_t i = 1; i < kScanThreads / 32; ++i) v = min(v, tops[i]);
+      low = max(v << 32, 1ull);
     }
-    if (n_tops * kScanElems <= kBuf) {
-      append();
-      pend += n_tops * kScanElems;
-      continue;
-    }
-    // Many (the first tile, rising rows): bounded from below by the least of the
-    // largest values of as many groups of threads as there are to choose: 8
-    // warps, or 64 groups of 4 lanes.
-    float g = t;
-    const uint32_t span = K <= kScanThreads / 32 ? 32 : 4;
-    for (uint32_t o = 1; o < span; o <<= 1) g = fmaxf(g, __shfl_xor_sync(0xFFFFFFFFu, g, o));
-    for (uint32_t o = span; o < 32; o <<= 1) g = fminf(g, __shfl_xor_sync(0xFFFFFFFFu, g, o));
-    if (tid % 32 == 0) tops[tid / 32] = float_key(g);
-    __syncthreads();
-    unsigned long long v = tops[0];
-#pragma unroll
-    for (uint32_t i = 1; i < kScanThreads / 32; ++i) v = min(v, tops[i]);
-    low = max(v << 32, 1ull);
-    append();
+    append(v0, low);
     __syncthreads();
     if (n_buf > kBuf) {
       // still too many: the exact bound, the k-th largest of the threads'
@@ -221,14 +275,39 @@ __global__ void __launch_bounds__(kScanThreads, 4) k_beam_scan(const BeamParams 
       if (best && above == K - 1) bound = best;  // n_tops > 64 >= K: one thread's
       if (tid == 0) n_buf = 0;
       __syncthreads();
-      low = bound;
-      append();
+      append(v0, bound);
       __syncthreads();
     }
     flush();
+  };
+  next(begin);
+  choose(begin);
+  uint32_t group = 1;
+  for (uint32_t v0 = begin + kTile; v0 < end; v0 += group * kTile, group *= 2) {
+    const uint32_t g_end = min(end, v0 + group * kTile);
+    bool some = false;
+    for (uint32_t v = v0; v < g_end; v += kTile) {
+      next(v);
+      some = some || t > kv;
+      append(v, 1);
+    }
+    if (!__syncthreads_count(some)) continue;
+    if (n_buf <= kBuf) {
+      flush();
+      continue;
+    }
+    // more than the buffer holds: the group again, tile by tile
+    __syncthreads();
+    if (tid == 0) n_buf = 0;
+    for (uint32_t v = v0; v < g_end; v += kTile) {
+      Raw<T> raw;
+      load_tile(x_row, v, g_end, raw);
+      take(raw);
+      clean();
+      largest();
+      choose(v);
+    }
   }
-  __syncthreads();
-  flush();
   // the range's (max, sum), warps then lanes in a fixed order
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
