@@ -240,6 +240,46 @@ def test_attention_many_chunks(t):
 
 
 @pytest.mark.parametrize("t", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("heads,kvh,hd", [(2, 1, 64), (12, 3, 128), (16, 2, 80), (4, 4, 256)])
+@pytest.mark.parametrize("qs,kvs,window", [([1], [511], 0), ([2], [2], 0), ([1, 0, 1], [130, 9, 1], 0), ([2, 1], [0, 700], 0),
+                                           ([1, 2], [90, 1], 33), ([1], [8000], 0), ([1], [40], 1)])
+def test_attention_of_few_chunks_in_a_small_and_a_large_table(t, heads, kvh, hd, qs, kvs, window):
+    """the kernels for short caches and those for long ones (the table's width decides), rows that see nothing among them"""
+    dtype = R.TYPES[t]
+    pages, table = R.make_cache(kvs, 2, kvh, hd, dtype, 41, junk=10 ** 6)
+    wide = torch.full((len(kvs), 1100), 10 ** 6, dtype=torch.int32, device="cuda")
+    wide[:, : table.shape[1]] = table
+    start = [sum(qs[:i]) for i in range(len(qs) + 1)]
+    q = randn(9, start[-1] + 1, heads * hd, dtype=dtype)
+    want, tol = R.attention(pages, table, 1, q, i32(start), i32(kvs), None, heads, 0.0, window)
+    for tb in (table, wide):
+        err = torch.zeros(1, dtype=torch.int32, device="cuda")
+        out = attn(pages, tb, q, start, kvs, heads, max_q=max(qs), window=window, layer=1, out=torch.full_like(q, 7.0), err=err)
+        assert int(err) == 0 and bool((out[start[-1]:] == 7.0).all())
+        got = out[: start[-1]].double().view(-1, heads, hd)
+        assert bool(((got - want[: start[-1]]).abs() <= tol[: start[-1]]).all())
+
+
+@pytest.mark.parametrize("t", ["f16", "f32"])
+def test_attention_refuses_and_flags_in_a_small_table_too(t):
+    """a chunk that is refused beside one that is not, and a page out of range, where each item is a cluster"""
+    dtype = R.TYPES[t]
+    pages, table = R.make_cache([40, 50], 1, 2, 64, dtype, 42)
+    q = randn(10, 4, 4 * 64, dtype=dtype)
+    good = attn(pages, table, q, [0, 1, 2], [40, 50], 4)
+    for start, lens, seqs, flag in (([0, 1, 2], [40, 10 ** 6], None, paged.FLAG_RANGE), ([0, 1, 2], [40, 50], [0, 2], paged.FLAG_RANGE),
+                                    ([0, 1, 9], [40, 50], None, paged.FLAG_RANGE)):
+        err, out = torch.zeros(1, dtype=torch.int32, device="cuda"), torch.full_like(q, 7.0)
+        attn(pages, table, q, start, lens, 4, max_q=1, seqs=seqs, out=out, err=err)
+        assert int(err) == flag and same_bits(out[:1], good[:1]) and bool((out[1:] == 7.0).all())
+    bad = table.clone()
+    bad[1, 2] = pages.shape[1]
+    err, out = torch.zeros(1, dtype=torch.int32, device="cuda"), torch.full_like(q, 7.0)
+    attn(pages, bad, q, [0, 1, 2], [40, 50], 4, out=out, err=err)
+    assert int(err) == paged.FLAG_PAGE and same_bits(out[:1], good[:1]) and bool((out[2:] == 7.0).all())
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16", "f32"])
 def test_attention_scale_and_sharp_scores(t):
     attn_check([3, 200], [300, 260], 8, 2, 64, R.TYPES[t], scale=1.5, seed=10)
     attn_check([3, 200], [300, 260], 8, 2, 64, R.TYPES[t], scale=0.001, seed=10)
