@@ -14,9 +14,10 @@
 // 4096 logits and then after groups of 1, 2, 4, .. tiles: in random order each
 // group has about k candidates.  Within a group nothing waits for other warps; a
 // group that fills the buffer (rows that rise) is gone through once more, tile by
-// tile.  256 rows of 128256 f32, k = 8: 35 us, of which the stream of logits is 24
-// (5.4 TB/s), the first tile, the lists and the pick the rest; bf16 36, k = 64 101.
-// (A barrier a tile and a list whenever the buffer might overflow: 41, 63 and 111.)
+// tile.  256 rows of 128256 f32, k = 8: 30 us, of which the stream of logits is 24
+// (5.4 TB/s), the first tile, the lists and the pick the rest; bf16 35, k = 64 104.
+// (A barrier a tile, a list whenever the buffer might overflow and a pick in k
+// rounds: 41, 63 and 111.)
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -373,6 +374,9 @@ __global__ void __launch_bounds__(kPickThreads) k_beam_pick(const BeamParams p) 
   __shared__ Best wbest[2][kWarps];
   __shared__ uint32_t wthread[2][kWarps];
   __shared__ Best won[kBeamMaxK];
+  __shared__ __align__(16) unsigned long long hi[kPickThreads];  // candidates, where there are as many as threads at most
+  __shared__ unsigned long long mid[kPickThreads];
+  __shared__ uint32_t lo[kPickThreads];
   const uint32_t b = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, NB = p.n_beams, K = p.k;
   // the inputs, which the scan does not write: before it ends
   for (uint32_t j = tid; j < NB; j += kPickThreads) {
@@ -411,6 +415,35 @@ __global__ void __launch_bounds__(kPickThreads) k_beam_pick(const BeamParams p) 
     if (kind[j] == 2 && i == j * each) return {double_key(base[j]), (unsigned long long)~j << 32, ~p.pad};
     return {0, 0, 0};
   };
+  auto write = [&](uint32_t r, const Best &w) {
+    const bool some = w.hi != 0;
+    const uint32_t parent = some ? ~(uint32_t)(w.mid >> 32) : r % NB, token = some ? ~w.lo : p.pad;
+    const uint64_t o = (uint64_t)b * K + r;
+    p.out_scores[o] = some ? (float)key_double(w.hi) : -INFINITY;
+    p.out_parents[o] = parent;
+    p.out_tokens[o] = token;
+    if (p.out_done) p.out_done[o] = !some || kind[parent] == 2 || token == p.eos;
+  };
+  if (N <= kPickThreads) {
+    // a candidate a thread: its place is the number of better ones (all differ).
+    // Counting takes 0.3 us for 128, a round below as long.
+    const Best c = tid < N ? make(tid, raw[0]) : Best{0, 0, 0};
+    hi[tid] = c.hi;
+    mid[tid] = c.mid;
+    lo[tid] = c.lo;
+    const uint32_t found = __syncthreads_count(c.hi != 0);
+    uint32_t place = 0, same = 0;
+    for (uint32_t j = 0; j < N; j += 2) {  // an odd N: hi[N] is 0
+      const ulonglong2 x = *reinterpret_cast<const ulonglong2 *>(hi + j);
+      place += (x.x > c.hi) + (x.y > c.hi);
+      same += (x.x == c.hi) + (x.y == c.hi);
+    }
+    if (c.hi && same > 1)
+      for (uint32_t j = 0; j < N; ++j) place += hi[j] == c.hi && (mid[j] > c.mid || (mid[j] == c.mid && lo[j] > c.lo));
+    if (c.hi && place < K) write(place, c);
+    if (tid >= found && tid < K) write(tid, Best{0, 0, 0});
+    return;
+  }
   Best held[kHold];
 #pragma unroll
   for (uint32_t h = 0; h < kHold; ++h) {
@@ -451,16 +484,7 @@ __global__ void __launch_bounds__(kPickThreads) k_beam_pick(const BeamParams p) 
     if (tid == wthread[buf][l]) mine = scan(top);
   }
   __syncthreads();
-  for (uint32_t r = tid; r < K; r += kPickThreads) {
-    const Best w = won[r];
-    const bool some = w.hi != 0;
-    const uint32_t parent = some ? ~(uint32_t)(w.mid >> 32) : r % NB, token = some ? ~w.lo : p.pad;
-    const uint64_t o = (uint64_t)b * K + r;
-    p.out_scores[o] = some ? (float)key_double(w.hi) : -INFINITY;
-    p.out_parents[o] = parent;
-    p.out_tokens[o] = token;
-    if (p.out_done) p.out_done[o] = !some || kind[parent] == 2 || token == p.eos;
-  }
+  for (uint32_t r = tid; r < K; r += kPickThreads) write(r, won[r]);
 }
 
 template <typename T>
