@@ -14,8 +14,8 @@
 // 4096 logits and then after groups of 1, 2, 4, .. tiles: in random order each
 // group has about k candidates.  Within a group nothing waits for other warps; a
 // group that fills the buffer (rows that rise) is gone through once more, tile by
-// tile.  256 rows of 128256 f32, k = 8: 30 us, of which the stream of logits is 24
-// (5.4 TB/s), the first tile, the lists and the pick the rest; bf16 35, k = 64 104.
+// tile.  256 rows of 128256 f32, k = 8: 31 us, of which the stream of logits is 24
+// (5.4 TB/s), the first tile, the lists and the pick the rest; bf16 35, k = 64 62.
 // (A barrier a tile, a list whenever the buffer might overflow and a pick in k
 // rounds: 41, 63 and 111.)
 #include <cuda_bf16.h>
@@ -238,46 +238,45 @@ __global__ void __launch_bounds__(kScanThreads, 4) k_beam_scan(const BeamParams 
   auto choose = [&](uint32_t v0) {
     const uint32_t n_tops = __syncthreads_count(t > kv);
     if (!n_tops) return;
-    unsigned long long low = 1;
-    if (n_tops * kScanElems > kBuf) {
-      // Many (the first tile, rising rows): bounded from below by the least of the
-      // largest values of as many groups of threads as there are to choose: 8
-      // warps, or 64 groups of 4 lanes.
-      float g = t;
-      const uint32_t span = K <= kScanThreads / 32 ? 32 : 4;
-      for (uint32_t o = 1; o < span; o <<= 1) g = fmaxf(g, __shfl_xor_sync(0xFFFFFFFFu, g, o));
-      for (uint32_t o = span; o < 32; o <<= 1) g = fminf(g, __shfl_xor_sync(0xFFFFFFFFu, g, o));
-      if (tid % 32 == 0) tops[tid / 32] = float_key(g);
-      __syncthreads();
-      unsigned long long v = tops[0];
+    const bool many = n_tops * kScanElems > kBuf;  // the first tile, rising rows
+    for (bool exact = many && K > kScanThreads / 32;; exact = true) {
+      unsigned long long low = 1;
+      if (exact) {
+        // the k-th largest of the threads' largest, which at most 16 k elements reach
+        unsigned long long best = 0;
+        if (t > kv) {
 #pragma unroll
-      for (uint32_t i = 1; i < kScanThreads / 32; ++i) v = min(v, tops[i]);
-      low = max(v << 32, 1ull);
-    }
-    append(v0, low);
-    __syncthreads();
-    if (n_buf > kBuf) {
-      // still too many: the exact bound, the k-th largest of the threads'
-      // largest, which at most 16 k elements reach
-      unsigned long long best = 0;
-      if (t > kv) {
-#pragma unroll
-        for (int i = kScanElems - 1; i >= 0; --i)
-          if (x[i] == t) best = cand_key(t, v0 + (i / 4 * kScanThreads + tid) * 4 + i % 4);
-      }
-      tops[tid] = best;
-      __syncthreads();
-      uint32_t above = 0;
+          for (int i = kScanElems - 1; i >= 0; --i)
+            if (x[i] == t) best = cand_key(t, v0 + (i / 4 * kScanThreads + tid) * 4 + i % 4);
+        }
+        tops[tid] = best;
+        if (tid == 0) n_buf = 0;
+        __syncthreads();
+        uint32_t above = 0;
 #pragma unroll 8
-      for (uint32_t i = 0; i < kScanThreads; i += 2) {
-        const ulonglong2 o = *reinterpret_cast<const ulonglong2 *>(tops + i);
-        above += (o.x > best) + (o.y > best);
+        for (uint32_t i = 0; i < kScanThreads; i += 2) {
+          const ulonglong2 o = *reinterpret_cast<const ulonglong2 *>(tops + i);
+          above += (o.x > best) + (o.y > best);
+        }
+        if (best && above == K - 1) bound = best;  // n_tops > 64 >= K: one thread's
+        __syncthreads();
+        low = bound;
+      } else if (many) {
+        // the least of the warps' largest, which 8 elements reach
+        float g = t;
+#pragma unroll
+        for (uint32_t o = 16; o; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xFFFFFFFFu, g, o));
+        if (tid % 32 == 0) tops[tid / 32] = float_key(g);
+        __syncthreads();
+        unsigned long long v = tops[0];
+#pragma unroll
+        for (uint32_t i = 1; i < kScanThreads / 32; ++i) v = min(v, tops[i]);
+        low = max(v << 32, 1ull);
       }
-      if (best && above == K - 1) bound = best;  // n_tops > 64 >= K: one thread's
-      if (tid == 0) n_buf = 0;
+      append(v0, low);
       __syncthreads();
-      append(v0, bound);
-      __syncthreads();
+      if (exact || n_buf <= kBuf) break;
+      __syncthreads();  // still too many
     }
     flush();
   };
@@ -367,16 +366,26 @@ __device__ __forceinline__ uint32_t best_lane(const Best &x) {
   return __ffs(in) - 1;
 }
 
+// The ranges' lists stand in descending order.  Of the threads' best candidates
+// (each thread has some of the lists' first ones, or of all) the k-th is a bound
+// that at least k candidates reach; what reaches it, from each list's beginning,
+// goes to shared memory, and a candidate's place is the number of better ones.
+// (k rounds of the best of the threads' best, each followed by a scan: 1 x 12
+// beams, k = 16: 161 us, 19 so; 1 x 64, k = 64: 2.9 ms, 50 so.)
+constexpr uint32_t kPlaced = 1024;  // candidates that are placed by counting; in random order some 2 k reach the bound
+template <bool MANY>  // more candidates than threads
 __global__ void __launch_bounds__(kPickThreads) k_beam_pick(const BeamParams p) {
-  constexpr uint32_t kWarps = kPickThreads / 32, kHold = 4;  // candidates a thread holds
+  constexpr uint32_t kWarps = kPickThreads / 32, kHold = MANY ? 8 : 1, kRoom = MANY ? kPlaced : kPickThreads;
   __shared__ double base[kBeamMaxBeams], lse[kBeamMaxBeams];  // score, log sum exp
   __shared__ uint32_t kind[kBeamMaxBeams];                    // 0 out, 1 open, 2 done
+  __shared__ __align__(16) unsigned long long hi[kRoom + 2];
+  __shared__ unsigned long long mid[kRoom];
+  __shared__ uint32_t lo[kRoom];
+  __shared__ uint32_t bound, n_placed, n_reach;
+  __shared__ __align__(16) uint32_t tops[MANY ? kPickThreads : 1];
+  __shared__ uint16_t reach[MANY ? kBeamMaxBeams * kBeamMaxSplits : 1];  // lists
   __shared__ Best wbest[2][kWarps];
   __shared__ uint32_t wthread[2][kWarps];
-  __shared__ Best won[kBeamMaxK];
-  __shared__ __align__(16) unsigned long long hi[kPickThreads];  // candidates, where there are as many as threads at most
-  __shared__ unsigned long long mid[kPickThreads];
-  __shared__ uint32_t lo[kPickThreads];
   const uint32_t b = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, NB = p.n_beams, K = p.k;
   // the inputs, which the scan does not write: before it ends
   for (uint32_t j = tid; j < NB; j += kPickThreads) {
@@ -385,14 +394,18 @@ __global__ void __launch_bounds__(kPickThreads) k_beam_pick(const BeamParams p) 
     base[j] = sc;
     kind[j] = !isfinite(sc) ? 0 : dn ? 2 : 1;
   }
-  const uint32_t each = p.splits * K, N = NB * each;
+  const uint32_t each = p.splits * K, N = NB * each, lists = NB * p.splits;
   const uint2 *cand = p.cand + (uint64_t)b * N;
   pdl_wait();
+  // the thread's candidates tid, tid + 256, ..; the first ones of lists where
+  // there are enough of them (2048 at most)
+  const bool heads = MANY && lists >= kPickThreads;
+  const uint32_t step = heads ? K : 1, have = heads ? lists : N;
   uint2 raw[kHold];
 #pragma unroll
   for (uint32_t h = 0; h < kHold; ++h) {
     const uint32_t i = tid + h * kPickThreads;
-    raw[h] = i < N ? __ldcg(cand + i) : make_uint2(0, 0);  // of a beam that is not open: not used
+    raw[h] = i < have ? __ldcg(cand + i * step) : make_uint2(0, 0);  // of a beam that is not open: not used
   }
   for (uint32_t j = warp; j < NB; j += kWarps) {
     const float2 st = lane < p.splits ? __ldcg(p.stats + (b * NB + j) * p.splits + lane) : make_float2(-INFINITY, 0.0f);
@@ -404,6 +417,7 @@ __global__ void __launch_bounds__(kPickThreads) k_beam_pick(const BeamParams p) 
     for (int o = 16; o; o >>= 1) S += __shfl_xor_sync(0xFFFFFFFFu, S, o);
     if (lane == 0) lse[j] = (double)M + log(S);
   }
+  if (tid == 0) n_placed = n_reach = 0;
   __syncthreads();
   // candidate i of the request; a done beam's only one stands in its first place
   auto make = [&](uint32_t i, const uint2 &c) -> Best {
@@ -424,46 +438,96 @@ __global__ void __launch_bounds__(kPickThreads) k_beam_pick(const BeamParams p) 
     p.out_tokens[o] = token;
     if (p.out_done) p.out_done[o] = !some || kind[parent] == 2 || token == p.eos;
   };
-  if (N <= kPickThreads) {
-    // a candidate a thread: its place is the number of better ones (all differ).
-    // Counting takes 0.3 us for 128, a round below as long.
-    const Best c = tid < N ? make(tid, raw[0]) : Best{0, 0, 0};
-    hi[tid] = c.hi;
-    mid[tid] = c.mid;
-    lo[tid] = c.lo;
-    const uint32_t found = __syncthreads_count(c.hi != 0);
-    uint32_t place = 0, same = 0;
-    for (uint32_t j = 0; j < N; j += 2) {  // an odd N: hi[N] is 0
+  auto keep = [&](uint32_t at, const Best &c) {
+    hi[at] = c.hi;
+    mid[at] = c.mid;
+    lo[at] = c.lo;
+  };
+  // Candidate `at` of the first n (0 in hi[n]) by the number of better ones
+  auto place = [&](uint32_t at, uint32_t n) {
+    const Best c{hi[at], mid[at], lo[at]};
+    uint32_t r = 0, same = 0;
+    for (uint32_t j = 0; j < n; j += 2) {
       const ulonglong2 x = *reinterpret_cast<const ulonglong2 *>(hi + j);
-      place += (x.x > c.hi) + (x.y > c.hi);
+      r += (x.x > c.hi) + (x.y > c.hi);
       same += (x.x == c.hi) + (x.y == c.hi);
     }
-    if (c.hi && same > 1)
-      for (uint32_t j = 0; j < N; ++j) place += hi[j] == c.hi && (mid[j] > c.mid || (mid[j] == c.mid && lo[j] > c.lo));
-    if (c.hi && place < K) write(place, c);
-    if (tid >= found && tid < K) write(tid, Best{0, 0, 0});
+    if (same > 1)
+      for (uint32_t j = 0; j < n; ++j) r += hi[j] == c.hi && (mid[j] > c.mid || (mid[j] == c.mid && lo[j] > c.lo));
+    if (r < K) write(r, c);
+  };
+  if constexpr (!MANY) {  // all of them, a thread each
+    const Best c = tid < N ? make(tid, raw[0]) : Best{0, 0, 0};
+    keep(tid, c);
+    if (tid < 2) hi[kPickThreads + tid] = 0;
+    const uint32_t some = __syncthreads_count(c.hi != 0);
+    if (c.hi) place(tid, N);
+    if (tid >= some && tid < K) write(tid, Best{0, 0, 0});
     return;
   }
-  Best held[kHold];
+  // the scores' first 32 bits do for the bound
+  uint32_t top = 0;
 #pragma unroll
   for (uint32_t h = 0; h < kHold; ++h) {
     const uint32_t i = tid + h * kPickThreads;
-    held[h] = i < N ? make(i, raw[h]) : Best{0, 0, 0};
+    if (i < have) top = max(top, (uint32_t)(make(i * step, raw[h]).hi >> 32));
   }
-  // k rounds: the best of the threads' own best; the winner looks for its next
+  for (uint32_t i = tid + kHold * kPickThreads; i < have; i += kPickThreads) top = max(top, (uint32_t)(make(i, __ldcg(cand + i)).hi >> 32));
+  tops[tid] = top;
+  __syncthreads();
+  uint32_t above = 0;
+#pragma unroll 4
+  for (uint32_t j = 0; j < kPickThreads; j += 4) {
+    const uint4 x = *reinterpret_cast<const uint4 *>(tops + j);
+    above += (x.x > top || (x.x == top && j < tid)) + (x.y > top || (x.y == top && j + 1 < tid)) + (x.z > top || (x.z == top && j + 2 < tid)) +
+             (x.w > top || (x.w == top && j + 3 < tid));
+  }
+  if (above == K - 1) bound = top;  // one thread's
+  __syncthreads();
+  const uint32_t low = max(bound, 1u);  // of a candidate it is never 0
+  auto gather = [&](uint32_t i, const uint2 &c) {
+    const Best x = make(i, c);
+    if ((uint32_t)(x.hi >> 32) < low) return;
+    const uint32_t at = atomicAdd(&n_placed, 1u);
+    if (at < kPlaced) keep(at, x);
+  };
+#pragma unroll
+  for (uint32_t h = 0; h < kHold; ++h) {
+    const uint32_t i = tid + h * kPickThreads;
+    if (i >= have) continue;
+    if (!heads) gather(i, raw[h]);
+    else if ((uint32_t)(make(i * step, raw[h]).hi >> 32) >= low) reach[atomicAdd(&n_reach, 1u)] = i;
+  }
+  for (uint32_t i = tid + kHold * kPickThreads; i < have; i += kPickThreads) gather(i, __ldcg(cand + i));
+  if (heads) {  // the lists whose first one reaches it
+    __syncthreads();
+    for (uint32_t i = tid; i < n_reach * K; i += kPickThreads) {
+      const uint32_t at = reach[i / K] * K + i % K;
+      gather(at, __ldcg(cand + at));
+    }
+  }
+  __syncthreads();
+  const uint32_t found = n_placed;
+  if (found <= kPlaced) {
+    if (tid < 2) hi[found + tid] = 0;
+    __syncthreads();
+    for (uint32_t i = tid; i < found; i += kPickThreads) place(i, found);
+    for (uint32_t r = found + tid; r < K; r += kPickThreads) write(r, Best{0, 0, 0});
+    return;
+  }
+  // More (equal scores, or most of the best in few ranges): k rounds, the best of
+  // the threads' own best; the winner looks for its next
   auto scan = [&](const Best &below) -> Best {
     Best r{0, 0, 0};
-#pragma unroll
-    for (uint32_t h = 0; h < kHold; ++h)
-      if (better(below, held[h]) && better(held[h], r)) r = held[h];
-    for (uint32_t i = tid + kHold * kPickThreads; i < N; i += kPickThreads) {
+#pragma unroll 4
+    for (uint32_t i = tid; i < N; i += kPickThreads) {
       const Best c = make(i, __ldcg(cand + i));
       if (better(below, c) && better(c, r)) r = c;
     }
     return r;
   };
   Best mine = scan(Best{~0ull, ~0ull, ~0u});
-  for (uint32_t r = 0; r < K; ++r) {
+  for (uint32_t r = 0; r < K; ++r) {  // found > k: every round has a winner
     const uint32_t buf = r & 1;
     uint32_t l = best_lane(mine);
     if (lane == l) {
@@ -473,24 +537,27 @@ __global__ void __launch_bounds__(kPickThreads) k_beam_pick(const BeamParams p) 
     __syncthreads();
     const Best w = lane < kWarps ? wbest[buf][lane] : Best{0, 0, 0};
     l = best_lane(w);
-    if (l >= kWarps) l = 0;  // nothing is left anywhere: all are {0, 0, 0}
-    const Best top = wbest[buf][l];
-    if (tid == 0) won[r] = top;
-    if (top.hi == 0) {  // the same for every thread
-      if (tid == 0)
-        for (uint32_t i = r; i < K; ++i) won[i] = Best{0, 0, 0};
-      break;
-    }
-    if (tid == wthread[buf][l]) mine = scan(top);
+    const Best best = wbest[buf][l];
+    if (tid == 0) write(r, best);
+    if (tid == wthread[buf][l]) mine = scan(best);
   }
-  __syncthreads();
-  for (uint32_t r = tid; r < K; r += kPickThreads) write(r, won[r]);
 }
 
+// How a kernel's SMs split their memory.  Before k_beam_pick<true>, which has 27 KB
+// of shared memory, the scan takes the same split, or the pick's CTAs wait for
+// the SMs to empty: 4 x 8 beams 24.4 us, 18.6 so.  Else its own: 32 x 8 beams 31.2
+// us, and 34.2 with the smaller L1.
+template <typename K>
+bool split_memory(K kern, bool shared) {
+  return cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout,
+                              shared ? cudaSharedmemCarveoutMaxShared : cudaSharedmemCarveoutDefault) == cudaSuccess;
+}
 template <typename T>
 int launch_t(const BeamParams &p, cudaStream_t st) {
   const uint32_t rows = p.n_batch * p.n_beams;
   const bool vec = reinterpret_cast<uintptr_t>(p.logits) % (4 * sizeof(T)) == 0 && p.ld % 4 == 0;
+  const bool many = p.n_beams * p.splits * p.k > kPickThreads;
+  if (!(vec ? split_memory(k_beam_scan<T, true>, many) : split_memory(k_beam_scan<T, false>, many))) return -1;
   for (uint32_t r0 = 0; r0 < rows; r0 += 65535) {  // grid y ends at 65535
     BeamParams q = p;
     q.logits = reinterpret_cast<const T *>(p.logits) + r0 * p.ld;
@@ -503,7 +570,9 @@ int launch_t(const BeamParams &p, cudaStream_t st) {
     else k_beam_scan<T, false><<<grid, kScanThreads, 0, st>>>(q);
     if (cudaGetLastError() != cudaSuccess) return -1;
   }
-  return launch_pdl(k_beam_pick, dim3(p.n_batch), dim3(kPickThreads), 0, st, p);
+  if (!many) return launch_pdl(k_beam_pick<false>, dim3(p.n_batch), dim3(kPickThreads), 0, st, p);
+  if (!split_memory(k_beam_pick<true>, true)) return -1;
+  return launch_pdl(k_beam_pick<true>, dim3(p.n_batch), dim3(kPickThreads), 0, st, p);
 }
 
 }  // namespace

@@ -473,6 +473,25 @@ def test_beam_select(t, nb, beams, vocab, k):
     beam_check(x, scores, None, k, eos=-1, pad=vocab - 1)
 
 
+@pytest.mark.parametrize("nb,beams,vocab,k", [(1, 12, 128256, 16), (1, 1, 128256, 64), (1, 64, 128256, 64), (3, 20, 9000, 33), (2, 40, 40000, 64)])
+def test_beam_select_of_many_lists(nb, beams, vocab, k):
+    """requests whose rows are split: more candidates than threads"""
+    x = 3 * randn(vocab + k, nb * beams, vocab)
+    scores = -0.1 * torch.rand(nb, beams, device="cuda", generator=torch.Generator("cuda").manual_seed(k))
+    done = torch.zeros(nb, beams, dtype=torch.int32, device="cuda")
+    done[:, beams // 2] = beams > 2
+    beam_check(x, scores, done, k)
+
+
+@pytest.mark.parametrize("nb,beams,vocab,k", [(1, 2, 128256, 64), (1, 64, 70000, 64), (1, 12, 50000, 16)])
+def test_beam_select_of_equal_candidates(nb, beams, vocab, k):
+    """every candidate as good as the next: more of them reach the bound than are placed at once"""
+    x = torch.zeros(nb * beams, vocab, device="cuda")
+    beam_check(x, torch.zeros(nb, beams, device="cuda"), None, k)
+    x[:, ::7] = 1.0
+    beam_check(x, torch.zeros(nb, beams, device="cuda"), None, k)
+
+
 def test_beam_select_ties_go_to_the_lowest():
     for vocab in (50, 5000, 70000):
         x = torch.zeros(6, vocab, device="cuda")
