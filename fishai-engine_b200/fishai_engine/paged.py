@@ -45,7 +45,7 @@ def _code(t, name):
 
 def _index(t, name, n):
     """address of a contiguous array of n 32-bit whole numbers"""
-    if t.dtype not in _INTS or t.stride() != _ONE or t.shape[0] != n:
+    if t.shape != (n,) or t.dtype not in _INTS or (n > 1 and t.stride() != _ONE):
         if not _INTS:
             _learn()
             return _index(t, name, n)
@@ -53,19 +53,19 @@ def _index(t, name, n):
             raise ValueError(f"{name}: a contiguous 1-d int32 tensor is needed")
         if t.shape[0] != n:
             raise ValueError(f"{name}: {t.shape[0]} entries, {n} needed")
-        if n > 1:
-            raise ValueError(f"{name}: a contiguous 1-d int32 tensor is needed")
+        raise ValueError(f"{name}: a contiguous 1-d int32 tensor is needed")
     return t.data_ptr()
 
 
 def _rows(t, name, n, width):
     """address and row stride of n rows of `width` consecutive elements, [n, width] or [n, heads, head_dim]"""
     shape, stride = t.shape, t.stride()
-    if len(shape) == 2:
-        ok = shape[1] == width and stride[1] == 1
+    if shape == (n, width):
+        ok = stride[1] == 1
     else:
-        ok = len(shape) == 3 and shape[1] * shape[2] == width and stride[2] == 1 and (shape[1] == 1 or stride[1] == shape[2])
-    if not ok or shape[0] != n:
+        ok = len(shape) == 3 and shape[0] == n and shape[1] * shape[2] == width and stride[2] == 1 and \
+            (shape[1] == 1 or stride[1] == shape[2])
+    if not ok:
         raise ValueError(f"{name}: {n} rows of {width} consecutive elements are needed, got {list(shape)} with strides {stride}")
     return t.data_ptr(), stride[0] if n > 1 else width
 
