@@ -4,8 +4,9 @@
 // chunk being query token r / rep and query head kvh * rep + r % rep, so the
 // rows of an item read the same K and V.  It covers the positions that any of
 // its rows sees, in units of U positions.  The items' costs, in chunk, row tile,
-// head order, are one line, and each CTA takes an equal stretch of it: chunks of any lengths then load the GPU evenly, and a single long cache
-// is spread over all of it.  A CTA finishes the items that lie inside its
+// head order, are one line, and each CTA takes an equal stretch of it: chunks of
+// any lengths then load the GPU evenly, and a single long cache is spread over all
+// of it.  A CTA finishes the items that lie inside its
 // stretch; the ends of a stretch leave (max, sum, unnormalised output) in the
 // CTA's two slots, and k_attn_join adds the pieces in the order of the
 // positions, so results do not depend on timing.
@@ -327,9 +328,11 @@ struct JoinSet {
 };
 // One launch for few items, each a cluster; 1: the call is not of that kind.
 int launch_one_any(const AttnChunksParams &p, cudaStream_t st);
+int launch_one_few(const AttnChunksParams &p, cudaStream_t st);
 int launch_one_mma(const AttnChunksParams &p, cudaStream_t st);
 // The kernels; each returns its grid, or 0 where the launch failed.
 bool attn_mma_takes(const AttnChunksParams &p);
+uint32_t launch_attn_few(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st, uint32_t *R);  // no chunk above 16 rows
 uint32_t launch_attn_any(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st, uint32_t *R);
 uint32_t launch_attn_mma(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st);  // items of kMmaRows
 // overlap: the launch before is launch_attn_mma's, with which this one may run at the same time

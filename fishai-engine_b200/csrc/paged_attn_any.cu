@@ -1,32 +1,29 @@
-// Attention of chunks over paged K/V with f32 arithmetic, for every element
-// type and every head size (a multiple of 8 up to 256): the path of f32 caches
-// and of head sizes the tensor-core kernels are not made for.
+// Attention of chunks over paged K/V with f32 arithmetic and more than 16 rows per
+// kv head, for every element type and every head size (a multiple of 8 up to
+// 256): the path of f32 caches and of head sizes the tensor-core kernels are not
+// made for.
 //
 //   o_r = sum_t e^(s_rt - m_r) v_t / sum_t e^(s_rt - m_r),  s_rt = scale q_r.k_t
 //
 // over one pass of the positions, with a running maximum m and sum l of a row:
 // where m grows to m', l and o are multiplied by e^(m - m').
 //
-// An item is R rows of a kv head; tiles of 64 positions of K and V go through
-// shared memory.  Scores: a thread has R/8 rows x 4 positions, outputs: R/8
-// rows x hd/16 elements, each pair of operands read as float4, so 16 FMA per
-// (R/8 + 4) loads of 16 bytes, and the reads of shared memory bound it (75% of
-// its pipe for 8 rows), before HBM: 8 f32 sequences of 8192 positions, 32/8 heads
-// x 128, 210 us, 2.6 TB/s; one 42 us; 8 rows of one 8192-position f16 cache of
-// 8 heads x 256 63 us.  (A tile fetched only when the one before was done: 257, 50
-// and 205 us.)  A warp to its own positions, each lane one, reads K once but Q for
-// every position: 217, 38 and 57 us, and 13 against 10 us for short caches.
+// An item is 32 rows of a kv head; tiles of 64 positions of K and V go through
+// shared memory, copied one ahead.  Scores: a thread has 4 rows x 4 positions,
+// outputs: 4 rows x hd/16 elements, each pair of operands read as float4, so 64 FMA
+// per 8 loads of 16 bytes; the FMA pipes and shared memory bound it: 1024 f32
+// tokens over themselves, 32/8 heads x 128, 716 us, 64 over 8192 positions 420.
+// (Chunks of up to 16 rows: paged_attn_few.cu.  Its way of sharing the operands
+// out, with 32 rows: 668 and 585 us.)
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
-
-#include <type_traits>
 
 #include "paged_attn.cuh"
 
 namespace fa {
 namespace {
 
-constexpr uint32_t kAnyThreads = 128, kAnyPos = 64;
+constexpr uint32_t kAnyThreads = 128, kAnyPos = 64, R = 32;  // R: rows of an item
 
 // four elements, aligned to their size
 __device__ __forceinline__ float4 load4(const float *p) { return *reinterpret_cast<const float4 *>(p); }
@@ -77,13 +74,13 @@ __device__ __forceinline__ void copied_but_one() { asm volatile("cp.async.wait_g
 
 // bytes: Q rows and weights in f32, K and V tiles in their own type, rows 16 bytes apart
 template <typename T>
-constexpr uint32_t any_smem(uint32_t R, uint32_t hd) {
+constexpr uint32_t any_smem(uint32_t hd) {
   return (R * (hd + 4) + R * (kAnyPos + 4)) * 4 + 2 * kAnyPos * (hd * (uint32_t)sizeof(T) + 16);
 }
 
 // HJ: groups of 64 head elements (hd <= 64 HJ).  A thread's rows are ty + 8 i, its
 // elements 64 j + 4 tx + e.
-template <typename T, uint32_t R, uint32_t HJ>
+template <typename T, uint32_t HJ>
 struct AnyRows {
   static constexpr uint32_t RT = R / 8;
   float m[RT], l[RT], o[RT][HJ][4];
@@ -224,7 +221,7 @@ struct AnyRows {
   }
 };
 
-template <typename T, uint32_t R, uint32_t HJ>
+template <typename T, uint32_t HJ>
 __global__ void __launch_bounds__(kAnyThreads) k_attn_any(const AttnChunksParams p) {
   extern __shared__ __align__(16) float sm[];
   __shared__ uint64_t red[kAnyThreads / 32 + 2];
@@ -235,7 +232,7 @@ __global__ void __launch_bounds__(kAnyThreads) k_attn_any(const AttnChunksParams
   if (tid == 0) p.desc[blockIdx.x].w = 0;
   for (Segment s; w.next(p, s);) {
     __syncthreads();
-    AnyRows<T, R, HJ> x;
+    AnyRows<T, HJ> x;
     x.run(p, s, s.u0, s.u1, 1, sm);
     const bool whole = W::whole(s);
     float *slot = W::slot(p, s);
@@ -266,14 +263,14 @@ __global__ void __launch_bounds__(kAnyThreads) k_attn_any(const AttnChunksParams
   pdl_launch_dependents();
 }
 
-// few items of up to R rows: a cluster each (paged_attn.cuh)
-template <typename T, uint32_t R, uint32_t HJ>
+// few items of up to 32 rows: a cluster each (paged_attn.cuh)
+template <typename T, uint32_t HJ>
 __global__ void __launch_bounds__(kAnyThreads) k_attn_any_one(const AttnChunksParams p) {
   extern __shared__ __align__(16) float sm[];
   const uint32_t hd = p.pg.head_dim, tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
   Segment s;
   if (!one_item(p, s)) return;
-  AnyRows<T, R, HJ> x;
+  AnyRows<T, HJ> x;
   x.run(p, s, cluster_ctarank(), range_units<kAnyPos>(s.lo, s.hi), kOneCtas, sm);
   float *o = sm, *ml = o + R * hd;  // over Q and the weights, which have been read
   __syncthreads();
@@ -296,40 +293,33 @@ __global__ void __launch_bounds__(kAnyThreads) k_attn_any_one(const AttnChunksPa
   });
 }
 
-template <typename T, uint32_t R, uint32_t HJ>
+template <typename T, uint32_t HJ>
 uint32_t launch_hj(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st, uint32_t *rows) {
-  const uint32_t smem = any_smem<T>(R, p.pg.head_dim);
-  if (cudaFuncSetAttribute(k_attn_any<T, R, HJ>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)any_smem<T>(R, 64 * HJ)) !=
+  const uint32_t smem = any_smem<T>(p.pg.head_dim);
+  if (cudaFuncSetAttribute(k_attn_any<T, HJ>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)any_smem<T>(64 * HJ)) !=
       cudaSuccess)
     return 0;
   uint32_t per_sm = 224 * 1024 / (smem + 1024);
   per_sm = per_sm > 3 ? 3 : per_sm;
   const uint32_t grid = n_sm * per_sm < kAttnMaxCtas ? n_sm * per_sm : kAttnMaxCtas;
-  k_attn_any<T, R, HJ><<<grid, kAnyThreads, smem, st>>>(p);
+  k_attn_any<T, HJ><<<grid, kAnyThreads, smem, st>>>(p);
   *rows = R;
   return cudaGetLastError() == cudaSuccess ? grid : 0;
 }
-template <typename T, uint32_t R, uint32_t HJ>
+template <typename T, uint32_t HJ>
 struct LaunchAny {
-  static uint32_t walk(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st, uint32_t *rows) { return launch_hj<T, R, HJ>(p, n_sm, st, rows); }
+  static uint32_t walk(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st, uint32_t *rows) { return launch_hj<T, HJ>(p, n_sm, st, rows); }
   static int one(const AttnChunksParams &p, cudaStream_t st) {
-    return launch_one<k_attn_any_one<T, R, HJ>>(p, kAnyThreads, any_smem<T>(R, 64 * HJ), st);
+    return launch_one<k_attn_any_one<T, HJ>>(p, kAnyThreads, any_smem<T>(64 * HJ), st);
   }
 };
 // f(LaunchAny of the call's type, rows and head size)
 template <typename T, typename F>
 auto with_hd(const AttnChunksParams &p, F f) {
   const uint32_t hd = p.pg.head_dim;
-  // items of 8 or 16 rows while no chunk has more: few rows would leave most of
-  // 32 idle in the FMA loops
-  const uint64_t rows = (uint64_t)p.max_q * p.rep;
-  auto with_rows = [&](auto hj) {
-    constexpr uint32_t HJ = decltype(hj)::value;
-    return rows <= 8 ? f(LaunchAny<T, 8, HJ>()) : rows <= 16 ? f(LaunchAny<T, 16, HJ>()) : f(LaunchAny<T, 32, HJ>());
-  };
-  if (hd <= 64) return with_rows(std::integral_constant<uint32_t, 1>());
-  if (hd <= 128) return with_rows(std::integral_constant<uint32_t, 2>());
-  return with_rows(std::integral_constant<uint32_t, 4>());
+  if (hd <= 64) return f(LaunchAny<T, 1>());
+  if (hd <= 128) return f(LaunchAny<T, 2>());
+  return f(LaunchAny<T, 4>());
 }
 template <typename F>
 auto with_kind(const AttnChunksParams &p, F f) {
@@ -346,9 +336,9 @@ uint32_t launch_attn_any(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t 
   return with_kind(p, [&](auto k) { return k.walk(p, n_sm, st, R); });
 }
 int launch_one_any(const AttnChunksParams &p, cudaStream_t st) {
-  if ((uint64_t)p.max_q * p.rep > 32) return 1;
-  // While a CTA has one tile: 5 sequences of 512 positions with 12 rows, 2 kv heads
-  // x 64, 13.1 us against 18.1 in two launches; of 2048 36.7 against 23.3.
+  if ((uint64_t)p.max_q * p.rep > R) return 1;
+  // While a CTA has one tile: 4 tokens of 8 heads each over 512 positions 20.6 us
+  // against 29 in two launches; over 2048 59 against 38.
   if (one_span(p) > kOneCtas * kAnyPos) return 1;
   return with_kind(p, [&](auto k) { return k.one(p, st); });
 }

@@ -233,8 +233,8 @@ int launch_attn_chunks(const AttnChunksParams &p, void *ws, uint32_t n_sm, cudaS
   a.rows_min = 1;
   a.rows_max = 0xFFFFFFFFu;
   JoinSet ja{a.part, a.desc, 0, 0, 0}, jb{b.part, b.desc, 0, 0, 0};
-  const bool mma = attn_mma_takes(p);
-  const int one = mma ? launch_one_mma(a, st) : launch_one_any(a, st);
+  const bool mma = attn_mma_takes(p), few = (uint64_t)p.max_q * p.rep <= 16;
+  const int one = mma ? launch_one_mma(a, st) : few ? launch_one_few(a, st) : launch_one_any(a, st);
   if (one <= 0) return one;
   if (mma) {
     // Up to 16 rows mma.sync keeps up with the copies of K and V; above, the
@@ -257,7 +257,7 @@ int launch_attn_chunks(const AttnChunksParams &p, void *ws, uint32_t n_sm, cudaS
       if (!(jb.ctas = launch_attn_tc(b, n_sm, !alike, st, &jb.R))) return -1;
       jb.parts = jb.R / 32 * (p.pg.head_dim / 16) / kJoinWarps;  // a thread 16 elements of a row
     }
-  } else if (!(ja.ctas = launch_attn_any(a, n_sm, st, &ja.R))) {
+  } else if (!(ja.ctas = few ? launch_attn_few(a, n_sm, st, &ja.R) : launch_attn_any(a, n_sm, st, &ja.R))) {
     return -1;
   }
   // CTAs to an item: a row each, for the few rows of one long cache
