@@ -236,6 +236,7 @@ inline uint64_t one_span(const AttnChunksParams &p) {
   const uint64_t cap = (uint64_t)p.pg.max_pages * kPageLen, seen = (uint64_t)p.window + p.max_q;
   return p.window && seen < cap ? seen : cap;
 }
+inline uint64_t one_items(const AttnChunksParams &p) { return (uint64_t)p.n_chunks * p.pg.n_kv_heads; }
 // Cluster blockIdx.x / kOneCtas takes (chunk, head); false: the chunk has no
 // rows (the same for the whole cluster).
 __device__ __forceinline__ bool one_item(const AttnChunksParams &p, Segment &s) {
@@ -253,29 +254,29 @@ __device__ __forceinline__ bool one_item(const AttnChunksParams &p, Segment &s) 
 // unnormalised outputs [rows][hd] in shared memory (16-byte aligned), as in
 // k_attn_join, in the order of the CTAs: the threads of all CTAs share the
 // elements, with the loads of all pieces in flight.  put(row, d, f32 x 4).
-template <uint32_t THREADS, typename Put>
-__device__ __forceinline__ void one_join(const Segment &s, uint32_t hd, const float *o, const float *ml, Put put) {
+template <uint32_t THREADS, uint32_t C = kOneCtas, typename Put>
+__device__ __forceinline__ void one_join(const Segment &s, uint32_t hd, const float *o, uint32_t ld, const float *ml, Put put) {
   cluster_sync();
-  const uint32_t n4 = s.r1 * (hd / 4), per = (n4 + kOneCtas - 1) / kOneCtas, i0 = cluster_ctarank() * per;
+  const uint32_t n4 = (s.r1 - s.r0) * (hd / 4), per = (n4 + C - 1) / C, i0 = cluster_ctarank() * per;
   for (uint32_t i = i0 + threadIdx.x; i < min(n4, i0 + per); i += THREADS) {
     const uint32_t r = i / (hd / 4), d = (i - r * (hd / 4)) * 4;
-    float m[kOneCtas], l[kOneCtas];
-    float4 x[kOneCtas];
+    float m[C], l[C];
+    float4 x[C];
 #pragma unroll
-    for (uint32_t k = 0; k < kOneCtas; ++k) {
+    for (uint32_t k = 0; k < C; ++k) {
       asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(m[k]), "=f"(l[k]) : "r"(dsmem_addr(ml + 2 * r, k)) : "memory");
       asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
                    : "=f"(x[k].x), "=f"(x[k].y), "=f"(x[k].z), "=f"(x[k].w)
-                   : "r"(dsmem_addr(o + r * hd + d, k))
+                   : "r"(dsmem_addr(o + r * ld + d, k))
                    : "memory");
     }
     float M = m[0], L = 0.0f;
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-    for (uint32_t k = 1; k < kOneCtas; ++k) M = fmaxf(M, m[k]);
+    for (uint32_t k = 1; k < C; ++k) M = fmaxf(M, m[k]);
     const float Ms = M == -INFINITY ? 0.0f : M;
 #pragma unroll
-    for (uint32_t k = 0; k < kOneCtas; ++k) {
+    for (uint32_t k = 0; k < C; ++k) {
       const float e = exp2f(m[k] - Ms);
       L = fmaf(l[k], e, L);
       acc.x = fmaf(x[k].x, e, acc.x);
@@ -288,20 +289,18 @@ __device__ __forceinline__ void one_join(const Segment &s, uint32_t hd, const fl
   }
   cluster_sync();  // the pieces have been read
 }
-// Launches a cluster for each of (chunk, kv head), where the GPU holds that many
-// at once; 1: it does not, -1: an error.
-template <auto kern>
-int launch_one(const AttnChunksParams &p, uint32_t threads, uint32_t smem, cudaStream_t st) {
+// Launches a cluster for each of `items`, where the GPU holds that many at once; 1: it does not, -1: an error.
+template <auto kern, uint32_t C = kOneCtas>
+int launch_one(const AttnChunksParams &p, uint64_t items, uint32_t threads, uint32_t smem, cudaStream_t st) {
   static std::atomic<int> known[64];  // clusters at once, by device (0: not asked yet)
-  const uint64_t items = (uint64_t)p.n_chunks * p.pg.n_kv_heads;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(kOneCtas);
+  cfg.gridDim = dim3(C);
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = kOneCtas;
+  attr[0].val.clusterDim.x = C;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
@@ -315,7 +314,7 @@ int launch_one(const AttnChunksParams &p, uint32_t threads, uint32_t smem, cudaS
     if (keep && at_once > 0) known[device].store(at_once, std::memory_order_relaxed);
   }
   if (items > (uint64_t)(at_once > 0 ? at_once : 0)) return 1;
-  cfg.gridDim = dim3((uint32_t)items * kOneCtas);
+  cfg.gridDim = dim3((uint32_t)items * C);
   return cudaLaunchKernelEx(&cfg, kern, p) == cudaSuccess ? 0 : -1;
 }
 
@@ -330,6 +329,7 @@ struct JoinSet {
 int launch_one_any(const AttnChunksParams &p, cudaStream_t st);
 int launch_one_few(const AttnChunksParams &p, cudaStream_t st);
 int launch_one_mma(const AttnChunksParams &p, cudaStream_t st);
+int launch_short_mma(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st);
 // The kernels; each returns its grid, or 0 where the launch failed.
 bool attn_mma_takes(const AttnChunksParams &p);
 uint32_t launch_attn_few(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st, uint32_t *R);  // no chunk above 16 rows

@@ -284,7 +284,7 @@ __global__ void __launch_bounds__(kAnyThreads) k_attn_any_one(const AttnChunksPa
       if (d < hd) *reinterpret_cast<float4 *>(o + r * hd + d) = make_float4(x.o[i][j][0], x.o[i][j][1], x.o[i][j][2], x.o[i][j][3]);
     }
   }
-  one_join<kAnyThreads>(s, hd, o, ml, [&](uint32_t r, uint32_t d, float4 y) {
+  one_join<kAnyThreads>(s, hd, o, hd, ml, [&](uint32_t r, uint32_t d, float4 y) {
     T *out = reinterpret_cast<T *>(p.out) + (uint64_t)(s.chunk.q0 + r / p.rep) * p.os + (s.head * p.rep + r % p.rep) * hd + d;
     put(out, y.x);
     put(out + 1, y.y);
@@ -310,7 +310,7 @@ template <typename T, uint32_t HJ>
 struct LaunchAny {
   static uint32_t walk(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st, uint32_t *rows) { return launch_hj<T, HJ>(p, n_sm, st, rows); }
   static int one(const AttnChunksParams &p, cudaStream_t st) {
-    return launch_one<k_attn_any_one<T, HJ>>(p, kAnyThreads, any_smem<T>(64 * HJ), st);
+    return launch_one<k_attn_any_one<T, HJ>>(p, one_items(p), kAnyThreads, any_smem<T>(64 * HJ), st);
   }
 };
 // f(LaunchAny of the call's type, rows and head size)

@@ -308,7 +308,7 @@ __global__ void __launch_bounds__(kThreads) k_attn_few_one(const AttnChunksParam
     const uint32_t r = i / (hd / 4), d = (i - r * (hd / 4)) * 4;
     *reinterpret_cast<float4 *>(o + r * hd + d) = x.sum(few_sm, hd, r, d);
   }
-  one_join<kThreads>(s, hd, o, o + R * hd, [&](uint32_t r, uint32_t d, float4 y) { put_row<T>(p, s, r, d, y); });
+  one_join<kThreads>(s, hd, o, hd, o + R * hd, [&](uint32_t r, uint32_t d, float4 y) { put_row<T>(p, s, r, d, y); });
 }
 
 template <typename T, uint32_t R, uint32_t DPL>
@@ -325,7 +325,7 @@ struct LaunchFew {
     return cudaGetLastError() == cudaSuccess ? grid : 0;
   }
   static int one(const AttnChunksParams &p, cudaStream_t st) {
-    return launch_one<k_attn_few_one<T, R, DPL>>(p, kThreads, C::smem(32 * DPL), st);
+    return launch_one<k_attn_few_one<T, R, DPL>>(p, one_items(p), kThreads, C::smem(32 * DPL), st);
   }
 };
 // f(LaunchFew of the call's type, rows and head size)

@@ -234,10 +234,10 @@ int launch_attn_chunks(const AttnChunksParams &p, void *ws, uint32_t n_sm, cudaS
   a.rows_max = 0xFFFFFFFFu;
   JoinSet ja{a.part, a.desc, 0, 0, 0}, jb{b.part, b.desc, 0, 0, 0};
   const bool mma = attn_mma_takes(p), few = (uint64_t)p.max_q * p.rep <= 16;
-  const int one = mma ? launch_one_mma(a, st) : few ? launch_one_few(a, st) : launch_one_any(a, st);
+  const int one = mma ? few ? launch_one_mma(a, st) : launch_short_mma(a, n_sm, st) : few ? launch_one_few(a, st) : launch_one_any(a, st);
   if (one <= 0) return one;
   if (mma) {
-    // Up to 16 rows mma.sync keeps up with the copies of K and V; above, the
+    // (Short calls have gone to launch_short_mma.)  Up to 16 rows mma.sync keeps up with the copies of K and V; above, the
     // items of tcgen05, also where they are mostly empty: 64 sequences of 4096
     // positions with 32 and 64 rows take 200 and 208 us, and took 264 and 316
     // with mma.sync and a warp for each 16 rows (which was the faster one over

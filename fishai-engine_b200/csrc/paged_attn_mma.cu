@@ -424,7 +424,7 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 1 : 2) k_attn_one16(c
     *reinterpret_cast<float4 *>(o + r * HD + d) = pieces.sum(r, d, M, L);
     if (d == 0) *reinterpret_cast<float2 *>(ml + 2 * r) = make_float2(M, L);
   }
-  one_join<32 * WARPS>(s, HD, o, ml, [&](uint32_t r, uint32_t d, float4 x) { put4(p, out_row<T>(p, s, r, HD) + d, x); });
+  one_join<32 * WARPS>(s, HD, o, HD, ml, [&](uint32_t r, uint32_t d, float4 x) { put4(p, out_row<T>(p, s, r, HD) + d, x); });
 }
 // Eight warps, one CTA an SM, or six and two CTAs: the former keep more copies in
 // flight (8 kv heads over 8192 positions 11.9 us against 15.0), the latter take
@@ -433,13 +433,120 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 1 : 2) k_attn_one16(c
 template <typename T, uint32_t HD>
 int launch_one_hd(const AttnChunksParams &p, uint64_t span, cudaStream_t st) {
   if (span > kOneCtas * 6 * kSub) {
-    const int rc = launch_one<k_attn_one16<T, HD, 8>>(p, 256, OneCfg<HD, 8>::kBytes, st);
+    const int rc = launch_one<k_attn_one16<T, HD, 8>>(p, one_items(p), 256, OneCfg<HD, 8>::kBytes, st);
     if (rc <= 0) return rc;
   }
-  return launch_one<k_attn_one16<T, HD, 6>>(p, 192, OneCfg<HD, 6>::kBytes, st);
+  return launch_one<k_attn_one16<T, HD, 6>>(p, one_items(p), 192, OneCfg<HD, 6>::kBytes, st);
+}
+
+// --------------------------- short calls of more rows: a cluster to 64 rows each
+// An item is 64 rows of a kv head, a warp has 16 of them, and all warps share
+// tiles of 64 positions, the next one in flight.  The C CTAs of a cluster take the
+// item's tiles in turn; one launch, no work split and no second kernel, which
+// cost more than the work here.
+constexpr uint32_t kShortRows = 64, kShortPos = 64;
+template <uint32_t HD>
+struct ShortCfg {
+  static constexpr uint32_t kHalf = kSub * HD * 2, kTile = 2 * kHalf, LD = HD + 4;  // 32 positions, 64; floats of a row of a piece
+  static constexpr uint32_t kTiles = 2 * 2 * kTile, kPiece = kShortRows * LD * 4 + kShortRows * 8, kBytes = kTiles > kPiece ? kTiles : kPiece;
+};
+template <typename T, uint32_t HD, uint32_t C>
+__global__ void __launch_bounds__(kThreads, 2) k_attn_short(const AttnChunksParams p) {
+  using S = ShortCfg<HD>;
+  extern __shared__ __align__(128) uint8_t dsm[];
+  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
+  const T *base = reinterpret_cast<const T *>(p.pg.base) + (uint64_t)p.layer * p.pg.layer_stride;
+  const uint32_t item = blockIdx.x / C, kvh = p.pg.n_kv_heads, tiles = (p.max_q * p.rep + kShortRows - 1) / kShortRows;
+  Segment s;
+  s.chunk = load_chunk(p, item / (kvh * tiles));
+  s.tile = item / kvh % tiles;
+  s.head = item % kvh;
+  s.r0 = s.tile * kShortRows;
+  if (s.r0 >= s.chunk.rows) return;  // the whole cluster
+  s.r1 = min(s.chunk.rows, s.r0 + kShortRows);
+  tile_range(p, s.chunk, s.r0, s.r1, s.lo, s.hi);
+  const uint32_t n = s.hi > s.lo ? range_units<kShortPos>(s.lo, s.hi) : 0;
+  const uint32_t *pt = p.pg.page_table + (uint64_t)s.chunk.seq * p.pg.max_pages;
+  uint32_t u = cluster_ctarank(), t0 = (s.lo / kShortPos + u) * kShortPos;
+  // K and V of the tile at t to buffer `which`
+  auto fetch = [&](uint32_t t, uint32_t which) {
+    const uint32_t k = smem_u32(dsm) + which * 2 * S::kTile;
+#pragma unroll
+    for (uint32_t h = 0; h < 2; ++h) {
+      const PagePair pg = look_up(pt, t + h * kSub, s.lo, s.hi);
+      flag_bad_pages(p, pg);
+      stage<T, HD>(p, base, pg, s.head, 0, t + h * kSub, s.lo, s.hi, k + h * S::kHalf, tid, kThreads);
+      stage<T, HD>(p, base, pg, s.head, 1, t + h * kSub, s.lo, s.hi, k + S::kTile + h * S::kHalf, tid, kThreads);
+    }
+  };
+  if (u < n) fetch(t0, 0);
+  cp_commit();
+  if (u + C < n) fetch(t0 + C * kShortPos, 1);
+  cp_commit();
+  const uint32_t first = s.r0 + 16 * warp;
+  const bool mine = first < s.r1;
+  Rows<T, HD> rows;
+  rows.load(p, s, mine ? first : s.r0);
+  for (uint32_t which = 0; u < n; u += C, which ^= 1) {
+    cp_wait<1>();
+    __syncthreads();
+    const uint32_t k = smem_u32(dsm) + which * 2 * S::kTile;
+#pragma unroll
+    for (uint32_t h = 0; h < 2; ++h) {
+      const uint32_t t = t0 + h * kSub;
+      if (!mine || (int32_t)t > rows.pos_max) continue;  // nothing of it is seen
+      float sc[kSub / 8][4];
+      rows.scores(k + h * S::kHalf, sc);
+      rows.softmax(p, t, sc);
+      rows.add_values(k + S::kTile + h * S::kHalf, sc);
+    }
+    __syncthreads();
+    if (u + 2 * C < n) fetch(t0 + 2 * C * kShortPos, which);
+    cp_commit();
+    t0 += C * kShortPos;
+  }
+  cp_wait<0>();
+  rows.finish();
+  float *o = reinterpret_cast<float *>(dsm), *ml = o + kShortRows * S::LD;
+  __syncthreads();
+  if (mine) {
+#pragma unroll
+    for (uint32_t j = 0; j < HD / 8; ++j)
+#pragma unroll
+      for (uint32_t i = 0; i < 2; ++i)
+        *reinterpret_cast<float2 *>(o + (warp * 16 + g + 8 * i) * S::LD + 8 * j + 2 * c) = make_float2(rows.o[j][2 * i], rows.o[j][2 * i + 1]);
+    if (c == 0)
+#pragma unroll
+      for (uint32_t i = 0; i < 2; ++i) *reinterpret_cast<float2 *>(ml + (warp * 16 + g + 8 * i) * 2) = make_float2(rows.m[i], rows.l[i]);
+  }
+  one_join<kThreads, C>(s, HD, o, S::LD, ml, [&](uint32_t r, uint32_t d, float4 x) { put4(p, out_row<T>(p, s, s.r0 + r, HD) + d, x); });
+}
+template <typename T, uint32_t HD, uint32_t C>
+int launch_short_c(const AttnChunksParams &p, uint64_t items, cudaStream_t st) {
+  return launch_one<k_attn_short<T, HD, C>, C>(p, items, kThreads, ShortCfg<HD>::kBytes, st);
+}
+template <typename T, uint32_t HD>
+int launch_short_hd(const AttnChunksParams &p, uint64_t items, uint32_t c, cudaStream_t st) {
+  return c == 8 ? launch_short_c<T, HD, 8>(p, items, st) : c == 4 ? launch_short_c<T, HD, 4>(p, items, st)
+       : c == 2 ? launch_short_c<T, HD, 2>(p, items, st) : launch_short_c<T, HD, 1>(p, items, st);
 }
 
 }  // namespace
+
+int launch_short_mma(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st) {
+  const uint64_t tiles = ((uint64_t)p.max_q * p.rep + kShortRows - 1) / kShortRows, items = one_items(p) * tiles;
+  if (items > 2 * n_sm) return 1;
+  const uint32_t c = items * 8 <= 2 * n_sm ? 8 : items * 4 <= 2 * n_sm ? 4 : items * 2 <= 2 * n_sm ? 2 : 1;
+  const uint64_t units = (one_span(p) + kShortPos - 1) / kShortPos;
+  // A tile takes some 2 us, and the tcgen05 kernel with its join 12 to 16 us before
+  // its first.  32/8 heads x 128, here against there: 5 tokens of 100 positions 6.0
+  // us against 11.8, of 1000 (2 tiles a CTA) 9.0 against 19.1, of 4000 (8) 20.1
+  // against 22.3; 32 of 1000 (2) 12.5 against 20.4, of 4000 (8) 27.4 against 23.6; 128
+  // over themselves 9.4 against 15.5, 512 (8) 25.9 against 24.8.
+  if ((units + c - 1) / c > 6) return 1;
+  if (p.pg.dtype == FA_KV_F16) return p.pg.head_dim == 64 ? launch_short_hd<__half, 64>(p, items, c, st) : launch_short_hd<__half, 128>(p, items, c, st);
+  return p.pg.head_dim == 64 ? launch_short_hd<__nv_bfloat16, 64>(p, items, c, st) : launch_short_hd<__nv_bfloat16, 128>(p, items, c, st);
+}
 
 int launch_one_mma(const AttnChunksParams &p, cudaStream_t st) {
   if ((uint64_t)p.max_q * p.rep > kMmaRows) return 1;

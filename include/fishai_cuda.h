@@ -350,6 +350,8 @@ int fa_rope_append(const fa_rope *r, const fa_pages *pages, uint32_t layer, int3
  * The positions that some token of a chunk sees should hold finite K and V;
  * whatever is behind kv_len or before every token's window is not used.  A
  * page out of range (FA_FLAG_PAGE) spoils the chunk's own rows only.
+ * max_q and the table's width (max_pages) choose the kernels: the tighter they
+ * are, the faster a short call.
  * ws: at least fa_attn_chunks_ws(...) bytes of device memory, 16-byte aligned,
  * used by no other call that may run at the same time; its content is free. */
 int fa_attn_chunks(const fa_pages *pages, uint32_t layer, const void *q, uint64_t q_stride, uint32_t n_heads,

@@ -260,6 +260,28 @@ def test_attention_of_few_chunks_in_a_small_and_a_large_table(t, heads, kvh, hd,
         assert bool(((got - want[: start[-1]]).abs() <= tol[: start[-1]]).all())
 
 
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,kvh,hd", [(4, 1, 64), (12, 3, 128), (32, 8, 128)])
+@pytest.mark.parametrize("qs,kvs,window", [([17], [17], 0), ([70], [70], 0), ([20], [900], 0), ([33, 0, 5], [400, 9, 5], 0), ([20, 4], [0, 0], 0),
+                                           ([150], [3], 0), ([40, 9], [130, 4], 33), ([64], [300], 1), ([128, 1], [128, 200], 0)])
+def test_attention_of_short_chunks_in_a_small_and_a_large_table(t, heads, kvh, hd, qs, kvs, window):
+    """more than 16 rows a kv head: the kernel for short calls and those for long caches, rows of any alignment"""
+    dtype = R.TYPES[t]
+    pages, table = R.make_cache(kvs, 1, kvh, hd, dtype, 43, junk=10 ** 6)
+    wide = torch.full((len(kvs), 1100), 10 ** 6, dtype=torch.int32, device="cuda")
+    wide[:, : table.shape[1]] = table
+    start = [sum(qs[:i]) for i in range(len(qs) + 1)]
+    for spare in (0, 3):  # rows 16-byte aligned, and not
+        q = randn(11, start[-1] + 1, heads * hd + spare, dtype=dtype)[:, spare:]
+        want, tol = R.attention(pages, table, 0, q.contiguous(), i32(start), i32(kvs), None, heads, 0.0, window)
+        for tb in (table, wide):
+            err, out = torch.zeros(1, dtype=torch.int32, device="cuda"), torch.full_like(q, 7.0)
+            attn(pages, tb, q, start, kvs, heads, window=window, out=out, err=err)
+            assert int(err) == 0 and bool((out[start[-1]:] == 7.0).all())
+            got = out[: start[-1]].double().view(-1, heads, hd)
+            assert bool(((got - want[: start[-1]]).abs() <= tol[: start[-1]]).all())
+
+
 @pytest.mark.parametrize("t", ["f16", "f32"])
 def test_attention_refuses_and_flags_in_a_small_table_too(t):
     """a chunk that is refused beside one that is not, and a page out of range, where each item is a cluster"""
