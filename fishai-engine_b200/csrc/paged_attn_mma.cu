@@ -468,17 +468,23 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_short(const AttnChunksPara
   const uint32_t n = s.hi > s.lo ? range_units<kShortPos>(s.lo, s.hi) : 0;
   const uint32_t *pt = p.pg.page_table + (uint64_t)s.chunk.seq * p.pg.max_pages;
   uint32_t u = cluster_ctarank(), t0 = (s.lo / kShortPos + u) * kShortPos;
-  // K and V of the tile at t to buffer `which`
+  // K and V of the tile at t, whose pages are looked up a tile ahead, to buffer `which`
+  PagePair ahead[2];
+  auto pages = [&](uint32_t t) {
+#pragma unroll
+    for (uint32_t h = 0; h < 2; ++h) ahead[h] = look_up(pt, t + h * kSub, s.lo, s.hi);
+  };
   auto fetch = [&](uint32_t t, uint32_t which) {
     const uint32_t k = smem_u32(dsm) + which * 2 * S::kTile;
 #pragma unroll
     for (uint32_t h = 0; h < 2; ++h) {
-      const PagePair pg = look_up(pt, t + h * kSub, s.lo, s.hi);
-      flag_bad_pages(p, pg);
-      stage<T, HD>(p, base, pg, s.head, 0, t + h * kSub, s.lo, s.hi, k + h * S::kHalf, tid, kThreads);
-      stage<T, HD>(p, base, pg, s.head, 1, t + h * kSub, s.lo, s.hi, k + S::kTile + h * S::kHalf, tid, kThreads);
+      flag_bad_pages(p, ahead[h]);
+      stage<T, HD>(p, base, ahead[h], s.head, 0, t + h * kSub, s.lo, s.hi, k + h * S::kHalf, tid, kThreads);
+      stage<T, HD>(p, base, ahead[h], s.head, 1, t + h * kSub, s.lo, s.hi, k + S::kTile + h * S::kHalf, tid, kThreads);
     }
+    pages(t + C * kShortPos);
   };
+  pages(t0);
   if (u < n) fetch(t0, 0);
   cp_commit();
   if (u + C < n) fetch(t0 + C * kShortPos, 1);
