@@ -34,9 +34,12 @@ constexpr uint32_t kBuf = kScanElems * kBeamMaxK;  // candidates of a tile
 constexpr uint32_t kPickThreads = 256;
 constexpr float kLog2e = 1.4426950408889634f;
 
+// A value's place in the order; + 0 makes +0.0 of -0.0: the two are equal, here
+// as in the comparisons and maxima that the bounds below are taken with.
+__device__ __forceinline__ uint32_t value_key(float x) { return float_key(x + 0.0f); }
 // (ordered value, lower token first) as one number; 0: no candidate
 __device__ __forceinline__ unsigned long long cand_key(float x, uint32_t token) {
-  return ((unsigned long long)float_key(x) << 32) | (uint32_t)~token;
+  return ((unsigned long long)value_key(x) << 32) | (uint32_t)~token;
 }
 
 __device__ __forceinline__ float ex2(float x) {  // 2^x, 2 ulp
@@ -266,7 +269,7 @@ __global__ void __launch_bounds__(kScanThreads, 4) k_beam_scan(const BeamParams 
         float g = t;
 #pragma unroll
         for (uint32_t o = 16; o; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xFFFFFFFFu, g, o));
-        if (tid % 32 == 0) tops[tid / 32] = float_key(g);
+        if (tid % 32 == 0) tops[tid / 32] = value_key(g);
         __syncthreads();
         unsigned long long v = tops[0];
 #pragma unroll
@@ -344,7 +347,7 @@ __device__ __forceinline__ bool better(const Best &a, const Best &b) {
   return a.hi != b.hi ? a.hi > b.hi : a.mid != b.mid ? a.mid > b.mid : a.lo > b.lo;
 }
 __device__ __forceinline__ unsigned long long double_key(double f) {
-  const unsigned long long b = __double_as_longlong(f);
+  const unsigned long long b = __double_as_longlong(f + 0.0);  // zeros of both signs are equal
   return (b >> 63) ? ~b : (b | 0x8000000000000000ull);
 }
 __device__ __forceinline__ double key_double(unsigned long long k) {

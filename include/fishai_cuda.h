@@ -465,7 +465,7 @@ int fa_sampler_freq(fa_sampler *s, uint32_t seq, uint32_t token, uint32_t *count
  * computed in 64 bits; those of one beam stand in the order of its logits.  A
  * beam with done[b][j] != 0 (done may be NULL) has the
  * one candidate (j, pad) at its own score, and its logits are not read.  The
- * k best candidates of a request, equal scores by lowest beam then token, go
+ * k best candidates of a request, equal scores (-0.0 and +0.0 among them) by lowest beam then token, go
  * to out_*[b][0 .. k) in descending order: score, parent beam, token, and
  * whether the new beam is done (its parent was, or the token is eos; eos =
  * FA_NO_TOKEN: none).  Logits of -inf and NaN are no candidates and add

@@ -1,0 +1,43 @@
+"""Calls at the edges of what the operators on paged K/V and the beam selection
+allow, against plain 64-bit forms."""
+import pytest
+
+torch = pytest.importorskip("torch")
+
+import paged_ref as R  # noqa: E402
+from test_gpu_paged import beam_check, i32, randn  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------ beam selection
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("vocab", [50, 4096, 4099, 40000])
+@pytest.mark.parametrize("k", [1, 4, 16, 64])
+def test_beam_select_zeros_of_both_signs_are_equal(t, vocab, k):
+    """ties go to the lowest token whatever the zeros' signs, and no candidate is lost to them"""
+    v = torch.arange(vocab, device="cuda")
+    zero = torch.zeros(vocab, device="cuda")
+    last = v % 4096 >= min(3072, vocab // 2)
+    low = -1.0 - v / vocab
+    x = torch.stack([torch.where(last & (v % 4 == 3), zero, -zero),    # a thread's largest is +0.0, its first equal -0.0
+                     torch.where(last, zero, -zero),
+                     torch.where(v % 2 == 0, zero, -zero),
+                     -zero,
+                     torch.where(v == 5, -zero, torch.where(v == 10, zero, low)),
+                     torch.where(v % 7 == 3, -zero, torch.where(v % 7 == 5, zero, low))]).to(R.TYPES[t])
+    assert bool(torch.signbit(x).any()) and not bool(torch.signbit(x[:3]).all())
+    n = x.shape[0]
+    beam_check(x, torch.tensor([[0.0, -0.0, -0.0, 0.0, -0.0, 0.0]], device="cuda"), None, k)
+    beam_check(x, torch.zeros(1, n, device="cuda"), None, k, eos=0)
+    for j in range(n):  # each row alone
+        beam_check(x[j: j + 1], torch.full((1, 1), -0.0, device="cuda"), None, k)
+
+
+def test_beam_select_scores_of_zero_of_both_signs_are_equal():
+    """finished beams stand at their own score; equal ones go to the lowest beam"""
+    x = randn(3, 4, 900)
+    done = i32([[1, 1, 1, 0]])
+    for scores in ([-0.0, 0.0, -0.0, -3.0], [0.0, -0.0, 0.0, -3.0], [-0.0, -0.0, 0.0, 0.0]):
+        for k in (1, 2, 3, 8):
+            beam_check(x, torch.tensor([scores], device="cuda"), done, k, pad=3)
