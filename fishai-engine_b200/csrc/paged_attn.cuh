@@ -97,8 +97,8 @@ struct Segment {  // a piece of an item
 // A CTA's walk along its stretch.  Every thread holds the same state.
 template <uint32_t R, uint32_t U, uint32_t OVER, uint32_t THREADS>
 struct Walk {
-  uint32_t left, per;     // cost of the stretch that is left, and of a whole one (below 2^32: the line has at most
-                          // 2^31 rows / R items of 2^25 / U units for at least 100 CTAs)
+  uint32_t left, per;     // cost of the stretch that is left, and of a whole one (start() refuses a line whose
+                          // stretches need more bits)
   uint32_t c, tile, head;
   uint32_t rem;           // cost into the current item; its first OVER stand for no work
   Chunk chunk;
@@ -122,10 +122,15 @@ struct Walk {
     uint64_t total = 0;
 #pragma unroll
     for (uint32_t w = 0; w < THREADS / 32; ++w) total += red[w];
-    per = (uint32_t)((total + gridDim.x - 1) / gridDim.x);
-    if (per < min_cost) per = min_cost;
-    const uint64_t at = (uint64_t)blockIdx.x * per;
     c = tile = head = rem = left = 0;
+    // 2^32 units a CTA, an hour of work and more: nothing is done (the same for all CTAs)
+    const uint64_t share = (total + gridDim.x - 1) / gridDim.x;
+    per = share > min_cost ? (uint32_t)share : min_cost;
+    if (share > 0xFFFFFFFFull) {
+      if (p.err && blockIdx.x == 0 && tid == 0) atomicOr(p.err, kFlagRange);
+      return;
+    }
+    const uint64_t at = (uint64_t)blockIdx.x * per;
     if (at >= total) return;  // the same for all threads of the CTA
     left = (uint32_t)min((uint64_t)per, total - at);
     // the chunk that holds `at`: blocks of THREADS chunks, then a scan

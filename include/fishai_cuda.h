@@ -347,6 +347,8 @@ int fa_rope_append(const fa_rope *r, const fa_pages *pages, uint32_t layer, int3
  * are left as they were.  q and out have the pages' type and rows of n_heads *
  * head_dim elements, q_stride and out_stride apart; out must not
  * overlap q, the pages or ws.
+ * A call of 2^32 tiles a CTA or more (an hour of work at least) sets
+ * FA_FLAG_RANGE and leaves those rows as they were.
  * The positions that some token of a chunk sees should hold finite K and V;
  * whatever is behind kv_len or before every token's window is not used.  A
  * page out of range (FA_FLAG_PAGE) spoils the chunk's own rows only.

@@ -5,7 +5,8 @@ import pytest
 torch = pytest.importorskip("torch")
 
 import paged_ref as R  # noqa: E402
-from test_gpu_paged import beam_check, i32, randn  # noqa: E402
+from fishai_engine import paged  # noqa: E402
+from test_gpu_paged import attn, beam_check, i32, randn  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -41,3 +42,18 @@ def test_beam_select_scores_of_zero_of_both_signs_are_equal():
     for scores in ([-0.0, 0.0, -0.0, -3.0], [0.0, -0.0, 0.0, -3.0], [-0.0, -0.0, 0.0, 0.0]):
         for k in (1, 2, 3, 8):
             beam_check(x, torch.tensor([scores], device="cuda"), done, k, pad=3)
+
+
+# ------------------------------------------------------------------ attention
+@pytest.mark.parametrize("t,heads,hd,chunks", [("f32", 4096, 8, 1000), ("f16", 4096, 64, 500)])
+def test_attention_of_more_work_than_the_split_counts_is_refused(t, heads, hd, chunks):
+    """chunks over a cache of 2^25 positions (one page again and again): 2^32 tiles a CTA and more are flagged, no row is written"""
+    most = 1 << 21
+    tiles, ctas = most * 16 // (64 if t == "f32" else 32), 3 * torch.cuda.get_device_properties(0).multi_processor_count
+    assert chunks * heads * tiles >= ctas << 32
+    pages = torch.zeros(1, 1, 2, heads, 16, hd, dtype=R.TYPES[t], device="cuda")
+    table = torch.zeros(1, most, dtype=torch.int32, device="cuda")
+    q = randn(1, chunks, heads * hd, dtype=R.TYPES[t])
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out = attn(pages, table, q, list(range(chunks + 1)), [16 * most] * chunks, heads, seqs=[0] * chunks, err=err)
+    assert int(err) == paged.FLAG_RANGE and bool((out == 7.0).all())
