@@ -264,6 +264,7 @@ int fa_attn_chunks(const fa_pages *pages, uint32_t layer, const void *q, uint64_
     return invalid(who, "n_heads is a multiple of the pages' kv heads, at most 32767");
   if (!std::isfinite(scale) || scale < 0 || scale > 1e30f) return invalid(who, "scale is a number from 0 to 1e30");
   if ((uint64_t)n_tokens * n_heads > 0x7FFFFFFFu) return invalid(who, "2^31 or more query rows");
+  if (n_chunks > 0x7FFFFFFFu) return invalid(who, "2^31 or more chunks");
   if (window > 0x7FFFFFFFu) window = 0;  // wider than any cache: none
   const uint64_t hd = pages->head_dim, qw = n_heads * hd;
   if (n_tokens > 1 && (q_stride < qw || out_stride < qw)) return invalid(who, "a row stride is smaller than the row");
