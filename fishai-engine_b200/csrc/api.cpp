@@ -639,6 +639,10 @@ int fa_kv_get(const fa_kv *kv, uint32_t seq, uint32_t layer, float *k_host, floa
   const size_t page_elems = (size_t)2 * KVH * 16 * hd, esz = c.f16 ? 2 : 4;
   std::vector<uint8_t> buf(page_elems * esz);
   std::vector<uint32_t> pt(c.max_pages);
+  if (c.lent) {  // fa_kv_wait; the copies below follow the default stream by themselves
+    const int rc = c.m->sync();
+    if (rc) return rc;
+  }
   API_CUDA(cudaMemcpy(pt.data(), c.page_table + (size_t)seq * c.max_pages, c.max_pages * 4, cudaMemcpyDeviceToHost));
   for (uint32_t p = 0; p < pages; ++p) {
     const uint8_t *src = (const uint8_t *)c.base + ((size_t)layer * c.layer_stride + (size_t)pt[p] * page_elems) * esz;
@@ -657,12 +661,23 @@ int fa_kv_get(const fa_kv *kv, uint32_t seq, uint32_t layer, float *k_host, floa
   }
   return FA_OK;
 }
-int fa_kv_pages(const fa_kv *kv, fa_pages *out) {
+int fa_kv_pages(fa_kv *kv, fa_pages *out) {
   API_NULL(kv);
   API_NULL(out);
   if (!kv->kv.m) return fail(FA_ERR_INVALID, "fa_kv_pages: the cache's model was freed");
   *out = kv->kv.pages();
+  kv->kv.lent = true;
   return FA_OK;
+}
+int fa_kv_wait(fa_kv *kv, void *stream) {
+  API_NULL(kv);
+  if (!kv->kv.m) return fail(FA_ERR_INVALID, "fa_kv_wait: the cache's model was freed");
+  const cudaStream_t st = stream ? (cudaStream_t)stream : cudaStreamLegacy;
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  API_CUDA(cudaStreamIsCapturing(st, &capture));
+  if (capture != cudaStreamCaptureStatusNone)  // the model's stream would become part of the capture
+    return fail(FA_ERR_INVALID, "fa_kv_wait: the stream is being captured");
+  return kv->kv.follow(st);
 }
 int fa_kv_fork(fa_kv *kv, uint32_t src, uint32_t dst) {
   API_NULL(kv);
@@ -715,6 +730,7 @@ int fa_forward(fa_model *fm, fa_kv *kv, uint32_t seq, const uint32_t *tokens, ui
     if (tokens[i] >= m.cfg.vocab_size) return fail(FA_ERR_INVALID, "token id out of range");
   if ((rc = m.ensure_rope(pos + 1))) return rc;
   API_CUDA(cudaSetDevice(m.device));
+  if ((rc = kv->kv.settle())) return rc;
   if (n > 1) return forward_compat(fm, kv, seq, tokens, n, pos, logits, argmax, hidden);
   float *hid_dev = nullptr;
   if (hidden) API_CUDA(cudaMalloc(&hid_dev, (size_t)m.cfg.n_layers * m.cfg.n_embd * 4));
@@ -761,6 +777,7 @@ int fa_prefill(fa_model *fm, fa_kv *kv, uint32_t seq, const uint32_t *tokens, ui
     if (tokens[i] >= m.cfg.vocab_size) return fail(FA_ERR_INVALID, "token id out of range");
   if ((rc = m.ensure_rope(start_pos + n))) return rc;
   API_CUDA(cudaSetDevice(m.device));
+  if ((rc = kv->kv.settle())) return rc;
   if (m.want_tc_prefill && m.tc_ok) {  // bf16 tensor-core path
     if ((rc = m.prefill_tc(kv->kv, seq, tokens, n, start_pos))) return rc;
     if (last_logits)
@@ -797,6 +814,7 @@ int fa_decode_greedy(fa_model *fm, fa_kv *kv, uint32_t seq, uint32_t first_token
   if (first_token >= m.cfg.vocab_size) return fail(FA_ERR_INVALID, "token id out of range");
   if ((rc = m.ensure_rope(pos + steps))) return rc;
   API_CUDA(cudaSetDevice(m.device));
+  if ((rc = kv->kv.settle())) return rc;
   if ((rc = ensure_ids(m, steps))) return rc;
   if ((rc = set_state(m, m.ws.state, first_token, pos, kv->kv.len[seq], 0))) return rc;
   if ((rc = m.run_steps(kv->kv, seq, steps))) return rc;
@@ -1279,6 +1297,7 @@ extern "C" int fa_decode_batch(fa_model *fm, fa_kv *kv, uint32_t b, const uint32
   int rc;
   if ((rc = sampler_keys(s, sp))) return rc;
   API_CUDA(cudaStreamSynchronize(s->stream));  // observes / resets queued on the sampler's stream
+  if ((rc = kv->kv.settle())) return rc;
   return m.decode_batch(kv->kv, b, tokens, pos, sp, steps, ids_out, logits_out);
 }
 

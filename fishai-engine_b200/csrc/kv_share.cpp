@@ -95,11 +95,26 @@ int KvCache::copy(const std::vector<Move> &moves) {
   return FA_OK;
 }
 
+// The model's stream is a non-blocking one, so nothing else orders it with the
+// stream on which a caller has the operators on pages work.  An event costs less
+// than a host wait, and the calls behind it end with one.
+int KvCache::follow(cudaStream_t st) {
+  CUDA_TRY(cudaSetDevice(m->device));
+  if (!order) CUDA_TRY(cudaEventCreateWithFlags(&order, cudaEventDisableTiming));
+  cudaError_t e = cudaEventRecord(order, st);
+  if (e == cudaSuccess) e = cudaStreamWaitEvent(m->stream, order, 0);
+  if (e == cudaSuccess) return FA_OK;
+  cudaGetLastError();  // not sticky: later launch checks must not see it
+  return fail(FA_ERR_CUDA, std::string("the cache cannot follow the caller's stream: ") + cudaGetErrorString(e));
+}
+int KvCache::settle() { return lent && m ? follow(cudaStreamLegacy) : FA_OK; }
+
 int KvCache::fork(uint32_t src, uint32_t dst) {
   if (!m) return fail(FA_ERR_INVALID, "the cache's model was freed");
   if (src == dst) return FA_OK;
   CUDA_TRY(cudaSetDevice(m->device));
   TRY(ensure_scratch());  // nothing may fail between the table's change and its upload
+  TRY(settle());
   const uint32_t full = len[src] / 16, rest = len[src] % 16;
   uint32_t *s = row(src), *d = row(dst);
   for (uint32_t i = 0; i < full; ++i) {
@@ -126,6 +141,7 @@ int KvCache::reorder(const uint32_t *parents, uint32_t n) {
   if (same) return FA_OK;
   CUDA_TRY(cudaSetDevice(m->device));
   TRY(ensure_scratch());
+  TRY(settle());
   const std::vector<uint32_t> old(table.begin(), table.begin() + (size_t)n * max_pages), was(len.begin(), len.begin() + n);
   // one child of each parent takes over the parent's own pages: itself, else
   // the first; the other children get free ones
@@ -172,6 +188,7 @@ int KvCache::truncate(uint32_t seq, uint32_t n) {
   if (!m) return fail(FA_ERR_INVALID, "the cache's model was freed");
   CUDA_TRY(cudaSetDevice(m->device));
   TRY(ensure_scratch());
+  TRY(settle());
   for (uint32_t i = full; i < max_pages; ++i)
     if (refs[r[i]] > 1) {
       const uint32_t page = r[i];
@@ -192,6 +209,7 @@ int KvCache::compact(uint32_t seq, const uint32_t *keep, uint32_t n) {
   if (!m) return fail(FA_ERR_INVALID, "the cache's model was freed");
   CUDA_TRY(cudaSetDevice(m->device));
   TRY(ensure_scratch());
+  TRY(settle());
   // pages that are written become the sequence's own, with their contents
   uint32_t *r = row(seq);
   std::vector<Move> moves;

@@ -541,6 +541,7 @@ KvCache::~KvCache() {
   cudaFree(base);
   cudaFree(page_table);
   cudaFree(scratch);
+  if (order) cudaEventDestroy(order);
 }
 
 KvView KvCache::view() const {

@@ -225,6 +225,8 @@ struct KvCache {
   std::vector<uint32_t> table;      // host copy of page_table
   std::vector<uint32_t> refs, free_pages;
   uint32_t *scratch = nullptr;      // device lists of the page operators
+  bool lent = false;                // fa_kv_pages was called: callers' streams may work on the pages
+  cudaEvent_t order = nullptr;
   ~KvCache();
   KvView view() const;
   fa_pages pages() const;
@@ -233,6 +235,8 @@ struct KvCache {
   int truncate(uint32_t seq, uint32_t n);
   int compact(uint32_t seq, const uint32_t *keep, uint32_t n);
   uint32_t used_pages() const;
+  int follow(cudaStream_t st);  // the model's stream goes on behind what is on `st` now
+  int settle();                 // before any work on the pages: behind the default stream, where they are lent
 
  private:
   struct Move {

@@ -151,6 +151,7 @@ SIGNATURES = {
     "fa_sdpa_noalloc": ([_vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32, _vp, _vp], _i),
     "fa_sdpa_host": ([_pf, _pf, _pf, _u32, _u32, _u32, _u32, _u32, _pf], _i),
     "fa_kv_pages": ([_vp, C.POINTER(fa_pages)], _i),
+    "fa_kv_wait": ([_vp, _vp], _i),
     "fa_kv_fork": ([_vp, _u32, _u32], _i),
     "fa_kv_reorder": ([_vp, _pu32, _u32], _i),
     "fa_kv_truncate": ([_vp, _u32, _u32], _i),

@@ -87,6 +87,13 @@ class KVCache:
         a, p = L.u32_array(keep)
         L.check(L.lib().fa_kv_compact(self._h, seq, p, a.size))
 
+    def wait(self, stream: int = 0):
+        """The calls on this cache after this one follow what is on `stream` (a
+        cudaStream_t as int) now.  For work of paged's operators on the pages
+        (PagedKV.of) on another stream than the default one, which every call
+        follows by itself."""
+        L.check(L.lib().fa_kv_wait(self._h, stream))
+
     def pages_used(self):
         """(pages that hold positions, each shared one once; pages of the cache)"""
         u, t = C.c_uint32(), C.c_uint32()

@@ -103,7 +103,11 @@ class PagedKV:
 
     @classmethod
     def of(cls, kv_cache) -> "PagedKV":
-        """the pages of a model's KVCache (kept alive by this object)"""
+        """The pages of a model's KVCache (kept alive by this object).  The
+        cache's own calls follow work on the default stream; for work on another
+        one call KVCache.wait first.  Its lengths do not count rows that
+        rope_append writes behind them, and a row written below them changes in
+        every sequence that shares its page."""
         self = cls.__new__(cls)
         c = L.fa_pages()
         L.check(L.lib().fa_kv_pages(kv_cache._h, C.byref(c)))

@@ -279,8 +279,21 @@ typedef struct {
 #define FA_FLAG_PAGE 16   /* *err: a page number >= n_pages */
 #define FA_FLAG_RANGE 32  /* *err: a sequence, slot, length, row or index out of range */
 #define FA_FLAG_TIMEOUT 64  /* *err: a bounded device wait gave up; the outputs are not complete */
-/* the pages of a cache, for the calls below; valid until the cache is freed */
-int fa_kv_pages(const fa_kv *kv, fa_pages *out);
+/* The pages of a cache, for the calls below; valid until the cache is freed.
+ * The cache's own calls (fork, reorder, compact, fa_kv_get, prefill, decode ..)
+ * work on the model's stream.  From now on each of them follows what is on the
+ * legacy default stream when it is called; work on another stream has to be
+ * announced by fa_kv_wait or be done before.  They return when they are done,
+ * so what a caller enqueues behind them follows them.
+ * A sequence's length counts what the cache's own calls appended, not rows
+ * that fa_rope_append put behind it: a fork leaves those behind and the next
+ * prefill or decode step overwrites them.  A row that is written below the
+ * length changes in every sequence that shares its page. */
+int fa_kv_pages(fa_kv *kv, fa_pages *out);
+/* The calls on the cache after this one follow what is on `stream` now
+ * (cudaStream_t of the model's device, not one that is being captured; NULL:
+ * the legacy default stream).  Does not wait itself. */
+int fa_kv_wait(fa_kv *kv, void *stream);
 
 /* Rotary positions.  Pair i of the first rot_dim elements of a head (elements
  * 2i and 2i+1, or i and i + rot_dim/2) at position p is turned by p f_i, where
