@@ -105,12 +105,24 @@ int check_pages(const char *who, const fa_pages *p, bool table) {
     if (rc_ != FA_OK) return rc_;  \
   } while (0)
 
-bool overlap(const void *a, uint64_t an, const void *b, uint64_t bn) {
-  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-  return x < y + bn && y < x + an;
+// n rows of `bytes` each, `stride` bytes apart
+struct Rows {
+  uintptr_t at;
+  uint64_t stride, bytes;
+};
+Rows rows_of(const void *p, uint64_t stride, uint64_t row, uint32_t es) { return {reinterpret_cast<uintptr_t>(p), stride * es, row * es}; }
+// Whether n rows of a and of b share a byte.  With one stride, as column ranges of
+// one buffer have, row j of b starts r bytes behind the start of a's row j + d and
+// ends before a's row j + d + 2; with two, whole spans are compared.
+bool overlap(uint64_t n, const Rows &a, const Rows &b) {
+  if (n > 1 && a.stride == b.stride) {
+    if (a.at > b.at) return overlap(n, b, a);
+    const uint64_t d = (b.at - a.at) / a.stride, r = (b.at - a.at) % a.stride;
+    return (d < n && r < a.bytes) || (d + 1 < n && r + b.bytes > a.stride);
+  }
+  const uint64_t an = (n - 1) * a.stride + a.bytes, bn = (n - 1) * b.stride + b.bytes;
+  return a.at < b.at + bn && b.at < a.at + an;
 }
-// bytes from the first to behind the last element of n rows
-uint64_t span(uint64_t n, uint64_t stride, uint64_t row, uint32_t es) { return n ? ((n - 1) * stride + row) * es : 0; }
 
 }  // namespace
 
@@ -218,10 +230,8 @@ int fa_rope_append(const fa_rope *r, const fa_pages *pages, uint32_t layer, int3
     if (reinterpret_cast<uintptr_t>(b) % ei) return invalid(who, "q, k or v is not aligned to its element type");
   if (reinterpret_cast<uintptr_t>(out) % eo) return invalid(who, "out is not aligned to its element type");
   const bool in_place = q == out && in_dtype == pages->dtype && (q_stride == out_stride || n_tokens == 1);
-  if (!in_place && overlap(q, span(n_tokens, q_stride, qw, ei), out, span(n_tokens, out_stride, qw, eo))) {
-    // rows of one fused buffer may interleave with out only when out is q itself
+  if (!in_place && overlap(n_tokens, rows_of(q, q_stride, qw, ei), rows_of(out, out_stride, qw, eo)))
     return invalid(who, "out overlaps q without being q");
-  }
   OnDevice dev(who);
   TRY(dev.add("pages.base", pages->base));
   TRY(dev.add("pages.page_table", pages->page_table));
@@ -277,7 +287,7 @@ int fa_attn_chunks(const fa_pages *pages, uint32_t layer, const void *q, uint64_
   const uint32_t es = elem_size(pages->dtype);
   if (reinterpret_cast<uintptr_t>(q) % es || reinterpret_cast<uintptr_t>(out) % es)
     return invalid(who, "q or out is not aligned to its element type");
-  if (overlap(q, span(n_tokens, q_stride, qw, es), out, span(n_tokens, out_stride, qw, es)))
+  if (overlap(n_tokens, rows_of(q, q_stride, qw, es), rows_of(out, out_stride, qw, es)))
     return invalid(who, "out overlaps q");
   OnDevice dev(who);
   TRY(dev.add("pages.base", pages->base));

@@ -6,7 +6,7 @@ torch = pytest.importorskip("torch")
 
 import paged_ref as R  # noqa: E402
 from fishai_engine import paged  # noqa: E402
-from test_gpu_paged import attn, beam_check, i32, randn  # noqa: E402
+from test_gpu_paged import attn, beam_check, i32, randn, rope_case, rope_check, same_bits  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -57,3 +57,26 @@ def test_attention_of_more_work_than_the_split_counts_is_refused(t, heads, hd, c
     err = torch.zeros(1, dtype=torch.int32, device="cuda")
     out = attn(pages, table, q, list(range(chunks + 1)), [16 * most] * chunks, heads, seqs=[0] * chunks, err=err)
     assert int(err) == paged.FLAG_RANGE and bool((out == 7.0).all())
+
+
+# ------------------------------------------------------------------ buffers
+@pytest.mark.parametrize("n", [1, 3, 40, 150])
+@pytest.mark.parametrize("order", ["q first", "out first"])
+def test_q_and_out_as_column_ranges_of_one_buffer(n, order):
+    """rows of both interleave in memory, but no element is shared"""
+    pages, table = R.make_cache([200], 1, 2, 64, torch.float16, 12)
+    buf = randn(5, n, 1024 + 8, dtype=torch.float16)
+    a, b = buf[:, :512], buf[:, 520:]
+    q, out = (a, b) if order == "q first" else (b, a)
+    was = buf.clone()
+    attn(pages, table, q, [0, n], [200], 8, out=out)
+    want, tol = R.attention(pages, table, 0, q.contiguous(), i32([0, n]), i32([200]), None, 8, 0.0, 0)
+    assert bool(((out.double().reshape(want.shape) - want).abs() <= tol).all())
+    assert same_bits(q, was[:, :512] if order == "q first" else was[:, 520:]) and same_bits(buf[:, 512: 520], was[:, 512: 520])
+    c = rope_case(n, 8, 2, 64, torch.float16, torch.float16, seed=7)
+    q.copy_(c["q"])
+    paged.rope_append(paged.PagedKV(c["pages"], c["table"]), 1, c["r"], q, c["k"], c["v"], i32(c["pos"]), i32(c["seqs"]), out,
+                      slots=i32(c["slots"]))
+    c["out"] = out.contiguous()
+    rope_check(c, 8, 2, 64, "interleaved")
+    assert same_bits(q, c["q"])
