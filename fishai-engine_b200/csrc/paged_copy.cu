@@ -81,11 +81,11 @@ __global__ void __launch_bounds__(kCompactThreads) k_page_compact(const PageComp
       t.to[u] = kNone;
       if (e0 >= total || e >= total) continue;
       const uint32_t from = __ldg(keep + j);
-      if (from == j) continue;
       if (from < j || from >= cap || (j && __ldg(keep + j - 1) >= from)) {
         bad |= kFlagRange;
         continue;
       }
+      if (from == j) continue;
       const uint32_t sp = __ldg(pt + from / kPageLen), dp = __ldg(pt + j / kPageLen);
       if (sp >= p.pg.n_pages || dp >= p.pg.n_pages) {
         bad |= kFlagPage;

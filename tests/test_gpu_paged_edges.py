@@ -80,3 +80,18 @@ def test_q_and_out_as_column_ranges_of_one_buffer(n, order):
     c["out"] = out.contiguous()
     rope_check(c, 8, 2, 64, "interleaved")
     assert same_bits(q, c["q"])
+
+
+# ------------------------------------------------------------------ page copies
+@pytest.mark.parametrize("keep,moved", [([5, 1], {0: 5}), ([3, 1, 2, 9], {0: 3, 3: 9}), ([0, 7, 2, 3, 20], {1: 7, 4: 20}), ([1, 1], {0: 1})])
+def test_compact_flags_a_position_that_does_not_ascend_where_it_would_stay(keep, moved):
+    """keep[j] == j needs no copy, but is out of order behind a larger one"""
+    pages, table = R.make_cache([40], 2, 2, 64, torch.float16, 24)
+    want = pages.clone()
+    at = lambda p: (slice(None), int(table[0, p // 16]), slice(None), slice(None), p % 16)  # noqa: E731
+    for j, p in moved.items():
+        want[at(j)] = pages[at(p)]
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    paged.compact(paged.PagedKV(pages, table), i32([0]), i32(keep), i32([0, len(keep)]), err=err)
+    assert int(err) == paged.FLAG_RANGE
+    assert same_bits(pages, want)
