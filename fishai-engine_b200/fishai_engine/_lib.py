@@ -209,6 +209,22 @@ def check(rc: int) -> None:
         raise FishaiError(rc, last_error())
 
 
+def u32(**values):
+    """refuses what ctypes would cut to 32 bits"""
+    for name, v in values.items():
+        if not 0 <= v <= 0xFFFFFFFF:
+            raise ValueError(f"{name} = {v}: a whole number below 2^32 is needed")
+
+
+def u32_list(seq):
+    """u32_array of positions or sequence numbers, none of them cut to 32 bits"""
+    import numpy as np
+    a = np.asarray(seq)
+    if a.size and (a.dtype.kind not in "iu" or a.min() < 0 or a.max() > 0xFFFFFFFF):
+        raise ValueError("whole numbers below 2^32 are needed")
+    return u32_array(a)
+
+
 def u32_array(seq):
     import numpy as np
     a = np.ascontiguousarray(np.asarray(seq, dtype=np.uint32))

@@ -36,6 +36,8 @@ def select(logits, scores, done, out_scores, out_parents, out_tokens, out_done, 
     ld, inner = logits.stride()
     if rows != nb * beams or (inner != 1 and vocab > 1) or b[0] != nb:
         raise ValueError(f"logits: [{nb * beams}, vocab] with consecutive elements, and out of {nb} rows")
+    if pad >> 32 or (eos != NO_TOKEN and eos >> 32):
+        L.u32(pad=pad, eos=eos)
     wp, wn = _space(workspace)
     rc = L.lib().fa_beam_select(
         logits.data_ptr(), dt, ld if rows > 1 else vocab, nb, beams, vocab, _grid(scores, "scores", a, False),

@@ -69,22 +69,25 @@ class KVCache:
     def fork(self, src: int, dst: int):
         """sequence dst becomes a copy of sequence src: whole pages are shared,
         a partly filled last page is copied"""
+        L.u32(src=src, dst=dst)
         L.check(L.lib().fa_kv_fork(self._h, src, dst))
 
     def reorder(self, parents):
         """sequence i becomes a copy of what sequence parents[i] was, all at once
         (the step between two selections of a beam search)"""
-        a, p = L.u32_array(parents)
+        a, p = L.u32_list(parents)
         L.check(L.lib().fa_kv_reorder(self._h, p, a.size))
 
     def truncate(self, seq: int, length: int):
         """drops the positions from `length` on"""
+        L.u32(seq=seq, length=length)
         L.check(L.lib().fa_kv_truncate(self._h, seq, length))
 
     def compact(self, seq: int, keep):
         """keeps the given ascending positions, as positions 0, 1, ...; their keys
         stay turned as they were stored"""
-        a, p = L.u32_array(keep)
+        L.u32(seq=seq)
+        a, p = L.u32_list(keep)
         L.check(L.lib().fa_kv_compact(self._h, seq, p, a.size))
 
     def wait(self, stream: int = 0):

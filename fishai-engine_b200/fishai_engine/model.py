@@ -176,6 +176,7 @@ class ModelWeights:
         """Beam search (fa_generate_beams): [(ids, sum of log-probabilities)],
         best score / length^length_penalty first; ids include the eos."""
         p, pp = L.u32_array(prompt_tokens)
+        L.u32(n_beams=n_beams, max_new=max_new, eos=0 if eos in (None, -1) else eos)
         ids = np.zeros((n_beams, max_new), dtype=np.uint32)
         n, sc = np.zeros(n_beams, dtype=np.uint32), np.zeros(n_beams, dtype=np.float32)
         c = L.fa_beam_config(n_beams, max_new, L.NO_TOKEN if eos is None else eos, length_penalty, kv_dtype)

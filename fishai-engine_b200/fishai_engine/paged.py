@@ -141,6 +141,7 @@ class Rope:
             raise ValueError(f"layout is one of {sorted(_LAYOUTS)}, scaling one of {sorted(_SCALINGS)}")
         self._h = None
         self.head_dim, self.rot_dim = head_dim, head_dim if rot_dim is None else rot_dim
+        L.u32(head_dim=head_dim, rot_dim=self.rot_dim, context=context)
         c = L.fa_rope_config(head_dim, self.rot_dim, _LAYOUTS[layout], _SCALINGS[scaling], base, factor, context,
                              low_turns, high_turns, beta_fast, beta_slow, attn_factor)
         h = C.c_void_p()
@@ -168,6 +169,8 @@ def rope_append(kv: PagedKV, layer: int, rope: Rope, q, k, v, positions, seqs, o
     projection).  seqs[t] = NO_TOKEN leaves a row out."""
     n = q.shape[0]
     dt = _code(q, "q")
+    if layer >> 32:
+        L.u32(layer=layer)
     if k.dtype != q.dtype or v.dtype != q.dtype:
         raise ValueError("q, k and v have one element type")
     if _code(out, "out") != kv.dtype:
@@ -210,8 +213,8 @@ def attention(kv: PagedKV, layer: int, q, q_start, kv_len, out, max_q: int, work
     n, t = kv_len.shape[0], q.shape[0]
     if _code(q, "q") != kv.dtype or out.dtype != q.dtype:
         raise ValueError("q and out have the pages' element type")
-    if window < 0 or max_q < 0:
-        raise ValueError("window and max_q are not negative")
+    if (layer | max_q | window) >> 32:
+        L.u32(layer=layer, max_q=max_q, window=window)
     hd = kv.head_dim
     width = _width(q, hd)
     qp, qs = _rows(q, "q", t, width)

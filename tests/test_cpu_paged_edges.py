@@ -1,8 +1,12 @@
 """Calls at the edges of what the paged operators and the beam selection allow,
 as the host takes them: no GPU needed, no pointer is read."""
+import numpy as np
 import pytest
 
 from fishai_engine import _lib as L
+from fishai_engine import beam, paged
+from fishai_engine.kv_cache import KVCache
+from fishai_engine.model import ModelWeights
 from test_cpu_paged import P, call_attn, call_rope, pages
 
 
@@ -40,3 +44,54 @@ def test_overlap_of_rows_of_two_strides_or_types_goes_by_the_whole_span():
     kw.update(k=P * 256, v=P * 512, ks=128, vs=128, dt=L.KV_F32)  # q of four bytes, out of two: one stride in bytes
     for out, shared in ((P * 64 + 512, False), (P * 64 + 510, True), (P * 64 + 768, False), (P * 64 + 770, True), (P * 64, True)):
         assert refused_as_overlapping(call_rope(pg, out=out, os=512, **kw)) == shared, out
+
+
+BIG = 1 << 32  # would arrive as 0
+
+
+def test_wrappers_refuse_numbers_beyond_32_bits():
+    import torch
+    kv = paged.PagedKV(torch.zeros(1, 4, 2, 2, 16, 64), torch.zeros(2, 2, dtype=torch.int32))
+    q, i = torch.zeros(3, 128), torch.zeros(3, dtype=torch.int32)
+    ws = torch.empty(paged.workspace_bytes(64), dtype=torch.uint8)
+    for layer in (BIG, -BIG, -1):
+        with pytest.raises(ValueError):
+            paged.rope_append(kv, layer, paged.Rope(64), q, q.clone(), q.clone(), i, i, q.clone())
+        with pytest.raises(ValueError):
+            paged.attention(kv, layer, q, i, i[:2], q.clone(), 3, ws)
+    for bad in (dict(max_q=BIG), dict(max_q=-1), dict(window=BIG + 5), dict(window=-1)):
+        with pytest.raises(ValueError):
+            paged.attention(kv, 0, q, i, i[:2], q.clone(), **{"max_q": 3, **bad}, workspace=ws)
+    for bad in (dict(head_dim=BIG + 64), dict(rot_dim=BIG + 64), dict(rot_dim=-2), dict(context=BIG + 1)):
+        with pytest.raises(ValueError):
+            paged.Rope(**{"head_dim": 64, **bad})
+    sc, ii = torch.zeros(2, 3), torch.zeros(2, 3, dtype=torch.int32)
+    for bad in (dict(eos=BIG + 2), dict(eos=-2), dict(pad=BIG), dict(pad=-1)):
+        with pytest.raises(ValueError):
+            beam.select(torch.zeros(6, 10), sc, ii, sc, ii, ii, ii, ws, **bad)
+
+
+class NoLibrary:
+    """a cache or model whose calls would reach the library with a null handle, which answers ERR_INVALID"""
+    _h = None
+
+
+@pytest.mark.parametrize("call", [lambda kv: kv.fork(BIG, 0), lambda kv: kv.fork(0, BIG + 1), lambda kv: kv.fork(-1, 0),
+                                  lambda kv: kv.truncate(0, BIG + 5), lambda kv: kv.truncate(BIG, 1), lambda kv: kv.truncate(0, -1),
+                                  lambda kv: kv.reorder(np.array([0, BIG])), lambda kv: kv.reorder(np.array([-1])), lambda kv: kv.reorder([0, BIG]),
+                                  lambda kv: kv.compact(BIG, [0]), lambda kv: kv.compact(0, np.array([0, BIG + 3])), lambda kv: kv.compact(0, [-1])])
+def test_cache_calls_refuse_numbers_beyond_32_bits(call):
+    class Cache(NoLibrary, KVCache):
+        def __init__(self):
+            pass
+    with pytest.raises(ValueError):
+        call(Cache())
+
+
+@pytest.mark.parametrize("bad", [dict(n_beams=BIG + 2), dict(n_beams=-1), dict(max_new=-1), dict(eos=BIG), dict(eos=-2), dict(max_new=BIG + 1)])
+def test_generate_beams_refuses_numbers_beyond_32_bits(bad):
+    class Model(NoLibrary, ModelWeights):
+        def __init__(self):
+            pass
+    with pytest.raises(ValueError):
+        Model().generate_beams(**{**dict(prompt_tokens=[5], n_beams=2, max_new=2), **bad})
