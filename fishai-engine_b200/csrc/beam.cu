@@ -9,6 +9,15 @@
 // log-sum-exp.  k_beam_pick: one CTA per request joins the ranges' sums in 64
 // bits and picks the k best of beams x ranges x k candidates.
 //
+// The sum of a range is f32, so that an exponential is one instruction: the scan
+// is bound by its instructions.  With e = 2^-24: an exponential is good to 4 e and
+// its argument to 3 e times its distance d from the maximum, which over a row's
+// weights costs 3 e ln(vocab) at most (their mean d is below their entropy); a
+// tile's 16 add 9 e, each tile of a thread 5 e (the sum, and a factor where the
+// maximum moves), the warp's, the CTA's and the ranges' joins 48 e.  In all less than
+// (128 + vocab / 512) e in the log, which only the order of different beams feels
+// (measured over rows of 100 to 10^6 normal logits: 2.5e-7 at most).
+//
 // Candidates of a range: what beats the k-th best of the list so far goes to a
 // buffer, and the list is made anew, by counting ranks, after the first tile of
 // 4096 logits and then after groups of 1, 2, 4, .. tiles: in random order each

@@ -477,7 +477,10 @@ int fa_sampler_freq(fa_sampler *s, uint32_t seq, uint32_t token, uint32_t *count
  * (device, ld elements apart, type FA_KV_*) belongs to beam j of request b;
  * its candidates are (j, v), v < vocab, with the score
  *   scores[b][j] + logit_v - log(sum over the row of exp(logit)),
- * computed in 64 bits; those of one beam stand in the order of its logits.  A
+ * computed in 64 bits from a sum made in f32, whose log is off by at most
+ * (128 + vocab / 512) 2^-24 (2.3e-5 at 128256; some 10^-7 in practice): candidates of
+ * two beams that are nearer than twice that may change places.  Those of one
+ * beam stand in the order of its logits.  A
  * beam with done[b][j] != 0 (done may be NULL) has the
  * one candidate (j, pad) at its own score, and its logits are not read.  The
  * k best candidates of a request, equal scores (-0.0 and +0.0 among them) by lowest beam then token, go

@@ -6,7 +6,7 @@ torch = pytest.importorskip("torch")
 
 import paged_ref as R  # noqa: E402
 from fishai_engine import paged  # noqa: E402
-from test_gpu_paged import attn, beam_check, i32, randn, rope_case, rope_check, same_bits  # noqa: E402
+from test_gpu_paged import attn, beam_check, beam_run, i32, randn, rope_case, rope_check, same_bits  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -42,6 +42,29 @@ def test_beam_select_scores_of_zero_of_both_signs_are_equal():
     for scores in ([-0.0, 0.0, -0.0, -3.0], [0.0, -0.0, 0.0, -3.0], [-0.0, -0.0, 0.0, 0.0]):
         for k in (1, 2, 3, 8):
             beam_check(x, torch.tensor([scores], device="cuda"), done, k, pad=3)
+
+
+def lse_bound(vocab):
+    """what fa_beam_select allows a row's log-sum to be off by"""
+    return (128 + vocab / 512) * 2.0 ** -24
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("vocab,spread", [(100, 3.0), (32000, 3.0), (128256, 0.05), (128256, 3.0), (128256, 12.0)])
+def test_beam_select_tells_beams_apart_beyond_the_bound_of_the_sum(t, vocab, spread):
+    """the same logits in another order (one exact sum, other f32 ones), scores just more than twice the bound apart"""
+    gap = 2.05 * lse_bound(vocab)
+    for seed in range(6):
+        row = (spread * randn(seed, vocab)).to(R.TYPES[t])
+        row[0] = 14.0 * spread  # the best of every row by far, in another place of each
+        g = torch.Generator("cuda").manual_seed(seed)
+        x = torch.stack([row[torch.randperm(vocab, device="cuda", generator=g)] for _ in range(8)])
+        place = torch.randperm(8, generator=torch.Generator().manual_seed(seed))
+        scores = (-1.0 - gap * place.double()).float()[None].cuda()
+        got = beam_run(x, scores, None, 8)
+        want = R.beam_select(x.cpu(), scores.cpu(), None, 8, 2, 0)
+        assert got[1].tolist() == [torch.argsort(place).tolist()] and torch.equal(got[1], want[1]) and torch.equal(got[2], want[2])
+        assert bool(((got[0].double() - want[0]).abs() <= lse_bound(vocab) + 2.0 ** -24 * want[0].abs()).all())
 
 
 # ------------------------------------------------------------------ attention
