@@ -265,7 +265,7 @@ int fa_sdpa_noalloc(const float *q_dev, const float *k_dev, const float *v_dev, 
  *  - indices in device memory (pages, sequences, slots, lengths) are checked
  *    by the kernels: one out of range sets a bit in *err (device uint32, not
  *    cleared by the call; NULL: not reported) and is skipped, the rows or
- *    copies that it names stay as they were.
+ *    copies that it names stay as they were (but see fa_attn_chunks for pages).
  *  - element types are FA_KV_F32, FA_KV_F16, FA_KV_BF16; sums are f32. */
 typedef struct {
   void *base;             /* [n_layers][n_pages][k | v][n_kv_heads][16][head_dim], 16-byte aligned */
@@ -364,7 +364,12 @@ int fa_rope_append(const fa_rope *r, const fa_pages *pages, uint32_t layer, int3
  * FA_FLAG_RANGE and leaves those rows as they were.
  * The positions that some token of a chunk sees should hold finite K and V;
  * whatever is behind kv_len or before every token's window is not used.  A
- * page out of range (FA_FLAG_PAGE) spoils the chunk's own rows only.
+ * page out of range (FA_FLAG_PAGE) is read as zeros: it spoils the rows of its
+ * own chunk, which are written all the same, and no others.
+ * Scores, maxima, sums of weights and outputs are f32.  Over f16 and bf16 pages
+ * of head size 64 and 128 the weights are rounded to the pages' type for the
+ * product with V (relative 2^-11 or 2^-8 each; their sum is taken before), with
+ * other sizes and types they are not.  Scaled scores have to stay below 2^127.
  * max_q and the table's width (max_pages) choose the kernels: the tighter they
  * are, the faster a short call.
  * ws: at least fa_attn_chunks_ws(...) bytes of device memory, 16-byte aligned,
