@@ -3,7 +3,9 @@
 // paged_attn_any.cu, products on mma.sync m16n8k16 with f32 accumulators.  The
 // weights p = 2^(s - m) <= 1 are rounded to the cache's type for the product
 // with V (the type V itself was rounded to); their sum is taken before that
-// rounding, in f32.
+// rounding, in f32.  In f16 they are 2^15 times that, and so are their sums: f16
+// has full precision down to 2^-14 and nothing below 2^-25, and beside one
+// large weight the small ones of a long cache may be most of the output.
 //
 // HBM bounds it: every K and V row is used for at most 16 rows of Q, far below
 // the 250 operations a byte where tensor cores would bind, so all that counts
@@ -68,6 +70,8 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     return *reinterpret_cast<const uint32_t *>(&h);
   }
 }
+template <typename T>
+constexpr float kLift = __is_same(T, __half) ? 15.0f : 0.0f;  // weights are 2^(s - m + kLift)
 template <typename T>
 __device__ __forceinline__ T round_to(float x) {
   if constexpr (__is_same(T, __half)) return __float2half_rn(x);
@@ -166,7 +170,7 @@ struct Rows {
       for (uint32_t j = 0; j < kSub / 8; ++j)
 #pragma unroll
         for (uint32_t e = 2 * i; e < 2 * i + 2; ++e) {
-          s[j][e] = ex2(fmaf(s[j][e], p.scale_log2, -ms));
+          s[j][e] = ex2(fmaf(s[j][e], p.scale_log2, kLift<T> - ms));
           sum += s[j][e];
         }
       l[i] = fmaf(l[i], f, sum);  // of this thread's columns: summed over the four at the end

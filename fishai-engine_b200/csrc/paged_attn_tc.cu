@@ -28,7 +28,9 @@
 // The reference point m of a row only moves when a maximum exceeds it by 2^8:
 // weights stay below 2^8 and sums in f32 are exact to the same relative error,
 // and the output in tensor memory is rescaled only then (by the softmax warps,
-// after the P V before it is done).
+// after the P V before it is done).  In f16 the weights and their sums are 2^7
+// times that, up to 2^15: they keep their full precision down to 2^-21 of the
+// largest (paged_attn_mma.cu).
 // Waits are bounded; one that runs out sets an abort flag that the others see,
 // and the kernel drains its copies and MMAs, frees the tensor memory and sets
 // FA_FLAG_TIMEOUT.
@@ -307,7 +309,8 @@ __device__ void softmax_role(const AttnChunksParams &p, TcWalk<G> w, TcBars &b, 
         }
       }
       const float ms = m == -INFINITY ? 0.0f : m;
-      const uint64_t scale = pair(p.scale_log2, p.scale_log2), minus_m = pair(-ms, -ms);
+      constexpr float kLift = __is_same(T, __half) ? 7.0f : 0.0f;
+      const uint64_t scale = pair(p.scale_log2, p.scale_log2), minus_m = pair(kLift - ms, kLift - ms);
       uint64_t sum[2] = {0, 0};
 #pragma unroll
       for (uint32_t h = 0; h < 4; ++h) {

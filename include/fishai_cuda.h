@@ -368,8 +368,9 @@ int fa_rope_append(const fa_rope *r, const fa_pages *pages, uint32_t layer, int3
  * own chunk, which are written all the same, and no others.
  * Scores, maxima, sums of weights and outputs are f32.  Over f16 and bf16 pages
  * of head size 64 and 128 the weights are rounded to the pages' type for the
- * product with V (relative 2^-11 or 2^-8 each; their sum is taken before), with
- * other sizes and types they are not.  Scaled scores have to stay below 2^127.
+ * product with V (relative 2^-11 or 2^-8 each, f16 ones below 2^-21 of a row's
+ * largest within 2^-32 of it; their sum is taken before), with other sizes and
+ * types they are not.  Scaled scores have to stay below 2^127.
  * max_q and the table's width (max_pages) choose the kernels: the tighter they
  * are, the faster a short call.
  * ws: at least fa_attn_chunks_ws(...) bytes of device memory, 16-byte aligned,

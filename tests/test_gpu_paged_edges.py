@@ -82,6 +82,30 @@ def test_attention_of_more_work_than_the_split_counts_is_refused(t, heads, hd, c
     assert int(err) == paged.FLAG_RANGE and bool((out == 7.0).all())
 
 
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,kvh,hd", [(4, 1, 64), (4, 2, 128)])
+@pytest.mark.parametrize("n,kv,wide", [(1, 6000, 0), (1, 30000, 0), (3, 6000, 40000), (12, 1500, 0), (30, 5000, 0), (100, 9000, 0)])
+@pytest.mark.parametrize("nats", [12.0, 17.5, 20.0])
+def test_attention_weights_far_below_the_largest_count(t, heads, kvh, hd, n, kv, wide, nats):
+    """one position far above thousands of equal ones, whose weights together are what the output is made of.  A weight of
+    f16 has a relative half step of 2^-11 down to 2^-29 of the largest (2^-21 where items go to tcgen05) and is within
+    2^-40 (2^-32) of it below that"""
+    dtype = R.TYPES[t]
+    per = max(kv, wide) // 16 + 1
+    pages = torch.zeros(1, per, 2, kvh, 16, hd, dtype=dtype, device="cuda")
+    table = torch.arange(per, dtype=torch.int32, device="cuda")[None].contiguous()
+    pages[0, :, 1] = 1.0
+    pages[0, 0, 0, :, 0, 0] = nats * hd ** 0.5 / 4
+    pages[0, 0, 1, :, 0] = 0.0
+    q = torch.zeros(n, heads * hd, dtype=dtype, device="cuda")
+    q[:, ::hd] = 4.0
+    out = attn(pages, table, q, [0, n], [kv], heads)
+    want, tol = R.attention(pages, table, 0, q, i32([0, n]), i32([kv]), None, heads, 0.0, 0)
+    if t == "f16":
+        tol = tol + kv * (2.0 ** -40 if n * heads // kvh <= 16 else 2.0 ** -32)
+    assert bool(((out.double().view_as(want) - want).abs() <= tol).all())
+
+
 # ------------------------------------------------------------------ buffers
 @pytest.mark.parametrize("n", [1, 3, 40, 150])
 @pytest.mark.parametrize("order", ["q first", "out first"])
