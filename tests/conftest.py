@@ -19,3 +19,16 @@ def oracle():
     import oracle as o
     o.lib()
     return o
+
+
+@pytest.fixture(autouse=True)
+def kept_pages(monkeypatch):
+    """Some tests pass C.addressof of an fa_pages that nothing holds any more: each lives as long as its test."""
+    from fishai_engine import _lib as L
+    made, real = [], L.fa_pages
+
+    def keep(*args, **kw):
+        made.append(real(*args, **kw))
+        return made[-1]
+
+    monkeypatch.setattr(L, "fa_pages", keep)
