@@ -2,6 +2,7 @@
 // checks, the device a call runs on, parameters.
 #include <algorithm>
 #include <cmath>
+#include <initializer_list>
 #include <mutex>
 #include <new>
 #include <string>
@@ -78,6 +79,12 @@ int launched(const char *who, int rc) {
   return fail(FA_ERR_CUDA, std::string(who) + ": launch failed" +
                                (e != cudaSuccess ? std::string(": ") + cudaGetErrorString(e) : std::string()));
 }
+// arrays of 32-bit words (null: not given); a load from an odd address would fault
+int words(const char *who, std::initializer_list<const void *> arrays) {
+  for (const void *p : arrays)
+    if (reinterpret_cast<uintptr_t>(p) % 4) return invalid(who, "an array of 32-bit words is not 4-byte aligned");
+  return FA_OK;
+}
 bool known(int dtype) { return dtype == FA_KV_F32 || dtype == FA_KV_F16 || dtype == FA_KV_BF16; }
 
 // pages as every operator needs them; the table is not looked at where only
@@ -92,6 +99,7 @@ int check_pages(const char *who, const fa_pages *p, bool table) {
   if (p->n_kv_heads > 32767 || p->n_layers > 65535) return invalid(who, "more than 32767 kv heads or 65535 layers");
   if (table && (!p->n_seq || !p->max_pages)) return invalid(who, "empty page table");
   if (table && p->max_pages > (1u << 21)) return invalid(who, "more than 2^21 pages a sequence");
+  if (table && reinterpret_cast<uintptr_t>(p->page_table) % 4) return invalid(who, "pages.page_table is not 4-byte aligned");
   if (reinterpret_cast<uintptr_t>(p->base) % 16) return invalid(who, "pages.base is not 16-byte aligned");
   if (p->layer_stride % 8) return invalid(who, "pages.layer_stride is not a multiple of 8 elements");
   const uint64_t layer = (uint64_t)p->n_pages * 2 * p->n_kv_heads * kPageLen * p->head_dim;
@@ -232,6 +240,7 @@ int fa_rope_append(const fa_rope *r, const fa_pages *pages, uint32_t layer, int3
   const bool in_place = q == out && in_dtype == pages->dtype && (q_stride == out_stride || n_tokens == 1);
   if (!in_place && overlap(n_tokens, rows_of(q, q_stride, qw, ei), rows_of(out, out_stride, qw, eo)))
     return invalid(who, "out overlaps q without being q");
+  TRY(words(who, {pos, seq, slot, err}));
   OnDevice dev(who);
   TRY(dev.add("pages.base", pages->base));
   TRY(dev.add("pages.page_table", pages->page_table));
@@ -289,6 +298,7 @@ int fa_attn_chunks(const fa_pages *pages, uint32_t layer, const void *q, uint64_
     return invalid(who, "q or out is not aligned to its element type");
   if (overlap(n_tokens, rows_of(q, q_stride, qw, es), rows_of(out, out_stride, qw, es)))
     return invalid(who, "out overlaps q");
+  TRY(words(who, {q_start, kv_len, seq, err}));
   OnDevice dev(who);
   TRY(dev.add("pages.base", pages->base));
   TRY(dev.add("pages.page_table", pages->page_table));
@@ -331,6 +341,7 @@ int fa_pages_copy(const fa_pages *pages, const uint32_t *src, const uint32_t *ds
   if (n > 0x7FFFFFFFu) return invalid(who, "too many pages");
   if (!n) return FA_OK;
   if (!src || !dst) return invalid(who, "null argument");
+  TRY(words(who, {src, dst, slots, err}));
   OnDevice dev(who);
   TRY(dev.add("pages.base", pages->base));
   TRY(dev.add("src", src));
@@ -353,6 +364,7 @@ int fa_pages_compact(const fa_pages *pages, const uint32_t *seq, const uint32_t 
   if (n_keep > 0x7FFFFFFFu || n > 0x7FFFFFFFu) return invalid(who, "too many kept positions or sequences");
   if (!n || !n_keep) return FA_OK;
   if (!seq || !keep || !keep_start) return invalid(who, "null argument");
+  TRY(words(who, {seq, keep, keep_start, err}));
   OnDevice dev(who);
   TRY(dev.add("pages.base", pages->base));
   TRY(dev.add("pages.page_table", pages->page_table));
@@ -397,6 +409,7 @@ int fa_beam_select(const void *logits, int32_t dtype, uint64_t ld, uint32_t n_ba
   if (ws_bytes < need) return invalid(who, "workspace of " + std::to_string(ws_bytes) + " bytes, " + std::to_string(need) + " needed");
   if (reinterpret_cast<uintptr_t>(ws) % 16) return invalid(who, "the workspace is not 16-byte aligned");
   if (reinterpret_cast<uintptr_t>(logits) % elem_size(dtype)) return invalid(who, "logits are not aligned to their element type");
+  TRY(words(who, {scores, done, out_scores, out_parents, out_tokens, out_done}));
   OnDevice dev(who);
   TRY(dev.add("logits", logits));
   TRY(dev.add("scores", scores));

@@ -1,5 +1,7 @@
 """Calls at the edges of what the paged operators and the beam selection allow,
 as the host takes them: no GPU needed, no pointer is read."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
@@ -7,7 +9,7 @@ from fishai_engine import _lib as L
 from fishai_engine import beam, paged
 from fishai_engine.kv_cache import KVCache
 from fishai_engine.model import ModelWeights
-from test_cpu_paged import P, call_attn, call_rope, pages
+from test_cpu_paged import P, call_attn, call_beam, call_rope, pages
 
 
 @pytest.mark.parametrize("chunks", [1 << 31, (1 << 32) - 128, (1 << 32) - 1])
@@ -95,3 +97,35 @@ def test_generate_beams_refuses_numbers_beyond_32_bits(bad):
             pass
     with pytest.raises(ValueError):
         Model().generate_beams(**{**dict(prompt_tokens=[5], n_beams=2, max_new=2), **bad})
+
+
+ODD = P * 8 + 2
+
+
+def rope_with_err(err):
+    r, pg = paged.Rope(64), pages()
+    return L.lib().fa_rope_append(r._h, C.addressof(pg), 0, L.KV_F16, P, 512, P * 2, 256, P * 3, 256, 3, 8, P, P, None, P * 4, 512, err, None)
+
+
+PG = pages()
+
+
+@pytest.mark.parametrize("call", [lambda: call_rope(pos=ODD), lambda: call_rope(seq=ODD), lambda: call_rope(slot=ODD), lambda: call_rope(pages(page_table=ODD)),
+                                  lambda: call_attn(starts=ODD), lambda: call_attn(kv=ODD), lambda: call_attn(seq=ODD), lambda: call_attn(pages(page_table=ODD)),
+                                  lambda: call_beam(scores=ODD), lambda: call_beam(done=ODD), lambda: call_beam(os=ODD), lambda: call_beam(op=ODD),
+                                  lambda: call_beam(ot=ODD), lambda: call_beam(od=ODD),
+                                  lambda: rope_with_err(ODD),
+                                  lambda: L.lib().fa_attn_chunks(C.addressof(PG), 0, P, 512, 8, 2, P, P, None, 3, 3, 0.0, 0, P * 4, 512, P * 16,
+                                                                 L.lib().fa_attn_chunks_ws(64), ODD, None),
+                                  lambda: L.lib().fa_pages_copy(C.addressof(PG), ODD, P, None, 1, None, None),
+                                  lambda: L.lib().fa_pages_copy(C.addressof(PG), P, ODD, None, 1, None, None),
+                                  lambda: L.lib().fa_pages_copy(C.addressof(PG), P, P, ODD, 1, None, None),
+                                  lambda: L.lib().fa_pages_copy(C.addressof(PG), P, P, None, 1, ODD, None),
+                                  lambda: L.lib().fa_pages_compact(C.addressof(PG), ODD, P, P, 1, 4, None, None),
+                                  lambda: L.lib().fa_pages_compact(C.addressof(PG), P, ODD, P, 1, 4, None, None),
+                                  lambda: L.lib().fa_pages_compact(C.addressof(PG), P, P, ODD, 1, 4, None, None),
+                                  lambda: L.lib().fa_pages_compact(C.addressof(PG), P, P, P, 1, 4, ODD, None)])
+def test_arrays_of_words_at_odd_addresses_are_refused(call):
+    """a kernel's load of four bytes there would fault"""
+    assert call() == L.ERR_INVALID
+    assert "4-byte aligned" in L.last_error()
