@@ -15,6 +15,7 @@
 #include "fa_kernels.hpp"
 #include "gguf.hpp"
 #include "model.hpp"
+#include "paged_ops.hpp"
 #include "sdpa.hpp"
 #include "tp.hpp"
 
@@ -580,6 +581,10 @@ int fa_model_set_tc_prefill(fa_model *m, int32_t on) {
   return FA_OK;
 }
 int fa_debug_set(fa_model *fm, int32_t key, uint64_t value) {
+  if (key == FA_DEBUG_WITHHOLD_KV) {  // of the operators on pages, which have no model
+    attn_withhold((uint32_t)std::min<uint64_t>(value, 0xFFFFFFFFu));
+    return FA_OK;
+  }
   API_NULL(fm);
   Model &m = fm->m;
   if (key == FA_DEBUG_WAIT_LIMIT_NS) m.dbg_wait_ns = value;

@@ -5,6 +5,7 @@
 
 #include <cudaTypedefs.h>
 
+#include <atomic>
 #include <mutex>
 
 #include "paged_tma.cuh"
@@ -219,6 +220,9 @@ bool page_map(const AttnChunksParams &p, uint32_t rows, CUtensorMap *map) {
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+static std::atomic<uint32_t> g_withhold{0};
+void attn_withhold(uint32_t copy) { g_withhold.store(copy, std::memory_order_relaxed); }
+
 // slots of the launch for few rows, of the one for many, descriptors
 size_t attn_chunks_ws(uint32_t head_dim) {
   return (kSmallSlots + kTcSlots) * (head_dim + 2) * 4 + (kAttnMaxCtas + 2 * kTcMaxCtas) * sizeof(uint4);
@@ -226,6 +230,7 @@ size_t attn_chunks_ws(uint32_t head_dim) {
 
 int launch_attn_chunks(const AttnChunksParams &p, void *ws, uint32_t n_sm, cudaStream_t st) {
   AttnChunksParams a = p, b = p;
+  b.withhold = g_withhold.load(std::memory_order_relaxed);
   a.part = static_cast<float *>(ws);
   b.part = a.part + kSmallSlots * (p.pg.head_dim + 2);
   a.desc = reinterpret_cast<uint4 *>(b.part + kTcSlots * (p.pg.head_dim + 2));

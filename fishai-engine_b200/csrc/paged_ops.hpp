@@ -55,7 +55,11 @@ struct AttnChunksParams {
   float *part;                       // split items: two slots a CTA
   uint4 *desc;                       // per CTA: the item it starts and later CTAs continue (w = CTAs, 0: none)
   uint32_t *err;
+  uint32_t withhold;                 // k_attn_tc: a CTA leaves out its copy of this number (from 1; 0: none), so that
+                                     // the waits for it run out
 };
+// the `withhold` of the calls from now on (fa_debug_set)
+void attn_withhold(uint32_t copy);
 size_t attn_chunks_ws(uint32_t head_dim);
 // ws: attn_chunks_ws(head_dim) bytes; p.part and p.desc are set from it
 int launch_attn_chunks(const AttnChunksParams &p, void *ws, uint32_t n_sm, cudaStream_t st);

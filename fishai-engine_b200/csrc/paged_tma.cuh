@@ -16,11 +16,13 @@ __device__ __forceinline__ void tma_2d(uint32_t dst, const void *map, int32_t x,
 // Bounded wait of a whole warp; false, for all its lanes (they take the same
 // way through later barriers and votes): it ran out here or elsewhere in the CTA
 // (`abort`, in shared memory, is set).  The phase cannot pass while the warp
-// waits: what completes the next one waits for the warp.
+// waits: what completes the next one waits for the warp.  A try suspends the warp
+// for 4 us at most, so 2^19 of them are two seconds (measured: 2.0).
+constexpr uint32_t kWarpWaitTries = 1u << 19;
 __device__ __forceinline__ bool wait_bar(uint32_t *abort, uint64_t *bar, uint32_t parity) {
   const uint32_t addr = smem_u32(bar);
   uint32_t ok = 0;
-  for (uint32_t i = 0; i < kMaxWaitTries && !ok; ++i) {
+  for (uint32_t i = 0; i < kWarpWaitTries && !ok; ++i) {
     asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
                  : "=r"(ok)
                  : "r"(addr), "r"(parity)

@@ -20,7 +20,7 @@ FLAG_PAGE, FLAG_RANGE, FLAG_TIMEOUT = 16, 32, 64
 ROPE_INTERLEAVED, ROPE_HALF = 0, 1
 ROPE_PLAIN, ROPE_LINEAR, ROPE_NTK, ROPE_LLAMA3, ROPE_YARN = 0, 1, 2, 3, 4
 NO_TOKEN = 4294967295
-DEBUG_WAIT_LIMIT_NS, DEBUG_WITHHOLD_WEIGHTS, DEBUG_FIXED_ORDER_SUMS = 1, 2, 3
+DEBUG_WAIT_LIMIT_NS, DEBUG_WITHHOLD_WEIGHTS, DEBUG_FIXED_ORDER_SUMS, DEBUG_WITHHOLD_KV = 1, 2, 3, 4
 
 
 class FishaiError(RuntimeError):

@@ -179,6 +179,12 @@ int fa_model_step_launches(const fa_model *m, uint32_t *n);
  * a vector red.add, which removes a reduction pass per launch but leaves the
  * order of the f32 additions to the hardware. */
 #define FA_DEBUG_FIXED_ORDER_SUMS 3
+/* FA_DEBUG_WITHHOLD_KV: value n > 0 makes each CTA of fa_attn_chunks on tcgen05
+ * leave out its n-th copy of a K or V tile, so that the waits for it run out
+ * after two seconds and the call sets FA_FLAG_TIMEOUT; 0 restores normal
+ * operation.  For the whole process (m is not looked at and may be NULL), not for
+ * graphs captured before. */
+#define FA_DEBUG_WITHHOLD_KV 4
 int fa_debug_set(fa_model *m, int32_t key, uint64_t value);
 
 /* ------------------------------------------------------------- KV cache */
