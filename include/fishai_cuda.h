@@ -376,7 +376,8 @@ int fa_rope_append(const fa_rope *r, const fa_pages *pages, uint32_t layer, int3
  * of head size 64 and 128 the weights are rounded to the pages' type for the
  * product with V (relative 2^-11 or 2^-8 each, f16 ones below 2^-21 of a row's
  * largest within 2^-32 of it; their sum is taken before), with other sizes and
- * types they are not.  Scaled scores have to stay below 2^127.
+ * types they are not.  Scaled scores have to stay below 2^127, and a column's sum
+ * of |v| over what a token sees below 2^119.
  * max_q and the table's width (max_pages) choose the kernels: the tighter they
  * are, the faster a short call.
  * ws: at least fa_attn_chunks_ws(...) bytes of device memory, 16-byte aligned,

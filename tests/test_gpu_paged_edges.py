@@ -142,3 +142,54 @@ def test_compact_flags_a_position_that_does_not_ascend_where_it_would_stay(keep,
     paged.compact(paged.PagedKV(pages, table), i32([0]), i32(keep), i32([0, len(keep)]), err=err)
     assert int(err) == paged.FLAG_RANGE
     assert same_bits(pages, want)
+
+
+# ------------------------------------------------------------------ rotary append
+@pytest.mark.parametrize("tokens", [601, 1199, 1203, 1601, 2050])
+@pytest.mark.parametrize("tin,tout,kw", [("f16", "f16", {}), ("bf16", "bf16", dict(layout="half")), ("f32", "f32", {}), ("f32", "f16", dict(rot_dim=24))])
+def test_rope_append_of_several_tokens_a_cta(tokens, tin, tout, kw):
+    """two and four tokens a CTA, the last one with fewer, a row left out inside a group"""
+    c = rope_case(tokens, 6, 2, 64, R.TYPES[tin], R.TYPES[tout], seed=tokens, spare_row=True, **kw)
+    paged.rope_append(paged.PagedKV(c["pages"], c["table"]), 1, c["r"], c["q"], c["k"], c["v"], i32(c["pos"]), i32(c["seqs"]), c["out"],
+                      slots=i32(c["slots"]))
+    rope_check(c, 6, 2, 64, kw.get("layout", "interleaved"))
+
+
+# ------------------------------------------------------------------ more than a grid's 65535
+def test_copy_pages_of_more_pairs_than_a_grid_holds():
+    n = 65535 + 200
+    pages = randn(1, 2, 2 * n, 2, 1, 16, 8, dtype=torch.float16)
+    src = torch.randperm(2 * n, generator=torch.Generator().manual_seed(1)).to(torch.int32).cuda()
+    src, dst = src[:n].contiguous(), src[n:].contiguous()
+    slots = (torch.arange(n, device="cuda") % 17).int()
+    want = pages.clone()
+    copied = (torch.arange(16, device="cuda") < slots[:, None])[None, :, None, None, :, None]
+    want[:, dst.long()] = torch.where(copied, pages[:, src.long()], pages[:, dst.long()])
+    paged.copy_pages(paged.PagedKV(pages, i32([[0]])), src, dst, slots=slots)
+    assert same_bits(pages, want)
+
+
+@pytest.mark.parametrize("layers,n", [(1, 65535 + 70), (3, 21845 * 2 + 5)])
+def test_compact_of_more_sequences_than_a_grid_holds(layers, n):
+    """one page a sequence: positions 3, 5, 11 stay"""
+    pages = randn(2, layers, n, 2, 1, 16, 8, dtype=torch.float16)
+    table = torch.randperm(n, generator=torch.Generator().manual_seed(2)).to(torch.int32).cuda()[:, None].contiguous()
+    want = pages.clone()
+    want[:, :, :, :, :3] = pages[:, :, :, :, [3, 5, 11]]
+    paged.compact(paged.PagedKV(pages, table), torch.arange(n, dtype=torch.int32, device="cuda"), i32([3, 5, 11] * n),
+                  (3 * torch.arange(n + 1, device="cuda")).int())
+    assert same_bits(pages, want)
+
+
+def test_beam_select_of_more_rows_than_a_grid_holds():
+    """1100 x 64 beams: the same as in parts of 100 requests"""
+    nb, beams, vocab, k = 1100, 64, 40, 5
+    x = randn(4, nb * beams, vocab)
+    scores = -torch.rand(nb, beams, device="cuda", generator=torch.Generator("cuda").manual_seed(5))
+    done = (torch.rand(nb, beams, device="cuda", generator=torch.Generator("cuda").manual_seed(6)) < 0.2).int()
+    got = beam_run(x, scores, done, k)
+    for a in range(0, nb, 100):
+        part = beam_run(x[a * beams: (a + 100) * beams], scores[a: a + 100], done[a: a + 100], k)
+        assert all(torch.equal(g[a: a + 100], p) for g, p in zip(got, part))
+    for a in (0, 1023, 1024, 1099):  # row 65535 is a beam of request 1023
+        beam_check(x[a * beams: (a + 1) * beams], scores[a: a + 1], done[a: a + 1], k)
