@@ -54,7 +54,7 @@ template <typename F>
 int guarded(F f) {
   try {
     return f();
-  } catch (const std::bad_alloc &) {
+  } catch (const std::exception &) {  // bad_alloc, and length_error of sizes beyond any memory
     return fail(FA_ERR_OOM, "out of host memory");
   }
 }
@@ -156,6 +156,7 @@ int create_kv(Model &m, uint32_t n_seq, uint32_t max_ctx, int dtype, KvCache *kv
   API_CUDA(cudaMemcpy(kv->page_table, pt.data(), pages * 4, cudaMemcpyHostToDevice));
   kv->table = std::move(pt);
   kv->refs.assign(pages, 1);
+  kv->free_pages.reserve(pages);  // one that becomes free has a place
   return m.ensure_rope(max_ctx + 1);
 }
 
@@ -607,7 +608,7 @@ int fa_kv_create(fa_model *m, uint32_t n_seq, uint32_t max_ctx, int32_t dtype, f
   API_NULL(out);
   fa_kv *kv = new (std::nothrow) fa_kv();
   if (!kv) return fail(FA_ERR_OOM, "out of memory");
-  int rc = create_kv(m->m, n_seq, max_ctx, dtype, &kv->kv);
+  const int rc = guarded([&] { return create_kv(m->m, n_seq, max_ctx, dtype, &kv->kv); });
   if (rc) {
     std::string e = last_error();
     delete kv;

@@ -1,7 +1,10 @@
 // Pages of a model's K/V cache shared between its sequences: fork, reorder
 // (beam search), truncation and compaction.  The tables are kept on the host
-// and uploaded where they change; only partly filled pages are copied.  (The
-// reference clones whole caches: src/kv_cache.rs:13 derives Clone.)
+// and uploaded where they change; only partly filled pages are copied.  What a
+// call needs of memory is there before it changes the tables (ready, and the free
+// list has room for every page from the beginning), so that one that fails leaves
+// them as they were.  (The reference clones whole caches: src/kv_cache.rs:13
+// derives Clone.)
 #include <algorithm>
 
 #include "model.hpp"
@@ -63,7 +66,11 @@ int KvCache::upload(uint32_t seq) {
   return FA_OK;
 }
 
-int KvCache::ensure_scratch() {
+int KvCache::ready() {
+  const size_t most = std::max(n_seq, max_pages);  // at most a move a sequence, or one an entry of a row
+  moves.clear();
+  moves.reserve(most);
+  list.reserve(3 * most);
   if (scratch) return FA_OK;
   const size_t words = 3 * (size_t)std::max(n_seq, max_pages) + (size_t)max_pages * 16 + 8;
   if (cudaMalloc(&scratch, words * 4) != cudaSuccess) {
@@ -74,11 +81,10 @@ int KvCache::ensure_scratch() {
   return FA_OK;
 }
 
-int KvCache::copy(const std::vector<Move> &moves) {
+int KvCache::copy() {
   if (moves.empty()) return FA_OK;
-  TRY(ensure_scratch());
-  const uint32_t n = (uint32_t)moves.size();  // at most one a sequence, or one an entry of a row
-  std::vector<uint32_t> list(3 * (size_t)n);
+  const uint32_t n = (uint32_t)moves.size();
+  list.resize(3 * (size_t)n);
   for (uint32_t i = 0; i < n; ++i) {
     list[i] = moves[i].src;
     list[n + i] = moves[i].dst;
@@ -113,7 +119,7 @@ int KvCache::fork(uint32_t src, uint32_t dst) {
   if (!m) return fail(FA_ERR_INVALID, "the cache's model was freed");
   if (src == dst) return FA_OK;
   CUDA_TRY(cudaSetDevice(m->device));
-  TRY(ensure_scratch());  // nothing may fail between the table's change and its upload
+  TRY(ready());
   TRY(settle());
   const uint32_t full = len[src] / 16, rest = len[src] % 16;
   uint32_t *s = row(src), *d = row(dst);
@@ -130,7 +136,8 @@ int KvCache::fork(uint32_t src, uint32_t dst) {
     }
   len[dst] = len[src];
   TRY(upload(dst));
-  if (rest) TRY(copy({{s[full], d[full], rest}}));
+  if (rest) moves.push_back({s[full], d[full], rest});
+  TRY(copy());
   return m->sync();
 }
 
@@ -140,7 +147,7 @@ int KvCache::reorder(const uint32_t *parents, uint32_t n) {
   for (uint32_t i = 0; i < n; ++i) same = same && parents[i] == i;
   if (same) return FA_OK;
   CUDA_TRY(cudaSetDevice(m->device));
-  TRY(ensure_scratch());
+  TRY(ready());
   TRY(settle());
   const std::vector<uint32_t> old(table.begin(), table.begin() + (size_t)n * max_pages), was(len.begin(), len.begin() + n);
   // one child of each parent takes over the parent's own pages: itself, else
@@ -162,7 +169,6 @@ int KvCache::reorder(const uint32_t *parents, uint32_t n) {
   free_pages.clear();
   for (uint32_t p = (uint32_t)refs.size(); p-- > 0;)
     if (!refs[p]) free_pages.push_back(p);
-  std::vector<Move> moves;
   for (uint32_t i = 0; i < n; ++i) {
     const uint32_t p = parents[i], full = was[p] / 16;
     if (heir[p] == i) continue;
@@ -171,14 +177,13 @@ int KvCache::reorder(const uint32_t *parents, uint32_t n) {
   }
   for (uint32_t i = 0; i < n; ++i)
     if (parents[i] != i) TRY(upload(i));
-  TRY(copy(moves));
+  TRY(copy());
   return m->sync();
 }
 
 int KvCache::truncate(uint32_t seq, uint32_t n) {
   const uint32_t full = n / 16, rest = n % 16;
   uint32_t *r = row(seq);
-  std::vector<Move> moves;
   bool changed = false;
   for (uint32_t i = full; i < max_pages; ++i) changed = changed || refs[r[i]] > 1;
   if (!changed) {
@@ -187,7 +192,7 @@ int KvCache::truncate(uint32_t seq, uint32_t n) {
   }
   if (!m) return fail(FA_ERR_INVALID, "the cache's model was freed");
   CUDA_TRY(cudaSetDevice(m->device));
-  TRY(ensure_scratch());
+  TRY(ready());
   TRY(settle());
   for (uint32_t i = full; i < max_pages; ++i)
     if (refs[r[i]] > 1) {
@@ -198,7 +203,7 @@ int KvCache::truncate(uint32_t seq, uint32_t n) {
     }
   len[seq] = n;
   TRY(upload(seq));
-  TRY(copy(moves));
+  TRY(copy());
   return m->sync();
 }
 
@@ -208,11 +213,10 @@ int KvCache::compact(uint32_t seq, const uint32_t *keep, uint32_t n) {
   if (j0 == n) return truncate(seq, n);
   if (!m) return fail(FA_ERR_INVALID, "the cache's model was freed");
   CUDA_TRY(cudaSetDevice(m->device));
-  TRY(ensure_scratch());
+  TRY(ready());
   TRY(settle());
   // pages that are written become the sequence's own, with their contents
   uint32_t *r = row(seq);
-  std::vector<Move> moves;
   for (uint32_t i = j0 / 16; i <= (n - 1) / 16; ++i)
     if (refs[r[i]] > 1) {
       const uint32_t page = r[i];
@@ -221,7 +225,7 @@ int KvCache::compact(uint32_t seq, const uint32_t *keep, uint32_t n) {
       moves.push_back({page, r[i], 16});
     }
   if (!moves.empty()) TRY(upload(seq));
-  TRY(copy(moves));
+  TRY(copy());
   const uint32_t head[3] = {seq, 0, n};
   uint32_t *at = scratch + 3 * (size_t)std::max(n_seq, max_pages);
   CUDA_TRY(cudaMemcpyAsync(at, head, sizeof head, cudaMemcpyHostToDevice, m->stream));

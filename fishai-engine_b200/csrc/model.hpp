@@ -245,9 +245,11 @@ struct KvCache {
   uint32_t *row(uint32_t seq) { return table.data() + (size_t)seq * max_pages; }
   uint32_t take();
   void drop(uint32_t page);
-  int upload(uint32_t seq);                          // a sequence's table row to the device
-  int copy(const std::vector<Move> &moves);          // pages, in every layer
-  int ensure_scratch();
+  std::vector<Move> moves;          // of the call at hand
+  std::vector<uint32_t> list;       // `moves` as the kernel takes them
+  int upload(uint32_t seq);         // a sequence's table row to the device
+  int copy();                       // `moves`, in every layer
+  int ready();                      // memory for a call's moves; no moves yet
 };
 
 int config_from_gguf(const Gguf &g, fa_config *cfg);
