@@ -51,7 +51,7 @@ __global__ void __launch_bounds__(kCopyThreads) k_page_copy(const PageCopyParams
 // at or below its own sources and below every later tile's.  So a tile may be
 // written as soon as it and all before it are read: the next tile is read
 // ahead, a barrier, this one written.  Four sequences of 2048 positions thinned
-// to half, 8 heads x 128 f16, 32 layers: 111 us, 6.0 TB/s (without reading
+// to half, 8 heads x 128 f16, 32 layers: 111 us, 5.2 TB/s (without reading
 // ahead 139).
 constexpr uint32_t kCompactThreads = 256, kCompactUnroll = 4;
 __global__ void __launch_bounds__(kCompactThreads) k_page_compact(const PageCompactParams p, uint32_t row16) {

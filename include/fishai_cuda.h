@@ -313,7 +313,7 @@ int fa_kv_wait(fa_kv *kv, void *stream);
  *          between them blended evenly over i, and the result times
  *          attn_factor (0: 0.1 ln(factor) + 1).
  * The other elements of a head are copied.  Angles are reduced in 64 bits, so
- * positions of any size keep their exactness. */
+ * positions of any size keep their exactness (2^-51 of the angle, then f32). */
 #define FA_ROPE_INTERLEAVED 0
 #define FA_ROPE_HALF 1
 #define FA_ROPE_PLAIN 0
