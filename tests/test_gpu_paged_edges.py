@@ -193,3 +193,52 @@ def test_beam_select_of_more_rows_than_a_grid_holds():
         assert all(torch.equal(g[a: a + 100], p) for g, p in zip(got, part))
     for a in (0, 1023, 1024, 1099):  # row 65535 is a beam of request 1023
         beam_check(x[a * beams: (a + 1) * beams], scores[a: a + 1], done[a: a + 1], k)
+
+
+# ------------------------------------------------------------------ graphs
+@pytest.mark.parametrize("t", ["f16", "f32"])
+def test_append_copies_and_compaction_captured_and_replayed(t):
+    """one graph of a step's rope_append, a fork's copies, a compaction and the attention over it; the lists in its
+    buffers change between replays"""
+    kvh, hd, heads = 2, 64, 8
+    pages, table = R.make_cache([200, 90, 40], 2, kvh, hd, R.TYPES[t], 60, spare=6)
+    at = int(pages.shape[1])
+    was = pages.clone()
+    used = {int(x) for s, n in enumerate((200, 90, 40)) for x in table[s, : -(-n // 16)]}
+    free = [p for p in range(at) if p not in used]
+    rope, kv = paged.Rope(hd), paged.PagedKV(pages, table)
+    rows = randn(7, 3, (heads + 2 * kvh) * hd, dtype=R.TYPES[t])
+    q, k, v = rows[:, : heads * hd], rows[:, heads * hd: (heads + kvh) * hd], rows[:, (heads + kvh) * hd:]
+    ws = torch.empty(paged.workspace_bytes(hd), dtype=torch.uint8, device="cuda")
+    lists = [dict(pos=[199, 89, 39], src=[int(table[0, 3]), int(table[1, 0])], dst=free[:2], slots=[16, 5], keep=[0, 3, 50, 51, 120], ks=[0, 5],
+                  lens=[5, 90, 40]),
+             dict(pos=[10, 20, 30], src=[int(table[2, 1]), int(table[0, 7])], dst=free[2:4], slots=[8, 16], keep=[1, 2, 4, 100, 199], ks=[0, 4],
+                  lens=[4, 60, 31])]
+    b = {n: i32(x) for n, x in lists[0].items()}
+    seqs, one, start = i32([0, 1, 2]), i32([0]), i32([0, 1, 2, 3])
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    turned, out = torch.empty_like(rows[:, : heads * hd]), torch.empty_like(rows[:, : heads * hd])
+
+    def step(stream):
+        paged.rope_append(kv, 1, rope, q, k, v, b["pos"], seqs, turned, err=err, stream=stream)
+        paged.copy_pages(kv, b["src"], b["dst"], slots=b["slots"], err=err, stream=stream)
+        paged.compact(kv, one, b["keep"], b["ks"], err=err, stream=stream)
+        paged.attention(kv, 1, turned, start, b["lens"], out, 1, ws, err=err, stream=stream)
+
+    g = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g):
+        step(torch.cuda.current_stream().cuda_stream)
+    for values in lists + lists[:1]:
+        for n, x in values.items():
+            b[n].copy_(i32(x))
+        results = []
+        for run in (lambda: step(0), g.replay):
+            pages.copy_(was)
+            turned.fill_(9.0), out.fill_(9.0)
+            torch.cuda.synchronize()
+            run()
+            torch.cuda.synchronize()
+            results.append((pages.clone(), turned.clone(), out.clone()))
+        assert int(err) == 0 and all(same_bits(x, y) for x, y in zip(*results))
+        assert not same_bits(results[0][0], was) and not bool(results[0][2].isnan().any())
