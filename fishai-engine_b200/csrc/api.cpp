@@ -638,6 +638,7 @@ int fa_kv_get(const fa_kv *kv, uint32_t seq, uint32_t layer, float *k_host, floa
   API_NULL(kv);
   const KvCache &c = kv->kv;
   if (seq >= c.n_seq) return fail(FA_ERR_INVALID, "sequence index out of range");
+  if (!c.m) return fail(FA_ERR_INVALID, "fa_kv_get: the cache's model was freed");
   if (layer >= c.m->cfg.n_layers)
     return fail(FA_ERR_INVALID, "KV cache layer index out of range: " + std::to_string(layer));
   const uint32_t KVH = c.m->cfg.n_kv_heads, hd = c.m->cfg.head_dim, len = c.len[seq];

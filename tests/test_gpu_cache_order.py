@@ -5,6 +5,7 @@ import pytest
 
 from fishai_engine import _lib as L
 from fishai_engine import paged
+from fishai_engine.model import ModelWeights
 from fishai_engine.sampling import Sampler, SamplerConfig
 from test_gpu_beam import dev, fill, path  # noqa: F401
 
@@ -103,3 +104,18 @@ def test_wait_refuses_a_stream_that_is_captured(dev):  # noqa: F811
     fill(dev, kv, [20])  # and the model's stream is not part of it
     kv.fork(0, 1)
     assert L.lib().fa_kv_wait(None, None) == L.ERR_INVALID
+
+
+def test_calls_on_a_cache_whose_model_is_freed_are_refused(path):  # noqa: F811
+    model = ModelWeights.load_from_gguf(path)
+    kv = model.new_kv_cache(64, dtype=L.KV_F16, n_seq=3)
+    fill(model, kv, [37, 20])
+    kv.fork(0, 2)
+    model.close()
+    for call in (lambda: kv.get(0, 0), lambda: kv.fork(0, 1), lambda: kv.reorder([1, 0]), lambda: kv.truncate(2, 18), lambda: kv.compact(0, [1, 5]),
+                 lambda: kv.wait(), lambda: paged.PagedKV.of(kv)):
+        with pytest.raises(L.FishaiError) as e:
+            call()
+        assert e.value.code == L.ERR_INVALID
+    kv.truncate(1, 3)  # nothing shared: no work on the GPU
+    assert kv.seq_len_with_dim(0, kv.kv_dim, 1) == 3
