@@ -17,8 +17,10 @@ __device__ __forceinline__ void tma_2d(uint32_t dst, const void *map, int32_t x,
 // way through later barriers and votes): it ran out here or elsewhere in the CTA
 // (`abort`, in shared memory, is set).  The phase cannot pass while the warp
 // waits: what completes the next one waits for the warp.  A try suspends the warp
-// for 4 us at most, so 2^19 of them are two seconds (measured: 2.0).
-constexpr uint32_t kWarpWaitTries = 1u << 19;
+// for 4 us at most, so 2^20 of them are four seconds (measured: 4.1).  The longest
+// wait of a call that works is that of the warps that hold the next item's Q rows
+// ready, for an item of 2^25 positions: 2^18 tiles of up to 4 us, a second.
+constexpr uint32_t kWarpWaitTries = 1u << 20;
 __device__ __forceinline__ bool wait_bar(uint32_t *abort, uint64_t *bar, uint32_t parity) {
   const uint32_t addr = smem_u32(bar);
   uint32_t ok = 0;

@@ -181,7 +181,7 @@ int fa_model_step_launches(const fa_model *m, uint32_t *n);
 #define FA_DEBUG_FIXED_ORDER_SUMS 3
 /* FA_DEBUG_WITHHOLD_KV: value n > 0 makes each CTA of fa_attn_chunks on tcgen05
  * leave out its n-th copy of a K or V tile, so that the waits for it run out
- * after two seconds and the call sets FA_FLAG_TIMEOUT; 0 restores normal
+ * after four seconds and the call sets FA_FLAG_TIMEOUT; 0 restores normal
  * operation.  For the whole process (m is not looked at and may be NULL), not for
  * graphs captured before. */
 #define FA_DEBUG_WITHHOLD_KV 4

@@ -1,6 +1,6 @@
 """A bounded wait of the attention on tcgen05 that runs out: each CTA is told to
 leave out one of its copies (fa_debug_set), so that what waits for it gives up
-after two seconds, all roles leave, the copies in flight land and the call
+after four seconds, all roles leave, the copies in flight land and the call
 sets FLAG_TIMEOUT.  Nothing faults or hangs; the next call is right again."""
 import pytest
 
