@@ -19,7 +19,7 @@ def test_beam_select_zeros_of_both_signs_are_equal(t, vocab, k):
     """ties go to the lowest token whatever the zeros' signs, and no candidate is lost to them"""
     v = torch.arange(vocab, device="cuda")
     zero = torch.zeros(vocab, device="cuda")
-    last = v % 4096 >= min(3072, vocab // 2)
+    last = v % 4096 >= min(4096 - 1024, vocab // 2)
     low = -1.0 - v / vocab
     x = torch.stack([torch.where(last & (v % 4 == 3), zero, -zero),    # a thread's largest is +0.0, its first equal -0.0
                      torch.where(last, zero, -zero),
