@@ -14,6 +14,7 @@ using namespace fa;
 
 struct fa_rope {
   fa_rope_config cfg;
+  uint32_t n_axes;
   RopeTable tab;
   double freqs[kMaxHeadDim / 2];
   double scale;
@@ -153,8 +154,7 @@ void fa_rope_config_default(fa_rope_config *c, uint32_t head_dim, double base) {
   c->attn_factor = 0.0;
 }
 
-int fa_rope_create(const fa_rope_config *c, fa_rope **out) {
-  const char *who = "fa_rope_create";
+static int rope_create(const char *who, const fa_rope_config *c, const fa_rope_axes *ax, fa_rope **out) {
   if (!c) return invalid(who, "null argument cfg");
   if (!out) return invalid(who, "null argument out");
   *out = nullptr;
@@ -169,6 +169,21 @@ int fa_rope_create(const fa_rope_config *c, fa_rope **out) {
   const bool blend = c->scaling == FA_ROPE_LLAMA3 || c->scaling == FA_ROPE_YARN;
   if (blend && !c->context) return invalid(who, "context is zero");
   if (c->scaling == FA_ROPE_NTK && c->rot_dim < 4) return invalid(who, "NTK scaling needs rot_dim of at least 4");
+  const uint32_t half = c->rot_dim / 2, n_axes = ax ? ax->n_axes : 1;
+  if (ax) {
+    if (!n_axes || n_axes > FA_ROPE_MAX_AXES) return invalid(who, "1 to 4 axes");
+    if (ax->order != FA_AXES_BLOCKS && ax->order != FA_AXES_TURNS) return invalid(who, "unknown order of the axes");
+    if (ax->freqs != FA_AXES_SHARED && ax->freqs != FA_AXES_OWN) return invalid(who, "unknown frequencies of the axes");
+    uint64_t sum = 0;
+    for (uint32_t a = 0; a < n_axes; ++a) {
+      const uint32_t n = ax->pairs[a];
+      if (!n) return invalid(who, "an axis without pairs");
+      if (ax->order == FA_AXES_TURNS && a && a + (uint64_t)n_axes * (n - 1) >= half) return invalid(who, "an axis has more pairs than turns");
+      if (ax->freqs == FA_AXES_OWN && c->scaling == FA_ROPE_NTK && n < 2) return invalid(who, "NTK scaling needs two pairs of each axis");
+      sum += n;
+    }
+    if (sum != half) return invalid(who, "the axes' pairs do not add up to rot_dim / 2");
+  }
   if (c->scaling == FA_ROPE_LLAMA3 && (!(c->low_turns > 0) || !(c->high_turns > c->low_turns) || !std::isfinite(c->high_turns)))
     return invalid(who, "0 < low_turns < high_turns");
   if (c->scaling == FA_ROPE_YARN && (!(c->beta_slow > 0) || !(c->beta_fast > c->beta_slow) || !std::isfinite(c->beta_fast) ||
@@ -176,20 +191,29 @@ int fa_rope_create(const fa_rope_config *c, fa_rope **out) {
     return invalid(who, "0 < beta_slow < beta_fast and attn_factor >= 0");
   fa_rope *r = new (std::nothrow) fa_rope();
   if (!r) return fail(FA_ERR_OOM, std::string(who) + ": out of memory");
-  const double two_pi = 6.283185307179586476925286766559;
-  const double rot = c->rot_dim, ctx = c->context;
-  double base = c->base;
-  if (c->scaling == FA_ROPE_NTK) base *= std::pow(c->factor, rot / (rot - 2.0));
-  double lo = 0.0, hi = 0.0;
-  if (c->scaling == FA_ROPE_YARN) {  // the pair that turns `beta` times in the context
-    auto pair = [&](double beta) { return rot * std::log(ctx / (beta * two_pi)) / (2.0 * std::log(base)); };
-    lo = std::max(std::floor(pair(c->beta_fast)), 0.0);
-    hi = std::min(std::ceil(pair(c->beta_slow)), rot - 1.0);
-  }
   r->cfg = *c;
+  r->n_axes = n_axes;
+  if (ax) {
+    uint32_t a = 0, begun = 0;
+    for (uint32_t i = 0; i < half; ++i) {
+      if (ax->order == FA_AXES_BLOCKS) {
+        if (i - begun == ax->pairs[a]) begun = i, ++a;
+      } else {
+        a = i % n_axes;
+        if (i / n_axes >= ax->pairs[a]) a = 0;  // the axis has had its turns
+      }
+      r->tab.axis[i] = (uint8_t)a;
+    }
+  }
+  const double two_pi = 6.283185307179586476925286766559, ctx = c->context;
   r->scale = 1.0;
   if (c->scaling == FA_ROPE_YARN) r->scale = c->attn_factor > 0 ? c->attn_factor : 0.1 * std::log(c->factor) + 1.0;
-  for (uint32_t i = 0; i < c->rot_dim / 2; ++i) {
+  uint32_t seen[FA_ROPE_MAX_AXES] = {};
+  for (uint32_t j = 0; j < half; ++j) {
+    // pair i of a series over `rot` elements: the head's, or the axis's own
+    const uint32_t a = r->tab.axis[j], i = ax && ax->freqs == FA_AXES_OWN ? seen[a]++ : j;
+    const double rot = ax && ax->freqs == FA_AXES_OWN ? 2.0 * ax->pairs[a] : (double)c->rot_dim;
+    const double base = c->scaling == FA_ROPE_NTK ? c->base * std::pow(c->factor, rot / (rot - 2.0)) : c->base;
     double f = std::pow(base, -2.0 * i / rot);
     if (c->scaling == FA_ROPE_LINEAR) {
       f /= c->factor;
@@ -197,14 +221,26 @@ int fa_rope_create(const fa_rope_config *c, fa_rope **out) {
       const double t = std::min(1.0, std::max(0.0, (ctx * f / two_pi - c->low_turns) / (c->high_turns - c->low_turns)));
       f = f * t + f / c->factor * (1.0 - t);
     } else if (c->scaling == FA_ROPE_YARN) {
+      auto pair = [&](double beta) { return rot * std::log(ctx / (beta * two_pi)) / (2.0 * std::log(base)); };  // turns `beta` times in the context
+      const double lo = std::max(std::floor(pair(c->beta_fast)), 0.0), hi = std::min(std::ceil(pair(c->beta_slow)), rot - 1.0);
       const double t = std::min(1.0, std::max(0.0, (i - lo) / std::max(hi - lo, 0.001)));
       f = f / c->factor * t + f * (1.0 - t);
     }
-    r->freqs[i] = f;
-    r->tab.turns[i] = f / two_pi;
+    r->freqs[j] = f;
+    r->tab.turns[j] = f / two_pi;
   }
   r->tab.scale = (float)r->scale;
   *out = r;
+  return FA_OK;
+}
+int fa_rope_create(const fa_rope_config *c, fa_rope **out) { return rope_create("fa_rope_create", c, nullptr, out); }
+int fa_rope_create_axes(const fa_rope_config *c, const fa_rope_axes *ax, fa_rope **out) {
+  if (!ax) return invalid("fa_rope_create_axes", "null argument axes");
+  return rope_create("fa_rope_create_axes", c, ax, out);
+}
+int fa_rope_axis_of(const fa_rope *r, uint32_t *axis) {
+  if (!r || !axis) return invalid("fa_rope_axis_of", "null argument");
+  for (uint32_t i = 0; i < r->cfg.rot_dim / 2; ++i) axis[i] = r->tab.axis[i];
   return FA_OK;
 }
 void fa_rope_free(fa_rope *r) { delete r; }
@@ -216,12 +252,13 @@ int fa_rope_freqs(const fa_rope *r, double *freqs, double *scale) {
   return FA_OK;
 }
 
-int fa_rope_append(const fa_rope *r, const fa_pages *pages, uint32_t layer, int32_t in_dtype, const void *q,
-                   uint64_t q_stride, const void *k, uint64_t k_stride, const void *v, uint64_t v_stride,
-                   uint32_t n_tokens, uint32_t n_heads, const uint32_t *pos, const uint32_t *seq, const uint32_t *slot,
-                   void *out, uint64_t out_stride, uint32_t *err, void *stream) {
-  const char *who = "fa_rope_append";
+// axes: pos has a row for each axis, pos_stride apart
+static int rope_append(const char *who, bool axes, const fa_rope *r, const fa_pages *pages, uint32_t layer, int32_t in_dtype, const void *q,
+                       uint64_t q_stride, const void *k, uint64_t k_stride, const void *v, uint64_t v_stride, uint32_t n_tokens,
+                       uint32_t n_heads, const uint32_t *pos, uint64_t pos_stride, const uint32_t *seq, const uint32_t *slot, void *out,
+                       uint64_t out_stride, uint32_t *err, void *stream) {
   if (!r) return invalid(who, "null argument rope");
+  if (!axes && r->n_axes > 1) return invalid(who, "a rope of several axes: fa_rope_append_axes");
   TRY(check_pages(who, pages, true));
   if (layer >= pages->n_layers) return invalid(who, "layer out of range");
   if (r->cfg.head_dim != pages->head_dim) return invalid(who, "the rope's head_dim is not the pages'");
@@ -232,7 +269,8 @@ int fa_rope_append(const fa_rope *r, const fa_pages *pages, uint32_t layer, int3
   if (n_tokens > 1 && (q_stride < qw || out_stride < qw || k_stride < kw || v_stride < kw))
     return invalid(who, "a row stride is smaller than the row");
   if (!n_tokens) return FA_OK;
-  if (!q || !k || !v || !pos || !seq || !out) return invalid(who, "null argument");
+  if (!q || !k || !v || !pos || !seq || !out || (axes && !slot)) return invalid(who, "null argument");
+  if (r->n_axes > 1 && pos_stride && pos_stride < n_tokens) return invalid(who, "an axis's positions overlap the next one's");
   const uint32_t ei = elem_size(in_dtype), eo = elem_size(pages->dtype);
   for (const void *b : {q, k, v})
     if (reinterpret_cast<uintptr_t>(b) % ei) return invalid(who, "q, k or v is not aligned to its element type");
@@ -264,19 +302,33 @@ int fa_rope_append(const fa_rope *r, const fa_pages *pages, uint32_t layer, int3
   p.rot = r->cfg.rot_dim;
   p.half_layout = r->cfg.layout == FA_ROPE_HALF;
   p.pos = pos, p.seq = seq, p.slot = slot;
+  p.pos_stride = r->n_axes > 1 ? pos_stride : 0;
   p.out = out;
   p.err = err;
   return launched(who, launch_rope_append(p, r->tab, (cudaStream_t)stream));
+}
+int fa_rope_append(const fa_rope *r, const fa_pages *pages, uint32_t layer, int32_t in_dtype, const void *q,
+                   uint64_t q_stride, const void *k, uint64_t k_stride, const void *v, uint64_t v_stride,
+                   uint32_t n_tokens, uint32_t n_heads, const uint32_t *pos, const uint32_t *seq, const uint32_t *slot,
+                   void *out, uint64_t out_stride, uint32_t *err, void *stream) {
+  return rope_append("fa_rope_append", false, r, pages, layer, in_dtype, q, q_stride, k, k_stride, v, v_stride, n_tokens, n_heads, pos, 0, seq,
+                     slot, out, out_stride, err, stream);
+}
+int fa_rope_append_axes(const fa_rope *r, const fa_pages *pages, uint32_t layer, int32_t in_dtype, const void *q,
+                        uint64_t q_stride, const void *k, uint64_t k_stride, const void *v, uint64_t v_stride,
+                        uint32_t n_tokens, uint32_t n_heads, const uint32_t *pos, uint64_t pos_stride, const uint32_t *seq,
+                        const uint32_t *slot, void *out, uint64_t out_stride, uint32_t *err, void *stream) {
+  return rope_append("fa_rope_append_axes", true, r, pages, layer, in_dtype, q, q_stride, k, k_stride, v, v_stride, n_tokens, n_heads, pos,
+                     pos_stride, seq, slot, out, out_stride, err, stream);
 }
 
 // ------------------------------------------------------------ attention
 size_t fa_attn_chunks_ws(uint32_t head_dim) { return head_dim && head_dim <= kMaxHeadDim ? attn_chunks_ws(head_dim) : 0; }
 
-int fa_attn_chunks(const fa_pages *pages, uint32_t layer, const void *q, uint64_t q_stride, uint32_t n_heads,
-                   uint32_t n_chunks, const uint32_t *q_start, const uint32_t *kv_len, const uint32_t *seq,
-                   uint32_t n_tokens, uint32_t max_q, float scale, uint32_t window, void *out, uint64_t out_stride,
-                   void *ws, size_t ws_bytes, uint32_t *err, void *stream) {
-  const char *who = "fa_attn_chunks";
+static int attn_chunks(const char *who, const fa_pages *pages, uint32_t layer, const void *q, uint64_t q_stride, uint32_t n_heads,
+                       uint32_t n_chunks, const uint32_t *q_start, const uint32_t *kv_len, const uint32_t *seq, uint32_t n_tokens,
+                       uint32_t max_q, float scale, uint32_t window, uint32_t sinks, void *out, uint64_t out_stride, void *ws,
+                       size_t ws_bytes, uint32_t *err, void *stream) {
   TRY(check_pages(who, pages, true));
   if (layer >= pages->n_layers) return invalid(who, "layer out of range");
   if (!n_heads || n_heads > 32767 || n_heads % pages->n_kv_heads)
@@ -284,7 +336,9 @@ int fa_attn_chunks(const fa_pages *pages, uint32_t layer, const void *q, uint64_
   if (!std::isfinite(scale) || scale < 0 || scale > 1e30f) return invalid(who, "scale is a number from 0 to 1e30");
   if ((uint64_t)n_tokens * n_heads > 0x7FFFFFFFu) return invalid(who, "2^31 or more query rows");
   if (n_chunks > 0x7FFFFFFFu) return invalid(who, "2^31 or more chunks");
-  if (window > 0x7FFFFFFFu) window = 0;  // wider than any cache: none
+  // wider than any cache: none; the same where the first positions are all there can be
+  if (window > 0x7FFFFFFFu || sinks >= pages->max_pages * kPageLen) window = 0;
+  if (!window) sinks = 0;
   const uint64_t hd = pages->head_dim, qw = n_heads * hd;
   if (n_tokens > 1 && (q_stride < qw || out_stride < qw)) return invalid(who, "a row stride is smaller than the row");
   if (!n_tokens || !n_chunks || !max_q) return FA_OK;
@@ -327,10 +381,25 @@ int fa_attn_chunks(const fa_pages *pages, uint32_t layer, const void *q, uint64_
   p.seq = seq;
   p.scale_log2 = (float)((scale > 0 ? (double)scale : 1.0 / std::sqrt((double)hd)) * 1.4426950408889634);
   p.window = window;
+  p.sinks = sinks;
   p.aligned = reinterpret_cast<uintptr_t>(q) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0 &&
               q_stride * es % 16 == 0 && out_stride * es % 16 == 0;
   p.err = err;
   return launched(who, launch_attn_chunks(p, ws, (uint32_t)dev.sms(), (cudaStream_t)stream));
+}
+int fa_attn_chunks(const fa_pages *pages, uint32_t layer, const void *q, uint64_t q_stride, uint32_t n_heads,
+                   uint32_t n_chunks, const uint32_t *q_start, const uint32_t *kv_len, const uint32_t *seq,
+                   uint32_t n_tokens, uint32_t max_q, float scale, uint32_t window, void *out, uint64_t out_stride,
+                   void *ws, size_t ws_bytes, uint32_t *err, void *stream) {
+  return attn_chunks("fa_attn_chunks", pages, layer, q, q_stride, n_heads, n_chunks, q_start, kv_len, seq, n_tokens, max_q, scale, window, 0,
+                     out, out_stride, ws, ws_bytes, err, stream);
+}
+int fa_attn_chunks_sinks(const fa_pages *pages, uint32_t layer, const void *q, uint64_t q_stride, uint32_t n_heads,
+                         uint32_t n_chunks, const uint32_t *q_start, const uint32_t *kv_len, const uint32_t *seq,
+                         uint32_t n_tokens, uint32_t max_q, float scale, uint32_t window, uint32_t sinks, void *out,
+                         uint64_t out_stride, void *ws, size_t ws_bytes, uint32_t *err, void *stream) {
+  return attn_chunks("fa_attn_chunks_sinks", pages, layer, q, q_stride, n_heads, n_chunks, q_start, kv_len, seq, n_tokens, max_q, scale,
+                     window, sinks, out, out_stride, ws, ws_bytes, err, stream);
 }
 
 // ------------------------------------------------------------ pages

@@ -18,6 +18,19 @@
 
 namespace fa {
 
+// A call's parameters as the kernels take them, which are compiled twice: where
+// there are no first positions beside the window (most calls), `sinks` is a constant
+// and its arithmetic goes (kept at run time it cost those calls 2%).
+struct PlainParams : AttnChunksParams {
+  static constexpr uint32_t sinks = 0;
+};
+struct SinkParams : AttnChunksParams {};
+template <typename F>
+auto with_sinks(const AttnChunksParams &p, F f) {
+  if (p.sinks) return f(SinkParams{p});
+  return f(PlainParams{p});
+}
+
 struct Chunk {
   uint32_t q0, q_len, seq;
   int32_t first;  // position of its first token (kv_len - q_len; negative: tokens before the cache's start)
@@ -42,31 +55,65 @@ __device__ __forceinline__ Chunk load_chunk(const AttnChunksParams &p, uint32_t 
   return k;
 }
 
-// Positions [lo, hi) that the rows [r0, r1) of a chunk see (hi <= lo: none)
-__device__ __forceinline__ void tile_range(const AttnChunksParams &p, const Chunk &k, uint32_t r0, uint32_t r1, uint32_t &lo,
+// Positions [lo, hi) that the rows [r0, r1) of a chunk see (hi <= lo: none), and
+// where 0 < lo, also those below p.sinks < lo, with a gap between the two that
+// nobody sees
+template <typename PR>
+__device__ __forceinline__ void tile_range(const PR &p, const Chunk &k, uint32_t r0, uint32_t r1, uint32_t &lo,
                                            uint32_t &hi) {
   const int32_t last = k.first + (int32_t)((r1 - 1) / p.rep), first = k.first + (int32_t)(r0 / p.rep);
   hi = last < 0 ? 0u : (uint32_t)last + 1;
   lo = p.window && first >= (int32_t)p.window ? (uint32_t)first - p.window + 1 : 0u;
+  if (lo <= p.sinks) lo = 0;
+}
+// whether some row of the item [lo, hi) sees position t, or one of the page at t
+template <typename PR>
+__device__ __forceinline__ bool item_sees(const PR &p, uint32_t lo, uint32_t hi, uint32_t t) {
+  return t < hi && (t >= lo || t < p.sinks);
+}
+template <typename PR>
+__device__ __forceinline__ bool item_reads(const PR &p, uint32_t lo, uint32_t hi, uint32_t page_at) {
+  return page_at < hi && (page_at + kPageLen > lo || page_at < p.sinks);
+}
+// whether the token at pos sees position t
+template <typename PR>
+__device__ __forceinline__ bool token_sees(const PR &p, int32_t pos, int32_t t) {
+  return t <= pos && (!p.window || (uint32_t)(pos - t) < p.window || (uint32_t)t < p.sinks);
 }
 
-template <uint32_t U>
-__device__ __forceinline__ uint32_t range_units(uint32_t lo, uint32_t hi) {
-  return hi > lo ? (hi - 1) / U - lo / U + 1 : 1;  // at least one: somebody writes the zeros
+// Units before the gap: those of the first positions that [lo, hi) does not begin in
+template <uint32_t U, typename PR>
+__device__ __forceinline__ uint32_t sink_units(const PR &p, uint32_t lo) {
+  return p.sinks ? min((p.sinks + U - 1) / U, lo / U) : 0;
+}
+template <uint32_t U, typename PR>
+__device__ __forceinline__ uint32_t range_units(const PR &p, uint32_t lo, uint32_t hi) {
+  return hi > lo ? sink_units<U>(p, lo) + (hi - 1) / U - lo / U + 1 : 1;  // at least one: somebody writes the zeros
+}
+// first position of unit u of an item
+template <uint32_t U, typename PR>
+__device__ __forceinline__ uint32_t unit_at(const PR &p, uint32_t lo, uint32_t u) {
+  const uint32_t n = sink_units<U>(p, lo);
+  return (u < n ? u : u - n + lo / U) * U;
+}
+// that of unit u + step, where unit u is at t
+template <uint32_t U, typename PR>
+__device__ __forceinline__ uint32_t unit_after(const PR &p, uint32_t lo, uint32_t u, uint32_t t, uint32_t step) {
+  return p.sinks ? unit_at<U>(p, lo, u + step) : t + step * U;
 }
 // Cost of a row tile on the line: its units, and OVER for what an item costs
 // apart from them (Q, filling the pipeline, the output), so that many short
 // items do not make a CTA late.
-template <uint32_t R, uint32_t U, uint32_t OVER>
-__device__ __forceinline__ uint32_t tile_cost(const AttnChunksParams &p, const Chunk &k, uint32_t tile) {
+template <uint32_t R, uint32_t U, uint32_t OVER, typename PR>
+__device__ __forceinline__ uint32_t tile_cost(const PR &p, const Chunk &k, uint32_t tile) {
   uint32_t lo, hi;
   tile_range(p, k, tile * R, min(k.rows, tile * R + R), lo, hi);
-  return range_units<U>(lo, hi) + OVER;
+  return range_units<U>(p, lo, hi) + OVER;
 }
 // Cost of the lane's chunk, its row tiles times the heads; long chunks by the
 // whole warp (a thread to itself took 6 us for the 16 tiles of 1024 tokens)
-template <uint32_t R, uint32_t U, uint32_t OVER>
-__device__ __forceinline__ uint64_t chunk_cost(const AttnChunksParams &p, const Chunk &k) {
+template <uint32_t R, uint32_t U, uint32_t OVER, typename PR>
+__device__ __forceinline__ uint64_t chunk_cost(const PR &p, const Chunk &k) {
   const uint32_t lane = threadIdx.x & 31;
   uint64_t mine = 0;
   const bool small = k.rows <= 2 * R;
@@ -90,7 +137,7 @@ struct Segment {  // a piece of an item
   Chunk chunk;
   uint32_t tile, head;
   uint32_t r0, r1;       // rows of the item
-  uint32_t lo, hi;       // positions the item sees
+  uint32_t lo, hi;       // positions the item sees (tile_range)
   uint32_t u0, u1, n;    // units [u0, u1) of the item's n
 };
 
@@ -104,7 +151,8 @@ struct Walk {
   Chunk chunk;
 
   // All threads of the CTA; `red` is scratch of THREADS / 32 + 2 words.
-  __device__ void start(const AttnChunksParams &p, uint32_t min_cost, uint64_t *red) {
+  template <typename PR>
+  __device__ void start(const PR &p, uint32_t min_cost, uint64_t *red) {
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     auto cost = [&](uint32_t i) -> uint64_t {  // of chunk i, whole warps
       Chunk k;
@@ -191,7 +239,8 @@ struct Walk {
   }
   __device__ bool done() const { return left == 0; }
   // the next piece with work in it; false: there is none left
-  __device__ bool next(const AttnChunksParams &p, Segment &s) {
+  template <typename PR>
+  __device__ bool next(const PR &p, Segment &s) {
     while (left) {
       s.chunk = chunk;
       s.tile = tile;
@@ -199,7 +248,7 @@ struct Walk {
       s.r0 = tile * R;
       s.r1 = min(chunk.rows, s.r0 + R);
       tile_range(p, chunk, s.r0, s.r1, s.lo, s.hi);
-      s.n = range_units<U>(s.lo, s.hi);
+      s.n = range_units<U>(p, s.lo, s.hi);
       const uint32_t take = min(s.n + OVER - rem, left), end = rem + take;
       s.u0 = rem > OVER ? rem - OVER : 0;
       s.u1 = end > OVER ? end - OVER : 0;
@@ -238,13 +287,14 @@ constexpr uint32_t kOneCtas = 8;  // of a cluster (the portable most; of 16, the
 
 // Most positions that a token of the call can see, as far as the host knows.
 inline uint64_t one_span(const AttnChunksParams &p) {
-  const uint64_t cap = (uint64_t)p.pg.max_pages * kPageLen, seen = (uint64_t)p.window + p.max_q;
+  const uint64_t cap = (uint64_t)p.pg.max_pages * kPageLen, seen = (uint64_t)p.window + p.max_q + p.sinks;
   return p.window && seen < cap ? seen : cap;
 }
 inline uint64_t one_items(const AttnChunksParams &p) { return (uint64_t)p.n_chunks * p.pg.n_kv_heads; }
 // Cluster blockIdx.x / kOneCtas takes (chunk, head); false: the chunk has no
 // rows (the same for the whole cluster).
-__device__ __forceinline__ bool one_item(const AttnChunksParams &p, Segment &s) {
+template <typename PR>
+__device__ __forceinline__ bool one_item(const PR &p, Segment &s) {
   const uint32_t item = blockIdx.x / kOneCtas;
   s.chunk = load_chunk(p, item / p.pg.n_kv_heads);
   if (!s.chunk.rows) return false;
@@ -295,8 +345,8 @@ __device__ __forceinline__ void one_join(const Segment &s, uint32_t hd, const fl
   cluster_sync();  // the pieces have been read
 }
 // Launches a cluster for each of `items`, where the GPU holds that many at once; 1: it does not, -1: an error.
-template <auto kern, uint32_t C = kOneCtas>
-int launch_one(const AttnChunksParams &p, uint64_t items, uint32_t threads, uint32_t smem, cudaStream_t st) {
+template <auto kern, uint32_t C = kOneCtas, typename PR>
+int launch_one(const PR &p, uint64_t items, uint32_t threads, uint32_t smem, cudaStream_t st) {
   static std::atomic<int> known[64];  // clusters at once, by device (0: not asked yet)
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(C);

@@ -49,14 +49,15 @@ struct Copier {
     r0 = threadIdx.x / per_row, c0 = threadIdx.x - r0 * per_row;
     dr = kAnyThreads / per_row, dc = kAnyThreads - dr * per_row;
   }
-  // src: rows of a page from at[page of the tile] on; positions outside
-  // [lo, hi) and bad pages (~0) become zeros
-  template <typename T>
-  __device__ void copy(const T *src, const uint64_t *at, uint32_t t0, uint32_t lo, uint32_t hi, uint32_t hd, T *dst, uint32_t ld) const {
+  // src: rows of a page from at[page of the tile] on; positions that the item
+  // does not see and bad pages (~0) become zeros
+  template <typename T, typename PR>
+  __device__ void copy(const PR &p, const T *src, const uint64_t *at, uint32_t t0, uint32_t lo, uint32_t hi, T *dst, uint32_t ld) const {
     constexpr uint32_t kV = 16 / sizeof(T);
+    const uint32_t hd = p.pg.head_dim;
     for (uint32_t r = r0, c = c0; r < kAnyPos;) {
       const uint64_t row0 = at[r / kPageLen];
-      const bool ok = t0 + r >= lo && t0 + r < hi && row0 != ~0ull;
+      const bool ok = item_sees(p, lo, hi, t0 + r) && row0 != ~0ull;
       asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst + r * ld + c * kV)),
                    "l"(ok ? src + row0 + (r % kPageLen) * hd + c * kV : src), "r"(ok ? 16u : 0u)
                    : "memory");
@@ -87,7 +88,8 @@ struct AnyRows {
 
   // units u, u + step, .. < n of an item; the tile behind the one worked on is on
   // its way: its K once the scores are formed, its V once that product is done
-  __device__ void run(const AttnChunksParams &p, const Segment &s, uint32_t u, uint32_t n, uint32_t step, float *sm) {
+  template <typename PR>
+  __device__ void run(const PR &p, const Segment &s, uint32_t u, uint32_t n, uint32_t step, float *sm) {
     __shared__ uint64_t at[2][kAnyPos / kPageLen];  // element offsets of the tile's pages, and of the next tile's
     const uint32_t hd = p.pg.head_dim, ld = hd + 4, lds = kAnyPos + 4, ldk = hd + 16 / sizeof(T);
     float *sq = sm, *sp = sq + R * ld;
@@ -101,7 +103,7 @@ struct AnyRows {
     // thread j < 4: page j of the tile at t0; only pages that are read are looked up
     auto look_up = [&](uint32_t t0) -> uint32_t {
       const uint32_t t = t0 + tid * kPageLen;
-      return tid < kAnyPos / kPageLen && t < s.hi && t + kPageLen > s.lo ? __ldg(pt + t / kPageLen) : 0u;
+      return tid < kAnyPos / kPageLen && item_reads(p, s.lo, s.hi, t) ? __ldg(pt + t / kPageLen) : 0u;
     };
     auto note = [&](uint32_t page, uint32_t which) {
       if (tid >= kAnyPos / kPageLen) return;
@@ -110,11 +112,11 @@ struct AnyRows {
       if (!good && p.err) atomicOr(p.err, kFlagPage);
     };
     if (u < n) {
-      const uint32_t t0 = (s.lo / kAnyPos + u) * kAnyPos;
+      const uint32_t t0 = unit_at<kAnyPos>(p, s.lo, u);
       note(look_up(t0), 0);
       __syncthreads();
-      copier.copy(base, at[0], t0, s.lo, s.hi, hd, sk, ldk);
-      copier.copy(vbase, at[0], t0, s.lo, s.hi, hd, sv, ldk);
+      copier.copy(p, base, at[0], t0, s.lo, s.hi, sk, ldk);
+      copier.copy(p, vbase, at[0], t0, s.lo, s.hi, sv, ldk);
     }
     // Q rows; past the item's: zeros
     for (uint32_t r = tid / 32; r < R; r += kAnyThreads / 32) {  // a warp a row
@@ -137,7 +139,7 @@ struct AnyRows {
       for (uint32_t j = 0; j < HJ; ++j) o[i][j][0] = o[i][j][1] = o[i][j][2] = o[i][j][3] = 0.0f;
     }
     for (uint32_t which = 0; u < n; u += step, which ^= 1) {
-      const uint32_t t0 = (s.lo / kAnyPos + u) * kAnyPos, t1 = t0 + step * kAnyPos;
+      const uint32_t t0 = unit_at<kAnyPos>(p, s.lo, u), t1 = unit_after<kAnyPos>(p, s.lo, u, t0, step);
       const bool more = u + step < n;
       const uint32_t ahead = more ? look_up(t1) : 0;
       copied_but_one();
@@ -159,7 +161,7 @@ struct AnyRows {
       }
       if (more) note(ahead, which ^ 1);
       __syncthreads();
-      if (more) copier.copy(base, at[which ^ 1], t1, s.lo, s.hi, hd, sk, ldk);
+      if (more) copier.copy(p, base, at[which ^ 1], t1, s.lo, s.hi, sk, ldk);
       else asm volatile("cp.async.commit_group;" ::: "memory");
 #pragma unroll
       for (uint32_t i = 0; i < RT; ++i) {
@@ -167,8 +169,7 @@ struct AnyRows {
 #pragma unroll
         for (uint32_t j = 0; j < 4; ++j) {
           const int32_t t = (int32_t)(t0 + tx + 16 * j);
-          const bool see = t <= pos[i] && (!p.window || (uint32_t)(pos[i] - t) < p.window);
-          a[i][j] = see ? a[i][j] * p.scale_log2 : -INFINITY;
+          a[i][j] = token_sees(p, pos[i], t) ? a[i][j] * p.scale_log2 : -INFINITY;
           mx = fmaxf(mx, a[i][j]);
         }
 #pragma unroll
@@ -214,15 +215,15 @@ struct AnyRows {
         }
       }
       __syncthreads();
-      if (more) copier.copy(vbase, at[which ^ 1], t1, s.lo, s.hi, hd, sv, ldk);
+      if (more) copier.copy(p, vbase, at[which ^ 1], t1, s.lo, s.hi, sv, ldk);
       else asm volatile("cp.async.commit_group;" ::: "memory");
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
   }
 };
 
-template <typename T, uint32_t HJ>
-__global__ void __launch_bounds__(kAnyThreads) k_attn_any(const AttnChunksParams p) {
+template <typename T, uint32_t HJ, typename PR>
+__global__ void __launch_bounds__(kAnyThreads) k_attn_any(const PR p) {
   extern __shared__ __align__(16) float sm[];
   __shared__ uint64_t red[kAnyThreads / 32 + 2];
   const uint32_t hd = p.pg.head_dim, tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
@@ -264,14 +265,14 @@ __global__ void __launch_bounds__(kAnyThreads) k_attn_any(const AttnChunksParams
 }
 
 // few items of up to 32 rows: a cluster each (paged_attn.cuh)
-template <typename T, uint32_t HJ>
-__global__ void __launch_bounds__(kAnyThreads) k_attn_any_one(const AttnChunksParams p) {
+template <typename T, uint32_t HJ, typename PR>
+__global__ void __launch_bounds__(kAnyThreads) k_attn_any_one(const PR p) {
   extern __shared__ __align__(16) float sm[];
   const uint32_t hd = p.pg.head_dim, tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
   Segment s;
   if (!one_item(p, s)) return;
   AnyRows<T, HJ> x;
-  x.run(p, s, cluster_ctarank(), range_units<kAnyPos>(s.lo, s.hi), kOneCtas, sm);
+  x.run(p, s, cluster_ctarank(), range_units<kAnyPos>(p, s.lo, s.hi), kOneCtas, sm);
   float *o = sm, *ml = o + R * hd;  // over Q and the weights, which have been read
   __syncthreads();
 #pragma unroll
@@ -296,21 +297,22 @@ __global__ void __launch_bounds__(kAnyThreads) k_attn_any_one(const AttnChunksPa
 template <typename T, uint32_t HJ>
 uint32_t launch_hj(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st, uint32_t *rows) {
   const uint32_t smem = any_smem<T>(p.pg.head_dim);
-  if (cudaFuncSetAttribute(k_attn_any<T, HJ>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)any_smem<T>(64 * HJ)) !=
-      cudaSuccess)
-    return 0;
   uint32_t per_sm = 224 * 1024 / (smem + 1024);
   per_sm = per_sm > 3 ? 3 : per_sm;
   const uint32_t grid = n_sm * per_sm < kAttnMaxCtas ? n_sm * per_sm : kAttnMaxCtas;
-  k_attn_any<T, HJ><<<grid, kAnyThreads, smem, st>>>(p);
   *rows = R;
-  return cudaGetLastError() == cudaSuccess ? grid : 0;
+  return with_sinks(p, [&](auto a) -> uint32_t {
+    using PR = decltype(a);
+    if (cudaFuncSetAttribute(k_attn_any<T, HJ, PR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)any_smem<T>(64 * HJ)) != cudaSuccess) return 0;
+    k_attn_any<T, HJ><<<grid, kAnyThreads, smem, st>>>(a);
+    return cudaGetLastError() == cudaSuccess ? grid : 0;
+  });
 }
 template <typename T, uint32_t HJ>
 struct LaunchAny {
   static uint32_t walk(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st, uint32_t *rows) { return launch_hj<T, HJ>(p, n_sm, st, rows); }
   static int one(const AttnChunksParams &p, cudaStream_t st) {
-    return launch_one<k_attn_any_one<T, HJ>>(p, one_items(p), kAnyThreads, any_smem<T>(64 * HJ), st);
+    return with_sinks(p, [&](auto a) { return launch_one<k_attn_any_one<T, HJ, decltype(a)>>(a, one_items(p), kAnyThreads, any_smem<T>(64 * HJ), st); });
   }
 };
 // f(LaunchAny of the call's type, rows and head size)

@@ -70,7 +70,8 @@ struct FewRows {
   float m[R / 8], l[R / 8], o[R][DPL];  // m, l: of rows tid / 16 + 8 k; l: the thread's part
 
   // Units u, u + step, .. < n of an item.
-  __device__ void run(const AttnChunksParams &p, const Segment &s, uint32_t u, uint32_t n, uint32_t step, uint8_t *sm) {
+  template <typename PR>
+  __device__ void run(const PR &p, const Segment &s, uint32_t u, uint32_t n, uint32_t step, uint8_t *sm) {
     __shared__ uint64_t at[2][kPos / kPageLen];  // element offsets of the tile's pages, and of the next tile's
     const uint32_t hd = p.pg.head_dim, ld = C::row(hd), ldq = hd + 4, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     T *sk = reinterpret_cast<T *>(sm), *sv = sk + kPos * ld;
@@ -85,7 +86,7 @@ struct FewRows {
     // thread j < 4: page j of the tile at t0; only pages that are read are looked up
     auto look_up = [&](uint32_t t0) -> uint32_t {
       const uint32_t t = t0 + tid * kPageLen;
-      return tid < kPos / kPageLen && t < s.hi && t + kPageLen > s.lo ? __ldg(pt + t / kPageLen) : 0u;
+      return tid < kPos / kPageLen && item_reads(p, s.lo, s.hi, t) ? __ldg(pt + t / kPageLen) : 0u;
     };
     auto note = [&](uint32_t page, uint32_t which) {
       if (tid >= kPos / kPageLen) return;
@@ -93,11 +94,11 @@ struct FewRows {
       at[which][tid] = good ? page_row(p.pg, page, 0, s.head, 0) : ~0ull;
       if (!good && p.err) atomicOr(p.err, kFlagPage);
     };
-    // positions outside [lo, hi) and of bad pages become zeros
+    // positions that the item does not see and of bad pages become zeros
     auto copy = [&](const T *src, uint32_t which, uint32_t t0, T *dst) {
       for (uint32_t r = r0, c = c0; r < kPos;) {
         const uint64_t row0 = at[which][r / kPageLen];
-        const bool ok = t0 + r >= s.lo && t0 + r < s.hi && row0 != ~0ull;
+        const bool ok = item_sees(p, s.lo, s.hi, t0 + r) && row0 != ~0ull;
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst + r * ld + c * kV)),
                      "l"(ok ? src + row0 + (r % kPageLen) * hd + c * kV : src), "r"(ok ? 16u : 0u)
                      : "memory");
@@ -110,7 +111,7 @@ struct FewRows {
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    uint32_t t0 = (s.lo / kPos + u) * kPos;
+    uint32_t t0 = unit_at<kPos>(p, s.lo, u);
     if (u < n) {
       note(look_up(t0), 0);
       __syncthreads();
@@ -138,7 +139,7 @@ struct FewRows {
       for (uint32_t e = 0; e < DPL; ++e) o[r][e] = 0.0f;
     for (uint32_t which = 0; u < n; u += step, which ^= 1) {
       const bool more = u + step < n;
-      const uint32_t t1 = t0 + step * kPos, ahead = more ? look_up(t1) : 0;
+      const uint32_t t1 = unit_after<kPos>(p, s.lo, u, t0, step), ahead = more ? look_up(t1) : 0;
       asm volatile("cp.async.wait_group 1;" ::: "memory");
       __syncthreads();
       {
@@ -174,8 +175,7 @@ struct FewRows {
 #pragma unroll
         for (uint32_t e = 0; e < 4; ++e) {
           const int32_t t = (int32_t)(t0 + c4 + e);
-          const bool see = t <= pos[k] && (!p.window || (uint32_t)(pos[k] - t) < p.window);
-          a[e] = see ? a[e] * p.scale_log2 : -INFINITY;
+          a[e] = token_sees(p, pos[k], t) ? a[e] * p.scale_log2 : -INFINITY;
           mx = fmaxf(mx, a[e]);
         }
 #pragma unroll
@@ -260,8 +260,8 @@ __device__ __forceinline__ void put_row(const AttnChunksParams &p, const Segment
   put(o + 3, x.w);
 }
 
-template <typename T, uint32_t R, uint32_t DPL>
-__global__ void __launch_bounds__(kThreads) k_attn_few(const AttnChunksParams p) {
+template <typename T, uint32_t R, uint32_t DPL, typename PR>
+__global__ void __launch_bounds__(kThreads) k_attn_few(const PR p) {
   using C = FewCfg<T, R, DPL>;
   extern __shared__ __align__(16) uint8_t few_sm[];
   __shared__ uint64_t red[kWarps + 2];
@@ -294,15 +294,15 @@ __global__ void __launch_bounds__(kThreads) k_attn_few(const AttnChunksParams p)
 }
 
 // few items: a cluster each (paged_attn.cuh)
-template <typename T, uint32_t R, uint32_t DPL>
-__global__ void __launch_bounds__(kThreads) k_attn_few_one(const AttnChunksParams p) {
+template <typename T, uint32_t R, uint32_t DPL, typename PR>
+__global__ void __launch_bounds__(kThreads) k_attn_few_one(const PR p) {
   using C = FewCfg<T, R, DPL>;
   extern __shared__ __align__(16) uint8_t few_sm[];
   const uint32_t hd = p.pg.head_dim, tid = threadIdx.x;
   Segment s;
   if (!one_item(p, s)) return;
   FewRows<T, R, DPL> x;
-  x.run(p, s, cluster_ctarank(), range_units<kPos>(s.lo, s.hi), kOneCtas, few_sm);
+  x.run(p, s, cluster_ctarank(), range_units<kPos>(p, s.lo, s.hi), kOneCtas, few_sm);
   float *o = reinterpret_cast<float *>(few_sm + C::merge(hd));
   for (uint32_t i = tid; i < s.r1 * (hd / 4); i += kThreads) {
     const uint32_t r = i / (hd / 4), d = (i - r * (hd / 4)) * 4;
@@ -316,16 +316,19 @@ struct LaunchFew {
   using C = FewCfg<T, R, DPL>;
   static uint32_t walk(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st, uint32_t *rows) {
     const uint32_t smem = C::smem(p.pg.head_dim);
-    if (cudaFuncSetAttribute(k_attn_few<T, R, DPL>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::smem(32 * DPL)) != cudaSuccess) return 0;
     uint32_t per_sm = 228 * 1024 / (smem + 1024 + 256);  // 1 KB of the system, 256 bytes beside the tiles
     per_sm = per_sm > 3 ? 3 : per_sm;
     const uint32_t grid = n_sm * per_sm < kAttnMaxCtas ? n_sm * per_sm : kAttnMaxCtas;
-    k_attn_few<T, R, DPL><<<grid, kThreads, smem, st>>>(p);
     *rows = R;
-    return cudaGetLastError() == cudaSuccess ? grid : 0;
+    return with_sinks(p, [&](auto a) -> uint32_t {
+      using PR = decltype(a);
+      if (cudaFuncSetAttribute(k_attn_few<T, R, DPL, PR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::smem(32 * DPL)) != cudaSuccess) return 0;
+      k_attn_few<T, R, DPL><<<grid, kThreads, smem, st>>>(a);
+      return cudaGetLastError() == cudaSuccess ? grid : 0;
+    });
   }
   static int one(const AttnChunksParams &p, cudaStream_t st) {
-    return launch_one<k_attn_few_one<T, R, DPL>>(p, one_items(p), kThreads, C::smem(32 * DPL), st);
+    return with_sinks(p, [&](auto a) { return launch_one<k_attn_few_one<T, R, DPL, decltype(a)>>(a, one_items(p), kThreads, C::smem(32 * DPL), st); });
   }
 };
 // f(LaunchFew of the call's type, rows and head size)

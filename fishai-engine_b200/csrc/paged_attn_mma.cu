@@ -143,19 +143,17 @@ struct Rows {
   }
 
   // s -> weights; the running maximum, sum and output follow
-  __device__ void softmax(const AttnChunksParams &p, uint32_t t0, float (&s)[kSub / 8][4]) {
+  template <typename PR>
+  __device__ void softmax(const PR &p, uint32_t t0, float (&s)[kSub / 8][4]) {
     const uint32_t c = threadIdx.x & 3;
-    const bool all = (int32_t)(t0 + kSub - 1) <= pos_min && (!p.window || pos_max - (int32_t)t0 < (int32_t)p.window);
+    const bool all = (int32_t)(t0 + kSub - 1) <= pos_min && (!p.window || pos_max - (int32_t)t0 < (int32_t)p.window || t0 + kSub <= p.sinks);
     float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
     for (uint32_t j = 0; j < kSub / 8; ++j)
 #pragma unroll
       for (uint32_t e = 0; e < 4; ++e) {
         const int32_t t = (int32_t)(t0 + 8 * j + 2 * c + (e & 1));
-        if (!all) {
-          const bool see = t <= pos[e >> 1] && (!p.window || (uint32_t)(pos[e >> 1] - t) < p.window);
-          if (!see) s[j][e] = -INFINITY;
-        }
+        if (!all && !token_sees(p, pos[e >> 1], t)) s[j][e] = -INFINITY;
         mx[e >> 1] = fmaxf(mx[e >> 1], s[j][e]);
       }
 #pragma unroll
@@ -211,19 +209,20 @@ struct Rows {
 struct PagePair {
   uint32_t page[2];
 };
-__device__ __forceinline__ PagePair look_up(const uint32_t *pt, uint32_t t0, uint32_t lo, uint32_t hi) {
+template <typename PR>
+__device__ __forceinline__ PagePair look_up(const PR &p, const uint32_t *pt, uint32_t t0, uint32_t lo, uint32_t hi) {
   PagePair r;
 #pragma unroll
   for (uint32_t i = 0; i < 2; ++i) {
     const uint32_t t = t0 + 16 * i;
-    r.page[i] = t < hi && t + 16 > lo ? __ldg(pt + t / kPageLen) : 0u;  // only pages that are read are looked up
+    r.page[i] = item_reads(p, lo, hi, t) ? __ldg(pt + t / kPageLen) : 0u;  // only pages that are read are looked up
   }
   return r;
 }
 // K (is_v 0) or V rows of positions [t0, t0 + 32) to a tile; THREADS threads,
-// thread i of them.  Positions outside [lo, hi) and bad pages become zeros.
-template <typename T, uint32_t HD>
-__device__ __forceinline__ void stage(const AttnChunksParams &p, const T *base, const PagePair &pg, uint32_t head, uint32_t is_v,
+// thread i of them.  Positions that the item does not see and bad pages become zeros.
+template <typename T, uint32_t HD, typename PR>
+__device__ __forceinline__ void stage(const PR &p, const T *base, const PagePair &pg, uint32_t head, uint32_t is_v,
                                       uint32_t t0, uint32_t lo, uint32_t hi, uint32_t tile, uint32_t i, uint32_t threads) {
   constexpr uint32_t CH = HD / 8;  // pieces of a row
   const uint32_t c = i % CH, r0 = i / CH, step = threads / CH;
@@ -234,7 +233,7 @@ __device__ __forceinline__ void stage(const AttnChunksParams &p, const T *base, 
 #pragma unroll
     for (uint32_t r = 0; r < 16; r += step) {
       const uint32_t row = r + r0, t = t0 + 16 * half + row;
-      cp16(tile + sw<HD>(16 * half + row, c), src + row * HD, good && t >= lo && t < hi);
+      cp16(tile + sw<HD>(16 * half + row, c), src + row * HD, good && item_sees(p, lo, hi, t));
     }
   }
 }
@@ -308,13 +307,13 @@ __device__ __forceinline__ void put4(const AttnChunksParams &p, T *o, float4 x) 
 // A warp's sub-tiles u, u + step, .. < n of an item (from its first one on), its
 // K and V tiles the only ones it uses.  q: called once the first copies are on
 // their way.
-template <typename T, uint32_t HD, typename Q>
-__device__ __forceinline__ void walk_tiles(const AttnChunksParams &p, const T *base, const Segment &s, uint32_t u, uint32_t n, uint32_t step,
+template <typename T, uint32_t HD, typename Q, typename PR>
+__device__ __forceinline__ void walk_tiles(const PR &p, const T *base, const Segment &s, uint32_t u, uint32_t n, uint32_t step,
                                            uint32_t ktile, uint32_t vtile, Rows<T, HD> &rows, Q q) {
   const uint32_t *pt = p.pg.page_table + (uint64_t)s.chunk.seq * p.pg.max_pages;
   const uint32_t lane = threadIdx.x & 31;
-  uint32_t t0 = (s.lo / kSub + u) * kSub;
-  PagePair pg = look_up(pt, t0, s.lo, s.hi);
+  uint32_t t0 = unit_at<kSub>(p, s.lo, u);
+  PagePair pg = look_up(p, pt, t0, s.lo, s.hi);
   if (u < n) {
     flag_bad_pages(p, pg);
     stage<T, HD>(p, base, pg, s.head, 0, t0, s.lo, s.hi, ktile, lane, 32);
@@ -322,11 +321,11 @@ __device__ __forceinline__ void walk_tiles(const AttnChunksParams &p, const T *b
     stage<T, HD>(p, base, pg, s.head, 1, t0, s.lo, s.hi, vtile, lane, 32);
     cp_commit();
   }
-  PagePair ahead = look_up(pt, t0 + step * kSub, s.lo, s.hi);
+  PagePair ahead = look_up(p, pt, unit_after<kSub>(p, s.lo, u, t0, step), s.lo, s.hi);
   q();
   for (; u < n; u += step) {
     const bool more = u + step < n;
-    const uint32_t t1 = t0 + step * kSub;
+    const uint32_t t1 = unit_after<kSub>(p, s.lo, u, t0, step);
     float sc[kSub / 8][4];
     cp_wait<1>();
     __syncwarp();
@@ -338,7 +337,7 @@ __device__ __forceinline__ void walk_tiles(const AttnChunksParams &p, const T *b
       stage<T, HD>(p, base, pg, s.head, 0, t1, s.lo, s.hi, ktile, lane, 32);
     }
     cp_commit();
-    ahead = look_up(pt, t1 + step * kSub, s.lo, s.hi);
+    ahead = look_up(p, pt, unit_after<kSub>(p, s.lo, u + step, t1, step), s.lo, s.hi);
     rows.softmax(p, t0, sc);
     cp_wait<1>();
     __syncwarp();
@@ -353,8 +352,8 @@ __device__ __forceinline__ void walk_tiles(const AttnChunksParams &p, const T *b
 }
 
 // ------------------------------------------------------------ up to 16 rows
-template <typename T, uint32_t HD>
-__global__ void __launch_bounds__(kThreads, 3) k_attn_rows16(const AttnChunksParams p) {
+template <typename T, uint32_t HD, typename PR>
+__global__ void __launch_bounds__(kThreads, 3) k_attn_rows16(const PR p) {
   extern __shared__ __align__(128) uint8_t dsm[];
   __shared__ uint64_t red[kThreads / 32 + 2];
   constexpr uint32_t kTileBytes = kSub * HD * 2;
@@ -396,9 +395,12 @@ uint32_t launch_hd(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st) {
   // two tiles of 32 positions a warp, or the merge's 4 x 16 rows
   constexpr uint32_t kTiles = 4 * 2 * kSub * HD * 2, kMerge = Merge<HD, 4>::kBytes, kBytes = kTiles > kMerge ? kTiles : kMerge;
   const uint32_t grid = 3 * n_sm < kAttnMaxCtas ? 3 * n_sm : kAttnMaxCtas;
-  if (cudaFuncSetAttribute(k_attn_rows16<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kBytes) != cudaSuccess) return 0;
-  k_attn_rows16<T, HD><<<grid, kThreads, kBytes, st>>>(p);
-  return cudaGetLastError() == cudaSuccess ? grid : 0;
+  return with_sinks(p, [&](auto a) -> uint32_t {
+    using PR = decltype(a);
+    if (cudaFuncSetAttribute(k_attn_rows16<T, HD, PR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kBytes) != cudaSuccess) return 0;
+    k_attn_rows16<T, HD><<<grid, kThreads, kBytes, st>>>(a);
+    return cudaGetLastError() == cudaSuccess ? grid : 0;
+  });
 }
 
 // ------------------------------------- few items of up to 16 rows: a cluster each
@@ -408,8 +410,8 @@ struct OneCfg {
   static constexpr uint32_t kPiece = Merge<HD, WARPS>::kBytes;   // over them the warps' pieces, behind those the CTA's
   static constexpr uint32_t kEnd = kPiece + 16 * HD * 4 + 16 * 8, kBytes = kTiles > kEnd ? kTiles : kEnd;
 };
-template <typename T, uint32_t HD, uint32_t WARPS>
-__global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 1 : 2) k_attn_one16(const AttnChunksParams p) {
+template <typename T, uint32_t HD, uint32_t WARPS, typename PR>
+__global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 1 : 2) k_attn_one16(const PR p) {
   extern __shared__ __align__(128) uint8_t dsm[];
   constexpr uint32_t kTileBytes = kSub * HD * 2;
   const uint32_t tid = threadIdx.x, warp = tid >> 5;
@@ -417,7 +419,7 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 1 : 2) k_attn_one16(c
   const T *base = reinterpret_cast<const T *>(p.pg.base) + (uint64_t)p.layer * p.pg.layer_stride;
   Segment s;
   if (!one_item(p, s)) return;
-  const uint32_t n = s.hi > s.lo ? range_units<kSub>(s.lo, s.hi) : 0;
+  const uint32_t n = s.hi > s.lo ? range_units<kSub>(p, s.lo, s.hi) : 0;
   Rows<T, HD> rows;
   walk_tiles<T, HD>(p, base, s, cluster_ctarank() * WARPS + warp, n, kOneCtas * WARPS, ktile, vtile, rows, [&] { rows.load(p, s, 0); });
   const Merge<HD, WARPS> pieces(dsm, rows);
@@ -436,11 +438,14 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 1 : 2) k_attn_one16(c
 // positions: 5.8 us against 6.4).
 template <typename T, uint32_t HD>
 int launch_one_hd(const AttnChunksParams &p, uint64_t span, cudaStream_t st) {
-  if (span > kOneCtas * 6 * kSub) {
-    const int rc = launch_one<k_attn_one16<T, HD, 8>>(p, one_items(p), 256, OneCfg<HD, 8>::kBytes, st);
-    if (rc <= 0) return rc;
-  }
-  return launch_one<k_attn_one16<T, HD, 6>>(p, one_items(p), 192, OneCfg<HD, 6>::kBytes, st);
+  return with_sinks(p, [&](auto a) {
+    using PR = decltype(a);
+    if (span > kOneCtas * 6 * kSub) {
+      const int rc = launch_one<k_attn_one16<T, HD, 8, PR>>(a, one_items(p), 256, OneCfg<HD, 8>::kBytes, st);
+      if (rc <= 0) return rc;
+    }
+    return launch_one<k_attn_one16<T, HD, 6, PR>>(a, one_items(p), 192, OneCfg<HD, 6>::kBytes, st);
+  });
 }
 
 // --------------------------- short calls of more rows: a cluster to 64 rows each
@@ -454,8 +459,8 @@ struct ShortCfg {
   static constexpr uint32_t kHalf = kSub * HD * 2, kTile = 2 * kHalf, LD = HD + 4;  // 32 positions, 64; floats of a row of a piece
   static constexpr uint32_t kTiles = 2 * 2 * kTile, kPiece = kShortRows * LD * 4 + kShortRows * 8, kBytes = kTiles > kPiece ? kTiles : kPiece;
 };
-template <typename T, uint32_t HD, uint32_t C>
-__global__ void __launch_bounds__(kThreads, 2) k_attn_short(const AttnChunksParams p) {
+template <typename T, uint32_t HD, uint32_t C, typename PR>
+__global__ void __launch_bounds__(kThreads, 2) k_attn_short(const PR p) {
   using S = ShortCfg<HD>;
   extern __shared__ __align__(128) uint8_t dsm[];
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
@@ -469,29 +474,30 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_short(const AttnChunksPara
   if (s.r0 >= s.chunk.rows) return;  // the whole cluster
   s.r1 = min(s.chunk.rows, s.r0 + kShortRows);
   tile_range(p, s.chunk, s.r0, s.r1, s.lo, s.hi);
-  const uint32_t n = s.hi > s.lo ? range_units<kShortPos>(s.lo, s.hi) : 0;
+  const uint32_t n = s.hi > s.lo ? range_units<kShortPos>(p, s.lo, s.hi) : 0;
   const uint32_t *pt = p.pg.page_table + (uint64_t)s.chunk.seq * p.pg.max_pages;
-  uint32_t u = cluster_ctarank(), t0 = (s.lo / kShortPos + u) * kShortPos;
-  // K and V of the tile at t, whose pages are looked up a tile ahead, to buffer `which`
+  uint32_t u = cluster_ctarank();
+  // K and V of tile u, whose pages are looked up a tile ahead, to buffer `which`
   PagePair ahead[2];
-  auto pages = [&](uint32_t t) {
+  auto pages = [&](uint32_t u) {
+    const uint32_t t = unit_at<kShortPos>(p, s.lo, u);
 #pragma unroll
-    for (uint32_t h = 0; h < 2; ++h) ahead[h] = look_up(pt, t + h * kSub, s.lo, s.hi);
+    for (uint32_t h = 0; h < 2; ++h) ahead[h] = look_up(p, pt, t + h * kSub, s.lo, s.hi);
   };
-  auto fetch = [&](uint32_t t, uint32_t which) {
-    const uint32_t k = smem_u32(dsm) + which * 2 * S::kTile;
+  auto fetch = [&](uint32_t u, uint32_t which) {
+    const uint32_t k = smem_u32(dsm) + which * 2 * S::kTile, t = unit_at<kShortPos>(p, s.lo, u);
 #pragma unroll
     for (uint32_t h = 0; h < 2; ++h) {
       flag_bad_pages(p, ahead[h]);
       stage<T, HD>(p, base, ahead[h], s.head, 0, t + h * kSub, s.lo, s.hi, k + h * S::kHalf, tid, kThreads);
       stage<T, HD>(p, base, ahead[h], s.head, 1, t + h * kSub, s.lo, s.hi, k + S::kTile + h * S::kHalf, tid, kThreads);
     }
-    pages(t + C * kShortPos);
+    pages(u + C);
   };
-  pages(t0);
-  if (u < n) fetch(t0, 0);
+  pages(u);
+  if (u < n) fetch(u, 0);
   cp_commit();
-  if (u + C < n) fetch(t0 + C * kShortPos, 1);
+  if (u + C < n) fetch(u + C, 1);
   cp_commit();
   const uint32_t first = s.r0 + 16 * warp;
   const bool mine = first < s.r1;
@@ -500,7 +506,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_short(const AttnChunksPara
   for (uint32_t which = 0; u < n; u += C, which ^= 1) {
     cp_wait<1>();
     __syncthreads();
-    const uint32_t k = smem_u32(dsm) + which * 2 * S::kTile;
+    const uint32_t k = smem_u32(dsm) + which * 2 * S::kTile, t0 = unit_at<kShortPos>(p, s.lo, u);
 #pragma unroll
     for (uint32_t h = 0; h < 2; ++h) {
       const uint32_t t = t0 + h * kSub;
@@ -511,9 +517,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_short(const AttnChunksPara
       rows.add_values(k + S::kTile + h * S::kHalf, sc);
     }
     __syncthreads();
-    if (u + 2 * C < n) fetch(t0 + 2 * C * kShortPos, which);
+    if (u + 2 * C < n) fetch(u + 2 * C, which);
     cp_commit();
-    t0 += C * kShortPos;
   }
   cp_wait<0>();
   rows.finish();
@@ -533,7 +538,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_short(const AttnChunksPara
 }
 template <typename T, uint32_t HD, uint32_t C>
 int launch_short_c(const AttnChunksParams &p, uint64_t items, cudaStream_t st) {
-  return launch_one<k_attn_short<T, HD, C>, C>(p, items, kThreads, ShortCfg<HD>::kBytes, st);
+  return with_sinks(p, [&](auto a) { return launch_one<k_attn_short<T, HD, C, decltype(a)>, C>(a, items, kThreads, ShortCfg<HD>::kBytes, st); });
 }
 template <typename T, uint32_t HD>
 int launch_short_hd(const AttnChunksParams &p, uint64_t items, uint32_t c, cudaStream_t st) {

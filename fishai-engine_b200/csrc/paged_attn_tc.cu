@@ -16,7 +16,7 @@
 //                    was rounded), read by the second MMA as its A operand.
 //   warp 8           issues the MMAs (an elected lane); owns the tensor memory
 //   warp 9           TMA: K and V tiles of 128 positions, a box per page of 16
-//                    (pages outside the item's range start past the end of the
+//                    (pages that the item does not see start past the end of the
 //                    tensor and arrive as zeros), 128-byte swizzle, a ring
 //   warps 10, 11     copy the next item's Q rows (a row is a token and a head,
 //                    so they are gathered) as soon as the last scores of the
@@ -215,8 +215,8 @@ __device__ __forceinline__ void load_q(const AttnChunksParams &p, const Segment 
   }
 }
 
-template <typename T, uint32_t HD, uint32_t G>
-__device__ void q_role(const AttnChunksParams &p, TcWalk<G> w, TcBars &b, uint32_t smem) {
+template <typename T, uint32_t HD, uint32_t G, typename PR>
+__device__ void q_role(const PR &p, TcWalk<G> w, TcBars &b, uint32_t smem) {
   const uint32_t tid = threadIdx.x & 63;
   uint32_t n[2] = {0, 0};  // fills of each tile so far
   for (Segment s; w.next(p, s);) {
@@ -241,8 +241,8 @@ __device__ __forceinline__ void st8(void *p, const uint32_t (&v)[8]) {
                : "memory");
 }
 
-template <typename T, uint32_t HD, uint32_t G>
-__device__ void softmax_role(const AttnChunksParams &p, TcWalk<G> w, TcBars &b, uint32_t tmem, uint32_t g) {
+template <typename T, uint32_t HD, uint32_t G, typename PR>
+__device__ void softmax_role(const PR &p, TcWalk<G> w, TcBars &b, uint32_t tmem, uint32_t g) {
   const uint32_t tid = threadIdx.x & 127, warp = tid >> 5;
   const uint32_t lanes = tmem + ((warp * 32) << 16);
   uint32_t n = 0;  // tiles of this group so far
@@ -257,7 +257,7 @@ __device__ void softmax_role(const AttnChunksParams &p, TcWalk<G> w, TcBars &b, 
     const uint32_t tiles = s.hi > s.lo ? s.u1 - s.u0 : 0;
     float m = -INFINITY, l = 0.0f;
     for (uint32_t k = 0; k < tiles; ++k, ++n) {
-      const uint32_t t0 = (s.lo / kTcPos + s.u0 + k) * kTcPos;
+      const uint32_t t0 = unit_at<kTcPos>(p, s.lo, s.u0 + k);
       if (!wait_bar(&b.abort, &b.s_full[g], n & 1)) return;
       if (idle) {
         mbar_arrive(&b.p_half[g]);
@@ -277,10 +277,16 @@ __device__ void softmax_role(const AttnChunksParams &p, TcWalk<G> w, TcBars &b, 
           if (c >= to) x[c] = -INFINITY;
       }
       if (p.window && !__all_sync(0xFFFFFFFFu, !live || to <= (int32_t)p.window)) {
-        const int32_t from = to - (int32_t)p.window;
+        const int32_t from = to - (int32_t)p.window, keep = (int32_t)p.sinks - (int32_t)t0;  // columns below `keep` stay
+        if (keep <= 0) {
 #pragma unroll
-        for (int32_t c = 0; c < (int32_t)kTcPos; ++c)
-          if (c < from) x[c] = -INFINITY;
+          for (int32_t c = 0; c < (int32_t)kTcPos; ++c)
+            if (c < from) x[c] = -INFINITY;
+        } else if (keep < (int32_t)kTcPos) {
+#pragma unroll
+          for (int32_t c = 0; c < (int32_t)kTcPos; ++c)
+            if (c < from && c >= keep) x[c] = -INFINITY;
+        }
       }
       float mx[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
@@ -380,8 +386,8 @@ __device__ void softmax_role(const AttnChunksParams &p, TcWalk<G> w, TcBars &b, 
   }
 }
 
-template <typename T, uint32_t HD, uint32_t G>
-__device__ void mma_role(const AttnChunksParams &p, TcWalk<G> w, TcBars &b, uint32_t smem, uint32_t tmem, uint32_t lead) {
+template <typename T, uint32_t HD, uint32_t G, typename PR>
+__device__ void mma_role(const PR &p, TcWalk<G> w, TcBars &b, uint32_t smem, uint32_t tmem, uint32_t lead) {
   using C = TcCfg<HD, G>;
   constexpr uint32_t kType = __is_same(T, __half) ? 0u : 1u;  // f16 / bf16, A and B
   constexpr uint32_t kS = (1u << 4) | (kType << 7) | (kType << 10) | ((kTcPos / 8) << 17) | ((128 / 16) << 24);
@@ -460,8 +466,8 @@ __device__ void mma_role(const AttnChunksParams &p, TcWalk<G> w, TcBars &b, uint
 }
 
 // one warp; fills: how many it began
-template <typename T, uint32_t HD, uint32_t G>
-__device__ void load_role(const AttnChunksParams &p, TcWalk<G> w, TcBars &b, uint32_t smem, const CUtensorMap *map, const CUtensorMap *row_map,
+template <typename T, uint32_t HD, uint32_t G, typename PR>
+__device__ void load_role(const PR &p, TcWalk<G> w, TcBars &b, uint32_t smem, const CUtensorMap *map, const CUtensorMap *row_map,
                           uint32_t &fills) {
   using C = TcCfg<HD, G>;
   const uint32_t lane = threadIdx.x & 31, ring = smem + G * C::kTile;
@@ -469,22 +475,21 @@ __device__ void load_role(const AttnChunksParams &p, TcWalk<G> w, TcBars &b, uin
   for (Segment s; w.next(p, s);) {
     const uint32_t tiles = s.hi > s.lo ? s.u1 - s.u0 : 0;
     const uint32_t *pt = p.pg.page_table + (uint64_t)s.chunk.seq * p.pg.max_pages;
-    const uint32_t first = (s.lo / kTcPos + s.u0) * kTcPos;
     auto look_up = [&](uint32_t t0) -> uint32_t {  // the lane's page of the tile
       const uint32_t t = t0 + (lane & 7) * kPageLen;
-      return t < s.hi && t + kPageLen > s.lo ? __ldg(pt + t / kPageLen) : 0xFFFFFFFFu;
+      return item_reads(p, s.lo, s.hi, t) ? __ldg(pt + t / kPageLen) : 0xFFFFFFFFu;
     };
+    const uint32_t first = unit_at<kTcPos>(p, s.lo, s.u0);
     uint32_t ahead = tiles ? look_up(first) : 0;
     for (uint32_t k = 0; k < tiles; ++k) {
-      const uint32_t t0 = first + k * kTcPos, page = ahead;
-      if (k + 1 < tiles) ahead = look_up(t0 + kTcPos);
-      const bool used = t0 + (lane & 7) * kPageLen < s.hi && t0 + (lane & 7) * kPageLen + kPageLen > s.lo;
+      const uint32_t t0 = unit_after<kTcPos>(p, s.lo, s.u0, first, k), page = ahead, at = t0 + (lane & 7) * kPageLen;
+      if (k + 1 < tiles) ahead = look_up(unit_after<kTcPos>(p, s.lo, s.u0 + k, t0, 1));
+      const bool used = item_reads(p, s.lo, s.hi, at);
       if (used && page >= p.pg.n_pages && p.err) atomicOr(p.err, kFlagPage);
       // A page with slots that nobody sees: V must not be NaN there (its weight 0
       // would not help), so its rows come one by one, the unseen ones from past
       // the end of the tensor, as zeros.
-      const uint32_t at = t0 + (lane & 7) * kPageLen;
-      const bool part = used && (at < s.lo || at + kPageLen > s.hi);
+      const bool part = used && (at + kPageLen > s.hi || (at < s.lo && at + kPageLen > p.sinks));
       const uint32_t parts = __ballot_sync(0xFFFFFFFFu, part && lane < 8);
       for (uint32_t is_v = 0; is_v < 2; ++is_v) {
         const uint32_t dst = ring + st * C::kTile;
@@ -497,7 +502,7 @@ __device__ void load_role(const AttnChunksParams &p, TcWalk<G> w, TcBars &b, uin
         if (go && is_v)
           for (uint32_t m = parts; m; m &= m - 1) {
             const uint32_t j = __ffs(m) - 1, pg = __shfl_sync(0xFFFFFFFFu, page, j), t = t0 + j * kPageLen + (lane & 15), half = lane >> 4;
-            const bool seen = t >= s.lo && t < s.hi;
+            const bool seen = item_sees(p, s.lo, s.hi, t);
             if (half < HD / 64)
               tma_2d(dst + half * C::kHalf + j * 2048 + (lane & 15) * 128, row_map, (int32_t)half * 64,
                      map_row(p.pg, seen ? pg : 0xFFFFFFFFu, 1, s.head) + (int32_t)(seen && pg < p.pg.n_pages ? lane & 15 : 0), &b.full[st]);
@@ -512,8 +517,8 @@ __device__ void load_role(const AttnChunksParams &p, TcWalk<G> w, TcBars &b, uin
   }
 }
 
-template <typename T, uint32_t HD, uint32_t G>
-__global__ void __launch_bounds__(128 * G + 128, 3 - G) k_attn_tc(const AttnChunksParams p, const __grid_constant__ CUtensorMap map,
+template <typename T, uint32_t HD, uint32_t G, typename PR>
+__global__ void __launch_bounds__(128 * G + 128, 3 - G) k_attn_tc(const PR p, const __grid_constant__ CUtensorMap map,
                                                             const __grid_constant__ CUtensorMap row_map) {
   using C = TcCfg<HD, G>;
   extern __shared__ __align__(1024) uint8_t raw[];
@@ -602,11 +607,14 @@ uint32_t launch_g(const AttnChunksParams &p, uint32_t n_sm, bool overlap, cudaSt
   using C = TcCfg<HD, G>;
   CUtensorMap map, row_map;
   if (!page_map(p, kPageLen, &map) || !page_map(p, 1, &row_map)) return 0;
-  if (cudaFuncSetAttribute(k_attn_tc<T, HD, G>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::kSmem) != cudaSuccess) return 0;
   const uint32_t ctas = (n_sm < kTcMaxCtas ? n_sm : kTcMaxCtas) * (3 - G);  // one or two an SM
-  if (overlap) return launch_pdl(k_attn_tc<T, HD, G>, dim3(ctas), dim3(C::kThreads), C::kSmem, st, p, map, row_map) ? 0 : ctas;
-  k_attn_tc<T, HD, G><<<ctas, C::kThreads, C::kSmem, st>>>(p, map, row_map);
-  return cudaGetLastError() == cudaSuccess ? ctas : 0;
+  return with_sinks(p, [&](auto a) -> uint32_t {
+    using PR = decltype(a);
+    if (cudaFuncSetAttribute(k_attn_tc<T, HD, G, PR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::kSmem) != cudaSuccess) return 0;
+    if (overlap) return launch_pdl(k_attn_tc<T, HD, G, PR>, dim3(ctas), dim3(C::kThreads), C::kSmem, st, a, map, row_map) ? 0 : ctas;
+    k_attn_tc<T, HD, G><<<ctas, C::kThreads, C::kSmem, st>>>(a, map, row_map);
+    return cudaGetLastError() == cudaSuccess ? ctas : 0;
+  });
 }
 template <typename T>
 uint32_t launch_t(const AttnChunksParams &p, uint32_t n_sm, bool overlap, cudaStream_t st, uint32_t *R) {

@@ -23,6 +23,7 @@ inline uint64_t page_bytes(const fa_pages &p) {
 // ---- rotary positions with the append to the pages ----
 struct RopeTable {                   // a kernel parameter (constant bank)
   double turns[kMaxHeadDim / 2];     // f_i / 2 pi: turns per position
+  uint8_t axis[kMaxHeadDim / 2];     // the pair's row of positions
   float scale;                       // factor on the turned elements
 };
 struct RopeAppendParams {
@@ -33,6 +34,7 @@ struct RopeAppendParams {
   uint64_t qs, ks, vs, os;           // row strides, elements
   uint32_t n_tokens, n_heads, rot, half_layout;
   const uint32_t *pos, *seq, *slot;
+  uint64_t pos_stride;               // from one axis's positions to the next's; 0: one axis
   void *out;
   uint32_t *err;
 };
@@ -50,6 +52,7 @@ struct AttnChunksParams {
   const uint32_t *q_start, *kv_len, *seq;
   float scale_log2;                  // scale * log2(e)
   uint32_t window;
+  uint32_t sinks;                    // positions below it are seen beside the window (0 without a window)
   uint32_t aligned;                  // q and out rows are 16-byte aligned
   uint32_t rows_min, rows_max;       // a launch takes the chunks with rows_min <= q_len * rep <= rows_max
   float *part;                       // split items: two slots a CTA

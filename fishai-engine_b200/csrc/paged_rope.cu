@@ -9,7 +9,8 @@
 // bits (exact to 2^-53 of the turn count), its fraction in [-1/2, 1/2] in 32
 // bits, sincospi of that.  In 32 bits the product alone would be wrong by
 // 2^-24 * pos radians, 0.06 at position 10^6.  Then each thread turns or
-// copies a unit of up to 8 pairs or 16 elements.
+// copies a unit of up to 8 pairs or 16 elements.  With several axes (images and
+// video) a pair's position is that of its axis; all else is the same.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -65,7 +66,7 @@ __device__ __forceinline__ void store_n(T *p, const float (&x)[N]) {
 // token's is always in flight while one is turned and stored.  (A CTA a token,
 // loading after its angles: 46 us for 8192 tokens of 48 heads.)
 constexpr uint32_t kRopeTokens = 4;
-template <typename TI, typename TO, int W>
+template <typename TI, typename TO, int W, bool AXES>
 __global__ void __launch_bounds__(512) k_rope_append(const RopeAppendParams p, const __grid_constant__ RopeTable tab, uint32_t each) {
   __shared__ float cs[kRopeTokens][kMaxHeadDim / 2], sn[kRopeTokens][kMaxHeadDim / 2];
   __shared__ uint64_t place[kRopeTokens];  // element offset of the token's slot in a (K, head 0) block
@@ -103,7 +104,7 @@ __global__ void __launch_bounds__(512) k_rope_append(const RopeAppendParams p, c
   }
   for (uint32_t i = threadIdx.x; i < nt * half; i += blockDim.x) {
     const uint32_t k = i / half, j = i - k * half;
-    const double a = (double)p.pos[t0 + k] * tab.turns[j];
+    const double a = (double)p.pos[t0 + k + (AXES ? tab.axis[j] * p.pos_stride : 0)] * tab.turns[j];
     float s, c;
     sincospif(2.0f * (float)(a - rint(a)), &s, &c);
     cs[k][j] = c * tab.scale;
@@ -152,7 +153,7 @@ __global__ void __launch_bounds__(512) k_rope_append(const RopeAppendParams p, c
   }
 }
 
-template <typename TI, typename TO>
+template <typename TI, typename TO, bool AXES>
 int launch_io(const RopeAppendParams &p, const RopeTable &t, cudaStream_t st) {
   const uint32_t half = p.rot / 2, hd = p.pg.head_dim;
   // every unit starts on a multiple of n elements of every buffer (pages: hd is
@@ -176,29 +177,34 @@ int launch_io(const RopeAppendParams &p, const RopeTable &t, cudaStream_t st) {
   if ((units + block - 1) / block > 65535) block = 512;  // grid y (thousands of heads)
   const dim3 grid((p.n_tokens + each - 1) / each, (units + block - 1) / block);
   if constexpr (sizeof(TI) == 2 && sizeof(TO) == 2) {
-    if (W == 8) k_rope_append<TI, TO, 8><<<grid, block, 0, st>>>(p, t, each);
+    if (W == 8) k_rope_append<TI, TO, 8, AXES><<<grid, block, 0, st>>>(p, t, each);
   }
-  if (W == 4) k_rope_append<TI, TO, 4><<<grid, block, 0, st>>>(p, t, each);
-  if (W == 1) k_rope_append<TI, TO, 1><<<grid, block, 0, st>>>(p, t, each);
+  if (W == 4) k_rope_append<TI, TO, 4, AXES><<<grid, block, 0, st>>>(p, t, each);
+  if (W == 1) k_rope_append<TI, TO, 1, AXES><<<grid, block, 0, st>>>(p, t, each);
   return cudaGetLastError() == cudaSuccess ? 0 : -1;
 }
-template <typename TI>
+template <typename TI, bool AXES>
 int launch_in(const RopeAppendParams &p, const RopeTable &t, cudaStream_t st) {
   switch (p.pg.dtype) {
-    case FA_KV_F32: return launch_io<TI, float>(p, t, st);
-    case FA_KV_F16: return launch_io<TI, __half>(p, t, st);
-    default: return launch_io<TI, __nv_bfloat16>(p, t, st);
+    case FA_KV_F32: return launch_io<TI, float, AXES>(p, t, st);
+    case FA_KV_F16: return launch_io<TI, __half, AXES>(p, t, st);
+    default: return launch_io<TI, __nv_bfloat16, AXES>(p, t, st);
+  }
+}
+
+template <bool AXES>
+int launch_axes(const RopeAppendParams &p, const RopeTable &t, cudaStream_t st) {
+  switch (p.in_dtype) {
+    case FA_KV_F32: return launch_in<float, AXES>(p, t, st);
+    case FA_KV_F16: return launch_in<__half, AXES>(p, t, st);
+    default: return launch_in<__nv_bfloat16, AXES>(p, t, st);
   }
 }
 
 }  // namespace
 
 int launch_rope_append(const RopeAppendParams &p, const RopeTable &t, cudaStream_t st) {
-  switch (p.in_dtype) {
-    case FA_KV_F32: return launch_in<float>(p, t, st);
-    case FA_KV_F16: return launch_in<__half>(p, t, st);
-    default: return launch_in<__nv_bfloat16>(p, t, st);
-  }
+  return p.pos_stride ? launch_axes<true>(p, t, st) : launch_axes<false>(p, t, st);
 }
 
 }  // namespace fa

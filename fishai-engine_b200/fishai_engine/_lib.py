@@ -19,6 +19,7 @@ KV_F32, KV_F16, KV_BF16 = 0, 1, 2
 FLAG_PAGE, FLAG_RANGE, FLAG_TIMEOUT = 16, 32, 64
 ROPE_INTERLEAVED, ROPE_HALF = 0, 1
 ROPE_PLAIN, ROPE_LINEAR, ROPE_NTK, ROPE_LLAMA3, ROPE_YARN = 0, 1, 2, 3, 4
+AXES_BLOCKS, AXES_TURNS, AXES_SHARED, AXES_OWN = 0, 1, 0, 1
 NO_TOKEN = 4294967295
 DEBUG_WAIT_LIMIT_NS, DEBUG_WITHHOLD_WEIGHTS, DEBUG_FIXED_ORDER_SUMS, DEBUG_WITHHOLD_KV = 1, 2, 3, 4
 
@@ -73,6 +74,10 @@ class fa_rope_config(C.Structure):
                 ("base", C.c_double), ("factor", C.c_double), ("context", C.c_uint32), ("low_turns", C.c_double),
                 ("high_turns", C.c_double), ("beta_fast", C.c_double), ("beta_slow", C.c_double),
                 ("attn_factor", C.c_double)]
+
+
+class fa_rope_axes(C.Structure):
+    _fields_ = [("n_axes", C.c_uint32), ("pairs", C.c_uint32 * 4), ("order", C.c_int32), ("freqs", C.c_int32)]
 
 
 class fa_beam_config(C.Structure):
@@ -163,9 +168,15 @@ SIGNATURES = {
     "fa_rope_freqs": ([_vp, C.POINTER(C.c_double), C.POINTER(C.c_double)], _i),
     "fa_rope_append": ([_vp, _vp, _u32, C.c_int32, _vp, _u64, _vp, _u64, _vp, _u64, _u32, _u32, _vp, _vp, _vp, _vp,
                         _u64, _vp, _vp], _i),
+    "fa_rope_create_axes": ([C.POINTER(fa_rope_config), C.POINTER(fa_rope_axes), C.POINTER(_vp)], _i),
+    "fa_rope_axis_of": ([_vp, _pu32], _i),
+    "fa_rope_append_axes": ([_vp, _vp, _u32, C.c_int32, _vp, _u64, _vp, _u64, _vp, _u64, _u32, _u32, _vp, _u64, _vp, _vp, _vp,
+                             _u64, _vp, _vp], _i),
     "fa_attn_chunks": ([_vp, _u32, _vp, _u64, _u32, _u32, _vp, _vp, _vp, _u32, _u32, _f, _u32, _vp, _u64, _vp, _sz,
                         _vp, _vp], _i),
     "fa_attn_chunks_ws": ([_u32], _sz),
+    "fa_attn_chunks_sinks": ([_vp, _u32, _vp, _u64, _u32, _u32, _vp, _vp, _vp, _u32, _u32, _f, _u32, _u32, _vp, _u64, _vp,
+                              _sz, _vp, _vp], _i),
     "fa_pages_copy": ([_vp, _vp, _vp, _vp, _u32, _vp, _vp], _i),
     "fa_pages_compact": ([_vp, _vp, _vp, _vp, _u32, _u32, _vp, _vp], _i),
     "fa_beam_select": ([_vp, C.c_int32, _u64, _u32, _u32, _u32, _vp, _vp, _u32, _u32, _u32, _vp, _vp, _vp, _vp, _vp,

@@ -126,17 +126,25 @@ class PagedKV:
 _LAYOUTS = {"interleaved": L.ROPE_INTERLEAVED, "half": L.ROPE_HALF}
 _SCALINGS = {"none": L.ROPE_PLAIN, "linear": L.ROPE_LINEAR, "ntk": L.ROPE_NTK, "llama3": L.ROPE_LLAMA3,
              "yarn": L.ROPE_YARN}
+_ORDERS = {"blocks": L.AXES_BLOCKS, "turns": L.AXES_TURNS}
+_FREQS = {"shared": L.AXES_SHARED, "own": L.AXES_OWN}
 
 
 class Rope:
     """Rotary frequencies of a head (fa_rope_create): layout "interleaved"
     (pairs 2i, 2i+1, as the model's own, src/tensor.rs:331-392) or "half" (pairs
     i, i + rot_dim/2), rot_dim elements turned, scaling "none", "linear", "ntk",
-    "llama3" or "yarn" by `factor` beyond `context` positions."""
+    "llama3" or "yarn" by `factor` beyond `context` positions.
+
+    axes: pairs of each of up to four axes (time, height, width ..; together
+    rot_dim / 2) whose positions a token has, one after another ("blocks") or in
+    "turns", with the head's frequencies ("shared") or a series of each axis's
+    "own"."""
 
     def __init__(self, head_dim: int, rot_dim: int = None, base: float = 10000.0, layout: str = "interleaved",
                  scaling: str = "none", factor: float = 1.0, context: int = 8192, low_turns: float = 1.0,
-                 high_turns: float = 4.0, beta_fast: float = 32.0, beta_slow: float = 1.0, attn_factor: float = 0.0):
+                 high_turns: float = 4.0, beta_fast: float = 32.0, beta_slow: float = 1.0, attn_factor: float = 0.0,
+                 axes=None, axis_order: str = "blocks", axis_freqs: str = "shared"):
         if layout not in _LAYOUTS or scaling not in _SCALINGS:
             raise ValueError(f"layout is one of {sorted(_LAYOUTS)}, scaling one of {sorted(_SCALINGS)}")
         self._h = None
@@ -145,7 +153,20 @@ class Rope:
         c = L.fa_rope_config(head_dim, self.rot_dim, _LAYOUTS[layout], _SCALINGS[scaling], base, factor, context,
                              low_turns, high_turns, beta_fast, beta_slow, attn_factor)
         h = C.c_void_p()
-        L.check(L.lib().fa_rope_create(C.byref(c), C.byref(h)))
+        self.n_axes = 1
+        if axes is None:
+            L.check(L.lib().fa_rope_create(C.byref(c), C.byref(h)))
+        else:
+            axes = list(axes)
+            if axis_order not in _ORDERS or axis_freqs not in _FREQS:
+                raise ValueError(f"axis_order is one of {sorted(_ORDERS)}, axis_freqs one of {sorted(_FREQS)}")
+            if not 1 <= len(axes) <= 4:
+                raise ValueError("axes: pairs of 1 to 4 axes")
+            for n in axes:
+                L.u32(axes=n)
+            a = L.fa_rope_axes(len(axes), (C.c_uint32 * 4)(*axes), _ORDERS[axis_order], _FREQS[axis_freqs])
+            L.check(L.lib().fa_rope_create_axes(C.byref(c), C.byref(a), C.byref(h)))
+            self.n_axes = len(axes)
         self._h = h
 
     def __del__(self):
@@ -159,6 +180,12 @@ class Rope:
         L.check(L.lib().fa_rope_freqs(self._h, f, C.byref(s)))
         return list(f), s.value
 
+    def axis_of(self):
+        """the axis of each of the rot_dim/2 pairs"""
+        a = (C.c_uint32 * (self.rot_dim // 2))()
+        L.check(L.lib().fa_rope_axis_of(self._h, a))
+        return list(a)
+
 
 def rope_append(kv: PagedKV, layer: int, rope: Rope, q, k, v, positions, seqs, out, slots=None, err=None,
                 stream: int = 0):
@@ -166,7 +193,8 @@ def rope_append(kv: PagedKV, layer: int, rope: Rope, q, k, v, positions, seqs, o
     head_dim] of the pages' type; q itself if the types agree), and puts k and v
     at cache position slots[t] (default positions[t]) of sequence seqs[t].  q, k
     and v are rows of one type, with any row stride (slices of a fused
-    projection).  seqs[t] = NO_TOKEN leaves a row out."""
+    projection).  seqs[t] = NO_TOKEN leaves a row out.  A rope of several axes
+    takes positions [axes, tokens] (any row stride) and needs slots."""
     n = q.shape[0]
     dt = _code(q, "q")
     if layer >> 32:
@@ -181,10 +209,20 @@ def rope_append(kv: PagedKV, layer: int, rope: Rope, q, k, v, positions, seqs, o
     kp, ks = _rows(k, "k", n, kw)
     vp, vs = _rows(v, "v", n, kw)
     op, os = _rows(out, "out", n, width)
-    rc = L.lib().fa_rope_append(rope._h, kv._ref, layer, dt, qp, qs, kp, ks, vp, vs, n, width // hd,
-                                _index(positions, "positions", n), _index(seqs, "seqs", n),
-                                None if slots is None else _index(slots, "slots", n), op, os,
-                                None if err is None else _index(err, "err", 1), stream)
+    if rope.n_axes > 1:
+        if slots is None:
+            raise ValueError("slots: needed with several axes")
+        shape, stride = positions.shape, positions.stride()
+        if shape != (rope.n_axes, n) or positions.dtype not in _INTS or (n > 1 and stride[1] != 1):
+            raise ValueError(f"positions: an int32 [{rope.n_axes}, {n}] tensor with consecutive elements is needed")
+        rc = L.lib().fa_rope_append_axes(rope._h, kv._ref, layer, dt, qp, qs, kp, ks, vp, vs, n, width // hd,
+                                         positions.data_ptr(), stride[0], _index(seqs, "seqs", n), _index(slots, "slots", n),
+                                         op, os, None if err is None else _index(err, "err", 1), stream)
+    else:
+        rc = L.lib().fa_rope_append(rope._h, kv._ref, layer, dt, qp, qs, kp, ks, vp, vs, n, width // hd,
+                                    _index(positions, "positions", n), _index(seqs, "seqs", n),
+                                    None if slots is None else _index(slots, "slots", n), op, os,
+                                    None if err is None else _index(err, "err", 1), stream)
     if rc:
         L.check(rc)
 
@@ -202,27 +240,28 @@ def workspace_bytes(head_dim: int) -> int:
 
 
 def attention(kv: PagedKV, layer: int, q, q_start, kv_len, out, max_q: int, workspace, seqs=None, scale: float = 0.0,
-              window: int = 0, err=None, stream: int = 0):
+              window: int = 0, sinks: int = 0, err=None, stream: int = 0):
     """Attention of chunks of new tokens over the pages: rows q_start[c] ..
     q_start[c+1] of q and out are a chunk of sequence seqs[c] (default c), whose
     cache holds kv_len[c] positions with the chunk's own last.  Each token sees
-    the positions up to its own (the last `window` of them where window > 0).
+    the positions up to its own (the last `window` of them where window > 0, and
+    beside those the first `sinks` of the sequence).
     max_q: no chunk is longer.  workspace: a uint8 tensor of
     workspace_bytes(head_dim), used by no other call that may run at the same
     time.  scale 0: 1 / sqrt(head_dim)."""
     n, t = kv_len.shape[0], q.shape[0]
     if _code(q, "q") != kv.dtype or out.dtype != q.dtype:
         raise ValueError("q and out have the pages' element type")
-    if (layer | max_q | window) >> 32:
-        L.u32(layer=layer, max_q=max_q, window=window)
+    if (layer | max_q | window | sinks) >> 32:
+        L.u32(layer=layer, max_q=max_q, window=window, sinks=sinks)
     hd = kv.head_dim
     width = _width(q, hd)
     qp, qs = _rows(q, "q", t, width)
     op, os = _rows(out, "out", t, width)
-    rc = L.lib().fa_attn_chunks(kv._ref, layer, qp, qs, width // hd, n, _index(q_start, "q_start", n + 1),
-                                _index(kv_len, "kv_len", n), None if seqs is None else _index(seqs, "seqs", n), t, max_q,
-                                scale, window, op, os, *_space(workspace), None if err is None else _index(err, "err", 1),
-                                stream)
+    rc = L.lib().fa_attn_chunks_sinks(kv._ref, layer, qp, qs, width // hd, n, _index(q_start, "q_start", n + 1),
+                                      _index(kv_len, "kv_len", n), None if seqs is None else _index(seqs, "seqs", n), t, max_q,
+                                      scale, window, sinks, op, os, *_space(workspace),
+                                      None if err is None else _index(err, "err", 1), stream)
     if rc:
         L.check(rc)
 

@@ -353,6 +353,37 @@ int fa_rope_append(const fa_rope *r, const fa_pages *pages, uint32_t layer, int3
                    uint32_t n_tokens, uint32_t n_heads, const uint32_t *pos, const uint32_t *seq, const uint32_t *slot,
                    void *out, uint64_t out_stride, uint32_t *err, void *stream);
 
+/* Several axes (time, height, width of images and video in a prompt): each pair
+ * turns with the position on its own axis.  pairs[a] of the rot_dim / 2 pairs
+ * belong to axis a: in blocks one axis after another, or in turns, pair i to axis
+ * i % n_axes until that axis has its pairs, what is left to axis 0.  Frequencies
+ * are those of the whole head, f_i as above with the pair's place i in it, or
+ * each axis's own: f_j with j the pair's place among the axis's and 2 pairs[a] in
+ * place of rot_dim, in the scalings too.  With all axes at the same position (text)
+ * shared frequencies turn as one axis does. */
+#define FA_ROPE_MAX_AXES 4
+#define FA_AXES_BLOCKS 0
+#define FA_AXES_TURNS 1
+#define FA_AXES_SHARED 0
+#define FA_AXES_OWN 1
+typedef struct {
+  uint32_t n_axes;                   /* 1 .. 4 */
+  uint32_t pairs[FA_ROPE_MAX_AXES];  /* at least 1 each, rot_dim / 2 together */
+  int32_t order, freqs;              /* FA_AXES_* */
+} fa_rope_axes;
+int fa_rope_create_axes(const fa_rope_config *cfg, const fa_rope_axes *axes, fa_rope **out);
+/* the axis of each of the rot_dim / 2 pairs (0 for a rope of one axis) */
+int fa_rope_axis_of(const fa_rope *r, uint32_t *axis);
+/* fa_rope_append with a position on each axis: that of token t on axis a is
+ * pos[a pos_stride + t] (pos_stride >= n_tokens, or 0: the same on all axes).
+ * slot is needed: the cache
+ * counts tokens, not positions.  A rope of several axes is refused by
+ * fa_rope_append, one of one axis is welcome here. */
+int fa_rope_append_axes(const fa_rope *r, const fa_pages *pages, uint32_t layer, int32_t in_dtype, const void *q,
+                        uint64_t q_stride, const void *k, uint64_t k_stride, const void *v, uint64_t v_stride,
+                        uint32_t n_tokens, uint32_t n_heads, const uint32_t *pos, uint64_t pos_stride, const uint32_t *seq,
+                        const uint32_t *slot, void *out, uint64_t out_stride, uint32_t *err, void *stream);
+
 /* Attention of chunks of new tokens over the pages of `layer`
  * (src/tensor.rs:451-551 with the causal order of src/model.rs:644-650).
  * Chunk c: rows q_start[c] .. q_start[c+1] - 1 of q and out, cache sequence
@@ -387,6 +418,15 @@ int fa_attn_chunks(const fa_pages *pages, uint32_t layer, const void *q, uint64_
                    uint32_t n_tokens, uint32_t max_q, float scale, uint32_t window, void *out, uint64_t out_stride,
                    void *ws, size_t ws_bytes, uint32_t *err, void *stream);
 size_t fa_attn_chunks_ws(uint32_t head_dim);
+/* The same with some first positions that stay visible: where window > 0, a
+ * token at p sees the positions t <= p with t > p - window or t < sinks (window
+ * 0: all, as above).  For streams that run on and on with a window, whose first
+ * tokens draw much of the weight.  Pages that hold only positions between the
+ * two are not looked up: the caller may have used them for something else. */
+int fa_attn_chunks_sinks(const fa_pages *pages, uint32_t layer, const void *q, uint64_t q_stride, uint32_t n_heads,
+                         uint32_t n_chunks, const uint32_t *q_start, const uint32_t *kv_len, const uint32_t *seq,
+                         uint32_t n_tokens, uint32_t max_q, float scale, uint32_t window, uint32_t sinks, void *out,
+                         uint64_t out_stride, void *ws, size_t ws_bytes, uint32_t *err, void *stream);
 
 /* Copies the first slots[i] positions (slots NULL: all 16) of page src[i] to
  * page dst[i], keys and values, in every layer, i < n; src, dst, slots are

@@ -1,0 +1,66 @@
+"""Plain 64-bit forms of the operators around a serving step, and error bounds
+derived from the arithmetic the kernels may use."""
+import math
+
+import torch
+
+import paged_ref as R
+
+PAGE = R.PAGE
+half_step = R.half_step
+
+
+def sees(n, q, window, sinks, device="cuda"):
+    """[q, n]: which positions each of a chunk's tokens sees"""
+    pos = torch.arange(n - q, n, device=device)[:, None]
+    t = torch.arange(n, device=device)[None]
+    return (t <= pos) & ((t > pos - window) | (t < sinks)) if window else t <= pos
+
+
+def empty_gap(pages, table, qs, kvs, window, sinks):
+    """What no token of a chunk sees: NaN in its slots, and no page at all where a whole page is unseen."""
+    pages, table = pages.clone(), table.clone()
+    for c, (q, n) in enumerate(zip(qs, kvs)):
+        if not q or not n:
+            continue
+        used = sees(n, q, window, sinks, "cpu").any(0)
+        for e in range(-(-n // PAGE)):
+            mine = used[e * PAGE: (e + 1) * PAGE]
+            for slot in (~mine).nonzero().flatten().tolist():
+                pages[:, int(table[c, e]), :, :, slot] = float("nan")
+            if not mine.any():
+                table[c, e] = 10 ** 6
+    return pages, table
+
+
+def attention(pages, table, q, q_start, kv_len, heads, scale, window, sinks):
+    """(output, bound) of layer 0, chunk c of sequence c; the bound as in paged_ref.attention: scores are sums of hd products
+    in f32, weights and their sums in f32, the weights rounded to the type once for their product, the result once."""
+    hd, rep = pages.shape[5], heads // pages.shape[3]
+    out = torch.zeros(q.shape[0], heads, hd, dtype=torch.float64, device=q.device)
+    tol = torch.zeros_like(out)
+    u, e = half_step(q.dtype), 2.0 ** -24
+    sc = scale or hd ** -0.5
+    for c, n in enumerate(kv_len):
+        a, b = q_start[c], q_start[c + 1]
+        if b == a or n == 0:
+            continue
+        k, v = R.rows_of(pages, table.clamp_max(pages.shape[1] - 1), 0, c, n)
+        k, v = k.double().repeat_interleave(rep, 1), v.double().repeat_interleave(rep, 1)
+        x = q[a:b].double().view(b - a, heads, hd)
+        see = sees(n, b - a, window, sinks)
+        used = see.any(0)
+        k, v = torch.where(used[:, None, None], k, 0), torch.where(used[:, None, None], v, 0)
+        s = torch.einsum("ihd,thd->hit", x, k) * sc
+        size = torch.einsum("ihd,thd->hit", x.abs(), k.abs()) * sc
+        s = s.masked_fill(~see, -math.inf)
+        p = torch.exp(s - s.amax(-1, keepdim=True).clamp_min(-1e300))
+        w = p.sum(-1, keepdim=True)
+        p = torch.where(w > 0, p / w.clamp_min(1e-300), 0)
+        out[a:b] = torch.einsum("hit,thd->ihd", p, v)
+        worst = torch.where(see, size, 0).amax(-1, keepdim=True)
+        rel = 2 * (2 * (hd + 5) * e * worst) + (2 * n + 12) * e + (u if q.dtype != torch.float32 else 0)
+        tol[a:b] = torch.einsum("hit,thd->ihd", p * rel, v.abs()) + out[a:b].abs() * (rel.permute(1, 0, 2) + u) + 1e-30
+        if q.dtype == torch.float16:
+            tol[a:b] += 2.0 ** -25  # the smallest step of f16
+    return out, tol

@@ -1,0 +1,107 @@
+"""Refusals of the operators around a serving step and what is computed on the host: no GPU needed.  Every case is refused
+before any pointer is looked at or any kernel runs."""
+import ctypes as C
+import math
+
+import pytest
+
+from fishai_engine import _lib as L
+from fishai_engine import paged
+
+P = 0x30000  # an address that is never read
+
+
+def pages(**kw):
+    f = dict(base=0x10000, layer_stride=2 * 4 * 16 * 64 * 8, dtype=L.KV_F16, n_layers=2, n_pages=8, n_kv_heads=4, head_dim=64,
+             page_table=0x20000, n_seq=2, max_pages=4)
+    f.update(kw)
+    return L.fa_pages(**f)
+
+
+# ------------------------------------------------------------------ attention with first positions
+def call_sinks(pg=None, layer=0, q=P, qs=512, heads=8, chunks=2, starts=P, kv=P, seq=None, n=3, max_q=3, scale=0.0, window=5, sinks=2,
+               out=P * 4, os=512, ws=P * 16, ws_bytes=None):
+    ws_bytes = L.lib().fa_attn_chunks_ws(64) if ws_bytes is None else ws_bytes
+    return L.lib().fa_attn_chunks_sinks(C.addressof(pg or pages()), layer, q, qs, heads, chunks, starts, kv, seq, n, max_q, scale, window,
+                                        sinks, out, os, ws, ws_bytes, None, None)
+
+
+@pytest.mark.parametrize("bad", [dict(layer=2), dict(heads=0), dict(heads=6), dict(qs=511), dict(os=500), dict(scale=-1.0), dict(scale=math.nan),
+                                 dict(q=None), dict(starts=None), dict(kv=None), dict(out=None), dict(ws=None), dict(chunks=3),
+                                 dict(ws_bytes=100), dict(ws=P * 16 + 8), dict(q=P + 1), dict(out=P), dict(n=1 << 30), dict(starts=P + 2),
+                                 dict(pg=pages(dtype=7)), dict(pg=pages(base=None)), dict(pg=pages(max_pages=0))], ids=str)
+def test_attention_with_sinks_refuses(bad):
+    assert call_sinks(**bad) == L.ERR_INVALID
+    assert "fa_attn_chunks_sinks" in L.last_error()
+
+
+def test_attention_with_sinks_of_nothing():
+    assert call_sinks(n=0, q=None, out=None) == L.OK
+    assert call_sinks(chunks=0, starts=None, kv=None) == L.OK
+
+
+# ------------------------------------------------------------------ rotary positions with several axes
+@pytest.mark.parametrize("bad", [dict(axes=[16, 17]), dict(axes=[32, 0]), dict(axes=[0, 32]), dict(axes=[8, 8, 8]), dict(axes=[2 ** 32 - 1, 33]),
+                                 dict(axes=[1, 31], axis_order="turns"), dict(axes=[10, 10, 12], axis_order="turns"),
+                                 dict(axes=[31, 1], axis_freqs="own", scaling="ntk", factor=2.0)], ids=str)
+def test_axes_that_do_not_fit_are_refused(bad):
+    with pytest.raises(L.FishaiError):
+        paged.Rope(64, **bad)
+
+
+@pytest.mark.parametrize("bad", [dict(axes=[]), dict(axes=[8] * 5), dict(axes=[32, -1]), dict(axes=[16, 16], axis_order="rows"),
+                                 dict(axes=[16, 16], axis_freqs="mine"), dict(axes=[2 ** 32, 32])], ids=str)
+def test_axes_that_python_refuses(bad):
+    with pytest.raises(ValueError):
+        paged.Rope(64, **bad)
+
+
+def test_unknown_orders_are_refused_by_the_library():
+    lib, cfg, h = L.lib(), L.fa_rope_config(), C.c_void_p()
+    lib.fa_rope_config_default(C.byref(cfg), 64, 10000.0)
+    four = C.c_uint32 * 4
+    for ax in (L.fa_rope_axes(2, four(16, 16), 2, 0), L.fa_rope_axes(2, four(16, 16), 0, 2), L.fa_rope_axes(0, four(), 0, 0),
+               L.fa_rope_axes(5, four(8, 8, 8, 8), 0, 0)):
+        assert lib.fa_rope_create_axes(C.byref(cfg), C.byref(ax), C.byref(h)) == L.ERR_INVALID
+    assert lib.fa_rope_create_axes(C.byref(cfg), None, C.byref(h)) == L.ERR_INVALID
+    assert lib.fa_rope_create_axes(None, C.byref(L.fa_rope_axes(1, four(32), 0, 0)), C.byref(h)) == L.ERR_INVALID
+    assert lib.fa_rope_axis_of(None, None) == L.ERR_INVALID
+
+
+def test_axis_and_frequency_of_each_pair():
+    assert paged.Rope(64).axis_of() == [0] * 32
+    r = paged.Rope(64, axes=[12, 10, 10])
+    assert r.axis_of() == [0] * 12 + [1] * 10 + [2] * 10
+    assert r.freqs() == paged.Rope(64).freqs()
+    # in turns: 0 1 2 0 1 2 .. as long as an axis has pairs, the rest is of axis 0
+    assert paged.Rope(16, axes=[4, 3, 1], axis_order="turns").axis_of() == [0, 1, 2, 0, 1, 0, 0, 1]
+    assert paged.Rope(16, axes=[5, 1, 2], axis_order="turns").axis_of() == [0, 1, 2, 0, 0, 2, 0, 0]
+    # an axis's own series: that of a rope of its width
+    r = paged.Rope(64, axes=[12, 10, 10], axis_freqs="own")
+    assert r.freqs()[0] == paged.Rope(64, rot_dim=24).freqs()[0] + 2 * paged.Rope(64, rot_dim=20).freqs()[0]
+    for scaling in ("linear", "ntk", "llama3", "yarn"):
+        kw = dict(scaling=scaling, factor=4.0, context=2048)
+        r = paged.Rope(64, axes=[14, 9, 9], axis_order="turns", axis_freqs="own", **kw)
+        want = {a: iter(paged.Rope(64, rot_dim=2 * n, **kw).freqs()[0]) for a, n in enumerate([14, 9, 9])}
+        assert r.freqs()[0] == [next(want[a]) for a in r.axis_of()]
+
+
+def call_axes(r=None, pg=None, layer=0, dt=L.KV_F16, q=P, qs=512, k=P * 2, ks=256, v=P * 3, vs=256, n=3, heads=8, pos=P, ps=3, seq=P, slot=P,
+              out=P * 4, os=512):
+    r = r or paged.Rope(64, axes=[16, 16])
+    return L.lib().fa_rope_append_axes(r._h, C.addressof(pg or pages()), layer, dt, q, qs, k, ks, v, vs, n, heads, pos, ps, seq, slot, out, os,
+                                       None, None)
+
+
+@pytest.mark.parametrize("bad", [dict(ps=2), dict(slot=None), dict(pos=None), dict(seq=None), dict(pos=P + 2), dict(q=None), dict(layer=2),
+                                 dict(dt=5), dict(qs=511), dict(out=P + 512), dict(pg=pages(head_dim=128))], ids=str)
+def test_append_with_axes_refuses(bad):
+    assert call_axes(**bad) == L.ERR_INVALID
+    assert "fa_rope_append_axes" in L.last_error()
+
+
+def test_a_rope_of_several_axes_needs_their_positions():
+    r = paged.Rope(64, axes=[16, 16])
+    assert L.lib().fa_rope_append(r._h, C.addressof(pages()), 0, 1, P, 512, P * 2, 256, P * 3, 256, 3, 8, P, P, None, P * 4, 512, None,
+                                  None) == L.ERR_INVALID
+    assert call_axes(n=0, q=None, pos=None, seq=None, slot=None) == L.OK
