@@ -451,6 +451,57 @@ int fa_pages_compact(const fa_pages *pages, const uint32_t *seq, const uint32_t 
   return launched(who, launch_page_compact(p, (cudaStream_t)stream));
 }
 
+// ------------------------------------------------------------ the plan of a step
+int fa_step_plan(const fa_page_pool *pool, const uint32_t *seq, const uint32_t *keep, const uint32_t *add, uint32_t n, uint32_t n_rows,
+                 const uint32_t *len, uint32_t *len_out, const uint32_t *n_free, uint32_t *n_free_out, uint32_t *q_start, uint32_t *kv_len,
+                 uint32_t *last, uint32_t *pos, uint32_t *row_seq, uint32_t *slot, uint32_t *err, void *stream) {
+  const char *who = "fa_step_plan";
+  if (!pool) return invalid(who, "null argument pool");
+  if (!pool->page_table || (!pool->free_pages && pool->free_cap)) return invalid(who, "null argument pool.page_table or pool.free_pages");
+  if (!pool->n_seq || !pool->max_pages) return invalid(who, "empty page table");
+  if (pool->max_pages > (1u << 21)) return invalid(who, "more than 2^21 pages a sequence");
+  if (pool->n_pages > 0x0FFFFFFFu && slot) return invalid(who, "slots of more than 2^28 - 1 pages");
+  if (n > kPlanMaxRequests) return fail(FA_ERR_UNSUPPORTED, std::string(who) + ": more than 4096 requests");
+  if (seq && pool->n_seq > kPlanMaxSeqs) return fail(FA_ERR_UNSUPPORTED, std::string(who) + ": more than 2^18 sequences");
+  if (!seq && n > pool->n_seq) return invalid(who, "more requests than sequences");
+  if (n_rows > 0x7FFFFFFFu) return invalid(who, "2^31 or more rows");
+  if (!q_start || !n_free || !n_free_out || (n && (!add || !len || !len_out || !kv_len)) || (n_rows && (!pos || !row_seq)))
+    return invalid(who, "null argument");
+  TRY(words(who, {pool->page_table, pool->free_pages, seq, keep, add, len, len_out, n_free, n_free_out, q_start, kv_len, last, pos, row_seq, slot, err}));
+  OnDevice dev(who);
+  TRY(dev.add("pool.page_table", pool->page_table));
+  if (pool->free_cap) TRY(dev.add("pool.free_pages", pool->free_pages));
+  TRY(dev.add("n_free", n_free));
+  TRY(dev.add("n_free_out", n_free_out));
+  TRY(dev.add("q_start", q_start));
+  if (n) {
+    TRY(dev.add("add", add));
+    TRY(dev.add("len", len));
+    TRY(dev.add("len_out", len_out));
+    TRY(dev.add("kv_len", kv_len));
+    if (seq) TRY(dev.add("seq", seq));
+    if (keep) TRY(dev.add("keep", keep));
+    if (last) TRY(dev.add("last", last));
+  }
+  if (n_rows) {
+    TRY(dev.add("pos", pos));
+    TRY(dev.add("row_seq", row_seq));
+    if (slot) TRY(dev.add("slot", slot));
+  }
+  if (err) TRY(dev.add("err", err));
+  TRY(dev.enter());
+  StepPlanParams p{};
+  p.table = pool->page_table, p.free_pages = pool->free_pages;
+  p.n_seq = pool->n_seq, p.max_pages = pool->max_pages, p.n_pages = pool->n_pages, p.free_cap = pool->free_cap;
+  p.seq = seq, p.keep = keep, p.add = add, p.len = len, p.n_free = n_free;
+  p.n = n, p.n_rows = n_rows;
+  p.len_out = len_out, p.n_free_out = n_free_out;
+  p.q_start = q_start, p.kv_len = kv_len, p.last = last;
+  p.pos = pos, p.row_seq = row_seq, p.slot = slot;
+  p.err = err;
+  return launched(who, launch_step_plan(p, (cudaStream_t)stream));
+}
+
 // ------------------------------------------------------------ beam search
 size_t fa_beam_select_ws(uint32_t n_batch, uint32_t n_beams, uint32_t vocab, uint32_t k) {
   if (!n_batch || !n_beams || !vocab || !k || n_beams > kBeamMaxBeams || k > kBeamMaxK || n_batch > (1u << 20) || vocab > (1u << 30)) return 0;

@@ -83,6 +83,18 @@ struct PageCompactParams {
 };
 int launch_page_compact(const PageCompactParams &p, cudaStream_t st);
 
+// ---- the plan of a step ----
+constexpr uint32_t kPlanMaxRequests = 4096, kPlanMaxSeqs = 1u << 18, kPlanMaxSmem = 200 * 1024;
+struct StepPlanParams {
+  uint32_t *table, *free_pages;
+  uint32_t n_seq, max_pages, n_pages, free_cap;
+  const uint32_t *seq, *keep, *add, *len, *n_free;
+  uint32_t n, n_rows;
+  uint32_t *len_out, *n_free_out, *q_start, *kv_len, *last, *pos, *row_seq, *slot;
+  uint32_t *err;
+};
+int launch_step_plan(const StepPlanParams &p, cudaStream_t st);
+
 // ---- beam search selection ----
 constexpr uint32_t kBeamMaxK = 64, kBeamMaxBeams = 64, kBeamMaxSplits = 32;
 struct BeamParams {

@@ -16,7 +16,7 @@ ERR_INVALID, ERR_GGUF, ERR_UNSUPPORTED, ERR_OOM, ERR_CUDA, ERR_NCCL, ERR_CONTEXT
 
 F32, F16, Q4_0, Q4_1, Q5_0, Q8_0, Q4_K, Q6_K = 0, 1, 2, 3, 6, 8, 12, 14
 KV_F32, KV_F16, KV_BF16 = 0, 1, 2
-FLAG_PAGE, FLAG_RANGE, FLAG_TIMEOUT = 16, 32, 64
+FLAG_PAGE, FLAG_RANGE, FLAG_TIMEOUT, FLAG_FULL = 16, 32, 64, 128
 ROPE_INTERLEAVED, ROPE_HALF = 0, 1
 ROPE_PLAIN, ROPE_LINEAR, ROPE_NTK, ROPE_LLAMA3, ROPE_YARN = 0, 1, 2, 3, 4
 AXES_BLOCKS, AXES_TURNS, AXES_SHARED, AXES_OWN = 0, 1, 0, 1
@@ -78,6 +78,11 @@ class fa_rope_config(C.Structure):
 
 class fa_rope_axes(C.Structure):
     _fields_ = [("n_axes", C.c_uint32), ("pairs", C.c_uint32 * 4), ("order", C.c_int32), ("freqs", C.c_int32)]
+
+
+class fa_page_pool(C.Structure):
+    _fields_ = [("page_table", C.c_void_p), ("n_seq", C.c_uint32), ("max_pages", C.c_uint32), ("n_pages", C.c_uint32),
+                ("free_pages", C.c_void_p), ("free_cap", C.c_uint32)]
 
 
 class fa_beam_config(C.Structure):
@@ -179,6 +184,7 @@ SIGNATURES = {
                               _sz, _vp, _vp], _i),
     "fa_pages_copy": ([_vp, _vp, _vp, _vp, _u32, _vp, _vp], _i),
     "fa_pages_compact": ([_vp, _vp, _vp, _vp, _u32, _u32, _vp, _vp], _i),
+    "fa_step_plan": ([_vp, _vp, _vp, _vp, _u32, _u32] + [_vp] * 12, _i),
     "fa_beam_select": ([_vp, C.c_int32, _u64, _u32, _u32, _u32, _vp, _vp, _u32, _u32, _u32, _vp, _vp, _vp, _vp, _vp,
                         _sz, _vp], _i),
     "fa_generate_beams": ([_vp, C.POINTER(fa_beam_config), _pu32, _u32, _pu32, _pu32, _pf], _i),

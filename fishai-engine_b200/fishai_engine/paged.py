@@ -1,6 +1,6 @@
 """paged — operators on paged K/V in device memory: rotary positions with the
 append of new keys and values, attention of chunks of new tokens, page copies
-(forks) and compaction.  Beside tensor.scaled_dot_product_attention_device
+(forks) and compaction, and the plan of a step.  Beside tensor.scaled_dot_product_attention_device
 (one contiguous cache) and KVCache (whose pages they also work on).
 
 Buffers are framework tensors on the GPU (objects with data_ptr(), dtype, shape
@@ -17,7 +17,7 @@ from . import _lib as L
 
 PAGE = 16  # positions of a page
 NO_TOKEN = -1  # in int32 `seqs` of rope_append: the row is left out
-FLAG_PAGE, FLAG_RANGE, FLAG_TIMEOUT = L.FLAG_PAGE, L.FLAG_RANGE, L.FLAG_TIMEOUT
+FLAG_PAGE, FLAG_RANGE, FLAG_TIMEOUT, FLAG_FULL = L.FLAG_PAGE, L.FLAG_RANGE, L.FLAG_TIMEOUT, L.FLAG_FULL
 
 _DTYPES = {}  # torch dtype -> FA_KV_*
 _INTS = set()  # the 32-bit index types
@@ -282,3 +282,35 @@ def compact(kv: PagedKV, seqs, keep, keep_start, err=None, stream: int = 0):
     L.check(L.lib().fa_pages_compact(kv._ref, _index(seqs, "seqs", n), _index(keep, "keep", keep.shape[0]),
                                      _index(keep_start, "keep_start", n + 1), n, keep.shape[0],
                                      None if err is None else _index(err, "err", 1), stream))
+
+
+def plan_step(kv: PagedKV, add, lengths, free_pages, n_free, q_start, kv_len, positions, row_seqs, seqs=None, keep=None,
+              lengths_out=None, n_free_out=None, slots=None, last=None, err=None, stream: int = 0):
+    """The plan of a step: request i cuts sequence seqs[i] (default i) to its
+    first keep[i] positions (default: all of lengths[seq]) and grows it by add[i]
+    tokens; pages go to and come from the stack free_pages, whose height is
+    n_free[0].  Writes kv's page table, lengths_out and n_free_out (default: in
+    place), and what the step's calls take: q_start [n + 1], kv_len [n], last [n],
+    the last row of each request, and for each of positions.shape[0] rows the
+    position, the sequence (NO_TOKEN behind the last) and slots, the place in the
+    pages counted in positions.  What is taken, refused and flagged: fa_step_plan."""
+    table = getattr(kv, "page_table", None)
+    if table is None:
+        raise ValueError("kv: pages of the caller's own; those of a KVCache are the cache's to give")
+    n, rows = add.shape[0], positions.shape[0]
+    if free_pages.dim() != 1:
+        raise ValueError("free_pages: a 1-d int32 tensor is needed")
+    cap = free_pages.shape[0]
+    ln = _index(lengths, "lengths", kv.n_seq)
+    nf = _index(n_free, "n_free", 1)
+    pool = L.fa_page_pool(kv._c.page_table, kv.n_seq, kv.max_pages, kv.n_pages, _index(free_pages, "free_pages", cap), cap)
+    rc = L.lib().fa_step_plan(C.addressof(pool), None if seqs is None else _index(seqs, "seqs", n),
+                              None if keep is None else _index(keep, "keep", n), _index(add, "add", n), n, rows, ln,
+                              ln if lengths_out is None else _index(lengths_out, "lengths_out", kv.n_seq), nf,
+                              nf if n_free_out is None else _index(n_free_out, "n_free_out", 1),
+                              _index(q_start, "q_start", n + 1), _index(kv_len, "kv_len", n),
+                              None if last is None else _index(last, "last", n), _index(positions, "positions", rows),
+                              _index(row_seqs, "row_seqs", rows), None if slots is None else _index(slots, "slots", rows),
+                              None if err is None else _index(err, "err", 1), stream)
+    if rc:
+        L.check(rc)

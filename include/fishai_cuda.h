@@ -443,6 +443,49 @@ int fa_pages_copy(const fa_pages *pages, const uint32_t *src, const uint32_t *ds
 int fa_pages_compact(const fa_pages *pages, const uint32_t *seq, const uint32_t *keep, const uint32_t *keep_start,
                      uint32_t n, uint32_t n_keep, uint32_t *err, void *stream);
 
+/* The plan of a step of a caller that keeps its page tables in device memory:
+ * sequences are cut and grown, their pages come from and go to a stack of free
+ * ones, and the arrays that fa_rope_append and fa_attn_chunks take are written.
+ * Request i < n: sequence seq[i] (seq NULL: i) keeps its first keep[i] of len[seq]
+ * positions (keep NULL: all) and grows by add[i] tokens.  A decode step adds one,
+ * a chunk of a prompt many, refused drafts are cut off by keep, an ended sequence
+ * has keep = add = 0.
+ *  - A request is taken if the tokens of all requests up to it are at most n_rows
+ *    and the pages that they need more than they have are at most the free ones and
+ *    those that the call's shrinking sequences give back.  From the first request
+ *    that is not taken because of this on (FA_FLAG_FULL, where its add > 0), none is:
+ *    those are cut to keep and do not grow.
+ *  - q_start [n + 1], kv_len [n]: rows and length of each request (0 rows where it
+ *    was not taken); last [n] (may be NULL): its last row, FA_NO_TOKEN where it has
+ *    none.  Rows r < n_rows: pos[r] the position in the cache, row_seq[r] the
+ *    sequence, slot[r] (slot may be NULL) page * 16 + position in the page; behind
+ *    the last request's 0, FA_NO_TOKEN and FA_NO_TOKEN.
+ *  - len_out[seq] = kv_len, for the sequences that are named; may be len.  *n_free
+ *    of free_pages are free, the last of them the next one taken; *n_free_out (may be
+ *    n_free) is their number after the call.  Pages that come back are put on the
+ *    stack first, by request and in ascending order; then each request takes the
+ *    pages it needs, in that order.  Table entries behind a sequence's end are left
+ *    as they were.
+ *  - A sequence out of range or named twice (all times), a length beyond the table,
+ *    keep above the length and a length beyond the table with add set FA_FLAG_RANGE:
+ *    the request is left out, its sequence as it was, kv_len 0.  So does a stack that
+ *    is or would grow longer than free_cap, and then nothing is taken or cut.  A page
+ *    number >= n_pages that is moved sets FA_FLAG_PAGE and is passed on.
+ *  - A partly filled last page that another sequence shares has to be copied before
+ *    (fa_pages_copy): rows go into it.
+ * n <= 4096, n_seq <= 2^18 where seq is given.  No array may overlap another but
+ * as said.  Device, stream and capture rules as for the others. */
+#define FA_FLAG_FULL 128  /* *err: rows or pages ran out, a request was left out */
+typedef struct {
+  uint32_t *page_table;  /* device [n_seq][max_pages] */
+  uint32_t n_seq, max_pages, n_pages;
+  uint32_t *free_pages;  /* device [free_cap] (NULL: free_cap 0) */
+  uint32_t free_cap;     /* room for every page that may be free at once */
+} fa_page_pool;
+int fa_step_plan(const fa_page_pool *pool, const uint32_t *seq, const uint32_t *keep, const uint32_t *add, uint32_t n, uint32_t n_rows,
+                 const uint32_t *len, uint32_t *len_out, const uint32_t *n_free, uint32_t *n_free_out, uint32_t *q_start, uint32_t *kv_len,
+                 uint32_t *last, uint32_t *pos, uint32_t *row_seq, uint32_t *slot, uint32_t *err, void *stream);
+
 /* ---- pages of a cache shared between its sequences ---- */
 /* Sequence dst becomes a copy of sequence src: whole pages are shared, the
  * last one is copied if it is partly filled.  src == dst does nothing. */

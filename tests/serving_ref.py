@@ -64,3 +64,58 @@ def attention(pages, table, q, q_start, kv_len, heads, scale, window, sinks):
         if q.dtype == torch.float16:
             tol[a:b] += 2.0 ** -25  # the smallest step of f16
     return out, tol
+
+
+def plan(seqs, keep, add, rows, lens, table, free, n_free, n_pages):
+    """The plan of a step, one request after another, on lists; returns (q_start, kv_len, last, pos, row_seq, slot, table, free,
+    lens, n_free, flags)."""
+    FULL, RANGE, PAGE_ = 128, 32, 16
+    up = lambda x: -(-x // PAGE)  # noqa: E731
+    table, free, lens, flags = [list(t) for t in table], list(free), list(lens), 0
+    n, most, cap = len(add), len(table[0]) * PAGE, len(free)
+    seqs = list(range(n)) if seqs is None else seqs
+    ok = []
+    for q, a, i in zip(seqs, add, range(n)):
+        fine = 0 <= q < len(lens) and seqs.count(q) == 1 and 0 <= lens[q] <= most
+        k = (lens[q] if 0 <= q < len(lens) else 0) if keep is None else keep[i]
+        fine = fine and 0 <= k <= lens[q] and 0 <= a and k + a <= most
+        ok.append((fine, k))
+        flags |= 0 if fine else RANGE
+    room = n_free + sum(max(0, up(lens[q]) - up(k + a)) for q, a, (f, k) in zip(seqs, add, ok) if f)
+    left, now, takes, put = rows, [], [], 0
+    for q, a, (f, k) in zip(seqs, add, ok):
+        if f:
+            left -= a
+            room -= max(0, up(k + a) - up(lens[q]))
+        takes.append(f and left >= 0 and room >= 0)
+        flags |= FULL if f and a and not takes[-1] else 0
+        now.append(k + a if takes[-1] else k)
+        put += max(0, up(lens[q]) - up(now[-1])) if f else 0
+    bad = n_free > cap or n_free + put > cap
+    if bad:
+        flags |= RANGE
+        ok, takes = [(False, 0)] * n, [False] * n
+    high = n_free
+    for q, m, (f, _) in zip(seqs, now, ok):
+        for e in range(up(m), up(lens[q])) if f else ():
+            free[high] = table[q][e]
+            flags |= PAGE_ if not 0 <= table[q][e] < n_pages else 0
+            high += 1
+    for q, m, (f, _) in zip(seqs, now, ok):
+        for e in range(up(lens[q]), up(m)) if f else ():
+            high -= 1
+            table[q][e] = free[high]
+            flags |= PAGE_ if not 0 <= free[high] < n_pages else 0
+    start, kv, last, pos, who, slot = [0], [], [], [], [], []
+    for q, m, a, (f, k), t in zip(seqs, now, add, ok, takes):
+        kv.append(m if f else 0)
+        start.append(start[-1] + (a if t else 0))
+        last.append(start[-1] - 1 if t and a else -1)
+        for x in range(k, m) if t else ():
+            pos.append(x)
+            who.append(q)
+            slot.append(table[q][x // PAGE] * PAGE + x % PAGE)
+        if f:
+            lens[q] = m
+    pad = rows - len(pos)
+    return start, kv, last, pos + [0] * pad, who + [-1] * pad, slot + [-1] * pad, table, free, lens, n_free if bad else high, flags

@@ -105,3 +105,22 @@ def test_a_rope_of_several_axes_needs_their_positions():
     assert L.lib().fa_rope_append(r._h, C.addressof(pages()), 0, 1, P, 512, P * 2, 256, P * 3, 256, 3, 8, P, P, None, P * 4, 512, None,
                                   None) == L.ERR_INVALID
     assert call_axes(n=0, q=None, pos=None, seq=None, slot=None) == L.OK
+
+
+# ------------------------------------------------------------------ the plan of a step
+def call_plan(pool=None, seq=P, keep=P, add=P, n=3, rows=9, ln=P, ln_out=P, nf=P, nf_out=P, q_start=P, kv=P, last=P, pos=P, row_seq=P, slot=P,
+              **fields):
+    f = dict(page_table=0x20000, n_seq=4, max_pages=8, n_pages=100, free_pages=0x40000, free_cap=100)
+    f.update(fields)
+    made = L.fa_page_pool(**f)
+    return L.lib().fa_step_plan(C.addressof(made) if pool is None else pool, seq, keep, add, n, rows, ln, ln_out, nf, nf_out, q_start, kv, last, pos, row_seq, slot, None, None)
+
+
+@pytest.mark.parametrize("bad", [dict(pool=0), dict(page_table=None), dict(free_pages=None), dict(n_seq=0), dict(max_pages=0),
+                                 dict(max_pages=(1 << 21) + 1), dict(n_pages=1 << 28), dict(n=4097), dict(n_seq=(1 << 18) + 1),
+                                 dict(seq=None, n=5), dict(rows=1 << 31), dict(add=None), dict(ln=None), dict(ln_out=None), dict(nf=None),
+                                 dict(nf_out=None), dict(q_start=None), dict(kv=None), dict(pos=None), dict(row_seq=None), dict(add=P + 1),
+                                 dict(slot=P + 2), dict(page_table=0x20001)], ids=str)
+def test_plan_refuses(bad):
+    assert call_plan(**bad) in (L.ERR_INVALID, L.ERR_UNSUPPORTED)
+    assert "fa_step_plan" in L.last_error()
