@@ -502,6 +502,47 @@ int fa_step_plan(const fa_page_pool *pool, const uint32_t *seq, const uint32_t *
   return launched(who, launch_step_plan(p, (cudaStream_t)stream));
 }
 
+// ------------------------------------------------------------ sampling
+int fa_sample_logits(const void *logits, int32_t dtype, uint64_t ld, uint32_t n_logits, uint32_t vocab, const uint32_t *rows, uint32_t n,
+                     const float *temperature, const uint32_t *top_k, const float *top_p, const float *min_p, const float *u, uint32_t *ids,
+                     float *logprobs, uint32_t *err, void *stream) {
+  const char *who = "fa_sample_logits";
+  if (!known(dtype)) return invalid(who, "unknown element type of the logits");
+  if (!vocab) return invalid(who, "empty vocabulary");
+  if (vocab > kSampleMaxVocab) return fail(FA_ERR_UNSUPPORTED, std::string(who) + ": vocabulary above " + std::to_string(kSampleMaxVocab));
+  if (n > (1u << 20)) return invalid(who, "more than 2^20 rows");
+  if (ld < vocab && n_logits > 1) return invalid(who, "a row stride is smaller than the row");
+  if (!rows && n > n_logits) return invalid(who, "more samples than rows of logits");
+  if (!n) return FA_OK;
+  if (!n_logits || !logits || !u || !ids) return invalid(who, "null argument");
+  if (reinterpret_cast<uintptr_t>(logits) % elem_size(dtype)) return invalid(who, "logits are not aligned to their element type");
+  TRY(words(who, {rows, temperature, top_k, top_p, min_p, u, ids, logprobs, err}));
+  OnDevice dev(who);
+  TRY(dev.add("logits", logits));
+  if (rows) TRY(dev.add("rows", rows));
+  if (temperature) TRY(dev.add("temperature", temperature));
+  if (top_k) TRY(dev.add("top_k", top_k));
+  if (top_p) TRY(dev.add("top_p", top_p));
+  if (min_p) TRY(dev.add("min_p", min_p));
+  TRY(dev.add("u", u));
+  TRY(dev.add("ids", ids));
+  if (logprobs) TRY(dev.add("logprobs", logprobs));
+  if (err) TRY(dev.add("err", err));
+  TRY(dev.enter());
+  SampleParams p{};
+  p.logits = logits;
+  p.dtype = dtype;
+  p.ld = ld;
+  p.n_logits = n_logits, p.n = n, p.vocab = vocab;
+  p.rows = rows, p.top_k = top_k;
+  p.temperature = temperature, p.top_p = top_p, p.min_p = min_p, p.u = u;
+  p.ids = ids;
+  p.logprobs = logprobs;
+  p.err = err;
+  p.aligned = reinterpret_cast<uintptr_t>(logits) % 16 == 0 && (ld * elem_size(dtype) % 16 == 0 || n_logits == 1);
+  return launched(who, launch_sample_logits(p, (cudaStream_t)stream));
+}
+
 // ------------------------------------------------------------ beam search
 size_t fa_beam_select_ws(uint32_t n_batch, uint32_t n_beams, uint32_t vocab, uint32_t k) {
   if (!n_batch || !n_beams || !vocab || !k || n_beams > kBeamMaxBeams || k > kBeamMaxK || n_batch > (1u << 20) || vocab > (1u << 30)) return 0;

@@ -95,6 +95,23 @@ struct StepPlanParams {
 };
 int launch_step_plan(const StepPlanParams &p, cudaStream_t st);
 
+// ---- sampling from given numbers ----
+constexpr uint32_t kSampleMaxVocab = 8 * 512 * 105, kSampleMaxSmem = 1024 * 8 + 105 * 512 * 4;
+struct SampleParams {
+  const void *logits;
+  int dtype;
+  uint64_t ld;
+  uint32_t n_logits, n, vocab;
+  const uint32_t *rows, *top_k;
+  const float *temperature, *top_p, *min_p, *u;
+  uint32_t *ids;
+  float *logprobs;
+  uint32_t *err;
+  uint32_t aligned;                  // rows start on 16 bytes
+  uint32_t ctas, each;               // CTAs of a row's cluster, elements of a thread
+};
+int launch_sample_logits(const SampleParams &p, cudaStream_t st);
+
 // ---- beam search selection ----
 constexpr uint32_t kBeamMaxK = 64, kBeamMaxBeams = 64, kBeamMaxSplits = 32;
 struct BeamParams {

@@ -185,6 +185,7 @@ SIGNATURES = {
     "fa_pages_copy": ([_vp, _vp, _vp, _vp, _u32, _vp, _vp], _i),
     "fa_pages_compact": ([_vp, _vp, _vp, _vp, _u32, _u32, _vp, _vp], _i),
     "fa_step_plan": ([_vp, _vp, _vp, _vp, _u32, _u32] + [_vp] * 12, _i),
+    "fa_sample_logits": ([_vp, C.c_int32, _u64, _u32, _u32, _vp, _u32] + [_vp] * 9, _i),
     "fa_beam_select": ([_vp, C.c_int32, _u64, _u32, _u32, _u32, _vp, _vp, _u32, _u32, _u32, _vp, _vp, _vp, _vp, _vp,
                         _sz, _vp], _i),
     "fa_generate_beams": ([_vp, C.POINTER(fa_beam_config), _pu32, _u32, _pu32, _pu32, _pf], _i),

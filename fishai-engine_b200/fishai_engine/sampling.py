@@ -1,4 +1,5 @@
-"""Sampler — src/sampling.rs:14-310 on the device (Philox4x32-10 uniforms)."""
+"""Sampler — src/sampling.rs:14-310 on the device (Philox4x32-10 uniforms) —
+and sample_logits, which draws from a caller's device logits and numbers."""
 from __future__ import annotations
 
 import ctypes as C
@@ -7,6 +8,7 @@ from dataclasses import dataclass
 import numpy as np
 
 from . import _lib as L
+from .paged import _DTYPES, _code, _index
 
 
 @dataclass
@@ -75,3 +77,35 @@ class Sampler:
         c = C.c_uint32()
         L.check(L.lib().fa_sampler_freq(self._h, 0, token_id, C.byref(c)))
         return c.value
+
+
+def _floats(t, name, n):
+    """address of a contiguous array of n float32"""
+    if t.shape != (n,) or _DTYPES.get(t.dtype) != L.KV_F32 or (n > 1 and t.stride() != (1,)):
+        raise ValueError(f"{name}: a contiguous float32 [{n}] tensor is needed")
+    return t.data_ptr()
+
+
+def sample_logits(logits, u, ids, temperature=None, top_k=None, top_p=None, min_p=None, rows=None, logprobs=None, err=None,
+                  stream: int = 0):
+    """Draws ids[i] from row rows[i] (default i; NO_TOKEN: none) of device logits
+    [rows, vocab] (float32, float16 or bfloat16, any row stride) with the random
+    number u[i] in [0, 1) and the row's own temperature (0: greedy), top_k (0: off),
+    top_p and min_p, and logprobs[i], its log-probability among what is kept.
+    Framework tensors on the GPU: float32 but ids, rows, top_k (int32) and err (one
+    int32, FLAG_* bits).  What is kept and drawn: fa_sample_logits."""
+    dt = _code(logits, "logits")
+    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise ValueError("logits: [rows, vocab] with consecutive elements")
+    m, vocab = logits.shape
+    n = ids.shape[0]
+    if m >> 32 or vocab >> 32 or n >> 32:
+        L.u32(rows=m, vocab=vocab, ids=n)
+    rc = L.lib().fa_sample_logits(
+        logits.data_ptr(), dt, logits.stride(0) if m > 1 else vocab, m, vocab, None if rows is None else _index(rows, "rows", n), n,
+        None if temperature is None else _floats(temperature, "temperature", n), None if top_k is None else _index(top_k, "top_k", n),
+        None if top_p is None else _floats(top_p, "top_p", n), None if min_p is None else _floats(min_p, "min_p", n), _floats(u, "u", n),
+        _index(ids, "ids", n), None if logprobs is None else _floats(logprobs, "logprobs", n),
+        None if err is None else _index(err, "err", 1), stream)
+    if rc:
+        L.check(rc)

@@ -567,6 +567,33 @@ int fa_sampler_reset(fa_sampler *s, int32_t seq);  /* seq < 0: every sequence */
 /* token_freq[token] of sequence seq (0 for ids never observed) */
 int fa_sampler_freq(fa_sampler *s, uint32_t seq, uint32_t token, uint32_t *count);
 
+/* Sampling from given random numbers, each row with settings of its own (no
+ * counterpart in the reference, whose sampler draws its own numbers, has one setting
+ * and a fixed nucleus, src/sampling.rs:110-152).  Sample i < n takes row rows[i] of
+ * logits (rows NULL: i; FA_NO_TOKEN: none, ids[i] is left as it was), type FA_KV_*,
+ * rows ld elements apart, and draws with u[i], 0 <= u < 1:
+ *   w_v = exp((x_v - max x) / temperature[i]), below 2^-64 none;
+ *   the tokens in the order of x, equal ones (-0.0 and +0.0 among them) by id;
+ *   the first top_k[i] of them (0: all);
+ *   of those the shortest beginning whose sum of w is at least top_p[i] of theirs
+ *   (1 and above: all; the first one always);
+ *   of those the ones with w >= min_p[i];
+ *   ids[i]: the lowest id at which the sum of w over the ids up to it exceeds
+ *   u[i] times the sum of all; logprobs[i] (may be NULL): log(w / that sum).
+ * temperature 0: the lowest id of the maximum, with log-probability 0, whatever the
+ * cuts.  temperature, top_k, top_p and min_p may be NULL: 1, 0, 1, 0.  Logits of
+ * -inf and NaN are no candidates, +inf counts as the largest f32.  Weights and sums
+ * have 64 bits (off by some 10^-14), so u that near to a border between two tokens, or
+ * a top_p that near to one between two beginnings, may fall on either side.
+ * Refused, with FA_FLAG_RANGE: a row >= n_logits, a temperature that is not 0 or 1e-6
+ * to 1e6, u outside [0, 1), top_p < 0, min_p outside [0, 1], NaN; ids[i] is left as it
+ * was.  A row without candidates gives FA_NO_TOKEN, -inf and FA_FLAG_RANGE.
+ * vocab <= 430080, n <= 2^20.  Device, stream, capture and err as for the operators
+ * on pages; no workspace. */
+int fa_sample_logits(const void *logits, int32_t dtype, uint64_t ld, uint32_t n_logits, uint32_t vocab, const uint32_t *rows, uint32_t n,
+                     const float *temperature, const uint32_t *top_k, const float *top_p, const float *min_p, const float *u, uint32_t *ids,
+                     float *logprobs, uint32_t *err, void *stream);
+
 /* --------------------------------------------------------- beam search */
 /* One selection step over n_batch requests of n_beams beams (no counterpart
  * in the reference; beside Sampler::sample).  Row b * n_beams + j of logits

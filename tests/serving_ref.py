@@ -119,3 +119,33 @@ def plan(seqs, keep, add, rows, lens, table, free, n_free, n_pages):
             lens[q] = m
     pad = rows - len(pos)
     return start, kv, last, pos + [0] * pad, who + [-1] * pad, slot + [-1] * pad, table, free, lens, n_free if bad else high, flags
+
+
+def sample(x, u, t=1.0, k=0, p=1.0, mp=0.0):
+    """One row in 64 bits: (ids that may be drawn, {id: log-probability}).  More than one id only where u is within 1e-11
+    of a border between two."""
+    x = torch.where(x.isnan(), -math.inf, x.double()).clamp_max(torch.finfo(torch.float32).max) + 0.0
+    top = x.max()
+    if float(top) == -math.inf:
+        return [-1], {-1: -math.inf}
+    if t == 0:
+        best = int((x == top).nonzero()[0])
+        return [best], {best: 0.0}
+    z = (top - x) / t
+    w = torch.where(z > 64 * math.log(2), 0.0, torch.exp(-z))
+    order = torch.sort(x, descending=True, stable=True).indices
+    ws = w[order]
+    n = int((ws > 0).sum())
+    if k:
+        n = min(n, k)
+    sums = ws[:n].cumsum(0)
+    if p < 1:
+        n = max(1, int((sums - ws[:n] < p * sums[-1]).sum()))
+    kept = order[:n]
+    kept = kept[w[kept] >= mp].sort().values
+    sums = w[kept].cumsum(0)
+    at = u * float(sums[-1])
+    slack = 1e-11 * float(sums[-1])
+    lo, hi = int((sums <= at - slack).sum()), int((sums <= at + slack).sum())
+    ids = kept[lo: min(hi, len(kept) - 1) + 1].tolist()
+    return ids, {i: float((w[i] / sums[-1]).log()) for i in ids}
