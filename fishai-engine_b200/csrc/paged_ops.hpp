@@ -96,7 +96,7 @@ struct StepPlanParams {
 int launch_step_plan(const StepPlanParams &p, cudaStream_t st);
 
 // ---- sampling from given numbers ----
-constexpr uint32_t kSampleMaxVocab = 8 * 512 * 105, kSampleMaxSmem = 1024 * 8 + 105 * 512 * 4;
+constexpr uint32_t kSampleMaxVocab = 8 * 2048 * 25, kSampleMaxSmem = 224 * 1024;
 struct SampleParams {
   const void *logits;
   int dtype;
@@ -108,7 +108,7 @@ struct SampleParams {
   float *logprobs;
   uint32_t *err;
   uint32_t aligned;                  // rows start on 16 bytes
-  uint32_t ctas, each;               // CTAs of a row's cluster, elements of a thread
+  uint32_t ctas, groups;             // CTAs of a row's cluster, groups of four elements a thread
 };
 int launch_sample_logits(const SampleParams &p, cudaStream_t st);
 
