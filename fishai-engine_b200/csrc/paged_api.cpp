@@ -540,7 +540,7 @@ int fa_sample_logits(const void *logits, int32_t dtype, uint64_t ld, uint32_t n_
   p.logprobs = logprobs;
   p.err = err;
   p.aligned = reinterpret_cast<uintptr_t>(logits) % 16 == 0 && (ld * elem_size(dtype) % 16 == 0 || n_logits == 1);
-  return launched(who, launch_sample_logits(p, (cudaStream_t)stream));
+  return launched(who, launch_sample_logits(p, (uint32_t)dev.sms(), (cudaStream_t)stream));
 }
 
 // ------------------------------------------------------------ beam search

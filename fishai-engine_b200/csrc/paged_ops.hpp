@@ -96,7 +96,7 @@ struct StepPlanParams {
 int launch_step_plan(const StepPlanParams &p, cudaStream_t st);
 
 // ---- sampling from given numbers ----
-constexpr uint32_t kSampleMaxVocab = 8 * 2048 * 25, kSampleMaxSmem = 224 * 1024;
+constexpr uint32_t kSampleMaxVocab = 8 * 2048 * 22, kSampleMaxSmem = 224 * 1024;
 struct SampleParams {
   const void *logits;
   int dtype;
@@ -108,9 +108,9 @@ struct SampleParams {
   float *logprobs;
   uint32_t *err;
   uint32_t aligned;                  // rows start on 16 bytes
-  uint32_t ctas, groups;             // CTAs of a row's cluster, groups of four elements a thread
+  uint32_t ctas, groups, slice;      // CTAs of a row's cluster, groups of four elements a thread, elements of a CTA
 };
-int launch_sample_logits(const SampleParams &p, cudaStream_t st);
+int launch_sample_logits(const SampleParams &p, uint32_t n_sm, cudaStream_t st);
 
 // ---- beam search selection ----
 constexpr uint32_t kBeamMaxK = 64, kBeamMaxBeams = 64, kBeamMaxSplits = 32;

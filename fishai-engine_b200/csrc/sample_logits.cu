@@ -6,19 +6,17 @@
 //   the token: the first by id at which the mass of the kept ones exceeds u times all of it.
 // Every cut keeps a beginning of the same order, so a row's cuts are one place in it.
 //
-// Each row is read once: a cluster of up to eight CTAs holds it in shared memory (in
-// f32) and exchanges sums over distributed shared memory.  A thread owns consecutive
-// ids, an odd number of them, so that the lanes' reads fall on distinct banks and a
-// prefix sum over threads is one over ids.  Masses are 64-bit sums of 64-bit
-// exponentials in a fixed order: which token is drawn from a flat row of 10^5 tokens
-// depends on 17 bits more than f32 has.
+// Each row is read once: a cluster of up to eight CTAs holds it in shared memory and
+// exchanges sums over distributed shared memory.  Masses are 64-bit sums of
+// 64-bit exponentials in a fixed order: which token is drawn from a flat row of 10^5
+// tokens depends on 17 bits more than f32 has.
 //
-// A cut's place is found without sorting the row: a histogram over z in 1/16 octave
-// (of counts, or of masses to 2^-15, which bracket the place), then the few elements of the
-// bins around it, which CTA 0 sorts.  Where few elements in all are above the place (top-k
-// and top-p as they mostly are), they are all in that list and the rest happens there; where
-// more are in the bracket than the list holds (flat rows, equal logits), its range of values is
-// halved until it holds them, or one value is left and the place is an id.
+// Rows are not sorted.  A small top-k: each CTA notes its elements from the k-th largest
+// of its threads' maxima on, a few more than k, and CTA 0 picks from those.  Other cuts: a histogram
+// over z (of counts, or of masses to 2^-15, which bracket the place of the cut) leads to
+// the few elements of the bins around the place, which CTA 0 sorts.  Where more are in the bracket
+// than it sorts (flat rows, equal logits), its range of values is halved until it does, or one
+// value is left and the place is an id.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -28,12 +26,15 @@
 namespace fa {
 namespace {
 
-constexpr uint32_t kThreads = 512, kWarps = kThreads / 32, kBins = 2048, kList = 1024, kMaxCtas = 8;
-constexpr float kOctaves = 64.0f, kPerOctave = kBins / kOctaves;
-constexpr double kHistError = 1.0 / 32768;  // of a sum of the histogram's masses: each is rounded to 2^-15 of its bin's largest, and exponentials are f32
-constexpr uint32_t kGroup = 4 * kThreads;   // elements of a CTA's group: four a thread, a warp's 128 in a row
+constexpr uint32_t kThreads = 512, kWarps = kThreads / 32, kMaxCtas = 8;
+constexpr uint32_t kList = 2048, kSort = 1024;  // noted elements of a CTA (and of a cluster); most that are sorted
+constexpr uint32_t kCtaBins = 1024;             // bins for each CTA of the cluster: finer for longer rows
+constexpr uint32_t kFewK = 128;                 // the top-k that goes by the threads' maxima
+constexpr float kOctaves = 64.0f;
+constexpr double kHistError = 1.0 / 32768;      // of a sum of the histogram's masses: each is rounded to 2^-15 of its bin's largest, and exponentials are f32
+constexpr uint32_t kGroup = 4 * kThreads;       // elements of a CTA's group: four a thread, a warp's 128 in a row
 
-struct Msg {  // what a CTA tells the others
+struct alignas(16) Msg {  // what a CTA tells the others
   double a, b;
   uint32_t c, d, e, f;
 };
@@ -41,51 +42,92 @@ struct Small {
   Msg msg[2][kMaxCtas];
   double red[kWarps];
   uint32_t redu[4][kWarps];
-  uint32_t bin, count;
+  uint32_t bin, count, bins[2];
   double power[32];  // 2^(i / 32)
 };
 
-__device__ __forceinline__ float to_logit(float x) { return x != x ? -INFINITY : fminf(x, 3.402823466e38f) + 0.0f; }  // -0 to +0
+// Two logits as they are kept: NaN as -inf, -0 as +0.  In f32 (to_f32) +inf is the largest number.
+__device__ __forceinline__ void clean(float &a, float &b, float &most) {
+  a = fmaxf(a, -INFINITY) + 0.0f;
+  b = fmaxf(b, -INFINITY) + 0.0f;
+  most = fmaxf(most, fmaxf(a, b));
+}
+template <typename T2>
+__device__ __forceinline__ void clean2(T2 &x, T2 zero, T2 none, T2 &most) {
+  x = __hadd2(__hmax2(x, none), zero);
+  most = __hmax2(most, x);
+}
+template <typename T>
+__device__ __forceinline__ T clean(T x) {
+  return (T)(fmaxf((float)x, -INFINITY) + 0.0f);
+}
+template <typename T>
+__device__ __forceinline__ float to_f32(T x) {
+  return fminf((float)x, 3.402823466e38f);
+}
+__device__ __forceinline__ double lanes_sum(double v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+  return v;
+}
 
 template <typename T>
-struct alignas(16) Vec {
-  T v[16 / sizeof(T)];
+struct Pair;
+template <>
+struct Pair<__half> {
+  using type = __half2;
+};
+template <>
+struct Pair<__nv_bfloat16> {
+  using type = __nv_bfloat162;
 };
 
-__device__ __forceinline__ void st_cluster(uint32_t addr, uint64_t v) {
-  asm volatile("st.shared::cluster.b64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
+__device__ __forceinline__ void st_cluster(uint32_t addr, const Msg &m) {
+  const uint64_t a = __double_as_longlong(m.a), b = __double_as_longlong(m.b), c = (uint64_t)m.d << 32 | m.c, d = (uint64_t)m.f << 32 | m.e;
+  asm volatile("st.shared::cluster.v2.b64 [%0], {%1, %2};" ::"r"(addr), "l"(a), "l"(b) : "memory");
+  asm volatile("st.shared::cluster.v2.b64 [%0], {%1, %2};" ::"r"(addr + 16), "l"(c), "l"(d) : "memory");
 }
 __device__ __forceinline__ uint64_t ld_cluster64(uint32_t addr) {
   uint64_t v;
   asm volatile("ld.shared::cluster.b64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
   return v;
 }
-__device__ __forceinline__ uint32_t ld_cluster32(uint32_t addr) {
-  uint32_t v;
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-  return v;
-}
+template <typename T>
+struct alignas(4 * sizeof(T)) Four {
+  T v[4];
+};
 
 // A cluster's work on one row.  Element e of the thread in group g is number
 // warp * 128 groups + 128 g + 4 lane + e of the CTA's part: a warp has consecutive ids.
+template <typename T>
 struct Row {
   const SampleParams &p;
   Small &s;
-  float *x;         // this CTA's part of the row; -inf behind its end
-  uint32_t *hist;   // [kBins]
-  double *binsum;   // [kBins / ctas] inclusive sums of this CTA's share of the cluster's bins
+  T *x;             // this CTA's part of the row; -inf behind its end
   uint64_t *list;   // [kList] (ordered value, ~id)
-  uint32_t tid, lane, warp, rank, ctas, groups, mine;  // mine: the thread's first element
+  uint32_t *hist;   // [bins], over the list
+  double *binsum;   // [kCtaBins] inclusive sums of this CTA's share of the cluster's bins
+  uint32_t tid, lane, warp, rank, ctas, bins, groups, mine;  // mine: the thread's first element
   uint32_t id0;     // id of the CTA's first element
   uint32_t turn = 0;
-  float mx, cf;     // the maximum, log2(e) / T
-  double mxd, c32;  // 32 log2(e) / T
-  // kept so far: value above the key, or equal and id at most cut_id
-  uint32_t cut_key = 0, cut_id = 0xFFFFFFFFu;
+  float mx, cb, last;  // the maximum; bins a unit of x; z = 64 in bins
+  double mxd, c32;     // 32 log2(e) / T
+  // kept so far: value above cut_at, or equal and id at most cut_id
+  float cut_at = -INFINITY;
+  uint32_t cut_id = 0xFFFFFFFFu;
 
   __device__ Row(const SampleParams &p, Small &s) : p(p), s(s) {}
 
-  __device__ float z(float v) const { return (mx - v) * cf; }
+  __device__ void scale(float top, float t) {
+    const double c = 1.4426950408889634074 / (double)t;
+    mx = top;
+    mxd = (double)top;
+    c32 = 32.0 * c;
+    bins = kCtaBins * ctas;
+    last = (float)bins;
+    cb = (float)c * (last / kOctaves);
+  }
+  __device__ float z(float v) const { return (mx - v) * cb; }  // in bins
   // 2^-z in 64 bits, table-driven: 2^(n / 32) from a table, 2^(f / 32), |f| <= 1/2, from the series to
   // f^5 (the next term is below 2^-48.6).  For z <= 64, so the exponent stays in range.
   __device__ double weight(float v) const {
@@ -104,10 +146,7 @@ struct Row {
   }
   template <bool CUT>
   __device__ bool kept(float v, uint32_t id) const {
-    if (!(z(v) <= kOctaves)) return false;
-    if (!CUT) return true;
-    const uint32_t k = float_key(v);
-    return k > cut_key || (k == cut_key && id <= cut_id);
+    return z(v) <= last && (!CUT || v > cut_at || (v == cut_at && id <= cut_id));
   }
   // Four values at once, without a branch: their chains of dependent operations run side by side.  Where
   // use[j] is false, 0.
@@ -118,13 +157,18 @@ struct Row {
     for (uint32_t j = 0; j < 4; ++j)
       if (!use[j]) w[j] = 0.0;
   }
+  __device__ void load(uint32_t at, float (&v)[4]) const {
+    const Four<T> f = *reinterpret_cast<const Four<T> *>(x + at);
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j) v[j] = to_f32(f.v[j]);
+  }
   // f(values, which are kept, first id) of the thread's groups of four, in the order of ids
   template <bool CUT, typename F>
   __device__ void each4(F f) const {
     for (uint32_t g = 0; g < groups; ++g) {
-      const float4 x4 = *reinterpret_cast<const float4 *>(x + mine + 128 * g);
+      float v[4];
+      load(mine + 128 * g, v);
       const uint32_t id = id0 + mine + 128 * g;
-      const float v[4] = {x4.x, x4.y, x4.z, x4.w};
       bool use[4];
 #pragma unroll
       for (uint32_t j = 0; j < 4; ++j) use[j] = kept<CUT>(v[j], id + j);
@@ -135,39 +179,34 @@ struct Row {
   template <bool CUT, typename F>
   __device__ void each(F f) const {
     for (uint32_t g = 0; g < groups; ++g) {
-      const float4 v = *reinterpret_cast<const float4 *>(x + mine + 128 * g);
+      float v[4];
+      load(mine + 128 * g, v);
       const uint32_t id = id0 + mine + 128 * g;
-      if (kept<CUT>(v.x, id)) f(v.x, id);
-      if (kept<CUT>(v.y, id + 1)) f(v.y, id + 1);
-      if (kept<CUT>(v.z, id + 2)) f(v.z, id + 2);
-      if (kept<CUT>(v.w, id + 3)) f(v.w, id + 3);
+#pragma unroll
+      for (uint32_t j = 0; j < 4; ++j)
+        if (kept<CUT>(v[j], id + j)) f(v[j], id + j);
     }
   }
 
-  // what every CTA says, from thread 0's m; valid until the call after the next
+  // what every CTA says, the same m in all its threads; valid until the call after the next
   __device__ const Msg *share(const Msg &m) {
     const uint32_t t = turn;
     turn ^= 1;
-    if (tid == 0) s.msg[t][rank] = m;
-    __syncthreads();
-    if (tid < 4 * ctas && tid / 4 != rank) {
-      const uint64_t *w = reinterpret_cast<const uint64_t *>(&s.msg[t][rank]) + tid % 4;
-      st_cluster(dsmem_addr(w, tid / 4), *w);
-    }
+    if (tid < ctas) st_cluster(dsmem_addr(&s.msg[t][rank], tid), m);
     cluster_sync();
     return s.msg[t];
   }
+  // sum of all CTAs' a, or b: in the order of a butterfly, the same everywhere
+  __device__ double all_a(const Msg *all) const { return lanes_sum(lane < ctas ? all[lane].a : 0.0); }
+  __device__ double all_b(const Msg *all) const { return lanes_sum(lane < ctas ? all[lane].b : 0.0); }
+  __device__ uint32_t all_c(const Msg *all) const { return __reduce_add_sync(0xFFFFFFFFu, lane < ctas ? all[lane].c : 0); }
   // sums over the CTA, the same for all threads
   __device__ double sum(double v) {
-#pragma unroll
-    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+    v = lanes_sum(v);
     __syncthreads();
     if (lane == 0) s.red[warp] = v;
     __syncthreads();
-    double t = 0;
-#pragma unroll
-    for (uint32_t w = 0; w < kWarps; ++w) t += s.red[w];
-    return t;
+    return lanes_sum(lane < kWarps ? s.red[lane] : 0.0);
   }
   // (sum of a, sum of b, smallest of c, largest of d)
   __device__ void sums(uint32_t &a, uint32_t &b, uint32_t &c, uint32_t &d) {
@@ -183,70 +222,49 @@ struct Row {
       s.redu[3][warp] = d;
     }
     __syncthreads();
-    a = b = d = 0;
-    c = 0xFFFFFFFFu;
-#pragma unroll
-    for (uint32_t w = 0; w < kWarps; ++w) {
-      a += s.redu[0][w];
-      b += s.redu[1][w];
-      c = min(c, s.redu[2][w]);
-      d = max(d, s.redu[3][w]);
-    }
+    const uint32_t l = lane % kWarps;
+    a = __reduce_add_sync(0xFFFFFFFFu, lane < kWarps ? s.redu[0][l] : 0);
+    b = __reduce_add_sync(0xFFFFFFFFu, lane < kWarps ? s.redu[1][l] : 0);
+    c = __reduce_min_sync(0xFFFFFFFFu, s.redu[2][l]);
+    d = __reduce_max_sync(0xFFFFFFFFu, s.redu[3][l]);
   }
-  // inclusive sum over the CTA's threads, and the total
-  __device__ double scan(double v, double &total) {
+  // inclusive sums over a warp's lanes
+  __device__ double lanes_scan(double v) const {
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const double y = __shfl_up_sync(0xFFFFFFFFu, v, o);
       if (lane >= (uint32_t)o) v += y;
     }
+    return v;
+  }
+  // inclusive sum over the CTA's threads, and the total
+  __device__ double scan(double v, double &total) {
+    v = lanes_scan(v);
     __syncthreads();
     if (lane == 31) s.red[warp] = v;
     __syncthreads();
-    double before = 0;
-    total = 0;
-#pragma unroll
-    for (uint32_t w = 0; w < kWarps; ++w) {
-      if (w == warp) before = total;
-      total += s.red[w];
-    }
-    return before + v;
+    const double in = lanes_scan(lane < kWarps ? s.red[lane] : 0.0);
+    total = __shfl_sync(0xFFFFFFFFu, in, kWarps - 1);
+    const double before = __shfl_sync(0xFFFFFFFFu, in, (warp + 31) % 32);
+    return warp ? before + v : v;
   }
 
-  // n more in bin b; those of one bin in a row are added at once
-  struct Bin {
-    uint32_t *hist, b = 0, n = 0;
-    __device__ void add(uint32_t to, uint32_t by) {
-      if (to != b) {
-        flush();
-        b = to;
-        n = 0;
-      }
-      n += by;
-    }
-    __device__ void flush() {
-      if (n) atomicAdd(hist + b, n);
-    }
-  };
-  __device__ uint32_t bin_of(float zv) const { return min((uint32_t)(zv * kPerOctave), kBins - 1); }
+  __device__ uint32_t bin_of(float zv) const { return min((uint32_t)zv, bins - 1); }
   __device__ void clear() {
-    for (uint32_t i = tid; i < kBins; i += kThreads) hist[i] = 0;
+    for (uint32_t i = tid; i < bins; i += kThreads) hist[i] = 0;
     __syncthreads();
   }
-  // histogram of the kept elements' counts
-  template <bool CUT>
+  // histogram of the elements' counts
   __device__ void fill_counts() {
     clear();
-    Bin bin{hist};
-    each<CUT>([&](float v, uint32_t) { bin.add(bin_of(z(v)), 1); });
-    bin.flush();
+    each<false>([&](float v, uint32_t) { atomicAdd(hist + bin_of(z(v)), 1u); });
   }
-  // of their masses, where elements above z_most only count for the whole mass, which is returned
+  // of the masses of those kept, where elements above z_most only count for the whole mass, which is returned
   template <bool CUT>
   __device__ double fill_masses(float z_most) {
     clear();
     double w = 0;
-    Bin bin{hist};
+    const float unit = kOctaves / last;
     each4<CUT>([&](const float (&v)[4], const bool (&use)[4], uint32_t) {
       double e[4];
       weights(v, use, e);
@@ -256,78 +274,91 @@ struct Row {
         const float zv = z(v[j]);
         if (!use[j] || zv > z_most) continue;
         const uint32_t b = bin_of(zv);
-        bin.add(b, __float2uint_rn(exp2f((float)b * (1.0f / kPerOctave) - zv) * 32768.0f));
+        atomicAdd(hist + b, __float2uint_rn(exp2f(((float)b - zv) * unit) * 32768.0f));
       }
     });
-    bin.flush();
     return sum(w);
   }
-  // The cluster's sums over bins: each CTA takes a share of the bins.  Returns that share's total.
+  // The cluster's sums over bins: each CTA takes a share of the bins, two a thread.  Returns that share's total.
   template <bool MASS>
   __device__ double reduce_bins() {
-    const uint32_t nb = kBins / ctas, per = nb > kThreads ? nb / kThreads : 1;  // at most 4 a thread
-    double v[4] = {0, 0, 0, 0};
+    static_assert(kCtaBins == 2 * kThreads, "two bins a thread");
     cluster_sync();
+    const uint32_t b = rank * kCtaBins + 2 * tid;
+    uint64_t h[kMaxCtas], t[2] = {0, 0};
 #pragma unroll
-    for (uint32_t j = 0; j < 4; ++j) {
-      const uint32_t i = tid * per + j;
-      if (j >= per || i >= nb) continue;
-      const uint32_t b = rank * nb + i;
-      uint32_t h[kMaxCtas];
+    for (uint32_t r = 0; r < kMaxCtas; ++r) h[r] = r < ctas ? ld_cluster64(dsmem_addr(hist + b, r)) : 0;
 #pragma unroll
-      for (uint32_t r = 0; r < kMaxCtas; ++r) h[r] = r < ctas ? ld_cluster32(dsmem_addr(hist + b, r)) : 0;
-      uint64_t t = 0;
-#pragma unroll
-      for (uint32_t r = 0; r < kMaxCtas; ++r) t += h[r];
-      v[j] = MASS ? (double)t * exp2(-(double)b / kPerOctave - 15.0) : (double)t;
+    for (uint32_t r = 0; r < kMaxCtas; ++r) {
+      t[0] += (uint32_t)h[r];
+      t[1] += h[r] >> 32;
+    }
+    double v[2] = {(double)t[0], (double)t[1]};
+    if (MASS) {  // in units of 2^-15 of the bin's largest weight
+      v[0] *= exp2((double)b * (-(double)kOctaves / bins) - 15.0);
+      v[1] *= exp2((double)(b + 1) * (-(double)kOctaves / bins) - 15.0);
     }
     double total;
-    double in = scan((v[0] + v[1]) + (v[2] + v[3]), total) - ((v[0] + v[1]) + (v[2] + v[3]));
-#pragma unroll
-    for (uint32_t j = 0; j < 4; ++j) {
-      in += v[j];
-      if (j < per && tid * per + j < nb) binsum[tid * per + j] = in;
-    }
+    const double in = scan(v[0] + v[1], total);
+    binsum[2 * tid] = in - v[1];
+    binsum[2 * tid + 1] = in;
     return total;
   }
-  // the first bin whose inclusive sum reaches `target` (the last bin where none does)
-  __device__ uint32_t find_bin(const Msg *all, double target) {
-    const uint32_t nb = kBins / ctas;
-    double before = 0;
-    uint32_t r = 0;
-    while (r + 1 < ctas && before + all[r].a < target) before += all[r++].a;
-    if (tid == 0) s.bin = nb - 1;
+  // the first bins whose inclusive sums reach two targets, the first not above the second (the last bin where none does)
+  __device__ void find_bins(const Msg *all, const double (&target)[2], uint32_t (&b)[2]) {
+    double before[2];
+    uint32_t r[2];
+    const double mine_a = lane < ctas ? all[lane].a : 0.0, in = lanes_scan(mine_a);
+#pragma unroll
+    for (uint32_t i = 0; i < 2; ++i) {
+      r[i] = min((uint32_t)__popc(__ballot_sync(0xFFFFFFFFu, lane < ctas && in < target[i])), ctas - 1);
+      before[i] = __shfl_sync(0xFFFFFFFFu, in - mine_a, r[i]);
+    }
+    if (tid < 2) s.bins[tid] = kCtaBins - 1;
     __syncthreads();
-    for (uint32_t i = tid; i < nb; i += kThreads)
-      if (before + __longlong_as_double((long long)ld_cluster64(dsmem_addr(binsum + i, r))) >= target) atomicMin(&s.bin, i);
+    double v[2][2];
+#pragma unroll
+    for (uint32_t i = 0; i < 2; ++i)
+#pragma unroll
+      for (uint32_t j = 0; j < 2; ++j)
+        v[i][j] = __longlong_as_double((long long)ld_cluster64(dsmem_addr(binsum + tid + j * kThreads, r[i])));
+#pragma unroll
+    for (uint32_t i = 0; i < 2; ++i)
+#pragma unroll
+      for (uint32_t j = 0; j < 2; ++j) {
+        const uint32_t ok = __ballot_sync(0xFFFFFFFFu, before[i] + v[i][j] >= target[i]);
+        if (ok && lane == __ffs(ok) - 1) atomicMin(&s.bins[i], tid + j * kThreads);
+      }
     __syncthreads();
-    const uint32_t b = r * nb + s.bin;
+    b[0] = r[0] * kCtaBins + s.bins[0];
+    b[1] = r[1] * kCtaBins + s.bins[1];
     __syncthreads();
-    return b;
   }
   __device__ void note(uint32_t key, uint32_t id) {
     if (*reinterpret_cast<volatile uint32_t *>(&s.count) >= kList) return;  // a list that is full is of no use
     const uint32_t at = atomicAdd(&s.count, 1u);
     if (at < kList) list[at] = (uint64_t)key << 32 | (uint32_t)~id;
   }
-  // Sorts list[0 .. n) in descending order, entries all different; behind them zeros to the next power of
-  // two.  Up to 128 by counting the larger ones, four threads an entry: two barriers (a bitonic sort of 128: 28).
+  // Sorts list[0 .. some) in descending order, entries all different but for zeros; behind them zeros to the
+  // next power of two.  Up to 256 by counting the larger ones, with two threads an entry or more: four
+  // barriers (a bitonic sort of 256: 36).
   __device__ void sort(uint32_t some) {
-    if (some <= 128) {
-      const uint32_t i = tid / 4;
+    if (some <= 256) {
+      uint32_t log = 1;
+      while (log < 5 && some << (log + 1) <= kThreads) ++log;
+      const uint32_t i = tid >> log, step = 1u << log;
       uint64_t e = 0;
       uint32_t place = 0;
       __syncthreads();
       if (i < some) {
         e = list[i];
-        for (uint32_t j = tid % 4; j < some; j += 4) place += list[j] > e;
+        for (uint32_t j = tid & (step - 1); j < some; j += step) place += list[j] > e;
       }
-      place += __shfl_xor_sync(0xFFFFFFFFu, place, 1);
-      place += __shfl_xor_sync(0xFFFFFFFFu, place, 2);
+      for (uint32_t o = 1; o < step; o <<= 1) place += __shfl_xor_sync(0xFFFFFFFFu, place, o);
       __syncthreads();
       if (tid < some) list[tid] = 0;
       __syncthreads();
-      if (e && tid % 4 == 0) list[place] = e;
+      if (e && (tid & (step - 1)) == 0) list[place] = e;
       __syncthreads();
       return;
     }
@@ -351,8 +382,7 @@ struct Row {
   // no CTA reads another's memory.
   __device__ bool gather(const Msg *all, uint32_t &n) {
     uint64_t mine[2] = {0, 0};
-    n = 0;
-    for (uint32_t r = 0; r < ctas; ++r) n += all[r].c;
+    n = all_c(all);
     if (rank == 0)
 #pragma unroll
       for (uint32_t e = 0; e < 2; ++e) {
@@ -369,7 +399,10 @@ struct Row {
     sort(n);
     return true;
   }
-  __device__ double list_weight(uint64_t e) const { return e ? weight(key_float((uint32_t)(e >> 32))) : 0.0; }
+  __device__ double list_weight(uint64_t e) const {
+    const float v = key_float((uint32_t)(e >> 32));
+    return e && z(v) <= last ? weight(v) : 0.0;
+  }
 
   __device__ void answer(uint32_t row, uint32_t id, double prob) {
     p.ids[row] = id;
@@ -389,7 +422,7 @@ struct Row {
     for (uint32_t j = 0; j < 2; ++j) {
       const uint32_t i = 2 * tid + j;
       const double before = j ? in - w[1] : in - w[1] - w[0];
-      const bool stay = i < min(n, k) && (i == 0 || pp >= 1.0 || before < target) && w[j] >= min_p;
+      const bool stay = i < min(n, k) && (i == 0 || pp >= 1.0 || before < target) && w[j] >= min_p && w[j] > 0;
       list[i] = stay ? (e[j] & 0xFFFFFFFFull) << 32 | (uint32_t)(e[j] >> 32) : 0;  // (~id, value): by id
     }
     sort(n);
@@ -416,36 +449,107 @@ struct Row {
     }
   }
 
-  // What top-k needs, where k is small beside the threads: the elements down to the bin in which
-  // the threads' k-th largest maximum lies, a few more than k.  True: the row is finished.
-  __device__ bool few_largest(uint32_t row, float best, uint32_t k, double pp, double min_p, double u) {
-    clear();
+  // Notes this CTA's elements from the k-th largest of its threads' maxima on: what the row's first k are among.
+  __device__ void note_largest(float best, uint32_t k) {
+    const uint32_t key = float_key(best);
+    const bool some = best > -INFINITY;
+    uint32_t o1 = 0, have = some, lo = some ? key : 0xFFFFFFFFu, hi = key;
+    sums(have, o1, lo, hi);
+    if (have < k) lo = hi = 0;  // all there are
+    while (lo < hi) {  // at least k maxima are not below lo
+      const uint32_t mid = lo + (hi - lo + 1) / 2, n = __syncthreads_count(key >= mid);
+      if (n >= k) lo = mid;
+      else hi = mid - 1;
+      if (n >= k && n <= k + k / 4 + 2) break;
+    }
+    const float from = lo ? key_float(lo) : -3.402823466e38f;
     if (tid == 0) s.count = 0;
-    if (z(best) <= kOctaves) atomicAdd(hist + bin_of(z(best)), 1u);
-    const Msg *all = share(Msg{reduce_bins<false>(), 0, 0, 0, 0, 0});
-    double n = 0;
-    for (uint32_t r = 0; r < ctas; ++r) n += all[r].a;
-    if (n < (double)k) return false;
-    const uint32_t b = find_bin(all, (double)k);
-    uint32_t own = 0, o1 = 0, o2 = 0, o3 = 0;
-    each<false>([&](float v, uint32_t id) {
-      if (bin_of(z(v)) > b) return;
-      note(float_key(v), id);
-      ++own;
-    });
-    sums(own, o1, o2, o3);
-    all = share(Msg{0, 0, own, 0, 0, 0});
-    own = 0;
-    for (uint32_t r = 0; r < ctas; ++r) own += all[r].c;
-    if (own > kList) return false;
-    uint32_t m;
-    if (gather(all, m)) finish_list(row, m, k, pp, -1.0, min_p, u);
-    return true;
+    __syncthreads();
+    for (uint32_t g = 0; g < groups; ++g) {
+      float v[4];
+      load(mine + 128 * g, v);
+      if (fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])) < from) continue;
+      const uint32_t id = id0 + mine + 128 * g;
+#pragma unroll
+      for (uint32_t j = 0; j < 4; ++j)
+        if (v[j] >= from) note(float_key(v[j]), id + j);
+    }
+    __syncthreads();
+  }
+  // The row from what all CTAs noted, n together.
+  __device__ void pick_largest(uint32_t row, const Msg *all, uint32_t n, uint32_t k, double pp, double min_p, double u) {
+    constexpr uint32_t kPer = kList / kThreads;
+    uint64_t e[kPer];
+    if (rank == 0)
+#pragma unroll
+      for (uint32_t j = 0; j < kPer; ++j) {
+        uint32_t i = tid + j * kThreads, r = 0;
+        e[j] = 0;
+        if (i >= n) continue;
+        while (i >= all[r].d) i -= all[r++].d;
+        e[j] = ld_cluster64(dsmem_addr(list + i, r));
+      }
+    cluster_sync();
+    if (rank) return;
+    // a value that at least k are not below, and few more
+    uint32_t lo = 0xFFFFFFFFu, hi = 0, o0 = 0, o1 = 0;
+#pragma unroll
+    for (uint32_t j = 0; j < kPer; ++j)
+      if (e[j]) {
+        lo = min(lo, (uint32_t)(e[j] >> 32));
+        hi = max(hi, (uint32_t)(e[j] >> 32));
+      }
+    sums(o0, o1, lo, hi);
+    while (n > 256 && lo < hi) {
+      const uint32_t mid = lo + (hi - lo + 1) / 2;
+      uint32_t c = 0;
+#pragma unroll
+      for (uint32_t j = 0; j < kPer; ++j)
+        if (j * kThreads < n) c += __syncthreads_count((uint32_t)(e[j] >> 32) >= mid);
+      if (c >= k) lo = mid;
+      else hi = mid - 1;
+      if (c >= k && c <= 256) break;
+    }
+    if (tid == 0) s.count = 0;
+    for (uint32_t i = tid; i < kSort; i += kThreads) list[i] = 0;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t j = 0; j < kPer; ++j)
+      if (e[j] && (uint32_t)(e[j] >> 32) >= lo) {
+        const uint32_t at = atomicAdd(&s.count, 1u);
+        if (at < kSort) list[at] = e[j];
+      }
+    __syncthreads();
+    uint32_t m = s.count;
+    __syncthreads();
+    if (m > kSort) {  // equal values at the place: of those the lowest ids, the k largest entries
+      uint64_t a = (uint64_t)lo << 32, b = (uint64_t)hi << 32 | 0xFFFFFFFFu;
+      while (a < b) {
+        const uint64_t mid = a + (b - a + 1) / 2;
+        uint32_t c = 0;
+#pragma unroll
+        for (uint32_t j = 0; j < kPer; ++j) c += __syncthreads_count(e[j] >= mid);
+        if (c >= k) a = mid;
+        else b = mid - 1;
+        if (c == k) break;
+      }
+      if (tid == 0) s.count = 0;
+      for (uint32_t i = tid; i < kSort; i += kThreads) list[i] = 0;
+      __syncthreads();
+#pragma unroll
+      for (uint32_t j = 0; j < kPer; ++j)
+        if (e[j] && e[j] >= a) list[atomicAdd(&s.count, 1u)] = e[j];
+      __syncthreads();
+      m = s.count;
+      __syncthreads();
+    }
+    sort(m);
+    finish_list(row, m, k, pp, -1.0, min_p, u);
   }
 
   // mass of the thread's elements above `upto`, where a cut has formed it
   double strict = 0;
-  uint32_t upto = 0xFFFFFFFFu;
+  float upto = INFINITY;
 
   // Finds the place of a cut whose bracket is the bins [b0, b1]: the shortest beginning with
   // the count or mass `target`, and takes it over into cut_key and cut_id.  CUT: there is one already.
@@ -454,17 +558,19 @@ struct Row {
   __device__ bool cut(uint32_t row, uint32_t b0, uint32_t b1, double target, uint32_t k, double pp, double whole, double min_p, double u) {
     if (tid == 0) s.count = 0;
     __syncthreads();
+    // the bins b0 to b1 are z0 <= z < z1; the last one has all that is left
+    const float z0 = (float)b0, z1 = b1 + 1 == bins ? INFINITY : (float)(b1 + 1);
     double a = 0;
     uint32_t above = 0, m = 0, kmin = 0xFFFFFFFFu, kmax = 0;
     each4<CUT>([&](const float (&v)[4], const bool (&use)[4], uint32_t id) {
       bool over[4], any = false;
 #pragma unroll
       for (uint32_t j = 0; j < 4; ++j) {
-        const uint32_t b = bin_of(z(v[j]));
-        over[j] = use[j] && b < b0;
+        const float zv = z(v[j]);
+        over[j] = use[j] && zv < z0;
         any |= over[j];
         above += over[j];
-        if (use[j] && b >= b0 && b <= b1) {
+        if (use[j] && !over[j] && zv < z1) {
           const uint32_t key = float_key(v[j]);
           note(key, id + j);
           ++m;
@@ -484,19 +590,14 @@ struct Row {
     sums(above, m, kmin, kmax);
     if (MASS) a = sum(a);
     const Msg *all = share(Msg{MASS ? a : (double)above, 0, above + m, m, kmin, kmax});
-    double A = 0;
-    uint32_t total = 0;
-    m = 0;
-    for (uint32_t r = 0; r < ctas; ++r) {
-      A += all[r].a;
-      total += all[r].c;
-      m += all[r].d;
-      kmin = min(kmin, all[r].e);
-      kmax = max(kmax, all[r].f);
-    }
-    if (total <= kList) {  // all of them to the list
+    double A = all_a(all);
+    const uint32_t total = all_c(all), l = lane % ctas;
+    m = __reduce_add_sync(0xFFFFFFFFu, lane < ctas ? all[lane].d : 0);
+    kmin = __reduce_min_sync(0xFFFFFFFFu, all[l].e);
+    kmax = __reduce_max_sync(0xFFFFFFFFu, all[l].f);
+    if (total <= kSort) {  // all of them to the list
       each<CUT>([&](float v, uint32_t id) {
-        if (bin_of(z(v)) < b0) note(float_key(v), id);
+        if (z(v) < z0) note(float_key(v), id);
       });
       __syncthreads();
       all = share(Msg{0, 0, s.count, 0, 0, 0});
@@ -504,10 +605,10 @@ struct Row {
       if (gather(all, n)) finish_list(row, n, k, pp, whole, min_p, u);
       return true;
     }
-    const bool listed = m <= kList;
-    if (MASS) upto = kmax;
+    const bool listed = m <= kSort;
+    if (MASS) upto = key_float(kmax);
     // halve the range of values until the list holds it, or one value is left
-    while (m > kList && kmin < kmax) {
+    while (m > kSort && kmin < kmax) {
       const uint32_t mid = kmin + (kmax - kmin + 1) / 2;
       double b = 0;
       uint32_t up = 0, o1 = 0, o2 = 0, o3 = 0;
@@ -520,12 +621,8 @@ struct Row {
       sums(up, o1, o2, o3);
       if (MASS) b = sum(b);
       all = share(Msg{MASS ? b : (double)up, 0, up, 0, 0, 0});
-      double B = 0;
-      uint32_t n = 0;
-      for (uint32_t r = 0; r < ctas; ++r) {
-        B += all[r].a;
-        n += all[r].c;
-      }
+      const double B = all_a(all);
+      const uint32_t n = all_c(all);
       if (A + B >= target) {
         kmin = mid;
         m = n;
@@ -549,9 +646,9 @@ struct Row {
       for (uint32_t i = 0; i < warp; ++i) before += s.redu[0][i];
       if (before < need && need <= before + of_warp)
         for (uint32_t g = 0; g < groups; ++g) {
-          const float4 v = *reinterpret_cast<const float4 *>(x + mine + 128 * g);
+          float e[4];
+          load(mine + 128 * g, e);
           const uint32_t id = id0 + mine + 128 * g;
-          const float e[4] = {v.x, v.y, v.z, v.w};
           bool yes[4];
           uint32_t n = 0;
 #pragma unroll
@@ -572,7 +669,7 @@ struct Row {
       sums(o1, o2, found, o3);
       all = share(Msg{0, 0, found, 0, 0, 0});
       for (uint32_t r = 0; r < ctas; ++r) found = min(found, all[r].c);
-      cut_key = kmin;
+      cut_at = key_float(kmin);
       cut_id = found;
       return false;
     }
@@ -605,11 +702,20 @@ struct Row {
       place.d = ~(uint32_t)at;
     }
     all = share(place);
-    cut_key = all[0].c;
+    cut_at = key_float(all[0].c);
     cut_id = all[0].d;
     return false;
   }
 
+  // The first lane up to which the sums of v exceed `at`, or (rounding) the last with any; `at` becomes
+  // what is left of it there.  The same in all warps.
+  __device__ uint32_t find_sum(double v, double &at) const {
+    const double in = lanes_scan(v);
+    const uint32_t over = __ballot_sync(0xFFFFFFFFu, v > 0 && in > at), some = __ballot_sync(0xFFFFFFFFu, v > 0);
+    const uint32_t l = over ? __ffs(over) - 1 : some ? 31 - __clz(some) : 0;
+    at -= __shfl_sync(0xFFFFFFFFu, in - v, l);
+    return l;
+  }
   // the draw from what is kept, by id
   template <bool CUT>
   __device__ void draw(uint32_t row, double min_p, double u) {
@@ -618,7 +724,7 @@ struct Row {
       bool add[4], any = false;
 #pragma unroll
       for (uint32_t j = 0; j < 4; ++j) {
-        add[j] = use[j] && !(CUT && float_key(v[j]) > upto);  // those above are counted
+        add[j] = use[j] && !(CUT && v[j] > upto);  // those above are counted
         any |= add[j];
       }
       if (CUT && !any) return;
@@ -628,39 +734,17 @@ struct Row {
       for (uint32_t j = 0; j < 4; ++j)
         if (w[j] >= min_p) own += w[j];
     });
-    double of_warp = own;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) of_warp += __shfl_xor_sync(0xFFFFFFFFu, of_warp, o);
-    __syncthreads();
-    if (lane == 0) s.red[warp] = of_warp;
-    __syncthreads();
-    double total = 0;
-#pragma unroll
-    for (uint32_t i = 0; i < kWarps; ++i) total += s.red[i];
-    const Msg *all = share(Msg{total, 0, 0, 0, 0, 0});
-    double M = 0, at, before = 0;
-    for (uint32_t r = 0; r < ctas; ++r) M += all[r].a;
-    at = u * M;
-    // the CTA with the token, then its warp: the first whose sum is above, or (rounding) the last with any mass
-    uint32_t r = 0, last = 0;
-    for (uint32_t i = 0; i < ctas; ++i)
-      if (all[i].a > 0) last = i;
-    while (r < last && before + all[r].a <= at) before += all[r++].a;
-    if (rank != r) return;
-    at -= before;
-    before = 0;
-    uint32_t who = 0;
-    for (uint32_t i = 0; i < kWarps; ++i)
-      if (s.red[i] > 0) last = i;
-    if (s.red[last] == 0) last = kWarps - 1;
-    while (who < last && before + s.red[who] <= at) before += s.red[who++];
+    const Msg *all = share(Msg{sum(own), 0, 0, 0, 0, 0});  // the warps' sums stay in s.red
+    const double M = all_a(all);
+    double at = u * M;
+    // the CTA with the token, then its warp
+    if (rank != find_sum(lane < ctas ? all[lane].a : 0.0, at)) return;
+    const uint32_t who = find_sum(lane < kWarps ? s.red[lane] : 0.0, at);
     // that warp's groups, one to each warp
-    at -= before;
     const uint32_t chunk = who * 128 * groups + 4 * lane;
     auto group = [&](uint32_t g, float (&v)[4], double (&w)[4]) {
-      const float4 x4 = *reinterpret_cast<const float4 *>(x + chunk + 128 * g);
+      load(chunk + 128 * g, v);
       const uint32_t id = id0 + chunk + 128 * g;
-      v[0] = x4.x, v[1] = x4.y, v[2] = x4.z, v[3] = x4.w;
       bool use[4];
 #pragma unroll
       for (uint32_t j = 0; j < 4; ++j) use[j] = kept<CUT>(v[j], id + j);
@@ -674,28 +758,15 @@ struct Row {
     double w[4];
     for (uint32_t g = warp; g < groups; g += kWarps) {
       group(g, v, w);
-      double t = (w[0] + w[1]) + (w[2] + w[3]);
-#pragma unroll
-      for (int o = 16; o; o >>= 1) t += __shfl_xor_sync(0xFFFFFFFFu, t, o);
+      const double t = lanes_sum((w[0] + w[1]) + (w[2] + w[3]));
       if (lane == 0) of_group[g] = t;
     }
     __syncthreads();
-    uint32_t g = 0;
-    before = 0;
-    last = 0;
-    for (uint32_t i = 0; i < groups; ++i)
-      if (of_group[i] > 0) last = i;
-    while (g < last && before + of_group[g] <= at) before += of_group[g++];
+    const uint32_t g = find_sum(lane < groups ? of_group[lane] : 0.0, at);
     if (g % kWarps != warp) return;
-    at -= before;
     group(g, v, w);
     const double four = (w[0] + w[1]) + (w[2] + w[3]);
-    double in = four;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const double y = __shfl_up_sync(0xFFFFFFFFu, in, o);
-      if (lane >= (uint32_t)o) in += y;
-    }
+    const double in = lanes_scan(four);
     const uint32_t over = __ballot_sync(0xFFFFFFFFu, four > 0 && in > at), some = __ballot_sync(0xFFFFFFFFu, four > 0);
     if (lane != (over ? __ffs(over) - 1 : 31 - __clz(some))) return;
     double sum = in - four, best_w = 0;
@@ -712,12 +783,15 @@ struct Row {
   }
 };
 
+// bytes of the list, or the bins over it
+__host__ __device__ constexpr uint32_t region(uint32_t ctas) { return kList * 8 > kCtaBins * 4 * ctas ? kList * 8 : kCtaBins * 4 * ctas; }
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 2) k_sample_logits(const SampleParams p) {
   extern __shared__ __align__(16) uint8_t dsm[];
   __shared__ Small s;
   const uint32_t ctas = p.ctas, row = blockIdx.x / ctas;
-  Row w(p, s);
+  Row<T> w(p, s);
   w.tid = threadIdx.x;
   w.lane = w.tid & 31;
   w.warp = w.tid >> 5;
@@ -725,64 +799,92 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_logits(const SampleParam
   w.ctas = ctas;
   w.groups = p.groups;
   w.list = reinterpret_cast<uint64_t *>(dsm);
-  w.hist = reinterpret_cast<uint32_t *>(dsm + kList * 8);
-  w.binsum = reinterpret_cast<double *>(dsm + kList * 8 + kBins * 4);
-  w.x = reinterpret_cast<float *>(dsm + kList * 8 + kBins * 4 + kBins / ctas * 8);
-  const uint32_t slice = p.groups * kGroup;
-  w.id0 = w.rank * slice;
+  w.hist = reinterpret_cast<uint32_t *>(dsm);
+  w.binsum = reinterpret_cast<double *>(dsm + region(ctas));
+  w.x = reinterpret_cast<T *>(dsm + region(ctas) + kCtaBins * 8);
+  w.id0 = w.rank * p.slice;
   w.mine = w.warp * 128 * p.groups + 4 * w.lane;
   if (w.tid < 32) s.power[w.tid] = exp2((double)w.tid / 32.0);
-  // the row's own settings; one that does not hold leaves it as it was (the same for all CTAs)
   const uint32_t at = p.rows ? p.rows[row] : row;
   if (at == FA_NO_TOKEN) return;
+  // the row's own settings: on their way while the logits are read
   const float t = p.temperature ? p.temperature[row] : 1.0f, u = p.u[row], pp = p.top_p ? p.top_p[row] : 1.0f, mp = p.min_p ? p.min_p[row] : 0.0f;
-  uint32_t k = p.top_k ? p.top_k[row] : 0;
-  if (at >= p.n_logits || !(t == 0.0f || (t >= 1e-6f && t <= 1e6f)) || !(u >= 0.0f && u < 1.0f) || !(pp >= 0.0f) || !(mp >= 0.0f && mp <= 1.0f)) {
-    if (p.err && w.rank == 0 && w.tid == 0) atomicOr(p.err, kFlagRange);
-    return;
-  }
-  // the CTA's part of the row, in f32; behind its end nothing
-  const uint32_t len = w.id0 < p.vocab ? min(slice, p.vocab - w.id0) : 0;
+  const uint32_t k = p.top_k ? p.top_k[row] : 0;
+  // the CTA's part of the row; behind its end -inf
+  const uint32_t len = at < p.n_logits && w.id0 < p.vocab ? min(p.slice, p.vocab - w.id0) : 0, room = p.groups * kGroup;
   const T *src = reinterpret_cast<const T *>(p.logits) + (uint64_t)at * p.ld + w.id0;
   float mx = -INFINITY;
   constexpr uint32_t kV = 16 / sizeof(T);
   uint32_t i = 0;
   if (p.aligned) {
     const uint32_t whole = len / kV;
-    constexpr uint32_t kAhead = 8;  // loads in flight
-    for (uint32_t j0 = w.tid; j0 < whole; j0 += kAhead * kThreads) {
-      Vec<T> v[kAhead];
+    constexpr uint32_t kAhead = sizeof(T) == 4 ? 8 : 4;  // loads in flight
+    if constexpr (sizeof(T) == 4) {
+      for (uint32_t j0 = w.tid; j0 < whole; j0 += kAhead * kThreads) {
+        float4 v[kAhead];
 #pragma unroll
-      for (uint32_t a = 0; a < kAhead; ++a)
-        if (j0 + a * kThreads < whole) v[a] = *reinterpret_cast<const Vec<T> *>(src + (uint64_t)(j0 + a * kThreads) * kV);
+        for (uint32_t a = 0; a < kAhead; ++a)
+          if (j0 + a * kThreads < whole) v[a] = *reinterpret_cast<const float4 *>(src + (uint64_t)(j0 + a * kThreads) * kV);
 #pragma unroll
-      for (uint32_t a = 0; a < kAhead; ++a) {
-        if (j0 + a * kThreads >= whole) break;
-        float f[kV];
-#pragma unroll
-        for (uint32_t e = 0; e < kV; ++e) {
-          f[e] = to_logit((float)v[a].v[e]);
-          mx = fmaxf(mx, f[e]);
+        for (uint32_t a = 0; a < kAhead; ++a) {
+          if (j0 + a * kThreads >= whole) break;
+          clean(v[a].x, v[a].y, mx);
+          clean(v[a].z, v[a].w, mx);
+          *reinterpret_cast<float4 *>(w.x + (j0 + a * kThreads) * kV) = v[a];
         }
-#pragma unroll
-        for (uint32_t e = 0; e < kV; e += 4)
-          *reinterpret_cast<float4 *>(w.x + (j0 + a * kThreads) * kV + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
       }
+    } else {
+      using T2 = typename Pair<T>::type;
+      union Eight {
+        uint4 u;
+        T2 p[4];
+      };
+      T2 zero, none, most;
+      zero.x = zero.y = (T)0.0f;
+      none.x = none.y = (T)(-INFINITY);
+      most = none;
+      for (uint32_t j0 = w.tid; j0 < whole; j0 += kAhead * kThreads) {
+        uint4 v[kAhead];
+#pragma unroll
+        for (uint32_t a = 0; a < kAhead; ++a)
+          if (j0 + a * kThreads < whole) v[a] = *reinterpret_cast<const uint4 *>(src + (uint64_t)(j0 + a * kThreads) * kV);
+#pragma unroll
+        for (uint32_t a = 0; a < kAhead; ++a) {
+          if (j0 + a * kThreads >= whole) break;
+          Eight e;
+          e.u = v[a];
+#pragma unroll
+          for (uint32_t i2 = 0; i2 < 4; ++i2) clean2(e.p[i2], zero, none, most);
+          *reinterpret_cast<uint4 *>(w.x + (j0 + a * kThreads) * kV) = e.u;
+        }
+      }
+      mx = fmaxf(to_f32(most.x), to_f32(most.y));
     }
     i = whole * kV;
   }
-  for (uint32_t j = i + w.tid; j < slice; j += kThreads) {
-    const float f = j < len ? to_logit((float)src[j]) : -INFINITY;
+  for (uint32_t j = i + w.tid; j < room; j += kThreads) {
+    const T f = j < len ? clean(src[j]) : (T)(-INFINITY);
     w.x[j] = f;
-    mx = fmaxf(mx, f);
+    mx = fmaxf(mx, to_f32(f));
   }
-  const float own_max = mx;
+  mx = to_f32(mx);
+  // a setting that does not hold leaves the row as it was (the same for all CTAs)
+  if (at >= p.n_logits || !(t == 0.0f || (t >= 1e-6f && t <= 1e6f)) || !(u >= 0.0f && u < 1.0f) || !(pp >= 0.0f) || !(mp >= 0.0f && mp <= 1.0f)) {
+    if (p.err && w.rank == 0 && w.tid == 0) atomicOr(p.err, kFlagRange);
+    return;
+  }
+  const bool few = t > 0 && k && k < p.vocab && k <= kFewK;
+  if (few) {
+    __syncthreads();
+    w.note_largest(mx, k);
+  }
   uint32_t o0 = 0, o1 = 0, o2 = 0, key = float_key(mx);
   w.sums(o0, o1, o2, key);
-  const Msg *all = w.share(Msg{0, 0, key, 0, 0, 0});
-  for (uint32_t r = 0; r < ctas; ++r) key = max(key, all[r].c);
-  w.mx = key_float(key);
-  if (w.mx == -INFINITY) {  // no candidate at all
+  const Msg *all = w.share(Msg{0, 0, key, few ? s.count : 0, 0, 0});
+  key = __reduce_max_sync(0xFFFFFFFFu, all[w.lane % ctas].c);
+  const uint32_t noted = __reduce_add_sync(0xFFFFFFFFu, w.lane < ctas ? all[w.lane].d : 0);
+  const float top = key_float(key);
+  if (top == -INFINITY) {  // no candidate at all
     if (w.rank == 0 && w.tid == 0) {
       p.ids[row] = FA_NO_TOKEN;
       if (p.logprobs) p.logprobs[row] = -INFINITY;
@@ -792,53 +894,58 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_logits(const SampleParam
   }
   if (t == 0.0f) {  // the lowest id of the maximum
     uint32_t best = 0xFFFFFFFFu;
-    for (uint32_t j = w.tid; j < len; j += kThreads)
-      if (w.x[j] == w.mx) best = min(best, w.id0 + j);
+    for (uint32_t g = w.groups; g-- > 0;) {
+      float v[4];
+      w.load(w.mine + 128 * g, v);
+#pragma unroll
+      for (int j = 3; j >= 0; --j)
+        if (v[j] == top) best = w.id0 + w.mine + 128 * g + j;
+    }
     w.sums(o0, o1, best, o2);
     all = w.share(Msg{0, 0, best, 0, 0, 0});
     for (uint32_t r = 0; r < ctas; ++r) best = min(best, all[r].c);
     if (w.rank == 0 && w.tid == 0) w.answer(row, best, 1.0);
     return;
   }
-  const double c = 1.4426950408889634074 / (double)t;
-  w.cf = (float)c;
-  w.c32 = 32.0 * c;
-  w.mxd = (double)w.mx;
+  w.scale(top, t);
+  if (few && noted < kList) {  // a CTA whose list ran over has at least kList
+    w.pick_largest(row, all, noted, k, pp, mp, u);
+    return;
+  }
   bool has_cut = false;
   if (k && k < p.vocab) {
-    // a quarter of the threads: beyond it the maxima stand for more and more elements
-    if (k <= ctas * kThreads / 4 && w.few_largest(row, own_max, k, pp, mp, u)) return;
-    w.fill_counts<false>();
-    all = w.share(Msg{w.reduce_bins<false>(), 0, 0, 0, 0, 0});
-    double n = 0;
-    for (uint32_t r = 0; r < ctas; ++r) n += all[r].a;
-    if (n > (double)k) {
-      const uint32_t b = w.find_bin(all, (double)k);
-      if (w.cut<false, false>(row, b, b, (double)k, k, pp, -1.0, mp, u)) return;
+    w.fill_counts();
+    all = w.share(Msg{w.template reduce_bins<false>(), 0, 0, 0, 0, 0});
+    if (w.all_a(all) > (double)k) {
+      const double target[2] = {(double)k, (double)k};
+      uint32_t b[2];
+      w.find_bins(all, target, b);
+      if (w.template cut<false, false>(row, b[0], b[1], (double)k, k, pp, -1.0, mp, u)) return;
       has_cut = true;
     }
   }
   if (pp < 1.0f) {
     // all mass above z_most is less than half of what may be cut: the place is below it
-    const float z_most = log2f((float)p.vocab) - log2f(1.0f - pp) + 1.0f;
-    const double whole = has_cut ? w.fill_masses<true>(z_most) : w.fill_masses<false>(z_most);
-    const double total = w.reduce_bins<true>();
+    const float z_most = (log2f((float)p.vocab) - log2f(1.0f - pp) + 1.0f) * (w.last / kOctaves);
+    const double whole = has_cut ? w.template fill_masses<true>(z_most) : w.template fill_masses<false>(z_most);
+    const double total = w.template reduce_bins<true>();
     all = w.share(Msg{total, whole, 0, 0, 0, 0});
-    double W = 0;
-    for (uint32_t r = 0; r < ctas; ++r) W += all[r].b;
-    const double target = (double)pp * W;
-    const uint32_t b0 = w.find_bin(all, target * (1.0 - 2 * kHistError)), b1 = w.find_bin(all, target * (1.0 + 2 * kHistError));
-    if (has_cut ? w.cut<true, true>(row, b0, b1, target, 0xFFFFFFFFu, pp, W, mp, u) : w.cut<true, false>(row, b0, b1, target, 0xFFFFFFFFu, pp, W, mp, u))
+    const double W = w.all_b(all), target = (double)pp * W;
+    const double around[2] = {target * (1.0 - 2 * kHistError), target * (1.0 + 2 * kHistError)};
+    uint32_t b[2];
+    w.find_bins(all, around, b);
+    if (has_cut ? w.template cut<true, true>(row, b[0], b[1], target, 0xFFFFFFFFu, pp, W, mp, u)
+                : w.template cut<true, false>(row, b[0], b[1], target, 0xFFFFFFFFu, pp, W, mp, u))
       return;
     has_cut = true;
   }
-  if (has_cut) w.draw<true>(row, (double)mp, (double)u);
-  else w.draw<false>(row, (double)mp, (double)u);
+  if (has_cut) w.template draw<true>(row, (double)mp, (double)u);
+  else w.template draw<false>(row, (double)mp, (double)u);
 }
 
 template <typename T>
 int launch(const SampleParams &p, cudaStream_t st) {
-  const uint32_t smem = kList * 8 + kBins * 4 + kBins / p.ctas * 8 + p.groups * kGroup * 4;
+  const uint32_t smem = region(p.ctas) + kCtaBins * 8 + p.groups * kGroup * (uint32_t)sizeof(T);
   if (cudaFuncSetAttribute(k_sample_logits<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSampleMaxSmem) != cudaSuccess) return -1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(p.n * p.ctas);
@@ -856,14 +963,20 @@ int launch(const SampleParams &p, cudaStream_t st) {
 
 }  // namespace
 
-int launch_sample_logits(const SampleParams &in, cudaStream_t st) {
+int launch_sample_logits(const SampleParams &in, uint32_t n_sm, cudaStream_t st) {
   SampleParams p = in;
-  // the smallest cluster that leaves four groups or fewer; eight CTAs at most
+  const uint32_t es = elem_size(p.dtype);
   auto groups = [&](uint32_t ctas) { return (p.vocab + ctas * kGroup - 1) / (ctas * kGroup); };
+  auto fits = [&](uint32_t ctas) { return region(ctas) + kCtaBins * 8 + groups(ctas) * kGroup * es <= kSampleMaxSmem; };
   p.ctas = 1;
-  while (p.ctas < kMaxCtas && groups(p.ctas) > 4) p.ctas *= 2;
+  while (!fits(p.ctas)) p.ctas *= 2;
+  // As many CTAs to a row as keep four an SM (two of which run at once): shorter rows a CTA, but more barriers
+  // of clusters.  64 rows of 128256, f32, cuts of all kinds: 55 us with 8, 65 with 4; 200 of 32000, bf16: 40 with 2, 56
+  // with 1, 81 with 4 .. 8.
+  while (p.ctas < kMaxCtas && groups(p.ctas) > 1 && p.n * p.ctas * 2 <= 4 * n_sm) p.ctas *= 2;
   p.groups = groups(p.ctas);
-  static_assert(kSampleMaxVocab == kMaxCtas * kGroup * 25 && kList * 8 + kBins * 4 + kBins / kMaxCtas * 8 + 25 * kGroup * 4 <= kSampleMaxSmem,
+  p.slice = ((p.vocab + p.ctas - 1) / p.ctas + 15) / 16 * 16;
+  static_assert(region(kMaxCtas) + kCtaBins * 8 + kSampleMaxVocab / kMaxCtas * 4 <= kSampleMaxSmem && kSampleMaxVocab % (kMaxCtas * kGroup) == 0,
                 "shared memory of the largest vocabulary");
   switch (p.dtype) {
     case FA_KV_F32: return launch<float>(p, st);
