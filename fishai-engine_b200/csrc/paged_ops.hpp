@@ -96,7 +96,7 @@ struct StepPlanParams {
 int launch_step_plan(const StepPlanParams &p, cudaStream_t st);
 
 // ---- sampling from given numbers ----
-constexpr uint32_t kSampleMaxVocab = 8 * 2048 * 22, kSampleMaxSmem = 224 * 1024;
+constexpr uint32_t kSampleMaxVocab = 8 * 2048 * 24, kSampleMaxSmem = 220 * 1024;
 struct SampleParams {
   const void *logits;
   int dtype;

@@ -28,7 +28,7 @@ namespace {
 
 constexpr uint32_t kThreads = 512, kWarps = kThreads / 32, kMaxCtas = 8;
 constexpr uint32_t kList = 2048, kSort = 1024;  // noted elements of a CTA (and of a cluster); most that are sorted
-constexpr uint32_t kCtaBins = 1024;             // bins for each CTA of the cluster: finer for longer rows
+constexpr uint32_t kCtaBins = 512;              // bins for each CTA of the cluster: finer for longer rows
 constexpr uint32_t kFewK = 128;                 // the top-k that goes by the threads' maxima
 constexpr float kOctaves = 64.0f;
 constexpr double kHistError = 1.0 / 32768;      // of a sum of the histogram's masses: each is rounded to 2^-15 of its bin's largest, and exponentials are f32
@@ -43,7 +43,7 @@ struct Small {
   double red[kWarps];
   uint32_t redu[4][kWarps];
   uint32_t bin, count, bins[2];
-  double power[32];  // 2^(i / 32)
+  double power[512];  // 2^(i / 512)
 };
 
 // Two logits as they are kept: NaN as -inf, -0 as +0.  In f32 (to_f32) +inf is the largest number.
@@ -87,11 +87,25 @@ __device__ __forceinline__ void st_cluster(uint32_t addr, const Msg &m) {
   asm volatile("st.shared::cluster.v2.b64 [%0], {%1, %2};" ::"r"(addr), "l"(a), "l"(b) : "memory");
   asm volatile("st.shared::cluster.v2.b64 [%0], {%1, %2};" ::"r"(addr + 16), "l"(c), "l"(d) : "memory");
 }
+__device__ __forceinline__ uint32_t ld_cluster32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
 __device__ __forceinline__ uint64_t ld_cluster64(uint32_t addr) {
   uint64_t v;
   asm volatile("ld.shared::cluster.b64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
   return v;
 }
+// Dynamic shared memory: the list of noted elements, over it the cluster's bins; sums over this CTA's
+// share of the bins; the CTA's part of the row.  (Reached by the array's name, which lets the compiler
+// see that it is shared memory.)
+__device__ __forceinline__ uint8_t *space() {
+  extern __shared__ __align__(16) uint8_t sample_sm[];
+  return sample_sm;
+}
+__host__ __device__ constexpr uint32_t region(uint32_t ctas) { return kList * 8 > kCtaBins * 4 * ctas ? kList * 8 : kCtaBins * 4 * ctas; }
+
 template <typename T>
 struct alignas(4 * sizeof(T)) Four {
   T v[4];
@@ -103,15 +117,12 @@ template <typename T>
 struct Row {
   const SampleParams &p;
   Small &s;
-  T *x;             // this CTA's part of the row; -inf behind its end
-  uint64_t *list;   // [kList] (ordered value, ~id)
-  uint32_t *hist;   // [bins], over the list
-  double *binsum;   // [kCtaBins] inclusive sums of this CTA's share of the cluster's bins
+  uint32_t x_at;    // where the row is
   uint32_t tid, lane, warp, rank, ctas, bins, groups, mine;  // mine: the thread's first element
   uint32_t id0;     // id of the CTA's first element
   uint32_t turn = 0;
   float mx, cb, last;  // the maximum; bins a unit of x; z = 64 in bins
-  double mxd, c32;     // 32 log2(e) / T
+  double mxd, c512;    // 512 log2(e) / T
   // kept so far: value above cut_at, or equal and id at most cut_id
   float cut_at = -INFINITY;
   uint32_t cut_id = 0xFFFFFFFFu;
@@ -122,27 +133,31 @@ struct Row {
     const double c = 1.4426950408889634074 / (double)t;
     mx = top;
     mxd = (double)top;
-    c32 = 32.0 * c;
+    c512 = 512.0 * c;
     bins = kCtaBins * ctas;
     last = (float)bins;
     cb = (float)c * (last / kOctaves);
   }
   __device__ float z(float v) const { return (mx - v) * cb; }  // in bins
-  // 2^-z in 64 bits, table-driven: 2^(n / 32) from a table, 2^(f / 32), |f| <= 1/2, from the series to
-  // f^5 (the next term is below 2^-48.6).  For z <= 64, so the exponent stays in range.
+  __device__ T *x() const { return reinterpret_cast<T *>(space() + x_at); }                    // -inf behind its end
+  __device__ uint64_t *list() const { return reinterpret_cast<uint64_t *>(space()); }            // [kList] (ordered value, ~id)
+  __device__ uint32_t *hist() const { return reinterpret_cast<uint32_t *>(space()); }            // [bins]
+  __device__ double *binsum() const { return reinterpret_cast<double *>(space() + x_at) - kCtaBins; }  // [kCtaBins], inclusive
+
+  // 2^-z in 64 bits, table-driven: 2^(n / 512) from a table, 2^(f / 512), |f| <= 1/2, from the series to
+  // f^3 (the next term is below 2^-46.7).  For z <= 64, so the exponent stays in range.  The 64-bit
+  // pipe (64 lanes a clock and SM) is what a pass waits for: a table of 32 and the series to f^5
+  // took TIME_A.
   __device__ double weight(float v) const {
     const double d = (double)v - mxd, big = 6755399441055744.0;  // 1.5 * 2^52: the sum's low word is the nearest whole number
-    const double t = fma(d, c32, big);
+    const double t = fma(d, c512, big);
     const int n = __double2loint(t);
-    const double f = fma(d, c32, big - t);
-    double y = 3.97370998454941613e-11;  // (ln 2 / 32)^k / k!
-    y = fma(y, f, 9.17256270182464329e-9);
-    y = fma(y, f, 1.69385097243718201e-6);
-    y = fma(y, f, 0.000234596198202246789);
-    y = fma(y, f, 0.0216608493924982909);
-    y = fma(y, f, 1.0);
-    y *= s.power[n & 31];
-    return __hiloint2double(__double2hiint(y) + ((n >> 5) << 20), __double2loint(y));
+    const double f = fma(d, c512, big - t);
+    double y = 4.13537835067671388e-10;  // (ln 2 / 512)^k / k!
+    y = fma(y, f, 9.16391399227526521e-7);
+    y = fma(y, f, 0.00135380308703114318);
+    y = fma(y, f, 1.0) * s.power[n & 511];
+    return __hiloint2double(__double2hiint(y) + ((n >> 9) << 20), __double2loint(y));
   }
   template <bool CUT>
   __device__ bool kept(float v, uint32_t id) const {
@@ -158,7 +173,7 @@ struct Row {
       if (!use[j]) w[j] = 0.0;
   }
   __device__ void load(uint32_t at, float (&v)[4]) const {
-    const Four<T> f = *reinterpret_cast<const Four<T> *>(x + at);
+    const Four<T> f = *reinterpret_cast<const Four<T> *>(x() + at);
 #pragma unroll
     for (uint32_t j = 0; j < 4; ++j) v[j] = to_f32(f.v[j]);
   }
@@ -251,13 +266,13 @@ struct Row {
 
   __device__ uint32_t bin_of(float zv) const { return min((uint32_t)zv, bins - 1); }
   __device__ void clear() {
-    for (uint32_t i = tid; i < bins; i += kThreads) hist[i] = 0;
+    for (uint32_t i = tid; i < bins; i += kThreads) hist()[i] = 0;
     __syncthreads();
   }
   // histogram of the elements' counts
   __device__ void fill_counts() {
     clear();
-    each<false>([&](float v, uint32_t) { atomicAdd(hist + bin_of(z(v)), 1u); });
+    each<false>([&](float v, uint32_t) { atomicAdd(hist() + bin_of(z(v)), 1u); });
   }
   // of the masses of those kept, where elements above z_most only count for the whole mass, which is returned
   template <bool CUT>
@@ -274,105 +289,132 @@ struct Row {
         const float zv = z(v[j]);
         if (!use[j] || zv > z_most) continue;
         const uint32_t b = bin_of(zv);
-        atomicAdd(hist + b, __float2uint_rn(exp2f(((float)b - zv) * unit) * 32768.0f));
+        atomicAdd(hist() + b, __float2uint_rn(exp2f(((float)b - zv) * unit) * 32768.0f));
       }
     });
     return sum(w);
   }
-  // The cluster's sums over bins: each CTA takes a share of the bins, two a thread.  Returns that share's total.
+  // The cluster's sums over bins: each CTA takes a share of the bins, one a thread.  Returns that share's total.
   template <bool MASS>
   __device__ double reduce_bins() {
-    static_assert(kCtaBins == 2 * kThreads, "two bins a thread");
+    static_assert(kCtaBins == kThreads, "a bin a thread");
     cluster_sync();
-    const uint32_t b = rank * kCtaBins + 2 * tid;
-    uint64_t h[kMaxCtas], t[2] = {0, 0};
+    const uint32_t b = rank * kCtaBins + tid;
+    uint32_t h[kMaxCtas];
 #pragma unroll
-    for (uint32_t r = 0; r < kMaxCtas; ++r) h[r] = r < ctas ? ld_cluster64(dsmem_addr(hist + b, r)) : 0;
+    for (uint32_t r = 0; r < kMaxCtas; ++r) h[r] = r < ctas ? ld_cluster32(dsmem_addr(hist() + b, r)) : 0;
+    uint64_t t = 0;
 #pragma unroll
-    for (uint32_t r = 0; r < kMaxCtas; ++r) {
-      t[0] += (uint32_t)h[r];
-      t[1] += h[r] >> 32;
-    }
-    double v[2] = {(double)t[0], (double)t[1]};
-    if (MASS) {  // in units of 2^-15 of the bin's largest weight
-      v[0] *= exp2((double)b * (-(double)kOctaves / bins) - 15.0);
-      v[1] *= exp2((double)(b + 1) * (-(double)kOctaves / bins) - 15.0);
-    }
-    double total;
-    const double in = scan(v[0] + v[1], total);
-    binsum[2 * tid] = in - v[1];
-    binsum[2 * tid + 1] = in;
+    for (uint32_t r = 0; r < kMaxCtas; ++r) t += h[r];
+    double v = (double)t, total;
+    if (MASS) v *= exp2((double)b * (-(double)kOctaves / bins) - 15.0);  // counted in 2^-15 of the bin's largest weight
+    binsum()[tid] = scan(v, total);
     return total;
   }
-  // the first bins whose inclusive sums reach two targets, the first not above the second (the last bin where none does)
+  // The first bins whose inclusive sums reach two targets (the last bin where none does): the CTA by what all
+  // have said, then its warp and that one's lane, read from there by a warp for each target.  (Read whole
+  // by every CTA, the 4 KB of that one CTA took 3 us.)
   __device__ void find_bins(const Msg *all, const double (&target)[2], uint32_t (&b)[2]) {
-    double before[2];
-    uint32_t r[2];
-    const double mine_a = lane < ctas ? all[lane].a : 0.0, in = lanes_scan(mine_a);
-#pragma unroll
-    for (uint32_t i = 0; i < 2; ++i) {
-      r[i] = min((uint32_t)__popc(__ballot_sync(0xFFFFFFFFu, lane < ctas && in < target[i])), ctas - 1);
-      before[i] = __shfl_sync(0xFFFFFFFFu, in - mine_a, r[i]);
+    if (warp < 2) {
+      const double to = target[warp], of_cta = lane < ctas ? all[lane].a : 0.0, in = lanes_scan(of_cta);
+      const uint32_t r = min((uint32_t)__popc(__ballot_sync(0xFFFFFFFFu, lane < ctas && in < to)), ctas - 1);
+      const double before = __shfl_sync(0xFFFFFFFFu, in - of_cta, r);
+      const double *far = binsum();
+      auto at = [&](uint32_t i) { return before + __longlong_as_double((long long)ld_cluster64(dsmem_addr(far + i, r))); };
+      const double ends = at(min(lane, kWarps - 1) * 32 + 31);
+      const uint32_t w = min((uint32_t)__popc(__ballot_sync(0xFFFFFFFFu, lane < kWarps && ends < to)), kWarps - 1);
+      const uint32_t l = min((uint32_t)__popc(__ballot_sync(0xFFFFFFFFu, at(w * 32 + lane) < to)), 31u);
+      if (lane == 0) s.bins[warp] = r * kCtaBins + w * 32 + l;
     }
-    if (tid < 2) s.bins[tid] = kCtaBins - 1;
     __syncthreads();
-    double v[2][2];
-#pragma unroll
-    for (uint32_t i = 0; i < 2; ++i)
-#pragma unroll
-      for (uint32_t j = 0; j < 2; ++j)
-        v[i][j] = __longlong_as_double((long long)ld_cluster64(dsmem_addr(binsum + tid + j * kThreads, r[i])));
-#pragma unroll
-    for (uint32_t i = 0; i < 2; ++i)
-#pragma unroll
-      for (uint32_t j = 0; j < 2; ++j) {
-        const uint32_t ok = __ballot_sync(0xFFFFFFFFu, before[i] + v[i][j] >= target[i]);
-        if (ok && lane == __ffs(ok) - 1) atomicMin(&s.bins[i], tid + j * kThreads);
-      }
-    __syncthreads();
-    b[0] = r[0] * kCtaBins + s.bins[0];
-    b[1] = r[1] * kCtaBins + s.bins[1];
+    b[0] = s.bins[0];
+    b[1] = s.bins[1];
     __syncthreads();
   }
   __device__ void note(uint32_t key, uint32_t id) {
     if (*reinterpret_cast<volatile uint32_t *>(&s.count) >= kList) return;  // a list that is full is of no use
     const uint32_t at = atomicAdd(&s.count, 1u);
-    if (at < kList) list[at] = (uint64_t)key << 32 | (uint32_t)~id;
+    if (at < kList) list()[at] = (uint64_t)key << 32 | (uint32_t)~id;
   }
-  // Sorts list[0 .. some) in descending order, entries all different but for zeros; behind them zeros to the
-  // next power of two.  Up to 256 by counting the larger ones, with two threads an entry or more: four
-  // barriers (a bitonic sort of 256: 36).
-  __device__ void sort(uint32_t some) {
-    if (some <= 256) {
-      uint32_t log = 1;
-      while (log < 5 && some << (log + 1) <= kThreads) ++log;
-      const uint32_t i = tid >> log, step = 1u << log;
-      uint64_t e = 0;
-      uint32_t place = 0;
+  // Sorts list[0 .. n) in descending order, entries all different but for zeros, which come last.  By buckets:
+  // the high words' range is cut into 1024 parts, entries are placed by the sums over those, and within a
+  // bucket by counting the larger ones; ten barriers.  Where a bucket is large (values that are equal, or nearly)
+  // by the bitonic network, 55 steps for 1024.
+  __device__ void sort(uint32_t n) {
+    uint32_t *count = reinterpret_cast<uint32_t *>(binsum());  // [1024], of no other use by now
+    static_assert(kCtaBins * 8 >= kSort * 4 && kSort == 2 * kThreads && kList >= 2 * kSort, "room to sort in");
+    uint64_t e[2];
+    uint32_t lo = 0xFFFFFFFFu, hi = 0, some = 0, o = 0;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t j = 0; j < 2; ++j) {
+      const uint32_t i = tid + j * kThreads;
+      e[j] = i < n ? list()[i] : 0;
+      count[i] = 0;
+      if (!e[j]) continue;
+      ++some;
+      lo = min(lo, (uint32_t)(e[j] >> 32));
+      hi = max(hi, (uint32_t)(e[j] >> 32));
+    }
+    sums(some, o, lo, hi);
+    const uint32_t shift = hi - lo < kSort ? 0 : 22 - __clz(hi - lo);  // (hi - lo) >> shift < 1024
+    uint32_t at[2] = {0, 0}, order[2] = {0, 0}, most = 0;
+#pragma unroll
+    for (uint32_t j = 0; j < 2; ++j)
+      if (e[j]) order[j] = atomicAdd(count + (at[j] = (hi - (uint32_t)(e[j] >> 32)) >> shift), 1u);
+    __syncthreads();
+    const uint2 c = reinterpret_cast<const uint2 *>(count)[tid];
+    most = __reduce_max_sync(0xFFFFFFFFu, max(c.x, c.y));
+    uint32_t in = c.x + c.y;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const uint32_t y = __shfl_up_sync(0xFFFFFFFFu, in, d);
+      if (lane >= (uint32_t)d) in += y;
+    }
+    if (lane == 31) {
+      s.redu[0][warp] = in;
+      s.redu[1][warp] = most;
+    }
+    __syncthreads();
+    const uint32_t before = __reduce_add_sync(0xFFFFFFFFu, lane < warp ? s.redu[0][lane % kWarps] : 0);
+    most = __reduce_max_sync(0xFFFFFFFFu, s.redu[1][lane % kWarps]);
+    if (most <= 16) {
+      in += before;
+      reinterpret_cast<uint2 *>(count)[tid] = make_uint2(in - c.x - c.y, in - c.y);  // exclusive
       __syncthreads();
-      if (i < some) {
-        e = list[i];
-        for (uint32_t j = tid & (step - 1); j < some; j += step) place += list[j] > e;
+      uint64_t *part = list() + kSort;
+      uint32_t first[2], end[2];
+#pragma unroll
+      for (uint32_t j = 0; j < 2; ++j) {
+        first[j] = e[j] ? count[at[j]] : 0;
+        end[j] = e[j] ? at[j] + 1 < kSort ? count[at[j] + 1] : some : 0;
+        if (e[j]) part[first[j] + order[j]] = e[j];
+        if (tid + j * kThreads < n) list()[tid + j * kThreads] = 0;
       }
-      for (uint32_t o = 1; o < step; o <<= 1) place += __shfl_xor_sync(0xFFFFFFFFu, place, o);
       __syncthreads();
-      if (tid < some) list[tid] = 0;
-      __syncthreads();
-      if (e && (tid & (step - 1)) == 0) list[place] = e;
+#pragma unroll
+      for (uint32_t j = 0; j < 2; ++j) {
+        uint32_t place = first[j];
+        for (uint32_t i = first[j]; i < end[j]; ++i) place += part[i] > e[j];
+        if (e[j]) list()[place] = e[j];
+      }
       __syncthreads();
       return;
     }
-    uint32_t n = 2;
-    while (n < some) n <<= 1;
-    for (uint32_t k = 2; k <= n; k <<= 1)
+    uint32_t n2 = 2;
+    while (n2 < n) n2 <<= 1;
+#pragma unroll
+    for (uint32_t j = 0; j < 2; ++j)
+      if (tid + j * kThreads < n2) list()[tid + j * kThreads] = e[j];  // zeros behind the last
+    for (uint32_t k = 2; k <= n2; k <<= 1)
       for (uint32_t j = k >> 1; j; j >>= 1) {
         __syncthreads();
-        if (tid < n / 2) {
+        if (tid < n2 / 2) {
           const uint32_t i = (tid / j) * 2 * j + tid % j;
-          const uint64_t a = list[i], b = list[i + j];
+          const uint64_t a = list()[i], b = list()[i + j];
           if ((a < b) == ((i & k) == 0)) {
-            list[i] = b;
-            list[i + j] = a;
+            list()[i] = b;
+            list()[i + j] = a;
           }
         }
       }
@@ -390,12 +432,12 @@ struct Row {
         if (i >= n) continue;
         uint32_t r = 0;
         while (i >= all[r].c) i -= all[r++].c;
-        mine[e] = ld_cluster64(dsmem_addr(list + i, r));
+        mine[e] = ld_cluster64(dsmem_addr(list() + i, r));
       }
     cluster_sync();
     if (rank) return false;
-    list[tid] = mine[0];
-    list[tid + kThreads] = mine[1];
+    list()[tid] = mine[0];
+    list()[tid + kThreads] = mine[1];
     sort(n);
     return true;
   }
@@ -411,7 +453,7 @@ struct Row {
   // The rest of a row whose candidates are all in CTA 0's sorted list: the first k of
   // them, of those the beginning with the mass p * whole (whole < 0: their own), min-p, the draw.
   __device__ void finish_list(uint32_t row, uint32_t n, uint32_t k, double pp, double whole, double min_p, double u) {
-    const uint64_t e[2] = {list[2 * tid], list[2 * tid + 1]};
+    const uint64_t e[2] = {list()[2 * tid], list()[2 * tid + 1]};
     double w[2];
 #pragma unroll
     for (uint32_t j = 0; j < 2; ++j) w[j] = 2 * tid + j < min(n, k) ? list_weight(e[j]) : 0.0;
@@ -423,10 +465,10 @@ struct Row {
       const uint32_t i = 2 * tid + j;
       const double before = j ? in - w[1] : in - w[1] - w[0];
       const bool stay = i < min(n, k) && (i == 0 || pp >= 1.0 || before < target) && w[j] >= min_p && w[j] > 0;
-      list[i] = stay ? (e[j] & 0xFFFFFFFFull) << 32 | (uint32_t)(e[j] >> 32) : 0;  // (~id, value): by id
+      list()[i] = stay ? (e[j] & 0xFFFFFFFFull) << 32 | (uint32_t)(e[j] >> 32) : 0;  // (~id, value): by id
     }
     sort(n);
-    const uint64_t f[2] = {list[2 * tid], list[2 * tid + 1]};
+    const uint64_t f[2] = {list()[2 * tid], list()[2 * tid + 1]};
 #pragma unroll
     for (uint32_t j = 0; j < 2; ++j) w[j] = f[j] ? weight(key_float((uint32_t)f[j])) : 0.0;
     const double incl = scan(w[0] + w[1], total), at = u * total;
@@ -487,7 +529,7 @@ struct Row {
         e[j] = 0;
         if (i >= n) continue;
         while (i >= all[r].d) i -= all[r++].d;
-        e[j] = ld_cluster64(dsmem_addr(list + i, r));
+        e[j] = ld_cluster64(dsmem_addr(list() + i, r));
       }
     cluster_sync();
     if (rank) return;
@@ -511,13 +553,13 @@ struct Row {
       if (c >= k && c <= 256) break;
     }
     if (tid == 0) s.count = 0;
-    for (uint32_t i = tid; i < kSort; i += kThreads) list[i] = 0;
+    for (uint32_t i = tid; i < kSort; i += kThreads) list()[i] = 0;
     __syncthreads();
 #pragma unroll
     for (uint32_t j = 0; j < kPer; ++j)
       if (e[j] && (uint32_t)(e[j] >> 32) >= lo) {
         const uint32_t at = atomicAdd(&s.count, 1u);
-        if (at < kSort) list[at] = e[j];
+        if (at < kSort) list()[at] = e[j];
       }
     __syncthreads();
     uint32_t m = s.count;
@@ -534,11 +576,11 @@ struct Row {
         if (c == k) break;
       }
       if (tid == 0) s.count = 0;
-      for (uint32_t i = tid; i < kSort; i += kThreads) list[i] = 0;
+      for (uint32_t i = tid; i < kSort; i += kThreads) list()[i] = 0;
       __syncthreads();
 #pragma unroll
       for (uint32_t j = 0; j < kPer; ++j)
-        if (e[j] && e[j] >= a) list[atomicAdd(&s.count, 1u)] = e[j];
+        if (e[j] && e[j] >= a) list()[atomicAdd(&s.count, 1u)] = e[j];
       __syncthreads();
       m = s.count;
       __syncthreads();
@@ -686,7 +728,7 @@ struct Row {
     uint32_t n;
     Msg place{};
     if (gather(all, n)) {
-      const uint64_t e[2] = {list[2 * tid], list[2 * tid + 1]};
+      const uint64_t e[2] = {list()[2 * tid], list()[2 * tid + 1]};
       double w[2];
 #pragma unroll
       for (uint32_t j = 0; j < 2; ++j) w[j] = 2 * tid + j >= n ? 0.0 : MASS ? list_weight(e[j]) : 1.0;
@@ -697,7 +739,7 @@ struct Row {
       if (2 * tid < n && A + (in - w[1]) >= target) atomicMin(&s.bin, 2 * tid);
       else if (2 * tid + 1 < n && A + in >= target) atomicMin(&s.bin, 2 * tid + 1);
       __syncthreads();
-      const uint64_t at = list[s.bin];
+      const uint64_t at = list()[s.bin];
       place.c = (uint32_t)(at >> 32);
       place.d = ~(uint32_t)at;
     }
@@ -753,7 +795,7 @@ struct Row {
       for (uint32_t j = 0; j < 4; ++j)
         if (w[j] < min_p) w[j] = 0.0;
     };
-    double *of_group = reinterpret_cast<double *>(list);
+    double *of_group = reinterpret_cast<double *>(list());
     float v[4];
     double w[4];
     for (uint32_t g = warp; g < groups; g += kWarps) {
@@ -783,12 +825,8 @@ struct Row {
   }
 };
 
-// bytes of the list, or the bins over it
-__host__ __device__ constexpr uint32_t region(uint32_t ctas) { return kList * 8 > kCtaBins * 4 * ctas ? kList * 8 : kCtaBins * 4 * ctas; }
-
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 2) k_sample_logits(const SampleParams p) {
-  extern __shared__ __align__(16) uint8_t dsm[];
   __shared__ Small s;
   const uint32_t ctas = p.ctas, row = blockIdx.x / ctas;
   Row<T> w(p, s);
@@ -798,13 +836,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_logits(const SampleParam
   w.rank = cluster_ctarank();
   w.ctas = ctas;
   w.groups = p.groups;
-  w.list = reinterpret_cast<uint64_t *>(dsm);
-  w.hist = reinterpret_cast<uint32_t *>(dsm);
-  w.binsum = reinterpret_cast<double *>(dsm + region(ctas));
-  w.x = reinterpret_cast<T *>(dsm + region(ctas) + kCtaBins * 8);
+  w.x_at = region(ctas) + kCtaBins * 8;
   w.id0 = w.rank * p.slice;
   w.mine = w.warp * 128 * p.groups + 4 * w.lane;
-  if (w.tid < 32) s.power[w.tid] = exp2((double)w.tid / 32.0);
+  s.power[w.tid] = exp2((double)w.tid / 512.0);
   const uint32_t at = p.rows ? p.rows[row] : row;
   if (at == FA_NO_TOKEN) return;
   // the row's own settings: on their way while the logits are read
@@ -830,7 +865,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_logits(const SampleParam
           if (j0 + a * kThreads >= whole) break;
           clean(v[a].x, v[a].y, mx);
           clean(v[a].z, v[a].w, mx);
-          *reinterpret_cast<float4 *>(w.x + (j0 + a * kThreads) * kV) = v[a];
+          *reinterpret_cast<float4 *>(w.x() + (j0 + a * kThreads) * kV) = v[a];
         }
       }
     } else {
@@ -855,7 +890,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_logits(const SampleParam
           e.u = v[a];
 #pragma unroll
           for (uint32_t i2 = 0; i2 < 4; ++i2) clean2(e.p[i2], zero, none, most);
-          *reinterpret_cast<uint4 *>(w.x + (j0 + a * kThreads) * kV) = e.u;
+          *reinterpret_cast<uint4 *>(w.x() + (j0 + a * kThreads) * kV) = e.u;
         }
       }
       mx = fmaxf(to_f32(most.x), to_f32(most.y));
@@ -864,7 +899,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_logits(const SampleParam
   }
   for (uint32_t j = i + w.tid; j < room; j += kThreads) {
     const T f = j < len ? clean(src[j]) : (T)(-INFINITY);
-    w.x[j] = f;
+    w.x()[j] = f;
     mx = fmaxf(mx, to_f32(f));
   }
   mx = to_f32(mx);

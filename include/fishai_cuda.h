@@ -588,7 +588,7 @@ int fa_sampler_freq(fa_sampler *s, uint32_t seq, uint32_t token, uint32_t *count
  * Refused, with FA_FLAG_RANGE: a row >= n_logits, a temperature that is not 0 or 1e-6
  * to 1e6, u outside [0, 1), top_p < 0, min_p outside [0, 1], NaN; ids[i] is left as it
  * was.  A row without candidates gives FA_NO_TOKEN, -inf and FA_FLAG_RANGE.
- * vocab <= 360448, n <= 2^20.  Device, stream, capture and err as for the operators
+ * vocab <= 393216, n <= 2^20.  Device, stream, capture and err as for the operators
  * on pages; no workspace. */
 int fa_sample_logits(const void *logits, int32_t dtype, uint64_t ld, uint32_t n_logits, uint32_t vocab, const uint32_t *rows, uint32_t n,
                      const float *temperature, const uint32_t *top_k, const float *top_p, const float *min_p, const float *u, uint32_t *ids,

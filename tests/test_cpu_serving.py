@@ -131,7 +131,7 @@ def call_sample(logits=P, dt=L.KV_F32, ld=100, m=3, vocab=100, rows=P, n=4, t=P,
     return L.lib().fa_sample_logits(logits, dt, ld, m, vocab, rows, n, t, k, p, mp, u, ids, logs, None, None)
 
 
-@pytest.mark.parametrize("bad", [dict(dt=3), dict(vocab=0), dict(vocab=360449, ld=1 << 20), dict(n=(1 << 20) + 1), dict(ld=99), dict(rows=None), dict(m=0),
+@pytest.mark.parametrize("bad", [dict(dt=3), dict(vocab=0), dict(vocab=393217, ld=1 << 20), dict(n=(1 << 20) + 1), dict(ld=99), dict(rows=None), dict(m=0),
                                  dict(logits=None), dict(u=None), dict(ids=None), dict(logits=P + 2), dict(u=P + 1), dict(ids=P + 2), dict(rows=P + 3),
                                  dict(t=P + 1), dict(k=P + 1), dict(p=P + 1), dict(mp=P + 1), dict(logs=P + 1)], ids=str)
 def test_sample_logits_refuses(bad):
