@@ -46,24 +46,14 @@ struct Small {
   double power[512];  // 2^(i / 512)
 };
 
-// Two logits as they are kept: NaN as -inf, -0 as +0.  In f32 (to_f32) +inf is the largest number.
-__device__ __forceinline__ void clean(float &a, float &b, float &most) {
-  a = fmaxf(a, -INFINITY) + 0.0f;
-  b = fmaxf(b, -INFINITY) + 0.0f;
-  most = fmaxf(most, fmaxf(a, b));
-}
-template <typename T2>
-__device__ __forceinline__ void clean2(T2 &x, T2 zero, T2 none, T2 &most) {
-  x = __hadd2(__hmax2(x, none), zero);
-  most = __hmax2(most, x);
-}
-template <typename T>
-__device__ __forceinline__ T clean(T x) {
-  return (T)(fmaxf((float)x, -INFINITY) + 0.0f);
-}
-template <typename T>
-__device__ __forceinline__ float to_f32(T x) {
-  return fminf((float)x, 3.402823466e38f);
+// the larger of both, NaN beside a number left out
+__device__ __forceinline__ __half2 larger(__half2 a, __half2 b) { return __hmax2(a, b); }
+__device__ __forceinline__ __nv_bfloat162 larger(__nv_bfloat162 a, __nv_bfloat162 b) { return __hmax2(a, b); }
+__device__ __forceinline__ uint32_t key_of(float v) { return float_key(v + 0.0f); }  // -0 as +0
+__device__ __forceinline__ float ex2(float x) {  // 2^x, 2 ulp
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 __device__ __forceinline__ double lanes_sum(double v) {
 #pragma unroll
@@ -71,16 +61,26 @@ __device__ __forceinline__ double lanes_sum(double v) {
   return v;
 }
 
+// how the maximum is kept while a row is read: in pairs for 16-bit types
 template <typename T>
-struct Pair;
+struct Pair {
+  using type = float;
+  __device__ static float none() { return -INFINITY; }
+  __device__ static float top(float x) { return x; }
+};
 template <>
 struct Pair<__half> {
   using type = __half2;
+  __device__ static __half2 none() { return __float2half2_rn(-INFINITY); }
+  __device__ static float top(__half2 x) { return fmaxf(__low2float(x), __high2float(x)); }
 };
 template <>
 struct Pair<__nv_bfloat16> {
   using type = __nv_bfloat162;
+  __device__ static __nv_bfloat162 none() { return __float2bfloat162_rn(-INFINITY); }
+  __device__ static float top(__nv_bfloat162 x) { return fmaxf(__low2float(x), __high2float(x)); }
 };
+__device__ __forceinline__ float larger(float a, float b) { return fmaxf(a, b); }
 
 __device__ __forceinline__ void st_cluster(uint32_t addr, const Msg &m) {
   const uint64_t a = __double_as_longlong(m.a), b = __double_as_longlong(m.b), c = (uint64_t)m.d << 32 | m.c, d = (uint64_t)m.f << 32 | m.e;
@@ -121,7 +121,7 @@ struct Row {
   uint32_t tid, lane, warp, rank, ctas, bins, groups, mine;  // mine: the thread's first element
   uint32_t id0;     // id of the CTA's first element
   uint32_t turn = 0;
-  float mx, cb, last;  // the maximum; bins a unit of x; z = 64 in bins
+  float mx, cb, low;   // the maximum; bins a unit of x; where z = 64 (to f32's rounding): below it and NaN is no candidate
   double mxd, c512;    // 512 log2(e) / T
   // kept so far: value above cut_at, or equal and id at most cut_id
   float cut_at = -INFINITY;
@@ -135,8 +135,8 @@ struct Row {
     mxd = (double)top;
     c512 = 512.0 * c;
     bins = kCtaBins * ctas;
-    last = (float)bins;
-    cb = (float)c * (last / kOctaves);
+    cb = (float)(c * (bins / kOctaves));
+    low = __double2float_ru(mxd - (double)kOctaves / c);  // upwards: weight() needs z <= 64
   }
   __device__ float z(float v) const { return (mx - v) * cb; }  // in bins
   __device__ T *x() const { return reinterpret_cast<T *>(space() + x_at); }                    // -inf behind its end
@@ -161,21 +161,17 @@ struct Row {
   }
   template <bool CUT>
   __device__ bool kept(float v, uint32_t id) const {
-    return z(v) <= last && (!CUT || v > cut_at || (v == cut_at && id <= cut_id));
+    return v >= low && (!CUT || v > cut_at || (v == cut_at && id <= cut_id));
   }
-  // Four values at once, without a branch: their chains of dependent operations run side by side.  Where
-  // use[j] is false, 0.
-  __device__ void weights(const float (&v)[4], const bool (&use)[4], double (&w)[4]) const {
+  // Four values at once, without a branch: their chains of dependent operations run side by side.
+  __device__ void weights(const float (&v)[4], double (&w)[4]) const {
 #pragma unroll
     for (uint32_t j = 0; j < 4; ++j) w[j] = weight(v[j]);
-#pragma unroll
-    for (uint32_t j = 0; j < 4; ++j)
-      if (!use[j]) w[j] = 0.0;
   }
   __device__ void load(uint32_t at, float (&v)[4]) const {
     const Four<T> f = *reinterpret_cast<const Four<T> *>(x() + at);
 #pragma unroll
-    for (uint32_t j = 0; j < 4; ++j) v[j] = to_f32(f.v[j]);
+    for (uint32_t j = 0; j < 4; ++j) v[j] = (float)f.v[j];
   }
   // f(values, which are kept, first id) of the thread's groups of four, in the order of ids
   template <bool CUT, typename F>
@@ -264,7 +260,7 @@ struct Row {
     return warp ? before + v : v;
   }
 
-  __device__ uint32_t bin_of(float zv) const { return min((uint32_t)zv, bins - 1); }
+  __device__ uint32_t bin_of(float zv) const { return min((uint32_t)zv, bins - 1); }  // (low may be a rounding beyond the last)
   __device__ void clear() {
     for (uint32_t i = tid; i < bins; i += kThreads) hist()[i] = 0;
     __syncthreads();
@@ -279,17 +275,17 @@ struct Row {
   __device__ double fill_masses(float z_most) {
     clear();
     double w = 0;
-    const float unit = kOctaves / last;
+    const float unit = kOctaves / bins;
     each4<CUT>([&](const float (&v)[4], const bool (&use)[4], uint32_t) {
       double e[4];
-      weights(v, use, e);
-      w += (e[0] + e[1]) + (e[2] + e[3]);
+      weights(v, e);
 #pragma unroll
       for (uint32_t j = 0; j < 4; ++j) {
+        if (use[j]) w += e[j];
         const float zv = z(v[j]);
         if (!use[j] || zv > z_most) continue;
         const uint32_t b = bin_of(zv);
-        atomicAdd(hist() + b, __float2uint_rn(exp2f(((float)b - zv) * unit) * 32768.0f));
+        atomicAdd(hist() + b, __float2uint_rn(ex2(fmaf((float)b - zv, unit, 15.0f))));
       }
     });
     return sum(w);
@@ -443,7 +439,7 @@ struct Row {
   }
   __device__ double list_weight(uint64_t e) const {
     const float v = key_float((uint32_t)(e >> 32));
-    return e && z(v) <= last ? weight(v) : 0.0;
+    return e && v >= low ? weight(v) : 0.0;
   }
 
   __device__ void answer(uint32_t row, uint32_t id, double prob) {
@@ -493,7 +489,7 @@ struct Row {
 
   // Notes this CTA's elements from the k-th largest of its threads' maxima on: what the row's first k are among.
   __device__ void note_largest(float best, uint32_t k) {
-    const uint32_t key = float_key(best);
+    const uint32_t key = key_of(best);
     const bool some = best > -INFINITY;
     uint32_t o1 = 0, have = some, lo = some ? key : 0xFFFFFFFFu, hi = key;
     sums(have, o1, lo, hi);
@@ -514,7 +510,7 @@ struct Row {
       const uint32_t id = id0 + mine + 128 * g;
 #pragma unroll
       for (uint32_t j = 0; j < 4; ++j)
-        if (v[j] >= from) note(float_key(v[j]), id + j);
+        if (v[j] >= from) note(key_of(v[j]), id + j);
     }
     __syncthreads();
   }
@@ -613,7 +609,7 @@ struct Row {
         any |= over[j];
         above += over[j];
         if (use[j] && !over[j] && zv < z1) {
-          const uint32_t key = float_key(v[j]);
+          const uint32_t key = key_of(v[j]);
           note(key, id + j);
           ++m;
           kmin = min(kmin, key);
@@ -622,11 +618,12 @@ struct Row {
       }
       if (MASS && any) {
         double w[4];
-        weights(v, over, w);
-        a += (w[0] + w[1]) + (w[2] + w[3]);
+        weights(v, w);
 #pragma unroll
-        for (uint32_t j = 0; j < 4; ++j)
-          if (w[j] >= min_p) strict += w[j];
+        for (uint32_t j = 0; j < 4; ++j) {
+          if (over[j]) a += w[j];
+          if (over[j] && w[j] >= min_p) strict += w[j];
+        }
       }
     });
     sums(above, m, kmin, kmax);
@@ -639,7 +636,7 @@ struct Row {
     kmax = __reduce_max_sync(0xFFFFFFFFu, all[l].f);
     if (total <= kSort) {  // all of them to the list
       each<CUT>([&](float v, uint32_t id) {
-        if (z(v) < z0) note(float_key(v), id);
+        if (z(v) < z0) note(key_of(v), id);
       });
       __syncthreads();
       all = share(Msg{0, 0, s.count, 0, 0, 0});
@@ -655,7 +652,7 @@ struct Row {
       double b = 0;
       uint32_t up = 0, o1 = 0, o2 = 0, o3 = 0;
       each<CUT>([&](float v, uint32_t) {
-        const uint32_t key = float_key(v);
+        const uint32_t key = key_of(v);
         if (key < mid || key > kmax) return;
         ++up;
         if (MASS) b += weight(v);
@@ -678,7 +675,7 @@ struct Row {
       const double w = MASS ? weight(key_float(kmin)) : 1.0, ratio = ceil((target - A) / w);
       const uint32_t need = ratio < 1.0 ? 1 : ratio >= (double)m ? m : (uint32_t)ratio;
       uint32_t own = 0, o1 = 0, o2 = 0, o3 = 0;
-      each<CUT>([&](float v, uint32_t) { own += float_key(v) == kmin; });
+      each<CUT>([&](float v, uint32_t) { own += key_of(v) == kmin; });
       // by ids: CTAs, warps, groups of a warp, lanes
       const uint32_t of_warp = __reduce_add_sync(0xFFFFFFFFu, own);
       sums(own, o1, o2, o3);  // leaves the warps' sums of `own`
@@ -694,7 +691,7 @@ struct Row {
           bool yes[4];
           uint32_t n = 0;
 #pragma unroll
-          for (uint32_t j = 0; j < 4; ++j) n += yes[j] = kept<CUT>(e[j], id + j) && float_key(e[j]) == kmin;
+          for (uint32_t j = 0; j < 4; ++j) n += yes[j] = kept<CUT>(e[j], id + j) && key_of(e[j]) == kmin;
           uint32_t in = n;
 #pragma unroll
           for (int o = 1; o < 32; o <<= 1) {
@@ -719,7 +716,7 @@ struct Row {
       if (tid == 0) s.count = 0;
       __syncthreads();
       each<CUT>([&](float v, uint32_t id) {
-        const uint32_t key = float_key(v);
+        const uint32_t key = key_of(v);
         if (key >= kmin && key <= kmax) note(key, id);
       });
     }
@@ -771,10 +768,10 @@ struct Row {
       }
       if (CUT && !any) return;
       double w[4];
-      weights(v, add, w);
+      weights(v, w);
 #pragma unroll
       for (uint32_t j = 0; j < 4; ++j)
-        if (w[j] >= min_p) own += w[j];
+        if (add[j] && w[j] >= min_p) own += w[j];
     });
     const Msg *all = share(Msg{sum(own), 0, 0, 0, 0, 0});  // the warps' sums stay in s.red
     const double M = all_a(all);
@@ -790,10 +787,10 @@ struct Row {
       bool use[4];
 #pragma unroll
       for (uint32_t j = 0; j < 4; ++j) use[j] = kept<CUT>(v[j], id + j);
-      weights(v, use, w);
+      weights(v, w);
 #pragma unroll
       for (uint32_t j = 0; j < 4; ++j)
-        if (w[j] < min_p) w[j] = 0.0;
+        if (!use[j] || w[j] < min_p) w[j] = 0.0;
     };
     double *of_group = reinterpret_cast<double *>(list());
     float v[4];
@@ -854,71 +851,49 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_logits(const SampleParam
   if (p.aligned) {
     const uint32_t whole = len / kV;
     constexpr uint32_t kAhead = sizeof(T) == 4 ? 8 : 4;  // loads in flight
-    if constexpr (sizeof(T) == 4) {
-      for (uint32_t j0 = w.tid; j0 < whole; j0 += kAhead * kThreads) {
-        float4 v[kAhead];
+    using T2 = typename Pair<T>::type;
+    union Piece {
+      uint4 u;
+      T2 p[16 / sizeof(T2)];
+    };
+    T2 most = Pair<T>::none();
+    for (uint32_t j0 = w.tid; j0 < whole; j0 += kAhead * kThreads) {
+      Piece v[kAhead];
 #pragma unroll
-        for (uint32_t a = 0; a < kAhead; ++a)
-          if (j0 + a * kThreads < whole) v[a] = *reinterpret_cast<const float4 *>(src + (uint64_t)(j0 + a * kThreads) * kV);
+      for (uint32_t a = 0; a < kAhead; ++a)
+        if (j0 + a * kThreads < whole) v[a].u = *reinterpret_cast<const uint4 *>(src + (uint64_t)(j0 + a * kThreads) * kV);
 #pragma unroll
-        for (uint32_t a = 0; a < kAhead; ++a) {
-          if (j0 + a * kThreads >= whole) break;
-          clean(v[a].x, v[a].y, mx);
-          clean(v[a].z, v[a].w, mx);
-          *reinterpret_cast<float4 *>(w.x() + (j0 + a * kThreads) * kV) = v[a];
-        }
+      for (uint32_t a = 0; a < kAhead; ++a) {
+        if (j0 + a * kThreads >= whole) break;
+#pragma unroll
+        for (uint32_t e = 0; e < 16 / sizeof(T2); ++e) most = larger(most, v[a].p[e]);
+        *reinterpret_cast<uint4 *>(w.x() + (j0 + a * kThreads) * kV) = v[a].u;
       }
-    } else {
-      using T2 = typename Pair<T>::type;
-      union Eight {
-        uint4 u;
-        T2 p[4];
-      };
-      T2 zero, none, most;
-      zero.x = zero.y = (T)0.0f;
-      none.x = none.y = (T)(-INFINITY);
-      most = none;
-      for (uint32_t j0 = w.tid; j0 < whole; j0 += kAhead * kThreads) {
-        uint4 v[kAhead];
-#pragma unroll
-        for (uint32_t a = 0; a < kAhead; ++a)
-          if (j0 + a * kThreads < whole) v[a] = *reinterpret_cast<const uint4 *>(src + (uint64_t)(j0 + a * kThreads) * kV);
-#pragma unroll
-        for (uint32_t a = 0; a < kAhead; ++a) {
-          if (j0 + a * kThreads >= whole) break;
-          Eight e;
-          e.u = v[a];
-#pragma unroll
-          for (uint32_t i2 = 0; i2 < 4; ++i2) clean2(e.p[i2], zero, none, most);
-          *reinterpret_cast<uint4 *>(w.x() + (j0 + a * kThreads) * kV) = e.u;
-        }
-      }
-      mx = fmaxf(to_f32(most.x), to_f32(most.y));
     }
+    mx = Pair<T>::top(most);
     i = whole * kV;
   }
   for (uint32_t j = i + w.tid; j < room; j += kThreads) {
-    const T f = j < len ? clean(src[j]) : (T)(-INFINITY);
+    const T f = j < len ? src[j] : (T)(-INFINITY);
     w.x()[j] = f;
-    mx = fmaxf(mx, to_f32(f));
+    mx = fmaxf(mx, (float)f);
   }
-  mx = to_f32(mx);
   // a setting that does not hold leaves the row as it was (the same for all CTAs)
   if (at >= p.n_logits || !(t == 0.0f || (t >= 1e-6f && t <= 1e6f)) || !(u >= 0.0f && u < 1.0f) || !(pp >= 0.0f) || !(mp >= 0.0f && mp <= 1.0f)) {
     if (p.err && w.rank == 0 && w.tid == 0) atomicOr(p.err, kFlagRange);
     return;
   }
-  const bool few = t > 0 && k && k < p.vocab && k <= kFewK;
+  bool few = t > 0 && k && k < p.vocab && k <= kFewK;
   if (few) {
     __syncthreads();
     w.note_largest(mx, k);
   }
-  uint32_t o0 = 0, o1 = 0, o2 = 0, key = float_key(mx);
+  uint32_t o0 = 0, o1 = 0, o2 = 0, key = key_of(mx);
   w.sums(o0, o1, o2, key);
   const Msg *all = w.share(Msg{0, 0, key, few ? s.count : 0, 0, 0});
   key = __reduce_max_sync(0xFFFFFFFFu, all[w.lane % ctas].c);
   const uint32_t noted = __reduce_add_sync(0xFFFFFFFFu, w.lane < ctas ? all[w.lane].d : 0);
-  const float top = key_float(key);
+  float top = key_float(key);
   if (top == -INFINITY) {  // no candidate at all
     if (w.rank == 0 && w.tid == 0) {
       p.ids[row] = FA_NO_TOKEN;
@@ -926,6 +901,16 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_logits(const SampleParam
       if (p.err) atomicOr(p.err, kFlagRange);
     }
     return;
+  }
+  if (top == INFINITY) {  // counts as the largest f32: beside it nothing in 16 bits is a candidate
+    few = false;
+    for (uint32_t j = w.tid; j < room; j += kThreads) {
+      const float f = (float)w.x()[j];
+      if (sizeof(T) == 4) w.x()[j] = (T)(f == INFINITY ? 3.402823466e38f : f);
+      else w.x()[j] = (T)(f == INFINITY ? 0.0f : -INFINITY);
+    }
+    top = sizeof(T) == 4 ? 3.402823466e38f : 0.0f;
+    __syncthreads();
   }
   if (t == 0.0f) {  // the lowest id of the maximum
     uint32_t best = 0xFFFFFFFFu;
@@ -961,7 +946,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_logits(const SampleParam
   }
   if (pp < 1.0f) {
     // all mass above z_most is less than half of what may be cut: the place is below it
-    const float z_most = (log2f((float)p.vocab) - log2f(1.0f - pp) + 1.0f) * (w.last / kOctaves);
+    const float z_most = (log2f((float)p.vocab) - log2f(1.0f - pp) + 1.0f) * (w.bins / kOctaves);
     const double whole = has_cut ? w.template fill_masses<true>(z_most) : w.template fill_masses<false>(z_most);
     const double total = w.template reduce_bins<true>();
     all = w.share(Msg{total, whole, 0, 0, 0, 0});

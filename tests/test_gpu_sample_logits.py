@@ -197,3 +197,24 @@ def test_captured_replayed_and_the_same_bits():
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(ids, first[0]) and torch.equal(logs, first[1])
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+def test_large_logits_and_small_temperatures(t):
+    """the step of the type at the maximum is far above what the temperature tells apart"""
+    big = {"f32": 1e7, "f16": 6e4, "bf16": 1e30}[t]
+    x = logits_of("text", 4, 3000, torch.float32, 11) / 16
+    for scale in (1.0, -1.0):
+        check((big * scale * (1 + x / 4096)).to(TYPES[t]), [0.0, 0.4, 0.8, NEAR_ONE], [1e-6, 1e-3, 1.0, 1e6], [0, 50, 0, 2000], [0.9, 1.0, 0.5, 1.0])
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+def test_infinity_beside_the_largest_number_of_a_type(t):
+    x = logits_of("text", 3, 5000, TYPES[t], 12)
+    x[:, 40] = torch.finfo(TYPES[t]).max
+    x[0, [7, 4000]] = math.inf
+    x[1, 4999] = math.inf
+    x[1, 3] = math.nan
+    for k in (None, [3] * 3, [600] * 3):
+        check(x, [0.2, 0.6, 0.9], [1.0, 0.5, 1.0], k, [0.9, 1.0, 0.7])
+        check(x, [0.2, 0.6, 0.9], [0.0] * 3, k)
