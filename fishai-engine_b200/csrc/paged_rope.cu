@@ -14,6 +14,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <cstring>
+
 #include "fa_device.cuh"
 #include "paged_ops.hpp"
 
@@ -58,6 +60,18 @@ __device__ __forceinline__ void store_n(T *p, const float (&x)[N]) {
     for (int i = 0; i < N; ++i) p[i] = w.v[i];
 }
 
+// 16-bit elements two at a time, from and to a 32-bit word
+__device__ __forceinline__ float2 unpack(const __half *p, uint32_t w) { return __half22float2(*reinterpret_cast<const __half2 *>(&w)); }
+__device__ __forceinline__ float2 unpack(const __nv_bfloat16 *p, uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u)); }
+__device__ __forceinline__ uint32_t pack(const __half *p, float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ uint32_t pack(const __nv_bfloat16 *p, float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+
 // W: pairs of a unit (8 or 4: every address a unit touches is aligned to W
 // elements; 1: any).  A head is hd / (2 W) units: the first rot / (2 W) turn W
 // pairs, the others copy 2 W elements.  A CTA takes `each` tokens (up to 4) and
@@ -67,8 +81,8 @@ __device__ __forceinline__ void store_n(T *p, const float (&x)[N]) {
 // loading after its angles: 46 us for 8192 tokens of 48 heads.)
 constexpr uint32_t kRopeTokens = 4;
 template <typename TI, typename TO, int W, bool AXES>
-__global__ void __launch_bounds__(512) k_rope_append(const RopeAppendParams p, const __grid_constant__ RopeTable tab, uint32_t each) {
-  __shared__ float cs[kRopeTokens][kMaxHeadDim / 2], sn[kRopeTokens][kMaxHeadDim / 2];
+__global__ void __launch_bounds__(512, 3) k_rope_append(const RopeAppendParams p, const __grid_constant__ RopeTable tab, uint32_t each) {
+  __shared__ __align__(16) float cs[kRopeTokens][kMaxHeadDim / 2], sn[kRopeTokens][kMaxHeadDim / 2];
   __shared__ uint64_t place[kRopeTokens];  // element offset of the token's slot in a (K, head 0) block
   const uint32_t hd = p.pg.head_dim, half = p.rot / 2, H = p.n_heads, KVH = p.pg.n_kv_heads;
   constexpr bool V = W > 1;
@@ -115,6 +129,55 @@ __global__ void __launch_bounds__(512) k_rope_append(const RopeAppendParams p, c
   TO *out = is_q ? reinterpret_cast<TO *>(p.out) + t0 * p.os + head * hd
                  : reinterpret_cast<TO *>(p.pg.base) + (uint64_t)p.layer * p.pg.layer_stride +
                        (uint64_t)(head - H) * kPageLen * hd;  // K heads, then V heads of a page
+  if constexpr (W == 8 && sizeof(TI) == 2 && sizeof(TO) == 2) {
+    // word by word, and at most 42 registers: more threads hold loads on their way (8192 tokens of 48 heads x
+    // 128, bf16: 41 us, 43 with three axes; all 16 elements as f32 at once in 61 registers 49 and 51; in 32
+    // registers 49.  A copy of as many bytes takes 34.)
+    const TI *ti = nullptr;
+    const TO *to = nullptr;
+    for (uint32_t k = 0; k < nt; ++k) {
+      uint32_t r[2][4], o[2][4];
+      memcpy(r[0], &a0, 16);
+      memcpy(r[1], &a1, 16);
+      if (k + 1 < nt) {
+        src += ss;
+        a0 = load_n<V, W>(src + o0);
+        a1 = load_n<V, W>(src + o1);
+      }
+      if (turn) {
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+          if (p.half_layout) {  // elements of two pairs in a word of each part
+            const float2 c = *reinterpret_cast<const float2 *>(&cs[k][w * W + 2 * i]), s = *reinterpret_cast<const float2 *>(&sn[k][w * W + 2 * i]);
+            const float2 va = unpack(ti, r[0][i]), vb = unpack(ti, r[1][i]);
+            o[0][i] = pack(to, va.x * c.x - vb.x * s.x, va.y * c.y - vb.y * s.y);
+            o[1][i] = pack(to, va.x * s.x + vb.x * c.x, va.y * s.y + vb.y * c.y);
+          } else {  // a pair in a word
+#pragma unroll
+            for (uint32_t h = 0; h < 2; ++h) {
+              const float c = cs[k][w * W + 4 * h + i], s = sn[k][w * W + 4 * h + i];
+              const float2 v = unpack(ti, r[h][i]);
+              o[h][i] = pack(to, v.x * c - v.y * s, v.x * s + v.y * c);
+            }
+          }
+        }
+      } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) {
+          const float2 v = unpack(ti, r[i / 4][i % 4]);
+          o[i / 4][i % 4] = __is_same(TI, TO) ? r[i / 4][i % 4] : pack(to, v.x, v.y);
+        }
+      }
+      const uint64_t at = place[k];
+      TO *dst = is_q ? out : out + at;
+      if (at != kSkip) {
+        *reinterpret_cast<uint4 *>(dst + o0) = make_uint4(o[0][0], o[0][1], o[0][2], o[0][3]);
+        *reinterpret_cast<uint4 *>(dst + o1) = make_uint4(o[1][0], o[1][1], o[1][2], o[1][3]);
+      }
+      if (is_q) out += p.os;
+    }
+    return;
+  }
   for (uint32_t k = 0; k < nt; ++k) {
     float x[2][W];
 #pragma unroll

@@ -21,7 +21,6 @@ FLAG_PAGE, FLAG_RANGE, FLAG_TIMEOUT, FLAG_FULL = L.FLAG_PAGE, L.FLAG_RANGE, L.FL
 
 _DTYPES = {}  # torch dtype -> FA_KV_*
 _INTS = set()  # the 32-bit index types
-_ONE = (1,)
 
 
 def _learn():
@@ -45,7 +44,7 @@ def _code(t, name):
 
 def _index(t, name, n):
     """address of a contiguous array of n 32-bit whole numbers"""
-    if t.shape != (n,) or t.dtype not in _INTS or (n > 1 and t.stride() != _ONE):
+    if t.dtype not in _INTS or t.shape != (n,) or not t.is_contiguous():
         if not _INTS:
             _learn()
             return _index(t, name, n)
