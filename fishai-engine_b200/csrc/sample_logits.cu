@@ -40,7 +40,8 @@ struct alignas(16) Msg {  // what a CTA tells the others
 };
 struct Small {
   Msg msg[2][kMaxCtas];
-  double red[kWarps];
+  double red[kWarps], red2[kWarps];
+  double group[32];   // of a warp's groups
   uint32_t redu[4][kWarps];
   uint32_t bin, count, bins[2];
   double power[512];  // 2^(i / 512)
@@ -105,6 +106,11 @@ __device__ __forceinline__ uint8_t *space() {
   return sample_sm;
 }
 __host__ __device__ constexpr uint32_t region(uint32_t ctas) { return kList * 8 > kCtaBins * 4 * ctas ? kList * 8 : kCtaBins * 4 * ctas; }
+
+template <bool CUTS>
+__host__ __device__ constexpr uint32_t row_at(uint32_t ctas) {
+  return CUTS ? region(ctas) + kCtaBins * 8 : 0;
+}
 
 template <typename T>
 struct alignas(4 * sizeof(T)) Four {
@@ -219,6 +225,18 @@ struct Row {
     __syncthreads();
     return lanes_sum(lane < kWarps ? s.red[lane] : 0.0);
   }
+  __device__ void sum2(double &a, double &b) {
+    a = lanes_sum(a);
+    b = lanes_sum(b);
+    __syncthreads();
+    if (lane == 0) {
+      s.red[warp] = a;
+      s.red2[warp] = b;
+    }
+    __syncthreads();
+    a = lanes_sum(lane < kWarps ? s.red[lane] : 0.0);
+    b = lanes_sum(lane < kWarps ? s.red2[lane] : 0.0);
+  }
   // (sum of a, sum of b, smallest of c, largest of d)
   __device__ void sums(uint32_t &a, uint32_t &b, uint32_t &c, uint32_t &d) {
     a = __reduce_add_sync(0xFFFFFFFFu, a);
@@ -270,25 +288,22 @@ struct Row {
     clear();
     each<false>([&](float v, uint32_t) { atomicAdd(hist() + bin_of(z(v)), 1u); });
   }
-  // of the masses of those kept, where elements above z_most only count for the whole mass, which is returned
+  // of the masses of those kept, in f32 and without those beyond z_most, whose mass is returned
   template <bool CUT>
   __device__ double fill_masses(float z_most) {
     clear();
-    double w = 0;
     const float unit = kOctaves / bins;
-    each4<CUT>([&](const float (&v)[4], const bool (&use)[4], uint32_t) {
-      double e[4];
-      weights(v, e);
-#pragma unroll
-      for (uint32_t j = 0; j < 4; ++j) {
-        if (use[j]) w += e[j];
-        const float zv = z(v[j]);
-        if (!use[j] || zv > z_most) continue;
-        const uint32_t b = bin_of(zv);
-        atomicAdd(hist() + b, __float2uint_rn(ex2(fmaf((float)b - zv, unit, 15.0f))));
+    float rest = 0.0f;
+    each<CUT>([&](float v, uint32_t) {
+      const float zv = z(v);
+      if (zv > z_most) {
+        rest += ex2(-zv * unit);
+        return;
       }
+      const uint32_t b = bin_of(zv);
+      atomicAdd(hist() + b, __float2uint_rn(ex2(fmaf((float)b - zv, unit, 15.0f))));
     });
-    return sum(w);
+    return sum((double)rest);
   }
   // The cluster's sums over bins: each CTA takes a share of the bins, one a thread.  Returns that share's total.
   template <bool MASS>
@@ -589,26 +604,31 @@ struct Row {
   double strict = 0;
   float upto = INFINITY;
 
-  // Finds the place of a cut whose bracket is the bins [b0, b1]: the shortest beginning with
-  // the count or mass `target`, and takes it over into cut_key and cut_id.  CUT: there is one already.
+  // Finds the place of a cut whose bracket is the bins [b0, b1], the shortest beginning with a count of k or
+  // (MASS) a mass of pp of the whole, and takes it over into cut_at and cut_id.  CUT: there is one already.
   // True: the row is finished (its elements up to b1 were few).
   template <bool MASS, bool CUT>
-  __device__ bool cut(uint32_t row, uint32_t b0, uint32_t b1, double target, uint32_t k, double pp, double whole, double min_p, double u) {
+  __device__ bool cut(uint32_t row, uint32_t b0, uint32_t b1, uint32_t k, double pp, double min_p, double u) {
     if (tid == 0) s.count = 0;
     __syncthreads();
     // the bins b0 to b1 are z0 <= z < z1; the last one has all that is left
     const float z0 = (float)b0, z1 = b1 + 1 == bins ? INFINITY : (float)(b1 + 1);
-    double a = 0;
+    double a = 0, whole = -1.0, target = (double)k, every = 0;
     uint32_t above = 0, m = 0, kmin = 0xFFFFFFFFu, kmax = 0;
     each4<CUT>([&](const float (&v)[4], const bool (&use)[4], uint32_t id) {
-      bool over[4], any = false;
+      double w[4];
+      if (MASS) weights(v, w);
 #pragma unroll
       for (uint32_t j = 0; j < 4; ++j) {
         const float zv = z(v[j]);
-        over[j] = use[j] && zv < z0;
-        any |= over[j];
-        above += over[j];
-        if (use[j] && !over[j] && zv < z1) {
+        const bool over = use[j] && zv < z0;
+        above += over;
+        if (MASS) {
+          if (use[j]) every += w[j];
+          if (over) a += w[j];
+          if (over && w[j] >= min_p) strict += w[j];
+        }
+        if (use[j] && !over && zv < z1) {
           const uint32_t key = key_of(v[j]);
           note(key, id + j);
           ++m;
@@ -616,20 +636,15 @@ struct Row {
           kmax = max(kmax, key);
         }
       }
-      if (MASS && any) {
-        double w[4];
-        weights(v, w);
-#pragma unroll
-        for (uint32_t j = 0; j < 4; ++j) {
-          if (over[j]) a += w[j];
-          if (over[j] && w[j] >= min_p) strict += w[j];
-        }
-      }
     });
     sums(above, m, kmin, kmax);
-    if (MASS) a = sum(a);
-    const Msg *all = share(Msg{MASS ? a : (double)above, 0, above + m, m, kmin, kmax});
+    if (MASS) sum2(a, every);
+    const Msg *all = share(Msg{MASS ? a : (double)above, every, above + m, m, kmin, kmax});
     double A = all_a(all);
+    if (MASS) {
+      whole = all_b(all);
+      target = pp * whole;
+    }
     const uint32_t total = all_c(all), l = lane % ctas;
     m = __reduce_add_sync(0xFFFFFFFFu, lane < ctas ? all[lane].d : 0);
     kmin = __reduce_min_sync(0xFFFFFFFFu, all[l].e);
@@ -641,7 +656,7 @@ struct Row {
       __syncthreads();
       all = share(Msg{0, 0, s.count, 0, 0, 0});
       uint32_t n;
-      if (gather(all, n)) finish_list(row, n, k, pp, whole, min_p, u);
+      if (gather(all, n)) finish_list(row, n, MASS ? 0xFFFFFFFFu : k, pp, whole, min_p, u);
       return true;
     }
     const bool listed = m <= kSort;
@@ -792,16 +807,15 @@ struct Row {
       for (uint32_t j = 0; j < 4; ++j)
         if (!use[j] || w[j] < min_p) w[j] = 0.0;
     };
-    double *of_group = reinterpret_cast<double *>(list());
     float v[4];
     double w[4];
     for (uint32_t g = warp; g < groups; g += kWarps) {
       group(g, v, w);
       const double t = lanes_sum((w[0] + w[1]) + (w[2] + w[3]));
-      if (lane == 0) of_group[g] = t;
+      if (lane == 0) s.group[g] = t;
     }
     __syncthreads();
-    const uint32_t g = find_sum(lane < groups ? of_group[lane] : 0.0, at);
+    const uint32_t g = find_sum(lane < groups ? s.group[lane] : 0.0, at);
     if (g % kWarps != warp) return;
     group(g, v, w);
     const double four = (w[0] + w[1]) + (w[2] + w[3]);
@@ -822,8 +836,10 @@ struct Row {
   }
 };
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads, 2) k_sample_logits(const SampleParams p) {
+// CUTS: top-k or top-p may be asked for.  Without, a row needs fewer registers and no lists, and three CTAs
+// fit on an SM (200 rows of 32000 in bf16: 18.4 us, with two 20.5).
+template <typename T, bool CUTS>
+__global__ void __launch_bounds__(kThreads, CUTS ? 2 : 3) k_sample_logits(const SampleParams p) {
   __shared__ Small s;
   const uint32_t ctas = p.ctas, row = blockIdx.x / ctas;
   Row<T> w(p, s);
@@ -833,15 +849,17 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_logits(const SampleParam
   w.rank = cluster_ctarank();
   w.ctas = ctas;
   w.groups = p.groups;
-  w.x_at = region(ctas) + kCtaBins * 8;
+  w.x_at = row_at<CUTS>(ctas);
   w.id0 = w.rank * p.slice;
   w.mine = w.warp * 128 * p.groups + 4 * w.lane;
+  // the others' shared memory may be written once all have begun: waited for before the first time
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   s.power[w.tid] = exp2((double)w.tid / 512.0);
   const uint32_t at = p.rows ? p.rows[row] : row;
   if (at == FA_NO_TOKEN) return;
   // the row's own settings: on their way while the logits are read
-  const float t = p.temperature ? p.temperature[row] : 1.0f, u = p.u[row], pp = p.top_p ? p.top_p[row] : 1.0f, mp = p.min_p ? p.min_p[row] : 0.0f;
-  const uint32_t k = p.top_k ? p.top_k[row] : 0;
+  const float t = p.temperature ? p.temperature[row] : 1.0f, u = p.u[row], pp = CUTS && p.top_p ? p.top_p[row] : 1.0f, mp = p.min_p ? p.min_p[row] : 0.0f;
+  const uint32_t k = CUTS && p.top_k ? p.top_k[row] : 0;
   // the CTA's part of the row; behind its end -inf
   const uint32_t len = at < p.n_logits && w.id0 < p.vocab ? min(p.slice, p.vocab - w.id0) : 0, room = p.groups * kGroup;
   const T *src = reinterpret_cast<const T *>(p.logits) + (uint64_t)at * p.ld + w.id0;
@@ -883,13 +901,14 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_logits(const SampleParam
     if (p.err && w.rank == 0 && w.tid == 0) atomicOr(p.err, kFlagRange);
     return;
   }
-  bool few = t > 0 && k && k < p.vocab && k <= kFewK;
-  if (few) {
+  bool few = CUTS && t > 0 && k && k < p.vocab && k <= kFewK;
+  if (CUTS && few) {
     __syncthreads();
     w.note_largest(mx, k);
   }
   uint32_t o0 = 0, o1 = 0, o2 = 0, key = key_of(mx);
   w.sums(o0, o1, o2, key);
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   const Msg *all = w.share(Msg{0, 0, key, few ? s.count : 0, 0, 0});
   key = __reduce_max_sync(0xFFFFFFFFu, all[w.lane % ctas].c);
   const uint32_t noted = __reduce_add_sync(0xFFFFFFFFu, w.lane < ctas ? all[w.lane].d : 0);
@@ -928,45 +947,47 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_logits(const SampleParam
     return;
   }
   w.scale(top, t);
-  if (few && noted < kList) {  // a CTA whose list ran over has at least kList
-    w.pick_largest(row, all, noted, k, pp, mp, u);
-    return;
-  }
-  bool has_cut = false;
-  if (k && k < p.vocab) {
-    w.fill_counts();
-    all = w.share(Msg{w.template reduce_bins<false>(), 0, 0, 0, 0, 0});
-    if (w.all_a(all) > (double)k) {
-      const double target[2] = {(double)k, (double)k};
-      uint32_t b[2];
-      w.find_bins(all, target, b);
-      if (w.template cut<false, false>(row, b[0], b[1], (double)k, k, pp, -1.0, mp, u)) return;
+  if constexpr (CUTS) {
+    if (few && noted < kList) {  // a CTA whose list ran over has at least kList
+      w.pick_largest(row, all, noted, k, pp, mp, u);
+      return;
+    }
+    bool has_cut = false;
+    uint32_t b[2];
+    if (k && k < p.vocab) {
+      w.fill_counts();
+      all = w.share(Msg{w.template reduce_bins<false>(), 0, 0, 0, 0, 0});
+      if (w.all_a(all) > (double)k) {
+        const double target[2] = {(double)k, (double)k};
+        w.find_bins(all, target, b);
+        if (w.template cut<false, false>(row, b[0], b[1], k, pp, mp, u)) return;
+        has_cut = true;
+      }
+    }
+    if (pp < 1.0f) {
+      // all mass above z_most is less than half of what may be cut: the place is below it
+      const float z_most = (log2f((float)p.vocab) - log2f(1.0f - pp) + 1.0f) * (w.bins / kOctaves);
+      const double rest = has_cut ? w.template fill_masses<true>(z_most) : w.template fill_masses<false>(z_most);
+      const double total = w.template reduce_bins<true>();
+      all = w.share(Msg{total, rest, 0, 0, 0, 0});
+      const double about = (double)pp * (w.all_a(all) + w.all_b(all));
+      const double around[2] = {about * (1.0 - 3 * kHistError), about * (1.0 + 3 * kHistError)};
+      w.find_bins(all, around, b);
+      if (has_cut ? w.template cut<true, true>(row, b[0], b[1], 0, pp, mp, u) : w.template cut<true, false>(row, b[0], b[1], 0, pp, mp, u)) return;
       has_cut = true;
     }
-  }
-  if (pp < 1.0f) {
-    // all mass above z_most is less than half of what may be cut: the place is below it
-    const float z_most = (log2f((float)p.vocab) - log2f(1.0f - pp) + 1.0f) * (w.bins / kOctaves);
-    const double whole = has_cut ? w.template fill_masses<true>(z_most) : w.template fill_masses<false>(z_most);
-    const double total = w.template reduce_bins<true>();
-    all = w.share(Msg{total, whole, 0, 0, 0, 0});
-    const double W = w.all_b(all), target = (double)pp * W;
-    const double around[2] = {target * (1.0 - 2 * kHistError), target * (1.0 + 2 * kHistError)};
-    uint32_t b[2];
-    w.find_bins(all, around, b);
-    if (has_cut ? w.template cut<true, true>(row, b[0], b[1], target, 0xFFFFFFFFu, pp, W, mp, u)
-                : w.template cut<true, false>(row, b[0], b[1], target, 0xFFFFFFFFu, pp, W, mp, u))
+    if (has_cut) {
+      w.template draw<true>(row, (double)mp, (double)u);
       return;
-    has_cut = true;
+    }
   }
-  if (has_cut) w.template draw<true>(row, (double)mp, (double)u);
-  else w.template draw<false>(row, (double)mp, (double)u);
+  w.template draw<false>(row, (double)mp, (double)u);
 }
 
-template <typename T>
+template <typename T, bool CUTS>
 int launch(const SampleParams &p, cudaStream_t st) {
-  const uint32_t smem = region(p.ctas) + kCtaBins * 8 + p.groups * kGroup * (uint32_t)sizeof(T);
-  if (cudaFuncSetAttribute(k_sample_logits<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSampleMaxSmem) != cudaSuccess) return -1;
+  const uint32_t smem = row_at<CUTS>(p.ctas) + p.groups * kGroup * (uint32_t)sizeof(T);
+  if (cudaFuncSetAttribute(k_sample_logits<T, CUTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSampleMaxSmem) != cudaSuccess) return -1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(p.n * p.ctas);
   cfg.blockDim = dim3(kThreads);
@@ -978,7 +999,7 @@ int launch(const SampleParams &p, cudaStream_t st) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, k_sample_logits<T>, p) == cudaSuccess ? 0 : -1;
+  return cudaLaunchKernelEx(&cfg, k_sample_logits<T, CUTS>, p) == cudaSuccess ? 0 : -1;
 }
 
 }  // namespace
@@ -998,10 +1019,11 @@ int launch_sample_logits(const SampleParams &in, uint32_t n_sm, cudaStream_t st)
   p.slice = ((p.vocab + p.ctas - 1) / p.ctas + 15) / 16 * 16;
   static_assert(region(kMaxCtas) + kCtaBins * 8 + kSampleMaxVocab / kMaxCtas * 4 <= kSampleMaxSmem && kSampleMaxVocab % (kMaxCtas * kGroup) == 0,
                 "shared memory of the largest vocabulary");
+  const bool cuts = p.top_k || p.top_p;
   switch (p.dtype) {
-    case FA_KV_F32: return launch<float>(p, st);
-    case FA_KV_F16: return launch<__half>(p, st);
-    default: return launch<__nv_bfloat16>(p, st);
+    case FA_KV_F32: return cuts ? launch<float, true>(p, st) : launch<float, false>(p, st);
+    case FA_KV_F16: return cuts ? launch<__half, true>(p, st) : launch<__half, false>(p, st);
+    default: return cuts ? launch<__nv_bfloat16, true>(p, st) : launch<__nv_bfloat16, false>(p, st);
   }
 }
 

@@ -296,10 +296,7 @@ def plan_step(kv: PagedKV, add, lengths, free_pages, n_free, q_start, kv_len, po
     table = getattr(kv, "page_table", None)
     if table is None:
         raise ValueError("kv: pages of the caller's own; those of a KVCache are the cache's to give")
-    n, rows = add.shape[0], positions.shape[0]
-    if free_pages.dim() != 1:
-        raise ValueError("free_pages: a 1-d int32 tensor is needed")
-    cap = free_pages.shape[0]
+    n, rows, cap = add.numel(), positions.numel(), free_pages.numel()  # 1-d: _index sees to it
     ln = _index(lengths, "lengths", kv.n_seq)
     nf = _index(n_free, "n_free", 1)
     pool = L.fa_page_pool(kv._c.page_table, kv.n_seq, kv.max_pages, kv.n_pages, _index(free_pages, "free_pages", cap), cap)

@@ -81,7 +81,7 @@ class Sampler:
 
 def _floats(t, name, n):
     """address of a contiguous array of n float32"""
-    if t.shape != (n,) or _DTYPES.get(t.dtype) != L.KV_F32 or (n > 1 and t.stride() != (1,)):
+    if _DTYPES.get(t.dtype) != L.KV_F32 or t.shape != (n,) or not t.is_contiguous():
         raise ValueError(f"{name}: a contiguous float32 [{n}] tensor is needed")
     return t.data_ptr()
 
@@ -95,14 +95,15 @@ def sample_logits(logits, u, ids, temperature=None, top_k=None, top_p=None, min_
     Framework tensors on the GPU: float32 but ids, rows, top_k (int32) and err (one
     int32, FLAG_* bits).  What is kept and drawn: fa_sample_logits."""
     dt = _code(logits, "logits")
-    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+    shape, stride = logits.shape, logits.stride()
+    if len(shape) != 2 or (shape[1] > 1 and stride[1] != 1):
         raise ValueError("logits: [rows, vocab] with consecutive elements")
-    m, vocab = logits.shape
-    n = ids.shape[0]
-    if m >> 32 or vocab >> 32 or n >> 32:
+    m, vocab = shape
+    n = ids.numel()
+    if (m | vocab | n) >> 32:
         L.u32(rows=m, vocab=vocab, ids=n)
     rc = L.lib().fa_sample_logits(
-        logits.data_ptr(), dt, logits.stride(0) if m > 1 else vocab, m, vocab, None if rows is None else _index(rows, "rows", n), n,
+        logits.data_ptr(), dt, stride[0] if m > 1 else vocab, m, vocab, None if rows is None else _index(rows, "rows", n), n,
         None if temperature is None else _floats(temperature, "temperature", n), None if top_k is None else _index(top_k, "top_k", n),
         None if top_p is None else _floats(top_p, "top_p", n), None if min_p is None else _floats(min_p, "min_p", n), _floats(u, "u", n),
         _index(ids, "ids", n), None if logprobs is None else _floats(logprobs, "logprobs", n),

@@ -141,3 +141,36 @@ def test_sample_logits_refuses(bad):
 
 def test_sampling_nothing():
     assert call_sample(n=0, logits=None, u=None, ids=None) == L.OK
+
+
+# ------------------------------------------------------------------ what Python refuses before the library is called
+def test_python_refuses_tensors_that_do_not_fit():
+    torch = pytest.importorskip("torch")
+    from fishai_engine import sampling
+    i = lambda *s: torch.zeros(*s, dtype=torch.int32)  # noqa: E731
+    kv = paged.PagedKV(torch.zeros(1, 8, 2, 4, 16, 64, dtype=torch.float16), i(2, 4))
+    args = dict(add=i(2), lengths=i(2), free_pages=i(8), n_free=i(1), q_start=i(3), kv_len=i(2), positions=i(5), row_seqs=i(5))
+    for name, bad in (("add", i(2, 1)), ("lengths", i(3)), ("free_pages", i(2, 4)), ("n_free", i(2)), ("q_start", i(2)), ("kv_len", i(3)),
+                      ("positions", torch.zeros(5)), ("row_seqs", i(4)), ("seqs", i(3)), ("keep", i(4)[::2]), ("slots", i(6)), ("last", i(1)),
+                      ("lengths_out", i(1)), ("n_free_out", i(0)), ("err", i(2))):
+        with pytest.raises(ValueError):
+            paged.plan_step(kv, **{**args, name: bad})
+
+    class OfACache:
+        n_seq = 2
+
+    with pytest.raises(ValueError, match="KVCache"):
+        paged.plan_step(OfACache(), **args)
+    x, f = torch.zeros(3, 50), lambda n: torch.zeros(n)  # noqa: E731
+    good = dict(logits=x, u=f(3), ids=i(3))
+    for name, bad in (("logits", x[0]), ("logits", x.t()), ("logits", x.double()), ("u", f(2)), ("u", i(3)), ("ids", f(3)), ("temperature", f(4)),
+                      ("top_k", f(3)), ("top_p", f(6)[::2]), ("min_p", f(3).double()), ("rows", i(2)), ("logprobs", i(3)), ("err", i(3))):
+        with pytest.raises(ValueError):
+            sampling.sample_logits(**{**good, name: bad})
+    r = paged.Rope(64, axes=[16, 16])
+    q, k = torch.zeros(3, 512, dtype=torch.float16), torch.zeros(3, 256, dtype=torch.float16)
+    for pos, slots in ((i(3), i(3)), (i(2, 3), None), (i(3, 2).t(), i(3)), (i(3, 3), i(3)), (f(6).view(2, 3), i(3)), (i(2, 6)[:, ::2], i(3))):
+        with pytest.raises(ValueError):
+            paged.rope_append(kv, 0, r, q, k, k, pos, i(3), torch.empty_like(q), slots=slots)
+    with pytest.raises(ValueError):
+        paged.attention(kv, 0, q, i(2), i(1), torch.empty_like(q), 3, torch.zeros(8, dtype=torch.uint8), window=5, sinks=2 ** 32)
