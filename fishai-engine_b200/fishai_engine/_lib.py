@@ -19,7 +19,7 @@ KV_F32, KV_F16, KV_BF16 = 0, 1, 2
 FLAG_PAGE, FLAG_RANGE, FLAG_TIMEOUT, FLAG_FULL = 16, 32, 64, 128
 ROPE_INTERLEAVED, ROPE_HALF = 0, 1
 ROPE_PLAIN, ROPE_LINEAR, ROPE_NTK, ROPE_LLAMA3, ROPE_YARN = 0, 1, 2, 3, 4
-AXES_BLOCKS, AXES_TURNS, AXES_SHARED, AXES_OWN = 0, 1, 0, 1
+ROPE_MAX_AXES, AXES_BLOCKS, AXES_TURNS, AXES_SHARED, AXES_OWN = 4, 0, 1, 0, 1
 NO_TOKEN = 4294967295
 DEBUG_WAIT_LIMIT_NS, DEBUG_WITHHOLD_WEIGHTS, DEBUG_FIXED_ORDER_SUMS, DEBUG_WITHHOLD_KV = 1, 2, 3, 4
 
@@ -77,7 +77,7 @@ class fa_rope_config(C.Structure):
 
 
 class fa_rope_axes(C.Structure):
-    _fields_ = [("n_axes", C.c_uint32), ("pairs", C.c_uint32 * 4), ("order", C.c_int32), ("freqs", C.c_int32)]
+    _fields_ = [("n_axes", C.c_uint32), ("pairs", C.c_uint32 * ROPE_MAX_AXES), ("order", C.c_int32), ("freqs", C.c_int32)]
 
 
 class fa_page_pool(C.Structure):

@@ -159,11 +159,11 @@ class Rope:
             axes = list(axes)
             if axis_order not in _ORDERS or axis_freqs not in _FREQS:
                 raise ValueError(f"axis_order is one of {sorted(_ORDERS)}, axis_freqs one of {sorted(_FREQS)}")
-            if not 1 <= len(axes) <= 4:
-                raise ValueError("axes: pairs of 1 to 4 axes")
+            if not 1 <= len(axes) <= L.ROPE_MAX_AXES:
+                raise ValueError(f"axes: pairs of 1 to {L.ROPE_MAX_AXES} axes")
             for n in axes:
                 L.u32(axes=n)
-            a = L.fa_rope_axes(len(axes), (C.c_uint32 * 4)(*axes), _ORDERS[axis_order], _FREQS[axis_freqs])
+            a = L.fa_rope_axes(len(axes), (C.c_uint32 * L.ROPE_MAX_AXES)(*axes), _ORDERS[axis_order], _FREQS[axis_freqs])
             L.check(L.lib().fa_rope_create_axes(C.byref(c), C.byref(a), C.byref(h)))
             self.n_axes = len(axes)
         self._h = h
@@ -257,10 +257,10 @@ def attention(kv: PagedKV, layer: int, q, q_start, kv_len, out, max_q: int, work
     width = _width(q, hd)
     qp, qs = _rows(q, "q", t, width)
     op, os = _rows(out, "out", t, width)
-    rc = L.lib().fa_attn_chunks_sinks(kv._ref, layer, qp, qs, width // hd, n, _index(q_start, "q_start", n + 1),
-                                      _index(kv_len, "kv_len", n), None if seqs is None else _index(seqs, "seqs", n), t, max_q,
-                                      scale, window, sinks, op, os, *_space(workspace),
-                                      None if err is None else _index(err, "err", 1), stream)
+    args = (kv._ref, layer, qp, qs, width // hd, n, _index(q_start, "q_start", n + 1), _index(kv_len, "kv_len", n),
+            None if seqs is None else _index(seqs, "seqs", n), t, max_q, scale, window)
+    rest = (op, os, *_space(workspace), None if err is None else _index(err, "err", 1), stream)
+    rc = L.lib().fa_attn_chunks_sinks(*args, sinks, *rest) if sinks else L.lib().fa_attn_chunks(*args, *rest)
     if rc:
         L.check(rc)
 

@@ -218,3 +218,12 @@ def test_infinity_beside_the_largest_number_of_a_type(t):
     for k in (None, [3] * 3, [600] * 3):
         check(x, [0.2, 0.6, 0.9], [1.0, 0.5, 1.0], k, [0.9, 1.0, 0.7])
         check(x, [0.2, 0.6, 0.9], [0.0] * 3, k)
+
+
+def test_rows_beyond_32_bits_of_elements():
+    x = torch.empty(34000, 128256, dtype=torch.float16, device="cuda")  # 4.36e9
+    for r in (0, 33999):
+        x[r] = logits_of("text", 1, 128256, torch.float16, r)[0]
+    check(x, [0.3, 0.6, 0.9, 0.5], [1.0, 1.0, 0.8, 0.0], [0, 50, 0, 0], [1.0, 1.0, 0.9, 1.0], rows=[33999, 33999, 33999, 33999])
+    del x
+    torch.cuda.empty_cache()

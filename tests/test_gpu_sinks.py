@@ -171,3 +171,21 @@ def test_repeated_calls_give_the_same_bits():
     first = call(pages, table, q, start, kvs, 700, 40)
     for _ in range(5):
         assert torch.equal(call(pages, table, q, start, kvs, 700, 40), first)
+
+
+@pytest.mark.parametrize("q", [1, 40, 200])
+def test_pages_beyond_32_bits_of_elements(q):
+    """a small cache whose pages lie at the end of a large one"""
+    small, table = R.make_cache([700, 333], 1, 8, 128, torch.float16, 31)
+    n = small.shape[1]
+    pages = torch.empty(1, 2 ** 17 + 9000, 2, 8, 16, 128, dtype=torch.float16, device="cuda")  # 4.6e9 elements
+    pages[0, -n:] = small[0]
+    moved = table + (pages.shape[1] - n)
+    x = randn(1, 2 * q, 16 * 128, dtype=torch.float16)
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out = call(pages, moved, x, [0, q, 2 * q], [700, 333], 100, 20, err=err)
+    assert int(err) == 0 and torch.equal(out, call(small, table, x, [0, q, 2 * q], [700, 333], 100, 20))
+    want, tol = S.attention(small, table, x, [0, q, 2 * q], [700, 333], 16, 0.0, 100, 20)
+    assert bool(((out.double().view_as(want) - want).abs() <= tol).all())
+    del pages
+    torch.cuda.empty_cache()

@@ -172,3 +172,36 @@ def test_captured_and_replayed():
         table, free, lens, n_free = want[6], want[7], want[8], want[9]
         assert t["pos"].tolist() == want[3] and t["lens"].tolist() == lens and kv.page_table.tolist() == table and int(t["n_free"]) == n_free
     assert int(t["err"]) == 0
+
+
+def test_two_calls_at_once_on_pools_of_their_own():
+    """streams side by side: nothing is shared between calls"""
+    rng = random.Random(3)
+    cases = []
+    for i in range(8):
+        n = [5, 300, 20, 700][i % 4]
+        lens = [rng.randint(0, 100) for _ in range(n)]
+        add = [rng.randint(0, 40) for _ in range(n)]
+        table, free, n_free, n_pages = world(lens, 10, 3 * n, i)
+        cases.append((kv_of(table, n_pages), add, lens, free, n_free, sum(add) + 3, S.plan(None, None, add, sum(add) + 3, lens, table, free, n_free, n_pages)))
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = []
+    for st, (kv, add, lens, free, n_free, rows, _) in zip(streams, cases):
+        with torch.cuda.stream(st):
+            got.append(run(kv, add, lens, free, n_free, rows, stream=st.cuda_stream))
+    torch.cuda.synchronize()
+    for g, c in zip(got, cases):
+        for a, w in zip(g, c[6]):
+            assert a.tolist() == (w if isinstance(w, list) else [w])
+
+
+@pytest.mark.parametrize("n", [4096])
+def test_the_most_requests(n):
+    rng = random.Random(4)
+    lens = [rng.randint(0, 60) for _ in range(n + 100)]
+    seqs = list(range(n + 100))
+    rng.shuffle(seqs)
+    keep = [rng.choice([lens[q], lens[q], lens[q] // 2, 0]) for q in seqs[:n]]
+    add = [min(64 - k, rng.choice([0, 1, 1, 17])) for k in keep]
+    check(add, lens, sum(add), 4, 4 * n, seqs[:n], keep)
