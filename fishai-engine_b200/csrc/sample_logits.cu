@@ -225,18 +225,6 @@ struct Row {
     __syncthreads();
     return lanes_sum(lane < kWarps ? s.red[lane] : 0.0);
   }
-  __device__ void sum2(double &a, double &b) {
-    a = lanes_sum(a);
-    b = lanes_sum(b);
-    __syncthreads();
-    if (lane == 0) {
-      s.red[warp] = a;
-      s.red2[warp] = b;
-    }
-    __syncthreads();
-    a = lanes_sum(lane < kWarps ? s.red[lane] : 0.0);
-    b = lanes_sum(lane < kWarps ? s.red2[lane] : 0.0);
-  }
   // (sum of a, sum of b, smallest of c, largest of d)
   __device__ void sums(uint32_t &a, uint32_t &b, uint32_t &c, uint32_t &d) {
     a = __reduce_add_sync(0xFFFFFFFFu, a);
@@ -251,11 +239,36 @@ struct Row {
       s.redu[3][warp] = d;
     }
     __syncthreads();
+    read_sums(a, b, c, d);
+  }
+  __device__ void read_sums(uint32_t &a, uint32_t &b, uint32_t &c, uint32_t &d) const {
     const uint32_t l = lane % kWarps;
     a = __reduce_add_sync(0xFFFFFFFFu, lane < kWarps ? s.redu[0][l] : 0);
     b = __reduce_add_sync(0xFFFFFFFFu, lane < kWarps ? s.redu[1][l] : 0);
     c = __reduce_min_sync(0xFFFFFFFFu, s.redu[2][l]);
     d = __reduce_max_sync(0xFFFFFFFFu, s.redu[3][l]);
+  }
+  // the same with the sums of x and y, in one exchange
+  __device__ void sums(double &x, double &y, uint32_t &a, uint32_t &b, uint32_t &c, uint32_t &d) {
+    x = lanes_sum(x);
+    y = lanes_sum(y);
+    a = __reduce_add_sync(0xFFFFFFFFu, a);
+    b = __reduce_add_sync(0xFFFFFFFFu, b);
+    c = __reduce_min_sync(0xFFFFFFFFu, c);
+    d = __reduce_max_sync(0xFFFFFFFFu, d);
+    __syncthreads();
+    if (lane == 0) {
+      s.red[warp] = x;
+      s.red2[warp] = y;
+      s.redu[0][warp] = a;
+      s.redu[1][warp] = b;
+      s.redu[2][warp] = c;
+      s.redu[3][warp] = d;
+    }
+    __syncthreads();
+    x = lanes_sum(lane < kWarps ? s.red[lane] : 0.0);
+    y = lanes_sum(lane < kWarps ? s.red2[lane] : 0.0);
+    read_sums(a, b, c, d);
   }
   // inclusive sums over a warp's lanes
   __device__ double lanes_scan(double v) const {
@@ -432,19 +445,25 @@ struct Row {
     __syncthreads();
   }
   // CTA 0 brings all CTAs' lists together in its own, sorted; true there.  After it
-  // no CTA reads another's memory.
-  __device__ bool gather(const Msg *all, uint32_t &n) {
+  // no CTA reads another's memory.  noted: of the lane's CTA.
+  __device__ bool gather(uint32_t noted, uint32_t &n) {
     uint64_t mine[2] = {0, 0};
-    n = all_c(all);
-    if (rank == 0)
+    if (lane >= ctas) noted = 0;
+    n = __reduce_add_sync(0xFFFFFFFFu, noted);
+    if (rank == 0) {
+      uint32_t c[kMaxCtas];
+#pragma unroll
+      for (uint32_t r = 0; r < kMaxCtas; ++r) c[r] = __shfl_sync(0xFFFFFFFFu, noted, r);
 #pragma unroll
       for (uint32_t e = 0; e < 2; ++e) {
-        uint32_t i = tid + e * kThreads;
+        uint32_t i = tid + e * kThreads, r = 0;
         if (i >= n) continue;
-        uint32_t r = 0;
-        while (i >= all[r].c) i -= all[r++].c;
+#pragma unroll
+        for (uint32_t k = 0; k + 1 < kMaxCtas; ++k)
+          if (r == k && i >= c[k]) i -= c[k], ++r;
         mine[e] = ld_cluster64(dsmem_addr(list() + i, r));
       }
+    }
     cluster_sync();
     if (rank) return false;
     list()[tid] = mine[0];
@@ -600,9 +619,12 @@ struct Row {
     finish_list(row, m, k, pp, -1.0, min_p, u);
   }
 
-  // mass of the thread's elements above `upto`, where a cut has formed it
+  // mass of the thread's elements above `upto`, where a cut has formed it, and which of its elements were in the
+  // cut's bracket (4 g + e of group g), where the groups are few enough
   double strict = 0;
   float upto = INFINITY;
+  uint64_t marks = 0;
+  __device__ bool marked() const { return groups <= 16; }
 
   // Finds the place of a cut whose bracket is the bins [b0, b1], the shortest beginning with a count of k or
   // (MASS) a mass of pp of the whole, and takes it over into cut_at and cut_id.  CUT: there is one already.
@@ -615,6 +637,7 @@ struct Row {
     const float z0 = (float)b0, z1 = b1 + 1 == bins ? INFINITY : (float)(b1 + 1);
     double a = 0, whole = -1.0, target = (double)k, every = 0;
     uint32_t above = 0, m = 0, kmin = 0xFFFFFFFFu, kmax = 0;
+    uint64_t bit = 1;  // of the group's first element
     each4<CUT>([&](const float (&v)[4], const bool (&use)[4], uint32_t id) {
       double w[4];
       if (MASS) weights(v, w);
@@ -634,11 +657,13 @@ struct Row {
           ++m;
           kmin = min(kmin, key);
           kmax = max(kmax, key);
+          if (MASS) marks |= bit << j;
         }
       }
+      bit <<= 4;
     });
-    sums(above, m, kmin, kmax);
-    if (MASS) sum2(a, every);
+    if (MASS) sums(a, every, above, m, kmin, kmax);
+    else sums(above, m, kmin, kmax);
     const Msg *all = share(Msg{MASS ? a : (double)above, every, above + m, m, kmin, kmax});
     double A = all_a(all);
     if (MASS) {
@@ -656,7 +681,7 @@ struct Row {
       __syncthreads();
       all = share(Msg{0, 0, s.count, 0, 0, 0});
       uint32_t n;
-      if (gather(all, n)) finish_list(row, n, MASS ? 0xFFFFFFFFu : k, pp, whole, min_p, u);
+      if (gather(all[l].c, n)) finish_list(row, n, MASS ? 0xFFFFFFFFu : k, pp, whole, min_p, u);
       return true;
     }
     const bool listed = m <= kSort;
@@ -734,12 +759,12 @@ struct Row {
         const uint32_t key = key_of(v);
         if (key >= kmin && key <= kmax) note(key, id);
       });
+      __syncthreads();
+      all = share(Msg{0, 0, 0, s.count, 0, 0});
     }
-    __syncthreads();
-    all = share(Msg{0, 0, s.count, 0, 0, 0});
     uint32_t n;
     Msg place{};
-    if (gather(all, n)) {
+    if (gather(all[l].d, n)) {
       const uint64_t e[2] = {list()[2 * tid], list()[2 * tid + 1]};
       double w[2];
 #pragma unroll
@@ -774,20 +799,30 @@ struct Row {
   template <bool CUT>
   __device__ void draw(uint32_t row, double min_p, double u) {
     double own = strict;
-    each4<CUT>([&](const float (&v)[4], const bool (&use)[4], uint32_t) {
-      bool add[4], any = false;
-#pragma unroll
-      for (uint32_t j = 0; j < 4; ++j) {
-        add[j] = use[j] && !(CUT && v[j] > upto);  // those above are counted
-        any |= add[j];
+    if (CUT && marked() && upto < INFINITY) {  // only what was in the bracket is left to look at
+      for (uint64_t m = marks; m; m &= m - 1) {
+        const uint32_t i = __ffsll((long long)m) - 1, at = mine + 128 * (i / 4) + i % 4;
+        const float v = (float)x()[at];
+        if (!kept<CUT>(v, id0 + at)) continue;
+        const double w = weight(v);
+        if (w >= min_p) own += w;
       }
-      if (CUT && !any) return;
-      double w[4];
-      weights(v, w);
+    } else {
+      each4<CUT>([&](const float (&v)[4], const bool (&use)[4], uint32_t) {
+        bool add[4], any = false;
 #pragma unroll
-      for (uint32_t j = 0; j < 4; ++j)
-        if (add[j] && w[j] >= min_p) own += w[j];
-    });
+        for (uint32_t j = 0; j < 4; ++j) {
+          add[j] = use[j] && !(CUT && v[j] > upto);  // those above are counted
+          any |= add[j];
+        }
+        if (CUT && !any) return;
+        double w[4];
+        weights(v, w);
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j)
+          if (add[j] && w[j] >= min_p) own += w[j];
+      });
+    }
     const Msg *all = share(Msg{sum(own), 0, 0, 0, 0, 0});  // the warps' sums stay in s.red
     const double M = all_a(all);
     double at = u * M;
