@@ -15,6 +15,8 @@
 // pages that are taken, and the rows, each finding its request by a binary search in
 // the sums, so that one long sequence does not keep a warp while the others wait;
 // a barrier of the cluster stands where one's writes are another's reads.
+#include <type_traits>
+
 #include "fa_device.cuh"
 #include "paged_ops.hpp"
 
@@ -69,7 +71,7 @@ __device__ __forceinline__ uint32_t find(const uint32_t *sums, uint32_t n, uint3
 }
 
 // words r0 .. r0 + 3 of an array of n, at once where it is aligned
-__device__ __forceinline__ void put4(uint32_t *to, uint32_t r0, uint32_t n, const uint32_t (&v)[4]) {
+__device__ __forceinline__ void put4(uint32_t *to, uint32_t r0, uint32_t n, const uint32_t *v) {
   if (reinterpret_cast<uintptr_t>(to) % 16 == 0 && r0 + 4 <= n) {
     *reinterpret_cast<uint4 *>(to + r0) = make_uint4(v[0], v[1], v[2], v[3]);
     return;
@@ -79,10 +81,10 @@ __device__ __forceinline__ void put4(uint32_t *to, uint32_t r0, uint32_t n, cons
     if (r0 + e < n) to[r0 + e] = v[e];
 }
 
-// inclusive sums over the CTA's threads of v[0 .. N), and the totals; scratch of N x kWarps words
-template <uint32_t kWarps, int N>
-__device__ __forceinline__ void scan(uint32_t (&v)[N], uint32_t (&total)[N], uint32_t (*red)[kWarps]) {
-  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+// inclusive sums over a warp's lanes
+template <int N>
+__device__ __forceinline__ void scan_lanes(uint32_t (&v)[N]) {
+  const uint32_t lane = threadIdx.x & 31;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1)
 #pragma unroll
@@ -90,22 +92,26 @@ __device__ __forceinline__ void scan(uint32_t (&v)[N], uint32_t (&total)[N], uin
       const uint32_t x = __shfl_up_sync(0xFFFFFFFFu, v[k], o);
       if (lane >= (uint32_t)o) v[k] = sat(v[k], x);
     }
+}
+// over the CTA's threads, and the totals; scratch of N x kWarps words
+template <uint32_t kWarps, int N>
+__device__ __forceinline__ void scan(uint32_t (&v)[N], uint32_t (&total)[N], uint32_t (*red)[kWarps]) {
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  scan_lanes(v);
   __syncthreads();
   if (lane == 31)
 #pragma unroll
     for (int k = 0; k < N; ++k) red[k][warp] = v[k];
   __syncthreads();
+  uint32_t of[N];  // the warps' totals, summed by every warp
+#pragma unroll
+  for (int k = 0; k < N; ++k) of[k] = lane < kWarps ? red[k][lane] : 0;
+  scan_lanes(of);
 #pragma unroll
   for (int k = 0; k < N; ++k) {
-    uint32_t before = 0;
-    total[k] = 0;
-#pragma unroll
-    for (uint32_t w = 0; w < kWarps; ++w) {
-      const uint32_t x = red[k][w];
-      if (w < warp) before = sat(before, x);
-      total[k] = sat(total[k], x);
-    }
-    v[k] = sat(v[k], before);
+    total[k] = __shfl_sync(0xFFFFFFFFu, of[k], kWarps - 1);
+    const uint32_t before = __shfl_sync(0xFFFFFFFFu, of[k], (warp + 31) % 32);
+    if (warp) v[k] = sat(v[k], before);
   }
 }
 
@@ -201,11 +207,8 @@ __global__ void __launch_bounds__(THREADS) k_step_plan(const StepPlanParams p) {
     red[1][warp] = A;
   }
   __syncthreads();
-#pragma unroll
-  for (uint32_t w = 0; w < kWarps; ++w) {
-    T = max(T, red[0][w]);
-    A = max(A, red[1][w]);
-  }
+  T = __reduce_max_sync(0xFFFFFFFFu, red[0][lane % kWarps]);
+  A = __reduce_max_sync(0xFFFFFFFFu, red[1][lane % kWarps]);
   // a stack that is longer than its array, or would be: nothing is done
   const bool bad = free0 > p.free_cap || sat(free0, freed) > p.free_cap;
   if (bad) {
@@ -245,28 +248,41 @@ __global__ void __launch_bounds__(THREADS) k_step_plan(const StepPlanParams p) {
     *p.n_free_out = top - A;
   }
   if (p.slot) cluster_sync();  // the table is complete
-  // four rows a thread: one search, and their loads at once
-  for (uint32_t r0 = 4 * at; r0 < p.n_rows; r0 += 4 * all) {
-    uint32_t pos[4], q[4], slot[4], i = r0 < T ? find(s.start, n, r0) : 0;
+  // Rows, four or eight in a row a thread: one search in the sums, then all their looks at the table at once
+  // (one where a page begins, each waited for, took twice as long).
+  auto put_rows = [&](auto count) {
+    constexpr uint32_t N = decltype(count)::value;
+    for (uint32_t r0 = N * at; r0 < p.n_rows; r0 += N * all) {
+      uint32_t pos[N], q[N], slot[N], i = r0 < T ? find(s.start, n, r0) : 0, end = r0 < T ? s.start[i + 1] : 0;
 #pragma unroll
-    for (uint32_t e = 0; e < 4; ++e) {
-      const uint32_t r = r0 + e;
-      pos[e] = 0;
-      q[e] = slot[e] = kNone;
-      if (r < T) {
-        while (s.start[i + 1] <= r) ++i;
-        pos[e] = s.now[i] - (s.start[i + 1] - r);
-        q[e] = s.seq[i];
-        if (p.slot) slot[e] = __ldcg(p.table + (uint64_t)q[e] * p.max_pages + pos[e] / kPageLen);
+      for (uint32_t e = 0; e < N; ++e) {
+        const uint32_t r = r0 + e;
+        pos[e] = 0;
+        q[e] = slot[e] = kNone;
+        if (r < T) {
+          while (end <= r) end = s.start[++i + 1];
+          pos[e] = s.now[i] - (end - r);
+          q[e] = s.seq[i];
+        }
+      }
+      if (p.slot) {
+#pragma unroll
+        for (uint32_t e = 0; e < N; ++e)
+          if (r0 + e < T) slot[e] = __ldcg(p.table + (uint64_t)q[e] * p.max_pages + pos[e] / kPageLen);
+#pragma unroll
+        for (uint32_t e = 0; e < N; ++e)
+          if (r0 + e < T) slot[e] = slot[e] * kPageLen + pos[e] % kPageLen;
+      }
+#pragma unroll
+      for (uint32_t e = 0; e < N; e += 4) {
+        put4(p.pos, r0 + e, p.n_rows, pos + e);
+        put4(p.row_seq, r0 + e, p.n_rows, q + e);
+        if (p.slot) put4(p.slot, r0 + e, p.n_rows, slot + e);
       }
     }
-#pragma unroll
-    for (uint32_t e = 0; e < 4; ++e)
-      if (p.slot && r0 + e < T) slot[e] = slot[e] * kPageLen + pos[e] % kPageLen;
-    put4(p.pos, r0, p.n_rows, pos);
-    put4(p.row_seq, r0, p.n_rows, q);
-    if (p.slot) put4(p.slot, r0, p.n_rows, slot);
-  }
+  };
+  if (p.n_rows <= 4 * all) put_rows(std::integral_constant<uint32_t, 4>());
+  else put_rows(std::integral_constant<uint32_t, 8>());
   if (flags && p.err && (at < THREADS || (flags & kFlagPage))) atomicOr(p.err, flags);
 }
 
