@@ -23,11 +23,20 @@ namespace fa {
 // and its arithmetic goes (kept at run time it cost those calls 2%).
 struct PlainParams : AttnChunksParams {
   static constexpr uint32_t sinks = 0;
+  static constexpr bool packed = false;
 };
-struct SinkParams : AttnChunksParams {};
-template <typename F>
+struct SinkParams : AttnChunksParams {
+  static constexpr bool packed = false;
+};
+// Units of whole pages one behind another, those of the first positions, then the window's: kernels whose pages
+// come one by one need no unit that is mostly gap (a window of 2000 and 33 first positions in tiles of 128: 17 for
+// 18 or 19).
+struct PackedParams : AttnChunksParams {
+  static constexpr bool packed = true;
+};
+template <typename S, typename F>
 auto with_sinks(const AttnChunksParams &p, F f) {
-  if (p.sinks) return f(SinkParams{p});
+  if (p.sinks) return f(S{p});
   return f(PlainParams{p});
 }
 
@@ -88,13 +97,21 @@ __device__ __forceinline__ uint32_t sink_units(const PR &p, uint32_t lo) {
 }
 template <uint32_t U, typename PR>
 __device__ __forceinline__ uint32_t range_units(const PR &p, uint32_t lo, uint32_t hi) {
-  return hi > lo ? sink_units<U>(p, lo) + (hi - 1) / U - lo / U + 1 : 1;  // at least one: somebody writes the zeros
+  if (hi <= lo) return 1;  // at least one: somebody writes the zeros
+  if constexpr (PR::packed) return (sink_units<kPageLen>(p, lo) + (hi - 1) / kPageLen - lo / kPageLen + U / kPageLen) / (U / kPageLen);
+  return sink_units<U>(p, lo) + (hi - 1) / U - lo / U + 1;
 }
 // first position of unit u of an item
 template <uint32_t U, typename PR>
 __device__ __forceinline__ uint32_t unit_at(const PR &p, uint32_t lo, uint32_t u) {
   const uint32_t n = sink_units<U>(p, lo);
   return (u < n ? u : u - n + lo / U) * U;
+}
+// first position of page h of unit u
+template <uint32_t U, typename PR>
+__device__ __forceinline__ uint32_t unit_page(const PR &p, uint32_t lo, uint32_t u, uint32_t h) {
+  if constexpr (PR::packed) return unit_at<kPageLen>(p, lo, u * (U / kPageLen) + h);
+  return unit_at<U>(p, lo, u) + h * kPageLen;
 }
 // that of unit u + step, where unit u is at t
 template <uint32_t U, typename PR>

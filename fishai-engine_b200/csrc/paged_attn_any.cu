@@ -301,7 +301,7 @@ uint32_t launch_hj(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st, ui
   per_sm = per_sm > 3 ? 3 : per_sm;
   const uint32_t grid = n_sm * per_sm < kAttnMaxCtas ? n_sm * per_sm : kAttnMaxCtas;
   *rows = R;
-  return with_sinks(p, [&](auto a) -> uint32_t {
+  return with_sinks<SinkParams>(p, [&](auto a) -> uint32_t {
     using PR = decltype(a);
     if (cudaFuncSetAttribute(k_attn_any<T, HJ, PR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)any_smem<T>(64 * HJ)) != cudaSuccess) return 0;
     k_attn_any<T, HJ><<<grid, kAnyThreads, smem, st>>>(a);
@@ -312,7 +312,7 @@ template <typename T, uint32_t HJ>
 struct LaunchAny {
   static uint32_t walk(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st, uint32_t *rows) { return launch_hj<T, HJ>(p, n_sm, st, rows); }
   static int one(const AttnChunksParams &p, cudaStream_t st) {
-    return with_sinks(p, [&](auto a) { return launch_one<k_attn_any_one<T, HJ, decltype(a)>>(a, one_items(p), kAnyThreads, any_smem<T>(64 * HJ), st); });
+    return with_sinks<SinkParams>(p, [&](auto a) { return launch_one<k_attn_any_one<T, HJ, decltype(a)>>(a, one_items(p), kAnyThreads, any_smem<T>(64 * HJ), st); });
   }
 };
 // f(LaunchAny of the call's type, rows and head size)

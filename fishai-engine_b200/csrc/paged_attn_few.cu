@@ -320,7 +320,7 @@ struct LaunchFew {
     per_sm = per_sm > 3 ? 3 : per_sm;
     const uint32_t grid = n_sm * per_sm < kAttnMaxCtas ? n_sm * per_sm : kAttnMaxCtas;
     *rows = R;
-    return with_sinks(p, [&](auto a) -> uint32_t {
+    return with_sinks<SinkParams>(p, [&](auto a) -> uint32_t {
       using PR = decltype(a);
       if (cudaFuncSetAttribute(k_attn_few<T, R, DPL, PR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::smem(32 * DPL)) != cudaSuccess) return 0;
       k_attn_few<T, R, DPL><<<grid, kThreads, smem, st>>>(a);
@@ -328,7 +328,7 @@ struct LaunchFew {
     });
   }
   static int one(const AttnChunksParams &p, cudaStream_t st) {
-    return with_sinks(p, [&](auto a) { return launch_one<k_attn_few_one<T, R, DPL, decltype(a)>>(a, one_items(p), kThreads, C::smem(32 * DPL), st); });
+    return with_sinks<SinkParams>(p, [&](auto a) { return launch_one<k_attn_few_one<T, R, DPL, decltype(a)>>(a, one_items(p), kThreads, C::smem(32 * DPL), st); });
   }
 };
 // f(LaunchFew of the call's type, rows and head size)

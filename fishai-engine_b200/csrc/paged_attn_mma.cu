@@ -84,6 +84,24 @@ __device__ __forceinline__ uint32_t sw(uint32_t r, uint32_t c) {
   return r * (HD * 2) + ((c ^ (r & 7)) << 4);
 }
 
+// where the two pages of a sub-tile begin
+struct Tile {
+  uint32_t t[2];
+};
+// sub-tile h of unit u
+template <uint32_t U, typename PR>
+__device__ __forceinline__ Tile tile_at(const PR &p, uint32_t lo, uint32_t u, uint32_t h = 0) {
+  const uint32_t t = unit_page<U>(p, lo, u, 2 * h);
+  return {{t, PR::packed ? unit_page<U>(p, lo, u, 2 * h + 1) : t + kPageLen}};
+}
+// that of unit u + step, where unit u is a sub-tile at `at`
+template <typename PR>
+__device__ __forceinline__ Tile tile_after(const PR &p, uint32_t lo, uint32_t u, const Tile &at, uint32_t step) {
+  if constexpr (PR::packed) return tile_at<kSub>(p, lo, u + step);
+  const uint32_t t = unit_after<kSub>(p, lo, u, at.t[0], step);
+  return {{t, t + kPageLen}};
+}
+
 // The rows of one warp: 16 rows of the item, this thread's rows g and g + 8
 // (MMA fragment layout), with the running softmax and output.
 template <typename T, uint32_t HD>
@@ -144,16 +162,17 @@ struct Rows {
 
   // s -> weights; the running maximum, sum and output follow
   template <typename PR>
-  __device__ void softmax(const PR &p, uint32_t t0, float (&s)[kSub / 8][4]) {
+  __device__ void softmax(const PR &p, const Tile &at, float (&s)[kSub / 8][4]) {
     const uint32_t c = threadIdx.x & 3;
-    const bool all = (int32_t)(t0 + kSub - 1) <= pos_min && (!p.window || pos_max - (int32_t)t0 < (int32_t)p.window || t0 + kSub <= p.sinks);
+    auto in = [&](uint32_t t) { return pos_max - (int32_t)t < (int32_t)p.window || t + kPageLen <= p.sinks; };
+    const bool all = (int32_t)(at.t[1] + kPageLen - 1) <= pos_min && (!p.window || (in(at.t[0]) && (!PR::packed || in(at.t[1]))));
     float mx[2] = {-INFINITY, -INFINITY};
     if (!all) {
 #pragma unroll
       for (uint32_t j = 0; j < kSub / 8; ++j)
 #pragma unroll
         for (uint32_t e = 0; e < 4; ++e)
-          if (!token_sees(p, pos[e >> 1], (int32_t)(t0 + 8 * j + 2 * c + (e & 1)))) s[j][e] = -INFINITY;
+          if (!token_sees(p, pos[e >> 1], (int32_t)(at.t[j / 2] + 8 * (j % 2) + 2 * c + (e & 1)))) s[j][e] = -INFINITY;
     }
 #pragma unroll
     for (uint32_t j = 0; j < kSub / 8; ++j)
@@ -207,31 +226,31 @@ struct Rows {
   }
 };
 
-// Where a warp's copies of 32 positions come from: pages of positions t0 and
-// t0 + 16 (looked up one sub-tile ahead).
+// Where a warp's copies of a sub-tile come from (looked up one sub-tile ahead).
 struct PagePair {
   uint32_t page[2];
 };
 template <typename PR>
-__device__ __forceinline__ PagePair look_up(const PR &p, const uint32_t *pt, uint32_t t0, uint32_t lo, uint32_t hi) {
+__device__ __forceinline__ PagePair look_up(const PR &p, const uint32_t *pt, const Tile &at, uint32_t lo, uint32_t hi) {
   PagePair r;
 #pragma unroll
   for (uint32_t i = 0; i < 2; ++i) {
-    const uint32_t t = t0 + 16 * i;
+    const uint32_t t = at.t[i];
     r.page[i] = item_reads(p, lo, hi, t) ? __ldg(pt + t / kPageLen) : 0u;  // only pages that are read are looked up
   }
   return r;
 }
-// K (is_v 0) or V rows of positions [t0, t0 + 32) to a tile; THREADS threads,
+// K (is_v 0) or V rows of a sub-tile's positions to shared memory; THREADS threads,
 // thread i of them.  Positions that the item does not see and bad pages become zeros.
 template <typename T, uint32_t HD, typename PR>
 __device__ __forceinline__ void stage(const PR &p, const T *base, const PagePair &pg, uint32_t head, uint32_t is_v,
-                                      uint32_t t0, uint32_t lo, uint32_t hi, uint32_t tile, uint32_t i, uint32_t threads) {
+                                      const Tile &at, uint32_t lo, uint32_t hi, uint32_t tile, uint32_t i, uint32_t threads) {
   constexpr uint32_t CH = HD / 8;  // pieces of a row
   const uint32_t c = i % CH, r0 = i / CH, step = threads / CH;
   // most sub-tiles are seen whole: no questions row by row (with first positions, those took a third of a
   // sub-tile's instructions: one token over 8160 positions and 4 first ones 18.5 us, 14.1 so)
-  const bool whole = t0 + kSub <= hi && (t0 >= lo || t0 + kSub <= p.sinks);
+  auto seen = [&](uint32_t t) { return t >= lo || t + kPageLen <= p.sinks; };
+  const bool whole = at.t[1] + kPageLen <= hi && seen(at.t[0]) && (!PR::packed || seen(at.t[1]));
 #pragma unroll
   for (uint32_t half = 0; half < 2; ++half) {
     const bool good = pg.page[half] < p.pg.n_pages;
@@ -242,7 +261,7 @@ __device__ __forceinline__ void stage(const PR &p, const T *base, const PagePair
     } else {
 #pragma unroll
       for (uint32_t r = 0; r < 16; r += step) {
-        const uint32_t row = r + r0, t = t0 + 16 * half + row;
+        const uint32_t row = r + r0, t = at.t[half] + row;
         cp16(tile + sw<HD>(16 * half + row, c), src + row * HD, good && item_sees(p, lo, hi, t));
       }
     }
@@ -323,20 +342,20 @@ __device__ __forceinline__ void walk_tiles(const PR &p, const T *base, const Seg
                                            uint32_t ktile, uint32_t vtile, Rows<T, HD> &rows, Q q) {
   const uint32_t *pt = p.pg.page_table + (uint64_t)s.chunk.seq * p.pg.max_pages;
   const uint32_t lane = threadIdx.x & 31;
-  uint32_t t0 = unit_at<kSub>(p, s.lo, u);
-  PagePair pg = look_up(p, pt, t0, s.lo, s.hi);
+  Tile at = tile_at<kSub>(p, s.lo, u);
+  PagePair pg = look_up(p, pt, at, s.lo, s.hi);
   if (u < n) {
     flag_bad_pages(p, pg);
-    stage<T, HD>(p, base, pg, s.head, 0, t0, s.lo, s.hi, ktile, lane, 32);
+    stage<T, HD>(p, base, pg, s.head, 0, at, s.lo, s.hi, ktile, lane, 32);
     cp_commit();
-    stage<T, HD>(p, base, pg, s.head, 1, t0, s.lo, s.hi, vtile, lane, 32);
+    stage<T, HD>(p, base, pg, s.head, 1, at, s.lo, s.hi, vtile, lane, 32);
     cp_commit();
   }
-  PagePair ahead = look_up(p, pt, unit_after<kSub>(p, s.lo, u, t0, step), s.lo, s.hi);
+  PagePair ahead = look_up(p, pt, tile_after(p, s.lo, u, at, step), s.lo, s.hi);
   q();
   for (; u < n; u += step) {
     const bool more = u + step < n;
-    const uint32_t t1 = unit_after<kSub>(p, s.lo, u, t0, step);
+    const Tile next = tile_after(p, s.lo, u, at, step);
     float sc[kSub / 8][4];
     cp_wait<1>();
     __syncwarp();
@@ -345,18 +364,18 @@ __device__ __forceinline__ void walk_tiles(const PR &p, const T *base, const Seg
     pg = ahead;
     if (more) {
       flag_bad_pages(p, pg);
-      stage<T, HD>(p, base, pg, s.head, 0, t1, s.lo, s.hi, ktile, lane, 32);
+      stage<T, HD>(p, base, pg, s.head, 0, next, s.lo, s.hi, ktile, lane, 32);
     }
     cp_commit();
-    ahead = look_up(p, pt, unit_after<kSub>(p, s.lo, u + step, t1, step), s.lo, s.hi);
-    rows.softmax(p, t0, sc);
+    ahead = look_up(p, pt, tile_after(p, s.lo, u + step, next, step), s.lo, s.hi);
+    rows.softmax(p, at, sc);
     cp_wait<1>();
     __syncwarp();
     rows.add_values(vtile, sc);
     __syncwarp();
-    if (more) stage<T, HD>(p, base, pg, s.head, 1, t1, s.lo, s.hi, vtile, lane, 32);
+    if (more) stage<T, HD>(p, base, pg, s.head, 1, next, s.lo, s.hi, vtile, lane, 32);
     cp_commit();
-    t0 = t1;
+    at = next;
   }
   cp_wait<0>();
   rows.finish();
@@ -406,7 +425,7 @@ uint32_t launch_hd(const AttnChunksParams &p, uint32_t n_sm, cudaStream_t st) {
   // two tiles of 32 positions a warp, or the merge's 4 x 16 rows
   constexpr uint32_t kTiles = 4 * 2 * kSub * HD * 2, kMerge = Merge<HD, 4>::kBytes, kBytes = kTiles > kMerge ? kTiles : kMerge;
   const uint32_t grid = 3 * n_sm < kAttnMaxCtas ? 3 * n_sm : kAttnMaxCtas;
-  return with_sinks(p, [&](auto a) -> uint32_t {
+  return with_sinks<PackedParams>(p, [&](auto a) -> uint32_t {
     using PR = decltype(a);
     if (cudaFuncSetAttribute(k_attn_rows16<T, HD, PR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kBytes) != cudaSuccess) return 0;
     k_attn_rows16<T, HD><<<grid, kThreads, kBytes, st>>>(a);
@@ -449,7 +468,7 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 1 : 2) k_attn_one16(c
 // positions: 5.8 us against 6.4).
 template <typename T, uint32_t HD>
 int launch_one_hd(const AttnChunksParams &p, uint64_t span, cudaStream_t st) {
-  return with_sinks(p, [&](auto a) {
+  return with_sinks<PackedParams>(p, [&](auto a) {
     using PR = decltype(a);
     if (span > kOneCtas * 6 * kSub) {
       const int rc = launch_one<k_attn_one16<T, HD, 8, PR>>(a, one_items(p), 256, OneCfg<HD, 8>::kBytes, st);
@@ -491,17 +510,17 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_short(const PR p) {
   // K and V of tile u, whose pages are looked up a tile ahead, to buffer `which`
   PagePair ahead[2];
   auto pages = [&](uint32_t u) {
-    const uint32_t t = unit_at<kShortPos>(p, s.lo, u);
 #pragma unroll
-    for (uint32_t h = 0; h < 2; ++h) ahead[h] = look_up(p, pt, t + h * kSub, s.lo, s.hi);
+    for (uint32_t h = 0; h < 2; ++h) ahead[h] = look_up(p, pt, tile_at<kShortPos>(p, s.lo, u, h), s.lo, s.hi);
   };
   auto fetch = [&](uint32_t u, uint32_t which) {
-    const uint32_t k = smem_u32(dsm) + which * 2 * S::kTile, t = unit_at<kShortPos>(p, s.lo, u);
+    const uint32_t k = smem_u32(dsm) + which * 2 * S::kTile;
 #pragma unroll
     for (uint32_t h = 0; h < 2; ++h) {
+      const Tile at = tile_at<kShortPos>(p, s.lo, u, h);
       flag_bad_pages(p, ahead[h]);
-      stage<T, HD>(p, base, ahead[h], s.head, 0, t + h * kSub, s.lo, s.hi, k + h * S::kHalf, tid, kThreads);
-      stage<T, HD>(p, base, ahead[h], s.head, 1, t + h * kSub, s.lo, s.hi, k + S::kTile + h * S::kHalf, tid, kThreads);
+      stage<T, HD>(p, base, ahead[h], s.head, 0, at, s.lo, s.hi, k + h * S::kHalf, tid, kThreads);
+      stage<T, HD>(p, base, ahead[h], s.head, 1, at, s.lo, s.hi, k + S::kTile + h * S::kHalf, tid, kThreads);
     }
     pages(u + C);
   };
@@ -517,14 +536,14 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_short(const PR p) {
   for (uint32_t which = 0; u < n; u += C, which ^= 1) {
     cp_wait<1>();
     __syncthreads();
-    const uint32_t k = smem_u32(dsm) + which * 2 * S::kTile, t0 = unit_at<kShortPos>(p, s.lo, u);
+    const uint32_t k = smem_u32(dsm) + which * 2 * S::kTile;
 #pragma unroll
     for (uint32_t h = 0; h < 2; ++h) {
-      const uint32_t t = t0 + h * kSub;
-      if (!mine || (int32_t)t > rows.pos_max) continue;  // nothing of it is seen
+      const Tile at = tile_at<kShortPos>(p, s.lo, u, h);
+      if (!mine || (int32_t)at.t[0] > rows.pos_max) continue;  // nothing of it is seen
       float sc[kSub / 8][4];
       rows.scores(k + h * S::kHalf, sc);
-      rows.softmax(p, t, sc);
+      rows.softmax(p, at, sc);
       rows.add_values(k + S::kTile + h * S::kHalf, sc);
     }
     __syncthreads();
@@ -549,7 +568,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_short(const PR p) {
 }
 template <typename T, uint32_t HD, uint32_t C>
 int launch_short_c(const AttnChunksParams &p, uint64_t items, cudaStream_t st) {
-  return with_sinks(p, [&](auto a) { return launch_one<k_attn_short<T, HD, C, decltype(a)>, C>(a, items, kThreads, ShortCfg<HD>::kBytes, st); });
+  return with_sinks<PackedParams>(p, [&](auto a) { return launch_one<k_attn_short<T, HD, C, decltype(a)>, C>(a, items, kThreads, ShortCfg<HD>::kBytes, st); });
 }
 template <typename T, uint32_t HD>
 int launch_short_hd(const AttnChunksParams &p, uint64_t items, uint32_t c, cudaStream_t st) {

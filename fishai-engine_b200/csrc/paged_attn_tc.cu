@@ -257,7 +257,18 @@ __device__ void softmax_role(const PR &p, TcWalk<G> w, TcBars &b, uint32_t tmem,
     const uint32_t tiles = s.hi > s.lo ? s.u1 - s.u0 : 0;
     float m = -INFINITY, l = 0.0f;
     for (uint32_t k = 0; k < tiles; ++k, ++n) {
-      const uint32_t t0 = unit_at<kTcPos>(p, s.lo, s.u0 + k);
+      // column c of the tile is position t0 + c; with first positions, its columns below `keep` are those
+      uint32_t t0;
+      int32_t keep = 0;
+      if constexpr (PR::packed) {
+        constexpr uint32_t kPages = kTcPos / kPageLen;
+        const uint32_t n = sink_units<kPageLen>(p, s.lo), j = (s.u0 + k) * kPages;
+        t0 = (s.lo / kPageLen + j - n) * kPageLen;
+        keep = (int32_t)p.sinks - (int32_t)(j * kPageLen);
+        if (n < s.lo / kPageLen) keep = min(keep, (int32_t)((n - min(n, j)) * kPageLen));  // the window's pages are elsewhere
+      } else {
+        t0 = unit_at<kTcPos>(p, s.lo, s.u0 + k);
+      }
       if (!wait_bar(&b.abort, &b.s_full[g], n & 1)) return;
       if (idle) {
         mbar_arrive(&b.p_half[g]);
@@ -277,7 +288,7 @@ __device__ void softmax_role(const PR &p, TcWalk<G> w, TcBars &b, uint32_t tmem,
           if (c >= to) x[c] = -INFINITY;
       }
       if (p.window && !__all_sync(0xFFFFFFFFu, !live || to <= (int32_t)p.window)) {
-        const int32_t from = to - (int32_t)p.window, keep = (int32_t)p.sinks - (int32_t)t0;  // columns below `keep` stay
+        const int32_t from = to - (int32_t)p.window;
         if (keep <= 0) {
 #pragma unroll
           for (int32_t c = 0; c < (int32_t)kTcPos; ++c)
@@ -475,15 +486,15 @@ __device__ void load_role(const PR &p, TcWalk<G> w, TcBars &b, uint32_t smem, co
   for (Segment s; w.next(p, s);) {
     const uint32_t tiles = s.hi > s.lo ? s.u1 - s.u0 : 0;
     const uint32_t *pt = p.pg.page_table + (uint64_t)s.chunk.seq * p.pg.max_pages;
-    auto look_up = [&](uint32_t t0) -> uint32_t {  // the lane's page of the tile
-      const uint32_t t = t0 + (lane & 7) * kPageLen;
+    auto look_up = [&](uint32_t t) -> uint32_t {
       return item_reads(p, s.lo, s.hi, t) ? __ldg(pt + t / kPageLen) : 0xFFFFFFFFu;
     };
-    const uint32_t first = unit_at<kTcPos>(p, s.lo, s.u0);
-    uint32_t ahead = tiles ? look_up(first) : 0;
+    uint32_t next = unit_page<kTcPos>(p, s.lo, s.u0, lane & 7);  // where the lane's page of the tile begins
+    uint32_t ahead = tiles ? look_up(next) : 0;
     for (uint32_t k = 0; k < tiles; ++k) {
-      const uint32_t t0 = unit_after<kTcPos>(p, s.lo, s.u0, first, k), page = ahead, at = t0 + (lane & 7) * kPageLen;
-      if (k + 1 < tiles) ahead = look_up(unit_after<kTcPos>(p, s.lo, s.u0 + k, t0, 1));
+      const uint32_t page = ahead, at = next;
+      next = PR::packed ? unit_page<kTcPos>(p, s.lo, s.u0 + k + 1, lane & 7) : at + kTcPos;
+      if (k + 1 < tiles) ahead = look_up(next);
       const bool used = item_reads(p, s.lo, s.hi, at);
       if (used && page >= p.pg.n_pages && p.err) atomicOr(p.err, kFlagPage);
       // A page with slots that nobody sees: V must not be NaN there (its weight 0
@@ -501,7 +512,7 @@ __device__ void load_role(const PR &p, TcWalk<G> w, TcBars &b, uint32_t smem, co
           tma_2d(dst + (lane >> 3) * C::kHalf + (lane & 7) * 2048, map, (int32_t)(lane >> 3) * 64, map_row(p.pg, page, is_v, s.head), &b.full[st]);
         if (go && is_v)
           for (uint32_t m = parts; m; m &= m - 1) {
-            const uint32_t j = __ffs(m) - 1, pg = __shfl_sync(0xFFFFFFFFu, page, j), t = t0 + j * kPageLen + (lane & 15), half = lane >> 4;
+            const uint32_t j = __ffs(m) - 1, pg = __shfl_sync(0xFFFFFFFFu, page, j), t = __shfl_sync(0xFFFFFFFFu, at, j) + (lane & 15), half = lane >> 4;
             const bool seen = item_sees(p, s.lo, s.hi, t);
             if (half < HD / 64)
               tma_2d(dst + half * C::kHalf + j * 2048 + (lane & 15) * 128, row_map, (int32_t)half * 64,
@@ -608,7 +619,7 @@ uint32_t launch_g(const AttnChunksParams &p, uint32_t n_sm, bool overlap, cudaSt
   CUtensorMap map, row_map;
   if (!page_map(p, kPageLen, &map) || !page_map(p, 1, &row_map)) return 0;
   const uint32_t ctas = (n_sm < kTcMaxCtas ? n_sm : kTcMaxCtas) * (3 - G);  // one or two an SM
-  return with_sinks(p, [&](auto a) -> uint32_t {
+  return with_sinks<PackedParams>(p, [&](auto a) -> uint32_t {
     using PR = decltype(a);
     if (cudaFuncSetAttribute(k_attn_tc<T, HD, G, PR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::kSmem) != cudaSuccess) return 0;
     if (overlap) return launch_pdl(k_attn_tc<T, HD, G, PR>, dim3(ctas), dim3(C::kThreads), C::kSmem, st, a, map, row_map) ? 0 : ctas;
