@@ -17,6 +17,10 @@
 // the few elements of the bins around the place, which CTA 0 sorts.  Where more are in the bracket
 // than it sorts (flat rows, equal logits), its range of values is halved until it does, or one
 // value is left and the place is an id.
+//
+// A row alone waits for its exchanges (1 us each) and three passes of 2 to 5 us: of 128256 in f32
+// 10 us without cuts, 12 with top-k, 26 with top-p.  Many rows are bound by issue slots and the rows that
+// have most to do: 64 with cuts of all kinds 39 us, without 26; 200 of 32000 in bf16 18.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

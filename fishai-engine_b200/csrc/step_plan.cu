@@ -15,6 +15,8 @@
 // pages that are taken, and the rows, each finding its request by a binary search in
 // the sums, so that one long sequence does not keep a warp while the others wait;
 // a barrier of the cluster stands where one's writes are another's reads.
+// Eight decode requests 6.2 us, 512 requests with 66000 rows 14.4 (a warp to a request's
+// pages and a thread to a row, eight CTAs of 512 threads: 28.7).
 #include <type_traits>
 
 #include "fa_device.cuh"
