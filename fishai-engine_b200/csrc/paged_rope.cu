@@ -80,7 +80,7 @@ __device__ __forceinline__ uint32_t pack(const __nv_bfloat16 *p, float a, float 
 // token's is always in flight while one is turned and stored.  (A CTA a token,
 // loading after its angles: 46 us for 8192 tokens of 48 heads.)
 constexpr uint32_t kRopeTokens = 4;
-template <typename TI, typename TO, int W, bool AXES>
+template <typename TI, typename TO, int W, bool AXES, int HALF>
 __global__ void __launch_bounds__(512, 3) k_rope_append(const RopeAppendParams p, const __grid_constant__ RopeTable tab, uint32_t each) {
   __shared__ __align__(16) float cs[kRopeTokens][kMaxHeadDim / 2], sn[kRopeTokens][kMaxHeadDim / 2];
   __shared__ uint64_t place[kRopeTokens];  // element offset of the token's slot in a (K, head 0) block
@@ -94,9 +94,12 @@ __global__ void __launch_bounds__(512, 3) k_rope_append(const RopeAppendParams p
   const uint32_t head = u / uph, w = u - head * uph;
   const bool turn = head < H + KVH && w < upr, is_q = head < H, is_v = head >= H + KVH;
   // offsets of the unit's two parts: pairs of the half layout, else 2 W
-  // consecutive elements
-  const uint32_t o0 = turn && p.half_layout ? w * W : w * 2 * W;
-  const uint32_t o1 = turn && p.half_layout ? half + w * W : w * 2 * W + W;
+  // consecutive elements, or (16-bit types) W in each half of the head, so that
+  // the accesses of neighbours adjoin
+  constexpr bool kWords = W == 8 && sizeof(TI) == 2 && sizeof(TO) == 2;
+  const bool in_halves = HALF < 0 ? p.half_layout : HALF, spread = kWords && (is_v || !in_halves);
+  const uint32_t o0 = (turn && in_halves) || spread ? w * W : w * 2 * W;
+  const uint32_t o1 = spread ? hd / 2 + w * W : turn && in_halves ? half + w * W : w * 2 * W + W;
   const uint64_t ss = is_q ? p.qs : is_v ? p.vs : p.ks;
   const TI *src = reinterpret_cast<const TI *>(is_q ? p.q : is_v ? p.v : p.k) + t0 * ss + (head - (is_q ? 0 : is_v ? H + KVH : H)) * hd;
   Vec<TI, W> a0{}, a1{};
@@ -121,18 +124,23 @@ __global__ void __launch_bounds__(512, 3) k_rope_append(const RopeAppendParams p
     const double a = (double)p.pos[t0 + k + (AXES ? tab.axis[j] * p.pos_stride : 0)] * tab.turns[j];
     float s, c;
     sincospif(2.0f * (float)(a - rint(a)), &s, &c);
-    cs[k][j] = c * tab.scale;
-    sn[k][j] = s * tab.scale;
+    // half layout in 16-bit types: units 4 to 7 find their angles' two pieces swapped, and the eight units of a head
+    // read from 32 banks (8192 tokens: 42.7 us unswapped, 41.2 so)
+    const uint32_t at = HALF == 1 ? j ^ (j >> 3 & 4) : j;
+    cs[k][at] = c * tab.scale;
+    sn[k][at] = s * tab.scale;
   }
   __syncthreads();
   if (!live) return;
   TO *out = is_q ? reinterpret_cast<TO *>(p.out) + t0 * p.os + head * hd
                  : reinterpret_cast<TO *>(p.pg.base) + (uint64_t)p.layer * p.pg.layer_stride +
                        (uint64_t)(head - H) * kPageLen * hd;  // K heads, then V heads of a page
-  if constexpr (W == 8 && sizeof(TI) == 2 && sizeof(TO) == 2) {
+  if constexpr (kWords) {
     // word by word, and at most 42 registers: more threads hold loads on their way (8192 tokens of 48 heads x
-    // 128, bf16: 41 us, 43 with three axes; all 16 elements as f32 at once in 61 registers 49 and 51; in 32
-    // registers 49.  A copy of as many bytes takes 34.)
+    // 128: 39 us interleaved, 41 halves with three axes; all 16 elements as f32 at once in 61 registers 49 and 51; in
+    // 32 registers 49; all four tokens' pieces to shared memory by cp.async at the start 51 and 41; CTAs that stay
+    // and go through 14 tokens one after another 58 and 60.  Interleaved in accesses to every other 16 bytes, as
+    // two pieces that adjoin would be: 44.  A copy of as many bytes takes 34.)
     const TI *ti = nullptr;
     const TO *to = nullptr;
     for (uint32_t k = 0; k < nt; ++k) {
@@ -144,28 +152,37 @@ __global__ void __launch_bounds__(512, 3) k_rope_append(const RopeAppendParams p
         a0 = load_n<V, W>(src + o0);
         a1 = load_n<V, W>(src + o1);
       }
-      if (turn) {
+      if (HALF == 1 && turn) {
 #pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) {
-          if (p.half_layout) {  // elements of two pairs in a word of each part
-            const float2 c = *reinterpret_cast<const float2 *>(&cs[k][w * W + 2 * i]), s = *reinterpret_cast<const float2 *>(&sn[k][w * W + 2 * i]);
-            const float2 va = unpack(ti, r[0][i]), vb = unpack(ti, r[1][i]);
-            o[0][i] = pack(to, va.x * c.x - vb.x * s.x, va.y * c.y - vb.y * s.y);
-            o[1][i] = pack(to, va.x * s.x + vb.x * c.x, va.y * s.y + vb.y * c.y);
-          } else {  // a pair in a word
+        for (uint32_t h = 0; h < 2; ++h) {  // elements of two pairs in a word of each part
+          const float4 c = *reinterpret_cast<const float4 *>(&cs[k][(w * W + 4 * h) ^ (w & 4)]), s = *reinterpret_cast<const float4 *>(&sn[k][(w * W + 4 * h) ^ (w & 4)]);
+          const float cv[4] = {c.x, c.y, c.z, c.w}, sv[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
-            for (uint32_t h = 0; h < 2; ++h) {
-              const float c = cs[k][w * W + 4 * h + i], s = sn[k][w * W + 4 * h + i];
-              const float2 v = unpack(ti, r[h][i]);
-              o[h][i] = pack(to, v.x * c - v.y * s, v.x * s + v.y * c);
-            }
+          for (uint32_t i = 0; i < 2; ++i) {
+            const float2 va = unpack(ti, r[0][2 * h + i]), vb = unpack(ti, r[1][2 * h + i]);
+            o[0][2 * h + i] = pack(to, va.x * cv[2 * i] - vb.x * sv[2 * i], va.y * cv[2 * i + 1] - vb.y * sv[2 * i + 1]);
+            o[1][2 * h + i] = pack(to, va.x * sv[2 * i] + vb.x * cv[2 * i], va.y * sv[2 * i + 1] + vb.y * cv[2 * i + 1]);
           }
         }
       } else {
 #pragma unroll
-        for (uint32_t i = 0; i < 8; ++i) {
-          const float2 v = unpack(ti, r[i / 4][i % 4]);
-          o[i / 4][i % 4] = __is_same(TI, TO) ? r[i / 4][i % 4] : pack(to, v.x, v.y);
+        for (uint32_t h = 0; h < 2; ++h) {
+          const uint32_t e = h ? o1 : o0;
+          if (!HALF && !is_v && e < p.rot) {  // a pair in a word
+            const float4 c = *reinterpret_cast<const float4 *>(&cs[k][e / 2]), s = *reinterpret_cast<const float4 *>(&sn[k][e / 2]);
+            const float cv[4] = {c.x, c.y, c.z, c.w}, sv[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+              const float2 v = unpack(ti, r[h][i]);
+              o[h][i] = pack(to, v.x * cv[i] - v.y * sv[i], v.x * sv[i] + v.y * cv[i]);
+            }
+          } else {
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+              const float2 v = unpack(ti, r[h][i]);
+              o[h][i] = __is_same(TI, TO) ? r[h][i] : pack(to, v.x, v.y);
+            }
+          }
         }
       }
       const uint64_t at = place[k];
@@ -240,10 +257,11 @@ int launch_io(const RopeAppendParams &p, const RopeTable &t, cudaStream_t st) {
   if ((units + block - 1) / block > 65535) block = 512;  // grid y (thousands of heads)
   const dim3 grid((p.n_tokens + each - 1) / each, (units + block - 1) / block);
   if constexpr (sizeof(TI) == 2 && sizeof(TO) == 2) {
-    if (W == 8) k_rope_append<TI, TO, 8, AXES><<<grid, block, 0, st>>>(p, t, each);
+    if (W == 8 && p.half_layout) k_rope_append<TI, TO, 8, AXES, 1><<<grid, block, 0, st>>>(p, t, each);
+    if (W == 8 && !p.half_layout) k_rope_append<TI, TO, 8, AXES, 0><<<grid, block, 0, st>>>(p, t, each);
   }
-  if (W == 4) k_rope_append<TI, TO, 4, AXES><<<grid, block, 0, st>>>(p, t, each);
-  if (W == 1) k_rope_append<TI, TO, 1, AXES><<<grid, block, 0, st>>>(p, t, each);
+  if (W == 4) k_rope_append<TI, TO, 4, AXES, -1><<<grid, block, 0, st>>>(p, t, each);
+  if (W == 1) k_rope_append<TI, TO, 1, AXES, -1><<<grid, block, 0, st>>>(p, t, each);
   return cudaGetLastError() == cudaSuccess ? 0 : -1;
 }
 template <typename TI, bool AXES>

@@ -111,6 +111,14 @@ def test_sizes(tokens, heads, kvh, hd):
     check(tokens, heads, kvh, hd, torch.float16, torch.float16, "half", seed=tokens, axes=[hd // 2 - 2, 1, 1], axis_order="turns")
 
 
+# heads that are turned in part, in 16-byte pieces: what is turned ends in either half of the head
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("hd,rot", [(16, 16), (80, 48), (96, 80), (112, 96), (128, 32), (240, 32), (256, 256)])
+@pytest.mark.parametrize("tin,tout", [("bf16", "bf16"), ("f16", "bf16"), ("bf16", "f16")])
+def test_partly_turned_heads(hd, rot, layout, tin, tout):
+    check(701, 5, 1, hd, R.TYPES[tin], R.TYPES[tout], layout, rot_dim=rot, axes=[rot // 2 - 3, 2, 1], axis_order="turns")
+
+
 def test_row_strides_of_the_positions():
     check(17, 4, 2, 64, torch.float16, torch.float16, "half", axes=[12, 10, 10], gap=5)
     check(17, 4, 2, 64, torch.float16, torch.float16, "half", axes=[12, 10, 10], broadcast=True)
