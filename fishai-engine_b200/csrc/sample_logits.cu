@@ -156,8 +156,7 @@ struct Row {
 
   // 2^-z in 64 bits, table-driven: 2^(n / 512) from a table, 2^(f / 512), |f| <= 1/2, from the series to
   // f^3 (the next term is below 2^-46.7).  For z <= 64, so the exponent stays in range.  The 64-bit
-  // pipe (64 lanes a clock and SM) is what a pass waits for: a table of 32 and the series to f^5
-  // took TIME_A.
+  // pipe has 64 lanes a clock and SM: a longer table for two terms less (a table of 32 needs the series to f^5).
   __device__ double weight(float v) const {
     const double d = (double)v - mxd, big = 6755399441055744.0;  // 1.5 * 2^52: the sum's low word is the nearest whole number
     const double t = fma(d, c512, big);
