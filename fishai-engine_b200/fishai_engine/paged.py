@@ -69,13 +69,23 @@ def _rows(t, name, n, width):
     return t.data_ptr(), stride[0] if n > 1 else width
 
 
-def _width(q, head_dim):
-    """elements of a row of whole heads"""
-    shape = q.shape
-    width = shape[1] if len(shape) == 2 else shape[1] * shape[2] if len(shape) == 3 else 0
+def _heads(q, head_dim):
+    """address, row stride, rows and elements of a row of q, rows of whole heads"""
+    shape, stride = q.shape, q.stride()
+    if len(shape) == 2:
+        n, width = shape
+        ok = stride[1] == 1
+    elif len(shape) == 3:
+        n, heads, hd = shape
+        width = heads * hd
+        ok = stride[2] == 1 and (heads == 1 or stride[1] == hd)
+    else:
+        n = width = ok = 0
     if not width or width % head_dim:
         raise ValueError(f"q: [tokens, heads * {head_dim}] or [tokens, heads, {head_dim}] needed, got {list(shape)}")
-    return width
+    if not ok:
+        _rows(q, "q", n, width)
+    return q.data_ptr(), stride[0] if n > 1 else width, n, width
 
 
 class PagedKV:
@@ -194,7 +204,6 @@ def rope_append(kv: PagedKV, layer: int, rope: Rope, q, k, v, positions, seqs, o
     and v are rows of one type, with any row stride (slices of a fused
     projection).  seqs[t] = NO_TOKEN leaves a row out.  A rope of several axes
     takes positions [axes, tokens] (any row stride) and needs slots."""
-    n = q.shape[0]
     dt = _code(q, "q")
     if layer >> 32:
         L.u32(layer=layer)
@@ -203,8 +212,7 @@ def rope_append(kv: PagedKV, layer: int, rope: Rope, q, k, v, positions, seqs, o
     if _code(out, "out") != kv.dtype:
         raise ValueError("out has another element type than the pages")
     hd, kw = kv.head_dim, kv._kv_width
-    width = _width(q, hd)
-    qp, qs = _rows(q, "q", n, width)
+    qp, qs, n, width = _heads(q, hd)
     kp, ks = _rows(k, "k", n, kw)
     vp, vs = _rows(v, "v", n, kw)
     op, os = _rows(out, "out", n, width)
@@ -248,14 +256,13 @@ def attention(kv: PagedKV, layer: int, q, q_start, kv_len, out, max_q: int, work
     max_q: no chunk is longer.  workspace: a uint8 tensor of
     workspace_bytes(head_dim), used by no other call that may run at the same
     time.  scale 0: 1 / sqrt(head_dim)."""
-    n, t = kv_len.shape[0], q.shape[0]
+    n = kv_len.shape[0]
     if _code(q, "q") != kv.dtype or out.dtype != q.dtype:
         raise ValueError("q and out have the pages' element type")
     if (layer | max_q | window | sinks) >> 32:
         L.u32(layer=layer, max_q=max_q, window=window, sinks=sinks)
     hd = kv.head_dim
-    width = _width(q, hd)
-    qp, qs = _rows(q, "q", t, width)
+    qp, qs, t, width = _heads(q, hd)
     op, os = _rows(out, "out", t, width)
     args = (kv._ref, layer, qp, qs, width // hd, n, _index(q_start, "q_start", n + 1), _index(kv_len, "kv_len", n),
             None if seqs is None else _index(seqs, "seqs", n), t, max_q, scale, window)
