@@ -20,7 +20,7 @@
 //
 // A row alone waits for its exchanges (1 us each) and three passes of 2 to 5 us: of 128256 in f32
 // 10 us without cuts, 12 with top-k, 26 with top-p.  Many rows are bound by issue slots and the rows that
-// have most to do: 64 with cuts of all kinds 39 us, without 26; 200 of 32000 in bf16 18.
+// have most to do: 64 with cuts of all kinds 31 us, without 27; 200 of 32000 in bf16 18.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -206,6 +206,27 @@ struct Row {
       for (uint32_t j = 0; j < 4; ++j)
         if (kept<CUT>(v[j], id + j)) f(v[j], id + j);
     }
+  }
+
+  // Whether row i goes by a histogram, which takes twice as long as all else.
+  __device__ bool lengthy(uint32_t i) const {
+    if (i >= p.n || (p.temperature && p.temperature[i] == 0.0f)) return false;
+    const uint32_t k = p.top_k && p.top_k[i] < p.vocab ? p.top_k[i] : 0;
+    return k ? k > kFewK : p.top_p && p.top_p[i] < 1.0f;
+  }
+  // The row that a call of at most a row a thread takes in place of row c: the lengthy ones first, which are else
+  // what the GPU ends with alone (64 rows of 128256, nine of them lengthy: 40 us as they are given, 42 with those
+  // last, 31 so; 64 lengthy ones 63.5, without the order 62).  In a kernel of its own: the choice at run time cost a row alone
+  // half a us.
+  __device__ uint32_t long_first(uint32_t c, bool lengthy) {
+    const uint32_t mask = __ballot_sync(0xFFFFFFFFu, lengthy);
+    if (lane == 0) s.redu[0][warp] = __popc(mask);
+    __syncthreads();
+    const uint32_t of = lane < kWarps ? s.redu[0][lane] : 0, all = __reduce_add_sync(0xFFFFFFFFu, of);
+    const uint32_t before = __reduce_add_sync(0xFFFFFFFFu, lane < warp ? of : 0) + __popc(mask & ((1u << lane) - 1));
+    if (tid < p.n && (lengthy ? before : all + tid - before) == c) s.bin = tid;
+    __syncthreads();
+    return s.bin;
   }
 
   // what every CTA says, the same m in all its threads; valid until the call after the next
@@ -875,11 +896,11 @@ struct Row {
 };
 
 // CUTS: top-k or top-p may be asked for.  Without, a row needs fewer registers and no lists, and three CTAs
-// fit on an SM (200 rows of 32000 in bf16: 18.4 us, with two 20.5).
-template <typename T, bool CUTS>
+// fit on an SM (200 rows of 32000 in bf16: 18.4 us, with two 20.5).  LONG_FIRST: rows in another order than given.
+template <typename T, bool CUTS, bool LONG_FIRST>
 __global__ void __launch_bounds__(kThreads, CUTS ? 2 : 3) k_sample_logits(const SampleParams p) {
   __shared__ Small s;
-  const uint32_t ctas = p.ctas, row = blockIdx.x / ctas;
+  const uint32_t ctas = p.ctas;
   Row<T> w(p, s);
   w.tid = threadIdx.x;
   w.lane = w.tid & 31;
@@ -892,7 +913,9 @@ __global__ void __launch_bounds__(kThreads, CUTS ? 2 : 3) k_sample_logits(const 
   w.mine = w.warp * 128 * p.groups + 4 * w.lane;
   // the others' shared memory may be written once all have begun: waited for before the first time
   asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  const bool lengthy = LONG_FIRST && w.lengthy(w.tid);
   s.power[w.tid] = exp2((double)w.tid / 512.0);
+  const uint32_t row = LONG_FIRST ? w.long_first(blockIdx.x / ctas, lengthy) : blockIdx.x / ctas;
   const uint32_t at = p.rows ? p.rows[row] : row;
   if (at == FA_NO_TOKEN) return;
   // the row's own settings: on their way while the logits are read
@@ -1022,10 +1045,10 @@ __global__ void __launch_bounds__(kThreads, CUTS ? 2 : 3) k_sample_logits(const 
   w.template draw<false>(row, (double)mp, (double)u);
 }
 
-template <typename T, bool CUTS>
+template <typename T, bool CUTS, bool LONG_FIRST = false>
 int launch(const SampleParams &p, cudaStream_t st) {
   const uint32_t smem = row_at<CUTS>(p.ctas) + p.groups * kGroup * (uint32_t)sizeof(T);
-  if (cudaFuncSetAttribute(k_sample_logits<T, CUTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSampleMaxSmem) != cudaSuccess) return -1;
+  if (cudaFuncSetAttribute(k_sample_logits<T, CUTS, LONG_FIRST>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSampleMaxSmem) != cudaSuccess) return -1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(p.n * p.ctas);
   cfg.blockDim = dim3(kThreads);
@@ -1037,7 +1060,7 @@ int launch(const SampleParams &p, cudaStream_t st) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, k_sample_logits<T, CUTS>, p) == cudaSuccess ? 0 : -1;
+  return cudaLaunchKernelEx(&cfg, k_sample_logits<T, CUTS, LONG_FIRST>, p) == cudaSuccess ? 0 : -1;
 }
 
 }  // namespace
@@ -1058,11 +1081,21 @@ int launch_sample_logits(const SampleParams &in, uint32_t n_sm, cudaStream_t st)
   static_assert(region(kMaxCtas) + kCtaBins * 8 + kSampleMaxVocab / kMaxCtas * 4 <= kSampleMaxSmem && kSampleMaxVocab % (kMaxCtas * kGroup) == 0,
                 "shared memory of the largest vocabulary");
   const bool cuts = p.top_k || p.top_p;
-  switch (p.dtype) {
-    case FA_KV_F32: return cuts ? launch<float, true>(p, st) : launch<float, false>(p, st);
-    case FA_KV_F16: return cuts ? launch<__half, true>(p, st) : launch<__half, false>(p, st);
-    default: return cuts ? launch<__nv_bfloat16, true>(p, st) : launch<__nv_bfloat16, false>(p, st);
-  }
+  // Where not all rows run at once the lengthy ones are taken first; not where a row's answer is written over
+  // settings that others have yet to look at.
+  auto apart = [&](const void *out, const void *in) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(out), b = reinterpret_cast<uintptr_t>(in), bytes = 4ull * p.n;
+    return !out || !in || a + bytes <= b || b + bytes <= a;
+  };
+  bool clear = true;
+  for (const void *out : {(const void *)p.ids, (const void *)p.logprobs, (const void *)p.err})
+    for (const void *in : {(const void *)p.temperature, (const void *)p.top_k, (const void *)p.top_p}) clear = clear && apart(out, in);
+  const bool first = cuts && clear && p.n <= kThreads && (uint64_t)p.n * p.ctas > 2 * n_sm;
+  auto run = [&](auto x) {
+    using T = decltype(x);
+    return first ? launch<T, true, true>(p, st) : cuts ? launch<T, true>(p, st) : launch<T, false>(p, st);
+  };
+  return p.dtype == FA_KV_F32 ? run(0.0f) : p.dtype == FA_KV_F16 ? run(__half()) : run(__nv_bfloat16());
 }
 
 }  // namespace fa

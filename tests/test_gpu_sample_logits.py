@@ -103,6 +103,41 @@ def test_many_rows(n):
           [rng.uniform(0.5, 1.0) for _ in range(n)], [rng.choice([0.0, 0.1]) for _ in range(n)])
 
 
+@pytest.mark.parametrize("n", [297, 480, 511, 512, 513])
+@pytest.mark.parametrize("where", ["none", "all", "first", "last", "scattered", "one"])
+def test_rows_with_long_cuts_anywhere(n, where):
+    """more rows than run at once, of which some go by a histogram: each is drawn once, whatever the order"""
+    rng = random.Random(n)
+    lengthy = {"none": [], "all": range(n), "first": range(40), "last": range(n - 40, n), "scattered": range(0, n, 7), "one": [n // 2]}[where]
+    vocab = 700
+    k, p, t = [rng.choice([0, 1, 20, 128, vocab]) for _ in range(n)], [1.0] * n, [rng.choice([0.7, 1.0, 1.5]) for _ in range(n)]
+    for i in lengthy:
+        k[i], p[i] = rng.choice([(0, 0.9), (vocab + 5, 0.5), (129, 1.0), (400, 0.8)])
+    for i in range(3, n, 11):
+        t[i] = 0.0
+    x = logits_of("text", n, vocab, torch.float32, n)
+    rows = list(range(n))
+    rng.shuffle(rows)
+    check(x, [rng.random() for _ in range(n)], t, k, p, None, rows)
+
+
+def test_answers_over_the_settings():
+    """ids in the place of top_k, log-probabilities in that of the temperatures or of top_p"""
+    n = 400
+    rng = random.Random(7)
+    x = logits_of("text", n, 900, torch.float32, 7)
+    u = f32([rng.random() for _ in range(n)])
+    k, p = i32([rng.choice([0, 0, 30, 200]) for _ in range(n)]), f32([rng.choice([1.0, 0.9, 0.6]) for _ in range(n)])
+    t = f32([rng.choice([0.0, 0.8, 1.2]) for _ in range(n)])
+    ids, logs = i32([-7] * n), torch.zeros(n, device="cuda")
+    sampling.sample_logits(x, u, ids, temperature=t, top_k=k, top_p=p, logprobs=logs)
+    for over in ("k and t", "p"):
+        kk, pp, tt, own = k.clone(), p.clone(), t.clone(), torch.zeros_like(ids)
+        out, lp = (kk, tt) if over == "k and t" else (own, pp)
+        sampling.sample_logits(x, u, out, temperature=tt, top_k=kk, top_p=pp, logprobs=lp)
+        assert torch.equal(out, ids) and torch.equal(lp, logs)
+
+
 def test_the_place_of_a_cut_among_equal_values():
     """a few distinct values, thousands of each: the cut falls inside one, at an id"""
     x = torch.tensor([[float((i * 7919) % 5) for i in range(40000)]] * 8, device="cuda")
