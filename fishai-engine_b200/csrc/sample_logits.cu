@@ -38,6 +38,8 @@ constexpr float kOctaves = 64.0f;
 constexpr double kHistError = 1.0 / 32768;      // of a sum of the histogram's masses: each is rounded to 2^-15 of its bin's largest, and exponentials are f32
 constexpr uint32_t kGroup = 4 * kThreads;       // elements of a CTA's group: four a thread, a warp's 128 in a row
 
+constexpr uint32_t kMostGroups = 32;            // of a CTA: a lane looks at each
+
 struct alignas(16) Msg {  // what a CTA tells the others
   double a, b;
   uint32_t c, d, e, f;
@@ -45,7 +47,7 @@ struct alignas(16) Msg {  // what a CTA tells the others
 struct Small {
   Msg msg[2][kMaxCtas];
   double red[kWarps], red2[kWarps];
-  double group[32];   // of a warp's groups
+  double group[kMostGroups];  // of a warp's groups
   uint32_t redu[4][kWarps];
   uint32_t bin, count, bins[2];
   double power[512];  // 2^(i / 512)
@@ -1069,7 +1071,8 @@ int launch_sample_logits(const SampleParams &in, uint32_t n_sm, cudaStream_t st)
   SampleParams p = in;
   const uint32_t es = elem_size(p.dtype);
   auto groups = [&](uint32_t ctas) { return (p.vocab + ctas * kGroup - 1) / (ctas * kGroup); };
-  auto fits = [&](uint32_t ctas) { return region(ctas) + kCtaBins * 8 + groups(ctas) * kGroup * es <= kSampleMaxSmem; };
+  // (in 16 bits more than kMostGroups of them go into shared memory)
+  auto fits = [&](uint32_t ctas) { return groups(ctas) <= kMostGroups && region(ctas) + kCtaBins * 8 + groups(ctas) * kGroup * es <= kSampleMaxSmem; };
   p.ctas = 1;
   while (!fits(p.ctas)) p.ctas *= 2;
   // As many CTAs to a row as keep four an SM (two of which run at once): shorter rows a CTA, but more barriers
@@ -1078,7 +1081,8 @@ int launch_sample_logits(const SampleParams &in, uint32_t n_sm, cudaStream_t st)
   while (p.ctas < kMaxCtas && groups(p.ctas) > 1 && p.n * p.ctas * 2 <= 4 * n_sm) p.ctas *= 2;
   p.groups = groups(p.ctas);
   p.slice = ((p.vocab + p.ctas - 1) / p.ctas + 15) / 16 * 16;
-  static_assert(region(kMaxCtas) + kCtaBins * 8 + kSampleMaxVocab / kMaxCtas * 4 <= kSampleMaxSmem && kSampleMaxVocab % (kMaxCtas * kGroup) == 0,
+  static_assert(region(kMaxCtas) + kCtaBins * 8 + kSampleMaxVocab / kMaxCtas * 4 <= kSampleMaxSmem && kSampleMaxVocab % (kMaxCtas * kGroup) == 0 &&
+                    kSampleMaxVocab / (kMaxCtas * kGroup) <= kMostGroups,
                 "shared memory of the largest vocabulary");
   const bool cuts = p.top_k || p.top_p;
   // Where not all rows run at once the lengthy ones are taken first; not where a row's answer is written over

@@ -103,6 +103,18 @@ def test_many_rows(n):
           [rng.uniform(0.5, 1.0) for _ in range(n)], [rng.choice([0.0, 0.1]) for _ in range(n)])
 
 
+@pytest.mark.parametrize("n,vocab", [(300, 65537), (300, 70000), (300, 100001), (150, 131073), (150, 151000), (150, 200000)])
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+def test_many_long_rows_in_16_bits(n, vocab, t):
+    """as few CTAs a row as shared memory allows would have more groups of elements than a warp has lanes"""
+    rng = random.Random(vocab)
+    x = logits_of("text", 4, vocab, TYPES[t], vocab)
+    rows = [rng.randrange(4) for _ in range(n)]
+    u, temp = [rng.choice([0.0, NEAR_ONE, rng.random(), rng.random()]) for _ in range(n)], [rng.choice([0.7, 1.0, 5.0, 40.0]) for _ in range(n)]
+    check(x, u, temp, rows=rows)
+    check(x, u, temp, [rng.choice([0, 30, 1500, vocab // 2]) for _ in range(n)], [rng.choice([1.0, 0.9, 0.5]) for _ in range(n)], rows=rows)
+
+
 @pytest.mark.parametrize("n", [297, 480, 511, 512, 513])
 @pytest.mark.parametrize("where", ["none", "all", "first", "last", "scattered", "one"])
 def test_rows_with_long_cuts_anywhere(n, where):
