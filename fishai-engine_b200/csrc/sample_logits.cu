@@ -24,6 +24,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
+
 #include "fa_device.cuh"
 #include "paged_ops.hpp"
 
@@ -1075,16 +1077,27 @@ int launch_sample_logits(const SampleParams &in, uint32_t n_sm, cudaStream_t st)
   auto fits = [&](uint32_t ctas) { return groups(ctas) <= kMostGroups && region(ctas) + kCtaBins * 8 + groups(ctas) * kGroup * es <= kSampleMaxSmem; };
   p.ctas = 1;
   while (!fits(p.ctas)) p.ctas *= 2;
-  // As many CTAs to a row as keep four an SM (two of which run at once): shorter rows a CTA, but more barriers
-  // of clusters.  64 rows of 128256, f32, cuts of all kinds: 55 us with 8, 65 with 4; 200 of 32000, bf16: 40 with 2, 56
-  // with 1, 81 with 4 .. 8.
-  while (p.ctas < kMaxCtas && groups(p.ctas) > 1 && p.n * p.ctas * 2 <= 4 * n_sm) p.ctas *= 2;
+  // More CTAs to a row are shorter passes, but more barriers of clusters.  Rows whose times differ little (no cuts;
+  // top-k, which mostly is small) take as many as run at once, where that goes: 64 rows of 128256 in bf16 without
+  // cuts 20.5 us with 4 CTAs, 24.6 with 8; 200 of 32000 18.4 with 2, 20.1 with 1, 22.6 with 4; with top-k 17.5 with 1,
+  // 26.7 with 2, 35.9 with 4.  Else as many as keep four an SM: 128 rows of 128256 in bf16 without cuts 33 with 4, 37
+  // with 2; 64 in f32, cuts of all kinds, 31 with 8, 45 with 4; 200 of 32000 in bf16 35 with 2, 55 with 1, 41 with 4.
+  const bool cuts = p.top_k || p.top_p;
+  auto at_once = [&](uint32_t ctas) {
+    const uint32_t smem = (cuts ? row_at<true>(ctas) : row_at<false>(ctas)) + groups(ctas) * kGroup * es + (uint32_t)sizeof(Small) + 1024;
+    return std::min<uint32_t>(cuts ? 2 : 3, 227 * 1024 / smem) * n_sm;
+  };
+  const uint32_t fewest = p.ctas;
+  if (!p.top_p)
+    for (uint32_t c = kMaxCtas; c >= fewest && p.ctas == fewest; c /= 2)
+      if (p.n * c <= at_once(c) && (c == 1 || groups(c / 2) > 1)) p.ctas = c;
+  if (p.top_p || p.n * p.ctas > at_once(p.ctas))
+    while (p.ctas < kMaxCtas && groups(p.ctas) > 1 && p.n * p.ctas * 2 <= 4 * n_sm) p.ctas *= 2;
   p.groups = groups(p.ctas);
   p.slice = ((p.vocab + p.ctas - 1) / p.ctas + 15) / 16 * 16;
   static_assert(region(kMaxCtas) + kCtaBins * 8 + kSampleMaxVocab / kMaxCtas * 4 <= kSampleMaxSmem && kSampleMaxVocab % (kMaxCtas * kGroup) == 0 &&
                     kSampleMaxVocab / (kMaxCtas * kGroup) <= kMostGroups,
                 "shared memory of the largest vocabulary");
-  const bool cuts = p.top_k || p.top_p;
   // Where not all rows run at once the lengthy ones are taken first; not where a row's answer is written over
   // settings that others have yet to look at.
   auto apart = [&](const void *out, const void *in) {
