@@ -247,7 +247,7 @@ def workspace_bytes(head_dim: int) -> int:
 
 
 def attention(kv: PagedKV, layer: int, q, q_start, kv_len, out, max_q: int, workspace, seqs=None, scale: float = 0.0,
-              window: int = 0, sinks: int = 0, err=None, stream: int = 0):
+              window: int = 0, err=None, stream: int = 0, sinks: int = 0):
     """Attention of chunks of new tokens over the pages: rows q_start[c] ..
     q_start[c+1] of q and out are a chunk of sequence seqs[c] (default c), whose
     cache holds kv_len[c] positions with the chunk's own last.  Each token sees
