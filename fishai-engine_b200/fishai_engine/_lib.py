@@ -95,7 +95,8 @@ _vp, _sz, _i, _u32, _u64, _f = C.c_void_p, C.c_size_t, C.c_int, C.c_uint32, C.c_
 _pu32, _pu64, _pf, _pi, _pi64 = C.POINTER(C.c_uint32), C.POINTER(C.c_uint64), C.POINTER(C.c_float), C.POINTER(C.c_int), C.POINTER(C.c_int64)
 # whole numbers and addresses of the calls in front of kernels of a few microseconds: an integer argument has the same
 # register or eight bytes of stack in any width, and ctypes converts a pointer's in half the time of a number's (18
-# arguments 2.7 us against 5)
+# arguments 2.7 us against 5).  It takes Python's own whole numbers only (and None, as 0): what a caller gives, which may
+# be numpy's, goes through operator.index first.
 _w = C.c_void_p
 SIGNATURES = {
     "fa_last_error": ([C.c_char_p, _sz], _sz),

@@ -2,6 +2,8 @@
 sampling.Sampler; the page tables follow through KVCache.reorder."""
 from __future__ import annotations
 
+from operator import index
+
 from . import _lib as L
 from .paged import _DTYPES, _INTS, _code, _space
 
@@ -36,6 +38,7 @@ def select(logits, scores, done, out_scores, out_parents, out_tokens, out_done, 
     ld, inner = logits.stride()
     if rows != nb * beams or (inner != 1 and vocab > 1) or b[0] != nb:
         raise ValueError(f"logits: [{nb * beams}, vocab] with consecutive elements, and out of {nb} rows")
+    eos, pad = index(eos), index(pad)
     if pad >> 32 or (eos != NO_TOKEN and eos >> 32):
         L.u32(pad=pad, eos=eos)
     wp, wn = _space(workspace)

@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes as C
 import sys
+from operator import index
 
 from . import _lib as L
 
@@ -204,7 +205,7 @@ def rope_append(kv: PagedKV, layer: int, rope: Rope, q, k, v, positions, seqs, o
     and v are rows of one type, with any row stride (slices of a fused
     projection).  seqs[t] = NO_TOKEN leaves a row out.  A rope of several axes
     takes positions [axes, tokens] (any row stride) and needs slots."""
-    dt = _code(q, "q")
+    dt, layer = _code(q, "q"), index(layer)
     if layer >> 32:
         L.u32(layer=layer)
     if k.dtype != q.dtype or v.dtype != q.dtype:
@@ -259,6 +260,7 @@ def attention(kv: PagedKV, layer: int, q, q_start, kv_len, out, max_q: int, work
     n = kv_len.shape[0]
     if _code(q, "q") != kv.dtype or out.dtype != q.dtype:
         raise ValueError("q and out have the pages' element type")
+    layer, max_q, window, sinks = index(layer), index(max_q), index(window), index(sinks)
     if (layer | max_q | window | sinks) >> 32:
         L.u32(layer=layer, max_q=max_q, window=window, sinks=sinks)
     hd = kv.head_dim

@@ -1,11 +1,13 @@
 """Calls of the operators on pages that Python has to pass on, or to refuse, before any kernel runs: no GPU needed."""
 import inspect
 
+import numpy as np
 import pytest
 
 torch = pytest.importorskip("torch")
 
-from fishai_engine import paged  # noqa: E402
+from fishai_engine import _lib as L  # noqa: E402
+from fishai_engine import beam, paged  # noqa: E402
 
 
 def i32(*shape):
@@ -25,3 +27,63 @@ def test_attention_takes_err_and_stream_behind_the_window():
     paged.attention(*args, None, 0)
     with pytest.raises(ValueError, match="err"):
         paged.attention(*args, i32(2), 0)
+
+
+# ------------------------------------------------------------------ whole numbers of other libraries
+class Whole:
+    def __init__(self, v):
+        self.v = v
+
+    def __index__(self):
+        return self.v
+
+
+KINDS = [np.int64, np.int32, np.uint32, np.uint8, Whole, torch.tensor]
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=lambda k: k.__name__)
+def test_whole_numbers_of_any_kind(kind):
+    """the maximum of an array of lengths is one of numpy's; its value arrives, and calls of no rows end before the device is asked"""
+    kv = paged.PagedKV(torch.zeros(1, 8, 2, 4, 16, 64, dtype=torch.float16), i32(2, 4))
+    q, k = torch.zeros(0, 512, dtype=torch.float16), torch.zeros(0, 256, dtype=torch.float16)
+    ws = torch.zeros(paged.workspace_bytes(64), dtype=torch.uint8)
+    for kw in (dict(), dict(window=kind(5)), dict(window=kind(5), sinks=kind(2)), dict(sinks=kind(0))):
+        paged.attention(kv, kind(0), q, i32(3), i32(2), torch.empty_like(q), kind(3), ws, **kw)
+    with pytest.raises(L.FishaiError, match="layer"):
+        paged.attention(kv, kind(1), q, i32(3), i32(2), torch.empty_like(q), kind(3), ws)
+    paged.rope_append(kv, kind(0), paged.Rope(64), q, k, k, i32(0), i32(0), torch.empty_like(q))
+    paged.rope_append(kv, kind(0), paged.Rope(64, axes=[16, 16]), q, k, k, i32(2, 0), i32(0), torch.empty_like(q), slots=i32(0))
+    with pytest.raises(L.FishaiError, match="layer"):
+        paged.rope_append(kv, kind(1), paged.Rope(64), q, k, k, i32(0), i32(0), torch.empty_like(q))
+    f = torch.zeros(0, 2)
+    beam.select(torch.zeros(0, 50), f, None, f.clone(), i32(0, 2), i32(0, 2), None, ws, eos=kind(3), pad=kind(49))
+    with pytest.raises(L.FishaiError, match="pad"):
+        beam.select(torch.zeros(0, 50), f, None, f.clone(), i32(0, 2), i32(0, 2), None, ws, eos=kind(3), pad=kind(50))
+
+
+@pytest.mark.parametrize("bad", [3.0, None, b"3", "3"], ids=str)
+def test_what_is_no_whole_number_is_refused(bad):
+    kv = paged.PagedKV(torch.zeros(1, 8, 2, 4, 16, 64, dtype=torch.float16), i32(2, 4))
+    q, k = torch.zeros(0, 512, dtype=torch.float16), torch.zeros(0, 256, dtype=torch.float16)
+    ws = torch.zeros(paged.workspace_bytes(64), dtype=torch.uint8)
+    good = dict(layer=0, max_q=3, window=5, sinks=2)
+    for name in good:
+        with pytest.raises(TypeError):
+            paged.attention(kv, q=q, q_start=i32(3), kv_len=i32(2), out=torch.empty_like(q), workspace=ws, **{**good, name: bad})
+    with pytest.raises(TypeError):
+        paged.rope_append(kv, bad, paged.Rope(64), q, k, k, i32(0), i32(0), torch.empty_like(q))
+    f = torch.zeros(0, 2)
+    for kw in (dict(eos=bad), dict(pad=bad)):
+        with pytest.raises(TypeError):
+            beam.select(torch.zeros(0, 50), f, None, f.clone(), i32(0, 2), i32(0, 2), None, ws, **kw)
+
+
+@pytest.mark.parametrize("name", ["layer", "max_q", "window", "sinks"])
+@pytest.mark.parametrize("v", [-1, 2 ** 32, 2 ** 70])
+def test_numbers_that_32_bits_do_not_hold(name, v):
+    kv = paged.PagedKV(torch.zeros(1, 8, 2, 4, 16, 64, dtype=torch.float16), i32(2, 4))
+    q, ws = torch.zeros(0, 512, dtype=torch.float16), torch.zeros(paged.workspace_bytes(64), dtype=torch.uint8)
+    good = dict(layer=0, max_q=3, window=5, sinks=2)
+    for w in (v, np.int64(v)) if v < 2 ** 63 else (v,):
+        with pytest.raises(ValueError):
+            paged.attention(kv, q=q, q_start=i32(3), kv_len=i32(2), out=torch.empty_like(q), workspace=ws, **{**good, name: w})
