@@ -4,7 +4,8 @@ append of new keys and values, attention of chunks of new tokens, page copies
 (one contiguous cache) and KVCache (whose pages they also work on).
 
 Buffers are framework tensors on the GPU (objects with data_ptr(), dtype, shape
-and stride(), such as torch tensors); nothing is copied, allocated or waited
+and stride(), such as torch tensors; pages, page table and workspace are torch's);
+nothing is copied, allocated or waited
 for, and `stream` is a cudaStream_t as int (0: the legacy default stream).
 Index arrays are contiguous int32 or uint32 tensors.  `err`, one int32 in
 device memory, collects FLAG_* bits of indices that the kernels refuse."""
@@ -43,18 +44,34 @@ def _code(t, name):
     return code
 
 
+def _flat(t, n):
+    """whether t is n elements in a row; is_contiguous, where there is one, takes half as long as stride"""
+    try:
+        return t.shape == (n,) and t.is_contiguous()
+    except AttributeError:
+        return n < 2 or t.stride() == (1,)
+
+
 def _index(t, name, n):
     """address of a contiguous array of n 32-bit whole numbers"""
-    if t.dtype not in _INTS or t.shape != (n,) or not t.is_contiguous():
+    if t.dtype not in _INTS or not _flat(t, n):
         if not _INTS:
             _learn()
             return _index(t, name, n)
-        if t.dtype not in _INTS or t.dim() != 1:
+        if t.dtype not in _INTS or len(t.shape) != 1:
             raise ValueError(f"{name}: a contiguous 1-d int32 tensor is needed")
         if t.shape[0] != n:
             raise ValueError(f"{name}: {t.shape[0]} entries, {n} needed")
         raise ValueError(f"{name}: a contiguous 1-d int32 tensor is needed")
     return t.data_ptr()
+
+
+def _count(t, name):
+    """entries of a 1-d array"""
+    shape = t.shape
+    if len(shape) != 1:
+        raise ValueError(f"{name}: a contiguous 1-d tensor is needed")
+    return shape[0]
 
 
 def _rows(t, name, n, width):
@@ -305,7 +322,7 @@ def plan_step(kv: PagedKV, add, lengths, free_pages, n_free, q_start, kv_len, po
     table = getattr(kv, "page_table", None)
     if table is None:
         raise ValueError("kv: pages of the caller's own; those of a KVCache are the cache's to give")
-    n, rows, cap = add.numel(), positions.numel(), free_pages.numel()  # 1-d: _index sees to it
+    n, rows, cap = _count(add, "add"), _count(positions, "positions"), _count(free_pages, "free_pages")
     ln = _index(lengths, "lengths", kv.n_seq)
     nf = _index(n_free, "n_free", 1)
     pool = L.fa_page_pool(kv._c.page_table, kv.n_seq, kv.max_pages, kv.n_pages, _index(free_pages, "free_pages", cap), cap)

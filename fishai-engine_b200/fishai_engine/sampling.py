@@ -8,7 +8,7 @@ from dataclasses import dataclass
 import numpy as np
 
 from . import _lib as L
-from .paged import _DTYPES, _code, _index
+from .paged import _DTYPES, _code, _count, _flat, _index
 
 
 @dataclass
@@ -81,7 +81,7 @@ class Sampler:
 
 def _floats(t, name, n):
     """address of a contiguous array of n float32"""
-    if _DTYPES.get(t.dtype) != L.KV_F32 or t.shape != (n,) or not t.is_contiguous():
+    if _DTYPES.get(t.dtype) != L.KV_F32 or not _flat(t, n):
         raise ValueError(f"{name}: a contiguous float32 [{n}] tensor is needed")
     return t.data_ptr()
 
@@ -99,7 +99,7 @@ def sample_logits(logits, u, ids, temperature=None, top_k=None, top_p=None, min_
     if len(shape) != 2 or (shape[1] > 1 and stride[1] != 1):
         raise ValueError("logits: [rows, vocab] with consecutive elements")
     m, vocab = shape
-    n = ids.numel()
+    n = _count(ids, "ids")
     if (m | vocab | n) >> 32:
         L.u32(rows=m, vocab=vocab, ids=n)
     rc = L.lib().fa_sample_logits(

@@ -7,7 +7,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 from fishai_engine import _lib as L  # noqa: E402
-from fishai_engine import beam, paged  # noqa: E402
+from fishai_engine import beam, paged, sampling  # noqa: E402
 
 
 def i32(*shape):
@@ -87,3 +87,40 @@ def test_numbers_that_32_bits_do_not_hold(name, v):
     for w in (v, np.int64(v)) if v < 2 ** 63 else (v,):
         with pytest.raises(ValueError):
             paged.attention(kv, q=q, q_start=i32(3), kv_len=i32(2), out=torch.empty_like(q), workspace=ws, **{**good, name: w})
+
+
+# ------------------------------------------------------------------ buffers that are not torch's
+class Buffer:
+    """what the module asks of a buffer, and nothing else"""
+
+    def __init__(self, t):
+        self._t, self.dtype, self.shape = t, t.dtype, tuple(t.shape)
+
+    def data_ptr(self):
+        return self._t.data_ptr()
+
+    def stride(self):
+        return tuple(self._t.stride())
+
+
+def test_buffers_with_an_address_type_shape_and_strides():
+    """all that is asked of them is looked at before the library sees the call; here it has no rows, or no device to look at"""
+    B = Buffer
+    kv = paged.PagedKV(torch.zeros(1, 8, 2, 4, 16, 64, dtype=torch.float16), i32(2, 4))
+    q, k = torch.zeros(0, 512, dtype=torch.float16), torch.zeros(0, 256, dtype=torch.float16)
+    ws = torch.zeros(paged.workspace_bytes(64), dtype=torch.uint8)
+    paged.rope_append(kv, 0, paged.Rope(64), B(q), B(k), B(k), B(i32(0)), B(i32(0)), B(q), slots=B(i32(0)), err=B(i32(1)))
+    paged.rope_append(kv, 0, paged.Rope(64, axes=[16, 16]), B(q), B(k), B(k), B(i32(2, 0)), B(i32(0)), B(q), slots=B(i32(0)))
+    paged.attention(kv, 0, B(q), B(i32(3)), B(i32(2)), B(q), 3, ws, seqs=B(i32(2)), err=B(i32(1)), window=5, sinks=2)
+    sampling.sample_logits(B(torch.zeros(3, 50)), B(torch.zeros(0)), B(i32(0)), temperature=B(torch.zeros(0)), top_k=B(i32(0)), rows=B(i32(0)))
+    args = dict(add=i32(2), lengths=i32(2), free_pages=i32(8), n_free=i32(1), q_start=i32(3), kv_len=i32(2), positions=i32(5), row_seqs=i32(5))
+    with pytest.raises(L.FishaiError, match="fa_step_plan"):
+        paged.plan_step(kv, **{n: B(t) for n, t in args.items()})
+    for name, bad in (("add", i32(2, 1)), ("add", i32(4)[::2]), ("positions", i32(5, 1)), ("row_seqs", i32(10)[::2]), ("free_pages", i32(2, 4)),
+                      ("free_pages", i32(16)[::2]), ("kv_len", torch.zeros(2))):
+        with pytest.raises(ValueError, match=name):
+            paged.plan_step(kv, **{**{n: B(t) for n, t in args.items()}, name: B(bad)})
+    x, f = torch.zeros(3, 50), torch.zeros
+    for name, bad in (("u", f(6)[::2]), ("u", f(3, 1)), ("ids", i32(3, 1)), ("ids", i32(6)[::2]), ("temperature", f(6)[::2]), ("top_k", i32(4))):
+        with pytest.raises(ValueError, match=name):
+            sampling.sample_logits(**{**dict(logits=B(x), u=B(f(3)), ids=B(i32(3))), name: B(bad)})
