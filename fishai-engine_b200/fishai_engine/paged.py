@@ -323,6 +323,8 @@ def plan_step(kv: PagedKV, add, lengths, free_pages, n_free, q_start, kv_len, po
     if table is None:
         raise ValueError("kv: pages of the caller's own; those of a KVCache are the cache's to give")
     n, rows, cap = _count(add, "add"), _count(positions, "positions"), _count(free_pages, "free_pages")
+    if (n | rows | cap) >> 32:
+        L.u32(add=n, positions=rows, free_pages=cap)
     ln = _index(lengths, "lengths", kv.n_seq)
     nf = _index(n_free, "n_free", 1)
     pool = L.fa_page_pool(kv._c.page_table, kv.n_seq, kv.max_pages, kv.n_pages, _index(free_pages, "free_pages", cap), cap)

@@ -124,3 +124,17 @@ def test_buffers_with_an_address_type_shape_and_strides():
     for name, bad in (("u", f(6)[::2]), ("u", f(3, 1)), ("ids", i32(3, 1)), ("ids", i32(6)[::2]), ("temperature", f(6)[::2]), ("top_k", i32(4))):
         with pytest.raises(ValueError, match=name):
             sampling.sample_logits(**{**dict(logits=B(x), u=B(f(3)), ids=B(i32(3))), name: B(bad)})
+
+
+@pytest.mark.parametrize("name", ["add", "positions", "free_pages"])
+def test_plans_of_more_entries_than_32_bits_count(name):
+    """2^32 and a few would be taken for those few"""
+    kv = paged.PagedKV(torch.zeros(1, 8, 2, 4, 16, 64, dtype=torch.float16), i32(2, 4))
+    long = torch.empty(2 ** 32 + 2, dtype=torch.int32, device="meta")
+    args = dict(add=i32(2), lengths=i32(2), free_pages=i32(8), n_free=i32(1), q_start=i32(3), kv_len=i32(2), positions=i32(5), row_seqs=i32(5))
+    with_it = {"add": ["add", "kv_len"], "positions": ["positions", "row_seqs"], "free_pages": ["free_pages"]}[name]
+    args.update({n: long for n in with_it})
+    if name == "add":
+        args["q_start"] = torch.empty(2 ** 32 + 3, dtype=torch.int32, device="meta")
+    with pytest.raises(ValueError, match=name):
+        paged.plan_step(kv, **args)
