@@ -480,7 +480,7 @@ typedef struct {
   uint32_t *page_table;  /* device [n_seq][max_pages] */
   uint32_t n_seq, max_pages, n_pages;
   uint32_t *free_pages;  /* device [free_cap] (NULL: free_cap 0) */
-  uint32_t free_cap;     /* room for every page that may be free at once */
+  uint32_t free_cap;     /* room for every page that may be free at once, below 2^31 */
 } fa_page_pool;
 int fa_step_plan(const fa_page_pool *pool, const uint32_t *seq, const uint32_t *keep, const uint32_t *add, uint32_t n, uint32_t n_rows,
                  const uint32_t *len, uint32_t *len_out, const uint32_t *n_free, uint32_t *n_free_out, uint32_t *q_start, uint32_t *kv_len,

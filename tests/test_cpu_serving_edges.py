@@ -6,6 +6,8 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
+from test_cpu_serving import call_plan  # noqa: E402
+
 from fishai_engine import _lib as L  # noqa: E402
 from fishai_engine import beam, paged, sampling  # noqa: E402
 
@@ -138,3 +140,12 @@ def test_plans_of_more_entries_than_32_bits_count(name):
         args["q_start"] = torch.empty(2 ** 32 + 3, dtype=torch.int32, device="meta")
     with pytest.raises(ValueError, match=name):
         paged.plan_step(kv, **args)
+
+
+@pytest.mark.parametrize("cap", [2 ** 31, 2 ** 32 - 8192, 2 ** 32 - 1])
+def test_a_stack_beyond_31_bits_is_refused(cap):
+    """the kernel steps through the pages that come back 8192 at a time: near 2^32 of them the count would wrap and not end"""
+    assert call_plan(free_cap=cap) == L.ERR_INVALID
+    assert "2^31" in L.last_error()
+    call_plan(free_cap=2 ** 31 - 1)
+    assert "2^31" not in L.last_error()
