@@ -243,7 +243,12 @@ __global__ void __launch_bounds__(THREADS) k_step_plan(const StepPlanParams p) {
     p.q_start[i] = a;
     p.kv_len[i] = q != kNone ? s.now[i] : 0;
     if (p.last) p.last[i] = b > a ? b - 1 : kNone;
-    if (q != kNone) p.len_out[q] = s.now[i];
+    if (q != kNone) {
+      p.len_out[q] = s.now[i];
+    } else if (p.len_out != p.len) {  // left out: its sequence keeps its length (all that name it write the same)
+      const uint32_t named = p.seq ? p.seq[i] : i;
+      if (named < p.n_seq) p.len_out[named] = p.len[named];
+    }
   }
   if (at == 0) {
     p.q_start[n] = T;

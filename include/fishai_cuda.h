@@ -460,7 +460,8 @@ int fa_pages_compact(const fa_pages *pages, const uint32_t *seq, const uint32_t 
  *    none.  Rows r < n_rows: pos[r] the position in the cache, row_seq[r] the
  *    sequence, slot[r] (slot may be NULL) page * 16 + position in the page; behind
  *    the last request's 0, FA_NO_TOKEN and FA_NO_TOKEN.
- *  - len_out[seq] = kv_len, for the sequences that are named; may be len.  *n_free
+ *  - len_out[seq]: the new length of each sequence that is named, where its request
+ *    was left out the old one; others are not written.  May be len.  *n_free
  *    of free_pages are free, the last of them the next one taken; *n_free_out (may be
  *    n_free) is their number after the call.  Pages that come back are put on the
  *    stack first, by request and in ascending order; then each request takes the

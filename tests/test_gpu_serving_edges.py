@@ -1,0 +1,40 @@
+"""Calls of the operators around a serving step that their documentation allows and their own files do not make."""
+import random
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+import serving_ref as S  # noqa: E402
+import test_gpu_step_plan as P  # noqa: E402
+from fishai_engine import paged  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+i32 = P.i32
+
+
+# ------------------------------------------------------------------ the plan with lengths of its own to write
+@pytest.mark.parametrize("kw", [dict(seqs=[0, 3, 1]), dict(seqs=[0, 7, 1]), dict(seqs=[0, -1, 1]), dict(seqs=[1, 0, 1]), dict(seqs=[2, 2, 2]),
+                                dict(keep=[10, 21, 30]), dict(keep=[10, -1, 30]), dict(lens=[10, 2000, 30, 8]), dict(lens=[10, -5, 30, 8]),
+                                dict(add=[1, 45, 2]), dict(add=[1, -1, 1]), dict(cap=1), dict(), dict(rows=3), dict(spare=0)], ids=str)
+@pytest.mark.parametrize("n_more", [0, 300])
+def test_lengths_of_requests_that_are_left_out(kw, n_more):
+    """lengths_out holds junk before the call: what is named has its length after it, the old one where the request was refused"""
+    a = dict(add=[1, 2, 3], lens=[10, 20, 30, 8], keep=None, seqs=[0, 1, 2], rows=80, cap=None, spare=9)
+    a.update(kw)
+    add, lens = a["add"] + [1] * n_more, a["lens"] + [5] * n_more
+    seqs, keep = a["seqs"] + list(range(4, 4 + n_more)), a["keep"] and a["keep"] + [5] * n_more
+    if a["cap"]:  # two pages come back, and the stack has room for one
+        keep = [0] * 3 + [5] * n_more
+    table, free, n_free, n_pages = P.world([max(0, min(x, 64)) for x in lens], 4, a["spare"])
+    free = free[: n_free + a["cap"]] if a["cap"] else free
+    want = S.plan(seqs, keep, add, a["rows"] + n_more, lens, table, free, n_free, n_pages)
+    kv, n, rows = P.kv_of(table, n_pages), len(add), a["rows"] + n_more
+    out, err = i32([-77] * len(lens)), i32([0])
+    arrays = [i32([9] * m) for m in (n + 1, n, rows, rows)]
+    before = i32(lens)
+    paged.plan_step(kv, i32(add), before, i32(free), i32([n_free]), *arrays, seqs=i32(seqs), keep=None if keep is None else i32(keep),
+                    lengths_out=out, n_free_out=i32([0]), err=err)
+    named = {q for q in seqs if 0 <= q < len(lens)}
+    assert out.tolist() == [m if q in named else -77 for q, m in enumerate(want[8])]
+    assert before.tolist() == lens and arrays[1].tolist() == want[1] and int(err) == want[10]
