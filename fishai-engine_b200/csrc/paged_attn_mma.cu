@@ -47,8 +47,8 @@ __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t &r0, uint32_t &r1,
 __device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t &r0, uint32_t &r1, uint32_t &r2, uint32_t &r3) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3) : "r"(addr) : "memory");
 }
-__device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool ok) {  // 16 bytes, or zeros
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16u : 0u) : "memory");
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src, uint32_t bytes) {  // 16 of them, or 0: zeros
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -247,24 +247,21 @@ __device__ __forceinline__ void stage(const PR &p, const T *base, const PagePair
                                       const Tile &at, uint32_t lo, uint32_t hi, uint32_t tile, uint32_t i, uint32_t threads) {
   constexpr uint32_t CH = HD / 8;  // pieces of a row
   const uint32_t c = i % CH, r0 = i / CH, step = threads / CH;
-  // most sub-tiles are seen whole: no questions row by row (with first positions, those took a third of a
-  // sub-tile's instructions: one token over 8160 positions and 4 first ones 18.5 us, 14.1 so)
-  auto seen = [&](uint32_t t) { return t >= lo || t + kPageLen <= p.sinks; };
-  const bool whole = at.t[1] + kPageLen <= hi && seen(at.t[0]) && (!PR::packed || seen(at.t[1]));
+  // A bit for each row of a page that is seen: a shift and an "and" a row, and one path for all sub-tiles.  (Bounds
+  // compared row by row were a third of a sub-tile's instructions where there are first positions beside a window.  With
+  // a path of its own for sub-tiles that are seen whole one token over 4096 positions and 4 first ones took 10.4 us, 8.7
+  // so, and calls of one short sub-tile, which fetch the code of both, 0.2 to 0.5 us more than the 4 to 6 they take.)
 #pragma unroll
   for (uint32_t half = 0; half < 2; ++half) {
     const bool good = pg.page[half] < p.pg.n_pages;
     const T *src = base + page_row(p.pg, good ? pg.page[half] : 0, is_v, head, 0) + c * 8;
-    if (whole) {
+    const uint32_t t = at.t[half];
+    auto below = [&](uint32_t x) { return (1u << (x > t ? min(x - t, kPageLen) : 0u)) - 1; };
+    uint32_t m = ~below(lo);
+    if (PR::packed) m |= below(p.sinks);
+    m = good ? (m & below(hi)) >> r0 << 4 : 0;
 #pragma unroll
-      for (uint32_t r = 0; r < 16; r += step) cp16(tile + sw<HD>(16 * half + r + r0, c), src + (r + r0) * HD, good);
-    } else {
-#pragma unroll
-      for (uint32_t r = 0; r < 16; r += step) {
-        const uint32_t row = r + r0, t = at.t[half] + row;
-        cp16(tile + sw<HD>(16 * half + row, c), src + row * HD, good && item_sees(p, lo, hi, t));
-      }
-    }
+    for (uint32_t r = 0; r < 16; r += step) cp16(tile + sw<HD>(16 * half + r + r0, c), src + (r + r0) * HD, m >> r & 16);
   }
 }
 

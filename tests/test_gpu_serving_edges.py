@@ -1,11 +1,11 @@
 """Calls of the operators around a serving step that their documentation allows and their own files do not make."""
-import random
-
 import pytest
 
 torch = pytest.importorskip("torch")
 
+import paged_ref as R  # noqa: E402
 import serving_ref as S  # noqa: E402
+import test_gpu_sinks as A  # noqa: E402
 import test_gpu_step_plan as P  # noqa: E402
 from fishai_engine import paged  # noqa: E402
 
@@ -38,3 +38,16 @@ def test_lengths_of_requests_that_are_left_out(kw, n_more):
     named = {q for q in seqs if 0 <= q < len(lens)}
     assert out.tolist() == [m if q in named else -77 for q, m in enumerate(want[8])]
     assert before.tolist() == lens and arrays[1].tolist() == want[1] and int(err) == want[10]
+
+
+# ------------------------------------------------------------------ which slots of a page are read
+@pytest.mark.parametrize("t", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n", [1, 15, 16, 17, 31, 32, 33, 47, 48, 49, 64, 65, 300])
+def test_only_slots_that_are_seen_are_read(t, hd, n):
+    """every other slot holds NaN, every other page is a bad one: edges of the cache, of the window and of the first positions
+    at every place of a page"""
+    for q in (1, 5, 40):
+        for window, sinks in ((0, 0), (1, 0), (7, 0), (16, 0), (17, 0), (1, 1), (3, 5), (16, 16), (15, 17), (2, 40)):
+            if q <= n:
+                A.check([q, q], [n, max(q, n - 3)], 4, 2, hd, R.TYPES[t], window, sinks, seed=n)
