@@ -44,17 +44,17 @@ def _code(t, name):
     return code
 
 
-def _flat(t, n):
-    """whether t is n elements in a row; is_contiguous, where there is one, takes half as long as stride"""
+def _dense(t):
+    """whether a 1-d array's elements are in a row; is_contiguous, where there is one, takes half as long as stride"""
     try:
-        return t.shape == (n,) and t.is_contiguous()
+        return t.is_contiguous()
     except AttributeError:
-        return n < 2 or t.stride() == (1,)
+        return t.stride() == (1,)
 
 
 def _index(t, name, n):
     """address of a contiguous array of n 32-bit whole numbers"""
-    if t.dtype not in _INTS or not _flat(t, n):
+    if t.dtype not in _INTS or t.shape != (n,) or (n > 1 and not _dense(t)):
         if not _INTS:
             _learn()
             return _index(t, name, n)

@@ -8,7 +8,7 @@ from dataclasses import dataclass
 import numpy as np
 
 from . import _lib as L
-from .paged import _DTYPES, _code, _count, _flat, _index
+from .paged import _DTYPES, _code, _count, _dense, _index
 
 
 @dataclass
@@ -81,7 +81,7 @@ class Sampler:
 
 def _floats(t, name, n):
     """address of a contiguous array of n float32"""
-    if _DTYPES.get(t.dtype) != L.KV_F32 or not _flat(t, n):
+    if _DTYPES.get(t.dtype) != L.KV_F32 or t.shape != (n,) or (n > 1 and not _dense(t)):
         raise ValueError(f"{name}: a contiguous float32 [{n}] tensor is needed")
     return t.data_ptr()
 
