@@ -318,7 +318,9 @@ def plan_step(kv: PagedKV, add, lengths, free_pages, n_free, q_start, kv_len, po
     place), and what the step's calls take: q_start [n + 1], kv_len [n], last [n],
     the last row of each request, and for each of positions.shape[0] rows the
     position, the sequence (NO_TOKEN behind the last) and slots, the place in the
-    pages counted in positions.  What is taken, refused and flagged: fa_step_plan."""
+    pages counted in positions.  Pages that a sequence gives back have to be its
+    alone: nobody counts who shares them.  What is taken, refused and flagged:
+    fa_step_plan."""
     table = getattr(kv, "page_table", None)
     if table is None:
         raise ValueError("kv: pages of the caller's own; those of a KVCache are the cache's to give")

@@ -472,8 +472,14 @@ int fa_pages_compact(const fa_pages *pages, const uint32_t *seq, const uint32_t 
  *    the request is left out, its sequence as it was, kv_len 0.  So does a stack that
  *    is or would grow longer than free_cap, and then nothing is taken or cut.  A page
  *    number >= n_pages that is moved sets FA_FLAG_PAGE and is passed on.
- *  - A partly filled last page that another sequence shares has to be copied before
- *    (fa_pages_copy): rows go into it.
+ *  - Nobody counts who else names a page.  What a sequence gives back, its pages
+ *    behind the first keep positions that its new end leaves over (keep 0: every page
+ *    it names), goes to the next that needs one: each has to be this sequence's alone,
+ *    neither shared with a sequence that goes on (a common prefix, a fork) nor given
+ *    back or used for something else before (pages between first positions and a
+ *    window).  Sequences may share pages as long as none of them is cut into those;
+ *    a partly filled last page that is shared has to be copied before the sequence
+ *    grows (fa_pages_copy): rows go into it.
  * n <= 4096, n_seq <= 2^18 where seq is given.  No array may overlap another but
  * as said.  Device, stream and capture rules as for the others. */
 #define FA_FLAG_FULL 128  /* *err: rows or pages ran out, a request was left out */

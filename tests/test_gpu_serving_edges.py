@@ -40,6 +40,23 @@ def test_lengths_of_requests_that_are_left_out(kw, n_more):
     assert before.tolist() == lens and arrays[1].tolist() == want[1] and int(err) == want[10]
 
 
+def test_a_shared_prefix_that_no_request_is_cut_into():
+    """two sequences with the same two pages in front: they grow, are cut down to the prefix and grow again, and the pages stay"""
+    lens = [50, 39, 0]
+    table, free, n_free, n_pages = P.world(lens, 6, 9)
+    table[1][:2] = table[0][:2]  # the second one's own first two pages are nobody's now
+    prefix = set(table[0][:2])
+    kv, t, f, n = P.kv_of(table, n_pages), i32(lens), i32(free), i32([n_free])
+    for keep, add in (([50, 39, 0], [1, 1, 20]), ([40, 33, 20], [3, 30, 1]), ([32, 32, 0], [0, 0, 60]), ([32, 32, 60], [17, 40, 1])):
+        err, out = i32([0]), [i32([9] * m) for m in (4, 3, 100, 100)]
+        want = S.plan(None, keep, add, 100, lens, table, free, n_free, n_pages)
+        table, free, lens, n_free = want[6], want[7], want[8], want[9]
+        paged.plan_step(kv, i32(add), t, f, n, *out, keep=i32(keep), err=err)
+        assert int(err) == want[10] == 0
+        assert kv.page_table.tolist() == table and f.tolist() == free and t.tolist() == lens and int(n) == n_free
+        assert not prefix & set(free[:n_free]) and table[0][:2] == table[1][:2] and not prefix & set(table[2][: -(-lens[2] // 16)])
+
+
 # ------------------------------------------------------------------ which slots of a page are read
 @pytest.mark.parametrize("t", ["f16", "bf16", "f32"])
 @pytest.mark.parametrize("hd", [64, 128])
