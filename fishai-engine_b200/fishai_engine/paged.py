@@ -221,7 +221,8 @@ def rope_append(kv: PagedKV, layer: int, rope: Rope, q, k, v, positions, seqs, o
     at cache position slots[t] (default positions[t]) of sequence seqs[t].  q, k
     and v are rows of one type, with any row stride (slices of a fused
     projection).  seqs[t] = NO_TOKEN leaves a row out.  A rope of several axes
-    takes positions [axes, tokens] (any row stride) and needs slots."""
+    takes positions [axes, tokens] (any row stride) and needs slots: plan_step's
+    positions, not its slots, which count over the pages."""
     dt, layer = _code(q, "q"), index(layer)
     if layer >> 32:
         L.u32(layer=layer)
@@ -318,7 +319,8 @@ def plan_step(kv: PagedKV, add, lengths, free_pages, n_free, q_start, kv_len, po
     place), and what the step's calls take: q_start [n + 1], kv_len [n], last [n],
     the last row of each request, and for each of positions.shape[0] rows the
     position, the sequence (NO_TOKEN behind the last) and slots, the place in the
-    pages counted in positions.  Pages that a sequence gives back have to be its
+    pages counted in positions (for kernels of the caller's own: rope_append's slots
+    are the positions written here).  Pages that a sequence gives back have to be its
     alone: nobody counts who shares them.  What is taken, refused and flagged:
     fa_step_plan."""
     table = getattr(kv, "page_table", None)

@@ -341,8 +341,8 @@ void fa_rope_free(fa_rope *r);
 int fa_rope_freqs(const fa_rope *r, double *freqs, double *scale);
 /* Turns q and k of n_tokens tokens and puts k, v into the pages of `layer`.
  * Token t: RoPE position pos[t], cache sequence seq[t], cache position
- * slot[t] (slot NULL: pos[t]); q row t of n_heads * head_dim elements at
- * q + t q_stride goes to out + t out_stride (out may be q), k and v rows of
+ * slot[t] (slot NULL: pos[t]), counted in the sequence: the page table says which
+ * page holds it; q row t of n_heads * head_dim elements at q + t q_stride goes to out + t out_stride (out may be q), k and v rows of
  * n_kv_heads * head_dim elements.  q, k, v have type in_dtype, out the pages'
  * type.  out shares no memory with k, v or the pages.  seq[t] = FA_NO_TOKEN
  * marks a row that is left out (padding).  Two tokens of a call must not name
@@ -376,8 +376,8 @@ int fa_rope_create_axes(const fa_rope_config *cfg, const fa_rope_axes *axes, fa_
 int fa_rope_axis_of(const fa_rope *r, uint32_t *axis);
 /* fa_rope_append with a position on each axis: that of token t on axis a is
  * pos[a pos_stride + t] (pos_stride >= n_tokens, or 0: the same on all axes).
- * slot is needed: the cache
- * counts tokens, not positions.  A rope of several axes is refused by
+ * slot is needed: the cache counts tokens, not positions (fa_step_plan's pos is
+ * what belongs here, not its slot).  A rope of several axes is refused by
  * fa_rope_append, one of one axis is welcome here. */
 int fa_rope_append_axes(const fa_rope *r, const fa_pages *pages, uint32_t layer, int32_t in_dtype, const void *q,
                         uint64_t q_stride, const void *k, uint64_t k_stride, const void *v, uint64_t v_stride,
@@ -458,8 +458,10 @@ int fa_pages_compact(const fa_pages *pages, const uint32_t *seq, const uint32_t 
  *  - q_start [n + 1], kv_len [n]: rows and length of each request (0 rows where it
  *    was not taken); last [n] (may be NULL): its last row, FA_NO_TOKEN where it has
  *    none.  Rows r < n_rows: pos[r] the position in the cache, row_seq[r] the
- *    sequence, slot[r] (slot may be NULL) page * 16 + position in the page; behind
- *    the last request's 0, FA_NO_TOKEN and FA_NO_TOKEN.
+ *    sequence, slot[r] (slot may be NULL) page * 16 + position in the page, for a
+ *    caller's own kernels; behind the last request's 0, FA_NO_TOKEN and FA_NO_TOKEN.
+ *    fa_rope_append and fa_rope_append_axes look pages up themselves: their slot is
+ *    this pos, and this slot given to them would write to the wrong place.
  *  - len_out[seq]: the new length of each sequence that is named, where its request
  *    was left out the old one; others are not written.  May be len.  *n_free
  *    of free_pages are free, the last of them the next one taken; *n_free_out (may be
