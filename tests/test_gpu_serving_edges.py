@@ -1,4 +1,5 @@
 """Calls of the operators around a serving step that their documentation allows and their own files do not make."""
+import numpy as np
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -7,6 +8,7 @@ import paged_ref as R  # noqa: E402
 import serving_ref as S  # noqa: E402
 import test_gpu_sinks as A  # noqa: E402
 import test_gpu_step_plan as P  # noqa: E402
+from fishai_engine import _lib as L  # noqa: E402
 from fishai_engine import paged  # noqa: E402
 
 pytestmark = pytest.mark.gpu
@@ -68,3 +70,38 @@ def test_only_slots_that_are_seen_are_read(t, hd, n):
         for window, sinks in ((0, 0), (1, 0), (7, 0), (16, 0), (17, 0), (1, 1), (3, 5), (16, 16), (15, 17), (2, 40)):
             if q <= n:
                 A.check([q, q], [n, max(q, n - 3)], 4, 2, hd, R.TYPES[t], window, sinks, seed=n)
+
+
+# ------------------------------------------------------------------ the entry with first positions, and none of them
+@pytest.mark.parametrize("t", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("window", [0, 1, 30, 10 ** 6])
+def test_no_first_positions_through_their_entry(t, window):
+    """Python takes the other entry for these; from C both give the same bits"""
+    qs, kvs = [1, 40, 200, 0], [300, 90, 250, 8]
+    pages, table = R.make_cache(kvs, 1, 2, 64, R.TYPES[t], 3)
+    start, n = [0, 1, 41, 241, 241], 241
+    q = A.randn(4, n, 8 * 64, dtype=R.TYPES[t])
+    want = A.call(pages, table, q, start, kvs, window, 0)
+    kv, out, err = paged.PagedKV(pages, table), torch.full_like(q, 7.0), i32([0])
+    ws = torch.empty(paged.workspace_bytes(64), dtype=torch.uint8, device="cuda")
+    starts, lens = i32(start), i32(kvs)
+    L.check(L.lib().fa_attn_chunks_sinks(kv._ref, 0, q.data_ptr(), 8 * 64, 8, 4, starts.data_ptr(), lens.data_ptr(), None, n, 200, 0.0, window, 0,
+                                         out.data_ptr(), 8 * 64, ws.data_ptr(), ws.numel(), err.data_ptr(), None))
+    assert torch.equal(out, want) and int(err) == 0
+    exact, tol = S.attention(pages, table, q, start, kvs, 8, 0.0, window, 0)
+    assert bool(((out.double().view_as(exact) - exact).abs() <= tol).all())
+
+
+def test_numbers_of_numpy_and_err_by_place():
+    """the same bits and flags as with Python's own numbers, named"""
+    lens = np.array([1, 33, 7])
+    start = [0] + np.cumsum(lens).tolist()
+    pages, table = R.make_cache([50, 40, 90], 2, 2, 64, torch.float16, 9)
+    table[2, 1] = pages.shape[1]  # a bad page
+    q = A.randn(1, 41, 4 * 64, dtype=torch.float16)
+    kv, ws = paged.PagedKV(pages, table), torch.empty(paged.workspace_bytes(64), dtype=torch.uint8, device="cuda")
+    args = (i32(start), i32([50, 40, 90]))
+    a, b, ea, eb = torch.zeros_like(q), torch.zeros_like(q), i32([0]), i32([0])
+    paged.attention(kv, 1, q, *args, a, 33, ws, window=60, err=ea, sinks=4)
+    paged.attention(kv, np.int32(1), q, *args, b, np.max(lens), ws, None, 0.0, np.uint32(60), eb, 0, np.int64(4))
+    assert torch.equal(a, b) and int(ea) == int(eb) == paged.FLAG_PAGE
