@@ -899,10 +899,14 @@ struct Row {
   }
 };
 
-// CUTS: top-k or top-p may be asked for.  Without, a row needs fewer registers and no lists, and three CTAs
-// fit on an SM (200 rows of 32000 in bf16: 18.4 us, with two 20.5).  LONG_FIRST: rows in another order than given.
+// CTAs that fit on an SM.  Without top-k and top-p (CUTS) a row needs no lists, and in 16 bits 40 registers are
+// enough for three (200 rows of 32000 in bf16: 18.4 us, with two 20.5); f32 rows, whose loads hold more, would spill
+// (in a graph of calls 64 rows of 128256: 31.7 us with three, 25.0 with two; 200 of 32000: 22.2 and 19.8).
+__host__ __device__ constexpr uint32_t ctas_an_sm(bool cuts, uint32_t elem_bytes) { return cuts || elem_bytes == 4 ? 2 : 3; }
+
+// CUTS: top-k or top-p may be asked for.  LONG_FIRST: rows in another order than given.
 template <typename T, bool CUTS, bool LONG_FIRST>
-__global__ void __launch_bounds__(kThreads, CUTS ? 2 : 3) k_sample_logits(const SampleParams p) {
+__global__ void __launch_bounds__(kThreads, ctas_an_sm(CUTS, sizeof(T))) k_sample_logits(const SampleParams p) {
   __shared__ Small s;
   const uint32_t ctas = p.ctas;
   Row<T> w(p, s);
@@ -1085,7 +1089,7 @@ int launch_sample_logits(const SampleParams &in, uint32_t n_sm, cudaStream_t st)
   const bool cuts = p.top_k || p.top_p;
   auto at_once = [&](uint32_t ctas) {
     const uint32_t smem = (cuts ? row_at<true>(ctas) : row_at<false>(ctas)) + groups(ctas) * kGroup * es + (uint32_t)sizeof(Small) + 1024;
-    return std::min<uint32_t>(cuts ? 2 : 3, 227 * 1024 / smem) * n_sm;
+    return std::min<uint32_t>(ctas_an_sm(cuts, es), 227 * 1024 / smem) * n_sm;
   };
   const uint32_t fewest = p.ctas;
   if (!p.top_p)
