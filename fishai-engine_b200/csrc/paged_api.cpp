@@ -460,7 +460,7 @@ int fa_step_plan(const fa_page_pool *pool, const uint32_t *seq, const uint32_t *
   if (!pool->page_table || (!pool->free_pages && pool->free_cap)) return invalid(who, "null argument pool.page_table or pool.free_pages");
   if (!pool->n_seq || !pool->max_pages) return invalid(who, "empty page table");
   if (pool->max_pages > (1u << 21)) return invalid(who, "more than 2^21 pages a sequence");
-  if (pool->free_cap > 0x7FFFFFFFu) return invalid(who, "room for 2^31 or more free pages");  // the kernel counts beyond it in 32 bits
+  if (pool->free_cap > 0x7FFFFFFFu) return invalid(who, "room for 2^31 or more free pages");  // the kernel's 32-bit counts step past the last page
   if (pool->n_pages > 0x0FFFFFFFu && slot) return invalid(who, "slots of more than 2^28 - 1 pages");
   if (n > kPlanMaxRequests) return fail(FA_ERR_UNSUPPORTED, std::string(who) + ": more than 4096 requests");
   if (seq && pool->n_seq > kPlanMaxSeqs) return fail(FA_ERR_UNSUPPORTED, std::string(who) + ": more than 2^18 sequences");

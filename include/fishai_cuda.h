@@ -341,8 +341,9 @@ void fa_rope_free(fa_rope *r);
 int fa_rope_freqs(const fa_rope *r, double *freqs, double *scale);
 /* Turns q and k of n_tokens tokens and puts k, v into the pages of `layer`.
  * Token t: RoPE position pos[t], cache sequence seq[t], cache position
- * slot[t] (slot NULL: pos[t]), counted in the sequence: the page table says which
- * page holds it; q row t of n_heads * head_dim elements at q + t q_stride goes to out + t out_stride (out may be q), k and v rows of
+ * slot[t] (slot NULL: pos[t]), counted in the sequence: the page table says
+ * which page holds it; q row t of n_heads * head_dim elements at q + t q_stride
+ * goes to out + t out_stride (out may be q), k and v rows of
  * n_kv_heads * head_dim elements.  q, k, v have type in_dtype, out the pages'
  * type.  out shares no memory with k, v or the pages.  seq[t] = FA_NO_TOKEN
  * marks a row that is left out (padding).  Two tokens of a call must not name
